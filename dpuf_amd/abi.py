@@ -90,6 +90,61 @@ class DpufToolsSpec(C.Structure):
     ]
 
 
+class DpufAmdPages(C.Structure):
+    """One layer's KV pages (include/dpuf_amd.h)."""
+    _fields_ = [
+        ("type", C.c_int32),
+        ("n_pages", C.c_int32),
+        ("page_size", C.c_int32),
+        ("n_kv_heads", C.c_int32),
+        ("head_dim", C.c_int32),
+        ("page_stride", C.c_int64),
+        ("head_stride", C.c_int64),
+        ("row_stride", C.c_int64),
+        ("k", C.c_void_p),
+        ("v", C.c_void_p),
+        ("w", C.c_void_p),
+    ]
+
+
+class DpufAmdBatch(C.Structure):
+    """A ragged batch over KV pages (include/dpuf_amd.h)."""
+    _fields_ = [
+        ("n_seqs", C.c_int32),
+        ("n_rows", C.c_int32),
+        ("table_stride", C.c_int32),
+        ("max_ctx", C.c_int32),
+        ("row_start", C.c_void_p),
+        ("ctx_len", C.c_void_p),
+        ("page_table", C.c_void_p),
+    ]
+
+
+class DpufAmdRopeSpec(C.Structure):
+    """How a model turns positions into angles (include/dpuf_amd.h)."""
+    _fields_ = [
+        ("rot_dim", C.c_int32),
+        ("theta", C.c_float),
+        ("scaling", C.c_int32),
+        ("factor", C.c_float),
+        ("low_freq", C.c_float),
+        ("high_freq", C.c_float),
+        ("beta_fast", C.c_float),
+        ("beta_slow", C.c_float),
+        ("orig_max_pos", C.c_int32),
+    ]
+
+
+class DpufAmdRope(C.Structure):
+    """A rotation as the device takes it (include/dpuf_amd.h)."""
+    _fields_ = [
+        ("turns", C.c_void_p),
+        ("rot_dim", C.c_int32),
+        ("interleaved", C.c_int32),
+        ("scale", C.c_float),
+    ]
+
+
 P = C.c_void_p
 I32 = C.c_int32
 F32P = C.POINTER(C.c_float)
@@ -221,5 +276,16 @@ def load_engine():
     _sig(lib, "dpuf_amd_reduce_check_noalloc", I32, [P, I32, I32, C.c_float, P, P])
     _sig(lib, "dpuf_amd_verify_tiles_device", I32, [I32, I32, I32, P, P, P])
     _sig(lib, "dpuf_amd_engine_forward_slots", I32, [P, I32, P, P, P, P, P])
+    I64, F32 = C.c_int64, C.c_float
+    batch, pages = C.POINTER(DpufAmdBatch), C.POINTER(DpufAmdPages)
+    _sig(lib, "dpuf_amd_rope_turns", I32, [C.POINTER(DpufAmdRopeSpec), P, C.POINTER(F32)])
+    _sig(lib, "dpuf_amd_rope_append", I32, [batch, pages, C.POINTER(DpufAmdRope), P, I32, I32, P, P, P, I64, I64, I64,
+                                            P, P, F32, P, P])
+    _sig(lib, "dpuf_amd_paged_attn_workspace", C.c_size_t, [batch, pages, I32])
+    _sig(lib, "dpuf_amd_paged_attn", I32, [batch, pages, I32, P, F32, I32, P, P, P, C.c_size_t, P])
+    _sig(lib, "dpuf_amd_paged_attn_weights", I32, [batch, pages, I32, P, F32, P, F32, P, P])
+    _sig(lib, "dpuf_amd_paged_evict", I32, [batch, pages, I32, I32, I32, pages, P, I32, P, P, P])
+    _sig(lib, "dpuf_amd_sample_workspace", C.c_size_t, [I32, I32])
+    _sig(lib, "dpuf_amd_sample", I32, [I32, I32, I32, I64, P, P, P, P, P, P, P, P, P, C.c_size_t, P])
     _engine = lib
     return lib

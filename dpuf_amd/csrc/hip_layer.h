@@ -1,7 +1,7 @@
 /*
  * hip_layer.h -- the thin C ABI between the C host engine (engine.c) and the
  * gfx950 HIP code (rt.hip, gemv.hip, gemm.hip, attn.hip, attn_wide.hip,
- * attn_dec.hip).  Plain pointers and sizes only; every
+ * attn_dec.hip, paged_attn.hip, paged_cache.hip, sample.hip).  Plain pointers and sizes only; every
  * function that launches work takes the engine's stream as an opaque handle.
  */
 #ifndef DPUF_HIP_LAYER_H
@@ -9,6 +9,8 @@
 
 #include <stddef.h>
 #include <stdint.h>
+
+#include "../../include/dpuf_amd.h"
 
 #ifdef __cplusplus
 extern "C" {
@@ -288,6 +290,32 @@ void dpuf_hip_fwht_sign(void* s, int32_t M, int32_t K, const float* x, const uin
 void dpuf_hip_slab_pack(void* s, int32_t mc, int32_t K, DpufPrep rows, int32_t* sq, float* ss, int32_t* sm);
 void dpuf_hip_slab_unpack(void* s, int32_t M, int32_t K, const int32_t* sq, const float* ss, const int32_t* sm,
                           DpufPrep rows);
+
+/* The device a device-memory pointer is on; -1 for any other pointer. */
+int32_t dpuf_hip_ptr_device(const void* p);
+/* Makes dev the current device; returns what dpuf_hip_device_leave takes to
+ * go back (-1: nothing to do). */
+int32_t dpuf_hip_device_enter(int32_t dev);
+void dpuf_hip_device_leave(int32_t back);
+
+/* The paged-serving operators behind include/dpuf_amd.h's entry points of the
+ * same names, whose arguments have been checked. */
+void dpuf_hip_rope_append(void* s, const DpufAmdBatch* b, const DpufAmdPages* p, const DpufAmdRope* r,
+                          const int32_t* pos, int32_t in_type, int32_t nq, const void* q, const void* k, const void* v,
+                          int64_t qs, int64_t ks, int64_t vs, const float* qn, const float* kn, float eps,
+                          void* q_out);
+size_t dpuf_hip_paged_attn_workspace(const DpufAmdBatch* b, const DpufAmdPages* p, int32_t nq);
+void dpuf_hip_paged_attn(void* s, const DpufAmdBatch* b, const DpufAmdPages* p, int32_t nq, const void* q, float scale,
+                         int32_t out_f32, void* out, float* lse, void* ws);
+void dpuf_hip_paged_attn_weights(void* s, const DpufAmdBatch* b, const DpufAmdPages* p, int32_t nq, const void* q,
+                                 float scale, const float* lse, float decay, const float* w_in);
+void dpuf_hip_paged_evict(void* s, const DpufAmdBatch* b, const DpufAmdPages* p, int32_t keep, int32_t sink,
+                          int32_t recent, const DpufAmdPages* d, const int32_t* dtable, int32_t dstride,
+                          int32_t* kept, int32_t* new_len);
+size_t dpuf_hip_sample_workspace(int32_t n, int32_t V);
+void dpuf_hip_sample(void* s, int32_t type, int32_t n, int32_t V, int64_t stride, const void* x, const float* temp,
+                     const int32_t* top_k, const float* top_p, const float* min_p, const float* u, int32_t* tok,
+                     float* logp, void* ws);
 
 #ifdef __cplusplus
 }

@@ -1,0 +1,270 @@
+/*
+ * paged.c -- entry points of the paged-serving operators (include/dpuf_amd.h):
+ * every argument is checked here, on the host, before a kernel that relies on
+ * it is launched; what only the device knows (lengths, page numbers) the
+ * kernels clamp or mask themselves.
+ */
+#include <math.h>
+#include <stdint.h>
+#include <string.h>
+
+#include "../../include/dpuf_amd.h"
+#include "hip_layer.h"
+
+#define MAX_SEQS 16384
+#define MAX_ROWS 65536
+
+static int aligned(const void* p, uintptr_t n) { return p && ((uintptr_t)p & (n - 1)) == 0; }
+
+/* The device all of the n non-NULL pointers are on, or -1. */
+static int32_t device_of(const void* const* p, int n) {
+    int32_t dev = -1;
+    for (int i = 0; i < n; i++) {
+        if (!p[i]) continue;
+        const int32_t d = dpuf_hip_ptr_device(p[i]);
+        if (d < 0 || (dev >= 0 && d != dev)) return -1;
+        dev = d;
+    }
+    return dev;
+}
+
+static int overlap(const void* a, uint64_t an, const void* b, uint64_t bn) {
+    const uintptr_t x = (uintptr_t)a, y = (uintptr_t)b;
+    return a && b && an && bn && x < y + bn && y < x + an;
+}
+
+static int32_t check_pages(const DpufAmdPages* p) {
+    if (!p) return -1;
+    if (p->type != DPUF_AMD_BF16 && p->type != DPUF_AMD_F16) return -5;
+    if (p->head_dim != 64 && p->head_dim != 128 && p->head_dim != 256) return -5;
+    if (p->n_pages < 1 || p->n_kv_heads < 1 || p->n_kv_heads > 1024) return -2;
+    if (p->page_size < 16 || p->page_size > 1024 || (p->page_size & (p->page_size - 1))) return -2;
+    const int64_t s[3] = {p->page_stride, p->head_stride, p->row_stride};
+    for (int i = 0; i < 3; i++)
+        if (s[i] < p->head_dim || s[i] % 8 != 0) return -4;
+    if (!aligned(p->k, 16) || !aligned(p->v, 16)) return -1;
+    return 0;
+}
+
+static int32_t check_batch(const DpufAmdBatch* b, const DpufAmdPages* p) {
+    if (!b || !aligned(b->row_start, 4) || !aligned(b->ctx_len, 4) || !aligned(b->page_table, 4)) return -1;
+    if (b->n_seqs < 1 || b->n_seqs > MAX_SEQS || b->n_rows < 0 || b->n_rows > MAX_ROWS || b->table_stride < 1 ||
+        (int64_t)b->table_stride * p->page_size > (int64_t)1 << 30)
+        return -2;
+    return 0;
+}
+
+static int32_t check_heads(const DpufAmdPages* p, int32_t nq) {
+    return nq < 1 || nq % p->n_kv_heads != 0 || nq / p->n_kv_heads > 32 ? -2 : 0;
+}
+
+/* Bytes that the rows of an n-row operand of `cols` columns span. */
+static uint64_t span(int64_t n, int64_t stride, int64_t cols, int64_t size) {
+    return n > 0 ? (uint64_t)((n - 1) * stride + cols) * (uint64_t)size : 0;
+}
+
+static int64_t type_size(int32_t t) { return t == DPUF_AMD_F32 ? 4 : 2; }
+
+/* Runs `call` with the pointers' device current. */
+#define ON_DEVICE(dev, call)                               \
+    do {                                                   \
+        const int32_t back_ = dpuf_hip_device_enter(dev);  \
+        if (dpuf_hip_ok()) call;                           \
+        dpuf_hip_device_leave(back_);                      \
+        return dpuf_hip_ok() ? 0 : -6;                     \
+    } while (0)
+
+DPUF_EXPORT int32_t dpuf_amd_rope_turns(const DpufAmdRopeSpec* spec, double* turns, float* scale) {
+    if (!spec || !turns || !scale) return -1;
+    const int32_t r = spec->rot_dim;
+    const double theta = spec->theta, f = spec->factor, two_pi = 6.283185307179586476925;
+    const double orig = spec->orig_max_pos;
+    if (r < 2 || r > 256 || (r & 1) || !(theta > 1.0) || !isfinite(theta)) return -2;
+    if (spec->scaling < DPUF_AMD_ROPE_PLAIN || spec->scaling > DPUF_AMD_ROPE_YARN) return -2;
+    if (spec->scaling != DPUF_AMD_ROPE_PLAIN && !(f >= 1.0 && isfinite(f))) return -2;
+    if (spec->scaling >= DPUF_AMD_ROPE_LLAMA3 && spec->orig_max_pos < 1) return -2;
+    if (spec->scaling == DPUF_AMD_ROPE_LLAMA3 &&
+        !(spec->low_freq > 0.0f && spec->high_freq > spec->low_freq && isfinite(spec->high_freq)))
+        return -2;
+    if (spec->scaling == DPUF_AMD_ROPE_YARN &&
+        !(spec->beta_slow > 0.0f && spec->beta_fast > spec->beta_slow && isfinite(spec->beta_fast)))
+        return -2;
+    double lo = 0.0, hi = 0.0;
+    *scale = 1.0f;
+    if (spec->scaling == DPUF_AMD_ROPE_YARN) {
+        /* dims whose pair makes beta turns over the trained positions */
+        lo = floor(r * log(orig / (spec->beta_fast * two_pi)) / (2.0 * log(theta)));
+        hi = ceil(r * log(orig / (spec->beta_slow * two_pi)) / (2.0 * log(theta)));
+        if (lo < 0.0) lo = 0.0;
+        if (hi > r - 1) hi = r - 1;
+        *scale = (float)(f > 1.0 ? 0.1 * log(f) + 1.0 : 1.0);
+    }
+    for (int32_t j = 0; j < r / 2; j++) {
+        double t = pow(theta, -2.0 * j / r) / two_pi;
+        double keep = 1.0; /* share of the frequency left as it is */
+        if (spec->scaling == DPUF_AMD_ROPE_LINEAR) keep = 0.0;
+        if (spec->scaling == DPUF_AMD_ROPE_LLAMA3)
+            keep = (orig * t - spec->low_freq) / ((double)spec->high_freq - spec->low_freq);
+        if (spec->scaling == DPUF_AMD_ROPE_YARN) keep = 1.0 - (j - lo) / (hi - lo > 1e-3 ? hi - lo : 1e-3);
+        keep = keep < 0.0 ? 0.0 : keep > 1.0 ? 1.0 : keep;
+        turns[j] = t * keep + (1.0 - keep) * (keep < 1.0 ? t / f : 0.0);
+    }
+    return 0;
+}
+
+DPUF_EXPORT int32_t dpuf_amd_rope_append(const DpufAmdBatch* batch, const DpufAmdPages* pages,
+                                         const DpufAmdRope* rope, const int32_t* d_positions, int32_t in_type,
+                                         int32_t n_q_heads, const void* d_q, const void* d_k, const void* d_v,
+                                         int64_t q_stride, int64_t k_stride, int64_t v_stride,
+                                         const float* d_q_norm, const float* d_k_norm, float eps, void* d_q_out,
+                                         void* hip_stream) {
+    dpuf_hip_clear_error();
+    int32_t rc = check_pages(pages);
+    if (rc == 0) rc = check_batch(batch, pages);
+    if (rc != 0) return rc;
+    if (in_type != DPUF_AMD_F32 && in_type != DPUF_AMD_BF16 && in_type != DPUF_AMD_F16) return -5;
+    if (!rope || !aligned(rope->turns, 8)) return -1;
+    const int64_t hd = pages->head_dim, nkv = pages->n_kv_heads, es = type_size(in_type);
+    if (rope->rot_dim < 2 || (rope->rot_dim & 1) || rope->rot_dim > hd || !isfinite(rope->scale)) return -2;
+    if (n_q_heads < 0 || n_q_heads > 32 * nkv) return -2;
+    if ((n_q_heads == 0) != (d_q == NULL) || (n_q_heads == 0) != (d_q_out == NULL)) return -1;
+    if (batch->n_rows == 0) return 0;
+    if (!aligned(d_positions, 4) || !aligned(d_k, 16) || !aligned(d_v, 16)) return -1;
+    if (n_q_heads && (!aligned(d_q, 16) || !aligned(d_q_out, 16))) return -1;
+    if ((d_q_norm && !aligned(d_q_norm, 4)) || (d_k_norm && !aligned(d_k_norm, 4))) return -1;
+    if ((d_q_norm || d_k_norm) && !(eps >= 0.0f && isfinite(eps))) return -2;
+    const int64_t st[3] = {q_stride, k_stride, v_stride}, need[3] = {n_q_heads * hd, nkv * hd, nkv * hd};
+    for (int i = n_q_heads ? 0 : 1; i < 3; i++)
+        if (st[i] < need[i] || st[i] % 8 != 0) return -4;
+    const uint64_t out_n = (uint64_t)batch->n_rows * (uint64_t)need[0] * 2u;
+    const int in_place = d_q && d_q_out == d_q && in_type == pages->type && q_stride == need[0];
+    if ((!in_place && overlap(d_q_out, out_n, d_q, span(batch->n_rows, q_stride, need[0], es))) ||
+        overlap(d_q_out, out_n, d_k, span(batch->n_rows, k_stride, need[1], es)) ||
+        overlap(d_q_out, out_n, d_v, span(batch->n_rows, v_stride, need[2], es)))
+        return -1;
+    const void* ps[] = {pages->k, pages->v, pages->w, batch->row_start, batch->ctx_len, batch->page_table, rope->turns,
+                        d_positions, d_q, d_k, d_v, d_q_norm, d_k_norm, d_q_out};
+    const int32_t dev = device_of(ps, (int)(sizeof ps / sizeof ps[0]));
+    if (dev < 0) return -1;
+    ON_DEVICE(dev, dpuf_hip_rope_append(hip_stream, batch, pages, rope, d_positions, in_type, n_q_heads, d_q, d_k, d_v,
+                                        q_stride, k_stride, v_stride, d_q_norm, d_k_norm, eps, d_q_out));
+}
+
+DPUF_EXPORT size_t dpuf_amd_paged_attn_workspace(const DpufAmdBatch* batch, const DpufAmdPages* pages,
+                                                 int32_t n_q_heads) {
+    if (check_pages(pages) != 0 || check_batch(batch, pages) != 0 || check_heads(pages, n_q_heads) != 0) return 0;
+    return dpuf_hip_paged_attn_workspace(batch, pages, n_q_heads);
+}
+
+DPUF_EXPORT int32_t dpuf_amd_paged_attn(const DpufAmdBatch* batch, const DpufAmdPages* pages, int32_t n_q_heads,
+                                        const void* d_q, float scale, int32_t out_type, void* d_out, float* d_lse,
+                                        void* d_workspace, size_t workspace_bytes, void* hip_stream) {
+    dpuf_hip_clear_error();
+    int32_t rc = check_pages(pages);
+    if (rc == 0) rc = check_batch(batch, pages);
+    if (rc == 0) rc = check_heads(pages, n_q_heads);
+    if (rc != 0) return rc;
+    if (out_type != DPUF_AMD_F32 && out_type != pages->type) return -5;
+    if (!(scale > 0.0f) || !isfinite(scale)) return -2;
+    if (batch->n_rows == 0) return 0;
+    if (!aligned(d_q, 16) || !aligned(d_out, 16) || (d_lse && !aligned(d_lse, 4))) return -1;
+    const uint64_t n = (uint64_t)batch->n_rows * (uint64_t)n_q_heads * (uint64_t)pages->head_dim;
+    if (overlap(d_q, n * 2u, d_out, n * (uint64_t)type_size(out_type))) return -1;
+    const size_t ws = dpuf_hip_paged_attn_workspace(batch, pages, n_q_heads);
+    if (ws > 0 && !aligned(d_workspace, 16)) return -1;
+    if (workspace_bytes < ws) return -7;
+    const void* ps[] = {pages->k, pages->v, batch->row_start, batch->ctx_len, batch->page_table, d_q, d_out, d_lse,
+                        ws > 0 ? d_workspace : NULL};
+    const int32_t dev = device_of(ps, (int)(sizeof ps / sizeof ps[0]));
+    if (dev < 0) return -1;
+    ON_DEVICE(dev, dpuf_hip_paged_attn(hip_stream, batch, pages, n_q_heads, d_q, scale, out_type == DPUF_AMD_F32,
+                                       d_out, d_lse, ws > 0 ? d_workspace : NULL));
+}
+
+DPUF_EXPORT int32_t dpuf_amd_paged_attn_weights(const DpufAmdBatch* batch, const DpufAmdPages* pages,
+                                                int32_t n_q_heads, const void* d_q, float scale, const float* d_lse,
+                                                float decay, const float* d_w_in, void* hip_stream) {
+    dpuf_hip_clear_error();
+    int32_t rc = check_pages(pages);
+    if (rc == 0) rc = check_batch(batch, pages);
+    if (rc == 0) rc = check_heads(pages, n_q_heads);
+    if (rc != 0) return rc;
+    if (!(scale > 0.0f) || !isfinite(scale) || !isfinite(decay)) return -2;
+    if (!aligned(pages->w, 4) || (d_w_in && !aligned(d_w_in, 4))) return -1;
+    if (batch->n_rows > 0 && (!aligned(d_q, 16) || !aligned(d_lse, 4))) return -1;
+    const uint64_t n = (uint64_t)pages->n_pages * (uint64_t)pages->n_kv_heads * (uint64_t)pages->page_size * 4u;
+    if (d_w_in != pages->w && overlap(d_w_in, n, pages->w, n)) return -1;
+    const void* ps[] = {pages->k, pages->w, batch->row_start, batch->ctx_len, batch->page_table, d_w_in,
+                        batch->n_rows > 0 ? d_q : NULL, batch->n_rows > 0 ? (const void*)d_lse : NULL};
+    const int32_t dev = device_of(ps, (int)(sizeof ps / sizeof ps[0]));
+    if (dev < 0) return -1;
+    ON_DEVICE(dev, dpuf_hip_paged_attn_weights(hip_stream, batch, pages, n_q_heads, d_q, scale, d_lse, decay, d_w_in));
+}
+
+DPUF_EXPORT int32_t dpuf_amd_paged_evict(const DpufAmdBatch* batch, const DpufAmdPages* pages, int32_t keep,
+                                         int32_t sink, int32_t recent, const DpufAmdPages* dst,
+                                         const int32_t* d_dst_table, int32_t dst_table_stride, int32_t* d_kept,
+                                         int32_t* d_new_len, void* hip_stream) {
+    dpuf_hip_clear_error();
+    int32_t rc = check_pages(pages);
+    if (rc == 0) rc = check_pages(dst);
+    if (rc == 0) rc = check_batch(batch, pages);
+    if (rc != 0) return rc;
+    if (dst->type != pages->type || dst->head_dim != pages->head_dim) return -5;
+    if (dst->n_kv_heads != pages->n_kv_heads) return -2;
+    if (keep < 1 || sink < 0 || recent < 0 || (int64_t)sink + recent > keep) return -2;
+    if (dst_table_stride < 1 || (int64_t)dst_table_stride * dst->page_size > (int64_t)1 << 30 ||
+        keep > (int64_t)dst_table_stride * dst->page_size)
+        return -2;
+    if (!aligned(pages->w, 4) || !aligned(dst->w, 4) || !aligned(d_dst_table, 4) || !aligned(d_kept, 4) ||
+        !aligned(d_new_len, 4))
+        return -1;
+    const uint64_t ns = (uint64_t)batch->n_seqs * 4u, nk = ns * (uint64_t)pages->n_kv_heads * (uint64_t)keep;
+    const uint64_t nt = ns * (uint64_t)batch->table_stride, nd = ns * (uint64_t)dst_table_stride;
+    if (overlap(d_new_len, ns, batch->ctx_len, ns) || overlap(d_new_len, ns, batch->page_table, nt) ||
+        overlap(d_kept, nk, batch->ctx_len, ns) || overlap(d_kept, nk, batch->page_table, nt) ||
+        overlap(d_new_len, ns, d_dst_table, nd) || overlap(d_kept, nk, d_dst_table, nd) ||
+        overlap(d_new_len, ns, d_kept, nk))
+        return -1;
+    const void* ps[] = {pages->k, pages->v, pages->w, dst->k, dst->v, dst->w, batch->ctx_len, batch->page_table,
+                        d_dst_table, d_kept, d_new_len};
+    const int32_t dev = device_of(ps, (int)(sizeof ps / sizeof ps[0]));
+    if (dev < 0) return -1;
+    ON_DEVICE(dev, dpuf_hip_paged_evict(hip_stream, batch, pages, keep, sink, recent, dst, d_dst_table,
+                                        dst_table_stride, d_kept, d_new_len));
+}
+
+DPUF_EXPORT size_t dpuf_amd_sample_workspace(int32_t n, int32_t V) {
+    if (n < 1 || n > MAX_ROWS || V < 1 || V > DPUF_AMD_SAMPLE_MAX_VOCAB) return 0;
+    return dpuf_hip_sample_workspace(n, V);
+}
+
+DPUF_EXPORT int32_t dpuf_amd_sample(int32_t type, int32_t n, int32_t V, int64_t row_stride, const void* d_logits,
+                                    const float* d_temperature, const int32_t* d_top_k, const float* d_top_p,
+                                    const float* d_min_p, const float* d_u, int32_t* d_tokens, float* d_logprobs,
+                                    void* d_workspace, size_t workspace_bytes, void* hip_stream) {
+    dpuf_hip_clear_error();
+    if (type != DPUF_AMD_F32 && type != DPUF_AMD_BF16 && type != DPUF_AMD_F16) return -5;
+    if (n < 1 || n > MAX_ROWS || V < 1 || V > DPUF_AMD_SAMPLE_MAX_VOCAB) return -2;
+    if (row_stride < V) return -4;
+    if (!aligned(d_logits, (uintptr_t)type_size(type)) || !aligned(d_u, 4) || !aligned(d_tokens, 4)) return -1;
+    const void* opt[] = {d_temperature, d_top_k, d_top_p, d_min_p, d_logprobs};
+    for (int i = 0; i < 5; i++)
+        if (opt[i] && !aligned(opt[i], 4)) return -1;
+    const uint64_t nb = (uint64_t)n * 4u, nx = span(n, row_stride, V, type_size(type));
+    if (overlap(d_tokens, nb, d_logprobs, nb) || overlap(d_tokens, nb, d_logits, nx) ||
+        overlap(d_logprobs, nb, d_logits, nx))
+        return -1;
+    const void* in[] = {d_temperature, d_top_k, d_top_p, d_min_p, d_u};
+    for (int i = 0; i < 5; i++)
+        if (overlap(d_tokens, nb, in[i], nb) || overlap(d_logprobs, nb, in[i], nb)) return -1;
+    const size_t ws = dpuf_hip_sample_workspace(n, V);
+    if (ws > 0 && !aligned(d_workspace, 16)) return -1;
+    if (workspace_bytes < ws) return -7;
+    const void* ps[] = {d_logits, d_temperature, d_top_k, d_top_p, d_min_p, d_u, d_tokens, d_logprobs,
+                        ws > 0 ? d_workspace : NULL};
+    const int32_t dev = device_of(ps, (int)(sizeof ps / sizeof ps[0]));
+    if (dev < 0) return -1;
+    ON_DEVICE(dev, dpuf_hip_sample(hip_stream, type, n, V, row_stride, d_logits, d_temperature, d_top_k, d_top_p,
+                                   d_min_p, d_u, d_tokens, d_logprobs, d_workspace));
+}

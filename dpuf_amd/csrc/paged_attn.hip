@@ -1,0 +1,640 @@
+// paged_attn.hip -- attention of new tokens over a paged KV cache.
+//
+// For a new row i of a sequence (query head j, kv head h = j / G, G query
+// heads per kv head), over the cached rows t it sees:
+//     s_t = scale q.k_t,  m = max s_t,  l = sum exp(s_t - m),
+//     o = sum exp(s_t - m) v_t / l,  lse = m + ln l,
+// in one pass over the keys with a running m and l (o and l are multiplied by
+// exp(m_old - m_new) when m grows).  The G heads of a kv head share its keys,
+// so a kernel's row is a "packed" row r = i G + g: every key read serves
+// them all.
+//
+// Both kernels compute the transposed product S^T = K Q^T: a lane of the
+// matrix instruction's result then holds one row and some keys, so maxima and
+// sums are mostly within the lane, and its exponentials are, without any
+// movement, the right-hand operand of O^T = V^T P^T.  The order of the keys
+// within a matrix step is free as long as both operands agree, and V^T's
+// operand takes the order in which S^T left them: 4 keys of each half or
+// quarter of the wave, which is what one transposing LDS read gives.
+//
+// Exponentials are of base 2 with the scale folded in (one fma each); p is
+// rounded to the pages' type for the product with V (a relative half step,
+// 2^-8 in bf16 and 2^-11 in fp16, of each term), every sum is fp32.
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include "hip_internal.h"
+#include "paged.h"
+
+namespace {
+
+const float NEG_INF = -__builtin_huge_valf();
+
+struct PaArgs {
+    DpufAmdBatch b;
+    DpufAmdPages p;
+    int shift;          // log2 of page_size
+    int nq, G;
+    const uint16_t* q;
+    float c2;           // scale * log2 e
+    int few;            // packed rows up to which a sequence takes k_pa_few
+    int nz_few, nz_many; // key ranges a sequence is split into at most
+    int chunk_few, chunk_many;
+    int out_f32;
+    void* out;
+    float* lse;
+    // partial sums of rows whose keys are split: O unnormalised, (m, l);
+    // k_pa_few: [range][sequence][kv head][packed row], k_pa_many:
+    // [range][row][head]
+    float *few_o, *many_o;
+    float2 *few_ml, *many_ml;
+};
+
+// Keys per range of a sequence of ctx keys: `chunk`, or more where nz ranges
+// of it would not reach the end.
+DEV int range_keys(int ctx, int chunk, int nz) {
+    const int need = (ctx + nz - 1) / nz;
+    return need <= chunk ? chunk : (need + 127) & ~127;
+}
+
+// Partial of packed row r of (range z, sequence s, kv head) in k_pa_few's.
+DEV size_t few_at(const PaArgs& a, int z, int s, int kvh, int r) {
+    return (((size_t)z * a.b.n_seqs + s) * a.p.n_kv_heads + kvh) * a.few + r;
+}
+
+// Writes one packed row's four consecutive columns at d, or its partial.
+template <typename T>
+DEV void put4(const PaArgs& a, size_t at, const float* o, float inv) {
+    if (a.out_f32) {
+        *(float4*)((float*)a.out + at) = make_float4(o[0] * inv, o[1] * inv, o[2] * inv, o[3] * inv);
+    } else {
+        uint2 w;
+        w.x = pack2<T>(o[0] * inv, o[1] * inv);
+        w.y = pack2<T>(o[2] * inv, o[3] * inv);
+        *(uint2*)((uint16_t*)a.out + at) = w;
+    }
+}
+
+DEV float lse_of(float m2, float l) { return l > 0.0f ? (m2 + __log2f(l)) * 0.69314718055994531f : NEG_INF; }
+
+// ---------------------------------------------------------------------------
+// Few rows (decode): bound by reading K and V once.  One workgroup per
+// (kv head, sequence and tile of 16 packed rows, key range); its four waves
+// take every fourth tile of 32 keys with sums of their own and meet in LDS at
+// the end, so there is no barrier in the loop and each wave keeps a whole
+// next tile (K and V, 16 KB at 128 columns) in flight in registers.
+// ---------------------------------------------------------------------------
+template <typename T, int HD>
+__global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void k_pa_few(PaArgs a) {
+    constexpr int NC = HD / 32;          // 32-column steps of a key
+    constexpr int ND = HD / 16;          // 16-column tiles of the output
+    constexpr int PITCH = HD + 16;       // elements of a V row in LDS: 4 rows of a transposing read in 4 bank groups
+    typedef typename T::v8 v8;
+    __shared__ __align__(16) uint16_t lds[4][32 * PITCH];
+
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int col = lane & 15, g4 = lane >> 4;
+    const int kvh = blockIdx.x, tiles = (a.few + 15) >> 4;
+    const int s = blockIdx.y / tiles, tile = blockIdx.y - s * tiles;
+    const PgSeq sq = pg_seq(a.b, a.shift, s);
+    const int rows = sq.n * a.G;
+    if (rows > a.few || 16 * tile >= rows) return;
+    const int per = range_keys(sq.ctx, a.chunk_few, a.nz_few);
+    const int ranges = sq.ctx > per ? (sq.ctx + per - 1) / per : 1;
+    const int z = blockIdx.z;
+    if (z >= ranges) return;
+
+    const int r = 16 * tile + col;
+    const bool live = r < rows;
+    const int qi = live ? r / a.G : 0, head = kvh * a.G + (live ? r - qi * a.G : 0);
+    const size_t row = (size_t)(sq.r0 + qi) * a.nq + head;
+    const int limit = live ? sq.ctx - sq.n + qi : -1;             // last key this row sees
+    const int last = min(rows, 16 * tile + 16) - 1;
+    const int first_limit = sq.ctx - sq.n + 16 * tile / a.G;      // of the tile's first row
+    const int k0 = z * per, kend = min(min(sq.ctx - sq.n + last / a.G + 1, sq.ctx), k0 + per);
+
+    v8 qf[NC];
+#pragma unroll
+    for (int c = 0; c < NC; c++)
+        qf[c] = live ? vec_of<v8>(*(const u32x4*)(a.q + row * HD + 32 * c + 8 * g4)) : vec_of<v8>(u32x4{0, 0, 0, 0});
+
+    f32x4 o[ND];
+#pragma unroll
+    for (int d = 0; d < ND; d++) o[d] = f32x4{0.f, 0.f, 0.f, 0.f};
+    float m = NEG_INF, l = 0.0f;
+
+    const uint16_t* kp = (const uint16_t*)a.p.k + (size_t)kvh * a.p.head_stride + 8 * g4;
+    const uint16_t* vp = (const uint16_t*)a.p.v + (size_t)kvh * a.p.head_stride + 8 * g4;
+    const int* table = a.b.page_table + (size_t)s * a.b.table_stride;
+    const int top = sq.ctx > 0 ? (sq.ctx - 1) >> a.shift : 0;
+    uint16_t* lv = lds[wave];
+
+    u32x4 kf[2][NC], vf[2][NC];
+    int pg[2], pn[2];      // pages of the tile in kf / vf, and of the one after it
+    // A 16-key half of a tile lies in one page (pages hold a multiple of 16
+    // rows); halves past the last key repeat it, pages outside the pool read
+    // page 0: both are masked below.
+    auto pages = [&](int base, int* out) {
+#pragma unroll
+        for (int u = 0; u < 2; u++) out[u] = table[min((base + 16 * u) >> a.shift, top)];
+    };
+    auto load = [&](int base, const int* pid) {
+#pragma unroll
+        for (int u = 0; u < 2; u++) {
+            const int key = base + 16 * u + col;
+            const bool in = (unsigned)pid[u] < (unsigned)a.p.n_pages;
+            const size_t off = (size_t)(in ? pid[u] : 0) * a.p.page_stride +
+                               (size_t)(key & (a.p.page_size - 1)) * a.p.row_stride;
+#pragma unroll
+            for (int c = 0; c < NC; c++) kf[u][c] = *(const u32x4*)(kp + off + 32 * c);
+#pragma unroll
+            for (int c = 0; c < NC; c++) vf[u][c] = *(const u32x4*)(vp + off + 32 * c);
+        }
+    };
+
+    int base = k0 + 32 * wave;
+    if (base < kend) {
+        pages(base, pg);
+        load(base, pg);
+        pages(base + 128, pn);
+    }
+    for (; base < kend; base += 128) {
+        // V goes to LDS for the transposing reads; the wave's own LDS
+        // operations are in order, so nothing but the compiler has to be held
+        const bool whole = base + 32 <= min(kend, first_limit + 1) && (unsigned)pg[0] < (unsigned)a.p.n_pages &&
+                           (unsigned)pg[1] < (unsigned)a.p.n_pages;
+        if (!whole) {
+            // a V row that no row of the tile sees may hold anything: 0 * inf
+            // and 0 * NaN would reach the sums
+#pragma unroll
+            for (int u = 0; u < 2; u++)
+                if (base + 16 * u + col >= kend || (unsigned)pg[u] >= (unsigned)a.p.n_pages)
+#pragma unroll
+                    for (int c = 0; c < NC; c++) vf[u][c] = u32x4{0, 0, 0, 0};
+        }
+        lds_order();
+#pragma unroll
+        for (int u = 0; u < 2; u++)
+#pragma unroll
+            for (int c = 0; c < NC; c++) *(u32x4*)(lv + (16 * u + col) * PITCH + 32 * c + 8 * g4) = vf[u][c];
+        f32x4 sc[2] = {f32x4{0.f, 0.f, 0.f, 0.f}, f32x4{0.f, 0.f, 0.f, 0.f}};
+#pragma unroll
+        for (int c = 0; c < NC; c++)
+#pragma unroll
+            for (int u = 0; u < 2; u++) sc[u] = T::mma16(vec_of<v8>(kf[u][c]), qf[c], sc[u]);
+        const int here = base;
+        const bool ok[2] = {(unsigned)pg[0] < (unsigned)a.p.n_pages, (unsigned)pg[1] < (unsigned)a.p.n_pages};
+        if (base + 128 < kend) {
+            pg[0] = pn[0];
+            pg[1] = pn[1];
+            load(base + 128, pg);
+            pages(base + 256, pn);
+        }
+        // keys 16 u + 4 g4 + i of the tile
+        if (!whole) {
+#pragma unroll
+            for (int u = 0; u < 2; u++)
+#pragma unroll
+                for (int i = 0; i < 4; i++)
+                    if (!ok[u] || here + 16 * u + 4 * g4 + i > limit) sc[u][i] = NEG_INF;
+        }
+        float mt = fmaxf(fmaxf(fmaxf(sc[0][0], sc[0][1]), fmaxf(sc[0][2], sc[0][3])),
+                         fmaxf(fmaxf(sc[1][0], sc[1][1]), fmaxf(sc[1][2], sc[1][3])));
+        mt = max_xor32(max_xor16(mt)) * a.c2;
+        const float mn = fmaxf(m, mt), ms = mn == NEG_INF ? 0.0f : mn;
+        if (__any(mn != m)) {
+            const float f = __builtin_amdgcn_exp2f(m - ms);
+            l *= f;
+#pragma unroll
+            for (int d = 0; d < ND; d++) o[d] *= f;
+            m = mn;
+        }
+        float pr[8];
+#pragma unroll
+        for (int u = 0; u < 2; u++)
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                pr[4 * u + i] = __builtin_amdgcn_exp2f(fmaf(sc[u][i], a.c2, -ms));
+                l += pr[4 * u + i];
+            }
+        const u32x4 pw = {pack2<T>(pr[0], pr[1]), pack2<T>(pr[2], pr[3]), pack2<T>(pr[4], pr[5]),
+                          pack2<T>(pr[6], pr[7])};
+        const v8 pf = vec_of<v8>(pw);
+        lds_order();
+        const uint16_t* tr = lv + (4 * g4 + (col >> 2)) * PITCH + 4 * (col & 3);
+#pragma unroll
+        for (int d = 0; d < ND; d++) {
+            const s16x4 lo = lds_tr4(tr + 16 * d), hi = lds_tr4(tr + 16 * PITCH + 16 * d);
+            const uint2 a0 = __builtin_bit_cast(uint2, lo), a1 = __builtin_bit_cast(uint2, hi);
+            o[d] = T::mma16(vec_of<v8>(u32x4{a0.x, a0.y, a1.x, a1.y}), pf, o[d]);
+        }
+    }
+
+    // join the four waves: m, l of the 16 rows, then O by output column
+    l = add_xor32(add_xor16(l));
+    __shared__ float2 ml[4][16];
+    if (lane < 16) ml[wave][lane] = make_float2(m, l);
+    __syncthreads();
+    float M = NEG_INF, L = 0.0f;
+#pragma unroll
+    for (int w = 0; w < 4; w++) M = fmaxf(M, ml[w][col].x);
+    const float Ms = M == NEG_INF ? 0.0f : M;
+#pragma unroll
+    for (int w = 0; w < 4; w++) L += ml[w][col].y * __builtin_amdgcn_exp2f(ml[w][col].x - Ms);
+    const float f = __builtin_amdgcn_exp2f(m - Ms);
+    // [wave][16 rows][HD + 4] floats over the V tiles, a half of the columns
+    // at a time (16 * (HD / 2 + 4) floats fit a wave's 32 * (HD + 16) halves)
+    constexpr int OP = HD / 2 + 4;
+    float* lo = (float*)lds[0];
+    constexpr int WS = 32 * PITCH / 2;   // floats of a wave's region
+#pragma unroll
+    for (int hf = 0; hf < 2; hf++) {
+#pragma unroll
+        for (int d = 0; d < ND / 2; d++) {
+            const f32x4 v = o[hf * (ND / 2) + d] * f;
+            *(f32x4*)(lo + wave * WS + col * OP + 16 * d + 4 * g4) = v;
+        }
+        __syncthreads();
+        for (int e = threadIdx.x; e < 16 * (HD / 8); e += 256) {
+            const int rr = e / (HD / 8), d4 = 4 * (e - rr * (HD / 8));
+            const int pr = 16 * tile + rr;
+            if (pr < rows) {
+                f32x4 v = *(const f32x4*)(lo + rr * OP + d4);
+#pragma unroll
+                for (int w = 1; w < 4; w++) v += *(const f32x4*)(lo + w * WS + rr * OP + d4);
+                const int i = pr / a.G;
+                const size_t orow = (size_t)(sq.r0 + i) * a.nq + kvh * a.G + (pr - i * a.G);
+                const int d = hf * (HD / 2) + d4;
+                if (ranges > 1) {
+                    *(f32x4*)(a.few_o + few_at(a, z, s, kvh, pr) * HD + d) = v;
+                } else {
+                    float Lr = 0.0f, Mr = NEG_INF;
+#pragma unroll
+                    for (int w = 0; w < 4; w++) Mr = fmaxf(Mr, ml[w][rr].x);
+                    const float Mz = Mr == NEG_INF ? 0.0f : Mr;
+#pragma unroll
+                    for (int w = 0; w < 4; w++) Lr += ml[w][rr].y * __builtin_amdgcn_exp2f(ml[w][rr].x - Mz);
+                    const float ov[4] = {v[0], v[1], v[2], v[3]};
+                    put4<T>(a, orow * HD + d, ov, Lr > 0.0f ? 1.0f / Lr : Lr == 0.0f ? 0.0f : Lr);
+                }
+            }
+        }
+        __syncthreads();
+    }
+    if (threadIdx.x < 16 && live) {
+        if (ranges > 1) a.few_ml[few_at(a, z, s, kvh, r)] = make_float2(M, L);
+        else if (a.lse) a.lse[row] = lse_of(M, L);
+    }
+}
+
+// ---------------------------------------------------------------------------
+// Many rows (chunks of a prompt): bound by the matrix instructions and the
+// exponentials.  One workgroup per (kv head, 128 packed rows, key range); its
+// four waves take 32 rows each and share tiles of KT keys of K and V in LDS,
+// two of them: while one is computed, the other takes the tile after it from
+// registers, whose loads were issued a tile earlier.
+// ---------------------------------------------------------------------------
+template <typename T, int HD>
+__global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void k_pa_many(PaArgs a) {
+    constexpr int KT = HD == 256 ? 32 : 64;
+    constexpr int NC = HD / 16;          // 16-column steps of a key
+    constexpr int ND = HD / 32;          // 32-column tiles of the output
+    constexpr int KP = HD + 8;           // K row in LDS: 16 rows' 16 bytes in distinct banks
+    constexpr int VP = HD + 32;          // V row: 4 rows' 64 bytes in distinct banks
+    constexpr int CH = HD / 8;           // 16-byte pieces of a row
+    constexpr int RP = 256 / CH;         // rows a pass of the workgroup loads
+    constexpr int NP = KT / RP;
+    constexpr int NB = KT / 32;          // 32-key blocks of a tile
+    typedef typename T::v8 v8;
+    __shared__ __align__(16) uint16_t lk[2][KT * KP];
+    __shared__ __align__(16) uint16_t lv[2][KT * VP];
+
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int col = lane & 31, h = lane >> 5;
+    const int kvh = blockIdx.x;
+    // sequence and tile of blockIdx.y among the sequences with many rows
+    int s = -1, tile = blockIdx.y;
+    for (int s0 = 0; s0 < a.b.n_seqs && s < 0; s0 += 64) {
+        int n = 0;
+        if (s0 + lane < a.b.n_seqs) {
+            const PgSeq t = pg_seq(a.b, a.shift, s0 + lane);
+            const int rows = t.n * a.G;
+            n = rows > a.few ? (rows + 127) >> 7 : 0;
+        }
+        int sum = n;
+        for (int d = 1; d < 64; d <<= 1) {
+            const int o = __shfl_up(sum, d);
+            if (lane >= d) sum += o;
+        }
+        const uint64_t past = __ballot(sum > tile);
+        if (past) {
+            const int at = __ffsll((unsigned long long)past) - 1;
+            tile -= __shfl(sum - n, at);
+            s = s0 + at;
+        } else {
+            tile -= __shfl(sum, 63);
+        }
+    }
+    s = __builtin_amdgcn_readfirstlane(s);
+    tile = __builtin_amdgcn_readfirstlane(tile);
+    if (s < 0) return;
+    const PgSeq sq = pg_seq(a.b, a.shift, s);
+    const int rows = sq.n * a.G;
+    const int per = range_keys(sq.ctx, a.chunk_many, a.nz_many);
+    const int ranges = sq.ctx > per ? (sq.ctx + per - 1) / per : 1;
+    const int z = blockIdx.z;
+    if (z >= ranges) return;
+
+    const int r = 128 * tile + 32 * wave + col;
+    const bool live = r < rows;
+    const int qi = live ? r / a.G : 0, head = kvh * a.G + (live ? r - qi * a.G : 0);
+    const size_t row = (size_t)(sq.r0 + qi) * a.nq + head;
+    const int limit = live ? sq.ctx - sq.n + qi : -1;
+    // keys past a wave's last row's limit are skipped by the wave, past the
+    // workgroup's by all
+    const int wl = min(rows, 128 * tile + 32 * wave + 32) - 1, gl = min(rows, 128 * tile + 128) - 1;
+    const int first_limit = sq.ctx - sq.n + (128 * tile + 32 * wave) / a.G;
+    const int k0 = z * per;
+    const int wend = 128 * tile + 32 * wave < rows ? min(sq.ctx - sq.n + wl / a.G + 1, k0 + per) : 0;
+    const int kend = min(min(sq.ctx - sq.n + gl / a.G + 1, sq.ctx), k0 + per);
+
+    v8 qf[NC];
+#pragma unroll
+    for (int c = 0; c < NC; c++)
+        qf[c] = live ? vec_of<v8>(*(const u32x4*)(a.q + row * HD + 16 * c + 8 * h)) : vec_of<v8>(u32x4{0, 0, 0, 0});
+    f32x16 o[ND];
+#pragma unroll
+    for (int d = 0; d < ND; d++)
+#pragma unroll
+        for (int i = 0; i < 16; i++) o[d][i] = 0.0f;
+    float m = NEG_INF, l = 0.0f;
+
+    const int lr = threadIdx.x / CH, lc = 8 * (threadIdx.x % CH);   // row and column of this thread's pieces
+    const uint16_t* kp = (const uint16_t*)a.p.k + (size_t)kvh * a.p.head_stride + lc;
+    const uint16_t* vp = (const uint16_t*)a.p.v + (size_t)kvh * a.p.head_stride + lc;
+    const int* table = a.b.page_table + (size_t)s * a.b.table_stride;
+    const int top = sq.ctx > 0 ? (sq.ctx - 1) >> a.shift : 0;
+    const int wr = __builtin_amdgcn_readfirstlane(lr) & ~7;          // the wave's rows lie within 16 of a page
+    u32x4 kf[NP], vf[NP];
+    int pn[NP];
+    auto pages = [&](int base) {
+#pragma unroll
+        for (int u = 0; u < NP; u++) pn[u] = table[min((base + u * RP + wr) >> a.shift, top)];
+    };
+    auto load = [&](int base) {
+#pragma unroll
+        for (int u = 0; u < NP; u++) {
+            const int key = base + u * RP + lr;
+            const bool in = (unsigned)pn[u] < (unsigned)a.p.n_pages;
+            const size_t off = (size_t)(in ? pn[u] : 0) * a.p.page_stride +
+                               (size_t)(key & (a.p.page_size - 1)) * a.p.row_stride;
+            kf[u] = *(const u32x4*)(kp + off);
+            vf[u] = *(const u32x4*)(vp + off);
+            // rows that nobody sees: any bits, and 0 * NaN is NaN
+            if (!in || key >= kend) vf[u] = u32x4{0, 0, 0, 0};
+        }
+    };
+    auto store = [&](int buf) {
+#pragma unroll
+        for (int u = 0; u < NP; u++) {
+            *(u32x4*)(lk[buf] + (u * RP + lr) * KP + lc) = kf[u];
+            *(u32x4*)(lv[buf] + (u * RP + lr) * VP + lc) = vf[u];
+        }
+    };
+
+    if (k0 < kend) {
+        pages(k0);
+        load(k0);
+        pages(k0 + KT);
+        store(0);
+        if (k0 + KT < kend) {
+            load(k0 + KT);
+            pages(k0 + 2 * KT);
+        }
+    }
+    int buf = 0;
+    for (int base = k0; base < kend; base += KT, buf ^= 1) {
+        __syncthreads();
+        if (base + KT < kend) store(buf ^ 1);
+        // pages of this tile that are outside the pool: one bit per 16 keys
+        uint32_t bad = 0;
+        for (int u = 0; u < KT / 16; u++)
+            bad |= ((unsigned)table[min((base + 16 * u) >> a.shift, top)] >= (unsigned)a.p.n_pages) << u;
+        if (base + 2 * KT < kend) {
+            load(base + 2 * KT);
+            pages(base + 3 * KT);
+        }
+        if (base >= wend) continue;
+        f32x16 sc[NB];
+#pragma unroll
+        for (int b = 0; b < NB; b++)
+#pragma unroll
+            for (int i = 0; i < 16; i++) sc[b][i] = 0.0f;
+#pragma unroll
+        for (int c = 0; c < NC; c++)
+#pragma unroll
+            for (int b = 0; b < NB; b++) {
+                const v8 kv = vec_of<v8>(*(const u32x4*)(lk[buf] + (32 * b + col) * KP + 16 * c + 8 * h));
+                sc[b] = T::mma32(kv, qf[c], sc[b]);
+            }
+        // sc[b][i]: key 32 b + 8 (i / 4) + 4 h + i % 4
+        if (base + KT > min(wend, first_limit + 1) || bad) {
+#pragma unroll
+            for (int b = 0; b < NB; b++)
+#pragma unroll
+                for (int i = 0; i < 16; i++) {
+                    const int key = 32 * b + 8 * (i >> 2) + 4 * h + (i & 3);
+                    if (base + key > limit || ((bad >> (key >> 4)) & 1)) sc[b][i] = NEG_INF;
+                }
+        }
+        float mt = NEG_INF;
+#pragma unroll
+        for (int b = 0; b < NB; b++)
+#pragma unroll
+            for (int i = 0; i < 16; i++) mt = fmaxf(mt, sc[b][i]);
+        mt = max_xor32(mt) * a.c2;
+        const float mn = fmaxf(m, mt), ms = mn == NEG_INF ? 0.0f : mn;
+        if (__any(mn != m)) {
+            const float f = __builtin_amdgcn_exp2f(m - ms);
+            l *= f;
+#pragma unroll
+            for (int d = 0; d < ND; d++) o[d] *= f;
+            m = mn;
+        }
+#pragma unroll
+        for (int b = 0; b < NB; b++)
+#pragma unroll
+            for (int k = 0; k < 2; k++) {
+                float pr[8];
+#pragma unroll
+                for (int i = 0; i < 8; i++) {
+                    pr[i] = __builtin_amdgcn_exp2f(fmaf(sc[b][8 * k + i], a.c2, -ms));
+                    l += pr[i];
+                }
+                const u32x4 pw = {pack2<T>(pr[0], pr[1]), pack2<T>(pr[2], pr[3]), pack2<T>(pr[4], pr[5]),
+                                  pack2<T>(pr[6], pr[7])};
+                const v8 pf = vec_of<v8>(pw);
+                // keys 4 h .. + 3 and 8 + 4 h .. + 3 of the 16, columns 16 * (lane / 16 % 2) + lane % 16
+                const uint16_t* tr = lv[buf] + (32 * b + 16 * k + 4 * h + ((lane & 15) >> 2)) * VP +
+                                     16 * ((lane >> 4) & 1) + 4 * (lane & 3);
+#pragma unroll
+                for (int d = 0; d < ND; d++) {
+                    const uint2 a0 = __builtin_bit_cast(uint2, lds_tr4(tr + 32 * d));
+                    const uint2 a1 = __builtin_bit_cast(uint2, lds_tr4(tr + 8 * VP + 32 * d));
+                    o[d] = T::mma32(vec_of<v8>(u32x4{a0.x, a0.y, a1.x, a1.y}), pf, o[d]);
+                }
+            }
+    }
+    l = add_xor32(l);
+    if (!live) return;
+    // o[d][i]: column 32 d + 8 (i / 4) + 4 h + i % 4
+    if (ranges > 1) {
+        float* po = a.many_o + ((size_t)z * a.b.n_rows * a.nq + row) * HD;
+#pragma unroll
+        for (int d = 0; d < ND; d++)
+#pragma unroll
+            for (int i = 0; i < 16; i += 4)
+                *(f32x4*)(po + 32 * d + 2 * i + 4 * h) = f32x4{o[d][i], o[d][i + 1], o[d][i + 2], o[d][i + 3]};
+        if (h == 0) a.many_ml[(size_t)z * a.b.n_rows * a.nq + row] = make_float2(m, l);
+    } else {
+        const float inv = l > 0.0f ? 1.0f / l : l == 0.0f ? 0.0f : l;
+#pragma unroll
+        for (int d = 0; d < ND; d++)
+#pragma unroll
+            for (int i = 0; i < 16; i += 4) {
+                const float ov[4] = {o[d][i], o[d][i + 1], o[d][i + 2], o[d][i + 3]};
+                put4<T>(a, row * HD + 32 * d + 2 * i + 4 * h, ov, inv);
+            }
+        if (h == 0 && a.lse) a.lse[row] = lse_of(m, l);
+    }
+}
+
+// Joins the key ranges of rows that were split: one wave per (row, head).
+template <typename T, int HD>
+__global__ __launch_bounds__(256) void k_pa_join(PaArgs a) {
+    const int lane = threadIdx.x & 63;
+    const int64_t at = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+    const int64_t total = (int64_t)a.b.n_rows * a.nq;
+    if (at >= total) return;
+    const int s = pg_seq_of_row(a.b, (int)(at / a.nq), lane);
+    if (s < 0) return;
+    const PgSeq sq = pg_seq(a.b, a.shift, s);
+    const bool few = sq.n * a.G <= a.few;
+    const int per = range_keys(sq.ctx, few ? a.chunk_few : a.chunk_many, few ? a.nz_few : a.nz_many);
+    const int ranges = sq.ctx > per ? (sq.ctx + per - 1) / per : 1;
+    if (ranges == 1) return;
+    constexpr int E = HD / 64;
+    const int row = (int)(at / a.nq), head = (int)(at - (int64_t)row * a.nq), kvh = head / a.G;
+    const size_t first = few ? few_at(a, 0, s, kvh, (row - sq.r0) * a.G + head - kvh * a.G) : (size_t)at;
+    const size_t step = few ? (size_t)a.b.n_seqs * a.p.n_kv_heads * a.few : (size_t)total;
+    const float2* mls = few ? a.few_ml : a.many_ml;
+    const float* os = few ? a.few_o : a.many_o;
+    float M = NEG_INF;
+    for (int z = 0; z < ranges; z++) M = fmaxf(M, mls[z * step + first].x);
+    const float Ms = M == NEG_INF ? 0.0f : M;
+    float L = 0.0f, o[E] = {};
+    for (int z = 0; z < ranges; z++) {
+        const float2 ml = mls[z * step + first];
+        const float f = __builtin_amdgcn_exp2f(ml.x - Ms);
+        L = fmaf(ml.y, f, L);
+        const float* po = os + (z * step + first) * HD + lane * E;
+#pragma unroll
+        for (int e = 0; e < E; e++) o[e] = fmaf(po[e], f, o[e]);
+    }
+    const float inv = L > 0.0f ? 1.0f / L : L == 0.0f ? 0.0f : L;
+#pragma unroll
+    for (int e = 0; e < E; e++) {
+        const size_t i = (size_t)at * HD + lane * E + e;
+        if (a.out_f32) ((float*)a.out)[i] = o[e] * inv;
+        else ((typename T::e*)a.out)[i] = (typename T::e)(o[e] * inv);
+    }
+    if (lane == 0 && a.lse) a.lse[at] = lse_of(M, L);
+}
+
+struct PaPlan {
+    int few, nz_few, nz_many, chunk_few, chunk_many, y_few, y_many;
+    size_t few_rows, many_rows;   // partial sums in the workspace
+};
+
+int ceil_div(int64_t a, int64_t b) { return (int)((a + b - 1) / b); }
+
+PaPlan plan(const DpufAmdBatch& b, const DpufAmdPages& p, int nq) {
+    const int G = nq / p.n_kv_heads;
+    PaPlan r;
+    r.few = G > 16 ? 32 : 16;
+    const int64_t cap = (int64_t)b.table_stride * p.page_size;
+    const int64_t ctx = b.max_ctx < 1 ? 1 : b.max_ctx < cap ? b.max_ctx : cap;
+    const int64_t packed = (int64_t)b.n_rows * G;
+    r.y_few = b.n_seqs * ((r.few + 15) / 16);
+    const int64_t most = packed / (r.few + 1);
+    r.y_many = (int)(packed <= r.few ? 0 : packed / 128 + (most < b.n_seqs ? most : b.n_seqs));
+    r.chunk_few = 512;
+    r.nz_few = ceil_div(ctx, r.chunk_few);
+    // (kv heads x sequences) that fill the card by themselves need no ranges,
+    // and the partial sums stay below 16 384 x `few` rows
+    const int64_t cap_z = 16384 / ((int64_t)b.n_seqs * p.n_kv_heads);
+    if (r.nz_few > cap_z) r.nz_few = cap_z < 1 ? 1 : (int)cap_z;
+    const int64_t wgs = (packed + 127) / 128 * p.n_kv_heads;
+    int nz = wgs >= 512 ? 1 : ceil_div(512, wgs > 0 ? wgs : 1);
+    if (nz > 16) nz = 16;
+    r.chunk_many = ceil_div(ctx, nz);
+    if (r.chunk_many < 512) r.chunk_many = 512;
+    r.chunk_many = (r.chunk_many + 127) & ~127;
+    r.nz_many = ceil_div(ctx, r.chunk_many);
+    r.few_rows = r.nz_few > 1 ? (size_t)r.nz_few * b.n_seqs * p.n_kv_heads * r.few : 0;
+    r.many_rows = r.y_many > 0 && r.nz_many > 1 ? (size_t)r.nz_many * b.n_rows * nq : 0;
+    return r;
+}
+
+template <typename T, int HD>
+void launch(const PaArgs& a, const PaPlan& pl, hipStream_t st) {
+    const int nkv = a.p.n_kv_heads;
+    hipLaunchKernelGGL((k_pa_few<T, HD>), dim3(nkv, pl.y_few, pl.nz_few), dim3(256), 0, st, a);
+    if (pl.y_many > 0)
+        hipLaunchKernelGGL((k_pa_many<T, HD>), dim3(nkv, pl.y_many, pl.nz_many), dim3(256), 0, st, a);
+    if (pl.nz_few > 1 || (pl.y_many > 0 && pl.nz_many > 1))
+        hipLaunchKernelGGL((k_pa_join<T, HD>), dim3(ceil_div((int64_t)a.b.n_rows * a.nq, 4)), dim3(256), 0, st, a);
+    LAUNCHED("k_pa");
+}
+
+}  // namespace
+
+extern "C" {
+
+size_t dpuf_hip_paged_attn_workspace(const DpufAmdBatch* b, const DpufAmdPages* p, int32_t nq) {
+    const PaPlan pl = plan(*b, *p, nq);
+    return (pl.few_rows + pl.many_rows) * ((size_t)p->head_dim * 4 + 8);
+}
+
+void dpuf_hip_paged_attn(void* s, const DpufAmdBatch* b, const DpufAmdPages* p, int32_t nq, const void* q, float scale,
+                         int32_t out_f32, void* out, float* lse, void* ws) {
+    const PaPlan pl = plan(*b, *p, nq);
+    PaArgs a;
+    a.b = *b;
+    a.p = *p;
+    a.shift = __builtin_ctz(p->page_size);
+    a.nq = nq;
+    a.G = nq / p->n_kv_heads;
+    a.q = (const uint16_t*)q;
+    a.c2 = scale * 1.4426950408889634f;
+    a.few = pl.few;
+    a.nz_few = pl.nz_few;
+    a.nz_many = pl.nz_many;
+    a.chunk_few = pl.chunk_few;
+    a.chunk_many = pl.chunk_many;
+    a.out_f32 = out_f32;
+    a.out = out;
+    a.lse = lse;
+    a.few_o = (float*)ws;
+    a.many_o = a.few_o + pl.few_rows * p->head_dim;
+    a.few_ml = (float2*)(a.many_o + pl.many_rows * p->head_dim);
+    a.many_ml = a.few_ml + pl.few_rows;
+    const bool bf = p->type == DPUF_AMD_BF16;
+    switch (p->head_dim) {
+        case 64: bf ? launch<Bf16, 64>(a, pl, ST(s)) : launch<Fp16, 64>(a, pl, ST(s)); break;
+        case 128: bf ? launch<Bf16, 128>(a, pl, ST(s)) : launch<Fp16, 128>(a, pl, ST(s)); break;
+        default: bf ? launch<Bf16, 256>(a, pl, ST(s)) : launch<Fp16, 256>(a, pl, ST(s)); break;
+    }
+}
+
+}  // extern "C"

@@ -1,0 +1,526 @@
+// paged_cache.hip -- the operators that write a paged KV cache: RoPE with the
+// append of new rows, the attention weight each cached row accumulates, and
+// eviction by it.
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include "hip_internal.h"
+#include "paged.h"
+
+namespace {
+
+// ---------------------------------------------------------------------------
+// RoPE + append.  A head's columns are spread over HD / 8 lanes, 8 each; a
+// group of lanes keeps its columns for every head it takes, so the angles are
+// worked out once per row and lane: in turns, in 64 bits (a position of 2^31
+// times a frequency keeps 2^-22 of a turn), reduced to half a turn, then in
+// fp32.  Pairs half the rotated columns apart meet through LDS within a wave.
+// Bound by launch latency at few rows and by bytes at many.
+// ---------------------------------------------------------------------------
+struct RaArgs {
+    DpufAmdBatch b;
+    DpufAmdPages p;
+    int shift, nq;
+    const double* turns;
+    int rot, inter;
+    float mscale;
+    const int* pos;
+    const void *q, *k, *v;
+    int64_t qs, ks, vs;
+    const float *qn, *kn;
+    float eps;
+    uint16_t* q_out;
+};
+
+template <bool F32, typename T> DEV void load8(const void* base, int64_t at, float* x) {
+    if (F32) {
+        const float4 a = *(const float4*)((const float*)base + at), b = *(const float4*)((const float*)base + at + 4);
+        x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w;
+        x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
+    } else {
+        const typename T::v8 a = vec_of<typename T::v8>(*(const u32x4*)((const uint16_t*)base + at));
+#pragma unroll
+        for (int i = 0; i < 8; i++) x[i] = (float)a[i];
+    }
+}
+
+template <typename TI, bool F32, typename T, int HD>
+__global__ __launch_bounds__(256) void k_rope_append(RaArgs a) {
+    constexpr int LH = HD / 8;                 // lanes of a head
+    constexpr int GROUPS = 256 / LH;
+    __shared__ float xs[256 * 8];
+    const int lane = threadIdx.x & 63;
+    const int row = blockIdx.x;
+    const int s = pg_seq_of_row(a.b, row, lane);
+    if (s < 0) return;
+    const PgSeq sq = pg_seq(a.b, a.shift, s);
+    if (row < sq.r0 || row >= sq.r0 + sq.n) return;
+    const int slot = sq.ctx - sq.n + row - sq.r0;
+    int page = -1;
+    if (slot >= 0 && slot < sq.ctx) page = pg_page(a.b, a.shift, s, slot);
+    const bool put = (unsigned)page < (unsigned)a.p.n_pages;
+    const int in_page = slot & (a.p.page_size - 1);
+
+    const int sub = threadIdx.x % LH, grp = threadIdx.x / LH;
+    const int c0 = 8 * sub, half = a.rot >> 1;
+    const double pos = (double)a.pos[row];
+    float cs[8], sn[8];
+#pragma unroll
+    for (int e = 0; e < 8; e++) {
+        const int c = c0 + e;
+        cs[e] = 1.0f;
+        sn[e] = 0.0f;
+        if (c < a.rot) {
+            const double t = pos * a.turns[a.inter ? c >> 1 : (c < half ? c : c - half)];
+            const float f = (float)(t - rint(t));
+            float si, co;
+            sincospif(2.0f * f, &si, &co);
+            const bool second = a.inter ? (c & 1) : c >= half;
+            cs[e] = co * a.mscale;
+            sn[e] = (second ? si : -si) * a.mscale;
+        }
+    }
+    const int nkv = a.p.n_kv_heads, heads = a.nq + 2 * nkv;
+    for (int h0 = GROUPS * blockIdx.y; h0 < heads; h0 += GROUPS * gridDim.y) {
+        const int hh = h0 + grp;
+        const bool on = hh < heads;
+        const int kind = hh < a.nq ? 0 : hh < a.nq + nkv ? 1 : 2;    // q, k, v
+        const int kh = kind == 0 ? 0 : kind == 1 ? hh - a.nq : hh - a.nq - nkv;
+        float x[8] = {};
+        if (on) {
+            if (kind == 0) load8<F32, TI>(a.q, row * a.qs + (int64_t)hh * HD + c0, x);
+            else if (kind == 1) load8<F32, TI>(a.k, row * a.ks + (int64_t)kh * HD + c0, x);
+            else load8<F32, TI>(a.v, row * a.vs + (int64_t)kh * HD + c0, x);
+        }
+        const float* nw = kind == 0 ? a.qn : kind == 1 ? a.kn : nullptr;
+        if (a.qn || a.kn) {
+            float ss = 0.0f;
+#pragma unroll
+            for (int e = 0; e < 8; e++) ss = fmaf(x[e], x[e], ss);
+#pragma unroll
+            for (int d = 1; d < LH; d <<= 1) ss += __shfl_xor(ss, d);
+            if (nw) {
+                const float r = 1.0f / sqrtf(ss / (float)HD + a.eps);
+#pragma unroll
+                for (int e = 0; e < 8; e++) x[e] = x[e] * r * nw[c0 + e];
+            }
+        }
+        float y[8];
+        if (a.inter) {
+#pragma unroll
+            for (int e = 0; e < 8; e++) y[e] = x[e ^ 1];
+        } else {
+            float* mine = xs + grp * HD;
+            lds_order();
+#pragma unroll
+            for (int e = 0; e < 8; e += 4) *(float4*)(mine + c0 + e) = make_float4(x[e], x[e + 1], x[e + 2], x[e + 3]);
+            lds_order();
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+                const int c = c0 + e;
+                y[e] = mine[c < half ? c + half : c < a.rot ? c - half : c];
+            }
+        }
+        u32x4 w;
+#pragma unroll
+        for (int e = 0; e < 8; e += 2) {
+            float o0 = x[e], o1 = x[e + 1];
+            if (kind != 2) {
+                if (c0 + e < a.rot) o0 = fmaf(x[e], cs[e], y[e] * sn[e]);
+                if (c0 + e + 1 < a.rot) o1 = fmaf(x[e + 1], cs[e + 1], y[e + 1] * sn[e + 1]);
+            }
+            w[e >> 1] = pack2<T>(o0, o1);
+        }
+        if (!on) continue;
+        if (kind == 0) {
+            *(u32x4*)(a.q_out + ((int64_t)row * a.nq + hh) * HD + c0) = w;
+        } else if (put) {
+            uint16_t* dst = (uint16_t*)(kind == 1 ? a.p.k : a.p.v);
+            *(u32x4*)(dst + (int64_t)page * a.p.page_stride + kh * a.p.head_stride + in_page * a.p.row_stride + c0) = w;
+            if (kind == 1 && a.p.w && sub == 0)
+                a.p.w[((size_t)page * nkv + kh) * a.p.page_size + in_page] = 0.0f;
+        }
+    }
+}
+
+// ---------------------------------------------------------------------------
+// Attention weights of cached rows: w' = decay w + sum over packed rows of
+// exp(scale q.k - lse).  The keys stay: a wave holds 32 of them as the left
+// operand of S^T = K Q^T and walks the sequence's rows, 32 at a time, adding
+// the exponentials of its keys in registers; the 32 rows of a step are the
+// lanes, added up once at the end in one order.  A decode step reads K once;
+// a chunk is bound by the matrix instructions and the exponentials.
+// ---------------------------------------------------------------------------
+struct PwArgs {
+    DpufAmdBatch b;
+    DpufAmdPages p;
+    int shift, nq, G;
+    const uint16_t* q;
+    float c2;
+    const float* lse;
+    float decay;
+    const float* w_in;
+};
+
+template <typename T, int HD>
+__global__ __launch_bounds__(256) void k_pa_weights(PwArgs a) {
+    constexpr int NC = HD / 16;
+    typedef typename T::v8 v8;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int col = lane & 31, h = lane >> 5;
+    const int kvh = blockIdx.x, s = blockIdx.y;
+    const PgSeq sq = pg_seq(a.b, a.shift, s);
+    const int rows = sq.n * a.G;
+    for (int base = 128 * blockIdx.z + 32 * wave; base < sq.ctx; base += 128 * gridDim.z) {
+        const int key = min(base + col, sq.ctx - 1);
+        const int page = pg_page(a.b, a.shift, s, key);
+        const bool in = (unsigned)page < (unsigned)a.p.n_pages;
+        const uint16_t* kp = (const uint16_t*)a.p.k + (size_t)(in ? page : 0) * a.p.page_stride +
+                             (size_t)kvh * a.p.head_stride + (size_t)(key & (a.p.page_size - 1)) * a.p.row_stride + 8 * h;
+        v8 kf[NC];
+#pragma unroll
+        for (int c = 0; c < NC; c++) kf[c] = vec_of<v8>(*(const u32x4*)(kp + 16 * c));
+        float acc[16] = {};
+        // rows before the first key of the tile see none of it
+        const int i0 = max(0, base - (sq.ctx - sq.n));
+        for (int r0 = i0 * a.G & ~31; r0 < rows; r0 += 32) {
+            const int r = r0 + col;
+            const bool live = r < rows;
+            const int qi = live ? r / a.G : 0;
+            const size_t row = (size_t)(sq.r0 + qi) * a.nq + kvh * a.G + (live ? r - qi * a.G : 0);
+            const float ls = live ? a.lse[row] : 0.0f;
+            // rows that saw no key (lse -infinity) give nothing
+            const int limit = live && ls != -__builtin_huge_valf() ? sq.ctx - sq.n + qi : -1;
+            const float l2 = ls * 1.4426950408889634f;
+            f32x16 sc;
+#pragma unroll
+            for (int i = 0; i < 16; i++) sc[i] = 0.0f;
+#pragma unroll
+            for (int c = 0; c < NC; c++) {
+                const u32x4 qv = *(const u32x4*)(a.q + row * HD + 16 * c + 8 * h);
+                sc = T::mma32(kf[c], vec_of<v8>(qv), sc);
+            }
+#pragma unroll
+            for (int i = 0; i < 16; i++) {
+                const int kk = base + 8 * (i >> 2) + 4 * h + (i & 3);
+                const float e = __builtin_amdgcn_exp2f(fmaf(sc[i], a.c2, -l2));
+                acc[i] += kk <= limit ? e : 0.0f;
+            }
+        }
+        // over the 32 lanes of each half
+#pragma unroll
+        for (int i = 0; i < 16; i++) {
+#pragma unroll
+            for (int d = 1; d < 32; d <<= 1) acc[i] += __shfl_xor(acc[i], d);
+        }
+        // lane 16 h' + ... : key i of half h is written by lane i of that half
+        float mine = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 16; i++) mine = col == i ? acc[i] : mine;
+        const int kk = base + 8 * (col >> 2) + 4 * h + (col & 3);
+        if (col < 16 && kk < sq.ctx) {
+            const int pg = pg_page(a.b, a.shift, s, kk);
+            if ((unsigned)pg < (unsigned)a.p.n_pages) {
+                const size_t at = ((size_t)pg * a.p.n_kv_heads + kvh) * a.p.page_size + (kk & (a.p.page_size - 1));
+                a.p.w[at] = a.w_in ? fmaf(a.decay, a.w_in[at], mine) : mine;
+            }
+        }
+    }
+}
+
+// ---------------------------------------------------------------------------
+// Eviction.  k_ev_pick: one workgroup per (sequence, kv head) finds the
+// keep - sink - recent largest weights of the middle by radix selection on
+// order-preserving integers (4 passes of 8 bits over LDS, or over memory where
+// the row is longer), then lists the kept rows in order.  k_ev_move copies
+// them, 16 bytes a lane: bound by bytes.
+// ---------------------------------------------------------------------------
+struct EvArgs {
+    DpufAmdBatch b;
+    DpufAmdPages p, d;
+    int shift, dshift;
+    int keep, sink, recent;
+    const int* dtable;
+    int dstride;
+    int* kept;
+    int* new_len;
+    int lds_keys;
+};
+
+// Larger weight, larger integer; NaN and absent rows are 0, below every
+// number (-infinity gives 0x007fffff), and -0 equals +0.
+DEV uint32_t weight_key(float w) {
+    const uint32_t u = __float_as_uint(w + 0.0f);
+    if (w != w) return 0;
+    return u & 0x80000000u ? ~u : u | 0x80000000u;
+}
+
+constexpr int EV_T = 1024;
+
+// Inclusive sums of (a, b) over the workgroup's threads, in thread order, and
+// the totals.
+DEV void scan2(int& x, int& y, int& tx, int& ty, int (*sums)[2]) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+        const int ox = __shfl_up(x, d), oy = __shfl_up(y, d);
+        if (lane >= d) { x += ox; y += oy; }
+    }
+    if (lane == 63) { sums[wave][0] = x; sums[wave][1] = y; }
+    __syncthreads();
+    tx = ty = 0;
+    int bx = 0, by = 0;
+    for (int w = 0; w < EV_T / 64; w++) {
+        if (w == wave) { bx = tx; by = ty; }
+        tx += sums[w][0];
+        ty += sums[w][1];
+    }
+    x += bx;
+    y += by;
+    __syncthreads();
+}
+
+__global__ __launch_bounds__(EV_T) void k_ev_pick(EvArgs a) {
+    extern __shared__ __align__(16) uint32_t keys[];
+    __shared__ int hist[4][256];
+    __shared__ int sums[EV_T / 64][2];
+    __shared__ uint32_t sh_prefix;
+    __shared__ int sh_need;
+    const int kvh = blockIdx.x, s = blockIdx.y, t = threadIdx.x;
+    const PgSeq sq = pg_seq(a.b, a.shift, s);
+    const int c = sq.ctx, n = min(c, a.keep);
+    if (kvh == 0 && t == 0) a.new_len[s] = n;
+    int* kept = a.kept + ((size_t)s * a.p.n_kv_heads + kvh) * a.keep;
+    if (c <= a.keep) {
+        for (int i = t; i < n; i += EV_T) kept[i] = i;
+        return;
+    }
+    const int lo = a.sink, hi = c - a.recent, need = a.keep - a.sink - a.recent;   // of the middle [lo, hi)
+    const int mid = hi - lo;
+    const bool staged = mid <= a.lds_keys;
+    auto fetch = [&](int i) -> uint32_t {
+        const int slot = lo + i, page = pg_page(a.b, a.shift, s, slot);
+        if ((unsigned)page >= (unsigned)a.p.n_pages) return 0;
+        return weight_key(a.p.w[((size_t)page * a.p.n_kv_heads + kvh) * a.p.page_size + (slot & (a.p.page_size - 1))]);
+    };
+    if (staged)
+        for (int i = t; i < mid; i += EV_T) keys[i] = fetch(i);
+    auto key_at = [&](int i) -> uint32_t { return staged ? keys[i] : fetch(i); };
+    if (t == 0) { sh_prefix = 0; sh_need = need; }
+    // the need-th largest key, 8 bits at a time from the top
+    for (int shift = 24; shift >= 0 && need > 0; shift -= 8) {
+        hist[t >> 8][t & 255] = 0;
+        __syncthreads();
+        const uint32_t prefix = sh_prefix;
+        const int left = sh_need;
+        const uint32_t mask = shift == 24 ? 0u : ~0u << (shift + 8);
+        for (int i = t; i < mid; i += EV_T) {
+            const uint32_t k = key_at(i);
+            if ((k & mask) == prefix) atomicAdd(&hist[(t >> 6) & 3][(k >> shift) & 255], 1);
+        }
+        __syncthreads();
+        // the largest digit with at least `left` keys at or above it: threads
+        // 0 .. 255 take the digits from the top
+        int x = t < 256 ? hist[0][255 - t] + hist[1][255 - t] + hist[2][255 - t] + hist[3][255 - t] : 0, y = 0, tx, ty;
+        const int own = x;
+        scan2(x, y, tx, ty, sums);
+        if (t < 256 && x >= left && x - own < left) {
+            sh_prefix = prefix | (uint32_t)(255 - t) << shift;
+            sh_need = left - (x - own);
+        }
+        __syncthreads();
+    }
+    __syncthreads();
+    const uint32_t cut = sh_prefix;
+    const int ties = sh_need;      // of the keys equal to cut, the first this many stay
+    // every thread takes a run of rows; a run's places follow from the counts
+    // of the runs before it
+    const int per = (mid + EV_T - 1) / EV_T, b0 = min(t * per, mid), b1 = min(b0 + per, mid);
+    int above = 0, equal = 0;
+    if (need > 0)
+        for (int i = b0; i < b1; i++) {
+            const uint32_t k = key_at(i);
+            above += k > cut;
+            equal += k == cut;
+        }
+    int xa = above, xe = equal, ta, te;
+    scan2(xa, xe, ta, te, sums);
+    xa -= above;
+    xe -= equal;
+    if (need > 0) {
+        int at = a.sink + xa + min(xe, ties);
+        for (int i = b0; i < b1; i++) {
+            const uint32_t k = key_at(i);
+            if (k > cut || (k == cut && xe < ties)) kept[at++] = lo + i;
+            xe += k == cut;
+        }
+    }
+    for (int i = t; i < a.sink; i += EV_T) kept[i] = i;
+    for (int i = t; i < a.recent; i += EV_T) kept[a.keep - a.recent + i] = hi + i;
+}
+
+template <int HD>
+__global__ __launch_bounds__(256) void k_ev_move(EvArgs a) {
+    constexpr int CH = HD / 8, RP = 256 / CH, NR = 4;
+    const int kvh = blockIdx.x, s = blockIdx.y;
+    const int c = min(max(a.b.ctx_len[s], 0), a.b.table_stride << a.shift), n = min(c, a.keep);
+    const int* kept = a.kept + ((size_t)s * a.p.n_kv_heads + kvh) * a.keep;
+    const int sub = threadIdx.x % CH, rw = threadIdx.x / CH;
+    for (int i0 = blockIdx.z * RP * NR; i0 < n; i0 += gridDim.z * RP * NR) {
+        int from[NR], sp[NR], dp[NR];
+#pragma unroll
+        for (int u = 0; u < NR; u++) {
+            const int i = i0 + u * RP + rw;
+            from[u] = i < n ? kept[i] : 0;
+            dp[u] = i < n ? a.dtable[(size_t)s * a.dstride + (i >> a.dshift)] : -1;
+        }
+#pragma unroll
+        for (int u = 0; u < NR; u++) sp[u] = pg_page(a.b, a.shift, s, min(max(from[u], 0), c - 1));
+        u32x4 kv[NR], vv[NR];
+        float w[NR];
+#pragma unroll
+        for (int u = 0; u < NR; u++) {
+            kv[u] = vv[u] = u32x4{0, 0, 0, 0};
+            w[u] = 0.0f;
+            if ((unsigned)sp[u] < (unsigned)a.p.n_pages) {
+                const int in_page = from[u] & (a.p.page_size - 1);
+                const size_t at = (size_t)sp[u] * a.p.page_stride + (size_t)kvh * a.p.head_stride +
+                                  (size_t)in_page * a.p.row_stride + 8 * sub;
+                kv[u] = *(const u32x4*)((const uint16_t*)a.p.k + at);
+                vv[u] = *(const u32x4*)((const uint16_t*)a.p.v + at);
+                if (sub == 0) w[u] = a.p.w[((size_t)sp[u] * a.p.n_kv_heads + kvh) * a.p.page_size + in_page];
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < NR; u++) {
+            const int i = i0 + u * RP + rw;
+            if (i >= n || (unsigned)dp[u] >= (unsigned)a.d.n_pages) continue;
+            const int in_page = i & (a.d.page_size - 1);
+            const size_t at = (size_t)dp[u] * a.d.page_stride + (size_t)kvh * a.d.head_stride +
+                              (size_t)in_page * a.d.row_stride + 8 * sub;
+            *(u32x4*)((uint16_t*)a.d.k + at) = kv[u];
+            *(u32x4*)((uint16_t*)a.d.v + at) = vv[u];
+            if (sub == 0) a.d.w[((size_t)dp[u] * a.p.n_kv_heads + kvh) * a.d.page_size + in_page] = w[u];
+        }
+    }
+}
+
+template <typename TI, bool F32, typename T> void rope_hd(const RaArgs& a, dim3 g, hipStream_t st) {
+    switch (a.p.head_dim) {
+        case 64: hipLaunchKernelGGL((k_rope_append<TI, F32, T, 64>), g, dim3(256), 0, st, a); break;
+        case 128: hipLaunchKernelGGL((k_rope_append<TI, F32, T, 128>), g, dim3(256), 0, st, a); break;
+        default: hipLaunchKernelGGL((k_rope_append<TI, F32, T, 256>), g, dim3(256), 0, st, a); break;
+    }
+}
+template <typename T> void rope_in(const RaArgs& a, int in_type, dim3 g, hipStream_t st) {
+    if (in_type == DPUF_AMD_F32) rope_hd<Bf16, true, T>(a, g, st);
+    else if (in_type == DPUF_AMD_BF16) rope_hd<Bf16, false, T>(a, g, st);
+    else rope_hd<Fp16, false, T>(a, g, st);
+}
+
+}  // namespace
+
+extern "C" {
+
+void dpuf_hip_rope_append(void* s, const DpufAmdBatch* b, const DpufAmdPages* p, const DpufAmdRope* r, const int32_t* pos,
+                          int32_t in_type, int32_t nq, const void* q, const void* k, const void* v, int64_t qs,
+                          int64_t ks, int64_t vs, const float* qn, const float* kn, float eps, void* q_out) {
+    RaArgs a;
+    a.b = *b;
+    a.p = *p;
+    a.shift = __builtin_ctz(p->page_size);
+    a.nq = nq;
+    a.turns = r->turns;
+    a.rot = r->rot_dim;
+    a.inter = r->interleaved != 0;
+    a.mscale = r->scale;
+    a.pos = pos;
+    a.q = q;
+    a.k = k;
+    a.v = v;
+    a.qs = qs;
+    a.ks = ks;
+    a.vs = vs;
+    a.qn = qn;
+    a.kn = kn;
+    a.eps = eps;
+    a.q_out = (uint16_t*)q_out;
+    // a row's heads by one workgroup, or spread over several while the rows
+    // alone do not give every CU one
+    const int groups = 256 / (p->head_dim / 8), turns = (nq + 2 * p->n_kv_heads + groups - 1) / groups;
+    int y = (dpuf_hip_cu_count() + b->n_rows - 1) / b->n_rows;
+    if (y > turns) y = turns;
+    const dim3 g(b->n_rows, y);
+    if (p->type == DPUF_AMD_BF16) rope_in<Bf16>(a, in_type, g, ST(s));
+    else rope_in<Fp16>(a, in_type, g, ST(s));
+    LAUNCHED("k_rope_append");
+}
+
+void dpuf_hip_paged_attn_weights(void* s, const DpufAmdBatch* b, const DpufAmdPages* p, int32_t nq, const void* q,
+                                 float scale, const float* lse, float decay, const float* w_in) {
+    PwArgs a;
+    a.b = *b;
+    a.p = *p;
+    a.shift = __builtin_ctz(p->page_size);
+    a.nq = nq;
+    a.G = nq / p->n_kv_heads;
+    a.q = (const uint16_t*)q;
+    a.c2 = scale * 1.4426950408889634f;
+    a.lse = lse;
+    a.decay = decay;
+    a.w_in = w_in;
+    const int64_t cap = (int64_t)b->table_stride * p->page_size;
+    const int64_t ctx = b->max_ctx < 1 ? 1 : b->max_ctx < cap ? b->max_ctx : cap;
+    const int64_t z = (ctx + 127) / 128;
+    const dim3 g(p->n_kv_heads, b->n_seqs, (unsigned)(z < 65535 ? z : 65535));
+    const bool bf = p->type == DPUF_AMD_BF16;
+    switch (p->head_dim) {
+        case 64:
+            if (bf) hipLaunchKernelGGL((k_pa_weights<Bf16, 64>), g, dim3(256), 0, ST(s), a);
+            else hipLaunchKernelGGL((k_pa_weights<Fp16, 64>), g, dim3(256), 0, ST(s), a);
+            break;
+        case 128:
+            if (bf) hipLaunchKernelGGL((k_pa_weights<Bf16, 128>), g, dim3(256), 0, ST(s), a);
+            else hipLaunchKernelGGL((k_pa_weights<Fp16, 128>), g, dim3(256), 0, ST(s), a);
+            break;
+        default:
+            if (bf) hipLaunchKernelGGL((k_pa_weights<Bf16, 256>), g, dim3(256), 0, ST(s), a);
+            else hipLaunchKernelGGL((k_pa_weights<Fp16, 256>), g, dim3(256), 0, ST(s), a);
+    }
+    LAUNCHED("k_pa_weights");
+}
+
+void dpuf_hip_paged_evict(void* s, const DpufAmdBatch* b, const DpufAmdPages* p, int32_t keep, int32_t sink,
+                          int32_t recent, const DpufAmdPages* d, const int32_t* dtable, int32_t dstride, int32_t* kept,
+                          int32_t* new_len) {
+    EvArgs a;
+    a.b = *b;
+    a.p = *p;
+    a.d = *d;
+    a.shift = __builtin_ctz(p->page_size);
+    a.dshift = __builtin_ctz(d->page_size);
+    a.keep = keep;
+    a.sink = sink;
+    a.recent = recent;
+    a.dtable = dtable;
+    a.dstride = dstride;
+    a.kept = kept;
+    a.new_len = new_len;
+    // rows of up to 36 864 keys are held in LDS (144 KB of the 160)
+    const int64_t cap = (int64_t)b->table_stride * p->page_size;
+    a.lds_keys = (int)(cap < 36864 ? cap : 36864);
+    const size_t lds = (size_t)a.lds_keys * 4;
+    hipLaunchKernelGGL(k_ev_pick, dim3(p->n_kv_heads, b->n_seqs), dim3(EV_T), lds, ST(s), a);
+    const int rows = 4 * 256 / (p->head_dim / 8);
+    int z = (keep + rows - 1) / rows;
+    if (z > 1024) z = 1024;
+    const dim3 g(p->n_kv_heads, b->n_seqs, z);
+    switch (p->head_dim) {
+        case 64: hipLaunchKernelGGL(k_ev_move<64>, g, dim3(256), 0, ST(s), a); break;
+        case 128: hipLaunchKernelGGL(k_ev_move<128>, g, dim3(256), 0, ST(s), a); break;
+        default: hipLaunchKernelGGL(k_ev_move<256>, g, dim3(256), 0, ST(s), a);
+    }
+    LAUNCHED("k_ev_pick/k_ev_move");
+}
+
+}  // extern "C"

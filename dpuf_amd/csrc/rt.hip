@@ -705,6 +705,25 @@ void dpuf_hip_fill_f32(float* dst, size_t n, float v, void* s) {
     LAUNCHED("k_fill_f32");
 }
 
+int32_t dpuf_hip_ptr_device(const void* p) {
+    hipPointerAttribute_t at;
+    if (hipPointerGetAttributes(&at, p) != hipSuccess) {
+        (void)hipGetLastError();
+        return -1;
+    }
+    return at.type == hipMemoryTypeDevice ? at.device : -1;
+}
+int32_t dpuf_hip_device_enter(int32_t dev) {
+    int cur = -1;
+    CK(hipGetDevice(&cur));
+    if (cur == dev) return -1;
+    CK(hipSetDevice(dev));
+    return cur;
+}
+void dpuf_hip_device_leave(int32_t back) {
+    if (back >= 0) CK(hipSetDevice(back));
+}
+
 void* dpuf_hip_event_create(void) {
     hipEvent_t e = nullptr;
     CK(hipEventCreate(&e));

@@ -151,6 +151,178 @@ DPUF_EXPORT int32_t dpuf_amd_verify_tiles_device(int32_t mode, int32_t n_tiles, 
                                                  const uint8_t* tensor_base, const uint64_t* tile_offsets,
                                                  uint8_t* tile_ok_out);
 
+/* ---- Paged serving -------------------------------------------------------
+ * A KV cache in pages shared by many sequences, and the operators over it:
+ * RoPE with the append of new rows, attention of new tokens, accumulation of
+ * the attention weight each cached row receives, eviction by that weight, and
+ * sampling.  All pointers inside the descriptors and all d_ arguments are
+ * device memory of one device, which need not be the current one; work is
+ * enqueued on hip_stream (a hipStream_t of that device; NULL: its default
+ * stream) without synchronising and may be captured into a HIP graph: lengths,
+ * tables and sampling settings are read on the device, so a replay takes their
+ * current contents.  Nothing is allocated; calls that share a workspace must
+ * not overlap.  No counterparts in the reference.
+ *
+ * Return codes: 0 enqueued; -1 NULL or misaligned pointer, host memory where
+ * device memory is needed, pointers of different devices, or overlapping
+ * arguments; -2 a size or setting out of range; -4 a stride that is not a
+ * multiple of 8 elements or too small; -5 a type or head dim that is not
+ * built; -6 device error (dpuf_amd_last_error); -7 workspace too small. */
+
+/* Element types. */
+enum {
+    DPUF_AMD_F32  = 0,
+    DPUF_AMD_BF16 = 1,
+    DPUF_AMD_F16  = 2
+};
+
+/* One layer's pages.  Row r of page p of kv head h starts at element
+ * p * page_stride + h * head_stride + r * row_stride of k and of v (any order
+ * of the three, each a multiple of 8 elements and at least head_dim; k and v
+ * on 16 bytes).  w holds one accumulated weight per row,
+ * [n_pages][n_kv_heads][page_size], or is NULL where no operator needs it. */
+typedef struct {
+    int32_t type;         /* DPUF_AMD_BF16 or DPUF_AMD_F16 */
+    int32_t n_pages;
+    int32_t page_size;    /* rows: a power of two, 16 to 1024 */
+    int32_t n_kv_heads;
+    int32_t head_dim;     /* 64, 128 or 256 */
+    int64_t page_stride;
+    int64_t head_stride;
+    int64_t row_stride;
+    void* k;
+    void* v;
+    float* w;
+} DpufAmdPages;
+
+/* A ragged batch: sequence s has new rows row_start[s] .. row_start[s + 1] - 1
+ * of the call's n_rows, which are the last of its ctx_len[s] cached rows
+ * (new ones included); its cached row i is row i % page_size of page
+ * page_table[s * table_stride + i / page_size].  A sequence may have no new
+ * rows.  Lengths are clamped to the table and to n_rows; a cached row on a
+ * page outside [0, n_pages) is absent: never read, written or attended to. */
+typedef struct {
+    int32_t n_seqs;              /* 1 to 16384 */
+    int32_t n_rows;              /* 0 to 65536 */
+    int32_t table_stride;        /* table entries per sequence; times page_size at most 2^30 */
+    int32_t max_ctx;             /* about the longest ctx_len: how the work is split, not a bound */
+    const int32_t* row_start;    /* [n_seqs + 1], ascending from 0 */
+    const int32_t* ctx_len;      /* [n_seqs] */
+    const int32_t* page_table;   /* [n_seqs][table_stride] */
+} DpufAmdBatch;
+
+/* How a model turns positions into angles. */
+enum {
+    DPUF_AMD_ROPE_PLAIN  = 0,
+    DPUF_AMD_ROPE_LINEAR = 1,    /* every frequency / factor */
+    DPUF_AMD_ROPE_LLAMA3 = 2,    /* / factor below low_freq turns over orig_max_pos, as is above high_freq */
+    DPUF_AMD_ROPE_YARN   = 3     /* ramp between the dims of beta_fast and beta_slow turns; rotated columns scaled */
+};
+typedef struct {
+    int32_t rot_dim;             /* rotated columns of each head, even, 2 to 256 */
+    float   theta;
+    int32_t scaling;
+    float   factor;
+    float   low_freq, high_freq; /* llama3 */
+    float   beta_fast, beta_slow; /* yarn */
+    int32_t orig_max_pos;        /* llama3, yarn: positions the model was trained on */
+} DpufAmdRopeSpec;
+
+/* Host only: turns[j] = turns per position of pair j (rot_dim / 2 of them)
+ * and *scale, the factor on rotated columns (yarn: 0.1 ln factor + 1, else 1).
+ * 0 ok, -1 NULL, -2 a setting out of range. */
+DPUF_EXPORT int32_t dpuf_amd_rope_turns(const DpufAmdRopeSpec* spec, double* turns, float* scale);
+
+/* A rotation as the device takes it: columns 0 .. rot_dim - 1 of a head in
+ * pairs (j, j + rot_dim / 2), or (2j, 2j + 1) when interleaved; the other
+ * columns stay as they are. */
+typedef struct {
+    const double* turns;         /* device, [rot_dim / 2] */
+    int32_t rot_dim;             /* even, 2 to head_dim */
+    int32_t interleaved;
+    float   scale;
+} DpufAmdRope;
+
+/* New rows of q, k and v (elements of in_type; row strides in elements, each
+ * head's head_dim columns contiguous, rows on 16 bytes): with d_q_norm /
+ * d_k_norm set, the RMSNorm of each head with these head_dim weights; the
+ * rotation by d_positions[row] (0 to 2^31 - 1); then q into d_q_out
+ * [n_rows][n_q_heads][head_dim] (the pages' type; it may be d_q itself where
+ * the types and strides agree) and k and v into the rows' places in the pages,
+ * each rounded once; a written row's weight (pages->w set) becomes 0.  Rows
+ * behind the last sequence's are left as they were.  d_q and d_q_out may both
+ * be NULL (n_q_heads 0): the append alone. */
+DPUF_EXPORT int32_t dpuf_amd_rope_append(const DpufAmdBatch* batch, const DpufAmdPages* pages,
+                                         const DpufAmdRope* rope, const int32_t* d_positions, int32_t in_type,
+                                         int32_t n_q_heads, const void* d_q, const void* d_k, const void* d_v,
+                                         int64_t q_stride, int64_t k_stride, int64_t v_stride,
+                                         const float* d_q_norm, const float* d_k_norm, float eps, void* d_q_out,
+                                         void* hip_stream);
+
+/* Attention of the new rows over the pages: row i of a sequence's n attends
+ * to cached rows 0 .. ctx_len - n + i; query head j to kv head
+ * j / (n_q_heads / n_kv_heads), at most 32 query heads per kv head.  d_q
+ * [n_rows][n_q_heads][head_dim] of the pages' type, on 16 bytes; d_out of the
+ * same shape, out_type that type or DPUF_AMD_F32; d_lse [n_rows][n_q_heads]
+ * (or NULL) the logarithm of each row's sum of exp(scale q.k).  A row with no
+ * cached row to attend to gives 0 and -infinity; rows behind the last
+ * sequence's are left as they were.  Probabilities are rounded to the pages'
+ * type before the product with V, sums are fp32.  d_workspace of at least
+ * dpuf_amd_paged_attn_workspace bytes, on 16 bytes (NULL when that is 0). */
+DPUF_EXPORT size_t dpuf_amd_paged_attn_workspace(const DpufAmdBatch* batch, const DpufAmdPages* pages,
+                                                 int32_t n_q_heads);
+DPUF_EXPORT int32_t dpuf_amd_paged_attn(const DpufAmdBatch* batch, const DpufAmdPages* pages, int32_t n_q_heads,
+                                        const void* d_q, float scale, int32_t out_type, void* d_out, float* d_lse,
+                                        void* d_workspace, size_t workspace_bytes, void* hip_stream);
+
+/* pages->w[row] = decay * d_w_in[row] + the probabilities exp(scale q.k - lse)
+ * that the new rows of the row's sequence give it, summed over rows and over
+ * the query heads of its kv head, for every cached row of the batch; d_w_in is
+ * laid out as w, may be w itself, and counts as 0 when NULL.  d_q and d_lse
+ * are what dpuf_amd_paged_attn took and gave.  No page may be in two of the
+ * batch's sequences.  The same inputs give the same bits. */
+DPUF_EXPORT int32_t dpuf_amd_paged_attn_weights(const DpufAmdBatch* batch, const DpufAmdPages* pages,
+                                                int32_t n_q_heads, const void* d_q, float scale, const float* d_lse,
+                                                float decay, const float* d_w_in, void* hip_stream);
+
+/* Shortens every sequence longer than `keep` rows to keep rows, each kv head
+ * on its own: its first `sink` and last `recent` rows stay, and of the others
+ * the keep - sink - recent with the largest w (NaN and absent rows last; ties:
+ * the earliest); shorter sequences stay whole.  The rows that stay, in order,
+ * and their weights are copied to rows 0 .. of the sequence's pages in
+ * d_dst_table [n_seqs][dst_table_stride] of dst (same type, heads and
+ * head_dim; its w must be set), which must not be pages that any of the
+ * batch's sequences reads (absent source rows copy as zeros).  d_kept
+ * [n_seqs][n_kv_heads][keep] receives their old row numbers (entries past a
+ * sequence's new length are left as they were), d_new_len [n_seqs] the new
+ * lengths.  row_start and n_rows are not read. */
+DPUF_EXPORT int32_t dpuf_amd_paged_evict(const DpufAmdBatch* batch, const DpufAmdPages* pages, int32_t keep,
+                                         int32_t sink, int32_t recent, const DpufAmdPages* dst,
+                                         const int32_t* d_dst_table, int32_t dst_table_stride, int32_t* d_kept,
+                                         int32_t* d_new_len, void* hip_stream);
+
+/* One token from each of n rows (1 to 65536) of V logits (1 to
+ * DPUF_AMD_SAMPLE_MAX_VOCAB; rows row_stride elements apart).
+ * Settings are arrays of n on the device; each may be NULL (off).  Row i:
+ * weights exp((x - max) / temperature), NaN logits counting as -infinity and
+ * +infinity leaving only its like;
+ * top_k (0 or less, or V or more: off) keeps the k largest (ties: the lowest
+ * indices); top_p (1 or more: off) of those the shortest run of largest ones
+ * whose weights reach top_p of their sum, one at least; min_p (0 or less: off)
+ * of those the ones whose weight is at least min_p times the largest.  The
+ * token is the first, in index order, whose running sum of the weights kept
+ * exceeds d_u[i] (in [0, 1); outside: clamped) times their sum; its
+ * logarithmic share of that sum goes to d_logprobs (or NULL).  temperature 0
+ * or less (or NaN): the first largest logit, and 0.  A row with no logit above
+ * -infinity: -1, and -infinity.  Weights are held as integers of at least
+ * 2^-38 of the largest, so sums do not depend on any order. */
+#define DPUF_AMD_SAMPLE_MAX_VOCAB (1 << 24)
+DPUF_EXPORT size_t dpuf_amd_sample_workspace(int32_t n, int32_t V);
+DPUF_EXPORT int32_t dpuf_amd_sample(int32_t type, int32_t n, int32_t V, int64_t row_stride, const void* d_logits,
+                                    const float* d_temperature, const int32_t* d_top_k, const float* d_top_p,
+                                    const float* d_min_p, const float* d_u, int32_t* d_tokens, float* d_logprobs,
+                                    void* d_workspace, size_t workspace_bytes, void* hip_stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,240 @@
+"""Attention of new tokens over a paged cache, and the attention weights of
+cached rows, against float64 from the definition: ragged batches, odd lengths,
+every head dim and grouping the kernels are built for, rows nobody may see."""
+import ctypes as C
+
+import numpy as np
+import pytest
+
+import paged_ref as R
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture()
+def hip(eng):
+    h = R.Hip()
+    yield h
+    h.free_all()
+
+
+def say(*a):
+    print(*a, flush=True)
+
+
+def call(eng, hip, cache, nq, q, scale, out_t=None, max_ctx=None, extra=0, stream=None, lse=True):
+    """Outputs and lse of one call; `extra` rows behind the last sequence's."""
+    out_t = cache.t if out_t is None else out_t
+    n = cache.n_rows + extra
+    qs = np.concatenate([q, np.zeros((extra,) + q.shape[1:], q.dtype)])
+    dq = hip.put(qs)
+    fill = R.to_type(np.full((n, nq, cache.hd), 7.5, np.float32), out_t)
+    do, dl = hip.put(fill), hip.put(np.full((n, nq), 7.5, np.float32))
+    b, p = cache.batch(max_ctx, n), cache.pages(w=False)
+    ws = int(eng.dpuf_amd_paged_attn_workspace(C.byref(b), C.byref(p), nq))
+    dws = hip.put(np.full(max(ws, 16), 0xFF, np.uint8))        # NaN: nothing may rely on a cleared workspace
+    rc = eng.dpuf_amd_paged_attn(C.byref(b), C.byref(p), nq, dq.p, scale, out_t, do.p, dl.p if lse else None,
+                                 dws.p if ws else None, ws, stream)
+    assert rc == 0, (rc, eng.dpuf_amd_last_error())
+    return R.from_type(do.get(), out_t), dl.get(), dq, dl, ws
+
+
+def check(cache, nq, q, scale, out, lse, out_t):
+    n = cache.n_rows
+    ref, rl, A, S, vmax, _ = R.attention(cache, R.from_type(q, cache.t), scale, nq)
+    bound = R.attention_bound(cache.t, out_t, ref, A, S, vmax, cache.hd, max(cache.ctx))
+    err = np.abs(out[:n] - ref)
+    worst = float((err / bound).max()) if err.size else 0.0
+    say(f"  worst error {worst:.3f} of the bound")
+    assert np.all(err <= bound)
+    empty = np.isneginf(rl)
+    assert np.array_equal(np.isneginf(lse[:n]), empty)
+    assert np.all(out[:n][empty] == 0.0)
+    dl = np.abs(lse[:n][~empty] - rl[~empty])
+    assert np.all(dl <= R.score_error(S, cache.hd)[~empty] + np.abs(rl[~empty]) * 2.0 ** -22 + 2.0 ** -20)
+    assert np.all(out[n:] == 7.5) and np.all(lse[n:] == 7.5)
+
+
+# rows, contexts: a first token, lengths around 16, 32, 64 and 128, an empty sequence, one without new rows, one with
+# more new rows than cached ones, a chunk of a longer context
+RAGGED = ([1, 1, 0, 3, 1, 40, 2, 1, 0, 5], [1, 17, 0, 3, 130, 95, 64, 33, 50, 3])
+
+
+@pytest.mark.parametrize("t", [R.BF16, R.F16])
+@pytest.mark.parametrize("nq,nkv,hd,page", [(4, 1, 64, 16), (4, 4, 128, 32), (10, 2, 128, 16), (8, 1, 256, 64),
+                                            (16, 2, 64, 128), (32, 1, 128, 16), (14, 2, 64, 1024), (21, 7, 256, 16)])
+def test_ragged(eng, hip, nq, nkv, hd, page, t):
+    rng = np.random.default_rng(nq * 1000 + hd + t)
+    cache = R.Cache(hip, rng, t, *RAGGED, nkv, hd, page, slots_first=bool(nq & 2))
+    q = R.to_type(rng.standard_normal((cache.n_rows, nq, hd)) * 1.5, t)
+    scale = float(np.float32(1 / np.sqrt(hd)))
+    say(f"ragged: {nq}/{nkv} heads of {hd}, pages of {page}, type {t}")
+    out, lse, *_ = call(eng, hip, cache, nq, q, scale, extra=3)
+    check(cache, nq, q, scale, out, lse, t)
+
+
+@pytest.mark.parametrize("max_ctx", [1, 700, 100000])
+@pytest.mark.parametrize("hd,rows,ctx", [(128, [1, 1, 2], [1300, 5, 2111]), (64, [150], [1999]), (256, [70, 1], [1100, 900])])
+def test_split_over_the_keys(eng, hip, hd, rows, ctx, max_ctx):
+    """Long contexts of few rows go over several workgroups, whatever the
+    caller's estimate of the longest context is."""
+    rng = np.random.default_rng(hd + max_ctx)
+    cache = R.Cache(hip, rng, R.BF16, rows, ctx, 2, hd, 32, table_extra=3100)
+    q = R.to_type(rng.standard_normal((cache.n_rows, 6, hd)) * 1.5, R.BF16)
+    say(f"split: hd {hd}, rows {rows}, contexts {ctx}, max_ctx {max_ctx}")
+    out, lse, *_, ws = call(eng, hip, cache, 6, q, 0.11, out_t=R.F32, max_ctx=max_ctx)
+    assert (ws > 0) == (max_ctx > 512)
+    check(cache, 6, q, 0.11, out, lse, R.F32)
+
+
+@pytest.mark.parametrize("rows,ctx", [([1, 2, 60], [90, 140, 180]), ([600], [700])])
+def test_pages_outside_the_pool_are_absent(eng, hip, rows, ctx):
+    rng = np.random.default_rng(5)
+    bad = [(0, 1), (0, 4), (0, 5)] + ([(1, 0), (2, 3), (2, 7)] if len(ctx) > 1 else [(0, 0), (0, 43)])
+    cache = R.Cache(hip, rng, R.F16, rows, ctx, 2, 64, 16, bad=bad)
+    q = R.to_type(rng.standard_normal((cache.n_rows, 4, 64)), R.F16)
+    say(f"bad pages: rows {rows}")
+    out, lse, *_ = call(eng, hip, cache, 4, q, 0.125, extra=1)
+    check(cache, 4, q, 0.125, out, lse, R.F16)
+
+
+def test_lengths_beyond_the_table(eng, hip):
+    """Lengths are clamped to the page table: a context of more rows than the
+    table's pages hold reads those."""
+    rng = np.random.default_rng(6)
+    cache = R.Cache(hip, rng, R.BF16, [1, 4], [32, 32], 1, 64, 16, table_extra=0)
+    q = R.to_type(rng.standard_normal((5, 2, 64)), R.BF16)
+    say("lengths beyond the table")
+    cache.d_ctx.set(np.array([2 ** 31 - 1, 40], np.int32))
+    out, lse, *_ = call(eng, hip, cache, 2, q, 0.125)
+    check(cache, 2, q, 0.125, out, lse, R.BF16)
+
+
+def test_scores_far_apart(eng, hip):
+    """Scores of a few hundred: the running maximum moves, what it left is 0."""
+    rng = np.random.default_rng(8)
+    for rows, ctx in (([1, 3], [300, 77]), ([90], [333])):
+        cache = R.Cache(hip, rng, R.BF16, rows, ctx, 2, 128, 16, kscale=9.0)
+        q = R.to_type(rng.standard_normal((cache.n_rows, 8, 128)) * 9.0, R.BF16)
+        say(f"far scores: rows {rows}")
+        out, lse, *_ = call(eng, hip, cache, 8, q, 0.088)
+        check(cache, 8, q, 0.088, out, lse, R.BF16)
+
+
+@pytest.mark.parametrize("t", [R.BF16, R.F16])
+@pytest.mark.parametrize("nq,nkv,hd,page", [(4, 1, 64, 16), (10, 2, 128, 32), (8, 1, 256, 64), (32, 1, 128, 16)])
+def test_weights(eng, hip, nq, nkv, hd, page, t):
+    rng = np.random.default_rng(nq + hd)
+    bad = [(4, 3), (5, 0)] if page == 16 else []
+    cache = R.Cache(hip, rng, t, *RAGGED, nkv, hd, page, slots_first=t == R.F16, bad=bad)
+    q = R.to_type(rng.standard_normal((cache.n_rows, nq, hd)) * 1.5, t)
+    scale, decay = 1 / np.sqrt(hd), 0.75
+    say(f"weights: {nq}/{nkv} heads of {hd}, pages of {page}, type {t}")
+    _, lse, dq, dl, _ = call(eng, hip, cache, nq, q, scale)
+    _, rl, _, S, _, fresh = R.attention(cache, R.from_type(q, t), float(np.float32(scale)), nq)
+    outs = []
+    for w_in in (cache.dw, cache.dw, None):
+        dst = hip.put(np.full_like(cache.w, -3.0))
+        b, p = cache.batch(max_ctx=60), cache.pages(dw=dst)
+        rc = eng.dpuf_amd_paged_attn_weights(C.byref(b), C.byref(p), nq, dq.p, scale, dl.p, decay,
+                                             w_in.p if w_in else None, None)
+        assert rc == 0, (rc, eng.dpuf_amd_last_error())
+        outs.append(dst.get())
+    assert np.array_equal(outs[0].view(np.uint32), outs[1].view(np.uint32))
+    # exp(score - lse): two score errors, the lse's own rounding; sums of every row's share in fp32
+    rel = 2 * R.score_error(S.max(initial=0), hd) + np.abs(rl[np.isfinite(rl)]).max() * 2.0 ** -22 + 2.0 ** -20
+    rel += (max(cache.rows) * nq // nkv + 40) * 2.0 ** -24
+    for out, d in ((outs[0], decay), (outs[2], 0.0)):
+        left = np.ones_like(out, bool)
+        for s, c in enumerate(cache.ctx):
+            for i in range(c):
+                if not cache.ok(s, i):
+                    continue
+                pg, r = cache.table[s, i // page], i % page
+                left[pg, :, r] = False
+                old = cache.w[pg, :, r].astype(np.float64) * d
+                want = old + fresh[s][:, i]
+                assert np.all(np.abs(out[pg, :, r] - want) <= rel * fresh[s][:, i] + 2.0 ** -22 * np.abs(old) + 1e-30), \
+                    (s, i)
+        assert np.all(out[left] == -3.0)
+    # in place, and without new rows: the decay alone
+    b, p = cache.batch(n_rows=0), cache.pages()
+    assert eng.dpuf_amd_paged_attn_weights(C.byref(b), C.byref(p), nq, None, scale, None, decay, cache.dw.p, None) == 0
+    got = cache.dw.get()
+    for s, c in enumerate(cache.ctx):
+        for i in range(c):
+            if cache.ok(s, i):
+                pg, r = cache.table[s, i // page], i % page
+                assert np.array_equal(got[pg, :, r], cache.w[pg, :, r] * np.float32(decay))
+
+
+def test_two_streams_and_a_graph(eng, hip):
+    """Two calls at once on streams of their own with workspaces of their own;
+    then a captured call replayed over new lengths and values between eager
+    calls gives what the eager call gives."""
+    rng = np.random.default_rng(11)
+    nq, hd = 8, 128
+    caches = [R.Cache(hip, rng, R.BF16, rows, ctx, 2, hd, 32) for rows, ctx in
+              (([1, 1, 1], [900, 1500, 3]), ([200, 1], [800, 700]))]
+    work = []
+    for cache in caches:
+        q = R.to_type(rng.standard_normal((cache.n_rows, nq, hd)) * 1.5, R.BF16)
+        b, p = cache.batch(), cache.pages(w=False)
+        n = int(eng.dpuf_amd_paged_attn_workspace(C.byref(b), C.byref(p), nq))
+        work.append((cache, q, hip.put(q), hip.put(np.zeros((cache.n_rows, nq, hd), np.uint16)),
+                     hip.put(np.zeros((cache.n_rows, nq), np.float32)), hip.put(np.zeros(max(16, n), np.uint8)), n, b,
+                     p, hip.stream()))
+
+    def launch(wk, s):
+        cache, q, dq, do, dl, ws, n, b, p, _ = wk
+        assert eng.dpuf_amd_paged_attn(C.byref(b), C.byref(p), nq, dq.p, 0.09, R.BF16, do.p, dl.p, ws.p, n, s) == 0
+
+    say("two streams")
+    for _ in range(3):
+        for wk in work:
+            launch(wk, wk[-1])
+    for wk in work:
+        assert hip.lib.hipStreamSynchronize(wk[-1]) == 0
+        check(wk[0], nq, wk[1], 0.09, R.from_type(wk[3].get(), R.BF16), wk[4].get(), R.BF16)
+    say("graph")
+    wk = work[0]
+    cache, q, dq, do, dl, *_, s = wk
+    graph, ge = C.c_void_p(), C.c_void_p()
+    assert hip.lib.hipStreamBeginCapture(s, 1) == 0
+    launch(wk, s)
+    assert hip.lib.hipStreamEndCapture(s, C.byref(graph)) == 0
+    assert hip.lib.hipGraphInstantiate(C.byref(ge), graph, None, None, 0) == 0
+    for ctx in ([900, 1500, 3], [10, 1480, 3], [33, 0, 1], [899, 1499, 2]):
+        cache.d_ctx.set(np.array(ctx, np.int32))
+        cache.ctx = ctx
+        do.set(np.full((3, nq, hd), 0x7FC0, np.uint16))
+        assert hip.lib.hipGraphLaunch(ge, s) == 0
+        assert hip.lib.hipStreamSynchronize(s) == 0
+        got, gl = do.get(), dl.get()
+        check(cache, nq, q, 0.09, R.from_type(got, R.BF16), gl, R.BF16)
+        launch(wk, s)
+        assert hip.lib.hipStreamSynchronize(s) == 0
+        assert np.array_equal(do.get(), got) and np.array_equal(dl.get().view(np.uint32), gl.view(np.uint32))
+    hip.lib.hipGraphExecDestroy(ge)
+    hip.lib.hipGraphDestroy(graph)
+    for wk in work:
+        hip.lib.hipStreamDestroy(wk[-1])
+
+
+def test_host_memory_is_refused(eng, hip):
+    rng = np.random.default_rng(12)
+    cache = R.Cache(hip, rng, R.BF16, [1], [20], 1, 64, 16)
+    q = hip.put(np.zeros((1, 1, 64), np.uint16))
+    out = hip.put(np.zeros((1, 1, 64), np.uint16))
+    host = np.zeros(4096, np.int32)
+    b, p = cache.batch(), cache.pages(w=False)
+    ok = lambda: eng.dpuf_amd_paged_attn(C.byref(b), C.byref(p), 1, q.p, 1.0, R.BF16, out.p, None, None, 0, None)
+    assert ok() == 0
+    for name in ("row_start", "ctx_len", "page_table"):
+        keep = getattr(b, name)
+        setattr(b, name, host.ctypes.data)
+        assert ok() == -1, name
+        setattr(b, name, keep)
+    p.k = host.ctypes.data & ~15
+    assert ok() == -1
+    hip.sync()
