@@ -145,6 +145,17 @@ class DpufAmdRope(C.Structure):
     ]
 
 
+class DpufAmdSampling(C.Structure):
+    """Host arrays of an engine call's sampling settings (include/dpuf_amd.h)."""
+    _fields_ = [
+        ("temperature", C.c_void_p),
+        ("top_k", C.c_void_p),
+        ("top_p", C.c_void_p),
+        ("min_p", C.c_void_p),
+        ("u", C.c_void_p),
+    ]
+
+
 P = C.c_void_p
 I32 = C.c_int32
 F32P = C.POINTER(C.c_float)
@@ -287,5 +298,12 @@ def load_engine():
     _sig(lib, "dpuf_amd_paged_evict", I32, [batch, pages, I32, I32, I32, pages, P, I32, P, P, P])
     _sig(lib, "dpuf_amd_sample_workspace", C.c_size_t, [I32, I32])
     _sig(lib, "dpuf_amd_sample", I32, [I32, I32, I32, I64, P, P, P, P, P, P, P, P, P, C.c_size_t, P])
+    smp = C.POINTER(DpufAmdSampling)
+    _sig(lib, "dpuf_amd_engine_forward_sample", I32, [P, I32, P, I32, P, I32, smp, P, P, P])
+    _sig(lib, "dpuf_amd_engine_forward_slots_sample", I32, [P, I32, P, P, P, smp, P, P, P])
+    _sig(lib, "dpuf_amd_engine_pages_create", I32, [P, I32, I32, I32])
+    _sig(lib, "dpuf_amd_engine_pages", I32, [P, I32, pages])
+    _sig(lib, "dpuf_amd_engine_forward_pages", I32, [P, I32, P, P, P, I32, P, P, F32, smp, P, P, P])
+    _sig(lib, "dpuf_amd_engine_evict_pages", I32, [P, I32, P, P, I32, I32, I32, I32, P, I32, P])
     _engine = lib
     return lib

@@ -131,6 +131,26 @@ typedef struct {
     int32_t host_pos0;
     int32_t capturing;
     int32_t cap_lmax;
+    /* sampling (dpuf_amd_sample): settings and random numbers of up to B
+     * tokens [5][B] through pinned staging, tokens and log probabilities */
+    float *h_smp, *d_smp;
+    void* d_smp_ws;
+    size_t smp_ws;
+    /* the paged cache (dpuf_amd_engine_pages_create): every layer's pages one
+     * after the other; the rotated queries and the rows' lse of the layer at
+     * work; the tables of the call at work through pinned staging */
+    int32_t pg_type, pg_n, pg_size;
+    uint16_t *pg_k, *pg_v, *pg_q;
+    float *pg_w, *pg_lse;
+    double* pg_turns;
+    DpufAmdRope pg_rope;
+    void* pg_ws;
+    size_t pg_ws_bytes;
+    int32_t *h_pg, *d_pg;
+    size_t pg_ints;
+    DpufAmdBatch pg_b;   /* of the call at work; n_seqs 0: the layers run over slots */
+    int32_t* pg_pos;
+    float pg_decay;
 } Engine;
 
 #define IO_POS DPUF_AMD_MAX_BATCH
@@ -482,10 +502,27 @@ static void prefix_copy(Engine* e, int32_t s, int32_t p, int32_t len, int to_pre
     }
 }
 
+static void pages_free(Engine* e) {
+    void* const d[] = {e->pg_k, e->pg_v, e->pg_w, e->pg_q, e->pg_lse, e->pg_turns, e->pg_ws, e->d_pg};
+    for (size_t i = 0; i < sizeof d / sizeof d[0]; i++) dpuf_hip_free(d[i]);
+    dpuf_hip_host_free(e->h_pg);
+    e->pg_k = e->pg_v = e->pg_q = NULL;
+    e->pg_w = e->pg_lse = NULL;
+    e->pg_turns = NULL;
+    e->pg_ws = NULL;
+    e->h_pg = e->d_pg = NULL;
+    e->pg_ws_bytes = e->pg_ints = 0;
+    e->pg_n = 0;
+}
+
 static void engine_free(Engine* e) {
     if (!e) return;
     dpuf_hip_bind_error_word(NULL);
     if (e->stream) dpuf_hip_sync(e->stream);
+    pages_free(e);
+    dpuf_hip_host_free(e->h_smp);
+    dpuf_hip_free(e->d_smp);
+    dpuf_hip_free(e->d_smp_ws);
     for (int i = 0; i < N_GRAPHS; i++) dpuf_hip_graph_destroy(e->graphs[i]);
     for (int32_t i = 0; i < e->n_ups; i++) {
         dpuf_hip_free(e->ups[i].d_groups); dpuf_hip_free(e->ups[i].d_sign);
@@ -646,6 +683,11 @@ DPUF_EXPORT void* dpuf_engine_create(const DpufModelConfig* cfg, const DpufLayer
         e->d_ms_vc = e->d_ms_kc + B;
         e->d_ms_pos = (int32_t*)(e->d_ms_vc + B);
         e->d_ms_tok = e->d_ms_pos + B;
+        e->h_smp = (float*)dpuf_hip_host_alloc(B * 7 * 4);
+        e->d_smp = (float*)dpuf_hip_malloc(B * 7 * 4);
+        e->smp_ws = e->V <= DPUF_AMD_SAMPLE_MAX_VOCAB ? dpuf_hip_sample_workspace((int32_t)B, e->V) : 0;
+        if (e->smp_ws) e->d_smp_ws = dpuf_hip_malloc(e->smp_ws);
+        if (!e->h_smp || !e->d_smp || (e->smp_ws && !e->d_smp_ws)) goto fail;
         if (!e->h || !e->h2 || !e->hn || !e->q || !e->k || !e->v || !e->ao || !e->gate || !e->up || !e->logits ||
             !e->scores || !e->embeds || !e->d_ids || !e->h_pinned || !e->h_io || !e->h_logits || !e->h_emb || !e->d_red || !e->d_lmred || !e->h_ms || !e->h_tok)
             goto fail;
@@ -949,6 +991,36 @@ static void enqueue_ms_attention(Engine* e, int32_t l, int32_t M, float eps, flo
     if (ns < M) dpuf_hip_prep(s, M, e->qd, e->ao, o_sign, e->prep[0]);
 }
 
+/* Layer l's pages. */
+static DpufAmdPages pages_of(const Engine* e, int32_t l) {
+    const size_t rows = (size_t)e->pg_n * e->nkv * e->pg_size, at = (size_t)l * rows;
+    DpufAmdPages p;
+    p.type = e->pg_type;
+    p.n_pages = e->pg_n;
+    p.page_size = e->pg_size;
+    p.n_kv_heads = e->nkv;
+    p.head_dim = e->hd;
+    p.row_stride = e->hd;
+    p.head_stride = (int64_t)e->pg_size * e->hd;
+    p.page_stride = e->nkv * p.head_stride;
+    p.k = e->pg_k + at * e->hd;
+    p.v = e->pg_v + at * e->hd;
+    p.w = e->pg_w + at;
+    return p;
+}
+
+/* QK-norm, RoPE, the append to layer l's pages and the attention of the
+ * call's rows over them, into e->ao; with pg_decay >= 0 the weights too. */
+static void enqueue_paged_attention(Engine* e, int32_t l, float scale, float eps) {
+    void* s = e->stream;
+    const DpufAmdPages p = pages_of(e, l);
+    dpuf_hip_rope_append(s, &e->pg_b, &p, &e->pg_rope, e->pg_pos, DPUF_AMD_F32, e->nq, e->q, e->k, e->v, e->qd, e->kvd,
+                         e->kvd, e->d_norm[4 * l + 1], e->d_norm[4 * l + 2], eps, e->pg_q);
+    dpuf_hip_paged_attn(s, &e->pg_b, &p, e->nq, e->pg_q, scale, 1, e->ao, e->pg_lse, e->pg_ws);
+    if (e->pg_decay >= 0.0f)
+        dpuf_hip_paged_attn_weights(s, &e->pg_b, &p, e->nq, e->pg_q, scale, e->pg_lse, e->pg_decay, p.w);
+}
+
 static void enqueue_layers(Engine* e, int32_t M, int32_t keep_tiles) {
     void* s = e->stream;
     const int32_t H = e->H, I = e->I;
@@ -1000,7 +1072,12 @@ static void enqueue_layers(Engine* e, int32_t M, int32_t keep_tiles) {
         {
             const int tm = tm_begin(e, K_ATTN, 0);
             int fused = 0;
-            if (e->ms_n > 0) {
+            if (e->pg_b.n_seqs > 0) {
+                enqueue_paged_attention(e, l, scale, eps);
+                if (M > 1) dpuf_hip_prep(s, M, e->qd, e->ao, W[W_O].sign, e->prep[0]);
+                o_prep = M == 1;
+                fused = 1;
+            } else if (e->ms_n > 0) {
                 /* one token per session, each against its own slot's cache */
                 enqueue_ms_attention(e, l, M, eps, scale, W[W_O].sign);
                 fused = 1;
@@ -1184,10 +1261,36 @@ static int enqueue_head(Engine* e, int32_t M, int32_t only_last, int32_t early_t
     return 0;
 }
 
+static int sampling_ok(const Engine* e, const DpufAmdSampling* smp) {
+    return smp && smp->u && e->V <= DPUF_AMD_SAMPLE_MAX_VOCAB;
+}
+
+/* Draws a token from each of the first n rows of e->logits (row m by the
+ * caller's settings ord[m], or m) into h_smp: [5] the tokens, [6] the log
+ * probabilities, valid once the stream has drained. */
+static void enqueue_sample(Engine* e, int32_t n, const int32_t* ord, const DpufAmdSampling* smp) {
+    const size_t B = DPUF_AMD_MAX_BATCH;
+    const void* src[5] = {smp->temperature, smp->top_k, smp->top_p, smp->min_p, smp->u};
+    const void* dev[5];
+    for (int k = 0; k < 5; k++) {
+        dev[k] = src[k] ? e->d_smp + k * B : NULL;
+        if (!src[k]) continue;
+        for (int32_t m = 0; m < n; m++)
+            memcpy(e->h_smp + k * B + m, (const float*)src[k] + (ord ? ord[m] : m), 4);
+        dpuf_hip_h2d(e->d_smp + k * B, e->h_smp + k * B, (size_t)n * 4, e->stream);
+    }
+    dpuf_hip_sample(e->stream, DPUF_AMD_F32, n, e->V, e->V, e->logits, (const float*)dev[0], (const int32_t*)dev[1],
+                    (const float*)dev[2], (const float*)dev[3], (const float*)dev[4], (int32_t*)(e->d_smp + 5 * B),
+                    e->d_smp + 6 * B, e->d_smp_ws);
+    dpuf_hip_d2h(e->h_smp + 5 * B, e->d_smp + 5 * B, (size_t)n * 4, e->stream);
+    dpuf_hip_d2h(e->h_smp + 6 * B, e->d_smp + 6 * B, (size_t)n * 4, e->stream);
+}
+
 static int32_t forward_common(Engine* e, int32_t n_tokens, const int32_t* token_ids, int32_t pos0,
                               const float* embeds_in, const int32_t* pos_t, const int32_t* pos_h,
                               const int32_t* pos_w, const float* const* deepstack_in, int32_t only_last,
-                              float* logits_out, int32_t* token_out, int32_t use_graph) {
+                              float* logits_out, int32_t* token_out, int32_t use_graph, const DpufAmdSampling* smp,
+                              float* logprob_out) {
     if (!e || (!token_ids && !embeds_in) || (!logits_out && !token_out && only_last != 2)) return -1;
     if (n_tokens <= 0 || n_tokens > DPUF_AMD_MAX_BATCH) return -2;
     if (pos0 < 0 || pos0 + n_tokens > e->max_seq) return -3;
@@ -1224,9 +1327,9 @@ static int32_t forward_common(Engine* e, int32_t n_tokens, const int32_t* token_
     /* a one-row LM head whose logits go to the host writes them to h_logits
      * itself (the same for every step of a graph key: want_argmax clear and
      * only_last != 2 imply logits_out) */
-    const int32_t want_argmax = token_out != NULL;
+    const int32_t want_argmax = token_out != NULL && !smp;
     const int32_t lm_rows = only_last ? 1 : M;
-    float* lm_host = only_last != 2 && logits_out && !want_argmax && lm_rows == 1 && !head_early(e, 1, early)
+    float* lm_host = only_last != 2 && logits_out && !token_out && lm_rows == 1 && !head_early(e, 1, early)
                          ? e->h_logits
                          : NULL;
 
@@ -1236,7 +1339,8 @@ static int32_t forward_common(Engine* e, int32_t n_tokens, const int32_t* token_
     e->capturing = 0;
     if (graphable) {
         const int32_t bucket = attn_bucket(e, pos0 + 1);
-        int32_t key[7] = {only_last, keep, early, e->active, 0, bucket, want_argmax};
+        /* a step whose token is sampled leaves its logits on the device */
+        int32_t key[7] = {only_last, keep, early, e->active, 0, bucket, smp ? 2 : want_argmax};
         memcpy(&key[4], &margin, 4);
         int gi = -1;
         for (int i = 0; i < N_GRAPHS && gi < 0; i++)
@@ -1268,6 +1372,7 @@ static int32_t forward_common(Engine* e, int32_t n_tokens, const int32_t* token_
     } else {
         enqueue_forward(e, M, embeds_in != NULL, only_last, keep, early, margin, want_argmax, lm_host);
     }
+    if (smp) enqueue_sample(e, 1, NULL, smp);
     tm_end(e, tm13);
     if (only_last != 2 && logits_out && !lm_host)
         dpuf_hip_d2h(logits_out, e->logits, (size_t)lm_rows * e->V * 4, e->stream);
@@ -1278,7 +1383,8 @@ static int32_t forward_common(Engine* e, int32_t n_tokens, const int32_t* token_
     if (rc == 0 && only_last != 2) {
         if (lm_host) memcpy(logits_out, e->h_logits, (size_t)e->V * 4);
         if (flag) e->early_exits++;
-        if (token_out) *token_out = tok;
+        if (token_out) *token_out = smp ? ((int32_t*)e->h_smp)[5 * DPUF_AMD_MAX_BATCH] : tok;
+        if (smp && logprob_out) *logprob_out = e->h_smp[6 * DPUF_AMD_MAX_BATCH];
     }
     return rc;
 }
@@ -1292,7 +1398,7 @@ DPUF_EXPORT int32_t dpuf_engine_forward_batch_ex(void* handle, int32_t n_tokens,
     if (!e || (!logits_out && only_last_logits != 2)) return -1;
     /* one-token steps replay a captured graph (forward_common decides) */
     return forward_common(e, n_tokens, token_ids, pos0, embeds_in, pos_t, pos_h, pos_w, deepstack_in,
-                          only_last_logits, logits_out, NULL, 1);
+                          only_last_logits, logits_out, NULL, 1, NULL, NULL);
 }
 
 DPUF_EXPORT int32_t dpuf_engine_forward_batch(void* handle, int32_t n_tokens, const int32_t* token_ids, int32_t pos0,
@@ -1310,10 +1416,9 @@ DPUF_EXPORT int32_t dpuf_engine_forward_token(void* handle, int32_t token_id, in
  * session slot_ids[i] (distinct) at positions[i], every row of every GEMM
  * serves all n.  Per token the arithmetic is the one-token decode's, with the
  * decode keep-tiles setting and no Zone-A early exit. */
-DPUF_EXPORT int32_t dpuf_amd_engine_forward_slots(void* handle, int32_t n, const int32_t* slot_ids,
-                                                  const int32_t* token_ids, const int32_t* positions,
-                                                  float* logits_out, int32_t* tokens_out) {
-    Engine* e = (Engine*)handle;
+static int32_t forward_slots(Engine* e, int32_t n, const int32_t* slot_ids, const int32_t* token_ids,
+                             const int32_t* positions, const DpufAmdSampling* smp, float* logits_out,
+                             int32_t* tokens_out, float* logprobs_out) {
     if (!e || n <= 0 || !slot_ids || !token_ids || !positions || (!logits_out && !tokens_out)) return -1;
     if (n > DPUF_AMD_MAX_BATCH) return -2;
     if (e->hd != 64 && e->hd != 128 && e->hd != 256) return -5;
@@ -1370,7 +1475,8 @@ DPUF_EXPORT int32_t dpuf_amd_engine_forward_slots(void* handle, int32_t n, const
     enqueue_forward(e, n, 0, 0, keep, 0, 1.25f, 0, NULL);
     e->ms_n = 0;
     e->ms_short = 0;
-    if (tokens_out) dpuf_hip_argmax_rows(e->stream, e->logits, e->V, n, e->d_ms_tok, e->h_tok, e->d_lmred);
+    if (smp) enqueue_sample(e, n, ord, smp);
+    else if (tokens_out) dpuf_hip_argmax_rows(e->stream, e->logits, e->V, n, e->d_ms_tok, e->h_tok, e->d_lmred);
     tm_end(e, tm);
     if (logits_out) dpuf_hip_d2h(lg, e->logits, (size_t)n * e->V * 4, e->stream);
     const int32_t rc = dpuf_hip_sync(e->stream);
@@ -1379,12 +1485,303 @@ DPUF_EXPORT int32_t dpuf_amd_engine_forward_slots(void* handle, int32_t n, const
     if (out == 0) {
         for (int32_t m = 0; m < n; m++) {
             if (logits_out) memcpy(logits_out + (size_t)ord[m] * e->V, lg + (size_t)m * e->V, (size_t)e->V * 4);
-            if (tokens_out) tokens_out[ord[m]] = ((volatile int32_t*)e->h_tok)[m];
+            if (tokens_out)
+                tokens_out[ord[m]] = smp ? ((int32_t*)e->h_smp)[5 * DPUF_AMD_MAX_BATCH + m]
+                                         : ((volatile int32_t*)e->h_tok)[m];
+            if (smp && logprobs_out) logprobs_out[ord[m]] = e->h_smp[6 * DPUF_AMD_MAX_BATCH + m];
         }
     }
     free(ord);
     free(lg);
     return out;
+}
+
+DPUF_EXPORT int32_t dpuf_amd_engine_forward_slots(void* handle, int32_t n, const int32_t* slot_ids,
+                                                  const int32_t* token_ids, const int32_t* positions,
+                                                  float* logits_out, int32_t* tokens_out) {
+    return forward_slots((Engine*)handle, n, slot_ids, token_ids, positions, NULL, logits_out, tokens_out, NULL);
+}
+
+DPUF_EXPORT int32_t dpuf_amd_engine_forward_slots_sample(void* handle, int32_t n, const int32_t* slot_ids,
+                                                         const int32_t* token_ids, const int32_t* positions,
+                                                         const DpufAmdSampling* sampling, float* logits_out,
+                                                         int32_t* tokens_out, float* logprobs_out) {
+    Engine* e = (Engine*)handle;
+    if (!e || !tokens_out || !sampling_ok(e, sampling)) return -1;
+    return forward_slots(e, n, slot_ids, token_ids, positions, sampling, logits_out, tokens_out, logprobs_out);
+}
+
+/* ------------------------------------------------------------------------- */
+/* The paged cache                                                            */
+/* ------------------------------------------------------------------------- */
+
+DPUF_EXPORT int32_t dpuf_amd_engine_pages_create(void* handle, int32_t n_pages, int32_t page_size, int32_t type) {
+    Engine* e = (Engine*)handle;
+    if (!e) return -1;
+    dpuf_hip_clear_error();
+    if (n_pages < 0) return -2;
+    if (n_pages == 0) {
+        dpuf_hip_sync(e->stream);
+        pages_free(e);
+        return dpuf_hip_ok() ? 0 : -6;
+    }
+    if (type != DPUF_AMD_BF16 && type != DPUF_AMD_F16) return -5;
+    if (page_size < 16 || page_size > 1024 || (page_size & (page_size - 1))) return -2;
+    DpufAmdRopeSpec spec;
+    memset(&spec, 0, sizeof spec);
+    const DpufModelConfig* c = &e->cfg;
+    spec.rot_dim = e->hd;
+    spec.theta = c->rope_theta;
+    spec.scaling = c->use_llama3_rope ? DPUF_AMD_ROPE_LLAMA3 : DPUF_AMD_ROPE_PLAIN;
+    spec.factor = c->use_llama3_rope ? c->rope_factor : 1.0f;
+    spec.low_freq = c->rope_low_freq;
+    spec.high_freq = c->rope_high_freq;
+    spec.orig_max_pos = c->rope_orig_max_pos;
+    double turns[128];
+    float scale = 1.0f;
+    if (dpuf_amd_rope_turns(&spec, turns, &scale) != 0) return -5;
+    dpuf_hip_sync(e->stream);
+    pages_free(e);
+    const size_t B = DPUF_AMD_MAX_BATCH, half = (size_t)e->hd / 2;
+    const size_t rows = (size_t)(e->L > 0 ? e->L : 1) * (size_t)n_pages * e->nkv * page_size;
+    e->pg_k = (uint16_t*)dpuf_hip_malloc(rows * e->hd * 2);
+    e->pg_v = (uint16_t*)dpuf_hip_malloc(rows * e->hd * 2);
+    e->pg_w = (float*)dpuf_hip_malloc(rows * 4);
+    e->pg_q = (uint16_t*)dpuf_hip_malloc(B * e->qd * 2);
+    e->pg_lse = (float*)dpuf_hip_malloc(B * e->nq * 4);
+    e->pg_turns = (double*)dpuf_hip_malloc(half * 8);
+    if (!e->pg_k || !e->pg_v || !e->pg_w || !e->pg_q || !e->pg_lse || !e->pg_turns) {
+        pages_free(e);
+        return -2;
+    }
+    e->pg_type = type;
+    e->pg_n = n_pages;
+    e->pg_size = page_size;
+    e->pg_rope.turns = e->pg_turns;
+    e->pg_rope.rot_dim = e->hd;
+    e->pg_rope.interleaved = 0;
+    e->pg_rope.scale = scale;
+    dpuf_hip_h2d(e->pg_turns, turns, half * 8, e->stream);
+    dpuf_hip_fill_zero(e->pg_k, rows * e->hd * 2, e->stream);
+    dpuf_hip_fill_zero(e->pg_v, rows * e->hd * 2, e->stream);
+    dpuf_hip_fill_zero(e->pg_w, rows * 4, e->stream);
+    if (dpuf_hip_sync(e->stream) != 0) {
+        pages_free(e);
+        return -6;
+    }
+    return 0;
+}
+
+DPUF_EXPORT int32_t dpuf_amd_engine_pages(void* handle, int32_t layer, DpufAmdPages* pages) {
+    Engine* e = (Engine*)handle;
+    if (!e || !pages || e->pg_n == 0 || layer < 0 || layer >= e->L) return -1;
+    *pages = pages_of(e, layer);
+    return 0;
+}
+
+/* Staging of `ints` table entries, host and device; grown when needed (no
+ * call is in flight: every one ends with its stream drained). */
+static int pages_staging(Engine* e, size_t ints) {
+    if (ints <= e->pg_ints) return 1;
+    dpuf_hip_host_free(e->h_pg);
+    dpuf_hip_free(e->d_pg);
+    e->pg_ints = 0;
+    e->h_pg = (int32_t*)dpuf_hip_host_alloc(ints * 4);
+    e->d_pg = (int32_t*)dpuf_hip_malloc(ints * 4);
+    if (!e->h_pg || !e->d_pg) {
+        dpuf_hip_host_free(e->h_pg);
+        dpuf_hip_free(e->d_pg);
+        e->h_pg = e->d_pg = NULL;
+        return 0;
+    }
+    e->pg_ints = ints;
+    return 1;
+}
+
+/* Lengths and tables of n sequences: every length fits its row of the table
+ * and every page it needs is in the pool.  uses (pg_n counters, zeroed) counts
+ * each page's sequences. */
+static int32_t check_tables(const Engine* e, int32_t n, const int32_t* len, const int32_t* table, int32_t stride,
+                            int32_t least, uint8_t* uses) {
+    for (int32_t i = 0; i < n; i++) {
+        if (len[i] < least || (int64_t)len[i] > (int64_t)stride * e->pg_size) return -3;
+        const int32_t np = (len[i] + e->pg_size - 1) / e->pg_size;
+        for (int32_t j = 0; j < np; j++) {
+            const int32_t p = table[(size_t)i * stride + j];
+            if (p < 0 || p >= e->pg_n) return -3;
+            if (uses[p] < 2) uses[p]++;
+        }
+    }
+    return 0;
+}
+
+DPUF_EXPORT int32_t dpuf_amd_engine_forward_pages(void* handle, int32_t n, const int32_t* rows,
+                                                  const int32_t* ctx_len, const int32_t* page_table,
+                                                  int32_t table_stride, const int32_t* token_ids,
+                                                  const int32_t* positions, float weight_decay,
+                                                  const DpufAmdSampling* sampling, float* logits_out,
+                                                  int32_t* tokens_out, float* logprobs_out) {
+    Engine* e = (Engine*)handle;
+    if (!e || e->pg_n == 0 || !rows || !ctx_len || !page_table || !token_ids || !positions ||
+        (!logits_out && !tokens_out) || (sampling && (!tokens_out || !sampling_ok(e, sampling))) ||
+        (logprobs_out && !sampling) || !(weight_decay == weight_decay) || isinf(weight_decay))
+        return -1;
+    if (n < 1 || n > DPUF_AMD_MAX_BATCH || table_stride < 1 || (int64_t)table_stride * e->pg_size > (int64_t)1 << 30)
+        return -2;
+    int32_t M = 0, longest = 0;
+    for (int32_t i = 0; i < n; i++) {
+        if (rows[i] < 1 || rows[i] > DPUF_AMD_MAX_BATCH - M) return -2;
+        M += rows[i];
+        if (ctx_len[i] < rows[i]) return -3;
+        if (ctx_len[i] > longest) longest = ctx_len[i];
+    }
+    for (int32_t m = 0; m < M; m++) {
+        if (positions[m] < 0) return -3;
+        if (token_ids[m] < 0 || token_ids[m] >= e->V) return -4;
+    }
+    uint8_t* uses = (uint8_t*)calloc((size_t)e->pg_n, 1);
+    if (!uses) return -2;
+    int32_t rc = check_tables(e, n, ctx_len, page_table, table_stride, 1, uses);
+    for (int32_t i = 0; i < n && rc == 0; i++) {
+        /* pages that new rows go into, and with weights kept all pages, are
+         * this sequence's alone */
+        const int32_t j0 = weight_decay >= 0.0f ? 0 : (ctx_len[i] - rows[i]) / e->pg_size;
+        for (int32_t j = j0; j <= (ctx_len[i] - 1) / e->pg_size; j++)
+            if (uses[page_table[(size_t)i * table_stride + j]] > 1) rc = -1;
+    }
+    free(uses);
+    if (rc != 0) return rc;
+
+    begin_call(e);
+    /* [n + 1] row starts, [n] lengths, [n] last rows, [M] positions, tables */
+    const size_t ints = (size_t)3 * n + 1 + M + (size_t)n * table_stride;
+    if (!pages_staging(e, ints)) return -2;
+    int32_t *hs = e->h_pg, *hc = hs + n + 1, *hl = hc + n, *hp = hl + n, *ht = hp + M;
+    volatile int32_t* io = e->h_io;
+    hs[0] = 0;
+    for (int32_t i = 0; i < n; i++) {
+        hs[i + 1] = hs[i] + rows[i];
+        hc[i] = ctx_len[i];
+        hl[i] = hs[i + 1] - 1;
+    }
+    memcpy(hp, positions, (size_t)M * 4);
+    memcpy(ht, page_table, (size_t)n * table_stride * 4);
+    for (int32_t m = 0; m < M; m++) io[m] = token_ids[m];
+    io[IO_POS] = 0;
+    io[IO_POS + 1] = next_serial(e);
+    DpufAmdBatch b;
+    b.n_seqs = n;
+    b.n_rows = M;
+    b.table_stride = table_stride;
+    b.max_ctx = longest;
+    b.row_start = e->d_pg;
+    b.ctx_len = e->d_pg + (hc - hs);
+    b.page_table = e->d_pg + (ht - hs);
+    const DpufAmdPages p0 = pages_of(e, 0);
+    const size_t ws = dpuf_hip_paged_attn_workspace(&b, &p0, e->nq);
+    if (ws > e->pg_ws_bytes) {
+        dpuf_hip_free(e->pg_ws);
+        e->pg_ws = dpuf_hip_malloc(ws);
+        e->pg_ws_bytes = e->pg_ws ? ws : 0;
+        if (!e->pg_ws) return -2;
+    }
+    dpuf_hip_h2d(e->d_pg, e->h_pg, ints * 4, e->stream);
+    /* the decode setting when every sequence appends one token, as for
+     * sessions; the prefill setting with a prompt among them */
+    int32_t keep = 0;
+    env_int(M > n ? "DPUF_PREFILL_KEEP_TILES" : "DPUF_GEN_KEEP_TILES", &keep);
+    const int tm = tm_begin(e, K_CALL, (double)e->weight_bytes);
+    e->host_pos0 = 0;
+    e->capturing = 0;
+    dpuf_hip_embed(e->stream, e->tok, e->h_io, M, M == 1 ? e->h_emb : NULL, M == 1, e->h, e->h_io + IO_POS, e->d_pos0,
+                   e->d_serial);
+    e->hcur = e->h;
+    e->pg_b = b;
+    e->pg_pos = e->d_pg + (hp - hs);
+    e->pg_decay = weight_decay;
+    enqueue_layers(e, M, keep);
+    e->pg_b.n_seqs = 0;
+    /* the sequences' last rows, one after the other, then the head over them */
+    float* hx = h_other(e);
+    dpuf_hip_gather_sum(e->stream, n, e->H, e->d_pg + (hl - hs), e->hcur, e->L > 0 ? e->hn : NULL, hx);
+    const uint8_t* ps[1] = {e->lm.sign};
+    dpuf_hip_resnorm_prep(e->stream, n, e->H, hx, NULL, NULL, e->d_out_norm, e->cfg.rms_eps, 1, ps, e->prep, NULL);
+    const DpufGemvJob j = job(&e->lm, 0, n_tiles_of(&e->lm), e->prep[0], e->logits, e->V);
+    dpuf_hip_gemv(e->stream, n, 1, &j, NULL, 0.0f);
+    if (sampling) enqueue_sample(e, n, NULL, sampling);
+    else if (tokens_out) dpuf_hip_argmax_rows(e->stream, e->logits, e->V, n, e->d_ms_tok, e->h_tok, e->d_lmred);
+    dpuf_hip_publish(e->stream, e->d_flag, 0, e->h_io + IO_OUT);
+    tm_end(e, tm);
+    if (logits_out) dpuf_hip_d2h(logits_out, e->logits, (size_t)n * e->V * 4, e->stream);
+    rc = dpuf_hip_sync(e->stream);
+    tm_collect(e);
+    rc = rc != 0 ? -6 : end_call(e, io[IO_OUT + 2]);
+    if (rc == 0 && tokens_out) {
+        for (int32_t i = 0; i < n; i++)
+            tokens_out[i] = sampling ? ((int32_t*)e->h_smp)[5 * DPUF_AMD_MAX_BATCH + i]
+                                     : ((volatile int32_t*)e->h_tok)[i];
+        if (logprobs_out) memcpy(logprobs_out, e->h_smp + 6 * DPUF_AMD_MAX_BATCH, (size_t)n * 4);
+    }
+    return rc;
+}
+
+DPUF_EXPORT int32_t dpuf_amd_engine_evict_pages(void* handle, int32_t n, const int32_t* ctx_len,
+                                                const int32_t* page_table, int32_t table_stride, int32_t keep,
+                                                int32_t sink, int32_t recent, const int32_t* dst_table,
+                                                int32_t dst_stride, int32_t* new_len) {
+    Engine* e = (Engine*)handle;
+    if (!e || e->pg_n == 0 || !ctx_len || !page_table || !dst_table || !new_len) return -1;
+    if (n < 1 || n > DPUF_AMD_MAX_BATCH || table_stride < 1 || dst_stride < 1 ||
+        (int64_t)table_stride * e->pg_size > (int64_t)1 << 30 || (int64_t)dst_stride * e->pg_size > (int64_t)1 << 30 ||
+        keep < 1 || sink < 0 || recent < 0 || (int64_t)sink + recent > keep || keep > (int64_t)dst_stride * e->pg_size)
+        return -2;
+    int32_t* len = (int32_t*)malloc((size_t)n * 4);
+    uint8_t* uses = (uint8_t*)calloc((size_t)e->pg_n, 1);
+    uint8_t* dst_uses = (uint8_t*)calloc((size_t)e->pg_n, 1);
+    int32_t rc = len && uses && dst_uses ? 0 : -2;
+    if (rc == 0) rc = check_tables(e, n, ctx_len, page_table, table_stride, 0, uses);
+    if (rc == 0) {
+        for (int32_t i = 0; i < n; i++) len[i] = ctx_len[i] < keep ? ctx_len[i] : keep;
+        rc = check_tables(e, n, len, dst_table, dst_stride, 0, dst_uses);
+    }
+    for (int32_t p = 0; p < e->pg_n && rc == 0; p++)
+        if (dst_uses[p] > 1 || (dst_uses[p] && uses[p])) rc = -1;
+    free(uses);
+    free(dst_uses);
+    if (rc != 0) {
+        free(len);
+        return rc;
+    }
+    begin_call(e);
+    const size_t ints = (size_t)2 * n + (size_t)n * table_stride + (size_t)n * dst_stride;
+    int32_t* kept = (int32_t*)dpuf_hip_malloc((size_t)n * e->nkv * keep * 4);
+    if (!kept || !pages_staging(e, ints)) {
+        dpuf_hip_free(kept);
+        free(len);
+        return -2;
+    }
+    int32_t *hc = e->h_pg, *ht = hc + n, *hd = ht + (size_t)n * table_stride;
+    int32_t* d_len = e->d_pg + (hd - hc) + (size_t)n * dst_stride;
+    memcpy(hc, ctx_len, (size_t)n * 4);
+    memcpy(ht, page_table, (size_t)n * table_stride * 4);
+    memcpy(hd, dst_table, (size_t)n * dst_stride * 4);
+    dpuf_hip_h2d(e->d_pg, e->h_pg, (ints - (size_t)n) * 4, e->stream);
+    DpufAmdBatch b;
+    memset(&b, 0, sizeof b);
+    b.n_seqs = n;
+    b.table_stride = table_stride;
+    b.row_start = NULL;
+    b.ctx_len = e->d_pg;
+    b.page_table = e->d_pg + (ht - hc);
+    for (int32_t l = 0; l < e->L; l++) {
+        const DpufAmdPages p = pages_of(e, l);
+        dpuf_hip_paged_evict(e->stream, &b, &p, keep, sink, recent, &p, e->d_pg + (hd - hc), dst_stride, kept, d_len);
+    }
+    rc = dpuf_hip_sync(e->stream) == 0 && dpuf_hip_ok() ? 0 : -6;
+    dpuf_hip_free(kept);
+    if (rc == 0) memcpy(new_len, len, (size_t)n * 4);
+    free(len);
+    return rc;
 }
 
 DPUF_EXPORT int32_t dpuf_amd_engine_forward_argmax(void* handle, int32_t n_tokens, const int32_t* token_ids,
@@ -1393,7 +1790,17 @@ DPUF_EXPORT int32_t dpuf_amd_engine_forward_argmax(void* handle, int32_t n_token
     Engine* e = (Engine*)handle;
     if (!e || !token_out) return -1;
     return forward_common(e, n_tokens, token_ids, pos0, embeds_in, NULL, NULL, NULL, NULL, 1, logits_out, token_out,
-                          use_graph);
+                          use_graph, NULL, NULL);
+}
+
+DPUF_EXPORT int32_t dpuf_amd_engine_forward_sample(void* handle, int32_t n_tokens, const int32_t* token_ids,
+                                                   int32_t pos0, const float* embeds_in, int32_t use_graph,
+                                                   const DpufAmdSampling* sampling, int32_t* token_out,
+                                                   float* logprob_out, float* logits_out) {
+    Engine* e = (Engine*)handle;
+    if (!e || !token_out || !sampling_ok(e, sampling)) return -1;
+    return forward_common(e, n_tokens, token_ids, pos0, embeds_in, NULL, NULL, NULL, NULL, 1, logits_out, token_out,
+                          use_graph, sampling, logprob_out);
 }
 
 /* ------------------------------------------------------------------------- */

@@ -291,6 +291,10 @@ void dpuf_hip_slab_pack(void* s, int32_t mc, int32_t K, DpufPrep rows, int32_t* 
 void dpuf_hip_slab_unpack(void* s, int32_t M, int32_t K, const int32_t* sq, const float* ss, const int32_t* sm,
                           DpufPrep rows);
 
+/* out[i] = h[rows[i]] + res[rows[i]] (res NULL: no addend), n rows of H. */
+void dpuf_hip_gather_sum(void* s, int32_t n, int32_t H, const int32_t* rows, const float* h, const float* res,
+                         float* out);
+
 /* The device a device-memory pointer is on; -1 for any other pointer. */
 int32_t dpuf_hip_ptr_device(const void* p);
 /* Makes dev the current device; returns what dpuf_hip_device_leave takes to

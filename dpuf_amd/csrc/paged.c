@@ -208,7 +208,12 @@ DPUF_EXPORT int32_t dpuf_amd_paged_evict(const DpufAmdBatch* batch, const DpufAm
     dpuf_hip_clear_error();
     int32_t rc = check_pages(pages);
     if (rc == 0) rc = check_pages(dst);
-    if (rc == 0) rc = check_batch(batch, pages);
+    if (rc == 0 && !batch) rc = -1;
+    if (rc != 0) return rc;
+    DpufAmdBatch b = *batch;    /* without new rows */
+    b.row_start = b.ctx_len;
+    b.n_rows = 0;
+    rc = check_batch(&b, pages);
     if (rc != 0) return rc;
     if (dst->type != pages->type || dst->head_dim != pages->head_dim) return -5;
     if (dst->n_kv_heads != pages->n_kv_heads) return -2;
@@ -230,7 +235,7 @@ DPUF_EXPORT int32_t dpuf_amd_paged_evict(const DpufAmdBatch* batch, const DpufAm
                         d_dst_table, d_kept, d_new_len};
     const int32_t dev = device_of(ps, (int)(sizeof ps / sizeof ps[0]));
     if (dev < 0) return -1;
-    ON_DEVICE(dev, dpuf_hip_paged_evict(hip_stream, batch, pages, keep, sink, recent, dst, d_dst_table,
+    ON_DEVICE(dev, dpuf_hip_paged_evict(hip_stream, &b, pages, keep, sink, recent, dst, d_dst_table,
                                         dst_table_stride, d_kept, d_new_len));
 }
 

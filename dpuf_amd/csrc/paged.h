@@ -80,11 +80,14 @@ DEV float add_xor16(float v) { const float2 b = both_of_16(v); return b.x + b.y;
 struct PgSeq {
     int r0, n, ctx;
 };
+DEV int pg_ctx(const DpufAmdBatch& b, int shift, int s) {
+    return min(max(b.ctx_len[s], 0), b.table_stride << shift);
+}
 DEV PgSeq pg_seq(const DpufAmdBatch& b, int shift, int s) {
     PgSeq q;
     q.r0 = min(max(b.row_start[s], 0), b.n_rows);
     q.n = min(max(b.row_start[s + 1], q.r0), b.n_rows) - q.r0;
-    q.ctx = min(max(b.ctx_len[s], 0), b.table_stride << shift);
+    q.ctx = pg_ctx(b, shift, s);
     return q;
 }
 

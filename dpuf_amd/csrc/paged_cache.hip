@@ -287,8 +287,7 @@ __global__ __launch_bounds__(EV_T) void k_ev_pick(EvArgs a) {
     __shared__ uint32_t sh_prefix;
     __shared__ int sh_need;
     const int kvh = blockIdx.x, s = blockIdx.y, t = threadIdx.x;
-    const PgSeq sq = pg_seq(a.b, a.shift, s);
-    const int c = sq.ctx, n = min(c, a.keep);
+    const int c = pg_ctx(a.b, a.shift, s), n = min(c, a.keep);
     if (kvh == 0 && t == 0) a.new_len[s] = n;
     int* kept = a.kept + ((size_t)s * a.p.n_kv_heads + kvh) * a.keep;
     if (c <= a.keep) {
@@ -363,7 +362,7 @@ template <int HD>
 __global__ __launch_bounds__(256) void k_ev_move(EvArgs a) {
     constexpr int CH = HD / 8, RP = 256 / CH, NR = 4;
     const int kvh = blockIdx.x, s = blockIdx.y;
-    const int c = min(max(a.b.ctx_len[s], 0), a.b.table_stride << a.shift), n = min(c, a.keep);
+    const int c = pg_ctx(a.b, a.shift, s), n = min(c, a.keep);
     const int* kept = a.kept + ((size_t)s * a.p.n_kv_heads + kvh) * a.keep;
     const int sub = threadIdx.x % CH, rw = threadIdx.x / CH;
     for (int i0 = blockIdx.z * RP * NR; i0 < n; i0 += gridDim.z * RP * NR) {

@@ -773,6 +773,19 @@ void dpuf_hip_embed(void* s, DpufDevW w, const int32_t* ids, int32_t M, const fl
     LAUNCHED("k_embed");
 }
 
+// out[i] = h[rows[i]] + res[rows[i]]: the residual stream of the rows whose
+// logits a batch of sequences wants.
+__global__ void k_gather_sum(int H, const int32_t* __restrict__ rows, const float* __restrict__ h,
+                             const float* __restrict__ res, float* __restrict__ out) {
+    const size_t from = (size_t)rows[blockIdx.x] * H, to = (size_t)blockIdx.x * H;
+    for (int c = threadIdx.x; c < H; c += blockDim.x) out[to + c] = res ? h[from + c] + res[from + c] : h[from + c];
+}
+void dpuf_hip_gather_sum(void* s, int32_t n, int32_t H, const int32_t* rows, const float* h, const float* res,
+                         float* out) {
+    hipLaunchKernelGGL(k_gather_sum, dim3(n), dim3(256), 0, ST(s), H, rows, h, res, out);
+    LAUNCHED("k_gather_sum");
+}
+
 // Copies a step's result words (early-exit flag, argmax token, error word)
 // to host memory with vector stores, so the host reads them after the
 // stream drains without a copy; the flag is 0 when no top-2 check ran.

@@ -323,6 +323,83 @@ DPUF_EXPORT int32_t dpuf_amd_sample(int32_t type, int32_t n, int32_t V, int64_t 
                                     const float* d_min_p, const float* d_u, int32_t* d_tokens, float* d_logprobs,
                                     void* d_workspace, size_t workspace_bytes, void* hip_stream);
 
+/* ---- The engine over pages and with sampling ----------------------------- */
+
+/* Sampling settings of an engine call: host arrays, entry i for token or
+ * sequence i, with the meaning they have in dpuf_amd_sample; all but u may be
+ * NULL (off). */
+typedef struct {
+    const float*   temperature;
+    const int32_t* top_k;
+    const float*   top_p;
+    const float*   min_p;
+    const float*   u;
+} DpufAmdSampling;
+
+/* dpuf_amd_engine_forward_argmax with the last row's token drawn by
+ * dpuf_amd_sample (one entry of each setting) instead of its largest logit;
+ * logprob_out (or NULL) its logarithmic share.  Same return codes, -1 also
+ * without sampling->u. */
+DPUF_EXPORT int32_t dpuf_amd_engine_forward_sample(void* handle, int32_t n_tokens, const int32_t* token_ids,
+                                                   int32_t pos0, const float* embeds_in, int32_t use_graph,
+                                                   const DpufAmdSampling* sampling, int32_t* token_out,
+                                                   float* logprob_out, float* logits_out);
+
+/* dpuf_amd_engine_forward_slots with session i's token drawn from its logits
+ * by entry i of the settings. */
+DPUF_EXPORT int32_t dpuf_amd_engine_forward_slots_sample(void* handle, int32_t n, const int32_t* slot_ids,
+                                                         const int32_t* token_ids, const int32_t* positions,
+                                                         const DpufAmdSampling* sampling, float* logits_out,
+                                                         int32_t* tokens_out, float* logprobs_out);
+
+/* Gives the engine a KV cache of n_pages pages of page_size rows per layer
+ * (type DPUF_AMD_BF16 or DPUF_AMD_F16; 2 x 2 x n_kv_heads x head_dim bytes and
+ * 4 x n_kv_heads of weights per row and layer), next to its slots, for
+ * dpuf_amd_engine_forward_pages; n_pages 0 frees it.  An earlier one is
+ * replaced, its contents lost.  0 ok; -1 NULL handle, -2 a size out of range
+ * or out of memory, -5 another type, or a rotation the config does not
+ * describe, -6 device error. */
+DPUF_EXPORT int32_t dpuf_amd_engine_pages_create(void* handle, int32_t n_pages, int32_t page_size, int32_t type);
+
+/* Layer `layer`'s pages as the operators above take them.  0 ok, -1 no pages
+ * or no such layer. */
+DPUF_EXPORT int32_t dpuf_amd_engine_pages(void* handle, int32_t layer, DpufAmdPages* pages);
+
+/* One forward pass over n sequences of any mix (prompts, chunks of prompts,
+ * single tokens) on the engine's pages; host pointers.  Sequence i appends
+ * rows[i] >= 1 tokens (token_ids: all sequences' one after the other, at most
+ * DPUF_AMD_MAX_BATCH) whose rotary positions are positions[...] (any, not
+ * bounded by max_seq_len); ctx_len[i] is its cached rows with them, in the
+ * pages page_table[i * table_stride ...].  Which pages those are, and when
+ * one is free, is the caller's affair: pages may be shared between sequences
+ * as long as no new row goes into them and no weights are kept.  With
+ * weight_decay >= 0 every cached row's weight becomes weight_decay times
+ * itself plus the attention it receives in this pass (dpuf_amd_paged_attn_weights);
+ * below 0 weights stay as they are.  Out, for each sequence's last row:
+ * logits_out [n][V], and tokens_out [n] with logprobs_out [n] drawn by
+ * sampling (tokens_out alone, the greedy token, when sampling is NULL); each
+ * may be NULL, not all.  Attention runs on the pages' 16-bit type with fp32
+ * sums, so results are close to, not bit-equal with, the slots'.
+ * 0 ok; -1 NULL or contradicting arguments, no pages, a page used twice
+ * where that is not allowed; -2 sizes; -3 a length or position out of range;
+ * -4 a token id out of range; -6 device error. */
+DPUF_EXPORT int32_t dpuf_amd_engine_forward_pages(void* handle, int32_t n, const int32_t* rows,
+                                                  const int32_t* ctx_len, const int32_t* page_table,
+                                                  int32_t table_stride, const int32_t* token_ids,
+                                                  const int32_t* positions, float weight_decay,
+                                                  const DpufAmdSampling* sampling, float* logits_out,
+                                                  int32_t* tokens_out, float* logprobs_out);
+
+/* dpuf_amd_paged_evict on every layer of n sequences of the engine's pages
+ * (host pointers): sequence i's min(ctx_len[i], keep) rows that stay go to the
+ * pages dst_table[i * dst_stride ...], none of which any of the sequences
+ * has, or has twice; new_len [n] receives the lengths.  Codes as for
+ * dpuf_amd_engine_forward_pages. */
+DPUF_EXPORT int32_t dpuf_amd_engine_evict_pages(void* handle, int32_t n, const int32_t* ctx_len,
+                                                const int32_t* page_table, int32_t table_stride, int32_t keep,
+                                                int32_t sink, int32_t recent, const int32_t* dst_table,
+                                                int32_t dst_stride, int32_t* new_len);
+
 #ifdef __cplusplus
 }
 #endif
