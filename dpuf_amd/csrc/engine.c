@@ -685,7 +685,11 @@ DPUF_EXPORT void* dpuf_engine_create(const DpufModelConfig* cfg, const DpufLayer
         e->d_ms_tok = e->d_ms_pos + B;
         e->h_smp = (float*)dpuf_hip_host_alloc(B * 7 * 4);
         e->d_smp = (float*)dpuf_hip_malloc(B * 7 * 4);
-        e->smp_ws = e->V <= DPUF_AMD_SAMPLE_MAX_VOCAB ? dpuf_hip_sample_workspace((int32_t)B, e->V) : 0;
+        /* fewer rows are cut finer, so the largest need is not the last */
+        for (int32_t n = 1; n <= (int32_t)B && e->V <= DPUF_AMD_SAMPLE_MAX_VOCAB; n++) {
+            const size_t w = dpuf_hip_sample_workspace(n, e->V);
+            if (w > e->smp_ws) e->smp_ws = w;
+        }
         if (e->smp_ws) e->d_smp_ws = dpuf_hip_malloc(e->smp_ws);
         if (!e->h_smp || !e->d_smp || (e->smp_ws && !e->d_smp_ws)) goto fail;
         if (!e->h || !e->h2 || !e->hn || !e->q || !e->k || !e->v || !e->ao || !e->gate || !e->up || !e->logits ||
