@@ -2,7 +2,7 @@
 // and min-p, drawn with a given uniform number.
 //
 // With M the row's largest logit, the weight of token i is
-//     w_i = rint(2^S exp((x_i - M) / T)),  S = 62 - ceil(log2 V),
+//     w_i = rint(2^S exp((x_i - M) / T)),  S = min(51, 62 - ceil(log2 V)),
 // a 64-bit integer: the V weights of a row sum below 2^63, sums of them are
 // the same in any order (LDS atomics included), and a token whose weight
 // rounds to 0 has less than 2^-38 of the largest token's.  Such tokens can
@@ -17,15 +17,15 @@
 //   k_smp_max   the chunks' largest logits;
 //   k_smp_hist  tokens and weight in each of NB bins of (M - x) / T per chunk
 //               (only the sum where neither top-k nor top-p is on); the
-//               workgroup that ends last adds the chunks' bins up and finds
-//               the bins in which the prefixes end;
+//               workgroup that ends last adds the chunks' bins up, groups of
+//               16 first, and finds the bins in which the prefixes end;
 //   k_smp_pick  collects the tokens that decide: all of the prefix's where
 //               they fit, else those of the bins the borders lie in; the
-//               workgroup that ends last sorts them, finds the border and
-//               draws, from the list or, in index order, from the chunk in
-//               which the running sum passes the draw.
-// Rows whose border bin alone holds more tokens than can be sorted (long runs
-// of equal logits) are left to one workgroup that splits the bin further.
+//               workgroup that ends last finds the borders among them by
+//               radix selection and draws, from the list or, in index order,
+//               from the chunk in which the running sum passes the draw.
+// Rows whose border bin alone holds more tokens than the list (long runs of
+// equal logits) are left to one workgroup that splits the bin further.
 //
 // The last workgroup is found with a counter per row; what it reads from the
 // others was stored past the L2 of their XCD (agent scope) and acknowledged
@@ -41,7 +41,9 @@ namespace {
 constexpr int NT = 256;          // threads of a workgroup
 constexpr int NW = NT / 64;
 constexpr int NB = 1024;         // bins
-constexpr int CAP = 2048;        // tokens sorted in LDS
+constexpr int GB = 16;           // bins of a group
+constexpr int NG = NB / GB;      // groups: a wave's lanes
+constexpr int CAP = 2048;        // tokens listed in LDS
 constexpr int ROWS = 1024;       // rows of one set of launches
 constexpr int MAX_CHUNKS = 64;   // a wave's lanes take a row's chunks
 
@@ -67,7 +69,7 @@ struct SmArgs {
     const float *top_p, *min_p, *u;
     int* tok;
     float* logp;
-    uint64_t *best, *csum, *wsum, *list;
+    uint64_t *best, *csum, *wsum, *gsum, *list;   // gsum: weight, tokens of each group of bins
     uint32_t* count;
     SmState* state;
 };
@@ -103,16 +105,14 @@ DEV float logit_of(uint64_t c) { return from_bits((uint32_t)(c >> 32)); }
 DEV int index_of(uint64_t c) { return (int)(0xffffffffu - (uint32_t)c); }
 
 // 2^s exp(-a) for 0 <= a < 64: exp(-a) = 2^-n exp(r) with n = rint(a / ln 2) and
-// r = n ln 2 - a, by the Taylor series of exp up to r^13 / 13! (|r| <= ln 2 / 2:
-// what is left out is below 2^-56).
+// r = n ln 2 - a, by the Taylor series of exp up to r^11 / 11! (|r| <= ln 2 / 2:
+// what is left out is below 2^-47).
 DEV double exp_neg(double a, int s) {
     const double n = rint(a * 1.4426950408889634074);
     // ln 2 in two parts, the first of 40 bits: n times it is exact
     double r = fma(n, 0x1.62e42fefa2000p-1, -a);
     r = fma(n, 0x1.9ef35793c7673p-41, r);
-    double e = 1.0 / 6227020800.0;
-    e = fma(e, r, 1.0 / 479001600.0);
-    e = fma(e, r, 1.0 / 39916800.0);
+    double e = 1.0 / 39916800.0;
     e = fma(e, r, 1.0 / 3628800.0);
     e = fma(e, r, 1.0 / 362880.0);
     e = fma(e, r, 1.0 / 40320.0);
@@ -125,6 +125,10 @@ DEV double exp_neg(double a, int s) {
     e = fma(e, r, 1.0);
     e = fma(e, r, 1.0);
     return ldexp(e, s - (int)n);
+}
+// rint(e) for 0 <= e <= 2^51: the sum's last bit is worth one
+DEV uint64_t to_int(double e) {
+    return __builtin_bit_cast(uint64_t, e + 0x1p52) - __builtin_bit_cast(uint64_t, 0x1p52);
 }
 
 // f(token, logit) for the tokens [lo, hi) of a row, in no particular order; lo
@@ -162,14 +166,19 @@ template <typename L> struct Row {
     double invT, A, p_goal;
     float bins;                  // bins per temperature
     int k, by_k, by_p, by_m;
-    double min_p, edge;          // min_p and -ln min_p
+    double min_w, edge;          // 2^S min_p (0: off) and -ln min_p
 
     // (M - x) / T, or infinity for tokens that cannot be drawn
     DEV double depth(float x) const {
         const double d = (double)M - (double)x;
         return x == M ? 0.0 : d < __builtin_huge_val() ? d * invT : __builtin_huge_val();
     }
-    DEV uint64_t weight(double a) const { return a < A ? (uint64_t)(exp_neg(a, S) + 0.5) : 0; }
+    DEV uint64_t weight(double a) const { return a < A ? to_int(exp_neg(a, S)) : 0; }
+    // with min_p's say
+    DEV uint64_t weight_min(double a) const {
+        const double e = exp_neg(a < A ? a : A, S);
+        return a < A && e >= min_w ? to_int(e) : 0;
+    }
     DEV uint64_t weight_of(uint64_t c) const { return weight(depth(logit_of(c))); }
     DEV int bin(double a) const {
         const int b = (int)((float)a * bins);
@@ -177,7 +186,6 @@ template <typename L> struct Row {
     }
     // a token with a weight: only the last bin's need the exponential to tell
     DEV bool alive(double a, int b) const { return a < A && (b < NB - 1 || weight(a) != 0); }
-    DEV bool above_min(double a) const { return !by_m || exp_neg(a, 0) >= min_p; }
 
     DEV void open(const SmArgs& a, int r) {
         p = (const char*)a.x + r * a.stride * L::SIZE;
@@ -199,9 +207,10 @@ template <typename L> struct Row {
         const float tp = a.top_p ? a.top_p[r] : 1.0f, mp = a.min_p ? a.min_p[r] : 0.0f;
         by_p = tp < 1.0f;
         p_goal = tp > 0.0f ? (double)tp : 0.0;
-        min_p = mp > 1.0f ? 1.0 : mp > 0.0f ? (double)mp : 0.0;
+        const double min_p = mp > 1.0f ? 1.0 : mp > 0.0f ? (double)mp : 0.0;
         edge = min_p > 0.0 ? -log(min_p) : 0.0;
         by_m = min_p > 0.0 && edge < A;
+        min_w = by_m ? ldexp(min_p, S) : 0.0;
         return true;
     }
     // Top-p's goal for a total: one token at least.
@@ -305,90 +314,152 @@ template <typename L> __global__ __launch_bounds__(NT) void k_smp_max(SmArgs a) 
 struct HistShared {
     unsigned long long wsum[NB];
     uint32_t count[NB];
+    unsigned long long gw[NG], fw[GB];     // a group's, a fine bin's weight over all chunks
+    uint32_t gc[NG], fc[GB];
     uint64_t red[NW];
-    uint64_t v0, v1;
-    int flag, b;
+    int flag;
 };
 
-// Finds the border bins from the row's bins (in sh, all chunks added up).
-template <typename L> DEV void find_borders(const SmArgs& a, HistShared& sh, const Row<L>& row, SmState* st) {
-    constexpr int PER = NB / NT;
-    const int t = threadIdx.x;
-    uint64_t c = 0, w = 0, tc, tw;
-#pragma unroll
-    for (int e = 0; e < PER; e++) {
-        c += sh.count[PER * t + e];
-        w += sh.wsum[PER * t + e];
+// What a prefix search looks for: the first `count` tokens, or the shortest
+// prefix whose weights reach `goal`, or whose sum passes `count`.
+enum { BY_COUNT, BY_GOAL, BY_SUM };
+struct Want {
+    int by;
+    uint64_t count;
+    double goal;
+    DEV bool met(uint64_t n, uint64_t w) const {
+        return by == BY_COUNT ? n >= count : by == BY_GOAL ? (double)w >= goal : w > count;
     }
-    const uint64_t c0 = scan64(sh.red, c, &tc) - c, w0 = scan64(sh.red, w, &tw) - w;
-    __shared__ int bk, pl, ph;
-    __shared__ uint64_t nk, wk, wp;
-    if (t == 0) {
-        bk = pl = ph = -1;
-        nk = wk = wp = 0;
+};
+
+// A bin with the tokens and weight above it and in it.
+struct Border {
+    int bin;               // -1: the search's end lies past the last bin
+    uint64_t n, w, n_in, w_in;
+};
+
+DEV uint64_t lane_of(uint64_t v, int l) {
+    return (uint64_t)__shfl((uint32_t)(v >> 32), l) << 32 | __shfl((uint32_t)v, l);
+}
+
+// The first of `lanes` lanes' (count, weight) pairs at which a prefix with n
+// tokens and w weight before them meets `want` (-1: none); every wave alike.
+DEV int cross(const Want& want, int lanes, uint64_t c, uint64_t v, uint64_t* n, uint64_t* w) {
+    const int lane = threadIdx.x & 63;
+    uint64_t ic = lane < lanes ? c : 0, iv = lane < lanes ? v : 0;
+    for (int d = 1; d < lanes; d <<= 1) {
+        const uint64_t oc = shfl_up64(ic, d), ov = shfl_up64(iv, d);
+        if (lane >= d) {
+            ic += oc;
+            iv += ov;
+        }
+    }
+    const uint64_t hit = __ballot(lane < lanes && want.met(*n + ic, *w + iv));
+    if (!hit) return -1;
+    const int at = __ffsll((unsigned long long)hit) - 1;
+    *n += lane_of(ic - c, at);
+    *w += lane_of(iv - v, at);
+    return at;
+}
+
+// The 16 bins of group g over all chunks, into sh.fc / sh.fw.
+DEV void load_group(const SmArgs& a, HistShared& sh, int r, int g) {
+    const int t = threadIdx.x, b = t & (GB - 1);
+    __syncthreads();
+    if (t < GB) {
+        sh.fc[t] = 0;
+        sh.fw[t] = 0;
     }
     __syncthreads();
-    if (row.by_k) {
-        uint64_t n = c0, s = w0;
+    if (a.chunks == 1) {
+        if (t < GB) {
+            sh.fc[t] = sh.count[g * GB + t];
+            sh.fw[t] = sh.wsum[g * GB + t];
+        }
+    } else {
+        constexpr int KG = NT / GB;        // threads of a bin
+        uint64_t v[MAX_CHUNKS / KG];
+        uint32_t c[MAX_CHUNKS / KG];
+        const size_t at = (size_t)r * a.chunks * NB + g * GB + b;
 #pragma unroll
-        for (int e = 0; e < PER; e++) {
-            const int b = PER * t + e;
-            if (n < (uint64_t)row.k && n + sh.count[b] >= (uint64_t)row.k) {
-                bk = b;
-                nk = n;
-                wk = s;
-            }
-            n += sh.count[b];
-            s += sh.wsum[b];
+        for (int i = 0; i < MAX_CHUNKS / KG; i++) {
+            const int k = t / GB + i * KG;
+            const size_t x = at + (size_t)min(k, a.chunks - 1) * NB;
+            v[i] = get_agent(a.wsum + x);
+            c[i] = __hip_atomic_load(a.count + x, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            if (k >= a.chunks) v[i] = c[i] = 0;
+        }
+        for (int i = 1; i < MAX_CHUNKS / KG; i++) {
+            v[0] += v[i];
+            c[0] += c[i];
+        }
+        if (c[0]) {
+            atomicAdd(&sh.fc[b], c[0]);
+            atomicAdd(&sh.fw[b], (unsigned long long)v[0]);
         }
     }
     __syncthreads();
-    const bool by_k = bk >= 0;       // fewer tokens than k: all stay
+}
+
+DEV Border find_border(const SmArgs& a, HistShared& sh, int r, const Want& want, int* loaded) {
+    const int lane = threadIdx.x & 63;
+    Border o = {-1, 0, 0, 0, 0};
+    const int g = cross(want, NG, sh.gc[lane], sh.gw[lane], &o.n, &o.w);
+    if (g < 0) return o;
+    if (*loaded != g) load_group(a, sh, r, g);
+    *loaded = g;
+    const uint64_t c = sh.fc[lane & (GB - 1)], w = sh.fw[lane & (GB - 1)];
+    const int f = cross(want, GB, c, w, &o.n, &o.w);
+    if (f < 0) return o;
+    o.bin = g * GB + f;
+    o.n_in = lane_of(c, f);
+    o.w_in = lane_of(w, f);
+    return o;
+}
+
+// Finds the border bins from the groups' sums.
+template <typename L> DEV void find_borders(const SmArgs& a, HistShared& sh, const Row<L>& row, SmState* st, int r) {
+    const int t = threadIdx.x, lane = t & 63;
+    uint64_t tn = sh.gc[lane], tw = sh.gw[lane];
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+        tn += lane_of(tn, lane ^ d);
+        tw += lane_of(tw, lane ^ d);
+    }
+    int loaded = -1;
+    Border k = {-1, 0, 0, 0, 0}, p0 = k, p1 = k;
+    if (row.by_k) k = find_border(a, sh, r, Want{BY_COUNT, (uint64_t)row.k, 0.0}, &loaded);
+    const bool by_k = k.bin >= 0;        // fewer tokens than k: all stay
     if (row.by_p) {
         // the weight that top-k leaves lies between these
-        const double g0 = row.goal(by_k ? wk : tw), g1 = row.goal(by_k ? wk + sh.wsum[bk] : tw);
-        uint64_t s = w0;
-#pragma unroll
-        for (int e = 0; e < PER; e++) {
-            const int b = PER * t + e;
-            const uint64_t s1 = s + sh.wsum[b];
-            if ((double)s < g0 && (double)s1 >= g0) {
-                pl = b;
-                wp = s;
-            }
-            if ((double)s < g1 && (double)s1 >= g1) ph = b;
-            s = s1;
-        }
+        p0 = find_border(a, sh, r, Want{BY_GOAL, 0, row.goal(by_k ? k.w : tw)}, &loaded);
+        p1 = by_k ? find_border(a, sh, r, Want{BY_GOAL, 0, row.goal(k.w + k.w_in)}, &loaded) : p0;
     }
-    __syncthreads();
-    const bool by_p = pl >= 0 && ph >= 0;
+    const bool by_p = p0.bin >= 0 && p1.bin >= 0;
     const int ml = row.by_m ? row.bin(row.edge * (1.0 - 1e-9)) : -1, mh = row.by_m ? row.bin(row.edge * (1.0 + 1e-9)) : -1;
-    const int last = by_k ? bk : by_p ? ph : NB - 1;
-    uint64_t n_up = 0, n_s = 0;
-#pragma unroll
-    for (int e = 0; e < PER; e++) {
-        const int b = PER * t + e;
-        if (b <= last) n_up += sh.count[b];
-        if ((by_k && b == bk) || (by_p && b >= pl && b <= ph) || (row.by_m && b >= ml && b <= mh)) n_s += sh.count[b];
-    }
-    uint64_t a_up, a_s;
-    scan64(sh.red, n_up, &a_up);
-    scan64(sh.red, n_s, &a_s);
+    const uint64_t upto = by_k ? k.n + k.n_in : by_p ? p1.n + p1.n_in : tn;
+    uint64_t in_s = (by_k ? k.n_in : 0) + (by_p ? p1.n + p1.n_in - p0.n : 0);
+    if (row.by_m && upto > CAP)
+        for (int b = ml; b <= mh; b++) {
+            if (loaded != b / GB) load_group(a, sh, r, b / GB);
+            loaded = b / GB;
+            in_s += sh.fc[b % GB];
+        }
     if (t == 0) {
         st->by_k = by_k;
         st->by_p = by_p;
         st->by_m = row.by_m;
-        st->last = last;
-        st->bk = bk;
-        st->pl = pl;
-        st->ph = ph;
+        st->last = by_k ? k.bin : by_p ? p1.bin : NB - 1;
+        st->bk = k.bin;
+        st->pl = p0.bin;
+        st->ph = p1.bin;
         st->ml = ml;
         st->mh = mh;
-        st->rk = by_k ? (unsigned)((uint64_t)row.k - nk) : 0;
-        st->wk = wk;
-        st->wp = wp;
+        st->rk = by_k ? (unsigned)((uint64_t)row.k - k.n) : 0;
+        st->wk = k.w;
+        st->wp = p0.w;
         st->total = tw;
-        st->mode = a_up <= CAP ? SM_LIST : a_s <= CAP ? SM_BINS : SM_SPLIT;
+        st->mode = upto <= CAP ? SM_LIST : in_s <= CAP ? SM_BINS : SM_SPLIT;
     }
 }
 
@@ -411,10 +482,7 @@ template <typename L> __global__ __launch_bounds__(NT) void k_smp_hist(SmArgs a)
     const int lo = c * a.chunk, hi = min(a.V, lo + a.chunk);
     if (!row.by_k && !row.by_p) {
         uint64_t s = 0, all;
-        each<L>(row.p, row.vec, lo, hi, [&](int, float x) {
-            const double d = row.depth(x);
-            if (row.above_min(d)) s += row.weight(d);
-        });
+        each<L>(row.p, row.vec, lo, hi, [&](int, float x) { s += row.weight_min(row.depth(x)); });
         scan64(sh.red, s, &all);
         if (t == 0) {
             a.csum[(size_t)r * a.chunks + c] = all;
@@ -437,32 +505,69 @@ template <typename L> __global__ __launch_bounds__(NT) void k_smp_hist(SmArgs a)
         }
     });
     __syncthreads();
-    const size_t at = ((size_t)r * a.chunks + c) * NB;
-    for (int b = t; b < NB; b += NT) put_agent(a.wsum + at + b, sh.wsum[b]);
-    for (int b = t; b < NB / 2; b += NT)
-        put_agent((uint64_t*)(a.count + at) + b, (uint64_t)sh.count[2 * b + 1] << 32 | sh.count[2 * b]);
-    if (!last_here(&st->tick[0], a.chunks, &sh.flag)) return;
-    if (a.chunks > 1) {
-        constexpr int PER = NB / NT;
-        const uint64_t* cp = (const uint64_t*)(a.count + (size_t)r * a.chunks * NB) + PER / 2 * t;
-        const uint64_t* wp = a.wsum + (size_t)r * a.chunks * NB + PER * t;
-        uint64_t n[PER / 2] = {}, w[PER] = {};
-#pragma unroll 4
-        for (int k = 0; k < a.chunks; k++) {
-            // two 32-bit sums in one word: a row has at most 2^24 tokens
+    // the groups' sums, four threads a group
+    {
+        constexpr int Q = GB / (NT / NG);
+        uint32_t n = 0;
+        uint64_t w = 0;
 #pragma unroll
-            for (int e = 0; e < PER / 2; e++) n[e] += get_agent(cp + (size_t)k * (NB / 2) + e);
-#pragma unroll
-            for (int e = 0; e < PER; e++) w[e] += get_agent(wp + (size_t)k * NB + e);
+        for (int e = 0; e < Q; e++) {
+            n += sh.count[Q * t + e];
+            w += sh.wsum[Q * t + e];
         }
 #pragma unroll
-        for (int e = 0; e < PER; e++) {
-            sh.count[PER * t + e] = (uint32_t)(n[e / 2] >> (32 * (e & 1)));
-            sh.wsum[PER * t + e] = w[e];
+        for (int d = 1; d < NT / NG; d <<= 1) {
+            n += __shfl_xor(n, d);
+            w += (uint64_t)__shfl_xor((uint32_t)(w >> 32), d) << 32 | __shfl_xor((uint32_t)w, d);
+        }
+        if (t % (NT / NG) == 0) {
+            sh.gc[t / (NT / NG)] = n;
+            sh.gw[t / (NT / NG)] = w;
+        }
+    }
+    __syncthreads();
+    if (a.chunks == 1) {
+        for (int b = t; b < NB; b += NT) a.wsum[(size_t)r * NB + b] = sh.wsum[b];
+    } else {
+        const size_t at = ((size_t)r * a.chunks + c) * NB, ag = ((size_t)r * a.chunks + c) * NG;
+        for (int b = t; b < NB; b += NT) put_agent(a.wsum + at + b, sh.wsum[b]);
+        for (int b = t; b < NB / 2; b += NT)
+            put_agent((uint64_t*)(a.count + at) + b, (uint64_t)sh.count[2 * b + 1] << 32 | sh.count[2 * b]);
+        if (t < NG) {
+            put_agent(a.gsum + 2 * (ag + t), sh.gw[t]);
+            put_agent(a.gsum + 2 * (ag + t) + 1, sh.gc[t]);
+        }
+        if (!last_here(&st->tick[0], a.chunks, &sh.flag)) return;
+        // a load of another XCD's store takes a microsecond or two: all of
+        // the groups' at a time, a group by each wave's lane, the chunks by
+        // the four waves in turn
+        uint64_t w[MAX_CHUNKS / NW], n[MAX_CHUNKS / NW];
+        const uint64_t* gp = a.gsum + 2 * ((size_t)r * a.chunks * NG + (t & 63));
+#pragma unroll
+        for (int i = 0; i < MAX_CHUNKS / NW; i++) {
+            const int k = min((t >> 6) + i * NW, a.chunks - 1);
+            w[i] = get_agent(gp + 2 * (size_t)k * NG);
+            n[i] = get_agent(gp + 2 * (size_t)k * NG + 1);
+        }
+        if (t < NG) {
+            sh.gc[t] = 0;
+            sh.gw[t] = 0;
+        }
+        __syncthreads();
+        uint64_t sw = 0, sn = 0;
+#pragma unroll
+        for (int i = 0; i < MAX_CHUNKS / NW; i++)
+            if ((t >> 6) + i * NW < a.chunks) {
+                sw += w[i];
+                sn += n[i];
+            }
+        if (sn) {
+            atomicAdd(&sh.gc[t & 63], (uint32_t)sn);
+            atomicAdd(&sh.gw[t & 63], (unsigned long long)sw);
         }
         __syncthreads();
     }
-    find_borders(a, sh, row, st);
+    find_borders(a, sh, row, st, r);
 }
 
 // ---------------------------------------------------------------------------
@@ -476,168 +581,125 @@ struct PickShared {
     uint32_t n_list;
 };
 
-// Descending sort of sh.list[0, n): short lists by counting the larger ones
-// (the composites differ), longer ones bitonic.
-DEV void sort_desc(PickShared& sh, int n) {
-    __syncthreads();
-    if (n <= 2 * NT) {
-        uint64_t v[2];
-        int rank[2] = {0, 0};
-#pragma unroll
-        for (int e = 0; e < 2; e++) v[e] = threadIdx.x + e * NT < n ? sh.list[threadIdx.x + e * NT] : 0;
-        for (int j = 0; j < n; j++) {
-            const uint64_t o = sh.list[j];
-            rank[0] += o > v[0];
-            rank[1] += o > v[1];
+// Entry of sh.list[0, n) (weights in sh.lw) at which a prefix in descending
+// order of key(entry) (distinct integers) meets `want`, n0 tokens and w0
+// weight before it, among the entries that in(entry) takes; *sum the weight up
+// to and with it.  -1: none does.  Radix selection, 8 bits at a time from the
+// highest bit in which two keys differ, until one entry is left.
+template <typename K, typename I>
+DEV int select(PickShared& sh, int n, const Want& want, uint64_t n0, uint64_t w0, K key, I in, uint64_t* sum) {
+    const int t = threadIdx.x;
+    // the bits in which keys differ: or and and of all
+    uint64_t any = 0, all = ~0ull;
+    for (int i = t; i < n; i += NT)
+        if (in(i)) {
+            any |= key(i);
+            all &= key(i);
         }
-        __syncthreads();
 #pragma unroll
-        for (int e = 0; e < 2; e++)
-            if (threadIdx.x + e * NT < n) sh.list[rank[e]] = v[e];
-        __syncthreads();
-        return;
+    for (int d = 1; d < 64; d <<= 1) {
+        any |= (uint64_t)__shfl_xor((uint32_t)(any >> 32), d) << 32 | __shfl_xor((uint32_t)any, d);
+        all &= (uint64_t)__shfl_xor((uint32_t)(all >> 32), d) << 32 | __shfl_xor((uint32_t)all, d);
     }
-    int n2 = 1;
-    while (n2 < n) n2 <<= 1;
-    for (int i = n + threadIdx.x; i < n2; i += NT) sh.list[i] = 0;
-    for (int k = 2; k <= n2; k <<= 1)
-        for (int j = k >> 1; j > 0; j >>= 1) {
-            __syncthreads();
-            for (int i = threadIdx.x; i < n2 / 2; i += NT) {
-                const int x = (i & ~(j - 1)) << 1 | (i & (j - 1)), y = x | j;
-                const uint64_t p = sh.list[x], q = sh.list[y];
-                if ((p < q) == !(x & k)) {
-                    sh.list[x] = q;
-                    sh.list[y] = p;
+    __syncthreads();
+    if ((t & 63) == 0) {
+        sh.wsum[t >> 6] = any;
+        sh.wsum[NW + (t >> 6)] = all;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < NW; w++) {
+        any |= sh.wsum[w];
+        all &= sh.wsum[NW + w];
+    }
+    const uint64_t differ = any & ~all;
+    int top = differ ? 64 - __clzll((long long)differ) : 1;      // keys agree from this bit up
+    uint64_t known = top < 64 ? all >> top << top : 0;
+    for (;;) {
+        const int low = top > 8 ? top - 8 : 0, mask = (1 << (top - low)) - 1;
+        __syncthreads();
+        sh.count[t] = 0;
+        sh.wsum[t] = 0;
+        if (t == 0) sh.i0 = -1;
+        __syncthreads();
+        for (int i = t; i < n; i += NT)
+            if (in(i)) {
+                const uint64_t k = key(i);
+                if (top == 64 || k >> top == known >> top) {
+                    const int b = mask - (int)(k >> low & mask);
+                    atomicAdd(&sh.count[b], 1u);
+                    atomicAdd(&sh.wsum[b], (unsigned long long)sh.lw[i]);
                 }
             }
+        __syncthreads();
+        const uint64_t c = sh.count[t], w = sh.wsum[t];
+        uint64_t tc, tw;
+        const uint64_t n1 = scan64(sh.red, c, &tc) + n0, w1 = scan64(sh.red, w, &tw) + w0;
+        if (want.met(n1, w1) && !want.met(n1 - c, w1 - w)) {
+            sh.i0 = t;
+            sh.i1 = (int)c;
+            sh.b0 = n1 - c;
+            sh.b1 = w1 - w;
         }
-    __syncthreads();
-}
-
-// What a prefix search looks for: the first `count` tokens, or the shortest
-// prefix whose weights reach `goal`.
-struct Want {
-    uint64_t count;
-    double goal;
-    bool by_weight;
-    DEV bool met(uint64_t n, uint64_t w) const { return by_weight ? (double)w >= goal : n >= count; }
-};
-
-// Position in sh.list[i0, i1) (sorted) at which a prefix with n0 tokens and w0
-// weight before it meets `want`, and *sum the weight up to and with it; i1 - 1
-// where it does not.
-template <typename L>
-DEV int walk(PickShared& sh, const Row<L>& row, const Want& want, int i0, int i1, uint64_t n0, uint64_t w0,
-             uint64_t* sum) {
-    constexpr int PER = CAP / NT;
-    const int t = threadIdx.x;
-    uint64_t w[PER], tot = 0, all;
-#pragma unroll
-    for (int e = 0; e < PER; e++) {
-        const int at = i0 + PER * t + e;
-        w[e] = at < i1 ? row.weight_of(sh.list[at]) : 0;
-        tot += w[e];
-    }
-    uint64_t s = scan64(sh.red, tot, &all) - tot + w0;
-    if (t == 0) {
-        sh.i0 = i1 - 1;
-        sh.b0 = w0 + all;
+        __syncthreads();
+        const int b = sh.i0;
+        if (b < 0) return -1;
+        n0 = sh.b0;
+        w0 = sh.b1;
+        const int left = sh.i1;
+        known |= (uint64_t)(mask - b) << low;
+        top = low;
+        if (left == 1 || top == 0) break;
     }
     __syncthreads();
-#pragma unroll
-    for (int e = 0; e < PER; e++) {
-        const int at = i0 + PER * t + e;
-        const uint64_t n = n0 + PER * t + e;
-        if (at < i1 && !want.met(n, s) && want.met(n + 1, s + w[e])) {
-            sh.i0 = at;
-            sh.b0 = s + w[e];
-        }
-        s += w[e];
-    }
+    for (int i = t; i < n; i += NT)
+        if (in(i) && key(i) >> top == known >> top) sh.i0 = i;
     __syncthreads();
     const int at = sh.i0;
-    *sum = sh.b0;
+    *sum = w0 + sh.lw[at];
     __syncthreads();
     return at;
 }
 
-// Draws from the sorted list's first m tokens, in index order.
-template <typename L> DEV void draw_list(const SmArgs& a, PickShared& sh, const Row<L>& row, int r, int m) {
-    const int t = threadIdx.x;
-    uint64_t own = 0, total;
-    for (int i = t; i < m; i += NT) {
-        sh.lw[i] = row.weight_of(sh.list[i]);
-        own += sh.lw[i];
-    }
-    scan64(sh.red, own, &total);
-    __syncthreads();
-    const uint64_t aim = aim_of(a.u[r], total);
-    if (m <= 2 * NT) {
-        // a token's running sum: the weights of the kept ones before it
-        for (int i = t; i < m; i += NT) {
-            const uint32_t me = (uint32_t)sh.list[i];       // larger for earlier tokens
-            uint64_t before = 0;
-            for (int j = 0; j < m; j++) before += (uint32_t)sh.list[j] > me ? sh.lw[j] : 0;
-            if (before <= aim && aim < before + sh.lw[i])
-                answer(a, row, r, index_of(sh.list[i]), logit_of(sh.list[i]), total);
-        }
-        return;
-    }
-    for (int i = t; i < m; i += NT) sh.list[i] = sh.list[i] << 32 | sh.list[i] >> 32;
-    sort_desc(sh, m);
-    constexpr int PER = CAP / NT;
-    uint64_t w[PER], tot = 0, all;
-#pragma unroll
-    for (int e = 0; e < PER; e++) {
-        const int at = PER * t + e;
-        w[e] = at < m ? row.weight(row.depth(from_bits((uint32_t)sh.list[at]))) : 0;
-        tot += w[e];
-    }
-    uint64_t s = scan64(sh.red, tot, &all) - tot;
-#pragma unroll
-    for (int e = 0; e < PER; e++) {
-        const int at = PER * t + e;
-        if (s <= aim && aim < s + w[e])
-            answer(a, row, r, index_of(sh.list[at] >> 32), from_bits((uint32_t)sh.list[at]), total);
-        s += w[e];
-    }
-}
-
 // The token of [lo, hi) whose running sum of kept(token, logit), `base` before
-// lo, passes aim: every wave sums a run, then all walk the run that holds it.
+// lo, passes aim: by tiles of TE consecutive tokens a thread, the next tile's
+// loads ahead of the current one's sums.
 template <typename L, typename F>
 DEV void draw_range(const SmArgs& a, PickShared& sh, const Row<L>& row, int r, int lo, int hi, uint64_t base,
                     uint64_t aim, uint64_t total, F kept) {
-    const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
-    const int run = (hi - lo + NW - 1) / NW, r0 = lo + wave * run, r1 = min(r0 + run, hi);
-    uint64_t s = 0;
-    for (int i = r0 + lane; i < r1; i += 64) s += kept(i, L::one(row.p, i));
+    constexpr int TE = 8;
+    const int t = threadIdx.x;
+    auto load = [&](int i0, float* x) {
+        if (row.vec && i0 + TE <= hi) {       // lo and the tiles are multiples of 8
 #pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-        const uint64_t o = shfl_up64(s, d);
-        if (lane >= d) s += o;
-    }
-    __syncthreads();
-    if (lane == 63) sh.red[wave] = s;
-    __syncthreads();
-    int w0 = 0;
-    while (w0 < NW - 1 && base + sh.red[w0] <= aim) base += sh.red[w0++];
-    const int s0 = lo + w0 * run, s1 = min(s0 + run, hi);
-    const int per = (run + NT - 1) / NT, i0 = min(s0 + t * per, s1), i1 = min(i0 + per, s1);
-    uint64_t own = 0, all;
-    for (int i = i0; i < i1; i++) own += kept(i, L::one(row.p, i));
-    const uint64_t end = scan64(sh.red, own, &all) + base;
-    if (own && end > aim && end - own <= aim) {
-        uint64_t at = end - own;
-        for (int i = i0; i < i1; i++) {
-            const float x = L::one(row.p, i);
-            at += kept(i, x);
-            if (at > aim) {
-                answer(a, row, r, i, x, total);
-                break;
-            }
+            for (int e = 0; e < TE; e += L::VE) L::many(row.p, i0 + e, x + e);
+        } else {
+#pragma unroll
+            for (int e = 0; e < TE; e++) x[e] = i0 + e < hi ? L::one(row.p, i0 + e) : -__builtin_huge_valf();
         }
+    };
+    float x[TE], nx[TE];
+    load(lo + t * TE, x);
+    for (int i0 = lo + t * TE; i0 - t * TE < hi; i0 += NT * TE) {
+        if (i0 - t * TE + NT * TE < hi) load(i0 + NT * TE, nx);
+        uint64_t w[TE], own = 0, all;
+#pragma unroll
+        for (int e = 0; e < TE; e++) {
+            w[e] = i0 + e < hi ? kept(i0 + e, x[e]) : 0;
+            own += w[e];
+        }
+        uint64_t s = scan64(sh.red, own, &all) - own + base;
+        if (base + all > aim) {
+#pragma unroll
+            for (int e = 0; e < TE; e++) {
+                if (s <= aim && aim < s + w[e]) answer(a, row, r, i0 + e, x[e], total);
+                s += w[e];
+            }
+            return;
+        }
+        base += all;
+#pragma unroll
+        for (int e = 0; e < TE; e++) x[e] = nx[e];
     }
 }
 
@@ -741,24 +803,24 @@ DEV uint64_t split_cut(PickShared& sh, const Row<L>& row, const Want& want, uint
         });
         __syncthreads();
         const int n = min((int)sh.n_list, CAP);
-        sort_desc(sh, n);
-        const int at = walk(sh, row, want, 0, n, bn, bw, sum);
-        return sh.list[at];
+        for (int i = t; i < n; i += NT) sh.lw[i] = row.weight_of(sh.list[i]);
+        __syncthreads();
+        const int at = select(sh, n, want, bn, bw, [&](int i) { return sh.list[i]; }, [](int) { return true; }, sum);
+        return at < 0 ? least : sh.list[at];
     }
     return least;
 }
 
 template <typename L> DEV void split_row(const SmArgs& a, PickShared& sh, const Row<L>& row, const SmState& st, int r) {
     uint64_t cut = 0, total = st.total;
-    if (st.by_k) cut = split_cut(sh, row, Want{(uint64_t)row.k, 0.0, false}, 0, &total);
+    if (st.by_k) cut = split_cut(sh, row, Want{BY_COUNT, (uint64_t)row.k, 0.0}, 0, &total);
     if (st.by_p) {
         uint64_t s;
-        const uint64_t c = split_cut(sh, row, Want{0, row.goal(total), true}, cut, &s);
+        const uint64_t c = split_cut(sh, row, Want{BY_GOAL, 0, row.goal(total)}, cut, &s);
         cut = c > cut ? c : cut;
     }
     auto kept = [&](int i, float x) -> uint64_t {
-        const double d = row.depth(x);
-        return comp_of(x, i) >= cut && row.above_min(d) ? row.weight(d) : 0;
+        return comp_of(x, i) >= cut ? row.weight_min(row.depth(x)) : 0;
     };
     uint64_t own = 0;
     each<L>(row.p, row.vec, 0, row.V, [&](int i, float x) { own += kept(i, x); });
@@ -779,10 +841,7 @@ template <typename L> __global__ __launch_bounds__(NT) void k_smp_pick(SmArgs a)
         uint64_t base, aim, total;
         const int at = pick_chunk(lane < a.chunks ? a.csum[(size_t)r * a.chunks + lane] : 0, a.u[r], &base, &aim, &total);
         draw_range(a, sh, row, r, at * a.chunk, min(a.V, (at + 1) * a.chunk), base, aim, total,
-                   [&](int, float x) -> uint64_t {
-                       const double d = row.depth(x);
-                       return row.above_min(d) ? row.weight(d) : 0;
-                   });
+                   [&](int, float x) -> uint64_t { return row.weight_min(row.depth(x)); });
         return;
     }
     const SmState st = *sp;
@@ -819,103 +878,73 @@ template <typename L> __global__ __launch_bounds__(NT) void k_smp_pick(SmArgs a)
         __syncthreads();
         for (int i = t; i < n; i += NT) sh.list[i] = get_agent(list + i);
     }
-    sort_desc(sh, n);
-    uint64_t sum = st.total;
-    if (mode == SM_LIST) {
-        // the list holds everything top-k or top-p could keep
-        int m = n;
-        if (st.by_k) {
-            m = walk(sh, row, Want{(uint64_t)row.k, 0.0, false}, 0, n, 0, 0, &sum) + 1;
-        }
-        if (st.by_p) {
-            uint64_t s;
-            m = min(m, walk(sh, row, Want{0, row.goal(sum), true}, 0, n, 0, 0, &s) + 1);
-        }
-        if (st.by_m) {
-            if (t == 0) sh.i1 = 0;
-            __syncthreads();
-            for (int i = t; i < m; i += NT)
-                if (row.above_min(row.depth(logit_of(sh.list[i])))) atomicMax(&sh.i1, i + 1);
-            __syncthreads();
-            m = max(1, min(m, sh.i1));
-        }
-        draw_list(a, sh, row, r, m);
-        return;
-    }
-    // first list entry of a bin, or n: bins ascend along the sorted list
-    auto first_of = [&](int b) -> int {
-        if (t == 0) sh.i1 = n;
-        __syncthreads();
-        for (int i = t; i < n; i += NT)
-            if (row.bin(row.depth(logit_of(sh.list[i]))) >= b) atomicMin(&sh.i1, i);
-        __syncthreads();
-        const int at = sh.i1;
-        __syncthreads();
-        return at;
-    };
-    int cb = NB;               // the border: bins above cb stay, and of it the composites from cc
-    uint64_t cc = 0;
-    auto cut_at = [&](int b, uint64_t comp) {
-        if (b < cb || (b == cb && comp > cc)) {
-            cb = b;
-            cc = comp;
-        }
-    };
+    __syncthreads();
+    for (int i = t; i < n; i += NT) sh.lw[i] = row.weight_of(sh.list[i]);
+    __syncthreads();
+    auto comp = [&](int i) { return sh.list[i]; };
+    auto bin_of = [&](int i) { return row.bin(row.depth(logit_of(sh.list[i]))); };
+    uint64_t sum = st.total, cut = 0;      // composites below cut are out
     if (st.by_k) {
-        const int i0 = first_of(st.bk), i1 = first_of(st.bk + 1);
-        const int at = walk(sh, row, Want{st.rk, 0.0, false}, i0, i1, 0, st.wk, &sum);
-        cut_at(st.bk, sh.list[at]);
+        const int at = mode == SM_LIST
+                           ? select(sh, n, Want{BY_COUNT, (uint64_t)row.k, 0.0}, 0, 0, comp, [](int) { return true; }, &sum)
+                           : select(sh, n, Want{BY_COUNT, st.rk, 0.0}, 0, st.wk, comp,
+                                    [&](int i) { return bin_of(i) == st.bk; }, &sum);
+        if (at >= 0) cut = sh.list[at];
     }
     if (st.by_p) {
-        const int i0 = first_of(st.pl), i1 = first_of(st.ph + 1);
+        const Want want = {BY_GOAL, 0, row.goal(sum)};
         uint64_t s;
-        const int at = walk(sh, row, Want{0, row.goal(sum), true}, i0, i1, 0, st.wp, &s);
-        cut_at(row.bin(row.depth(logit_of(sh.list[at]))), sh.list[at]);
+        const int at = mode == SM_LIST ? select(sh, n, want, 0, 0, comp, [](int) { return true; }, &s)
+                                       : select(sh, n, want, 0, st.wp, comp,
+                                                [&](int i) {
+                                                    const int b = bin_of(i);
+                                                    return b >= st.pl && b <= st.ph;
+                                                },
+                                                &s);
+        if (at >= 0 && sh.list[at] > cut) cut = sh.list[at];
     }
-    if (st.by_m) {
-        const int i0 = first_of(st.ml), i1 = first_of(st.mh + 1);
-        if (t == 0) sh.i0 = -1;
-        __syncthreads();
-        for (int i = i0 + t; i < i1; i += NT)
-            if (row.above_min(row.depth(logit_of(sh.list[i])))) atomicMax(&sh.i0, i);
-        __syncthreads();
-        const int at = sh.i0;
-        __syncthreads();
-        if (at < 0) cut_at(st.ml, ~0ull);
-        else cut_at(row.bin(row.depth(logit_of(sh.list[at]))), sh.list[at]);
-    }
-    // the chunks' sums: bins above the border, and what stays of its own
-    for (int k = wave; k < a.chunks; k += NW) {
-        const uint64_t* w = a.wsum + ((size_t)r * a.chunks + k) * NB;
-        uint64_t s = 0;
-        for (int b = lane; b < cb; b += 64) s += get_agent(w + b);
-#pragma unroll
-        for (int d = 1; d < 64; d <<= 1) {
-            const uint64_t o = shfl_up64(s, d);
-            if (lane >= d) s += o;
-        }
-        if (lane == 63) sh.lw[k] = s;
-    }
-    __syncthreads();
+    // what stays of the list
     for (int i = t; i < n; i += NT)
-        if (sh.list[i] >= cc && row.bin(row.depth(logit_of(sh.list[i]))) == cb)
-            atomicAdd((unsigned long long*)&sh.lw[index_of(sh.list[i]) / a.chunk],
-                      (unsigned long long)row.weight_of(sh.list[i]));
+        if (sh.list[i] < cut || row.weight_min(row.depth(logit_of(sh.list[i]))) == 0) sh.lw[i] = 0;
+    __syncthreads();
+    if (mode == SM_LIST) {
+        uint64_t own = 0, total;
+        for (int i = t; i < n; i += NT) own += sh.lw[i];
+        scan64(sh.red, own, &total);
+        const int at = select(sh, n, Want{BY_SUM, aim_of(a.u[r], total), 0.0}, 0, 0,
+                              [&](int i) { return sh.list[i] & 0xffffffffull; }, [](int) { return true; }, &sum);
+        if (t == 0 && at >= 0) answer(a, row, r, index_of(sh.list[at]), logit_of(sh.list[at]), total);
+        return;
+    }
+    // the chunks' sums: the bins above the highest border, and what stays of
+    // the list from there on
+    const int cb = min(cut ? row.bin(row.depth(logit_of(cut))) : NB, st.by_m ? st.ml : NB), g = cb / GB;
+    if (t < MAX_CHUNKS) sh.wsum[t] = 0;
+    __syncthreads();
+    for (int k = wave; k < a.chunks; k += NW) {
+        const size_t at = (size_t)r * a.chunks + k;
+        uint64_t s = 0;
+        if (a.chunks == 1) {
+            for (int b = lane; b < cb; b += 64) s += a.wsum[at * NB + b];
+        } else {
+            if (lane < g) s = get_agent(a.gsum + 2 * (at * NG + lane));
+            if (lane < cb - g * GB) s += get_agent(a.wsum + at * NB + g * GB + lane);
+        }
+        if (s) atomicAdd(&sh.wsum[k], (unsigned long long)s);
+    }
+    for (int i = t; i < n; i += NT)
+        if (sh.lw[i] && bin_of(i) >= cb)
+            atomicAdd(&sh.wsum[index_of(sh.list[i]) / a.chunk], (unsigned long long)sh.lw[i]);
     __syncthreads();
     uint64_t base, aim, total;
-    const int at = pick_chunk(lane < a.chunks ? sh.lw[lane] : 0, a.u[r], &base, &aim, &total);
+    const int at = pick_chunk(lane < a.chunks ? sh.wsum[lane] : 0, a.u[r], &base, &aim, &total);
     draw_range(a, sh, row, r, at * a.chunk, min(a.V, (at + 1) * a.chunk), base, aim, total,
-               [&](int i, float x) -> uint64_t {
-                   const double d = row.depth(x);
-                   if (!(d < row.A)) return 0;
-                   const int b = row.bin(d);
-                   return b < cb || (b == cb && comp_of(x, i) >= cc) ? row.weight(d) : 0;
-               });
+               [&](int i, float x) -> uint64_t { return comp_of(x, i) >= cut ? row.weight_min(row.depth(x)) : 0; });
 }
 
 struct SmPlan {
     int rows, chunk, chunks;
-    size_t best, csum, wsum, list, count, state, bytes;
+    size_t best, csum, wsum, gsum, list, count, state, bytes;
 };
 
 // Chunks of at least 4 096 tokens, as many as give about four workgroups a CU
@@ -932,7 +961,8 @@ SmPlan plan(int n, int V) {
     p.best = 0;
     p.csum = p.best + k * 8;
     p.wsum = p.csum + k * 8;
-    p.list = p.wsum + k * NB * 8;
+    p.gsum = p.wsum + k * NB * 8;
+    p.list = p.gsum + k * NG * 16;
     p.count = p.list + (size_t)p.rows * CAP * 8;
     p.state = p.count + k * NB * 4;
     p.bytes = p.state + (size_t)p.rows * sizeof(SmState);
@@ -963,7 +993,7 @@ void dpuf_hip_sample(void* s, int32_t type, int32_t n, int32_t V, int64_t stride
     a.V = V;
     int lg = 0;
     while ((1 << lg) < V) lg++;
-    a.S = 62 - lg;
+    a.S = 62 - lg < 51 ? 62 - lg : 51;
     a.vec = ((uintptr_t)x & 15) == 0 && (stride * es) % 16 == 0;
     a.chunk = pl.chunk;
     a.chunks = pl.chunks;
@@ -971,6 +1001,7 @@ void dpuf_hip_sample(void* s, int32_t type, int32_t n, int32_t V, int64_t stride
     a.best = (uint64_t*)(w + pl.best);
     a.csum = (uint64_t*)(w + pl.csum);
     a.wsum = (uint64_t*)(w + pl.wsum);
+    a.gsum = (uint64_t*)(w + pl.gsum);
     a.list = (uint64_t*)(w + pl.list);
     a.count = (uint32_t*)(w + pl.count);
     a.state = (SmState*)(w + pl.state);
