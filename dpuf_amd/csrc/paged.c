@@ -13,6 +13,7 @@
 
 #define MAX_SEQS 16384
 #define MAX_ROWS 65536
+#define MAX_ROW_STRIDE ((int64_t)1 << 26) /* the kernels hold 16 rows' offsets in 32 bits */
 
 static int aligned(const void* p, uintptr_t n) { return p && ((uintptr_t)p & (n - 1)) == 0; }
 
@@ -42,6 +43,7 @@ static int32_t check_pages(const DpufAmdPages* p) {
     const int64_t s[3] = {p->page_stride, p->head_stride, p->row_stride};
     for (int i = 0; i < 3; i++)
         if (s[i] < p->head_dim || s[i] % 8 != 0) return -4;
+    if (p->row_stride > MAX_ROW_STRIDE) return -4;
     if (!aligned(p->k, 16) || !aligned(p->v, 16)) return -1;
     return 0;
 }

@@ -17,6 +17,11 @@
 // operand takes the order in which S^T left them: 4 keys of each half or
 // quarter of the wave, which is what one transposing LDS read gives.
 //
+// The running maximum need not be the largest score so far, only near it: m is
+// moved (and l and o multiplied, a product per sum) when a score passes it by
+// more than 2^SLACK, so that most tiles move nothing; p is at most 2^SLACK
+// then, far inside fp16's range.
+//
 // Exponentials are of base 2 with the scale folded in (one fma each); p is
 // rounded to the pages' type for the product with V (a relative half step,
 // 2^-8 in bf16 and 2^-11 in fp16, of each term), every sum is fp32.
@@ -29,6 +34,7 @@
 namespace {
 
 const float NEG_INF = -__builtin_huge_valf();
+constexpr float SLACK = 6.0f;
 
 struct PaArgs {
     DpufAmdBatch b;
@@ -201,14 +207,15 @@ __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void k_pa_few(PaArgs a) {
         float mt = fmaxf(fmaxf(fmaxf(sc[0][0], sc[0][1]), fmaxf(sc[0][2], sc[0][3])),
                          fmaxf(fmaxf(sc[1][0], sc[1][1]), fmaxf(sc[1][2], sc[1][3])));
         mt = max_xor32(max_xor16(mt)) * a.c2;
-        const float mn = fmaxf(m, mt), ms = mn == NEG_INF ? 0.0f : mn;
-        if (__any(mn != m)) {
-            const float f = __builtin_amdgcn_exp2f(m - ms);
+        // m follows the maximum only when it is behind by more than 2^SLACK
+        if (__any(mt > m + SLACK)) {
+            const float mn = fmaxf(m, mt), f = __builtin_amdgcn_exp2f(m - (mn == NEG_INF ? 0.0f : mn));
             l *= f;
 #pragma unroll
             for (int d = 0; d < ND; d++) o[d] *= f;
             m = mn;
         }
+        const float ms = m == NEG_INF ? 0.0f : m;
         float pr[8];
 #pragma unroll
         for (int u = 0; u < 2; u++)
@@ -369,29 +376,46 @@ __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void k_pa_many(PaArgs a) {
         for (int i = 0; i < 16; i++) o[d][i] = 0.0f;
     float m = NEG_INF, l = 0.0f;
 
+    // A tile's pages, one for each 16 keys (pages hold a multiple of 16 rows),
+    // are the same for all lanes: a thread's address is its own offset within
+    // 16 rows plus a scalar base.
+    constexpr int NG = KT / 16;
     const int lr = threadIdx.x / CH, lc = 8 * (threadIdx.x % CH);   // row and column of this thread's pieces
-    const uint16_t* kp = (const uint16_t*)a.p.k + (size_t)kvh * a.p.head_stride + lc;
-    const uint16_t* vp = (const uint16_t*)a.p.v + (size_t)kvh * a.p.head_stride + lc;
+    const int wr = __builtin_amdgcn_readfirstlane(lr) & 16;          // first row of the wave's 16 (RP = 32)
+    const uint32_t lo = (uint32_t)((lr & 15) * (int)a.p.row_stride + lc);
+    const uint16_t* kp = (const uint16_t*)a.p.k + (size_t)kvh * a.p.head_stride;
+    const uint16_t* vp = (const uint16_t*)a.p.v + (size_t)kvh * a.p.head_stride;
     const int* table = a.b.page_table + (size_t)s * a.b.table_stride;
     const int top = sq.ctx > 0 ? (sq.ctx - 1) >> a.shift : 0;
-    const int wr = __builtin_amdgcn_readfirstlane(lr) & ~7;          // the wave's rows lie within 16 of a page
     u32x4 kf[NP], vf[NP];
-    int pn[NP];
+    int pn[NG];              // pages of the tile to be loaded next
+    uint32_t bad1 = 0, bad2 = 0;   // of the tile in kf / vf (one bit per 16 keys: outside the pool), and of the next
     auto pages = [&](int base) {
 #pragma unroll
-        for (int u = 0; u < NP; u++) pn[u] = table[min((base + u * RP + wr) >> a.shift, top)];
+        for (int g = 0; g < NG; g++) pn[g] = table[min((base + 16 * g) >> a.shift, top)];
     };
     auto load = [&](int base) {
+        bad2 = 0;
+#pragma unroll
+        for (int g = 0; g < NG; g++) bad2 |= ((unsigned)pn[g] >= (unsigned)a.p.n_pages) << g;
 #pragma unroll
         for (int u = 0; u < NP; u++) {
-            const int key = base + u * RP + lr;
-            const bool in = (unsigned)pn[u] < (unsigned)a.p.n_pages;
-            const size_t off = (size_t)(in ? pn[u] : 0) * a.p.page_stride +
-                               (size_t)(key & (a.p.page_size - 1)) * a.p.row_stride;
-            kf[u] = *(const u32x4*)(kp + off);
-            vf[u] = *(const u32x4*)(vp + off);
+            const int g = RP == 32 ? 2 * u + (wr >> 4) : u * RP / 16;
+            int pg = RP == 32 ? (wr ? pn[(2 * u + 1) % NG] : pn[2 * u % NG]) : pn[u * RP / 16 % NG];
+            if ((bad2 >> g) & 1) pg = 0;
+            const size_t at = (size_t)pg * a.p.page_stride +
+                              (size_t)((base + 16 * g) & (a.p.page_size - 1)) * a.p.row_stride +
+                              (RP == 8 ? (size_t)(u & 1) * 8 * a.p.row_stride : 0);
+            kf[u] = *(const u32x4*)(kp + at + lo);
+            vf[u] = *(const u32x4*)(vp + at + lo);
+        }
+        if (bad2 || base + KT > kend) {
             // rows that nobody sees: any bits, and 0 * NaN is NaN
-            if (!in || key >= kend) vf[u] = u32x4{0, 0, 0, 0};
+#pragma unroll
+            for (int u = 0; u < NP; u++) {
+                const int key = u * RP + lr;
+                if (base + key >= kend || ((bad2 >> (key >> 4)) & 1)) vf[u] = u32x4{0, 0, 0, 0};
+            }
         }
     };
     auto store = [&](int buf) {
@@ -407,6 +431,7 @@ __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void k_pa_many(PaArgs a) {
         load(k0);
         pages(k0 + KT);
         store(0);
+        bad1 = bad2;
         if (k0 + KT < kend) {
             load(k0 + KT);
             pages(k0 + 2 * KT);
@@ -416,26 +441,21 @@ __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void k_pa_many(PaArgs a) {
     for (int base = k0; base < kend; base += KT, buf ^= 1) {
         __syncthreads();
         if (base + KT < kend) store(buf ^ 1);
-        // pages of this tile that are outside the pool: one bit per 16 keys
-        uint32_t bad = 0;
-        for (int u = 0; u < KT / 16; u++)
-            bad |= ((unsigned)table[min((base + 16 * u) >> a.shift, top)] >= (unsigned)a.p.n_pages) << u;
+        const uint32_t bad = bad1;
+        bad1 = bad2;
         if (base + 2 * KT < kend) {
             load(base + 2 * KT);
             pages(base + 3 * KT);
         }
         if (base >= wend) continue;
+        const f32x16 zero = {};
         f32x16 sc[NB];
-#pragma unroll
-        for (int b = 0; b < NB; b++)
-#pragma unroll
-            for (int i = 0; i < 16; i++) sc[b][i] = 0.0f;
 #pragma unroll
         for (int c = 0; c < NC; c++)
 #pragma unroll
             for (int b = 0; b < NB; b++) {
                 const v8 kv = vec_of<v8>(*(const u32x4*)(lk[buf] + (32 * b + col) * KP + 16 * c + 8 * h));
-                sc[b] = T::mma32(kv, qf[c], sc[b]);
+                sc[b] = T::mma32(kv, qf[c], c ? sc[b] : zero);
             }
         // sc[b][i]: key 32 b + 8 (i / 4) + 4 h + i % 4
         if (base + KT > min(wend, first_limit + 1) || bad) {
@@ -453,14 +473,15 @@ __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void k_pa_many(PaArgs a) {
 #pragma unroll
             for (int i = 0; i < 16; i++) mt = fmaxf(mt, sc[b][i]);
         mt = max_xor32(mt) * a.c2;
-        const float mn = fmaxf(m, mt), ms = mn == NEG_INF ? 0.0f : mn;
-        if (__any(mn != m)) {
-            const float f = __builtin_amdgcn_exp2f(m - ms);
+        // m follows the maximum only when it is behind by more than 2^SLACK
+        if (__any(mt > m + SLACK)) {
+            const float mn = fmaxf(m, mt), f = __builtin_amdgcn_exp2f(m - (mn == NEG_INF ? 0.0f : mn));
             l *= f;
 #pragma unroll
             for (int d = 0; d < ND; d++) o[d] *= f;
             m = mn;
         }
+        const float ms = m == NEG_INF ? 0.0f : m;
 #pragma unroll
         for (int b = 0; b < NB; b++)
 #pragma unroll

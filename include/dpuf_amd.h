@@ -178,8 +178,8 @@ enum {
 
 /* One layer's pages.  Row r of page p of kv head h starts at element
  * p * page_stride + h * head_stride + r * row_stride of k and of v (any order
- * of the three, each a multiple of 8 elements and at least head_dim; k and v
- * on 16 bytes).  w holds one accumulated weight per row,
+ * of the three, each a multiple of 8 elements and at least head_dim,
+ * row_stride at most 2^26; k and v on 16 bytes).  w holds one accumulated weight per row,
  * [n_pages][n_kv_heads][page_size], or is NULL where no operator needs it. */
 typedef struct {
     int32_t type;         /* DPUF_AMD_BF16 or DPUF_AMD_F16 */
