@@ -38,7 +38,7 @@ static int32_t check_pages(const DpufAmdPages* p) {
     if (!p) return -1;
     if (p->type != DPUF_AMD_BF16 && p->type != DPUF_AMD_F16) return -5;
     if (p->head_dim != 64 && p->head_dim != 128 && p->head_dim != 256) return -5;
-    if (p->n_pages < 1 || p->n_kv_heads < 1 || p->n_kv_heads > 1024) return -2;
+    if (p->n_pages < 1 || p->n_kv_heads < 1 || p->n_kv_heads > 256) return -2;
     if (p->page_size < 16 || p->page_size > 1024 || (p->page_size & (p->page_size - 1))) return -2;
     const int64_t s[3] = {p->page_stride, p->head_stride, p->row_stride};
     for (int i = 0; i < 3; i++)

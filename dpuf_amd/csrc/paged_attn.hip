@@ -36,6 +36,8 @@ namespace {
 const float NEG_INF = -__builtin_huge_valf();
 constexpr float SLACK = 6.0f;
 
+enum { PA_BOTH = 0, PA_FEW, PA_MANY };
+
 struct PaArgs {
     DpufAmdBatch b;
     DpufAmdPages p;
@@ -43,15 +45,16 @@ struct PaArgs {
     int nq, G;
     const uint16_t* q;
     float c2;           // scale * log2 e
-    int few;            // packed rows up to which a sequence takes k_pa_few
+    int few;            // packed rows up to which a sequence takes the few-row kernel
+    int only;           // PA_BOTH, or the kernel that takes every sequence
     int nz_few, nz_many; // key ranges a sequence is split into at most
     int chunk_few, chunk_many;
     int out_f32;
     void* out;
     float* lse;
     // partial sums of rows whose keys are split: O unnormalised, (m, l);
-    // k_pa_few: [range][sequence][kv head][packed row], k_pa_many:
-    // [range][row][head]
+    // [range][row][head], or, for few rows where others have many,
+    // [range][sequence][kv head][packed row]
     float *few_o, *many_o;
     float2 *few_ml, *many_ml;
 };
@@ -63,8 +66,9 @@ DEV int range_keys(int ctx, int chunk, int nz) {
     return need <= chunk ? chunk : (need + 127) & ~127;
 }
 
-// Partial of packed row r of (range z, sequence s, kv head) in k_pa_few's.
-DEV size_t few_at(const PaArgs& a, int z, int s, int kvh, int r) {
+// Partial of a few-row sequence's packed row r (row: its place in the output).
+DEV size_t few_at(const PaArgs& a, int z, int s, int kvh, int r, size_t row) {
+    if (a.only == PA_FEW) return (size_t)z * a.b.n_rows * a.nq + row;
     return (((size_t)z * a.b.n_seqs + s) * a.p.n_kv_heads + kvh) * a.few + r;
 }
 
@@ -90,207 +94,212 @@ DEV float lse_of(float m2, float l) { return l > 0.0f ? (m2 + __log2f(l)) * 0.69
 // the end, so there is no barrier in the loop and each wave keeps a whole
 // next tile (K and V, 16 KB at 128 columns) in flight in registers.
 // ---------------------------------------------------------------------------
-template <typename T, int HD>
-__global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void k_pa_few(PaArgs a) {
+template <int HD> struct FewLds {
+    static constexpr int PITCH = HD + 16;   // elements of a V row: 4 rows of a transposing read in 4 bank groups
+    uint16_t v[4][32 * PITCH];
+    float2 ml[4][16];
+};
+
+template <typename T, int HD> DEV void few_rows(const PaArgs& a, FewLds<HD>& sh, int kvh, int y, int z) {
     constexpr int NC = HD / 32;          // 32-column steps of a key
     constexpr int ND = HD / 16;          // 16-column tiles of the output
-    constexpr int PITCH = HD + 16;       // elements of a V row in LDS: 4 rows of a transposing read in 4 bank groups
+    constexpr int PITCH = FewLds<HD>::PITCH;
     typedef typename T::v8 v8;
-    __shared__ __align__(16) uint16_t lds[4][32 * PITCH];
 
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int col = lane & 15, g4 = lane >> 4;
-    const int kvh = blockIdx.x, tiles = (a.few + 15) >> 4;
-    const int s = blockIdx.y / tiles, tile = blockIdx.y - s * tiles;
+    const int tiles = (a.few + 15) >> 4;
+    const int s = y / tiles;
     const PgSeq sq = pg_seq(a.b, a.shift, s);
     const int rows = sq.n * a.G;
-    if (rows > a.few || 16 * tile >= rows) return;
+    if (rows > a.few && a.only == PA_BOTH) return;
     const int per = range_keys(sq.ctx, a.chunk_few, a.nz_few);
     const int ranges = sq.ctx > per ? (sq.ctx + per - 1) / per : 1;
-    const int z = blockIdx.z;
     if (z >= ranges) return;
 
-    const int r = 16 * tile + col;
-    const bool live = r < rows;
-    const int qi = live ? r / a.G : 0, head = kvh * a.G + (live ? r - qi * a.G : 0);
-    const size_t row = (size_t)(sq.r0 + qi) * a.nq + head;
-    const int limit = live ? sq.ctx - sq.n + qi : -1;             // last key this row sees
-    const int last = min(rows, 16 * tile + 16) - 1;
-    const int first_limit = sq.ctx - sq.n + 16 * tile / a.G;      // of the tile's first row
-    const int k0 = z * per, kend = min(min(sq.ctx - sq.n + last / a.G + 1, sq.ctx), k0 + per);
+    // one tile of rows, unless a sequence has more than the others' few
+    for (int tile = y - s * tiles; 16 * tile < rows; tile += tiles) {
+        const int r = 16 * tile + col;
+        const bool live = r < rows;
+        const int qi = live ? r / a.G : 0, head = kvh * a.G + (live ? r - qi * a.G : 0);
+        const size_t row = (size_t)(sq.r0 + qi) * a.nq + head;
+        const int limit = live ? sq.ctx - sq.n + qi : -1;             // last key this row sees
+        const int last = min(rows, 16 * tile + 16) - 1;
+        const int first_limit = sq.ctx - sq.n + 16 * tile / a.G;      // of the tile's first row
+        const int k0 = z * per, kend = min(min(sq.ctx - sq.n + last / a.G + 1, sq.ctx), k0 + per);
 
-    v8 qf[NC];
-#pragma unroll
-    for (int c = 0; c < NC; c++)
-        qf[c] = live ? vec_of<v8>(*(const u32x4*)(a.q + row * HD + 32 * c + 8 * g4)) : vec_of<v8>(u32x4{0, 0, 0, 0});
-
-    f32x4 o[ND];
-#pragma unroll
-    for (int d = 0; d < ND; d++) o[d] = f32x4{0.f, 0.f, 0.f, 0.f};
-    float m = NEG_INF, l = 0.0f;
-
-    const uint16_t* kp = (const uint16_t*)a.p.k + (size_t)kvh * a.p.head_stride + 8 * g4;
-    const uint16_t* vp = (const uint16_t*)a.p.v + (size_t)kvh * a.p.head_stride + 8 * g4;
-    const int* table = a.b.page_table + (size_t)s * a.b.table_stride;
-    const int top = sq.ctx > 0 ? (sq.ctx - 1) >> a.shift : 0;
-    uint16_t* lv = lds[wave];
-
-    u32x4 kf[2][NC], vf[2][NC];
-    int pg[2], pn[2];      // pages of the tile in kf / vf, and of the one after it
-    // A 16-key half of a tile lies in one page (pages hold a multiple of 16
-    // rows); halves past the last key repeat it, pages outside the pool read
-    // page 0: both are masked below.
-    auto pages = [&](int base, int* out) {
-#pragma unroll
-        for (int u = 0; u < 2; u++) out[u] = table[min((base + 16 * u) >> a.shift, top)];
-    };
-    auto load = [&](int base, const int* pid) {
-#pragma unroll
-        for (int u = 0; u < 2; u++) {
-            const int key = base + 16 * u + col;
-            const bool in = (unsigned)pid[u] < (unsigned)a.p.n_pages;
-            const size_t off = (size_t)(in ? pid[u] : 0) * a.p.page_stride +
-                               (size_t)(key & (a.p.page_size - 1)) * a.p.row_stride;
-#pragma unroll
-            for (int c = 0; c < NC; c++) kf[u][c] = *(const u32x4*)(kp + off + 32 * c);
-#pragma unroll
-            for (int c = 0; c < NC; c++) vf[u][c] = *(const u32x4*)(vp + off + 32 * c);
-        }
-    };
-
-    int base = k0 + 32 * wave;
-    if (base < kend) {
-        pages(base, pg);
-        load(base, pg);
-        pages(base + 128, pn);
-    }
-    for (; base < kend; base += 128) {
-        // V goes to LDS for the transposing reads; the wave's own LDS
-        // operations are in order, so nothing but the compiler has to be held
-        const bool whole = base + 32 <= min(kend, first_limit + 1) && (unsigned)pg[0] < (unsigned)a.p.n_pages &&
-                           (unsigned)pg[1] < (unsigned)a.p.n_pages;
-        if (!whole) {
-            // a V row that no row of the tile sees may hold anything: 0 * inf
-            // and 0 * NaN would reach the sums
-#pragma unroll
-            for (int u = 0; u < 2; u++)
-                if (base + 16 * u + col >= kend || (unsigned)pg[u] >= (unsigned)a.p.n_pages)
-#pragma unroll
-                    for (int c = 0; c < NC; c++) vf[u][c] = u32x4{0, 0, 0, 0};
-        }
-        lds_order();
-#pragma unroll
-        for (int u = 0; u < 2; u++)
-#pragma unroll
-            for (int c = 0; c < NC; c++) *(u32x4*)(lv + (16 * u + col) * PITCH + 32 * c + 8 * g4) = vf[u][c];
-        f32x4 sc[2] = {f32x4{0.f, 0.f, 0.f, 0.f}, f32x4{0.f, 0.f, 0.f, 0.f}};
+        v8 qf[NC];
 #pragma unroll
         for (int c = 0; c < NC; c++)
+            qf[c] = live ? vec_of<v8>(*(const u32x4*)(a.q + row * HD + 32 * c + 8 * g4)) : vec_of<v8>(u32x4{0, 0, 0, 0});
+
+        f32x4 o[ND];
 #pragma unroll
-            for (int u = 0; u < 2; u++) sc[u] = T::mma16(vec_of<v8>(kf[u][c]), qf[c], sc[u]);
-        const int here = base;
-        const bool ok[2] = {(unsigned)pg[0] < (unsigned)a.p.n_pages, (unsigned)pg[1] < (unsigned)a.p.n_pages};
-        if (base + 128 < kend) {
-            pg[0] = pn[0];
-            pg[1] = pn[1];
-            load(base + 128, pg);
-            pages(base + 256, pn);
+        for (int d = 0; d < ND; d++) o[d] = f32x4{0.f, 0.f, 0.f, 0.f};
+        float m = NEG_INF, l = 0.0f;
+
+        const uint16_t* kp = (const uint16_t*)a.p.k + (size_t)kvh * a.p.head_stride + 8 * g4;
+        const uint16_t* vp = (const uint16_t*)a.p.v + (size_t)kvh * a.p.head_stride + 8 * g4;
+        const int* table = a.b.page_table + (size_t)s * a.b.table_stride;
+        const int top = sq.ctx > 0 ? (sq.ctx - 1) >> a.shift : 0;
+        uint16_t* lv = sh.v[wave];
+
+        u32x4 kf[2][NC], vf[2][NC];
+        int pg[2], pn[2];      // pages of the tile in kf / vf, and of the one after it
+        // A 16-key half of a tile lies in one page (pages hold a multiple of 16
+        // rows); halves past the last key repeat it, pages outside the pool read
+        // page 0: both are masked below.
+        auto pages = [&](int base, int* out) {
+#pragma unroll
+            for (int u = 0; u < 2; u++) out[u] = table[min((base + 16 * u) >> a.shift, top)];
+        };
+        auto load = [&](int base, const int* pid) {
+#pragma unroll
+            for (int u = 0; u < 2; u++) {
+                const int key = base + 16 * u + col;
+                const bool in = (unsigned)pid[u] < (unsigned)a.p.n_pages;
+                const size_t off = (size_t)(in ? pid[u] : 0) * a.p.page_stride +
+                                   (size_t)(key & (a.p.page_size - 1)) * a.p.row_stride;
+#pragma unroll
+                for (int c = 0; c < NC; c++) kf[u][c] = *(const u32x4*)(kp + off + 32 * c);
+#pragma unroll
+                for (int c = 0; c < NC; c++) vf[u][c] = *(const u32x4*)(vp + off + 32 * c);
+            }
+        };
+
+        int base = k0 + 32 * wave;
+        if (base < kend) {
+            pages(base, pg);
+            load(base, pg);
+            pages(base + 128, pn);
         }
-        // keys 16 u + 4 g4 + i of the tile
-        if (!whole) {
+        for (; base < kend; base += 128) {
+            // V goes to LDS for the transposing reads; the wave's own LDS
+            // operations are in order, so nothing but the compiler has to be held
+            const bool whole = base + 32 <= min(kend, first_limit + 1) && (unsigned)pg[0] < (unsigned)a.p.n_pages &&
+                               (unsigned)pg[1] < (unsigned)a.p.n_pages;
+            if (!whole) {
+                // a V row that no row of the tile sees may hold anything: 0 * inf
+                // and 0 * NaN would reach the sums
+#pragma unroll
+                for (int u = 0; u < 2; u++)
+                    if (base + 16 * u + col >= kend || (unsigned)pg[u] >= (unsigned)a.p.n_pages)
+#pragma unroll
+                        for (int c = 0; c < NC; c++) vf[u][c] = u32x4{0, 0, 0, 0};
+            }
+            lds_order();
 #pragma unroll
             for (int u = 0; u < 2; u++)
 #pragma unroll
-                for (int i = 0; i < 4; i++)
-                    if (!ok[u] || here + 16 * u + 4 * g4 + i > limit) sc[u][i] = NEG_INF;
-        }
-        float mt = fmaxf(fmaxf(fmaxf(sc[0][0], sc[0][1]), fmaxf(sc[0][2], sc[0][3])),
-                         fmaxf(fmaxf(sc[1][0], sc[1][1]), fmaxf(sc[1][2], sc[1][3])));
-        mt = max_xor32(max_xor16(mt)) * a.c2;
-        // m follows the maximum only when it is behind by more than 2^SLACK
-        if (__any(mt > m + SLACK)) {
-            const float mn = fmaxf(m, mt), f = __builtin_amdgcn_exp2f(m - (mn == NEG_INF ? 0.0f : mn));
-            l *= f;
+                for (int c = 0; c < NC; c++) *(u32x4*)(lv + (16 * u + col) * PITCH + 32 * c + 8 * g4) = vf[u][c];
+            f32x4 sc[2] = {f32x4{0.f, 0.f, 0.f, 0.f}, f32x4{0.f, 0.f, 0.f, 0.f}};
 #pragma unroll
-            for (int d = 0; d < ND; d++) o[d] *= f;
-            m = mn;
-        }
-        const float ms = m == NEG_INF ? 0.0f : m;
-        float pr[8];
+            for (int c = 0; c < NC; c++)
 #pragma unroll
-        for (int u = 0; u < 2; u++)
-#pragma unroll
-            for (int i = 0; i < 4; i++) {
-                pr[4 * u + i] = __builtin_amdgcn_exp2f(fmaf(sc[u][i], a.c2, -ms));
-                l += pr[4 * u + i];
+                for (int u = 0; u < 2; u++) sc[u] = T::mma16(vec_of<v8>(kf[u][c]), qf[c], sc[u]);
+            const int here = base;
+            const bool ok[2] = {(unsigned)pg[0] < (unsigned)a.p.n_pages, (unsigned)pg[1] < (unsigned)a.p.n_pages};
+            if (base + 128 < kend) {
+                pg[0] = pn[0];
+                pg[1] = pn[1];
+                load(base + 128, pg);
+                pages(base + 256, pn);
             }
-        const u32x4 pw = {pack2<T>(pr[0], pr[1]), pack2<T>(pr[2], pr[3]), pack2<T>(pr[4], pr[5]),
-                          pack2<T>(pr[6], pr[7])};
-        const v8 pf = vec_of<v8>(pw);
-        lds_order();
-        const uint16_t* tr = lv + (4 * g4 + (col >> 2)) * PITCH + 4 * (col & 3);
+            // keys 16 u + 4 g4 + i of the tile
+            if (!whole) {
 #pragma unroll
-        for (int d = 0; d < ND; d++) {
-            const s16x4 lo = lds_tr4(tr + 16 * d), hi = lds_tr4(tr + 16 * PITCH + 16 * d);
-            const uint2 a0 = __builtin_bit_cast(uint2, lo), a1 = __builtin_bit_cast(uint2, hi);
-            o[d] = T::mma16(vec_of<v8>(u32x4{a0.x, a0.y, a1.x, a1.y}), pf, o[d]);
+                for (int u = 0; u < 2; u++)
+#pragma unroll
+                    for (int i = 0; i < 4; i++)
+                        if (!ok[u] || here + 16 * u + 4 * g4 + i > limit) sc[u][i] = NEG_INF;
+            }
+            float mt = fmaxf(fmaxf(fmaxf(sc[0][0], sc[0][1]), fmaxf(sc[0][2], sc[0][3])),
+                             fmaxf(fmaxf(sc[1][0], sc[1][1]), fmaxf(sc[1][2], sc[1][3])));
+            mt = max_xor32(max_xor16(mt)) * a.c2;
+            // m follows the maximum only when it is behind by more than 2^SLACK
+            if (__any(mt > m + SLACK)) {
+                const float mn = fmaxf(m, mt), f = __builtin_amdgcn_exp2f(m - (mn == NEG_INF ? 0.0f : mn));
+                l *= f;
+#pragma unroll
+                for (int d = 0; d < ND; d++) o[d] *= f;
+                m = mn;
+            }
+            const float ms = m == NEG_INF ? 0.0f : m;
+            float pr[8];
+#pragma unroll
+            for (int u = 0; u < 2; u++)
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    pr[4 * u + i] = __builtin_amdgcn_exp2f(fmaf(sc[u][i], a.c2, -ms));
+                    l += pr[4 * u + i];
+                }
+            const u32x4 pw = {pack2<T>(pr[0], pr[1]), pack2<T>(pr[2], pr[3]), pack2<T>(pr[4], pr[5]),
+                              pack2<T>(pr[6], pr[7])};
+            const v8 pf = vec_of<v8>(pw);
+            lds_order();
+            const uint16_t* tr = lv + (4 * g4 + (col >> 2)) * PITCH + 4 * (col & 3);
+#pragma unroll
+            for (int d = 0; d < ND; d++) {
+                const s16x4 lo = lds_tr4(tr + 16 * d), hi = lds_tr4(tr + 16 * PITCH + 16 * d);
+                const uint2 a0 = __builtin_bit_cast(uint2, lo), a1 = __builtin_bit_cast(uint2, hi);
+                o[d] = T::mma16(vec_of<v8>(u32x4{a0.x, a0.y, a1.x, a1.y}), pf, o[d]);
+            }
         }
-    }
 
-    // join the four waves: m, l of the 16 rows, then O by output column
-    l = add_xor32(add_xor16(l));
-    __shared__ float2 ml[4][16];
-    if (lane < 16) ml[wave][lane] = make_float2(m, l);
-    __syncthreads();
-    float M = NEG_INF, L = 0.0f;
-#pragma unroll
-    for (int w = 0; w < 4; w++) M = fmaxf(M, ml[w][col].x);
-    const float Ms = M == NEG_INF ? 0.0f : M;
-#pragma unroll
-    for (int w = 0; w < 4; w++) L += ml[w][col].y * __builtin_amdgcn_exp2f(ml[w][col].x - Ms);
-    const float f = __builtin_amdgcn_exp2f(m - Ms);
-    // [wave][16 rows][HD + 4] floats over the V tiles, a half of the columns
-    // at a time (16 * (HD / 2 + 4) floats fit a wave's 32 * (HD + 16) halves)
-    constexpr int OP = HD / 2 + 4;
-    float* lo = (float*)lds[0];
-    constexpr int WS = 32 * PITCH / 2;   // floats of a wave's region
-#pragma unroll
-    for (int hf = 0; hf < 2; hf++) {
-#pragma unroll
-        for (int d = 0; d < ND / 2; d++) {
-            const f32x4 v = o[hf * (ND / 2) + d] * f;
-            *(f32x4*)(lo + wave * WS + col * OP + 16 * d + 4 * g4) = v;
-        }
+        // join the four waves: m, l of the 16 rows, then O by output column
+        l = add_xor32(add_xor16(l));
+        if (lane < 16) sh.ml[wave][lane] = make_float2(m, l);
         __syncthreads();
-        for (int e = threadIdx.x; e < 16 * (HD / 8); e += 256) {
-            const int rr = e / (HD / 8), d4 = 4 * (e - rr * (HD / 8));
-            const int pr = 16 * tile + rr;
-            if (pr < rows) {
-                f32x4 v = *(const f32x4*)(lo + rr * OP + d4);
+        float M = NEG_INF, L = 0.0f;
 #pragma unroll
-                for (int w = 1; w < 4; w++) v += *(const f32x4*)(lo + w * WS + rr * OP + d4);
-                const int i = pr / a.G;
-                const size_t orow = (size_t)(sq.r0 + i) * a.nq + kvh * a.G + (pr - i * a.G);
-                const int d = hf * (HD / 2) + d4;
-                if (ranges > 1) {
-                    *(f32x4*)(a.few_o + few_at(a, z, s, kvh, pr) * HD + d) = v;
-                } else {
-                    float Lr = 0.0f, Mr = NEG_INF;
+        for (int w = 0; w < 4; w++) M = fmaxf(M, sh.ml[w][col].x);
+        const float Ms = M == NEG_INF ? 0.0f : M;
 #pragma unroll
-                    for (int w = 0; w < 4; w++) Mr = fmaxf(Mr, ml[w][rr].x);
-                    const float Mz = Mr == NEG_INF ? 0.0f : Mr;
+        for (int w = 0; w < 4; w++) L += sh.ml[w][col].y * __builtin_amdgcn_exp2f(sh.ml[w][col].x - Ms);
+        const float f = __builtin_amdgcn_exp2f(m - Ms);
+        // [wave][16 rows][HD + 4] floats over the V tiles, a half of the columns
+        // at a time (16 * (HD / 2 + 4) floats fit a wave's 32 * (HD + 16) halves)
+        constexpr int OP = HD / 2 + 4;
+        float* lo = (float*)sh.v[0];
+        constexpr int WS = 32 * PITCH / 2;   // floats of a wave's region
 #pragma unroll
-                    for (int w = 0; w < 4; w++) Lr += ml[w][rr].y * __builtin_amdgcn_exp2f(ml[w][rr].x - Mz);
-                    const float ov[4] = {v[0], v[1], v[2], v[3]};
-                    put4<T>(a, orow * HD + d, ov, Lr > 0.0f ? 1.0f / Lr : Lr == 0.0f ? 0.0f : Lr);
+        for (int hf = 0; hf < 2; hf++) {
+#pragma unroll
+            for (int d = 0; d < ND / 2; d++) {
+                const f32x4 v = o[hf * (ND / 2) + d] * f;
+                *(f32x4*)(lo + wave * WS + col * OP + 16 * d + 4 * g4) = v;
+            }
+            __syncthreads();
+            for (int e = threadIdx.x; e < 16 * (HD / 8); e += 256) {
+                const int rr = e / (HD / 8), d4 = 4 * (e - rr * (HD / 8));
+                const int pr = 16 * tile + rr;
+                if (pr < rows) {
+                    f32x4 v = *(const f32x4*)(lo + rr * OP + d4);
+#pragma unroll
+                    for (int w = 1; w < 4; w++) v += *(const f32x4*)(lo + w * WS + rr * OP + d4);
+                    const int i = pr / a.G;
+                    const size_t orow = (size_t)(sq.r0 + i) * a.nq + kvh * a.G + (pr - i * a.G);
+                    const int d = hf * (HD / 2) + d4;
+                    if (ranges > 1) {
+                        *(f32x4*)(a.few_o + few_at(a, z, s, kvh, pr, orow) * HD + d) = v;
+                    } else {
+                        float Lr = 0.0f, Mr = NEG_INF;
+#pragma unroll
+                        for (int w = 0; w < 4; w++) Mr = fmaxf(Mr, sh.ml[w][rr].x);
+                        const float Mz = Mr == NEG_INF ? 0.0f : Mr;
+#pragma unroll
+                        for (int w = 0; w < 4; w++) Lr += sh.ml[w][rr].y * __builtin_amdgcn_exp2f(sh.ml[w][rr].x - Mz);
+                        const float ov[4] = {v[0], v[1], v[2], v[3]};
+                        put4<T>(a, orow * HD + d, ov, Lr > 0.0f ? 1.0f / Lr : Lr == 0.0f ? 0.0f : Lr);
+                    }
                 }
             }
+            __syncthreads();
         }
-        __syncthreads();
-    }
-    if (threadIdx.x < 16 && live) {
-        if (ranges > 1) a.few_ml[few_at(a, z, s, kvh, r)] = make_float2(M, L);
-        else if (a.lse) a.lse[row] = lse_of(M, L);
+        if (threadIdx.x < 16 && live) {
+            if (ranges > 1) a.few_ml[few_at(a, z, s, kvh, r, row)] = make_float2(M, L);
+            else if (a.lse) a.lse[row] = lse_of(M, L);
+        }
     }
 }
 
@@ -301,32 +310,36 @@ __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void k_pa_few(PaArgs a) {
 // two of them: while one is computed, the other takes the tile after it from
 // registers, whose loads were issued a tile earlier.
 // ---------------------------------------------------------------------------
-template <typename T, int HD>
-__global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void k_pa_many(PaArgs a) {
-    constexpr int KT = HD == 256 ? 32 : 64;
+template <int HD> struct ManyLds {
+    static constexpr int KT = HD == 256 ? 32 : 64;
+    static constexpr int KP = HD + 8;    // K row: 16 rows' 16 bytes in distinct banks
+    static constexpr int VP = HD + 32;   // V row: 4 rows' 64 bytes in distinct banks
+    uint16_t k[2][KT * KP];
+    uint16_t v[2][KT * VP];
+};
+
+template <typename T, int HD> DEV void many_rows(const PaArgs& a, ManyLds<HD>& sh, int kvh, int tile, int z) {
+    constexpr int KT = ManyLds<HD>::KT, KP = ManyLds<HD>::KP, VP = ManyLds<HD>::VP;
     constexpr int NC = HD / 16;          // 16-column steps of a key
     constexpr int ND = HD / 32;          // 32-column tiles of the output
-    constexpr int KP = HD + 8;           // K row in LDS: 16 rows' 16 bytes in distinct banks
-    constexpr int VP = HD + 32;          // V row: 4 rows' 64 bytes in distinct banks
     constexpr int CH = HD / 8;           // 16-byte pieces of a row
     constexpr int RP = 256 / CH;         // rows a pass of the workgroup loads
     constexpr int NP = KT / RP;
     constexpr int NB = KT / 32;          // 32-key blocks of a tile
     typedef typename T::v8 v8;
-    __shared__ __align__(16) uint16_t lk[2][KT * KP];
-    __shared__ __align__(16) uint16_t lv[2][KT * VP];
+    uint16_t (*lk)[KT * KP] = sh.k;
+    uint16_t (*lv)[KT * VP] = sh.v;
 
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int col = lane & 31, h = lane >> 5;
-    const int kvh = blockIdx.x;
-    // sequence and tile of blockIdx.y among the sequences with many rows
-    int s = -1, tile = blockIdx.y;
+    // sequence of the tile, and its tile there, among the sequences with many rows
+    int s = -1;
     for (int s0 = 0; s0 < a.b.n_seqs && s < 0; s0 += 64) {
         int n = 0;
         if (s0 + lane < a.b.n_seqs) {
             const PgSeq t = pg_seq(a.b, a.shift, s0 + lane);
             const int rows = t.n * a.G;
-            n = rows > a.few ? (rows + 127) >> 7 : 0;
+            n = rows > a.few || a.only == PA_MANY ? (rows + 127) >> 7 : 0;
         }
         int sum = n;
         for (int d = 1; d < 64; d <<= 1) {
@@ -349,7 +362,6 @@ __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void k_pa_many(PaArgs a) {
     const int rows = sq.n * a.G;
     const int per = range_keys(sq.ctx, a.chunk_many, a.nz_many);
     const int ranges = sq.ctx > per ? (sq.ctx + per - 1) / per : 1;
-    const int z = blockIdx.z;
     if (z >= ranges) return;
 
     const int r = 128 * tile + 32 * wave + col;
@@ -530,55 +542,98 @@ __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void k_pa_many(PaArgs a) {
     }
 }
 
-// Joins the key ranges of rows that were split: one wave per (row, head).
+// Blocks of the three kernels: kv heads fastest, so that the workgroups that
+// read the same keys run on the same XCDs (8 kv heads: one XCD each) and share
+// their L2.
+template <typename T, int HD> __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void k_pa_few(PaArgs a) {
+    __shared__ __align__(16) FewLds<HD> sh;
+    few_rows<T, HD>(a, sh, blockIdx.x, blockIdx.y, blockIdx.z);
+}
+template <typename T, int HD> __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void k_pa_many(PaArgs a) {
+    __shared__ __align__(16) ManyLds<HD> sh;
+    many_rows<T, HD>(a, sh, blockIdx.x, blockIdx.y, blockIdx.z);
+}
+// Chunks and decoding sequences in one call: the chunks' workgroups, which are
+// bound by arithmetic, first, and beside them those that are bound by memory.
+template <typename T, int HD>
+__global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void k_pa_mixed(PaArgs a, int y_many, int y_few) {
+    __shared__ __align__(16) char raw[sizeof(ManyLds<HD>) > sizeof(FewLds<HD>) ? sizeof(ManyLds<HD>)
+                                                                               : sizeof(FewLds<HD>)];
+    const int nkv = a.p.n_kv_heads, many = nkv * y_many * a.nz_many;
+    int b = blockIdx.x;
+    if (b < many) {
+        const int kvh = b % nkv;
+        b /= nkv;
+        many_rows<T, HD>(a, *(ManyLds<HD>*)raw, kvh, b % y_many, b / y_many);
+    } else {
+        b -= many;
+        const int kvh = b % nkv;
+        b /= nkv;
+        few_rows<T, HD>(a, *(FewLds<HD>*)raw, kvh, b % y_few, b / y_few);
+    }
+}
+
+// Joins the key ranges of rows that were split: HD / 4 lanes a (row, head),
+// four ranges' partials in flight.
 template <typename T, int HD>
 __global__ __launch_bounds__(256) void k_pa_join(PaArgs a) {
-    const int lane = threadIdx.x & 63;
-    const int64_t at = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-    const int64_t total = (int64_t)a.b.n_rows * a.nq;
-    if (at >= total) return;
-    const int s = pg_seq_of_row(a.b, (int)(at / a.nq), lane);
+    constexpr int LPR = HD / 4, PER = 256 / LPR;
+    const int lane = threadIdx.x & 63, row = blockIdx.x;
+    const int head = blockIdx.y * PER + threadIdx.x / LPR, d = 4 * (threadIdx.x % LPR);
+    const int s = pg_seq_of_row(a.b, row, lane);
     if (s < 0) return;
     const PgSeq sq = pg_seq(a.b, a.shift, s);
-    const bool few = sq.n * a.G <= a.few;
+    const bool few = a.only == PA_FEW || (a.only == PA_BOTH && sq.n * a.G <= a.few);
     const int per = range_keys(sq.ctx, few ? a.chunk_few : a.chunk_many, few ? a.nz_few : a.nz_many);
     const int ranges = sq.ctx > per ? (sq.ctx + per - 1) / per : 1;
-    if (ranges == 1) return;
-    constexpr int E = HD / 64;
-    const int row = (int)(at / a.nq), head = (int)(at - (int64_t)row * a.nq), kvh = head / a.G;
-    const size_t first = few ? few_at(a, 0, s, kvh, (row - sq.r0) * a.G + head - kvh * a.G) : (size_t)at;
-    const size_t step = few ? (size_t)a.b.n_seqs * a.p.n_kv_heads * a.few : (size_t)total;
-    const float2* mls = few ? a.few_ml : a.many_ml;
-    const float* os = few ? a.few_o : a.many_o;
-    float M = NEG_INF;
-    for (int z = 0; z < ranges; z++) M = fmaxf(M, mls[z * step + first].x);
-    const float Ms = M == NEG_INF ? 0.0f : M;
-    float L = 0.0f, o[E] = {};
-    for (int z = 0; z < ranges; z++) {
-        const float2 ml = mls[z * step + first];
-        const float f = __builtin_amdgcn_exp2f(ml.x - Ms);
-        L = fmaf(ml.y, f, L);
-        const float* po = os + (z * step + first) * HD + lane * E;
+    if (ranges == 1 || row >= sq.r0 + sq.n || head >= a.nq) return;
+    const int kvh = head / a.G;
+    const size_t at = (size_t)row * a.nq + head, total = (size_t)a.b.n_rows * a.nq;
+    const size_t first = few ? few_at(a, 0, s, kvh, (row - sq.r0) * a.G + head - kvh * a.G, at) : at;
+    const size_t step = few && a.only == PA_BOTH ? (size_t)a.b.n_seqs * a.p.n_kv_heads * a.few : total;
+    const float2* mls = (few ? a.few_ml : a.many_ml) + first;
+    const float* os = (few ? a.few_o : a.many_o) + first * HD + d;
+    float M = NEG_INF, L = 0.0f;
+    f32x4 o = {0.f, 0.f, 0.f, 0.f};
+    for (int z0 = 0; z0 < ranges; z0 += 4) {
+        float2 ml[4];
+        f32x4 po[4];
 #pragma unroll
-        for (int e = 0; e < E; e++) o[e] = fmaf(po[e], f, o[e]);
+        for (int e = 0; e < 4; e++) {
+            const size_t z = min(z0 + e, ranges - 1) * step;
+            ml[e] = mls[z];
+            po[e] = *(const f32x4*)(os + z * HD);
+        }
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            if (z0 + e >= ranges) break;
+            const float mn = fmaxf(M, ml[e].x), ms = mn == NEG_INF ? 0.0f : mn;
+            const float f0 = __builtin_amdgcn_exp2f(M - ms), f1 = __builtin_amdgcn_exp2f(ml[e].x - ms);
+            L = L * f0 + ml[e].y * f1;
+            o = o * f0 + po[e] * f1;
+            M = mn;
+        }
     }
     const float inv = L > 0.0f ? 1.0f / L : L == 0.0f ? 0.0f : L;
-#pragma unroll
-    for (int e = 0; e < E; e++) {
-        const size_t i = (size_t)at * HD + lane * E + e;
-        if (a.out_f32) ((float*)a.out)[i] = o[e] * inv;
-        else ((typename T::e*)a.out)[i] = (typename T::e)(o[e] * inv);
-    }
-    if (lane == 0 && a.lse) a.lse[at] = lse_of(M, L);
+    const float ov[4] = {o[0], o[1], o[2], o[3]};
+    put4<T>(a, at * HD + d, ov, inv);
+    if (d == 0 && a.lse) a.lse[at] = lse_of(M, L);
 }
 
 struct PaPlan {
-    int few, nz_few, nz_many, chunk_few, chunk_many, y_few, y_many;
+    int only, few, nz_few, nz_many, chunk_few, chunk_many, y_few, y_many;
     size_t few_rows, many_rows;   // partial sums in the workspace
 };
 
 int ceil_div(int64_t a, int64_t b) { return (int)((a + b - 1) / b); }
 
+// Which kernel takes which sequences.  Row counts are on the device; what the
+// host knows is their sum and the number of sequences.  No more rows than
+// sequences: a decode step (a sequence that has several rows all the same has
+// its tiles done in turn), the few-row kernel alone.  One sequence with more
+// than a tile of rows: the many-row kernel alone.  Otherwise each sequence by
+// its own count: up to `few` packed rows (a tile of 16; two where a single
+// row has more than 16 query heads per kv head) or more.
 PaPlan plan(const DpufAmdBatch& b, const DpufAmdPages& p, int nq) {
     const int G = nq / p.n_kv_heads;
     PaPlan r;
@@ -586,9 +641,11 @@ PaPlan plan(const DpufAmdBatch& b, const DpufAmdPages& p, int nq) {
     const int64_t cap = (int64_t)b.table_stride * p.page_size;
     const int64_t ctx = b.max_ctx < 1 ? 1 : b.max_ctx < cap ? b.max_ctx : cap;
     const int64_t packed = (int64_t)b.n_rows * G;
-    r.y_few = b.n_seqs * ((r.few + 15) / 16);
+    r.only = b.n_rows <= b.n_seqs || packed <= r.few ? PA_FEW : b.n_seqs == 1 ? PA_MANY : PA_BOTH;
     const int64_t most = packed / (r.few + 1);
-    r.y_many = (int)(packed <= r.few ? 0 : packed / 128 + (most < b.n_seqs ? most : b.n_seqs));
+    r.y_few = r.only == PA_MANY ? 0 : b.n_seqs * ((r.few + 15) / 16);
+    r.y_many = r.only == PA_FEW ? 0 : (int)(packed / 128 + (most < b.n_seqs ? most : b.n_seqs));
+    if (r.only == PA_MANY) r.y_many = ceil_div(packed, 128);
     r.chunk_few = 512;
     r.nz_few = ceil_div(ctx, r.chunk_few);
     // (kv heads x sequences) that fill the card by themselves need no ranges,
@@ -602,19 +659,24 @@ PaPlan plan(const DpufAmdBatch& b, const DpufAmdPages& p, int nq) {
     if (r.chunk_many < 512) r.chunk_many = 512;
     r.chunk_many = (r.chunk_many + 127) & ~127;
     r.nz_many = ceil_div(ctx, r.chunk_many);
-    r.few_rows = r.nz_few > 1 ? (size_t)r.nz_few * b.n_seqs * p.n_kv_heads * r.few : 0;
-    r.many_rows = r.y_many > 0 && r.nz_many > 1 ? (size_t)r.nz_many * b.n_rows * nq : 0;
+    const size_t all = (size_t)b.n_rows * nq, some = (size_t)b.n_seqs * p.n_kv_heads * r.few;
+    r.few_rows = r.only != PA_MANY && r.nz_few > 1 ? r.nz_few * (r.only == PA_FEW ? all : some) : 0;
+    r.many_rows = r.only != PA_FEW && r.nz_many > 1 ? r.nz_many * all : 0;
     return r;
 }
 
 template <typename T, int HD>
 void launch(const PaArgs& a, const PaPlan& pl, hipStream_t st) {
     const int nkv = a.p.n_kv_heads;
-    hipLaunchKernelGGL((k_pa_few<T, HD>), dim3(nkv, pl.y_few, pl.nz_few), dim3(256), 0, st, a);
-    if (pl.y_many > 0)
+    if (pl.only == PA_FEW)
+        hipLaunchKernelGGL((k_pa_few<T, HD>), dim3(nkv, pl.y_few, pl.nz_few), dim3(256), 0, st, a);
+    else if (pl.only == PA_MANY)
         hipLaunchKernelGGL((k_pa_many<T, HD>), dim3(nkv, pl.y_many, pl.nz_many), dim3(256), 0, st, a);
-    if (pl.nz_few > 1 || (pl.y_many > 0 && pl.nz_many > 1))
-        hipLaunchKernelGGL((k_pa_join<T, HD>), dim3(ceil_div((int64_t)a.b.n_rows * a.nq, 4)), dim3(256), 0, st, a);
+    else
+        hipLaunchKernelGGL((k_pa_mixed<T, HD>), dim3(nkv * (pl.y_many * pl.nz_many + pl.y_few * pl.nz_few)), dim3(256),
+                           0, st, a, pl.y_many, pl.y_few);
+    if (pl.few_rows + pl.many_rows > 0)
+        hipLaunchKernelGGL((k_pa_join<T, HD>), dim3(a.b.n_rows, ceil_div(a.nq, 256 / (HD / 4))), dim3(256), 0, st, a);
     LAUNCHED("k_pa");
 }
 
@@ -639,6 +701,7 @@ void dpuf_hip_paged_attn(void* s, const DpufAmdBatch* b, const DpufAmdPages* p, 
     a.q = (const uint16_t*)q;
     a.c2 = scale * 1.4426950408889634f;
     a.few = pl.few;
+    a.only = pl.only;
     a.nz_few = pl.nz_few;
     a.nz_many = pl.nz_many;
     a.chunk_few = pl.chunk_few;

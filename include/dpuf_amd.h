@@ -185,7 +185,7 @@ typedef struct {
     int32_t type;         /* DPUF_AMD_BF16 or DPUF_AMD_F16 */
     int32_t n_pages;
     int32_t page_size;    /* rows: a power of two, 16 to 1024 */
-    int32_t n_kv_heads;
+    int32_t n_kv_heads;   /* 1 to 256 */
     int32_t head_dim;     /* 64, 128 or 256 */
     int64_t page_stride;
     int64_t head_stride;
