@@ -145,11 +145,14 @@ __global__ __launch_bounds__(256) void k_rope_append(RaArgs a) {
 
 // ---------------------------------------------------------------------------
 // Attention weights of cached rows: w' = decay w + sum over packed rows of
-// exp(scale q.k - lse).  The keys stay: a wave holds 32 of them as the left
-// operand of S^T = K Q^T and walks the sequence's rows, 32 at a time, adding
-// the exponentials of its keys in registers; the 32 rows of a step are the
-// lanes, added up once at the end in one order.  A decode step reads K once;
-// a chunk is bound by the matrix instructions and the exponentials.
+// exp(scale q.k - lse).  The keys stay: a wave holds KB x 32 of them as the
+// left operand of S^T = K Q^T and walks the sequence's rows, 32 at a time,
+// adding the exponentials of its keys in registers; the 32 rows of a step are
+// the lanes, added up once at the end in one order.  A workgroup is KG x RG
+// waves: KG of them hold different keys and read the same rows (from the L1),
+// RG share keys and take every RG-th step, their sums joined in LDS in one
+// order.  A decode step (RG 1) reads K once; a chunk (RG 4) reads its queries
+// once per KB x KG x 32 keys, which bounds it together with the exponentials.
 // ---------------------------------------------------------------------------
 struct PwArgs {
     DpufAmdBatch b;
@@ -162,67 +165,130 @@ struct PwArgs {
     const float* w_in;
 };
 
-template <typename T, int HD>
-__global__ __launch_bounds__(256) void k_pa_weights(PwArgs a) {
-    constexpr int NC = HD / 16;
+// Sum over the 16 lanes of a row, in all of them.
+DEV float row_sum(float v) {
+#define ROW_ROR(n) v += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x120 + n, 0xF, 0xF, false))
+    ROW_ROR(8);
+    ROW_ROR(4);
+    ROW_ROR(2);
+    ROW_ROR(1);
+#undef ROW_ROR
+    return v;
+}
+
+template <typename T, int HD, int KB, int KG, int RG>
+__global__ __launch_bounds__(64 * KG * RG) void k_pa_weights(PwArgs a) {
+    constexpr int NC = HD / 16, KEYS = 32 * KB * KG;
     typedef typename T::v8 v8;
+    __shared__ float part[RG > 1 ? RG - 1 : 1][KEYS];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int col = lane & 31, h = lane >> 5;
+    const int col = lane & 31, h = lane >> 5, kg = wave % KG, rg = wave / KG;
     const int kvh = blockIdx.x, s = blockIdx.y;
     const PgSeq sq = pg_seq(a.b, a.shift, s);
     const int rows = sq.n * a.G;
-    for (int base = 128 * blockIdx.z + 32 * wave; base < sq.ctx; base += 128 * gridDim.z) {
-        const int key = min(base + col, sq.ctx - 1);
-        const int page = pg_page(a.b, a.shift, s, key);
-        const bool in = (unsigned)page < (unsigned)a.p.n_pages;
-        const uint16_t* kp = (const uint16_t*)a.p.k + (size_t)(in ? page : 0) * a.p.page_stride +
-                             (size_t)kvh * a.p.head_stride + (size_t)(key & (a.p.page_size - 1)) * a.p.row_stride + 8 * h;
-        v8 kf[NC];
+    const float NEG_INF = -__builtin_huge_valf();
+    for (int base0 = KEYS * blockIdx.z; base0 < sq.ctx; base0 += KEYS * gridDim.z) {
+        const int base = base0 + 32 * KB * kg;
+        v8 kf[KB][NC];
 #pragma unroll
-        for (int c = 0; c < NC; c++) kf[c] = vec_of<v8>(*(const u32x4*)(kp + 16 * c));
-        float acc[16] = {};
+        for (int b = 0; b < KB; b++) {
+            const int key = min(base + 32 * b + col, sq.ctx - 1);
+            const int page = pg_page(a.b, a.shift, s, key);
+            const bool in = (unsigned)page < (unsigned)a.p.n_pages;
+            const uint16_t* kp = (const uint16_t*)a.p.k + (size_t)(in ? page : 0) * a.p.page_stride +
+                                 (size_t)kvh * a.p.head_stride +
+                                 (size_t)(key & (a.p.page_size - 1)) * a.p.row_stride + 8 * h;
+#pragma unroll
+            for (int c = 0; c < NC; c++) kf[b][c] = vec_of<v8>(*(const u32x4*)(kp + 16 * c));
+        }
+        float acc[KB][16] = {};
         // rows before the first key of the tile see none of it
         const int i0 = max(0, base - (sq.ctx - sq.n));
-        for (int r0 = i0 * a.G & ~31; r0 < rows; r0 += 32) {
+        const int first = (i0 * a.G & ~31) + 32 * rg;
+        u32x4 qn[NC];
+        float ln = 0.0f;
+        int qi = 0;
+        bool live = false;
+        // the next step's queries and lse, while the current one is worked out
+        auto fetch = [&](int r0) {
             const int r = r0 + col;
-            const bool live = r < rows;
-            const int qi = live ? r / a.G : 0;
+            live = r < rows;
+            qi = live ? r / a.G : 0;
             const size_t row = (size_t)(sq.r0 + qi) * a.nq + kvh * a.G + (live ? r - qi * a.G : 0);
-            const float ls = live ? a.lse[row] : 0.0f;
-            // rows that saw no key (lse -infinity) give nothing
-            const int limit = live && ls != -__builtin_huge_valf() ? sq.ctx - sq.n + qi : -1;
-            const float l2 = ls * 1.4426950408889634f;
-            f32x16 sc;
+            ln = live ? a.lse[row] : NEG_INF;
 #pragma unroll
-            for (int i = 0; i < 16; i++) sc[i] = 0.0f;
+            for (int c = 0; c < NC; c++)
+                qn[c] = live ? *(const u32x4*)(a.q + row * HD + 16 * c + 8 * h) : u32x4{0, 0, 0, 0};
+        };
+        if (first < rows) fetch(first);
+        for (int r0 = first; r0 < rows; r0 += 32 * RG) {
+            v8 qf[NC];
 #pragma unroll
-            for (int c = 0; c < NC; c++) {
-                const u32x4 qv = *(const u32x4*)(a.q + row * HD + 16 * c + 8 * h);
-                sc = T::mma32(kf[c], vec_of<v8>(qv), sc);
+            for (int c = 0; c < NC; c++) qf[c] = vec_of<v8>(qn[c]);
+            // a row that saw no key (lse -infinity) or is none gives nothing
+            const float l2 = ln == NEG_INF ? -NEG_INF : ln * 1.4426950408889634f;
+            const int limit = live && ln != NEG_INF ? sq.ctx - sq.n + qi : -1;
+            if (r0 + 32 * RG < rows) fetch(r0 + 32 * RG);
+            f32x16 sc[KB];
+            const f32x16 zero = {};
+#pragma unroll
+            for (int c = 0; c < NC; c++)
+#pragma unroll
+                for (int b = 0; b < KB; b++) sc[b] = T::mma32(kf[b][c], qf[c], c ? sc[b] : zero);
+            // keys that the step's first row does not see: row by row
+            if (base + 32 * KB - 1 > sq.ctx - sq.n + r0 / a.G) {
+#pragma unroll
+                for (int b = 0; b < KB; b++)
+#pragma unroll
+                    for (int i = 0; i < 16; i++)
+                        if (base + 32 * b + 8 * (i >> 2) + 4 * h + (i & 3) > limit) sc[b][i] = NEG_INF;
             }
 #pragma unroll
-            for (int i = 0; i < 16; i++) {
-                const int kk = base + 8 * (i >> 2) + 4 * h + (i & 3);
-                const float e = __builtin_amdgcn_exp2f(fmaf(sc[i], a.c2, -l2));
-                acc[i] += kk <= limit ? e : 0.0f;
+            for (int b = 0; b < KB; b++)
+#pragma unroll
+                for (int i = 0; i < 16; i++) acc[b][i] += __builtin_amdgcn_exp2f(fmaf(sc[b][i], a.c2, -l2));
+        }
+        // over the 32 lanes of each half: entries i and i + 8 of the lower and
+        // the upper 16 lanes are exchanged, so each 16 add up 8 entries of all
+        // 32; lane i of the lower 16 then keeps entry i, of the upper 8 + i
+        float mine[KB];
+#pragma unroll
+        for (int b = 0; b < KB; b++) {
+            mine[b] = 0.0f;
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                const auto x = __builtin_amdgcn_permlane16_swap(__float_as_uint(acc[b][i]), __float_as_uint(acc[b][i + 8]),
+                                                                false, false);
+                const float v = row_sum(__uint_as_float(x[0]) + __uint_as_float(x[1]));
+                mine[b] = (lane & 7) == i ? v : mine[b];
             }
         }
-        // over the 32 lanes of each half
+        const int e = (lane & 7) + ((lane & 16) >> 1);                    // entry this lane keeps
+        const int at0 = 8 * (e >> 2) + 4 * h + (e & 3);                    // its key among 32
+        const bool keeps = !(lane & 8);
+        if (RG > 1) {
+            if (rg > 0 && keeps) {
 #pragma unroll
-        for (int i = 0; i < 16; i++) {
+                for (int b = 0; b < KB; b++) part[rg - 1][32 * (KB * kg + b) + at0] = mine[b];
+            }
+            __syncthreads();
+            if (rg == 0 && keeps) {
 #pragma unroll
-            for (int d = 1; d < 32; d <<= 1) acc[i] += __shfl_xor(acc[i], d);
+                for (int g = 0; g < RG - 1; g++)
+#pragma unroll
+                    for (int b = 0; b < KB; b++) mine[b] += part[g][32 * (KB * kg + b) + at0];
+            }
+            __syncthreads();
         }
-        // lane 16 h' + ... : key i of half h is written by lane i of that half
-        float mine = 0.0f;
+        if (rg == 0 && keeps) {
 #pragma unroll
-        for (int i = 0; i < 16; i++) mine = col == i ? acc[i] : mine;
-        const int kk = base + 8 * (col >> 2) + 4 * h + (col & 3);
-        if (col < 16 && kk < sq.ctx) {
-            const int pg = pg_page(a.b, a.shift, s, kk);
-            if ((unsigned)pg < (unsigned)a.p.n_pages) {
+            for (int b = 0; b < KB; b++) {
+                const int kk = base + 32 * b + at0;
+                if (kk >= sq.ctx) continue;
+                const int pg = pg_page(a.b, a.shift, s, kk);
+                if ((unsigned)pg >= (unsigned)a.p.n_pages) continue;
                 const size_t at = ((size_t)pg * a.p.n_kv_heads + kvh) * a.p.page_size + (kk & (a.p.page_size - 1));
-                a.p.w[at] = a.w_in ? fmaf(a.decay, a.w_in[at], mine) : mine;
+                a.p.w[at] = a.w_in ? fmaf(a.decay, a.w_in[at], mine[b]) : mine[b];
             }
         }
     }
@@ -404,6 +470,13 @@ __global__ __launch_bounds__(256) void k_ev_move(EvArgs a) {
     }
 }
 
+template <typename T, int HD> void weights_rg(const PwArgs& a, bool many, int64_t ctx, hipStream_t st) {
+    constexpr int KB = HD == 256 ? 1 : 2;      // 32 KB keys of 256 columns are all the registers hold
+    const int64_t keys = many ? 64 * KB : 128 * KB, z = (ctx + keys - 1) / keys;
+    const dim3 g(a.p.n_kv_heads, a.b.n_seqs, (unsigned)(z < 65535 ? z : 65535));
+    if (many) hipLaunchKernelGGL((k_pa_weights<T, HD, KB, 2, 4>), g, dim3(512), 0, st, a);
+    else hipLaunchKernelGGL((k_pa_weights<T, HD, KB, 4, 1>), g, dim3(256), 0, st, a);
+}
 template <typename TI, bool F32, typename T> void rope_hd(const RaArgs& a, dim3 g, hipStream_t st) {
     switch (a.p.head_dim) {
         case 64: hipLaunchKernelGGL((k_rope_append<TI, F32, T, 64>), g, dim3(256), 0, st, a); break;
@@ -470,21 +543,14 @@ void dpuf_hip_paged_attn_weights(void* s, const DpufAmdBatch* b, const DpufAmdPa
     a.w_in = w_in;
     const int64_t cap = (int64_t)b->table_stride * p->page_size;
     const int64_t ctx = b->max_ctx < 1 ? 1 : b->max_ctx < cap ? b->max_ctx : cap;
-    const int64_t z = (ctx + 127) / 128;
-    const dim3 g(p->n_kv_heads, b->n_seqs, (unsigned)(z < 65535 ? z : 65535));
+    // one sequence's rows are n_rows or fewer: with several steps of 32 the
+    // waves of a workgroup share them
+    const bool many = (int64_t)b->n_rows * a.G > (int64_t)b->n_seqs * 64;
     const bool bf = p->type == DPUF_AMD_BF16;
     switch (p->head_dim) {
-        case 64:
-            if (bf) hipLaunchKernelGGL((k_pa_weights<Bf16, 64>), g, dim3(256), 0, ST(s), a);
-            else hipLaunchKernelGGL((k_pa_weights<Fp16, 64>), g, dim3(256), 0, ST(s), a);
-            break;
-        case 128:
-            if (bf) hipLaunchKernelGGL((k_pa_weights<Bf16, 128>), g, dim3(256), 0, ST(s), a);
-            else hipLaunchKernelGGL((k_pa_weights<Fp16, 128>), g, dim3(256), 0, ST(s), a);
-            break;
-        default:
-            if (bf) hipLaunchKernelGGL((k_pa_weights<Bf16, 256>), g, dim3(256), 0, ST(s), a);
-            else hipLaunchKernelGGL((k_pa_weights<Fp16, 256>), g, dim3(256), 0, ST(s), a);
+        case 64: bf ? weights_rg<Bf16, 64>(a, many, ctx, ST(s)) : weights_rg<Fp16, 64>(a, many, ctx, ST(s)); break;
+        case 128: bf ? weights_rg<Bf16, 128>(a, many, ctx, ST(s)) : weights_rg<Fp16, 128>(a, many, ctx, ST(s)); break;
+        default: bf ? weights_rg<Bf16, 256>(a, many, ctx, ST(s)) : weights_rg<Fp16, 256>(a, many, ctx, ST(s));
     }
     LAUNCHED("k_pa_weights");
 }
