@@ -151,8 +151,8 @@ __global__ __launch_bounds__(256) void k_rope_append(RaArgs a) {
 // the lanes, added up once at the end in one order.  A workgroup is KG x RG
 // waves: KG of them hold different keys and read the same rows (from the L1),
 // RG share keys and take every RG-th step, their sums joined in LDS in one
-// order.  A decode step (RG 1) reads K once; a chunk (RG 4) reads its queries
-// once per KB x KG x 32 keys, which bounds it together with the exponentials.
+// order.  The queries are read once per KB x KG x 32 keys, which bounds it
+// together with the exponentials.
 // ---------------------------------------------------------------------------
 struct PwArgs {
     DpufAmdBatch b;
@@ -180,7 +180,7 @@ template <typename T, int HD, int KB, int KG, int RG>
 __global__ __launch_bounds__(64 * KG * RG) void k_pa_weights(PwArgs a) {
     constexpr int NC = HD / 16, KEYS = 32 * KB * KG;
     typedef typename T::v8 v8;
-    __shared__ float part[RG > 1 ? RG - 1 : 1][KEYS];
+    __shared__ float part[RG - 1][KEYS];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int col = lane & 31, h = lane >> 5, kg = wave % KG, rg = wave / KG;
     const int kvh = blockIdx.x, s = blockIdx.y;
@@ -266,20 +266,18 @@ __global__ __launch_bounds__(64 * KG * RG) void k_pa_weights(PwArgs a) {
         const int e = (lane & 7) + ((lane & 16) >> 1);                    // entry this lane keeps
         const int at0 = 8 * (e >> 2) + 4 * h + (e & 3);                    // its key among 32
         const bool keeps = !(lane & 8);
-        if (RG > 1) {
-            if (rg > 0 && keeps) {
+        if (rg > 0 && keeps) {
 #pragma unroll
-                for (int b = 0; b < KB; b++) part[rg - 1][32 * (KB * kg + b) + at0] = mine[b];
-            }
-            __syncthreads();
-            if (rg == 0 && keeps) {
-#pragma unroll
-                for (int g = 0; g < RG - 1; g++)
-#pragma unroll
-                    for (int b = 0; b < KB; b++) mine[b] += part[g][32 * (KB * kg + b) + at0];
-            }
-            __syncthreads();
+            for (int b = 0; b < KB; b++) part[rg - 1][32 * (KB * kg + b) + at0] = mine[b];
         }
+        __syncthreads();
+        if (rg == 0 && keeps) {
+#pragma unroll
+            for (int g = 0; g < RG - 1; g++)
+#pragma unroll
+                for (int b = 0; b < KB; b++) mine[b] += part[g][32 * (KB * kg + b) + at0];
+        }
+        __syncthreads();
         if (rg == 0 && keeps) {
 #pragma unroll
             for (int b = 0; b < KB; b++) {
@@ -289,6 +287,111 @@ __global__ __launch_bounds__(64 * KG * RG) void k_pa_weights(PwArgs a) {
                 if ((unsigned)pg >= (unsigned)a.p.n_pages) continue;
                 const size_t at = ((size_t)pg * a.p.n_kv_heads + kvh) * a.p.page_size + (kk & (a.p.page_size - 1));
                 a.p.w[at] = a.w_in ? fmaf(a.decay, a.w_in[at], mine[b]) : mine[b];
+            }
+        }
+    }
+}
+
+// The same for few rows: bound by reading K once.  16-key blocks as the left
+// operand of 16 x 16 steps, so that a load of the wave takes 64 consecutive
+// bytes of 16 rows (of 32 rows 32 bytes, as above, it reached 3.8 TB/s); NB
+// blocks a wave, and the next ones in flight.
+template <typename T, int HD>
+__global__ __launch_bounds__(256) void k_pa_weights_few(PwArgs a) {
+    constexpr int NC = HD / 32, NB = HD == 256 ? 2 : 4, WK = 16 * NB;
+    typedef typename T::v8 v8;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int col = lane & 15, g4 = lane >> 4;
+    const int kvh = blockIdx.x, s = blockIdx.y;
+    const PgSeq sq = pg_seq(a.b, a.shift, s);
+    const int rows = sq.n * a.G;
+    const float NEG_INF = -__builtin_huge_valf();
+    const uint16_t* kp = (const uint16_t*)a.p.k + (size_t)kvh * a.p.head_stride + 8 * g4;
+    const int* table = a.b.page_table + (size_t)s * a.b.table_stride;
+    const int step = 4 * WK * gridDim.z, top = sq.ctx > 0 ? (sq.ctx - 1) >> a.shift : 0;
+    u32x4 kn[NB][NC];
+    int pn[NB];              // pages: a block of 16 keys lies in one
+    auto find = [&](int base) {
+#pragma unroll
+        for (int b = 0; b < NB; b++) pn[b] = table[min((base + 16 * b) >> a.shift, top)];
+    };
+    auto load = [&](int base) {
+#pragma unroll
+        for (int b = 0; b < NB; b++) {
+            const bool in = (unsigned)pn[b] < (unsigned)a.p.n_pages;
+            const size_t at = (size_t)(in ? pn[b] : 0) * a.p.page_stride +
+                              (size_t)((base + 16 * b) & (a.p.page_size - 1)) * a.p.row_stride;
+#pragma unroll
+            for (int c = 0; c < NC; c++) kn[b][c] = *(const u32x4*)(kp + at + (size_t)col * a.p.row_stride + 32 * c);
+        }
+    };
+    v8 qf[NC];
+    float l2 = 0.0f;
+    int limit = -1, have = -1;
+    auto fetch = [&](int r0) {
+        const int r = r0 + col;
+        const bool live = r < rows;
+        const int qi = live ? r / a.G : 0;
+        const size_t row = (size_t)(sq.r0 + qi) * a.nq + kvh * a.G + (live ? r - qi * a.G : 0);
+        const float ln = live ? a.lse[row] : NEG_INF;
+        // a row that saw no key (lse -infinity) or is none gives nothing
+        l2 = ln == NEG_INF ? -NEG_INF : ln * 1.4426950408889634f;
+        limit = ln != NEG_INF ? sq.ctx - sq.n + qi : -1;
+        have = r0;
+#pragma unroll
+        for (int c = 0; c < NC; c++)
+            qf[c] = vec_of<v8>(live ? *(const u32x4*)(a.q + row * HD + 32 * c + 8 * g4) : u32x4{0, 0, 0, 0});
+    };
+    int base = WK * (4 * blockIdx.z + wave);
+    if (base < sq.ctx) {
+        find(base);
+        load(base);
+        if (base + step < sq.ctx) find(base + step);
+    }
+    for (; base < sq.ctx; base += step) {
+        v8 kf[NB][NC];
+#pragma unroll
+        for (int b = 0; b < NB; b++)
+#pragma unroll
+            for (int c = 0; c < NC; c++) kf[b][c] = vec_of<v8>(kn[b][c]);
+        const int first = max(0, base - (sq.ctx - sq.n)) * a.G & ~15;
+        if (first < rows && have != first) fetch(first);
+        if (base + step < sq.ctx) {
+            load(base + step);
+            if (base + 2 * step < sq.ctx) find(base + 2 * step);
+        }
+        f32x4 acc[NB] = {};
+        for (int r0 = first; r0 < rows; r0 += 16) {
+            if (have != r0) fetch(r0);
+            const f32x4 zero = {};
+            f32x4 sc[NB];
+#pragma unroll
+            for (int c = 0; c < NC; c++)
+#pragma unroll
+                for (int b = 0; b < NB; b++) sc[b] = T::mma16(kf[b][c], qf[c], c ? sc[b] : zero);
+#pragma unroll
+            for (int b = 0; b < NB; b++)
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    const float e = __builtin_amdgcn_exp2f(fmaf(sc[b][i], a.c2, -l2));
+                    acc[b][i] += base + 16 * b + 4 * g4 + i <= limit ? e : 0.0f;
+                }
+        }
+        // over the 16 rows; lane 4 b + i of 16 keeps key i of block b
+        float mine = 0.0f;
+#pragma unroll
+        for (int b = 0; b < NB; b++)
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const float v = row_sum(acc[b][i]);
+                mine = col == 4 * b + i ? v : mine;
+            }
+        const int kk = base + 16 * (col >> 2) + 4 * g4 + (col & 3);
+        if (col < 4 * NB && kk < sq.ctx) {
+            const int pg = table[kk >> a.shift];
+            if ((unsigned)pg < (unsigned)a.p.n_pages) {
+                const size_t at = ((size_t)pg * a.p.n_kv_heads + kvh) * a.p.page_size + (kk & (a.p.page_size - 1));
+                a.p.w[at] = a.w_in ? fmaf(a.decay, a.w_in[at], mine) : mine;
             }
         }
     }
@@ -471,11 +574,16 @@ __global__ __launch_bounds__(256) void k_ev_move(EvArgs a) {
 }
 
 template <typename T, int HD> void weights_rg(const PwArgs& a, bool many, int64_t ctx, hipStream_t st) {
-    constexpr int KB = HD == 256 ? 1 : 2;      // 32 KB keys of 256 columns are all the registers hold
-    const int64_t keys = many ? 64 * KB : 128 * KB, z = (ctx + keys - 1) / keys;
+    constexpr int KB = HD == 256 ? 1 : 2, WK = HD == 256 ? 32 : 64;   // what the registers hold
+    const int64_t keys = many ? 64 * KB : 4 * WK, tiles = (ctx + keys - 1) / keys;
+    // a chunk's tiles are long: one each; a decode step's workgroups, about
+    // four a CU, walk theirs with the next keys in flight
+    const int64_t by = (int64_t)a.p.n_kv_heads * a.b.n_seqs;
+    int64_t z = many ? tiles : (1024 + by - 1) / by;
+    z = z < tiles ? z : tiles;
     const dim3 g(a.p.n_kv_heads, a.b.n_seqs, (unsigned)(z < 65535 ? z : 65535));
     if (many) hipLaunchKernelGGL((k_pa_weights<T, HD, KB, 2, 4>), g, dim3(512), 0, st, a);
-    else hipLaunchKernelGGL((k_pa_weights<T, HD, KB, 4, 1>), g, dim3(256), 0, st, a);
+    else hipLaunchKernelGGL((k_pa_weights_few<T, HD>), g, dim3(256), 0, st, a);
 }
 template <typename TI, bool F32, typename T> void rope_hd(const RaArgs& a, dim3 g, hipStream_t st) {
     switch (a.p.head_dim) {
