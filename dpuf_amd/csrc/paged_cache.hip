@@ -400,8 +400,9 @@ __global__ __launch_bounds__(256) void k_pa_weights_few(PwArgs a) {
 // ---------------------------------------------------------------------------
 // Eviction.  k_ev_pick: one workgroup per (sequence, kv head) finds the
 // keep - sink - recent largest weights of the middle by radix selection on
-// order-preserving integers (4 passes of 8 bits over LDS, or over memory where
-// the row is longer), then lists the kept rows in order.  k_ev_move copies
+// order-preserving integers (10 bits a pass from the highest bit in which two
+// of them differ, over LDS, or over memory where the row is longer), then lists
+// the kept rows in order.  k_ev_move copies
 // them, 16 bytes a lane: bound by bytes.
 // ---------------------------------------------------------------------------
 struct EvArgs {
@@ -451,9 +452,10 @@ DEV void scan2(int& x, int& y, int& tx, int& ty, int (*sums)[2]) {
 
 __global__ __launch_bounds__(EV_T) void k_ev_pick(EvArgs a) {
     extern __shared__ __align__(16) uint32_t keys[];
-    __shared__ int hist[4][256];
+    __shared__ int hist[EV_T];
     __shared__ int sums[EV_T / 64][2];
-    __shared__ uint32_t sh_prefix;
+    __shared__ uint32_t bits[EV_T / 64][2];
+    __shared__ uint32_t sh_digit;
     __shared__ int sh_need;
     const int kvh = blockIdx.x, s = blockIdx.y, t = threadIdx.x;
     const int c = pg_ctx(a.b, a.shift, s), n = min(c, a.keep);
@@ -471,36 +473,74 @@ __global__ __launch_bounds__(EV_T) void k_ev_pick(EvArgs a) {
         if ((unsigned)page >= (unsigned)a.p.n_pages) return 0;
         return weight_key(a.p.w[((size_t)page * a.p.n_kv_heads + kvh) * a.p.page_size + (slot & (a.p.page_size - 1))]);
     };
-    if (staged)
-        for (int i = t; i < mid; i += EV_T) keys[i] = fetch(i);
+    // the bits in which keys differ, and with a row that fits the keys in LDS
+    uint32_t any = 0, all = ~0u;
+    constexpr int AT = 8;          // pages, then weights, in flight
+    for (int i0 = 0; i0 < mid; i0 += AT * EV_T) {
+        int pg[AT];
+        float w[AT];
+#pragma unroll
+        for (int u = 0; u < AT; u++)
+            if (i0 + u * EV_T < mid) pg[u] = pg_page(a.b, a.shift, s, lo + min(i0 + u * EV_T + t, mid - 1));
+#pragma unroll
+        for (int u = 0; u < AT; u++)
+            if (i0 + u * EV_T < mid) {
+                const int in_page = (lo + min(i0 + u * EV_T + t, mid - 1)) & (a.p.page_size - 1);
+                const bool in = (unsigned)pg[u] < (unsigned)a.p.n_pages;
+                w[u] = a.p.w[((size_t)(in ? pg[u] : 0) * a.p.n_kv_heads + kvh) * a.p.page_size + in_page];
+                if (!in) pg[u] = -1;
+            }
+#pragma unroll
+        for (int u = 0; u < AT; u++)
+            if (i0 + u * EV_T + t < mid) {
+                const uint32_t k = pg[u] < 0 ? 0 : weight_key(w[u]);
+                any |= k;
+                all &= k;
+                if (staged) keys[i0 + u * EV_T + t] = k;
+            }
+    }
     auto key_at = [&](int i) -> uint32_t { return staged ? keys[i] : fetch(i); };
-    if (t == 0) { sh_prefix = 0; sh_need = need; }
-    // the need-th largest key, 8 bits at a time from the top
-    for (int shift = 24; shift >= 0 && need > 0; shift -= 8) {
-        hist[t >> 8][t & 255] = 0;
-        __syncthreads();
-        const uint32_t prefix = sh_prefix;
-        const int left = sh_need;
-        const uint32_t mask = shift == 24 ? 0u : ~0u << (shift + 8);
-        for (int i = t; i < mid; i += EV_T) {
-            const uint32_t k = key_at(i);
-            if ((k & mask) == prefix) atomicAdd(&hist[(t >> 6) & 3][(k >> shift) & 255], 1);
-        }
-        __syncthreads();
-        // the largest digit with at least `left` keys at or above it: threads
-        // 0 .. 255 take the digits from the top
-        int x = t < 256 ? hist[0][255 - t] + hist[1][255 - t] + hist[2][255 - t] + hist[3][255 - t] : 0, y = 0, tx, ty;
-        const int own = x;
-        scan2(x, y, tx, ty, sums);
-        if (t < 256 && x >= left && x - own < left) {
-            sh_prefix = prefix | (uint32_t)(255 - t) << shift;
-            sh_need = left - (x - own);
-        }
-        __syncthreads();
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+        any |= __shfl_xor(any, d);
+        all &= __shfl_xor(all, d);
+    }
+    if ((t & 63) == 0) {
+        bits[t >> 6][0] = any;
+        bits[t >> 6][1] = all;
     }
     __syncthreads();
-    const uint32_t cut = sh_prefix;
-    const int ties = sh_need;      // of the keys equal to cut, the first this many stay
+    for (int w = 0; w < EV_T / 64; w++) {
+        any |= bits[w][0];
+        all &= bits[w][1];
+    }
+    int top = any & ~all ? 32 - __clz((int)(any & ~all)) : 0;      // keys agree from this bit up
+    uint32_t cut = top < 32 ? all >> top << top : 0;
+    int ties = need;               // of the keys equal to cut, the first this many stay
+    // the need-th largest key, 10 bits at a time
+    while (top > 0 && need > 0) {
+        const int low = top > 10 ? top - 10 : 0, mask = (1 << (top - low)) - 1;
+        hist[t] = 0;
+        __syncthreads();
+        for (int i = t; i < mid; i += EV_T) {
+            const uint32_t k = key_at(i);
+            if (top == 32 || k >> top == cut >> top) atomicAdd(&hist[mask - (int)(k >> low & mask)], 1);
+        }
+        __syncthreads();
+        // the digit, from the top, in which the count reaches what is left
+        const int own = hist[t];
+        int x = own, y = 0, tx, ty;
+        scan2(x, y, tx, ty, sums);
+        if (x >= ties && x - own < ties) {
+            sh_digit = (uint32_t)(mask - t);
+            sh_need = ties - (x - own);
+        }
+        __syncthreads();
+        cut |= sh_digit << low;
+        ties = sh_need;
+        top = low;
+    }
+    __syncthreads();
     // every thread takes a run of rows; a run's places follow from the counts
     // of the runs before it
     const int per = (mid + EV_T - 1) / EV_T, b0 = min(t * per, mid), b1 = min(b0 + per, mid);
