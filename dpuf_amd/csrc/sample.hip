@@ -7,7 +7,7 @@
 // the same in any order (LDS atomics included), and a token whose weight
 // rounds to 0 has less than 2^-38 of the largest token's.  Such tokens can
 // never be drawn, so they are dropped at once: what is left lies within
-// A = (S + 1) ln 2 temperatures of M.
+// (S + 1) ln 2 temperatures of M.
 //
 // The order "larger logit first, then lower index" is that of the integers
 // c_i = (order-preserving bits of x_i) << 32 | (2^32 - 1 - i).  Top-k, top-p
@@ -15,7 +15,7 @@
 //
 // A row is cut into chunks, one workgroup each, in three launches:
 //   k_smp_max   the chunks' largest logits;
-//   k_smp_hist  tokens and weight in each of NB bins of (M - x) / T per chunk
+//   k_smp_hist  tokens and weight in each bin of ln 2 / 16 temperatures per chunk
 //               (only the sum where neither top-k nor top-p is on); the
 //               workgroup that ends last adds the chunks' bins up, groups of
 //               16 first, and finds the bins in which the prefixes end;
@@ -69,7 +69,8 @@ struct SmArgs {
     const float *top_p, *min_p, *u;
     int* tok;
     float* logp;
-    uint64_t *best, *csum, *wsum, *gsum, *list;   // gsum: weight, tokens of each group of bins
+    // csum: weight of each chunk's quarters; gsum: weight, tokens of each group of bins
+    uint64_t *best, *csum, *wsum, *gsum, *list;
     uint32_t* count;
     SmState* state;
 };
@@ -104,27 +105,34 @@ DEV uint64_t comp_of(float x, int i) { return (uint64_t)order_bits(x) << 32 | (0
 DEV float logit_of(uint64_t c) { return from_bits((uint32_t)(c >> 32)); }
 DEV int index_of(uint64_t c) { return (int)(0xffffffffu - (uint32_t)c); }
 
-// 2^s exp(-a) for 0 <= a < 64: exp(-a) = 2^-n exp(r) with n = rint(a / ln 2) and
-// r = n ln 2 - a, by the Taylor series of exp up to r^11 / 11! (|r| <= ln 2 / 2:
-// what is left out is below 2^-47).
-DEV double exp_neg(double a, int s) {
-    const double n = rint(a * 1.4426950408889634074);
-    // ln 2 in two parts, the first of 40 bits: n times it is exact
-    double r = fma(n, 0x1.62e42fefa2000p-1, -a);
-    r = fma(n, 0x1.9ef35793c7673p-41, r);
-    double e = 1.0 / 39916800.0;
-    e = fma(e, r, 1.0 / 3628800.0);
-    e = fma(e, r, 1.0 / 362880.0);
-    e = fma(e, r, 1.0 / 40320.0);
-    e = fma(e, r, 1.0 / 5040.0);
-    e = fma(e, r, 1.0 / 720.0);
-    e = fma(e, r, 1.0 / 120.0);
+// 2^S exp(-a) = 2^(S - y / 16) exp(r) with y = rint(16 a / ln 2) and r = y ln 2 /
+// 16 - a: the sixteenth powers from a table, exp(r) by its Taylor series up to
+// r^6 / 6! (|r| <= ln 2 / 32: what is left out is below 2^-50; the rounding of
+// ln 2 / 16 times y, at most 1 024, below 2^-48).  y is also the token's bin.
+__device__ const double SIXTEENTHS[16] = {
+    0x1.0000000000000p+0, 0x1.ea4afa2a490dap-1, 0x1.d5818dcfba487p-1, 0x1.c199bdd85529cp-1,
+    0x1.ae89f995ad3adp-1, 0x1.9c49182a3f090p-1, 0x1.8ace5422aa0dbp-1, 0x1.7a11473eb0187p-1,
+    0x1.6a09e667f3bcdp-1, 0x1.5ab07dd485429p-1, 0x1.4bfdad5362a27p-1, 0x1.3dea64c123422p-1,
+    0x1.306fe0a31b715p-1, 0x1.2387a6e756238p-1, 0x1.172b83c7d517bp-1, 0x1.0b5586cf9890fp-1,
+};
+struct Exp {
+    double e;
+    int y;
+};
+DEV Exp exp_neg(const double* table, double a, int S) {
+    // the sum's last bits are the rounded integer
+    const double t = fma(a, 0x1.71547652b82fep+4, 0x1.8p52);
+    const int y = (int)(uint32_t)__builtin_bit_cast(uint64_t, t);
+    const double r = fma(t - 0x1.8p52, 0x1.62e42fefa39efp-5, -a);
+    double e = fma(r, 1.0 / 720.0, 1.0 / 120.0);
     e = fma(e, r, 1.0 / 24.0);
     e = fma(e, r, 1.0 / 6.0);
     e = fma(e, r, 0.5);
     e = fma(e, r, 1.0);
     e = fma(e, r, 1.0);
-    return ldexp(e, s - (int)n);
+    // the power of two goes into the table entry's exponent
+    const uint64_t p = __builtin_bit_cast(uint64_t, table[y & 15]) + ((uint64_t)(uint32_t)(S - (y >> 4)) << 52);
+    return Exp{e * __builtin_bit_cast(double, p), y};
 }
 // rint(e) for 0 <= e <= 2^51: the sum's last bit is worth one
 DEV uint64_t to_int(double e) {
@@ -132,22 +140,23 @@ DEV uint64_t to_int(double e) {
 }
 
 // f(token, logit) for the tokens [lo, hi) of a row, in no particular order; lo
-// is a multiple of 8.
-template <typename L, typename F> DEV void each(const void* p, int vec, int lo, int hi, F f) {
+// a multiple of 8; by N threads: the workgroup's, or a wave's lanes.
+template <typename L, int N = NT, typename F> DEV void each(const void* p, int vec, int lo, int hi, F f) {
     constexpr int VE = L::VE, U = 16 / VE;
+    const int t = threadIdx.x % N;
     int done = lo;
     if (vec) {
         const int v1 = hi / VE;
-        for (int v0 = lo / VE + threadIdx.x; v0 < v1; v0 += NT * U) {
+        for (int v0 = lo / VE + t; v0 < v1; v0 += N * U) {
             float x[U][VE];
 #pragma unroll
             for (int u = 0; u < U; u++) {
-                const int v = v0 + u * NT;
+                const int v = v0 + u * N;
                 L::many(p, (int64_t)(v < v1 ? v : v0) * VE, x[u]);
             }
 #pragma unroll
             for (int u = 0; u < U; u++) {
-                const int v = v0 + u * NT;
+                const int v = v0 + u * N;
                 if (v < v1)
 #pragma unroll
                     for (int e = 0; e < VE; e++) f(v * VE + e, x[u][e]);
@@ -155,39 +164,40 @@ template <typename L, typename F> DEV void each(const void* p, int vec, int lo, 
         }
         done = v1 * VE > lo ? v1 * VE : lo;
     }
-    for (int i = done + threadIdx.x; i < hi; i += NT) f(i, L::one(p, i));
+    for (int i = done + t; i < hi; i += N) f(i, L::one(p, i));
 }
 
 // A row with its settings.
 template <typename L> struct Row {
     const void* p;
+    const double* table;         // SIXTEENTHS in LDS
     int V, S, vec;
-    float M;
-    double invT, A, p_goal;
-    float bins;                  // bins per temperature
+    float M;                     // the largest logit; 0 where that is infinite (then only its like are left)
+    bool inf;
+    double invT, p_goal;
+    int dead;                    // the bin from which on weights are 0 (its own: some)
     int k, by_k, by_p, by_m;
     double min_w, edge;          // 2^S min_p (0: off) and -ln min_p
 
-    // (M - x) / T, or infinity for tokens that cannot be drawn
+    // (M - x) / T, at most 64: far past the last weight
     DEV double depth(float x) const {
-        const double d = (double)M - (double)x;
-        return x == M ? 0.0 : d < __builtin_huge_val() ? d * invT : __builtin_huge_val();
+        if (inf) x = x == __builtin_huge_valf() ? 0.0f : -__builtin_huge_valf();
+        return fmin(((double)M - (double)x) * invT, 64.0);
     }
-    DEV uint64_t weight(double a) const { return a < A ? to_int(exp_neg(a, S)) : 0; }
+    DEV Exp exp_of(double a) const { return exp_neg(table, a, S); }
+    DEV uint64_t weight_of(uint64_t c) const { return to_int(exp_of(depth(logit_of(c))).e); }
     // with min_p's say
-    DEV uint64_t weight_min(double a) const {
-        const double e = exp_neg(a < A ? a : A, S);
-        return a < A && e >= min_w ? to_int(e) : 0;
+    DEV uint64_t weight_min(float x) const {
+        const double e = exp_of(depth(x)).e;
+        return e >= min_w ? to_int(e) : 0;
     }
-    DEV uint64_t weight_of(uint64_t c) const { return weight(depth(logit_of(c))); }
     DEV int bin(double a) const {
-        const int b = (int)((float)a * bins);
-        return b < NB - 1 ? b : NB - 1;
+        return (int)(uint32_t)__builtin_bit_cast(uint64_t, fma(a, 0x1.71547652b82fep+4, 0x1.8p52));
     }
-    // a token with a weight: only the last bin's need the exponential to tell
-    DEV bool alive(double a, int b) const { return a < A && (b < NB - 1 || weight(a) != 0); }
+    DEV int bin_of(uint64_t c) const { return bin(depth(logit_of(c))); }
 
-    DEV void open(const SmArgs& a, int r) {
+    DEV void open(const SmArgs& a, int r, const double* powers) {
+        table = powers;
         p = (const char*)a.x + r * a.stride * L::SIZE;
         V = a.V;
         S = a.S;
@@ -199,9 +209,10 @@ template <typename L> struct Row {
         M = logit_of(best);
         const float T = a.temp ? a.temp[r] : 1.0f;
         if (best == 0 || M == -__builtin_huge_valf() || !(T > 0.0f)) return false;
+        inf = M == __builtin_huge_valf();
+        if (inf) M = 0.0f;
         invT = 1.0 / (double)T;
-        A = (S + 1) * 0.69314718055994530942;
-        bins = (float)(NB / A);
+        dead = 16 * (S + 1);
         k = a.top_k ? a.top_k[r] : 0;
         by_k = k > 0 && k < V;
         const float tp = a.top_p ? a.top_p[r] : 1.0f, mp = a.min_p ? a.min_p[r] : 0.0f;
@@ -209,13 +220,18 @@ template <typename L> struct Row {
         p_goal = tp > 0.0f ? (double)tp : 0.0;
         const double min_p = mp > 1.0f ? 1.0 : mp > 0.0f ? (double)mp : 0.0;
         edge = min_p > 0.0 ? -log(min_p) : 0.0;
-        by_m = min_p > 0.0 && edge < A;
+        by_m = min_p > 0.0 && edge < (S + 1) * 0.69314718055994530942;
         min_w = by_m ? ldexp(min_p, S) : 0.0;
         return true;
     }
     // Top-p's goal for a total: one token at least.
     DEV double goal(uint64_t total) const { return fmax(p_goal * (double)total, 0.5); }
 };
+
+// SIXTEENTHS into LDS; a barrier follows before it is read.
+DEV void load_table(double* table) {
+    if (threadIdx.x < 16) table[threadIdx.x] = SIXTEENTHS[threadIdx.x];
+}
 
 // The row's largest composite from its chunks'.
 DEV uint64_t row_best(const SmArgs& a, int r) {
@@ -230,19 +246,31 @@ DEV uint64_t row_best(const SmArgs& a, int r) {
     return b;
 }
 
-DEV uint64_t shfl_up64(uint64_t v, int d) {
-    const uint32_t lo = __shfl_up((uint32_t)v, d), hi = __shfl_up((uint32_t)(v >> 32), d);
+template <int CTRL, int ROWS> DEV uint64_t dpp64(uint64_t v) {
+    const uint32_t lo = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)v, CTRL, ROWS, 0xF, false);
+    const uint32_t hi = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)(v >> 32), CTRL, ROWS, 0xF, false);
     return (uint64_t)hi << 32 | lo;
+}
+// Inclusive sum over a wave's lanes: within rows of 16 (shifts by 1, 2, 4, 8),
+// then the last lane of a row, and of the lower half, to those after it.
+DEV uint64_t wave_scan64(uint64_t v) {
+    v += dpp64<0x111, 0xF>(v);
+    v += dpp64<0x112, 0xF>(v);
+    v += dpp64<0x114, 0xF>(v);
+    v += dpp64<0x118, 0xF>(v);
+    v += dpp64<0x142, 0xA>(v);
+    v += dpp64<0x143, 0xC>(v);
+    return v;
+}
+DEV uint64_t lane_of(uint64_t v, int l) {
+    return (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(v >> 32), l) << 32 |
+           (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)v, l);
 }
 
 // Inclusive sum over the workgroup's threads; *total gets the sum of all.
 DEV uint64_t scan64(uint64_t* red, uint64_t v, uint64_t* total) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-        const uint64_t o = shfl_up64(v, d);
-        if (lane >= d) v += o;
-    }
+    v = wave_scan64(v);
     __syncthreads();
     if (lane == 63) red[wave] = v;
     __syncthreads();
@@ -254,6 +282,24 @@ DEV uint64_t scan64(uint64_t* red, uint64_t v, uint64_t* total) {
     }
     *total = all;
     return v + base;
+}
+// The same of two sums at once.
+DEV void scan64x2(uint64_t* red, uint64_t& x, uint64_t& y) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    x = wave_scan64(x);
+    y = wave_scan64(y);
+    __syncthreads();
+    if (lane == 63) {
+        red[wave] = x;
+        red[NW + wave] = y;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < NW - 1; w++)
+        if (w < wave) {
+            x += red[w];
+            y += red[NW + w];
+        }
 }
 
 // Whether this workgroup is the last of `of` to get here; what the others
@@ -282,7 +328,7 @@ template <typename L> __global__ __launch_bounds__(NT) void k_smp_max(SmArgs a) 
     __shared__ uint64_t red[NW];
     const int r = blockIdx.y, c = blockIdx.x, t = threadIdx.x;
     Row<L> row;
-    row.open(a, r);
+    row.open(a, r, nullptr);
     if (c == 0 && t == 0) {
         a.state[r].tick[0] = a.state[r].tick[1] = 0;
         a.state[r].n_list = 0;
@@ -316,7 +362,8 @@ struct HistShared {
     uint32_t count[NB];
     unsigned long long gw[NG], fw[GB];     // a group's, a fine bin's weight over all chunks
     uint32_t gc[NG], fc[GB];
-    uint64_t red[NW];
+    uint64_t red[2 * NW];
+    double table[16];
     int flag;
 };
 
@@ -338,22 +385,11 @@ struct Border {
     uint64_t n, w, n_in, w_in;
 };
 
-DEV uint64_t lane_of(uint64_t v, int l) {
-    return (uint64_t)__shfl((uint32_t)(v >> 32), l) << 32 | __shfl((uint32_t)v, l);
-}
-
 // The first of `lanes` lanes' (count, weight) pairs at which a prefix with n
 // tokens and w weight before them meets `want` (-1: none); every wave alike.
 DEV int cross(const Want& want, int lanes, uint64_t c, uint64_t v, uint64_t* n, uint64_t* w) {
     const int lane = threadIdx.x & 63;
-    uint64_t ic = lane < lanes ? c : 0, iv = lane < lanes ? v : 0;
-    for (int d = 1; d < lanes; d <<= 1) {
-        const uint64_t oc = shfl_up64(ic, d), ov = shfl_up64(iv, d);
-        if (lane >= d) {
-            ic += oc;
-            iv += ov;
-        }
-    }
+    const uint64_t ic = wave_scan64(lane < lanes ? c : 0), iv = wave_scan64(lane < lanes ? v : 0);
     const uint64_t hit = __ballot(lane < lanes && want.met(*n + ic, *w + iv));
     if (!hit) return -1;
     const int at = __ffsll((unsigned long long)hit) - 1;
@@ -420,12 +456,7 @@ DEV Border find_border(const SmArgs& a, HistShared& sh, int r, const Want& want,
 // Finds the border bins from the groups' sums.
 template <typename L> DEV void find_borders(const SmArgs& a, HistShared& sh, const Row<L>& row, SmState* st, int r) {
     const int t = threadIdx.x, lane = t & 63;
-    uint64_t tn = sh.gc[lane], tw = sh.gw[lane];
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-        tn += lane_of(tn, lane ^ d);
-        tw += lane_of(tw, lane ^ d);
-    }
+    const uint64_t tn = lane_of(wave_scan64(sh.gc[lane]), 63), tw = lane_of(wave_scan64(sh.gw[lane]), 63);
     int loaded = -1;
     Border k = {-1, 0, 0, 0, 0}, p0 = k, p1 = k;
     if (row.by_k) k = find_border(a, sh, r, Want{BY_COUNT, (uint64_t)row.k, 0.0}, &loaded);
@@ -468,7 +499,8 @@ template <typename L> __global__ __launch_bounds__(NT) void k_smp_hist(SmArgs a)
     const int r = blockIdx.y, c = blockIdx.x, t = threadIdx.x;
     SmState* st = a.state + r;
     Row<L> row;
-    row.open(a, r);
+    row.open(a, r, sh.table);
+    load_table(sh.table);
     const uint64_t best = row_best(a, r);
     if (!row.set(a, r, best)) {
         if (c == 0 && t == 0) {
@@ -481,13 +513,14 @@ template <typename L> __global__ __launch_bounds__(NT) void k_smp_hist(SmArgs a)
     }
     const int lo = c * a.chunk, hi = min(a.V, lo + a.chunk);
     if (!row.by_k && !row.by_p) {
-        uint64_t s = 0, all;
-        each<L>(row.p, row.vec, lo, hi, [&](int, float x) { s += row.weight_min(row.depth(x)); });
-        scan64(sh.red, s, &all);
-        if (t == 0) {
-            a.csum[(size_t)r * a.chunks + c] = all;
-            if (c == 0) st->mode = SM_PLAIN;
-        }
+        // a sum for each wave's quarter of the chunk
+        __syncthreads();
+        const int q = a.chunk / NW, q0 = lo + (t >> 6) * q;
+        uint64_t s = 0;
+        each<L, 64>(row.p, row.vec, q0, min(hi, q0 + q), [&](int, float x) { s += row.weight_min(x); });
+        s = wave_scan64(s);
+        if ((t & 63) == 63) a.csum[((size_t)r * a.chunks + c) * NW + (t >> 6)] = s;
+        if (c == 0 && t == 0) st->mode = SM_PLAIN;
         return;
     }
     for (int b = t; b < NB; b += NT) {
@@ -496,12 +529,11 @@ template <typename L> __global__ __launch_bounds__(NT) void k_smp_hist(SmArgs a)
     }
     __syncthreads();
     each<L>(row.p, row.vec, lo, hi, [&](int, float x) {
-        const double d = row.depth(x);
-        const uint64_t w = row.weight(d);
+        const Exp e = row.exp_of(row.depth(x));
+        const uint64_t w = to_int(e.e);
         if (w) {
-            const int b = row.bin(d);
-            atomicAdd(&sh.count[b], 1u);
-            atomicAdd(&sh.wsum[b], (unsigned long long)w);
+            atomicAdd(&sh.count[e.y], 1u);
+            atomicAdd(&sh.wsum[e.y], (unsigned long long)w);
         }
     });
     __syncthreads();
@@ -575,7 +607,8 @@ struct PickShared {
     uint64_t list[CAP], lw[CAP];
     unsigned long long wsum[NB];
     uint32_t count[NB];
-    uint64_t red[NW];
+    uint64_t red[2 * NW];
+    double table[16];
     uint64_t b0, b1;
     int i0, i1, flag;
     uint32_t n_list;
@@ -633,8 +666,10 @@ DEV int select(PickShared& sh, int n, const Want& want, uint64_t n0, uint64_t w0
             }
         __syncthreads();
         const uint64_t c = sh.count[t], w = sh.wsum[t];
-        uint64_t tc, tw;
-        const uint64_t n1 = scan64(sh.red, c, &tc) + n0, w1 = scan64(sh.red, w, &tw) + w0;
+        uint64_t n1 = c, w1 = w;
+        scan64x2(sh.red, n1, w1);
+        n1 += n0;
+        w1 += w0;
         if (want.met(n1, w1) && !want.met(n1 - c, w1 - w)) {
             sh.i0 = t;
             sh.i1 = (int)c;
@@ -703,23 +738,13 @@ DEV void draw_range(const SmArgs& a, PickShared& sh, const Row<L>& row, int r, i
     }
 }
 
-// The chunk in which the running sum of the chunks' sums (lane c: chunk c's)
-// passes the draw.
-DEV int pick_chunk(uint64_t sum, float u, uint64_t* base, uint64_t* aim, uint64_t* total) {
-    const int lane = threadIdx.x & 63;
-    uint64_t s = sum;
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-        const uint64_t o = shfl_up64(s, d);
-        if (lane >= d) s += o;
-    }
-    const uint32_t lo = __shfl((uint32_t)s, 63), hi = __shfl((uint32_t)(s >> 32), 63);
-    *total = (uint64_t)hi << 32 | lo;
-    *aim = aim_of(u, *total);
-    const int c = __ffsll((unsigned long long)__ballot(s > *aim)) - 1;
-    const uint64_t b = s - sum;
-    *base = (uint64_t)__shfl((uint32_t)(b >> 32), c) << 32 | __shfl((uint32_t)b, c);
-    return c;
+// The lane at which a running sum of the lanes' sums passes aim, base before
+// the first; *base gets the sum before it.
+DEV int pick_lane(uint64_t sum, uint64_t aim, uint64_t* base) {
+    const uint64_t s = wave_scan64(sum) + *base;
+    const int l = __ffsll((unsigned long long)__ballot(s > aim)) - 1;
+    *base = lane_of(s - sum, l);
+    return l;
 }
 
 // ---------------------------------------------------------------------------
@@ -729,13 +754,16 @@ DEV int pick_chunk(uint64_t sum, float u, uint64_t* base, uint64_t* aim, uint64_
 DEV bool find_bin(PickShared& sh, const Want& want, uint64_t n0, uint64_t w0, int* bin, uint64_t* bn, uint64_t* bw) {
     constexpr int PER = NB / NT;
     const int t = threadIdx.x;
-    uint64_t c = 0, w = 0, tc, tw;
+    uint64_t c = 0, w = 0;
 #pragma unroll
     for (int e = 0; e < PER; e++) {
         c += sh.count[PER * t + e];
         w += sh.wsum[PER * t + e];
     }
-    uint64_t n = scan64(sh.red, c, &tc) - c + n0, s = scan64(sh.red, w, &tw) - w + w0;
+    uint64_t n = c, s = w;
+    scan64x2(sh.red, n, s);
+    n += n0 - c;
+    s += w0 - w;
     if (t == 0) sh.i0 = -1;
     __syncthreads();
 #pragma unroll
@@ -774,7 +802,7 @@ DEV uint64_t split_cut(PickShared& sh, const Row<L>& row, const Want& want, uint
         }
         __syncthreads();
         each<L>(row.p, row.vec, 0, row.V, [&](int i, float x) {
-            const uint64_t w = row.weight(row.depth(x)), c = comp_of(x, i);
+            const uint64_t w = to_int(row.exp_of(row.depth(x)).e), c = comp_of(x, i);
             if (w && c >= lo && c <= hi) {
                 atomicAdd(&sh.count[(hi - c) >> sf], 1u);
                 atomicAdd(&sh.wsum[(hi - c) >> sf], (unsigned long long)w);
@@ -796,7 +824,7 @@ DEV uint64_t split_cut(PickShared& sh, const Row<L>& row, const Want& want, uint
         __syncthreads();
         each<L>(row.p, row.vec, 0, row.V, [&](int i, float x) {
             const uint64_t c = comp_of(x, i);
-            if (c >= lo && c <= hi && row.weight(row.depth(x))) {
+            if (c >= lo && c <= hi && to_int(row.exp_of(row.depth(x)).e)) {
                 const uint32_t at = atomicAdd(&sh.n_list, 1u);
                 if (at < CAP) sh.list[at] = c;
             }
@@ -820,7 +848,7 @@ template <typename L> DEV void split_row(const SmArgs& a, PickShared& sh, const 
         cut = c > cut ? c : cut;
     }
     auto kept = [&](int i, float x) -> uint64_t {
-        return comp_of(x, i) >= cut ? row.weight_min(row.depth(x)) : 0;
+        return comp_of(x, i) >= cut ? row.weight_min(x) : 0;
     };
     uint64_t own = 0;
     each<L>(row.p, row.vec, 0, row.V, [&](int i, float x) { own += kept(i, x); });
@@ -835,13 +863,33 @@ template <typename L> __global__ __launch_bounds__(NT) void k_smp_pick(SmArgs a)
     const int mode = sp->mode;
     if (mode == SM_DONE || ((mode == SM_PLAIN || mode == SM_SPLIT) && c != 0)) return;
     Row<L> row;
-    row.open(a, r);
+    row.open(a, r, sh.table);
+    load_table(sh.table);
     row.set(a, r, row_best(a, r));
+    if (t == 0) sh.n_list = 0;
+    __syncthreads();
     if (mode == SM_PLAIN) {
-        uint64_t base, aim, total;
-        const int at = pick_chunk(lane < a.chunks ? a.csum[(size_t)r * a.chunks + lane] : 0, a.u[r], &base, &aim, &total);
-        draw_range(a, sh, row, r, at * a.chunk, min(a.V, (at + 1) * a.chunk), base, aim, total,
-                   [&](int, float x) -> uint64_t { return row.weight_min(row.depth(x)); });
+        // the chunk, then the quarter of it
+        uint64_t sums[NW] = {}, own = 0, base = 0;
+        if (lane < a.chunks)
+#pragma unroll
+            for (int w = 0; w < NW; w++) sums[w] = a.csum[((size_t)r * a.chunks + lane) * NW + w];
+#pragma unroll
+        for (int w = 0; w < NW; w++) own += sums[w];
+        const uint64_t total = lane_of(wave_scan64(own), 63), aim = aim_of(a.u[r], total);
+        const int at = pick_lane(own, aim, &base);
+        int w = 0;
+        uint64_t here = lane_of(sums[0], at);
+#pragma unroll
+        for (int e = 1; e < NW; e++)
+            if (w == e - 1 && base + here <= aim) {
+                base += here;
+                here = lane_of(sums[e], at);
+                w = e;
+            }
+        const int q = a.chunk / NW, lo = at * a.chunk + w * q;
+        draw_range(a, sh, row, r, lo, min(a.V, lo + q), base, aim, total,
+                   [&](int, float x) -> uint64_t { return row.weight_min(x); });
         return;
     }
     const SmState st = *sp;
@@ -849,17 +897,29 @@ template <typename L> __global__ __launch_bounds__(NT) void k_smp_pick(SmArgs a)
         split_row(a, sh, row, st, r);
         return;
     }
-    // the tokens that decide
-    if (t == 0) sh.n_list = 0;
-    __syncthreads();
+    // the tokens that decide; most are told by their logit alone
+    int b_lo = NB, b_hi = -1;
+    if (mode == SM_LIST) {
+        b_lo = 0;
+        b_hi = st.last;
+    } else {
+        if (st.by_k) b_lo = min(b_lo, st.bk), b_hi = max(b_hi, st.bk);
+        if (st.by_p) b_lo = min(b_lo, st.pl), b_hi = max(b_hi, st.ph);
+        if (st.by_m) b_lo = min(b_lo, st.ml), b_hi = max(b_hi, st.mh);
+    }
+    // (a bin and a half of slack, and the rounding of the difference)
+    const double per = 0.0433216987849965803891 / row.invT;      // ln 2 / 16 temperatures
+    const float x_lo = row.inf ? -__builtin_huge_valf() : (float)((double)row.M - (b_hi + 1.5) * per - 1e-6 * fabs((double)row.M));
+    const float x_hi = row.inf ? __builtin_huge_valf() : (float)((double)row.M - (b_lo - 1.5) * per + 1e-6 * fabs((double)row.M));
     each<L>(row.p, row.vec, c * a.chunk, min(a.V, (c + 1) * a.chunk), [&](int i, float x) {
+        if (!(x >= x_lo && x <= x_hi)) return;
         const double d = row.depth(x);
-        if (!(d < row.A)) return;
         const int b = row.bin(d);
         const bool in = mode == SM_LIST ? b <= st.last
                                         : (st.by_k && b == st.bk) || (st.by_p && b >= st.pl && b <= st.ph) ||
                                               (st.by_m && b >= st.ml && b <= st.mh);
-        if (in && row.alive(d, b)) {
+        // only the last bin has tokens without a weight
+        if (in && (b < row.dead || to_int(row.exp_of(d).e) != 0)) {
             const uint32_t at = atomicAdd(&sh.n_list, 1u);
             if (at < CAP) sh.list[at] = comp_of(x, i);
         }
@@ -882,7 +942,7 @@ template <typename L> __global__ __launch_bounds__(NT) void k_smp_pick(SmArgs a)
     for (int i = t; i < n; i += NT) sh.lw[i] = row.weight_of(sh.list[i]);
     __syncthreads();
     auto comp = [&](int i) { return sh.list[i]; };
-    auto bin_of = [&](int i) { return row.bin(row.depth(logit_of(sh.list[i]))); };
+    auto bin_of = [&](int i) { return row.bin_of(sh.list[i]); };
     uint64_t sum = st.total, cut = 0;      // composites below cut are out
     if (st.by_k) {
         const int at = mode == SM_LIST
@@ -905,7 +965,7 @@ template <typename L> __global__ __launch_bounds__(NT) void k_smp_pick(SmArgs a)
     }
     // what stays of the list
     for (int i = t; i < n; i += NT)
-        if (sh.list[i] < cut || row.weight_min(row.depth(logit_of(sh.list[i]))) == 0) sh.lw[i] = 0;
+        if (sh.list[i] < cut || row.weight_min(logit_of(sh.list[i])) == 0) sh.lw[i] = 0;
     __syncthreads();
     if (mode == SM_LIST) {
         uint64_t own = 0, total;
@@ -918,7 +978,7 @@ template <typename L> __global__ __launch_bounds__(NT) void k_smp_pick(SmArgs a)
     }
     // the chunks' sums: the bins above the highest border, and what stays of
     // the list from there on
-    const int cb = min(cut ? row.bin(row.depth(logit_of(cut))) : NB, st.by_m ? st.ml : NB), g = cb / GB;
+    const int cb = min(cut ? row.bin_of(cut) : NB, st.by_m ? st.ml : NB), g = cb / GB;
     if (t < MAX_CHUNKS) sh.wsum[t] = 0;
     __syncthreads();
     for (int k = wave; k < a.chunks; k += NW) {
@@ -936,10 +996,12 @@ template <typename L> __global__ __launch_bounds__(NT) void k_smp_pick(SmArgs a)
         if (sh.lw[i] && bin_of(i) >= cb)
             atomicAdd(&sh.wsum[index_of(sh.list[i]) / a.chunk], (unsigned long long)sh.lw[i]);
     __syncthreads();
-    uint64_t base, aim, total;
-    const int at = pick_chunk(lane < a.chunks ? sh.wsum[lane] : 0, a.u[r], &base, &aim, &total);
+    const uint64_t mine = lane < a.chunks ? sh.wsum[lane] : 0;
+    const uint64_t total = lane_of(wave_scan64(mine), 63), aim = aim_of(a.u[r], total);
+    uint64_t base = 0;
+    const int at = pick_lane(mine, aim, &base);
     draw_range(a, sh, row, r, at * a.chunk, min(a.V, (at + 1) * a.chunk), base, aim, total,
-               [&](int i, float x) -> uint64_t { return comp_of(x, i) >= cut ? row.weight_min(row.depth(x)) : 0; });
+               [&](int i, float x) -> uint64_t { return comp_of(x, i) >= cut ? row.weight_min(x) : 0; });
 }
 
 struct SmPlan {
@@ -947,20 +1009,20 @@ struct SmPlan {
     size_t best, csum, wsum, gsum, list, count, state, bytes;
 };
 
-// Chunks of at least 4 096 tokens, as many as give about four workgroups a CU
-// over all rows, 64 at most.
+// Chunks of 4 096 tokens, or a multiple where that would be more than about
+// four workgroups a CU over all rows, or more than 64 chunks a row.
 SmPlan plan(int n, int V) {
     SmPlan p;
     p.rows = n < ROWS ? n : ROWS;
     int c = (ROWS + p.rows - 1) / p.rows;
     if (c > MAX_CHUNKS) c = MAX_CHUNKS;
-    p.chunk = ((V + c - 1) / c + 7) & ~7;
-    if (p.chunk < 4096) p.chunk = 4096;
+    p.chunk = ((V + c - 1) / c + 4095) / 4096 * 4096;
+    if (p.chunk > 4096 && V / (p.chunk - 4096) < (c > 1 ? MAX_CHUNKS : 1)) p.chunk -= 4096;
     p.chunks = (V + p.chunk - 1) / p.chunk;
     const size_t k = (size_t)p.rows * p.chunks;
     p.best = 0;
     p.csum = p.best + k * 8;
-    p.wsum = p.csum + k * 8;
+    p.wsum = p.csum + k * NW * 8;
     p.gsum = p.wsum + k * NB * 8;
     p.list = p.gsum + k * NG * 16;
     p.count = p.list + (size_t)p.rows * CAP * 8;
