@@ -14,8 +14,8 @@
 // and min-p each keep a prefix of it, so together they keep the shortest.
 //
 // A row is cut into chunks, one workgroup each, in three launches:
-//   k_smp_max   the chunks' largest logits;
-//   k_smp_hist  tokens and weight in each bin of ln 2 / 16 temperatures per chunk
+//   k_smp_max   the chunks' largest and least logits;
+//   k_smp_hist  tokens and weight in each of NB bins of M - x per chunk
 //               (only the sum where neither top-k nor top-p is on); the
 //               workgroup that ends last adds the chunks' bins up, groups of
 //               16 first, and finds the bins in which the prefixes end;
@@ -41,6 +41,7 @@ namespace {
 constexpr int NT = 256;          // threads of a workgroup
 constexpr int NW = NT / 64;
 constexpr int NB = 1024;         // bins
+constexpr int FULL = 1000;       // of them for the tokens that surely have a weight
 constexpr int GB = 16;           // bins of a group
 constexpr int NG = NB / GB;      // groups: a wave's lanes
 constexpr int CAP = 2048;        // tokens listed in LDS
@@ -72,6 +73,7 @@ struct SmArgs {
     // csum: weight of each chunk's quarters; gsum: weight, tokens of each group of bins
     uint64_t *best, *csum, *wsum, *gsum, *list;
     uint32_t* count;
+    float* least;
     SmState* state;
 };
 
@@ -108,18 +110,14 @@ DEV int index_of(uint64_t c) { return (int)(0xffffffffu - (uint32_t)c); }
 // 2^S exp(-a) = 2^(S - y / 16) exp(r) with y = rint(16 a / ln 2) and r = y ln 2 /
 // 16 - a: the sixteenth powers from a table, exp(r) by its Taylor series up to
 // r^6 / 6! (|r| <= ln 2 / 32: what is left out is below 2^-50; the rounding of
-// ln 2 / 16 times y, at most 1 024, below 2^-48).  y is also the token's bin.
+// ln 2 / 16 times y, at most 1 024 for a weight, below 2^-48).
 __device__ const double SIXTEENTHS[16] = {
     0x1.0000000000000p+0, 0x1.ea4afa2a490dap-1, 0x1.d5818dcfba487p-1, 0x1.c199bdd85529cp-1,
     0x1.ae89f995ad3adp-1, 0x1.9c49182a3f090p-1, 0x1.8ace5422aa0dbp-1, 0x1.7a11473eb0187p-1,
     0x1.6a09e667f3bcdp-1, 0x1.5ab07dd485429p-1, 0x1.4bfdad5362a27p-1, 0x1.3dea64c123422p-1,
     0x1.306fe0a31b715p-1, 0x1.2387a6e756238p-1, 0x1.172b83c7d517bp-1, 0x1.0b5586cf9890fp-1,
 };
-struct Exp {
-    double e;
-    int y;
-};
-DEV Exp exp_neg(const double* table, double a, int S) {
+DEV double exp_neg(const double* table, double a, int S) {
     // the sum's last bits are the rounded integer
     const double t = fma(a, 0x1.71547652b82fep+4, 0x1.8p52);
     const int y = (int)(uint32_t)__builtin_bit_cast(uint64_t, t);
@@ -132,7 +130,7 @@ DEV Exp exp_neg(const double* table, double a, int S) {
     e = fma(e, r, 1.0);
     // the power of two goes into the table entry's exponent
     const uint64_t p = __builtin_bit_cast(uint64_t, table[y & 15]) + ((uint64_t)(uint32_t)(S - (y >> 4)) << 52);
-    return Exp{e * __builtin_bit_cast(double, p), y};
+    return e * __builtin_bit_cast(double, p);
 }
 // rint(e) for 0 <= e <= 2^51: the sum's last bit is worth one
 DEV uint64_t to_int(double e) {
@@ -175,26 +173,25 @@ template <typename L> struct Row {
     float M;                     // the largest logit; 0 where that is infinite (then only its like are left)
     bool inf;
     double invT, p_goal;
-    int dead;                    // the bin from which on weights are 0 (its own: some)
+    float bins;                  // bins per logit
     int k, by_k, by_p, by_m;
-    double min_w, edge;          // 2^S min_p (0: off) and -ln min_p
+    double min_w, edge;          // 2^S min_p (0: off) and -T ln min_p
 
-    // (M - x) / T, at most 64: far past the last weight
-    DEV double depth(float x) const {
+    DEV double below(float x) const {      // the largest logit less x
         if (inf) x = x == __builtin_huge_valf() ? 0.0f : -__builtin_huge_valf();
-        return fmin(((double)M - (double)x) * invT, 64.0);
+        return (double)M - (double)x;
     }
-    DEV Exp exp_of(double a) const { return exp_neg(table, a, S); }
-    DEV uint64_t weight_of(uint64_t c) const { return to_int(exp_of(depth(logit_of(c))).e); }
+    // 2^S exp(-d / T); 64 temperatures are far past the last weight
+    DEV double exp_of(double d) const { return exp_neg(table, fmin(d * invT, 64.0), S); }
+    DEV uint64_t weight(double d) const { return to_int(exp_of(d)); }
+    DEV uint64_t weight_of(uint64_t c) const { return weight(below(logit_of(c))); }
     // with min_p's say
     DEV uint64_t weight_min(float x) const {
-        const double e = exp_of(depth(x)).e;
+        const double e = exp_of(below(x));
         return e >= min_w ? to_int(e) : 0;
     }
-    DEV int bin(double a) const {
-        return (int)(uint32_t)__builtin_bit_cast(uint64_t, fma(a, 0x1.71547652b82fep+4, 0x1.8p52));
-    }
-    DEV int bin_of(uint64_t c) const { return bin(depth(logit_of(c))); }
+    DEV int bin(double d) const { return min((int)((float)d * bins), NB - 1); }
+    DEV int bin_of(uint64_t c) const { return bin(below(logit_of(c))); }
 
     DEV void open(const SmArgs& a, int r, const double* powers) {
         table = powers;
@@ -203,16 +200,19 @@ template <typename L> struct Row {
         S = a.S;
         vec = a.vec;
     }
-    // The settings of row r with largest logit m; false where the row needs
-    // no weights (nothing above -infinity, or greedy).
-    DEV bool set(const SmArgs& a, int r, uint64_t best) {
+    // The settings of row r with its largest and its least logit above
+    // -infinity; false where the row needs no weights (there is none, or
+    // greedy).
+    DEV bool set(const SmArgs& a, int r, uint64_t best, float least) {
         M = logit_of(best);
         const float T = a.temp ? a.temp[r] : 1.0f;
         if (best == 0 || M == -__builtin_huge_valf() || !(T > 0.0f)) return false;
         inf = M == __builtin_huge_valf();
+        // FULL bins over the row's logits, or over those with a weight
+        const float span = fminf(M - least, T * ((float)(S + 1) * 0.6931472f));
+        bins = (float)FULL / fmaxf(span, 1e-30f);
         if (inf) M = 0.0f;
         invT = 1.0 / (double)T;
-        dead = 16 * (S + 1);
         k = a.top_k ? a.top_k[r] : 0;
         by_k = k > 0 && k < V;
         const float tp = a.top_p ? a.top_p[r] : 1.0f, mp = a.min_p ? a.min_p[r] : 0.0f;
@@ -221,6 +221,7 @@ template <typename L> struct Row {
         const double min_p = mp > 1.0f ? 1.0 : mp > 0.0f ? (double)mp : 0.0;
         edge = min_p > 0.0 ? -log(min_p) : 0.0;
         by_m = min_p > 0.0 && edge < (S + 1) * 0.69314718055994530942;
+        edge *= (double)T;
         min_w = by_m ? ldexp(min_p, S) : 0.0;
         return true;
     }
@@ -233,16 +234,20 @@ DEV void load_table(double* table) {
     if (threadIdx.x < 16) table[threadIdx.x] = SIXTEENTHS[threadIdx.x];
 }
 
-// The row's largest composite from its chunks'.
-DEV uint64_t row_best(const SmArgs& a, int r) {
+// The row's largest composite and least logit from its chunks'.
+DEV uint64_t row_best(const SmArgs& a, int r, float* least) {
     const int lane = threadIdx.x & 63;
-    uint64_t b = lane < a.chunks ? a.best[(size_t)r * a.chunks + lane] : 0;
+    const size_t at = (size_t)r * a.chunks + min(lane, a.chunks - 1);
+    uint64_t b = a.best[at];
+    float m = a.least[at];
 #pragma unroll
     for (int d = 1; d < 64; d <<= 1) {
         const uint32_t lo = __shfl_xor((uint32_t)b, d), hi = __shfl_xor((uint32_t)(b >> 32), d);
         const uint64_t o = (uint64_t)hi << 32 | lo;
         b = o > b ? o : b;
+        m = fminf(m, __shfl_xor(m, d));
     }
+    *least = m;
     return b;
 }
 
@@ -320,12 +325,13 @@ DEV uint64_t aim_of(float u, uint64_t total) {
 }
 template <typename L> DEV void answer(const SmArgs& a, const Row<L>& row, int r, int tok, float x, uint64_t total) {
     a.tok[r] = tok;
-    if (a.logp) a.logp[r] = (float)(-row.depth(x) - log((double)total / (double)(1ull << row.S)));
+    if (a.logp) a.logp[r] = (float)(-row.below(x) * row.invT - log((double)total / (double)(1ull << row.S)));
 }
 
 // ---------------------------------------------------------------------------
 template <typename L> __global__ __launch_bounds__(NT) void k_smp_max(SmArgs a) {
     __shared__ uint64_t red[NW];
+    __shared__ float red_min[NW];
     const int r = blockIdx.y, c = blockIdx.x, t = threadIdx.x;
     Row<L> row;
     row.open(a, r, nullptr);
@@ -333,13 +339,14 @@ template <typename L> __global__ __launch_bounds__(NT) void k_smp_max(SmArgs a) 
         a.state[r].tick[0] = a.state[r].tick[1] = 0;
         a.state[r].n_list = 0;
     }
-    float m = -__builtin_huge_valf();
+    float m = -__builtin_huge_valf(), least = -m;
     int at = -1;
     each<L>(row.p, row.vec, c * a.chunk, min(a.V, (c + 1) * a.chunk), [&](int i, float x) {
         if (x > m) {
             m = x;
             at = i;
         }
+        if (x > -__builtin_huge_valf()) least = fminf(least, x);
     });
     uint64_t b = at >= 0 ? comp_of(m, at) : 0;
 #pragma unroll
@@ -347,12 +354,20 @@ template <typename L> __global__ __launch_bounds__(NT) void k_smp_max(SmArgs a) 
         const uint32_t lo = __shfl_xor((uint32_t)b, d), hi = __shfl_xor((uint32_t)(b >> 32), d);
         const uint64_t o = (uint64_t)hi << 32 | lo;
         b = o > b ? o : b;
+        least = fminf(least, __shfl_xor(least, d));
     }
-    if ((t & 63) == 0) red[t >> 6] = b;
+    if ((t & 63) == 0) {
+        red[t >> 6] = b;
+        red_min[t >> 6] = least;
+    }
     __syncthreads();
     if (t == 0) {
-        for (int w = 1; w < NW; w++) b = red[w] > b ? red[w] : b;
+        for (int w = 1; w < NW; w++) {
+            b = red[w] > b ? red[w] : b;
+            least = fminf(least, red_min[w]);
+        }
         a.best[(size_t)r * a.chunks + c] = b;
+        a.least[(size_t)r * a.chunks + c] = least;
     }
 }
 
@@ -467,7 +482,7 @@ template <typename L> DEV void find_borders(const SmArgs& a, HistShared& sh, con
         p1 = by_k ? find_border(a, sh, r, Want{BY_GOAL, 0, row.goal(k.w + k.w_in)}, &loaded) : p0;
     }
     const bool by_p = p0.bin >= 0 && p1.bin >= 0;
-    const int ml = row.by_m ? row.bin(row.edge * (1.0 - 1e-9)) : -1, mh = row.by_m ? row.bin(row.edge * (1.0 + 1e-9)) : -1;
+    const int ml = row.by_m ? row.bin(row.edge * (1.0 - 1e-6)) : -1, mh = row.by_m ? row.bin(row.edge * (1.0 + 1e-6)) : -1;
     const uint64_t upto = by_k ? k.n + k.n_in : by_p ? p1.n + p1.n_in : tn;
     uint64_t in_s = (by_k ? k.n_in : 0) + (by_p ? p1.n + p1.n_in - p0.n : 0);
     if (row.by_m && upto > CAP)
@@ -501,8 +516,9 @@ template <typename L> __global__ __launch_bounds__(NT) void k_smp_hist(SmArgs a)
     Row<L> row;
     row.open(a, r, sh.table);
     load_table(sh.table);
-    const uint64_t best = row_best(a, r);
-    if (!row.set(a, r, best)) {
+    float least;
+    const uint64_t best = row_best(a, r, &least);
+    if (!row.set(a, r, best, least)) {
         if (c == 0 && t == 0) {
             const bool none = best == 0 || logit_of(best) == -__builtin_huge_valf();
             a.tok[r] = none ? -1 : index_of(best);
@@ -529,11 +545,12 @@ template <typename L> __global__ __launch_bounds__(NT) void k_smp_hist(SmArgs a)
     }
     __syncthreads();
     each<L>(row.p, row.vec, lo, hi, [&](int, float x) {
-        const Exp e = row.exp_of(row.depth(x));
-        const uint64_t w = to_int(e.e);
+        const double d = row.below(x);
+        const uint64_t w = row.weight(d);
         if (w) {
-            atomicAdd(&sh.count[e.y], 1u);
-            atomicAdd(&sh.wsum[e.y], (unsigned long long)w);
+            const int b = row.bin(d);
+            atomicAdd(&sh.count[b], 1u);
+            atomicAdd(&sh.wsum[b], (unsigned long long)w);
         }
     });
     __syncthreads();
@@ -802,7 +819,7 @@ DEV uint64_t split_cut(PickShared& sh, const Row<L>& row, const Want& want, uint
         }
         __syncthreads();
         each<L>(row.p, row.vec, 0, row.V, [&](int i, float x) {
-            const uint64_t w = to_int(row.exp_of(row.depth(x)).e), c = comp_of(x, i);
+            const uint64_t w = row.weight(row.below(x)), c = comp_of(x, i);
             if (w && c >= lo && c <= hi) {
                 atomicAdd(&sh.count[(hi - c) >> sf], 1u);
                 atomicAdd(&sh.wsum[(hi - c) >> sf], (unsigned long long)w);
@@ -824,7 +841,7 @@ DEV uint64_t split_cut(PickShared& sh, const Row<L>& row, const Want& want, uint
         __syncthreads();
         each<L>(row.p, row.vec, 0, row.V, [&](int i, float x) {
             const uint64_t c = comp_of(x, i);
-            if (c >= lo && c <= hi && to_int(row.exp_of(row.depth(x)).e)) {
+            if (c >= lo && c <= hi && row.weight(row.below(x))) {
                 const uint32_t at = atomicAdd(&sh.n_list, 1u);
                 if (at < CAP) sh.list[at] = c;
             }
@@ -865,7 +882,9 @@ template <typename L> __global__ __launch_bounds__(NT) void k_smp_pick(SmArgs a)
     Row<L> row;
     row.open(a, r, sh.table);
     load_table(sh.table);
-    row.set(a, r, row_best(a, r));
+    float least;
+    const uint64_t best = row_best(a, r, &least);
+    row.set(a, r, best, least);
     if (t == 0) sh.n_list = 0;
     __syncthreads();
     if (mode == SM_PLAIN) {
@@ -907,19 +926,19 @@ template <typename L> __global__ __launch_bounds__(NT) void k_smp_pick(SmArgs a)
         if (st.by_p) b_lo = min(b_lo, st.pl), b_hi = max(b_hi, st.ph);
         if (st.by_m) b_lo = min(b_lo, st.ml), b_hi = max(b_hi, st.mh);
     }
-    // (a bin and a half of slack, and the rounding of the difference)
-    const double per = 0.0433216987849965803891 / row.invT;      // ln 2 / 16 temperatures
-    const float x_lo = row.inf ? -__builtin_huge_valf() : (float)((double)row.M - (b_hi + 1.5) * per - 1e-6 * fabs((double)row.M));
-    const float x_hi = row.inf ? __builtin_huge_valf() : (float)((double)row.M - (b_lo - 1.5) * per + 1e-6 * fabs((double)row.M));
+    // (with a bin of slack for the rounding of differences and products)
+    const float inf = __builtin_huge_valf();
+    const double per = 1.0 / (double)row.bins, slack = 1e-6 * fabs((double)row.M);
+    const float x_lo = row.inf || b_hi >= NB - 1 ? -inf : (float)((double)row.M - (b_hi + 2) * per - slack);
+    const float x_hi = row.inf || b_lo < 2 ? inf : (float)((double)row.M - (b_lo - 2) * per + slack);
     each<L>(row.p, row.vec, c * a.chunk, min(a.V, (c + 1) * a.chunk), [&](int i, float x) {
         if (!(x >= x_lo && x <= x_hi)) return;
-        const double d = row.depth(x);
+        const double d = row.below(x);
         const int b = row.bin(d);
         const bool in = mode == SM_LIST ? b <= st.last
                                         : (st.by_k && b == st.bk) || (st.by_p && b >= st.pl && b <= st.ph) ||
                                               (st.by_m && b >= st.ml && b <= st.mh);
-        // only the last bin has tokens without a weight
-        if (in && (b < row.dead || to_int(row.exp_of(d).e) != 0)) {
+        if (in && row.weight(d) != 0) {
             const uint32_t at = atomicAdd(&sh.n_list, 1u);
             if (at < CAP) sh.list[at] = comp_of(x, i);
         }
@@ -1006,7 +1025,7 @@ template <typename L> __global__ __launch_bounds__(NT) void k_smp_pick(SmArgs a)
 
 struct SmPlan {
     int rows, chunk, chunks;
-    size_t best, csum, wsum, gsum, list, count, state, bytes;
+    size_t best, csum, wsum, gsum, list, count, least, state, bytes;
 };
 
 // Chunks of 4 096 tokens, or a multiple where that would be more than about
@@ -1026,7 +1045,8 @@ SmPlan plan(int n, int V) {
     p.gsum = p.wsum + k * NB * 8;
     p.list = p.gsum + k * NG * 16;
     p.count = p.list + (size_t)p.rows * CAP * 8;
-    p.state = p.count + k * NB * 4;
+    p.least = p.count + k * NB * 4;
+    p.state = (p.least + k * 4 + 7) / 8 * 8;
     p.bytes = p.state + (size_t)p.rows * sizeof(SmState);
     return p;
 }
@@ -1066,6 +1086,7 @@ void dpuf_hip_sample(void* s, int32_t type, int32_t n, int32_t V, int64_t stride
     a.gsum = (uint64_t*)(w + pl.gsum);
     a.list = (uint64_t*)(w + pl.list);
     a.count = (uint32_t*)(w + pl.count);
+    a.least = (float*)(w + pl.least);
     a.state = (SmState*)(w + pl.state);
     for (int32_t r0 = 0; r0 < n; r0 += ROWS) {
         a.x = (const char*)x + r0 * stride * es;
