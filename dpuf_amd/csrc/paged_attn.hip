@@ -26,6 +26,7 @@
 // rounded to the pages' type for the product with V (a relative half step,
 // 2^-8 in bf16 and 2^-11 in fp16, of each term), every sum is fp32.
 #include <hip/hip_runtime.h>
+#include <math.h>
 #include <stdint.h>
 
 #include "hip_internal.h"
@@ -36,7 +37,7 @@ namespace {
 const float NEG_INF = -__builtin_huge_valf();
 constexpr float SLACK = 6.0f;
 
-enum { PA_BOTH = 0, PA_FEW, PA_MANY };
+enum { PA_BOTH = 0, PA_FEW, PA_MANY, PA_WIDE };
 
 struct PaArgs {
     DpufAmdBatch b;
@@ -131,7 +132,7 @@ template <typename T, int HD> DEV void few_rows(const PaArgs& a, FewLds<HD>& sh,
         v8 qf[NC];
 #pragma unroll
         for (int c = 0; c < NC; c++)
-            qf[c] = live ? vec_of<v8>(*(const u32x4*)(a.q + row * HD + 32 * c + 8 * g4)) : vec_of<v8>(u32x4{0, 0, 0, 0});
+            qf[c] = vec_of<v8>(live ? *(const u32x4*)(a.q + row * HD + 32 * c + 8 * g4) : u32x4{0, 0, 0, 0});
 
         f32x4 o[ND];
 #pragma unroll
@@ -305,10 +306,12 @@ template <typename T, int HD> DEV void few_rows(const PaArgs& a, FewLds<HD>& sh,
 
 // ---------------------------------------------------------------------------
 // Many rows (chunks of a prompt): bound by the matrix instructions and the
-// exponentials.  One workgroup per (kv head, 128 packed rows, key range); its
-// four waves take 32 rows each and share tiles of KT keys of K and V in LDS,
-// two of them: while one is computed, the other takes the tile after it from
-// registers, whose loads were issued a tile earlier.
+// exponentials.  One workgroup per (kv head, 32 WAVES packed rows, key range);
+// its waves take 32 rows each and share tiles of KT keys of K and V in LDS, two
+// of them: while one is computed, the other takes the tile after it from
+// registers, whose loads were issued a tile earlier.  Two workgroups of four
+// waves a CU, whose vector and matrix work overlap, or one of eight, which
+// loads and stores half the tiles for the same rows.
 // ---------------------------------------------------------------------------
 template <int HD> struct ManyLds {
     static constexpr int KT = HD == 256 ? 32 : 64;
@@ -318,12 +321,14 @@ template <int HD> struct ManyLds {
     uint16_t v[2][KT * VP];
 };
 
-template <typename T, int HD> DEV void many_rows(const PaArgs& a, ManyLds<HD>& sh, int kvh, int tile, int z) {
+template <typename T, int HD, int WAVES>
+DEV void many_rows(const PaArgs& a, ManyLds<HD>& sh, int kvh, int tile, int z) {
     constexpr int KT = ManyLds<HD>::KT, KP = ManyLds<HD>::KP, VP = ManyLds<HD>::VP;
     constexpr int NC = HD / 16;          // 16-column steps of a key
     constexpr int ND = HD / 32;          // 32-column tiles of the output
     constexpr int CH = HD / 8;           // 16-byte pieces of a row
-    constexpr int RP = 256 / CH;         // rows a pass of the workgroup loads
+    constexpr int TR = 32 * WAVES;       // packed rows of a workgroup
+    constexpr int RP = 64 * WAVES / CH;  // rows a pass of the workgroup loads
     constexpr int NP = KT / RP;
     constexpr int NB = KT / 32;          // 32-key blocks of a tile
     typedef typename T::v8 v8;
@@ -339,7 +344,7 @@ template <typename T, int HD> DEV void many_rows(const PaArgs& a, ManyLds<HD>& s
         if (s0 + lane < a.b.n_seqs) {
             const PgSeq t = pg_seq(a.b, a.shift, s0 + lane);
             const int rows = t.n * a.G;
-            n = rows > a.few || a.only == PA_MANY ? (rows + 127) >> 7 : 0;
+            n = rows > a.few || a.only != PA_BOTH ? (rows + TR - 1) / TR : 0;
         }
         int sum = n;
         for (int d = 1; d < 64; d <<= 1) {
@@ -364,23 +369,23 @@ template <typename T, int HD> DEV void many_rows(const PaArgs& a, ManyLds<HD>& s
     const int ranges = sq.ctx > per ? (sq.ctx + per - 1) / per : 1;
     if (z >= ranges) return;
 
-    const int r = 128 * tile + 32 * wave + col;
+    const int r = TR * tile + 32 * wave + col;
     const bool live = r < rows;
     const int qi = live ? r / a.G : 0, head = kvh * a.G + (live ? r - qi * a.G : 0);
     const size_t row = (size_t)(sq.r0 + qi) * a.nq + head;
     const int limit = live ? sq.ctx - sq.n + qi : -1;
     // keys past a wave's last row's limit are skipped by the wave, past the
     // workgroup's by all
-    const int wl = min(rows, 128 * tile + 32 * wave + 32) - 1, gl = min(rows, 128 * tile + 128) - 1;
-    const int first_limit = sq.ctx - sq.n + (128 * tile + 32 * wave) / a.G;
+    const int wl = min(rows, TR * tile + 32 * wave + 32) - 1, gl = min(rows, TR * tile + TR) - 1;
+    const int first_limit = sq.ctx - sq.n + (TR * tile + 32 * wave) / a.G;
     const int k0 = z * per;
-    const int wend = 128 * tile + 32 * wave < rows ? min(sq.ctx - sq.n + wl / a.G + 1, k0 + per) : 0;
+    const int wend = TR * tile + 32 * wave < rows ? min(sq.ctx - sq.n + wl / a.G + 1, k0 + per) : 0;
     const int kend = min(min(sq.ctx - sq.n + gl / a.G + 1, sq.ctx), k0 + per);
 
     v8 qf[NC];
 #pragma unroll
     for (int c = 0; c < NC; c++)
-        qf[c] = live ? vec_of<v8>(*(const u32x4*)(a.q + row * HD + 16 * c + 8 * h)) : vec_of<v8>(u32x4{0, 0, 0, 0});
+        qf[c] = vec_of<v8>(live ? *(const u32x4*)(a.q + row * HD + 16 * c + 8 * h) : u32x4{0, 0, 0, 0});
     f32x16 o[ND];
 #pragma unroll
     for (int d = 0; d < ND; d++)
@@ -393,7 +398,7 @@ template <typename T, int HD> DEV void many_rows(const PaArgs& a, ManyLds<HD>& s
     // 16 rows plus a scalar base.
     constexpr int NG = KT / 16;
     const int lr = threadIdx.x / CH, lc = 8 * (threadIdx.x % CH);   // row and column of this thread's pieces
-    const int wr = __builtin_amdgcn_readfirstlane(lr) & 16;          // first row of the wave's 16 (RP = 32)
+    const int wr = __builtin_amdgcn_readfirstlane(lr) >> 4;          // the wave's 16 of a pass of 32 or 64
     const uint32_t lo = (uint32_t)((lr & 15) * (int)a.p.row_stride + lc);
     const uint16_t* kp = (const uint16_t*)a.p.k + (size_t)kvh * a.p.head_stride;
     const uint16_t* vp = (const uint16_t*)a.p.v + (size_t)kvh * a.p.head_stride;
@@ -412,8 +417,10 @@ template <typename T, int HD> DEV void many_rows(const PaArgs& a, ManyLds<HD>& s
         for (int g = 0; g < NG; g++) bad2 |= ((unsigned)pn[g] >= (unsigned)a.p.n_pages) << g;
 #pragma unroll
         for (int u = 0; u < NP; u++) {
-            const int g = RP == 32 ? 2 * u + (wr >> 4) : u * RP / 16;
-            int pg = RP == 32 ? (wr ? pn[(2 * u + 1) % NG] : pn[2 * u % NG]) : pn[u * RP / 16 % NG];
+            const int g = u * RP / 16 + (RP > 16 ? wr : 0);
+            int pg = pn[u * RP / 16 % NG];
+#pragma unroll
+            for (int e = 1; e < RP / 16; e++) pg = wr == e ? pn[(u * RP / 16 + e) % NG] : pg;
             if ((bad2 >> g) & 1) pg = 0;
             const size_t at = (size_t)pg * a.p.page_stride +
                               (size_t)((base + 16 * g) & (a.p.page_size - 1)) * a.p.row_stride +
@@ -551,7 +558,11 @@ template <typename T, int HD> __global__ __launch_bounds__(256, HD == 256 ? 1 : 
 }
 template <typename T, int HD> __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void k_pa_many(PaArgs a) {
     __shared__ __align__(16) ManyLds<HD> sh;
-    many_rows<T, HD>(a, sh, blockIdx.x, blockIdx.y, blockIdx.z);
+    many_rows<T, HD, 4>(a, sh, blockIdx.x, blockIdx.y, blockIdx.z);
+}
+template <typename T, int HD> __global__ __launch_bounds__(512, 2) void k_pa_wide(PaArgs a) {
+    __shared__ __align__(16) ManyLds<HD> sh;
+    many_rows<T, HD, 8>(a, sh, blockIdx.x, blockIdx.y, blockIdx.z);
 }
 // Chunks and decoding sequences in one call: the chunks' workgroups, which are
 // bound by arithmetic, first, and beside them those that are bound by memory.
@@ -564,7 +575,7 @@ __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void k_pa_mixed(PaArgs a, i
     if (b < many) {
         const int kvh = b % nkv;
         b /= nkv;
-        many_rows<T, HD>(a, *(ManyLds<HD>*)raw, kvh, b % y_many, b / y_many);
+        many_rows<T, HD, 4>(a, *(ManyLds<HD>*)raw, kvh, b % y_many, b / y_many);
     } else {
         b -= many;
         const int kvh = b % nkv;
@@ -627,13 +638,26 @@ struct PaPlan {
 
 int ceil_div(int64_t a, int64_t b) { return (int)((a + b - 1) / b); }
 
+// Keys per range: about `times` sqrt(ctx), in whole 128.
+int range_of(int64_t ctx, double times) { return ((int)(times * sqrt((double)ctx)) + 127) & ~127; }
+
 // Which kernel takes which sequences.  Row counts are on the device; what the
 // host knows is their sum and the number of sequences.  No more rows than
 // sequences: a decode step (a sequence that has several rows all the same has
 // its tiles done in turn), the few-row kernel alone.  One sequence with more
-// than a tile of rows: the many-row kernel alone.  Otherwise each sequence by
-// its own count: up to `few` packed rows (a tile of 16; two where a single
-// row has more than 16 query heads per kv head) or more.
+// than a tile of rows: the many-row kernel alone, in workgroups of 256 rows
+// where there are at least 384 and 2 048 keys (512 rows of 4 heads over 16 384
+// keys 150 us against 169, 100 rows over 4 096 29 against 32; over 600 keys
+// 19.9 against 17.2).  Otherwise each sequence by its own count: up to `few`
+// packed rows (a tile of 16; two where a single row has more than 16 query
+// heads per kv head) or more.
+//
+// How many ranges the keys are split into: enough to fill the card, but a
+// range costs its workgroup's start and a partial result, so that the best
+// length grows like the square root of the context.  One row of 32 heads, 8
+// kv heads: over 1 500 keys 22 us in ranges of 1 024, 15.5 in 512, 13.4 in
+// 256, 13.7 in 128; over 4 096 23, 18.0, 18.1, 21; over 16 384 28.7, 30, 41,
+// 64; over 300 10.0 in one, 11.8 in two.
 PaPlan plan(const DpufAmdBatch& b, const DpufAmdPages& p, int nq) {
     const int G = nq / p.n_kv_heads;
     PaPlan r;
@@ -641,26 +665,29 @@ PaPlan plan(const DpufAmdBatch& b, const DpufAmdPages& p, int nq) {
     const int64_t cap = (int64_t)b.table_stride * p.page_size;
     const int64_t ctx = b.max_ctx < 1 ? 1 : b.max_ctx < cap ? b.max_ctx : cap;
     const int64_t packed = (int64_t)b.n_rows * G;
-    r.only = b.n_rows <= b.n_seqs || packed <= r.few ? PA_FEW : b.n_seqs == 1 ? PA_MANY : PA_BOTH;
+    r.only = b.n_rows <= b.n_seqs || packed <= r.few ? PA_FEW : b.n_seqs > 1 ? PA_BOTH
+             : packed >= 384 && ctx >= 2048 && p.head_dim <= 128 ? PA_WIDE : PA_MANY;
+    const int tr = r.only == PA_WIDE ? 256 : 128;
     const int64_t most = packed / (r.few + 1);
-    r.y_few = r.only == PA_MANY ? 0 : b.n_seqs * ((r.few + 15) / 16);
-    r.y_many = r.only == PA_FEW ? 0 : (int)(packed / 128 + (most < b.n_seqs ? most : b.n_seqs));
-    if (r.only == PA_MANY) r.y_many = ceil_div(packed, 128);
-    r.chunk_few = 512;
+    r.y_few = r.only >= PA_MANY ? 0 : b.n_seqs * ((r.few + 15) / 16);
+    r.y_many = r.only == PA_FEW ? 0 : r.only == PA_BOTH ? (int)(packed / 128 + (most < b.n_seqs ? most : b.n_seqs))
+                                                        : ceil_div(packed, tr);
+    r.chunk_few = ctx <= 512 ? 512 : range_of(ctx, 8.0);
     r.nz_few = ceil_div(ctx, r.chunk_few);
+    if (r.nz_few > 64) r.nz_few = 64;
     // (kv heads x sequences) that fill the card by themselves need no ranges,
     // and the partial sums stay below 16 384 x `few` rows
     const int64_t cap_z = 16384 / ((int64_t)b.n_seqs * p.n_kv_heads);
     if (r.nz_few > cap_z) r.nz_few = cap_z < 1 ? 1 : (int)cap_z;
-    const int64_t wgs = (packed + 127) / 128 * p.n_kv_heads;
-    int nz = wgs >= 512 ? 1 : ceil_div(512, wgs > 0 ? wgs : 1);
-    if (nz > 16) nz = 16;
-    r.chunk_many = ceil_div(ctx, nz);
-    if (r.chunk_many < 512) r.chunk_many = 512;
-    r.chunk_many = (r.chunk_many + 127) & ~127;
+    // as many ranges of a chunk's keys as fit on the card beside its tiles at
+    // once: two workgroups of 128 rows a CU, or one of 256
+    const int64_t wgs = (packed + tr - 1) / tr * p.n_kv_heads, room = r.only == PA_WIDE ? 256 : 512;
+    const int64_t nz = wgs >= room ? 1 : room / (wgs > 0 ? wgs : 1);
+    r.chunk_many = (ceil_div(ctx, nz) + 127) & ~127;
+    if (r.chunk_many < range_of(ctx, 4.0)) r.chunk_many = range_of(ctx, 4.0);
     r.nz_many = ceil_div(ctx, r.chunk_many);
     const size_t all = (size_t)b.n_rows * nq, some = (size_t)b.n_seqs * p.n_kv_heads * r.few;
-    r.few_rows = r.only != PA_MANY && r.nz_few > 1 ? r.nz_few * (r.only == PA_FEW ? all : some) : 0;
+    r.few_rows = r.only <= PA_FEW && r.nz_few > 1 ? r.nz_few * (r.only == PA_FEW ? all : some) : 0;
     r.many_rows = r.only != PA_FEW && r.nz_many > 1 ? r.nz_many * all : 0;
     return r;
 }
@@ -672,7 +699,10 @@ void launch(const PaArgs& a, const PaPlan& pl, hipStream_t st) {
         hipLaunchKernelGGL((k_pa_few<T, HD>), dim3(nkv, pl.y_few, pl.nz_few), dim3(256), 0, st, a);
     else if (pl.only == PA_MANY)
         hipLaunchKernelGGL((k_pa_many<T, HD>), dim3(nkv, pl.y_many, pl.nz_many), dim3(256), 0, st, a);
-    else
+    else if (pl.only == PA_WIDE) {
+        if constexpr (HD <= 128)
+            hipLaunchKernelGGL((k_pa_wide<T, HD>), dim3(nkv, pl.y_many, pl.nz_many), dim3(512), 0, st, a);
+    } else
         hipLaunchKernelGGL((k_pa_mixed<T, HD>), dim3(nkv * (pl.y_many * pl.nz_many + pl.y_few * pl.nz_few)), dim3(256),
                            0, st, a, pl.y_many, pl.y_few);
     if (pl.few_rows + pl.many_rows > 0)
