@@ -19,6 +19,7 @@ typedef s16x4 __attribute__((address_space(3))) * lds_s16x4;
 // The two 16-bit element types: vectors of 8 (one matrix operand) and the
 // matrix instructions with fp32 sums.
 struct Bf16 {
+    static constexpr uint32_t EXP = 0x7f80;     // exponent bits
     typedef __bf16 e;
     typedef __bf16 v8 __attribute__((ext_vector_type(8)));
     typedef __bf16 v4 __attribute__((ext_vector_type(4)));
@@ -27,6 +28,7 @@ struct Bf16 {
     static DEV f32x16 mma32(v8 a, v8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
 };
 struct Fp16 {
+    static constexpr uint32_t EXP = 0x7c00;
     typedef _Float16 e;
     typedef _Float16 v8 __attribute__((ext_vector_type(8)));
     typedef _Float16 v4 __attribute__((ext_vector_type(4)));

@@ -86,7 +86,31 @@ DEV void put4(const PaArgs& a, size_t at, const float* o, float inv) {
     }
 }
 
-DEV float lse_of(float m2, float l) { return l > 0.0f ? (m2 + __log2f(l)) * 0.69314718055994531f : NEG_INF; }
+DEV float lse_of(float m2, float l) { return l == 0.0f ? NEG_INF : (m2 + __log2f(l)) * 0.69314718055994531f; }
+
+// Infinities and NaN in V.  A row that does not see a key has p = 0 there, and
+// 0 * inf would reach its sums all the same.  So in a tile that some row does
+// not see whole they are taken out of V on its way to LDS, and, if there were
+// any, added at the end to the rows that see them.
+template <typename T> DEV uint32_t odd_mask(uint32_t e) {     // the halves of e that are infinite or NaN
+    return ((e & T::EXP) == T::EXP ? 0xffffu : 0u) | (((e >> 16) & T::EXP) == T::EXP ? 0xffff0000u : 0u);
+}
+template <typename T> DEV uint32_t take_odd(u32x4& v) {
+    uint32_t any = 0;
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        const uint32_t m = odd_mask<T>(v[i]);
+        any |= m;
+        v[i] &= ~m;
+    }
+    return any;
+}
+// The infinities and NaN of the four elements at v, 0 for the others.
+template <typename T> DEV f32x4 odd4(const uint16_t* v) {
+    const uint2 w = *(const uint2*)v;
+    return __builtin_convertvector(
+        __builtin_bit_cast(typename T::v4, make_uint2(w.x & odd_mask<T>(w.x), w.y & odd_mask<T>(w.y))), f32x4);
+}
 
 // ---------------------------------------------------------------------------
 // Few rows (decode): bound by reading K and V once.  One workgroup per
@@ -99,6 +123,7 @@ template <int HD> struct FewLds {
     static constexpr int PITCH = HD + 16;   // elements of a V row: 4 rows of a transposing read in 4 bank groups
     uint16_t v[4][32 * PITCH];
     float2 ml[4][16];
+    int odd[4];
 };
 
 template <typename T, int HD> DEV void few_rows(const PaArgs& a, FewLds<HD>& sh, int kvh, int y, int z) {
@@ -168,6 +193,11 @@ template <typename T, int HD> DEV void few_rows(const PaArgs& a, FewLds<HD>& sh,
             }
         };
 
+        auto whole_at = [&](int base, const int* pid) {
+            return base + 32 <= min(kend, first_limit + 1) && (unsigned)pid[0] < (unsigned)a.p.n_pages &&
+                   (unsigned)pid[1] < (unsigned)a.p.n_pages;
+        };
+        uint32_t odd = 0;
         int base = k0 + 32 * wave;
         if (base < kend) {
             pages(base, pg);
@@ -177,22 +207,20 @@ template <typename T, int HD> DEV void few_rows(const PaArgs& a, FewLds<HD>& sh,
         for (; base < kend; base += 128) {
             // V goes to LDS for the transposing reads; the wave's own LDS
             // operations are in order, so nothing but the compiler has to be held
-            const bool whole = base + 32 <= min(kend, first_limit + 1) && (unsigned)pg[0] < (unsigned)a.p.n_pages &&
-                               (unsigned)pg[1] < (unsigned)a.p.n_pages;
-            if (!whole) {
-                // a V row that no row of the tile sees may hold anything: 0 * inf
-                // and 0 * NaN would reach the sums
-#pragma unroll
-                for (int u = 0; u < 2; u++)
-                    if (base + 16 * u + col >= kend || (unsigned)pg[u] >= (unsigned)a.p.n_pages)
-#pragma unroll
-                        for (int c = 0; c < NC; c++) vf[u][c] = u32x4{0, 0, 0, 0};
-            }
+            const bool whole = whole_at(base, pg);
             lds_order();
 #pragma unroll
             for (int u = 0; u < 2; u++)
 #pragma unroll
                 for (int c = 0; c < NC; c++) *(u32x4*)(lv + (16 * u + col) * PITCH + 32 * c + 8 * g4) = vf[u][c];
+            if (!whole)
+#pragma unroll 1
+                for (int e = 0; e < 2 * NC; e++) {
+                    u32x4* at = (u32x4*)(lv + (e / NC * 16 + col) * PITCH + 32 * (e % NC) + 8 * g4);
+                    u32x4 v = *at;
+                    odd |= take_odd<T>(v);
+                    *at = v;
+                }
             f32x4 sc[2] = {f32x4{0.f, 0.f, 0.f, 0.f}, f32x4{0.f, 0.f, 0.f, 0.f}};
 #pragma unroll
             for (int c = 0; c < NC; c++)
@@ -250,7 +278,10 @@ template <typename T, int HD> DEV void few_rows(const PaArgs& a, FewLds<HD>& sh,
         // join the four waves: m, l of the 16 rows, then O by output column
         l = add_xor32(add_xor16(l));
         if (lane < 16) sh.ml[wave][lane] = make_float2(m, l);
+        const bool my_odd = __any(odd != 0);
+        if (lane == 0) sh.odd[wave] = my_odd;
         __syncthreads();
+        const bool some_odd = sh.odd[0] | sh.odd[1] | sh.odd[2] | sh.odd[3];
         float M = NEG_INF, L = 0.0f;
 #pragma unroll
         for (int w = 0; w < 4; w++) M = fmaxf(M, sh.ml[w][col].x);
@@ -279,6 +310,20 @@ template <typename T, int HD> DEV void few_rows(const PaArgs& a, FewLds<HD>& sh,
 #pragma unroll
                     for (int w = 1; w < 4; w++) v += *(const f32x4*)(lo + w * WS + rr * OP + d4);
                     const int i = pr / a.G;
+                    if (some_odd)
+                        for (int t0 = k0; t0 < kend; t0 += 32) {
+                            int pid[2];
+                            pages(t0, pid);
+                            if (whole_at(t0, pid)) continue;
+                            for (int t = t0; t < t0 + 32 && t <= sq.ctx - sq.n + i; t++) {
+                                const int p = pid[(t >> 4) & 1];
+                                if ((unsigned)p < (unsigned)a.p.n_pages)
+                                    v += odd4<T>((const uint16_t*)a.p.v + (size_t)kvh * a.p.head_stride +
+                                                 (size_t)p * a.p.page_stride +
+                                                 (size_t)(t & (a.p.page_size - 1)) * a.p.row_stride +
+                                                 hf * (HD / 2) + d4);
+                            }
+                        }
                     const size_t orow = (size_t)(sq.r0 + i) * a.nq + kvh * a.G + (pr - i * a.G);
                     const int d = hf * (HD / 2) + d4;
                     if (ranges > 1) {
@@ -319,6 +364,7 @@ template <int HD> struct ManyLds {
     static constexpr int VP = HD + 32;   // V row: 4 rows' 64 bytes in distinct banks
     uint16_t k[2][KT * KP];
     uint16_t v[2][KT * VP];
+    int odd;
 };
 
 template <typename T, int HD, int WAVES>
@@ -406,6 +452,8 @@ DEV void many_rows(const PaArgs& a, ManyLds<HD>& sh, int kvh, int tile, int z) {
     const int top = sq.ctx > 0 ? (sq.ctx - 1) >> a.shift : 0;
     u32x4 kf[NP], vf[NP];
     int pn[NG];              // pages of the tile to be loaded next
+    uint32_t odd = 0;
+    const int seen = min(kend, sq.ctx - sq.n + TR * tile / a.G + 1);     // keys before it: by all rows
     uint32_t bad1 = 0, bad2 = 0;   // of the tile in kf / vf (one bit per 16 keys: outside the pool), and of the next
     auto pages = [&](int base) {
 #pragma unroll
@@ -428,14 +476,9 @@ DEV void many_rows(const PaArgs& a, ManyLds<HD>& sh, int kvh, int tile, int z) {
             kf[u] = *(const u32x4*)(kp + at + lo);
             vf[u] = *(const u32x4*)(vp + at + lo);
         }
-        if (bad2 || base + KT > kend) {
-            // rows that nobody sees: any bits, and 0 * NaN is NaN
+        if (bad2 || base + KT > seen)
 #pragma unroll
-            for (int u = 0; u < NP; u++) {
-                const int key = u * RP + lr;
-                if (base + key >= kend || ((bad2 >> (key >> 4)) & 1)) vf[u] = u32x4{0, 0, 0, 0};
-            }
-        }
+            for (int u = 0; u < NP; u++) odd |= take_odd<T>(vf[u]);
     };
     auto store = [&](int buf) {
 #pragma unroll
@@ -445,6 +488,7 @@ DEV void many_rows(const PaArgs& a, ManyLds<HD>& sh, int kvh, int tile, int z) {
         }
     };
 
+    if (threadIdx.x == 0) sh.odd = 0;
     if (k0 < kend) {
         pages(k0);
         load(k0);
@@ -525,6 +569,31 @@ DEV void many_rows(const PaArgs& a, ManyLds<HD>& sh, int kvh, int tile, int z) {
                 }
             }
     }
+    __syncthreads();
+    if (__any(odd != 0) && lane == 0) sh.odd = 1;
+    __syncthreads();
+    if (sh.odd)
+        for (int base = k0; base < kend; base += 16) {
+            const int pg = table[min(base >> a.shift, top)], t0 = base & ~(KT - 1);
+            if ((unsigned)pg >= (unsigned)a.p.n_pages) continue;
+            bool whole = t0 + KT <= seen;
+            for (int g = 0; g < NG; g++)
+                whole = whole && (unsigned)table[min((t0 + 16 * g) >> a.shift, top)] < (unsigned)a.p.n_pages;
+            if (whole) continue;
+#pragma unroll 1
+            for (int key = base; key < base + 16; key++) {
+                const uint16_t* v = vp + (size_t)pg * a.p.page_stride +
+                                    (size_t)(key & (a.p.page_size - 1)) * a.p.row_stride + 4 * h;
+#pragma unroll
+                for (int d = 0; d < ND; d++)
+#pragma unroll
+                    for (int i = 0; i < 16; i += 4) {
+                        const f32x4 x = odd4<T>(v + 32 * d + 2 * i);
+#pragma unroll
+                        for (int e = 0; e < 4; e++) o[d][i + e] += key <= limit ? x[e] : 0.0f;
+                    }
+            }
+        }
     l = add_xor32(l);
     if (!live) return;
     // o[d][i]: column 32 d + 8 (i / 4) + 4 h + i % 4
@@ -552,7 +621,7 @@ DEV void many_rows(const PaArgs& a, ManyLds<HD>& sh, int kvh, int tile, int z) {
 // Blocks of the three kernels: kv heads fastest, so that the workgroups that
 // read the same keys run on the same XCDs (8 kv heads: one XCD each) and share
 // their L2.
-template <typename T, int HD> __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void k_pa_few(PaArgs a) {
+template <typename T, int HD> __global__ __launch_bounds__(256, HD == 256 ? 1 : 3) void k_pa_few(PaArgs a) {
     __shared__ __align__(16) FewLds<HD> sh;
     few_rows<T, HD>(a, sh, blockIdx.x, blockIdx.y, blockIdx.z);
 }

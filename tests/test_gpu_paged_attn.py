@@ -168,6 +168,72 @@ def test_weights(eng, hip, nq, nkv, hd, page, t):
                 assert np.array_equal(got[pg, :, r], cache.w[pg, :, r] * np.float32(decay))
 
 
+# Every kernel and split of the keys: (rows, contexts, max_ctx given).  No more rows than sequences, with a sequence
+# that has most of them; one sequence with fewer and more than 384 packed rows (4 heads a kv head), short and long;
+# chunks beside decoding sequences.
+MODES = {
+    "few, split": ([0, 5, 0, 1, 0, 0], [40, 1300, 1, 700, 0, 9], None),
+    "few, one row": ([1], [2111], None),
+    "many": ([40], [95], None),
+    "many, split": ([33], [1500], None),
+    "wide, short keys": ([150], [333], 5000),
+    "wide, split": ([97], [2300], None),
+    "wide, few rows of them": ([0], [50], 4096),
+    "mixed, split": ([1, 70, 2, 0, 1, 30], [1900, 1400, 600, 7, 33, 30], None),
+}
+
+
+@pytest.mark.parametrize("hd", [64, 128, 256])
+@pytest.mark.parametrize("mode", MODES)
+def test_kernels_and_splits(eng, hip, mode, hd):
+    """... and device row counts below n_rows: the rows behind stay."""
+    rows, ctx, max_ctx = MODES[mode]
+    rng = np.random.default_rng(len(mode) + hd)
+    t = R.F16 if hd == 64 else R.BF16
+    cache = R.Cache(hip, rng, t, rows, ctx, 2, hd, 32, slots_first=hd == 128, table_extra=160)
+    q = R.to_type(rng.standard_normal((cache.n_rows, 8, hd)) * 1.5, t)
+    extra = 100 if mode == "wide, few rows of them" else 0
+    say(f"{mode}: hd {hd}")
+    out, lse, *_ = call(eng, hip, cache, 8, q, 0.1, max_ctx=max_ctx, extra=extra)
+    check(cache, 8, q, 0.1, out, lse, t)
+
+
+@pytest.mark.parametrize("t", [R.BF16, R.F16])
+@pytest.mark.parametrize("hd", [64, 128, 256])
+@pytest.mark.parametrize("mode", [m for m in MODES if m not in ("few, one row", "wide, few rows of them")])
+def test_infinities_and_nan_that_a_row_does_not_see(eng, hip, mode, hd, t):
+    """K and V rows of new tokens hold infinities and NaN: the rows before
+    them, which do not see them, keep their values; those that do see them get
+    what the definition gives."""
+    rows, ctx, max_ctx = MODES[mode]
+    rng = np.random.default_rng(2 * len(mode) + hd)
+    nq, page = 8, 16
+    cache = R.Cache(hip, rng, t, rows, ctx, 2, hd, page, table_extra=320)
+    for s, (n, c) in enumerate(zip(rows, ctx)):
+        for i in range(max(1, c - n + 1), c):
+            pg, r = cache.table[s, i // page], i % page
+            for h in range(2):
+                at = rng.integers(0, hd, 3)
+                cache.v[pg, h, r, at] = R.to_type([np.inf, -np.inf, np.nan], t)[rng.integers(0, 3, 3)]
+        if n > 1:       # the last token's key: only the last row sees it
+            cache.k[cache.table[s, (c - 1) // page], 1, (c - 1) % page, 3] = R.to_type([np.nan], t)[0]
+    cache.dv.set(cache.v)
+    cache.dk.set(cache.k)
+    q = R.to_type(rng.standard_normal((cache.n_rows, nq, hd)), t)
+    say(f"odd values, {mode}: hd {hd}, type {t}")
+    out, lse, *_ = call(eng, hip, cache, nq, q, 0.1, max_ctx=max_ctx)
+    with np.errstate(all="ignore"):
+        ref, rl, A, S, _, _ = R.attention(cache, R.from_type(q, t), 0.1, nq)
+        # the values themselves are below 10 (standard normal)
+        bound = R.attention_bound(t, t, ref, A, S, np.full(S.shape, 10.0), hd, max(ctx))
+        assert np.array_equal(np.isnan(out), np.isnan(ref))
+        assert np.array_equal(np.isposinf(out), np.isposinf(ref)) and np.array_equal(np.isneginf(out), np.isneginf(ref))
+        ok = np.isfinite(ref)
+        assert ok.any() and not ok.all()
+        assert np.all(np.abs(out[ok] - ref[ok]) <= bound[ok])
+        assert np.array_equal(np.isnan(lse), np.isnan(rl)) and np.array_equal(np.isneginf(lse), np.isneginf(rl))
+
+
 def test_two_streams_and_a_graph(eng, hip):
     """Two calls at once on streams of their own with workspaces of their own;
     then a captured call replayed over new lengths and values between eager
