@@ -20,10 +20,10 @@
 //               workgroup that ends last adds the chunks' bins up, groups of
 //               16 first, and finds the bins in which the prefixes end;
 //   k_smp_pick  collects the tokens that decide: all of the prefix's where
-//               they fit, else those of the bins the borders lie in; the
-//               workgroup that ends last finds the borders among them by
-//               radix selection and draws, from the list or, in index order,
-//               from the chunk in which the running sum passes the draw.
+//               they are at most one a thread, else those of the bins the
+//               borders lie in; the workgroup that ends last finds the borders
+//               among them and draws, from the list or, in index order, from
+//               the chunk in which the running sum passes the draw.
 // Rows whose border bin alone holds more tokens than the list (long runs of
 // equal logits) are left to one workgroup that splits the bin further.
 //
@@ -383,14 +383,14 @@ struct HistShared {
 };
 
 // What a prefix search looks for: the first `count` tokens, or the shortest
-// prefix whose weights reach `goal`, or whose sum passes `count`.
-enum { BY_COUNT, BY_GOAL, BY_SUM };
+// prefix whose weights reach `goal`.
+enum { BY_COUNT, BY_GOAL };
 struct Want {
     int by;
     uint64_t count;
     double goal;
     DEV bool met(uint64_t n, uint64_t w) const {
-        return by == BY_COUNT ? n >= count : by == BY_GOAL ? (double)w >= goal : w > count;
+        return by == BY_COUNT ? n >= count : (double)w >= goal;
     }
 };
 
@@ -505,7 +505,7 @@ template <typename L> DEV void find_borders(const SmArgs& a, HistShared& sh, con
         st->wk = k.w;
         st->wp = p0.w;
         st->total = tw;
-        st->mode = upto <= CAP ? SM_LIST : in_s <= CAP ? SM_BINS : SM_SPLIT;
+        st->mode = upto <= NT ? SM_LIST : in_s <= CAP ? SM_BINS : SM_SPLIT;
     }
 }
 
@@ -621,9 +621,16 @@ template <typename L> __global__ __launch_bounds__(NT) void k_smp_hist(SmArgs a)
 
 // ---------------------------------------------------------------------------
 struct PickShared {
-    uint64_t list[CAP], lw[CAP];
-    unsigned long long wsum[NB];
-    uint32_t count[NB];
+    uint64_t list[CAP];
+    union {
+        uint64_t lw[CAP];        // the list's weights
+        struct {                 // split_cut's bins: before there is a list
+            unsigned long long wsum[NB];
+            uint32_t count[NB];
+        } bins;
+    };
+    unsigned long long wsum[NT];
+    uint32_t count[NT];
     uint64_t red[2 * NW];
     double table[16];
     uint64_t b0, b1;
@@ -774,8 +781,8 @@ DEV bool find_bin(PickShared& sh, const Want& want, uint64_t n0, uint64_t w0, in
     uint64_t c = 0, w = 0;
 #pragma unroll
     for (int e = 0; e < PER; e++) {
-        c += sh.count[PER * t + e];
-        w += sh.wsum[PER * t + e];
+        c += sh.bins.count[PER * t + e];
+        w += sh.bins.wsum[PER * t + e];
     }
     uint64_t n = c, s = w;
     scan64x2(sh.red, n, s);
@@ -786,7 +793,7 @@ DEV bool find_bin(PickShared& sh, const Want& want, uint64_t n0, uint64_t w0, in
 #pragma unroll
     for (int e = 0; e < PER; e++) {
         const int b = PER * t + e;
-        const uint64_t n1 = n + sh.count[b], s1 = s + sh.wsum[b];
+        const uint64_t n1 = n + sh.bins.count[b], s1 = s + sh.bins.wsum[b];
         if (want.met(n1, s1) && !want.met(n, s)) {
             sh.i0 = b;
             sh.b0 = n;
@@ -814,22 +821,22 @@ DEV uint64_t split_cut(PickShared& sh, const Row<L>& row, const Want& want, uint
         while (((hi - lo) >> sf) >= NB) sf++;
         __syncthreads();
         for (int b = t; b < NB; b += NT) {
-            sh.count[b] = 0;
-            sh.wsum[b] = 0;
+            sh.bins.count[b] = 0;
+            sh.bins.wsum[b] = 0;
         }
         __syncthreads();
         each<L>(row.p, row.vec, 0, row.V, [&](int i, float x) {
             const uint64_t w = row.weight(row.below(x)), c = comp_of(x, i);
             if (w && c >= lo && c <= hi) {
-                atomicAdd(&sh.count[(hi - c) >> sf], 1u);
-                atomicAdd(&sh.wsum[(hi - c) >> sf], (unsigned long long)w);
+                atomicAdd(&sh.bins.count[(hi - c) >> sf], 1u);
+                atomicAdd(&sh.bins.wsum[(hi - c) >> sf], (unsigned long long)w);
             }
         });
         __syncthreads();
         int b;
         uint64_t n1, w1;
         if (!find_bin(sh, want, bn, bw, &b, &n1, &w1)) break;     // all of them: only at the first turn
-        const uint32_t in = sh.count[b];
+        const uint32_t in = sh.bins.count[b];
         bn = n1;
         bw = w1;
         hi -= (uint64_t)b << sf;
@@ -871,6 +878,52 @@ template <typename L> DEV void split_row(const SmArgs& a, PickShared& sh, const 
     each<L>(row.p, row.vec, 0, row.V, [&](int i, float x) { own += kept(i, x); });
     scan64(sh.red, own, &total);
     draw_range(a, sh, row, r, 0, row.V, 0, aim_of(a.u[r], total), total, kept);
+}
+
+// A list of at most a token a thread needs no selection: each thread adds up
+// what lies above its token and then what lies before it in two passes over
+// the list, which are shorter than selection's barriers (50 tokens of one row
+// of 151 936: 11.8 us for the launch against 14; up to a list's full length
+// selection, and then the draw from a chunk by bins, is the shorter: top-p 0.9
+// of one row 19.5 us against 28.9).
+template <typename L>
+DEV void answer_few(const SmArgs& a, PickShared& sh, const Row<L>& row, const SmState& st, int r, int n) {
+    const int t = threadIdx.x;
+    const uint64_t c = t < n ? sh.list[t] : 0, w = t < n ? sh.lw[t] : 0;
+    unsigned above = 0;
+    uint64_t before = 0;
+#pragma unroll 8
+    for (int j = 0; j < n; j++) {
+        const bool up = sh.list[j] > c;
+        above += up;
+        before += up ? sh.lw[j] : 0;
+    }
+    if (t == 0) {
+        sh.b0 = sh.b1 = 0;
+        sh.red[0] = st.total;
+    }
+    __syncthreads();
+    if (st.by_k && t < n && above == (unsigned)row.k - 1) {
+        sh.b0 = c;
+        sh.red[0] = before + w;
+    }
+    __syncthreads();
+    const double goal = row.goal(sh.red[0]);
+    if (st.by_p && t < n && (double)before < goal && (double)(before + w) >= goal) sh.b1 = c;
+    __syncthreads();
+    const uint64_t cut = sh.b1 > sh.b0 ? sh.b1 : sh.b0;
+    const uint64_t left = c >= cut && t < n && row.weight_min(logit_of(c)) ? w : 0;
+    if (t < n) sh.lw[t] = left;
+    __syncthreads();
+    uint64_t total = 0;
+    before = 0;
+#pragma unroll 8
+    for (int j = 0; j < n; j++) {
+        total += sh.lw[j];
+        before += (uint32_t)sh.list[j] > (uint32_t)c ? sh.lw[j] : 0;     // a lower index
+    }
+    const uint64_t aim = aim_of(a.u[r], total);
+    if (before <= aim && aim < before + left) answer(a, row, r, index_of(c), logit_of(c), total);
 }
 
 template <typename L> __global__ __launch_bounds__(NT) void k_smp_pick(SmArgs a) {
@@ -960,57 +1013,57 @@ template <typename L> __global__ __launch_bounds__(NT) void k_smp_pick(SmArgs a)
     __syncthreads();
     for (int i = t; i < n; i += NT) sh.lw[i] = row.weight_of(sh.list[i]);
     __syncthreads();
+    if (mode == SM_LIST) {
+        answer_few(a, sh, row, st, r, n);
+        return;
+    }
     auto comp = [&](int i) { return sh.list[i]; };
     auto bin_of = [&](int i) { return row.bin_of(sh.list[i]); };
     uint64_t sum = st.total, cut = 0;      // composites below cut are out
     if (st.by_k) {
-        const int at = mode == SM_LIST
-                           ? select(sh, n, Want{BY_COUNT, (uint64_t)row.k, 0.0}, 0, 0, comp, [](int) { return true; }, &sum)
-                           : select(sh, n, Want{BY_COUNT, st.rk, 0.0}, 0, st.wk, comp,
-                                    [&](int i) { return bin_of(i) == st.bk; }, &sum);
+        const int at = select(sh, n, Want{BY_COUNT, st.rk, 0.0}, 0, st.wk, comp,
+                              [&](int i) { return bin_of(i) == st.bk; }, &sum);
         if (at >= 0) cut = sh.list[at];
     }
     if (st.by_p) {
-        const Want want = {BY_GOAL, 0, row.goal(sum)};
         uint64_t s;
-        const int at = mode == SM_LIST ? select(sh, n, want, 0, 0, comp, [](int) { return true; }, &s)
-                                       : select(sh, n, want, 0, st.wp, comp,
-                                                [&](int i) {
-                                                    const int b = bin_of(i);
-                                                    return b >= st.pl && b <= st.ph;
-                                                },
-                                                &s);
+        const int at = select(sh, n, Want{BY_GOAL, 0, row.goal(sum)}, 0, st.wp, comp,
+                              [&](int i) {
+                                  const int b = bin_of(i);
+                                  return b >= st.pl && b <= st.ph;
+                              },
+                              &s);
         if (at >= 0 && sh.list[at] > cut) cut = sh.list[at];
     }
     // what stays of the list
     for (int i = t; i < n; i += NT)
         if (sh.list[i] < cut || row.weight_min(logit_of(sh.list[i])) == 0) sh.lw[i] = 0;
     __syncthreads();
-    if (mode == SM_LIST) {
-        uint64_t own = 0, total;
-        for (int i = t; i < n; i += NT) own += sh.lw[i];
-        scan64(sh.red, own, &total);
-        const int at = select(sh, n, Want{BY_SUM, aim_of(a.u[r], total), 0.0}, 0, 0,
-                              [&](int i) { return sh.list[i] & 0xffffffffull; }, [](int) { return true; }, &sum);
-        if (t == 0 && at >= 0) answer(a, row, r, index_of(sh.list[at]), logit_of(sh.list[at]), total);
-        return;
-    }
     // the chunks' sums: the bins above the highest border, and what stays of
     // the list from there on
     const int cb = min(cut ? row.bin_of(cut) : NB, st.by_m ? st.ml : NB), g = cb / GB;
-    if (t < MAX_CHUNKS) sh.wsum[t] = 0;
-    __syncthreads();
-    for (int k = wave; k < a.chunks; k += NW) {
-        const size_t at = (size_t)r * a.chunks + k;
-        uint64_t s = 0;
-        if (a.chunks == 1) {
-            for (int b = lane; b < cb; b += 64) s += a.wsum[at * NB + b];
-        } else {
-            if (lane < g) s = get_agent(a.gsum + 2 * (at * NG + lane));
-            if (lane < cb - g * GB) s += get_agent(a.wsum + at * NB + g * GB + lane);
+    // (a chunk a wave, eight chunks' loads at a time)
+    for (int k0 = wave; k0 < MAX_CHUNKS; k0 += 8 * NW) {
+        uint64_t s[8];
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+            const size_t at = (size_t)r * a.chunks + min(k0 + e * NW, a.chunks - 1);
+            s[e] = 0;
+            if (a.chunks == 1) {
+                if (k0 + e == 0)
+                    for (int b = lane; b < cb; b += 64) s[e] += a.wsum[at * NB + b];
+            } else {
+                if (lane < g) s[e] = get_agent(a.gsum + 2 * (at * NG + lane));
+                if (lane < cb - g * GB) s[e] += get_agent(a.wsum + at * NB + g * GB + lane);
+            }
         }
-        if (s) atomicAdd(&sh.wsum[k], (unsigned long long)s);
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+            s[e] = wave_scan64(s[e]);
+            if (lane == 63) sh.wsum[k0 + e * NW] = k0 + e * NW < a.chunks ? s[e] : 0;
+        }
     }
+    __syncthreads();
     for (int i = t; i < n; i += NT)
         if (sh.lw[i] && bin_of(i) >= cb)
             atomicAdd(&sh.wsum[index_of(sh.list[i]) / a.chunk], (unsigned long long)sh.lw[i]);
