@@ -1531,6 +1531,7 @@ DPUF_EXPORT int32_t dpuf_amd_engine_pages_create(void* handle, int32_t n_pages, 
     }
     if (type != DPUF_AMD_BF16 && type != DPUF_AMD_F16) return -5;
     if (page_size < 16 || page_size > 1024 || (page_size & (page_size - 1))) return -2;
+    if (n_pages > (1 << 30) / page_size) return -2;
     DpufAmdRopeSpec spec;
     memset(&spec, 0, sizeof spec);
     const DpufModelConfig* c = &e->cfg;

@@ -175,6 +175,10 @@ DPUF_EXPORT int32_t dpuf_amd_paged_attn(const DpufAmdBatch* batch, const DpufAmd
     const size_t ws = dpuf_hip_paged_attn_workspace(batch, pages, n_q_heads);
     if (ws > 0 && !aligned(d_workspace, 16)) return -1;
     if (workspace_bytes < ws) return -7;
+    const uint64_t nl = (uint64_t)batch->n_rows * (uint64_t)n_q_heads * 4u, no = n * (uint64_t)type_size(out_type);
+    if (overlap(d_lse, nl, d_q, n * 2u) || overlap(d_lse, nl, d_out, no) || overlap(d_workspace, ws, d_q, n * 2u) ||
+        overlap(d_workspace, ws, d_out, no) || overlap(d_workspace, ws, d_lse, nl))
+        return -1;
     const void* ps[] = {pages->k, pages->v, batch->row_start, batch->ctx_len, batch->page_table, d_q, d_out, d_lse,
                         ws > 0 ? d_workspace : NULL};
     const int32_t dev = device_of(ps, (int)(sizeof ps / sizeof ps[0]));
@@ -196,6 +200,8 @@ DPUF_EXPORT int32_t dpuf_amd_paged_attn_weights(const DpufAmdBatch* batch, const
     if (batch->n_rows > 0 && (!aligned(d_q, 16) || !aligned(d_lse, 4))) return -1;
     const uint64_t n = (uint64_t)pages->n_pages * (uint64_t)pages->n_kv_heads * (uint64_t)pages->page_size * 4u;
     if (d_w_in != pages->w && overlap(d_w_in, n, pages->w, n)) return -1;
+    const uint64_t nl = (uint64_t)batch->n_rows * (uint64_t)n_q_heads * 4u;
+    if (overlap(d_lse, nl, pages->w, n)) return -1;
     const void* ps[] = {pages->k, pages->w, batch->row_start, batch->ctx_len, batch->page_table, d_w_in,
                         batch->n_rows > 0 ? d_q : NULL, batch->n_rows > 0 ? (const void*)d_lse : NULL};
     const int32_t dev = device_of(ps, (int)(sizeof ps / sizeof ps[0]));
@@ -268,6 +274,11 @@ DPUF_EXPORT int32_t dpuf_amd_sample(int32_t type, int32_t n, int32_t V, int64_t 
     const size_t ws = dpuf_hip_sample_workspace(n, V);
     if (ws > 0 && !aligned(d_workspace, 16)) return -1;
     if (workspace_bytes < ws) return -7;
+    if (overlap(d_workspace, ws, d_logits, nx) || overlap(d_workspace, ws, d_tokens, nb) ||
+        overlap(d_workspace, ws, d_logprobs, nb))
+        return -1;
+    for (int i = 0; i < 5; i++)
+        if (overlap(d_workspace, ws, in[i], nb)) return -1;
     const void* ps[] = {d_logits, d_temperature, d_top_k, d_top_p, d_min_p, d_u, d_tokens, d_logprobs,
                         ws > 0 ? d_workspace : NULL};
     const int32_t dev = device_of(ps, (int)(sizeof ps / sizeof ps[0]));

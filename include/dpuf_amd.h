@@ -179,8 +179,9 @@ enum {
 /* One layer's pages.  Row r of page p of kv head h starts at element
  * p * page_stride + h * head_stride + r * row_stride of k and of v (any order
  * of the three, each a multiple of 8 elements and at least head_dim,
- * row_stride at most 2^26; k and v on 16 bytes).  w holds one accumulated weight per row,
- * [n_pages][n_kv_heads][page_size], or is NULL where no operator needs it. */
+ * row_stride at most 2^26; k and v on 16 bytes).  w holds one accumulated
+ * weight per row, [n_pages][n_kv_heads][page_size], or is NULL where no
+ * operator needs it. */
 typedef struct {
     int32_t type;         /* DPUF_AMD_BF16 or DPUF_AMD_F16 */
     int32_t n_pages;
@@ -352,11 +353,11 @@ DPUF_EXPORT int32_t dpuf_amd_engine_forward_slots_sample(void* handle, int32_t n
                                                          const DpufAmdSampling* sampling, float* logits_out,
                                                          int32_t* tokens_out, float* logprobs_out);
 
-/* Gives the engine a KV cache of n_pages pages of page_size rows per layer
- * (type DPUF_AMD_BF16 or DPUF_AMD_F16; 2 x 2 x n_kv_heads x head_dim bytes and
- * 4 x n_kv_heads of weights per row and layer), next to its slots, for
- * dpuf_amd_engine_forward_pages; n_pages 0 frees it.  An earlier one is
- * replaced, its contents lost.  0 ok; -1 NULL handle, -2 a size out of range
+/* Gives the engine a KV cache of n_pages pages of page_size rows (2^30 rows at
+ * most) per layer (type DPUF_AMD_BF16 or DPUF_AMD_F16; 2 x 2 x n_kv_heads x
+ * head_dim bytes and 4 x n_kv_heads of weights per row and layer), next to its
+ * slots, for dpuf_amd_engine_forward_pages; n_pages 0 frees it.  An earlier
+ * one is replaced, its contents lost.  0 ok; -1 NULL handle, -2 a size out of range
  * or out of memory, -5 another type, or a rotation the config does not
  * describe, -6 device error. */
 DPUF_EXPORT int32_t dpuf_amd_engine_pages_create(void* handle, int32_t n_pages, int32_t page_size, int32_t type);

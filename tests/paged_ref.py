@@ -146,6 +146,11 @@ class Cache:
         self.dk, self.dv, self.dw = put(self.k), put(self.v), put(self.w)
         self.d_starts, self.d_ctx, self.d_table = put(self.starts), put(np.array(self.ctx, np.int32)), put(self.table)
 
+    def upload_into(self):
+        """The pools as they were, in the same device memory."""
+        for d, host in ((self.dk, self.k), (self.dv, self.v), (self.dw, self.w)):
+            d.set(host)
+
     def gather(self, pool, s, h):
         """Cached rows of (s, kv head h) in float64, NaN where absent."""
         out = np.full((self.ctx[s], self.hd), np.nan)

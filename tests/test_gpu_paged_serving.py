@@ -1,0 +1,200 @@
+"""The paged-serving operators one after the other, as a serving loop runs
+them: a step captured into a graph, steps on two streams at once, and the
+arguments that may not share memory."""
+import ctypes as C
+
+import numpy as np
+import pytest
+
+import paged_ref as R
+from dpuf_amd import abi
+
+pytestmark = pytest.mark.gpu
+
+NQ, NKV, HD, V, KEEP = 8, 2, 128, 5000, 40
+
+
+@pytest.fixture()
+def hip(eng):
+    h = R.Hip()
+    yield h
+    h.free_all()
+
+
+class Step:
+    """One decode step of a batch, everything on the device: append, attention,
+    weights, eviction into pages of another pool, sampling."""
+
+    def __init__(self, eng, hip, seed, rows, ctx):
+        rng = np.random.default_rng(seed)
+        self.eng, self.hip, self.rng = eng, hip, rng
+        n = len(ctx)
+        self.cache = c = R.Cache(hip, rng, R.BF16, rows, ctx, NKV, HD, 32)
+        self.dst = R.Cache(hip, rng, R.BF16, [0] * n, [KEEP] * n, NKV, HD, 16)
+        self.stream = hip.stream()
+        width = (NQ + 2 * NKV) * HD
+        self.qkv = hip.put(np.zeros((c.n_rows, width), np.float32))
+        self.pos = hip.put(np.zeros(c.n_rows, np.int32))
+        self.q = hip.put(np.zeros((c.n_rows, NQ, HD), np.uint16))
+        self.out = hip.put(np.zeros((c.n_rows, NQ, HD), np.float32))
+        self.lse = hip.put(np.zeros((c.n_rows, NQ), np.float32))
+        self.kept = hip.put(np.zeros((n, NKV, KEEP), np.int32))
+        self.new_len = hip.put(np.zeros(n, np.int32))
+        self.x = hip.put(np.zeros((n, V), np.float32))
+        self.settings = [hip.put(np.zeros(n, t)) for t in (np.float32, np.int32, np.float32, np.float32, np.float32)]
+        self.tok, self.lp = hip.put(np.zeros(n, np.int32)), hip.put(np.zeros(n, np.float32))
+        self.rope = abi.DpufAmdRope(turns=hip.put(1e4 ** (-np.arange(64) / 64) / 6.283185307179586).p, rot_dim=HD,
+                                    interleaved=0, scale=1.0)
+        self.b, self.p, self.dp = c.batch(), c.pages(), self.dst.pages()
+        self.ws_n = int(eng.dpuf_amd_paged_attn_workspace(C.byref(self.b), C.byref(self.p), NQ))
+        self.ws = hip.put(np.full(max(16, self.ws_n), 0xFF, np.uint8))
+        self.sws_n = int(eng.dpuf_amd_sample_workspace(n, V))
+        self.sws = hip.put(np.full(self.sws_n, 0xFF, np.uint8))
+
+    def enter(self, seed):
+        """Inputs of one step: new activations, lengths and settings, the
+        caches as they were."""
+        rng, c, n = np.random.default_rng(seed), self.cache, len(self.cache.ctx)
+        c.upload_into()
+        self.qkv.set(rng.standard_normal(self.qkv.like.shape).astype(np.float32))
+        self.pos.set(rng.integers(0, 1 << 20, c.n_rows).astype(np.int32))
+        c.d_ctx.set(np.array([rng.integers(0, m + 1) for m in c.ctx], np.int32))
+        self.x.set((rng.standard_normal((n, V)) * 3).astype(np.float32))
+        for d, v in zip(self.settings, (rng.random(n) + 0.3, rng.integers(0, 60, n), rng.random(n) + 0.3,
+                                        rng.random(n) * 0.1, rng.random(n))):
+            d.set(v.astype(d.like.dtype))
+
+    def run(self, stream):
+        e, r, b, p, es = self.eng, C.byref, self.b, self.p, 4
+        at = self.qkv.p
+        w = self.qkv.like.shape[1]
+        assert e.dpuf_amd_rope_append(r(b), r(p), r(self.rope), self.pos.p, R.F32, NQ, at, at + NQ * HD * es,
+                                      at + (NQ + NKV) * HD * es, w, w, w, None, None, 0.0, self.q.p, stream) == 0
+        assert e.dpuf_amd_paged_attn(r(b), r(p), NQ, self.q.p, 0.09, R.F32, self.out.p, self.lse.p, self.ws.p,
+                                     self.ws_n, stream) == 0
+        assert e.dpuf_amd_paged_attn_weights(r(b), r(p), NQ, self.q.p, 0.09, self.lse.p, 0.9, self.cache.dw.p,
+                                             stream) == 0
+        assert e.dpuf_amd_paged_evict(r(b), r(p), KEEP, 2, 8, r(self.dp), self.dst.d_table.p, self.dst.table.shape[1],
+                                      self.kept.p, self.new_len.p, stream) == 0
+        s = self.settings
+        assert e.dpuf_amd_sample(R.F32, len(self.cache.ctx), V, V, self.x.p, s[0].p, s[1].p, s[2].p, s[3].p, s[4].p,
+                                 self.tok.p, self.lp.p, self.sws.p, self.sws_n, stream) == 0
+
+    def results(self):
+        """Everything the step writes, as bits."""
+        assert self.hip.lib.hipStreamSynchronize(self.stream) == 0
+        d = (self.q, self.out, self.lse, self.kept, self.new_len, self.tok, self.lp, self.cache.dk, self.cache.dv,
+             self.cache.dw, self.dst.dk, self.dst.dv, self.dst.dw)
+        return [x.get().tobytes() for x in d]
+
+    def clear(self):
+        """Outputs that no step leaves."""
+        for d in (self.q, self.out, self.lse, self.kept, self.new_len, self.tok, self.lp):
+            d.set(np.full(d.like.shape, 77, d.like.dtype))
+        self.dst.upload_into()
+
+
+BATCHES = [([1, 1, 1], [900, 70, 1500]), ([1, 60, 0, 2], [33, 700, 20, 1200]), ([140], [300])]
+
+
+@pytest.mark.parametrize("rows,ctx", BATCHES)
+def test_a_captured_step_replays(eng, hip, rows, ctx):
+    print(f"graph: rows {rows}, contexts {ctx}", flush=True)
+    st = Step(eng, hip, 1, rows, ctx)
+    st.enter(0)
+    graph, ge = C.c_void_p(), C.c_void_p()
+    assert hip.lib.hipStreamBeginCapture(st.stream, 1) == 0
+    st.run(st.stream)
+    assert hip.lib.hipStreamEndCapture(st.stream, C.byref(graph)) == 0
+    assert hip.lib.hipGraphInstantiate(C.byref(ge), graph, None, None, 0) == 0
+    for seed in range(5):
+        st.enter(seed)
+        st.clear()
+        st.run(st.stream)
+        want = st.results()
+        for _ in range(2):
+            st.enter(seed)
+            st.clear()
+            assert hip.lib.hipGraphLaunch(ge, st.stream) == 0
+            assert st.results() == want, seed
+    hip.lib.hipGraphExecDestroy(ge)
+    hip.lib.hipGraphDestroy(graph)
+    hip.lib.hipStreamDestroy(st.stream)
+
+
+def test_steps_on_two_streams(eng, hip):
+    print("two streams", flush=True)
+    steps = [Step(eng, hip, 10 + i, *BATCHES[i]) for i in range(2)]
+    want = []
+    for i, st in enumerate(steps):
+        st.enter(50 + i)
+        st.clear()
+        st.run(st.stream)
+        want.append(st.results())
+    for turn in range(3):
+        for i, st in enumerate(steps):
+            st.enter(50 + i)
+            st.clear()
+        hip.sync()
+        for st in steps:
+            st.run(st.stream)
+        for i, st in enumerate(steps):
+            assert st.results() == want[i], (turn, i)
+    for st in steps:
+        hip.lib.hipStreamDestroy(st.stream)
+
+
+def test_a_query_with_nan_is_alone(eng, hip):
+    """NaN in one row's query stays in that row, whichever kernel takes it."""
+    for rows, ctx in (([5, 1, 1, 1, 1, 1, 1], [60, 3, 2, 90, 1, 1, 1]), ([100], [150])):
+        rng = np.random.default_rng(4)
+        cache = R.Cache(hip, rng, R.F16, rows, ctx, NKV, HD, 16)
+        q = R.to_type(rng.standard_normal((cache.n_rows, NQ, HD)), R.F16)
+        outs = []
+        print(f"NaN query: rows {rows}", flush=True)
+        for odd in (False, True):
+            if odd:
+                q[2, 3, 7] = R.to_type([np.nan], R.F16)[0]
+            dq, do = hip.put(q), hip.put(np.zeros((cache.n_rows, NQ, HD), np.float32))
+            dl = hip.put(np.zeros((cache.n_rows, NQ), np.float32))
+            b, p = cache.batch(), cache.pages(w=False)
+            n = int(eng.dpuf_amd_paged_attn_workspace(C.byref(b), C.byref(p), NQ))
+            ws = hip.put(np.zeros(max(n, 16), np.uint8))
+            assert eng.dpuf_amd_paged_attn(C.byref(b), C.byref(p), NQ, dq.p, 0.1, R.F32, do.p, dl.p, ws.p, n, None) == 0
+            outs.append((do.get(), dl.get()))
+        (o0, l0), (o1, l1) = outs
+        assert np.isnan(o1[2, 3]).all() and np.isnan(l1[2, 3])
+        o1[2, 3], l1[2, 3] = o0[2, 3], l0[2, 3]
+        assert np.array_equal(o0, o1) and np.array_equal(l0, l1)
+
+
+def test_arguments_that_share_memory_are_refused(eng, hip):
+    st = Step(eng, hip, 5, [1, 1], [900, 1500])
+    st.enter(0)
+    e, r, b, p = eng, C.byref, st.b, st.p
+    assert st.ws_n > 0
+    attn = dict(q=st.q.p, out=st.out.p, lse=st.lse.p, ws=st.ws.p)
+
+    def attention(**kw):
+        a = dict(attn, **kw)
+        return e.dpuf_amd_paged_attn(r(b), r(p), NQ, a["q"], 0.09, R.F32, a["out"], a["lse"], a["ws"], st.ws_n, None)
+
+    assert attention() == 0
+    for kw in (dict(lse=st.out.p), dict(lse=st.q.p + 16), dict(ws=st.out.p), dict(ws=st.q.p), dict(ws=st.lse.p),
+               dict(out=st.q.p)):
+        assert attention(**kw) == -1, kw
+    assert e.dpuf_amd_paged_attn_weights(r(b), r(p), NQ, st.q.p, 0.09, st.cache.dw.p, 1.0, None, None) == -1
+    s = st.settings
+    smp = dict(x=st.x.p, u=s[4].p, tok=st.tok.p, lp=st.lp.p, ws=st.sws.p)
+
+    def sample(**kw):
+        a = dict(smp, **kw)
+        return e.dpuf_amd_sample(R.F32, 2, V, V, a["x"], s[0].p, s[1].p, s[2].p, s[3].p, a["u"], a["tok"], a["lp"],
+                                 a["ws"], st.sws_n, None)
+
+    assert sample() == 0
+    for kw in (dict(tok=st.x.p), dict(lp=st.tok.p), dict(tok=s[4].p), dict(ws=st.x.p), dict(tok=st.sws.p + 64),
+               dict(u=st.sws.p), dict(lp=st.sws.p)):
+        assert sample(**kw) == -1, kw
+    hip.sync()
+    hip.lib.hipStreamDestroy(st.stream)
