@@ -749,8 +749,15 @@ PaPlan plan(const DpufAmdBatch& b, const DpufAmdPages& p, int nq) {
     const int64_t cap_z = 16384 / ((int64_t)b.n_seqs * p.n_kv_heads);
     if (r.nz_few > cap_z) r.nz_few = cap_z < 1 ? 1 : (int)cap_z;
     // as many ranges of a chunk's keys as fit on the card beside its tiles at
-    // once: two workgroups of 128 rows a CU, or one of 256
-    const int64_t wgs = (packed + tr - 1) / tr * p.n_kv_heads, room = r.only == PA_WIDE ? 256 : 512;
+    // once: two workgroups of 128 rows a CU, or one of 256.  Beside decoding
+    // sequences fewer, so that those, which wait for memory, run at the same
+    // time (a chunk of 256 rows and 31 single rows over 500 to 6 000 keys: 122
+    // us with room for 400, 134 for 512, 140 for 768), unless the chunks are
+    // nearly all of the work: then more, since the shorter contexts end sooner
+    // (three of 128 rows and a single one over 4 096 to 16 384: 201, 157, 119)
+    const bool chunks = (int64_t)(b.n_rows - b.n_seqs) * G > 220 * (int64_t)b.n_seqs;
+    const int64_t room = r.only == PA_WIDE ? 256 : r.only == PA_MANY ? 512 : chunks ? 768 : 400;
+    const int64_t wgs = (packed + tr - 1) / tr * p.n_kv_heads;
     const int64_t nz = wgs >= room ? 1 : room / (wgs > 0 ? wgs : 1);
     r.chunk_many = (ceil_div(ctx, nz) + 127) & ~127;
     if (r.chunk_many < range_of(ctx, 4.0)) r.chunk_many = range_of(ctx, 4.0);
