@@ -149,10 +149,13 @@ __global__ __launch_bounds__(256) void k_rope_append(RaArgs a) {
 // left operand of S^T = K Q^T and walks the sequence's rows, 32 at a time,
 // adding the exponentials of its keys in registers; the 32 rows of a step are
 // the lanes, added up once at the end in one order.  A workgroup is KG x RG
-// waves: KG of them hold different keys and read the same rows (from the L1),
-// RG share keys and take every RG-th step, their sums joined in LDS in one
-// order.  The queries are read once per KB x KG x 32 keys, which bounds it
-// together with the exponentials.
+// waves: KG of them hold different keys, RG share keys and take every RG-th
+// step, their sums joined in LDS in one order.  Its queries go through LDS, a
+// step ahead, so that each is read from memory once for all its keys (as the
+// matrix operand straight from the L1, 32 bytes of a row a load, it was that
+// which took the time: 256 rows of 4 heads, 8 kv heads over 4 096 keys 24.3 us
+// against 20.2).  Bound then by the matrix instructions and, of about the same
+// length, the exponentials and the queries' way through LDS.
 // ---------------------------------------------------------------------------
 struct PwArgs {
     DpufAmdBatch b;
@@ -179,14 +182,19 @@ DEV float row_sum(float v) {
 template <typename T, int HD, int KB, int KG, int RG>
 __global__ __launch_bounds__(64 * KG * RG) void k_pa_weights(PwArgs a) {
     constexpr int NC = HD / 16, KEYS = 32 * KB * KG;
+    constexpr int CH = HD / 8, RP = 64 * KG * RG / CH, ROWS = 32 * RG, NP = ROWS / RP, QP = HD + 8;
     typedef typename T::v8 v8;
     __shared__ float part[RG - 1][KEYS];
+    __shared__ __align__(16) uint16_t lq[2][ROWS * QP];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int col = lane & 31, h = lane >> 5, kg = wave % KG, rg = wave / KG;
     const int kvh = blockIdx.x, s = blockIdx.y;
     const PgSeq sq = pg_seq(a.b, a.shift, s);
     const int rows = sq.n * a.G;
     const float NEG_INF = -__builtin_huge_valf();
+    // r / G by a product: exact for r below 2^27 and G up to 32
+    const uint32_t inv = 0xffffffffu / (uint32_t)a.G + 1;
+    auto by_g = [&](int r) { return a.G == 1 ? r : (int)__umulhi((uint32_t)r, inv); };
     for (int base0 = KEYS * blockIdx.z; base0 < sq.ctx; base0 += KEYS * gridDim.z) {
         const int base = base0 + 32 * KB * kg;
         v8 kf[KB][NC];
@@ -203,40 +211,68 @@ __global__ __launch_bounds__(64 * KG * RG) void k_pa_weights(PwArgs a) {
         }
         float acc[KB][16] = {};
         // rows before the first key of the tile see none of it
-        const int i0 = max(0, base - (sq.ctx - sq.n));
-        const int first = (i0 * a.G & ~31) + 32 * rg;
-        u32x4 qn[NC];
+        const int first = max(0, base0 - (sq.ctx - sq.n)) * a.G & ~31;
+        // a step's queries go to LDS, once for all waves, while the step before
+        // it is worked out; the lse to registers
+        const int lr = threadIdx.x / CH, lc = 8 * (threadIdx.x % CH);
+        u32x4 qn[NP];
+        auto load = [&](int r0) {
+#pragma unroll
+            for (int u = 0; u < NP; u++) {
+                const int r = r0 + u * RP + lr, i = by_g(r);
+                const size_t row = (size_t)(sq.r0 + i) * a.nq + kvh * a.G + (r - i * a.G);
+                qn[u] = r < rows ? *(const u32x4*)(a.q + row * HD + lc) : u32x4{0, 0, 0, 0};
+            }
+        };
+        auto store = [&](int buf) {
+#pragma unroll
+            for (int u = 0; u < NP; u++) *(u32x4*)(lq[buf] + (u * RP + lr) * QP + lc) = qn[u];
+        };
         float ln = 0.0f;
         int qi = 0;
-        bool live = false;
-        // the next step's queries and lse, while the current one is worked out
         auto fetch = [&](int r0) {
-            const int r = r0 + col;
-            live = r < rows;
-            qi = live ? r / a.G : 0;
-            const size_t row = (size_t)(sq.r0 + qi) * a.nq + kvh * a.G + (live ? r - qi * a.G : 0);
-            ln = live ? a.lse[row] : NEG_INF;
+            const int r = r0 + 32 * rg + col;
+            const bool live = r < rows;
+            qi = live ? by_g(r) : 0;
+            ln = live ? a.lse[(size_t)(sq.r0 + qi) * a.nq + kvh * a.G + (r - qi * a.G)] : NEG_INF;
+        };
+        v8 qf[NC];
+        auto take = [&](int buf) {
 #pragma unroll
             for (int c = 0; c < NC; c++)
-                qn[c] = live ? *(const u32x4*)(a.q + row * HD + 16 * c + 8 * h) : u32x4{0, 0, 0, 0};
+                qf[c] = vec_of<v8>(*(const u32x4*)(lq[buf] + (32 * rg + col) * QP + 16 * c + 8 * h));
         };
-        if (first < rows) fetch(first);
-        for (int r0 = first; r0 < rows; r0 += 32 * RG) {
-            v8 qf[NC];
-#pragma unroll
-            for (int c = 0; c < NC; c++) qf[c] = vec_of<v8>(qn[c]);
-            // a row that saw no key (lse -infinity) or is none gives nothing
-            const float l2 = ln == NEG_INF ? -NEG_INF : ln * 1.4426950408889634f;
-            const int limit = live && ln != NEG_INF ? sq.ctx - sq.n + qi : -1;
-            if (r0 + 32 * RG < rows) fetch(r0 + 32 * RG);
+        if (first < rows) {
+            load(first);
+            fetch(first);
+            store(0);
+            if (first + ROWS < rows) load(first + ROWS);
+            __syncthreads();
+            take(0);
+        }
+        int buf = 0;
+        for (int w0 = first; w0 < rows; w0 += ROWS, buf ^= 1) {
+            const int r0 = w0 + 32 * rg;
             f32x16 sc[KB];
             const f32x16 zero = {};
 #pragma unroll
             for (int c = 0; c < NC; c++)
 #pragma unroll
                 for (int b = 0; b < KB; b++) sc[b] = T::mma32(kf[b][c], qf[c], c ? sc[b] : zero);
+            // a row that saw no key (lse -infinity) or is none gives nothing
+            const float l2 = ln == NEG_INF ? -NEG_INF : ln * 1.4426950408889634f;
+            const int limit = ln != NEG_INF ? sq.ctx - sq.n + qi : -1;
+            // the next step's queries: to LDS, and from there while the
+            // exponentials are worked out
+            if (w0 + ROWS < rows) {
+                store(buf ^ 1);
+                fetch(w0 + ROWS);
+                if (w0 + 2 * ROWS < rows) load(w0 + 2 * ROWS);
+                __syncthreads();
+                take(buf ^ 1);
+            }
             // keys that the step's first row does not see: row by row
-            if (base + 32 * KB - 1 > sq.ctx - sq.n + r0 / a.G) {
+            if (base + 32 * KB - 1 > sq.ctx - sq.n + by_g(r0)) {
 #pragma unroll
                 for (int b = 0; b < KB; b++)
 #pragma unroll
@@ -257,8 +293,8 @@ __global__ __launch_bounds__(64 * KG * RG) void k_pa_weights(PwArgs a) {
             mine[b] = 0.0f;
 #pragma unroll
             for (int i = 0; i < 8; i++) {
-                const auto x = __builtin_amdgcn_permlane16_swap(__float_as_uint(acc[b][i]), __float_as_uint(acc[b][i + 8]),
-                                                                false, false);
+                const auto x = __builtin_amdgcn_permlane16_swap(__float_as_uint(acc[b][i]),
+                                                                __float_as_uint(acc[b][i + 8]), false, false);
                 const float v = row_sum(__uint_as_float(x[0]) + __uint_as_float(x[1]));
                 mine[b] = (lane & 7) == i ? v : mine[b];
             }
@@ -613,17 +649,36 @@ __global__ __launch_bounds__(256) void k_ev_move(EvArgs a) {
     }
 }
 
-template <typename T, int HD> void weights_rg(const PwArgs& a, bool many, int64_t ctx, hipStream_t st) {
-    constexpr int KB = HD == 256 ? 1 : 2, WK = HD == 256 ? 32 : 64;   // what the registers hold
-    const int64_t keys = many ? 64 * KB : 4 * WK, tiles = (ctx + keys - 1) / keys;
-    // a chunk's tiles are long: one each; a decode step's workgroups, about
-    // four a CU, walk theirs with the next keys in flight
-    const int64_t by = (int64_t)a.p.n_kv_heads * a.b.n_seqs;
-    int64_t z = many ? tiles : (1024 + by - 1) / by;
-    z = z < tiles ? z : tiles;
+template <typename T, int HD, int KB, int KG, int RG>
+void weights_many(const PwArgs& a, int64_t ctx, hipStream_t st) {
+    const int64_t z = (ctx + 32 * KB * KG - 1) / (32 * KB * KG);
     const dim3 g(a.p.n_kv_heads, a.b.n_seqs, (unsigned)(z < 65535 ? z : 65535));
-    if (many) hipLaunchKernelGGL((k_pa_weights<T, HD, KB, 2, 4>), g, dim3(512), 0, st, a);
-    else hipLaunchKernelGGL((k_pa_weights_few<T, HD>), g, dim3(256), 0, st, a);
+    hipLaunchKernelGGL((k_pa_weights<T, HD, KB, KG, RG>), g, dim3(64 * KG * RG), 0, st, a);
+}
+// Chunks: as few keys a workgroup as gives every CU at most one, since its
+// steps are latency rather than work while the card is not full: 256 rows of 8
+// heads, 2 kv heads of 64 columns over 4 096 keys 10.9 us with 32 keys (256
+// workgroups), 14.5 with 64, 22 with 128; 256 rows of 4 heads, 8 kv heads of
+// 128 over 2 000 19.7, 12.8, 18.5 (500, 250, 125 workgroups); over 4 096 39,
+// 24.5, 20.2.
+template <typename T, int HD> void weights_rg(const PwArgs& a, bool many, int64_t ctx, hipStream_t st) {
+    const int64_t by = (int64_t)a.p.n_kv_heads * a.b.n_seqs, cus = dpuf_hip_cu_count();
+    if (many) {
+        if constexpr (HD == 256) {       // what registers and LDS hold
+            weights_many<T, HD, 1, 2, 4>(a, ctx, st);
+        } else {
+            if ((ctx + 31) / 32 * by <= cus) weights_many<T, HD, 1, 1, 8>(a, ctx, st);
+            else if ((ctx + 63) / 64 * by <= cus) weights_many<T, HD, 1, 2, 4>(a, ctx, st);
+            else weights_many<T, HD, 2, 2, 4>(a, ctx, st);
+        }
+        return;
+    }
+    // a decode step's workgroups, about four a CU, walk their keys with the
+    // next ones in flight
+    const int64_t keys = HD == 256 ? 128 : 256, tiles = (ctx + keys - 1) / keys, z = (1024 + by - 1) / by;
+    const int64_t nz = z < tiles ? z : tiles;
+    const dim3 g(a.p.n_kv_heads, a.b.n_seqs, (unsigned)(nz < 65535 ? nz : 65535));
+    hipLaunchKernelGGL((k_pa_weights_few<T, HD>), g, dim3(256), 0, st, a);
 }
 template <typename TI, bool F32, typename T> void rope_hd(const RaArgs& a, dim3 g, hipStream_t st) {
     switch (a.p.head_dim) {
@@ -642,8 +697,8 @@ template <typename T> void rope_in(const RaArgs& a, int in_type, dim3 g, hipStre
 
 extern "C" {
 
-void dpuf_hip_rope_append(void* s, const DpufAmdBatch* b, const DpufAmdPages* p, const DpufAmdRope* r, const int32_t* pos,
-                          int32_t in_type, int32_t nq, const void* q, const void* k, const void* v, int64_t qs,
+void dpuf_hip_rope_append(void* s, const DpufAmdBatch* b, const DpufAmdPages* p, const DpufAmdRope* r,
+                          const int32_t* pos, int32_t in_type, int32_t nq, const void* q, const void* k, const void* v, int64_t qs,
                           int64_t ks, int64_t vs, const float* qn, const float* kn, float eps, void* q_out) {
     RaArgs a;
     a.b = *b;

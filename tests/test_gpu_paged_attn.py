@@ -234,6 +234,38 @@ def test_infinities_and_nan_that_a_row_does_not_see(eng, hip, mode, hd, t):
         assert np.array_equal(np.isnan(lse), np.isnan(rl)) and np.array_equal(np.isneginf(lse), np.isneginf(rl))
 
 
+@pytest.mark.parametrize("max_ctx", [60, 6000, 20000])
+@pytest.mark.parametrize("nq,hd,rows,ctx", [(6, 64, [71], [300]), (2, 128, [200, 0, 1], [260, 40, 90]),
+                                            (16, 128, [50], [50]), (10, 256, [40], [333])])
+def test_weights_of_chunks(eng, hip, nq, hd, rows, ctx, max_ctx):
+    """Chunks of a prompt, over every split of the keys among workgroups."""
+    rng = np.random.default_rng(nq + hd)
+    t = R.F16 if nq == 6 else R.BF16
+    cache = R.Cache(hip, rng, t, rows, ctx, 2, hd, 16, table_extra=1300, bad=[(0, 1)])
+    q = R.to_type(rng.standard_normal((cache.n_rows, nq, hd)) * 1.5, t)
+    say(f"weights of chunks: hd {hd}, rows {rows}, contexts {ctx}, max_ctx {max_ctx}")
+    _, lse, dq, dl, _ = call(eng, hip, cache, nq, q, 0.1)
+    _, rl, _, S, _, fresh = R.attention(cache, R.from_type(q, t), float(np.float32(0.1)), nq)
+    dst = hip.put(np.full_like(cache.w, -3.0))
+    b, p = cache.batch(max_ctx=max_ctx), cache.pages(dw=dst)
+    rc = eng.dpuf_amd_paged_attn_weights(C.byref(b), C.byref(p), nq, dq.p, 0.1, dl.p, 0.5, cache.dw.p, None)
+    assert rc == 0, (rc, eng.dpuf_amd_last_error())
+    out = dst.get()
+    # as for test_weights
+    rel = 2 * R.score_error(S.max(initial=0), hd) + np.abs(rl[np.isfinite(rl)]).max() * 2.0 ** -22 + 2.0 ** -20
+    rel += (max(rows) * nq // 2 + 40) * 2.0 ** -24
+    for s, c in enumerate(ctx):
+        for i in range(c):
+            if not cache.ok(s, i):
+                continue
+            pg, r = cache.table[s, i // 16], i % 16
+            old = cache.w[pg, :, r].astype(np.float64) * 0.5
+            assert np.all(np.abs(out[pg, :, r] - old - fresh[s][:, i]) <=
+                          rel * fresh[s][:, i] + 2.0 ** -22 * np.abs(old) + 1e-30), (s, i)
+            out[pg, :, r] = -3.0
+    assert np.all(out == -3.0)
+
+
 def test_two_streams_and_a_graph(eng, hip):
     """Two calls at once on streams of their own with workspaces of their own;
     then a captured call replayed over new lengths and values between eager
