@@ -166,6 +166,7 @@ struct PwArgs {
     const float* lse;
     float decay;
     const float* w_in;
+    int lo, hi;         // packed rows of the sequences that the few-row kernel (up to hi), the other (above lo) takes
 };
 
 // Sum over the 16 lanes of a row, in all of them.
@@ -188,15 +189,38 @@ __global__ __launch_bounds__(64 * KG * RG) void k_pa_weights(PwArgs a) {
     __shared__ __align__(16) uint16_t lq[2][ROWS * QP];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int col = lane & 31, h = lane >> 5, kg = wave % KG, rg = wave / KG;
-    const int kvh = blockIdx.x, s = blockIdx.y;
-    const PgSeq sq = pg_seq(a.b, a.shift, s);
-    const int rows = sq.n * a.G;
     const float NEG_INF = -__builtin_huge_valf();
     // r / G by a product: exact for r below 2^27 and G up to 32
     const uint32_t inv = 0xffffffffu / (uint32_t)a.G + 1;
     auto by_g = [&](int r) { return a.G == 1 ? r : (int)__umulhi((uint32_t)r, inv); };
-    for (int base0 = KEYS * blockIdx.z; base0 < sq.ctx; base0 += KEYS * gridDim.z) {
-        const int base = base0 + 32 * KB * kg;
+    // a workgroup's tiles: kv heads fastest, then the tiles of the sequences
+    // with more than `lo` packed rows, one sequence after the other
+    for (int64_t it = blockIdx.x;; it += gridDim.x) {
+        int64_t tile = it / a.p.n_kv_heads;
+        const int kvh = (int)(it - tile * a.p.n_kv_heads);
+        int s = a.b.n_seqs == 1 ? 0 : -1;
+        for (int s0 = 0; s0 < a.b.n_seqs && s < 0; s0 += 64) {
+            long long n = 0;
+            if (s0 + lane < a.b.n_seqs) {
+                const PgSeq q = pg_seq(a.b, a.shift, s0 + lane);
+                n = q.n * a.G > a.lo ? (q.ctx + KEYS - 1) / KEYS : 0;
+            }
+            long long sum = n;
+            for (int d = 1; d < 64; d <<= 1) {
+                const long long o = __shfl_up(sum, d);
+                if (lane >= d) sum += o;
+            }
+            const uint64_t past = __ballot(sum > tile);
+            const int at = past ? __ffsll((unsigned long long)past) - 1 : 63;
+            tile -= __shfl(past ? sum - n : sum, at);
+            if (past) s = s0 + at;
+        }
+        s = __builtin_amdgcn_readfirstlane(s);
+        if (s < 0) return;
+        const PgSeq sq = pg_seq(a.b, a.shift, s);
+        const int rows = sq.n * a.G;
+        if (tile * KEYS >= sq.ctx) return;
+        const int base0 = __builtin_amdgcn_readfirstlane((int)tile) * KEYS, base = base0 + 32 * KB * kg;
         v8 kf[KB][NC];
 #pragma unroll
         for (int b = 0; b < KB; b++) {
@@ -341,6 +365,7 @@ __global__ __launch_bounds__(256) void k_pa_weights_few(PwArgs a) {
     const int kvh = blockIdx.x, s = blockIdx.y;
     const PgSeq sq = pg_seq(a.b, a.shift, s);
     const int rows = sq.n * a.G;
+    if (rows > a.hi) return;
     const float NEG_INF = -__builtin_huge_valf();
     const uint16_t* kp = (const uint16_t*)a.p.k + (size_t)kvh * a.p.head_stride + 8 * g4;
     const int* table = a.b.page_table + (size_t)s * a.b.table_stride;
@@ -650,34 +675,52 @@ __global__ __launch_bounds__(256) void k_ev_move(EvArgs a) {
 }
 
 template <typename T, int HD, int KB, int KG, int RG>
-void weights_many(const PwArgs& a, int64_t ctx, hipStream_t st) {
-    const int64_t z = (ctx + 32 * KB * KG - 1) / (32 * KB * KG);
-    const dim3 g(a.p.n_kv_heads, a.b.n_seqs, (unsigned)(z < 65535 ? z : 65535));
-    hipLaunchKernelGGL((k_pa_weights<T, HD, KB, KG, RG>), g, dim3(64 * KG * RG), 0, st, a);
+void weights_many(const PwArgs& a, int64_t ctx, int64_t rows_of_tiles, hipStream_t st) {
+    const int64_t tiles = (ctx + 32 * KB * KG - 1) / (32 * KB * KG) * rows_of_tiles, cus = dpuf_hip_cu_count();
+    hipLaunchKernelGGL((k_pa_weights<T, HD, KB, KG, RG>), dim3((unsigned)(tiles < cus ? tiles : cus)),
+                       dim3(64 * KG * RG), 0, st, a);
 }
-// Chunks: as few keys a workgroup as gives every CU at most one, since its
+
+// Which kernel takes which sequences: those of up to LIM packed rows the
+// few-row one (eight chunks of 80 rows over 1 000 to 3 000 keys 22 us against
+// 39, of 256 rows 41 against 47, but a single one of 256 over 4 096 14 against
+// 11), the others the other, a launch each where there may be both (one chunk
+// of 256 rows of 4 heads and 31 single rows over 500 to 6 000 keys 81 us, 381
+// by the few-row kernel alone).  One sequence, or a batch whose tiles would
+// leave CUs idle, is one launch (a chunk of 131 rows and two single ones over
+// 900 keys 14.6 us against 20.8).
+//
+// A workgroup has as few keys as gives every CU at most one tile, since its
 // steps are latency rather than work while the card is not full: 256 rows of 8
-// heads, 2 kv heads of 64 columns over 4 096 keys 10.9 us with 32 keys (256
-// workgroups), 14.5 with 64, 22 with 128; 256 rows of 4 heads, 8 kv heads of
-// 128 over 2 000 19.7, 12.8, 18.5 (500, 250, 125 workgroups); over 4 096 39,
-// 24.5, 20.2.
-template <typename T, int HD> void weights_rg(const PwArgs& a, bool many, int64_t ctx, hipStream_t st) {
-    const int64_t by = (int64_t)a.p.n_kv_heads * a.b.n_seqs, cus = dpuf_hip_cu_count();
-    if (many) {
-        if constexpr (HD == 256) {       // what registers and LDS hold
-            weights_many<T, HD, 1, 2, 4>(a, ctx, st);
+// heads, 2 kv heads of 64 columns over 4 096 keys 10.5 us with 32 keys (256
+// tiles), 14.5 with 64, 22 with 128; 256 rows of 4 heads, 8 kv heads of 128
+// over 2 000 19.7, 12.6, 18.5 (500, 250, 125 tiles); over 4 096 39, 24.5, 20.2.
+constexpr int LIM = 128;
+template <typename T, int HD> void weights_hd(PwArgs a, int64_t ctx, hipStream_t st) {
+    const int64_t G = a.G, nkv = a.p.n_kv_heads, n = a.b.n_seqs, packed = a.b.n_rows * G, cus = dpuf_hip_cu_count();
+    constexpr int MOST = HD == 256 ? 64 : 128;           // keys that registers and LDS hold
+    const bool none = a.b.n_rows <= n || packed <= LIM;
+    const bool all = !none && (n == 1 || (ctx + MOST - 1) / MOST * nkv * n <= cus);
+    a.lo = all ? -1 : LIM;
+    a.hi = none ? INT32_MAX : LIM;
+    if (!none) {
+        // sequences of chunks: at most, and if they have 256 packed rows each
+        const int64_t most = all || packed / (LIM + 1) > n ? n : packed / (LIM + 1);
+        const int64_t about = ((a.b.n_rows - n) * G + 255) / 256, by = nkv * (all || about > n ? n : about);
+        if constexpr (HD == 256) {
+            weights_many<T, HD, 1, 2, 4>(a, ctx, nkv * most, st);
         } else {
-            if ((ctx + 31) / 32 * by <= cus) weights_many<T, HD, 1, 1, 8>(a, ctx, st);
-            else if ((ctx + 63) / 64 * by <= cus) weights_many<T, HD, 1, 2, 4>(a, ctx, st);
-            else weights_many<T, HD, 2, 2, 4>(a, ctx, st);
+            if ((ctx + 31) / 32 * by <= cus) weights_many<T, HD, 1, 1, 8>(a, ctx, nkv * most, st);
+            else if ((ctx + 63) / 64 * by <= cus) weights_many<T, HD, 1, 2, 4>(a, ctx, nkv * most, st);
+            else weights_many<T, HD, 2, 2, 4>(a, ctx, nkv * most, st);
         }
-        return;
     }
+    if (all) return;
     // a decode step's workgroups, about four a CU, walk their keys with the
     // next ones in flight
-    const int64_t keys = HD == 256 ? 128 : 256, tiles = (ctx + keys - 1) / keys, z = (1024 + by - 1) / by;
-    const int64_t nz = z < tiles ? z : tiles;
-    const dim3 g(a.p.n_kv_heads, a.b.n_seqs, (unsigned)(nz < 65535 ? nz : 65535));
+    const int64_t by = nkv * n, keys = HD == 256 ? 128 : 256, tiles = (ctx + keys - 1) / keys;
+    const int64_t few = (1024 + by - 1) / by, z = few < tiles ? few : tiles;
+    const dim3 g((unsigned)nkv, (unsigned)n, (unsigned)z);
     hipLaunchKernelGGL((k_pa_weights_few<T, HD>), g, dim3(256), 0, st, a);
 }
 template <typename TI, bool F32, typename T> void rope_hd(const RaArgs& a, dim3 g, hipStream_t st) {
@@ -698,8 +741,9 @@ template <typename T> void rope_in(const RaArgs& a, int in_type, dim3 g, hipStre
 extern "C" {
 
 void dpuf_hip_rope_append(void* s, const DpufAmdBatch* b, const DpufAmdPages* p, const DpufAmdRope* r,
-                          const int32_t* pos, int32_t in_type, int32_t nq, const void* q, const void* k, const void* v, int64_t qs,
-                          int64_t ks, int64_t vs, const float* qn, const float* kn, float eps, void* q_out) {
+                          const int32_t* pos, int32_t in_type, int32_t nq, const void* q, const void* k, const void* v,
+                          int64_t qs, int64_t ks, int64_t vs, const float* qn, const float* kn, float eps,
+                          void* q_out) {
     RaArgs a;
     a.b = *b;
     a.p = *p;
@@ -746,14 +790,11 @@ void dpuf_hip_paged_attn_weights(void* s, const DpufAmdBatch* b, const DpufAmdPa
     a.w_in = w_in;
     const int64_t cap = (int64_t)b->table_stride * p->page_size;
     const int64_t ctx = b->max_ctx < 1 ? 1 : b->max_ctx < cap ? b->max_ctx : cap;
-    // one sequence's rows are n_rows or fewer: with several steps of 32 the
-    // waves of a workgroup share them
-    const bool many = (int64_t)b->n_rows * a.G > (int64_t)b->n_seqs * 64;
     const bool bf = p->type == DPUF_AMD_BF16;
     switch (p->head_dim) {
-        case 64: bf ? weights_rg<Bf16, 64>(a, many, ctx, ST(s)) : weights_rg<Fp16, 64>(a, many, ctx, ST(s)); break;
-        case 128: bf ? weights_rg<Bf16, 128>(a, many, ctx, ST(s)) : weights_rg<Fp16, 128>(a, many, ctx, ST(s)); break;
-        default: bf ? weights_rg<Bf16, 256>(a, many, ctx, ST(s)) : weights_rg<Fp16, 256>(a, many, ctx, ST(s));
+        case 64: bf ? weights_hd<Bf16, 64>(a, ctx, ST(s)) : weights_hd<Fp16, 64>(a, ctx, ST(s)); break;
+        case 128: bf ? weights_hd<Bf16, 128>(a, ctx, ST(s)) : weights_hd<Fp16, 128>(a, ctx, ST(s)); break;
+        default: bf ? weights_hd<Bf16, 256>(a, ctx, ST(s)) : weights_hd<Fp16, 256>(a, ctx, ST(s));
     }
     LAUNCHED("k_pa_weights");
 }
