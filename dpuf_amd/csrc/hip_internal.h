@@ -1,6 +1,7 @@
 // hip_internal.h -- host-side helpers shared by the HIP translation units of
-// the engine (rt.hip, gemv.hip, gemm.hip, gemt.hip, attn.hip, attn_wide.hip,
-// attn_dec.hip).
+// the engine (rt.hip, gemv.hip, gemm.hip, gemt.hip, attn.hip, attn_tile.hip,
+// attn_wide.hip, attn_dec.hip) and of the paged-serving operators
+// (paged_attn.hip, paged_cache.hip, sample.hip).
 #ifndef DPUF_HIP_INTERNAL_H
 #define DPUF_HIP_INTERNAL_H
 
