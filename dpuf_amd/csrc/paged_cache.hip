@@ -459,12 +459,14 @@ __global__ __launch_bounds__(256) void k_pa_weights_few(PwArgs a) {
 }
 
 // ---------------------------------------------------------------------------
-// Eviction.  k_ev_pick: one workgroup per (sequence, kv head) finds the
-// keep - sink - recent largest weights of the middle by radix selection on
-// order-preserving integers (10 bits a pass from the highest bit in which two
-// of them differ, over LDS, or over memory where the row is longer), then lists
-// the kept rows in order.  k_ev_move copies
-// them, 16 bytes a lane: bound by bytes.
+// Eviction.  k_ev_pick / k_ev_pick_long: one workgroup per (sequence, kv head)
+// finds the keep - sink - recent largest weights of the middle by radix
+// selection on order-preserving integers (10 bits a pass from the highest bit
+// in which two of them differ), then lists the kept rows in order: latency, of
+// the loads (length, page, weight) and of the passes' barriers.  k_ev_move
+// copies them, 16 bytes a lane, four rows in flight: bound by bytes (8
+// sequences of 6 100 to 9 000 rows to 4 096, 8 kv heads of 128: 59 us, 4.6 TB/s
+// read and written; one of 1 290 rows to 1 024: 4.4 us).
 // ---------------------------------------------------------------------------
 struct EvArgs {
     DpufAmdBatch b;
@@ -511,7 +513,9 @@ DEV void scan2(int& x, int& y, int& tx, int& ty, int (*sums)[2]) {
     __syncthreads();
 }
 
-__global__ __launch_bounds__(EV_T) void k_ev_pick(EvArgs a) {
+// Longer rows: keys in LDS, or read again in every pass where it does not hold
+// them (17 us for eight sequences of up to 9 000 rows).
+__global__ __launch_bounds__(EV_T) void k_ev_pick_long(EvArgs a) {
     extern __shared__ __align__(16) uint32_t keys[];
     __shared__ int hist[EV_T];
     __shared__ int sums[EV_T / 64][2];
@@ -626,6 +630,165 @@ __global__ __launch_bounds__(EV_T) void k_ev_pick(EvArgs a) {
     }
     for (int i = t; i < a.sink; i += EV_T) kept[i] = i;
     for (int i = t; i < a.recent; i += EV_T) kept[a.keep - a.recent + i] = hi + i;
+}
+
+// Rows of at most NT AT keys: they stay in registers, key u NT + t of the middle
+// with thread t, and the places of the rows that stay follow from ballots, in
+// row order.
+template <int NT, int AT> __global__ __launch_bounds__(NT) void k_ev_pick(EvArgs a) {
+    constexpr int BINS = 1024, OWN = BINS / NT, NW = NT / 64, CELLS = AT * NW, LC = (CELLS + 63) / 64;
+    __shared__ int hist[BINS];
+    __shared__ int sums[NW];
+    __shared__ uint32_t bits[NW][2];
+    __shared__ uint32_t sh_digit;
+    __shared__ int sh_need;
+    __shared__ int cells[2][64 * LC];      // rows above the cut, equal to it, of 64 consecutive ones
+    const int kvh = blockIdx.x, s = blockIdx.y, t = threadIdx.x, lane = t & 63, wave = t >> 6;
+    const int c = pg_ctx(a.b, a.shift, s), n = min(c, a.keep);
+    if (kvh == 0 && t == 0) a.new_len[s] = n;
+    int* kept = a.kept + ((size_t)s * a.p.n_kv_heads + kvh) * a.keep;
+    if (c <= a.keep) {
+        for (int i = t; i < n; i += NT) kept[i] = i;
+        return;
+    }
+    const int lo = a.sink, hi = c - a.recent, need = a.keep - a.sink - a.recent, mid = hi - lo;
+    int pg[AT];
+    uint32_t k[AT];
+#pragma unroll
+    for (int u = 0; u < AT; u++)
+        if (u * NT < mid) pg[u] = pg_page(a.b, a.shift, s, lo + min(u * NT + t, mid - 1));
+#pragma unroll
+    for (int u = 0; u < AT; u++) {
+        if (u * NT >= mid) continue;
+        const int in_page = (lo + min(u * NT + t, mid - 1)) & (a.p.page_size - 1);
+        const bool in = (unsigned)pg[u] < (unsigned)a.p.n_pages;
+        const float w = a.p.w[((size_t)(in ? pg[u] : 0) * a.p.n_kv_heads + kvh) * a.p.page_size + in_page];
+        k[u] = in ? weight_key(w) : 0;
+    }
+    for (int i = t; i < a.sink; i += NT) kept[i] = i;
+    for (int i = t; i < a.recent; i += NT) kept[a.keep - a.recent + i] = hi + i;
+    if (need == 0) return;
+    // the bits in which keys differ
+    uint32_t any = 0, all = ~0u;
+#pragma unroll
+    for (int u = 0; u < AT; u++)
+        if (u * NT + t < mid) {
+            any |= k[u];
+            all &= k[u];
+        }
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+        any |= __shfl_xor(any, d);
+        all &= __shfl_xor(all, d);
+    }
+    if (lane == 0) {
+        bits[wave][0] = any;
+        bits[wave][1] = all;
+    }
+#pragma unroll
+    for (int e = 0; e < OWN; e++) hist[OWN * t + e] = 0;
+    if (t < 64 * LC - CELLS) cells[0][CELLS + t] = cells[1][CELLS + t] = 0;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < NW; w++) {
+        any |= bits[w][0];
+        all &= bits[w][1];
+    }
+    int top = any & ~all ? 32 - __clz((int)(any & ~all)) : 0;      // keys agree from this bit up
+    uint32_t cut = top < 32 ? all >> top << top : 0;
+    int ties = need;               // of the keys equal to cut, the first this many stay
+    // the need-th largest key, 10 bits at a time
+    while (top > 0) {
+        const int low = top > 10 ? top - 10 : 0, mask = (1 << (top - low)) - 1;
+#pragma unroll
+        for (int u = 0; u < AT; u++)
+            if (u * NT + t < mid && (top == 32 || k[u] >> top == cut >> top))
+                atomicAdd(&hist[mask - (int)(k[u] >> low & mask)], 1);
+        __syncthreads();
+        // the digit, from the top, in which the count reaches what is left
+        int own[OWN], mine = 0;
+#pragma unroll
+        for (int e = 0; e < OWN; e++) mine += own[e] = hist[OWN * t + e];
+        int x = mine;
+#pragma unroll
+        for (int d = 1; d < 64; d <<= 1) {
+            const int o = __shfl_up(x, d);
+            if (lane >= d) x += o;
+        }
+        if (lane == 63) sums[wave] = x;
+#pragma unroll
+        for (int e = 0; e < OWN; e++) hist[OWN * t + e] = 0;
+        __syncthreads();
+        x -= mine;
+#pragma unroll
+        for (int w = 0; w < NW - 1; w++) x += w < wave ? sums[w] : 0;
+#pragma unroll
+        for (int e = 0; e < OWN; e++) {
+            if (x < ties && x + own[e] >= ties) {
+                sh_digit = (uint32_t)(mask - (OWN * t + e));
+                sh_need = ties - x;
+            }
+            x += own[e];
+        }
+        __syncthreads();
+        cut |= sh_digit << low;
+        ties = sh_need;
+        top = low;
+    }
+    // places: above the cut, or one of the first `ties` equal to it
+    uint64_t above[AT], equal[AT];
+#pragma unroll
+    for (int u = 0; u < AT; u++) {
+        const bool mine = u * NT + t < mid;
+        above[u] = __ballot(mine && k[u] > cut);
+        equal[u] = __ballot(mine && k[u] == cut);
+        if (lane == 0) {
+            cells[0][u * NW + wave] = __popcll(above[u]);
+            cells[1][u * NW + wave] = __popcll(equal[u]);
+        }
+    }
+    __syncthreads();
+    int ca[LC], ce[LC], sa = 0, se = 0;      // of the lane's cells, before which the lower lanes' lie
+#pragma unroll
+    for (int e = 0; e < LC; e++) {
+        ca[e] = cells[0][LC * lane + e];
+        ce[e] = cells[1][LC * lane + e];
+        sa += ca[e];
+        se += ce[e];
+    }
+    int xa = sa, xe = se;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+        const int oa = __shfl_up(xa, d), oe = __shfl_up(xe, d);
+        if (lane >= d) xa += oa, xe += oe;
+    }
+    xa -= sa;
+    xe -= se;
+#pragma unroll
+    for (int e = 0; e < LC; e++) {
+        const int na = ca[e], ne = ce[e];
+        ca[e] = xa;
+        ce[e] = xe;
+        xa += na;
+        xe += ne;
+    }
+    const uint64_t below = (1ull << lane) - 1;
+#pragma unroll
+    for (int u = 0; u < AT; u++) {
+        if (u * NT >= mid) continue;
+        const int cell = u * NW + wave;
+        int ba = 0, be = 0;
+#pragma unroll
+        for (int e = 0; e < LC; e++)
+            if (cell % LC == e) {
+                ba = __shfl(ca[e], cell / LC);
+                be = __shfl(ce[e], cell / LC);
+            }
+        ba += __popcll(above[u] & below);
+        be += __popcll(equal[u] & below);
+        if (u * NT + t < mid && (k[u] > cut || (k[u] == cut && be < ties)))
+            kept[a.sink + ba + min(be, ties)] = lo + u * NT + t;
+    }
 }
 
 template <int HD>
@@ -815,11 +978,17 @@ void dpuf_hip_paged_evict(void* s, const DpufAmdBatch* b, const DpufAmdPages* p,
     a.dstride = dstride;
     a.kept = kept;
     a.new_len = new_len;
-    // rows of up to 36 864 keys are held in LDS (144 KB of the 160)
     const int64_t cap = (int64_t)b->table_stride * p->page_size;
-    a.lds_keys = (int)(cap < 36864 ? cap : 36864);
-    const size_t lds = (size_t)a.lds_keys * 4;
-    hipLaunchKernelGGL(k_ev_pick, dim3(p->n_kv_heads, b->n_seqs), dim3(EV_T), lds, ST(s), a);
+    const dim3 gp(p->n_kv_heads, b->n_seqs);
+    a.lds_keys = (int)(cap < 36864 ? cap : 36864);      // 144 KB of the 160
+    // what the tables bound the rows by; the whole call, one sequence of 8 kv
+    // heads: 1 290 rows 14.4 us by the long rows' kernel, 12.7 by <1024, 4>,
+    // 11.6 by <512, 4>; 4 000 rows 17.2 and 14.6; 8 000 rows 23.3, and 21.3 by
+    // <1024, 8>; 9 000 rows 24.1, and 25.4 by <1024, 16>
+    if (cap <= 2048) hipLaunchKernelGGL((k_ev_pick<512, 4>), gp, dim3(512), 0, ST(s), a);
+    else if (cap <= 4096) hipLaunchKernelGGL((k_ev_pick<1024, 4>), gp, dim3(1024), 0, ST(s), a);
+    else if (cap <= 8192) hipLaunchKernelGGL((k_ev_pick<1024, 8>), gp, dim3(1024), 0, ST(s), a);
+    else hipLaunchKernelGGL(k_ev_pick_long, gp, dim3(EV_T), (size_t)a.lds_keys * 4, ST(s), a);
     const int rows = 4 * 256 / (p->head_dim / 8);
     int z = (keep + rows - 1) / rows;
     if (z > 1024) z = 1024;

@@ -223,3 +223,28 @@ def test_evict_long_rows(eng, hip):
     cache = R.Cache(hip, rng, R.F16, [0], [40000], 1, 64, 1024)
     say("evict: 40 000 rows")
     evict(eng, hip, cache, 37000, 4, 100, 256, False)
+
+
+@pytest.mark.parametrize("extra", [0, 100, 200, 400, 700])
+@pytest.mark.parametrize("keep,sink,recent", [(50, 3, 9), (1500, 0, 0), (60, 30, 30)])
+def test_evict_under_longer_tables(eng, hip, keep, sink, recent, extra):
+    """Tables that allow for more rows than the sequences have: selection from
+    registers, by every number of keys a thread, and from LDS."""
+    rng = np.random.default_rng(keep + extra)
+    cache = R.Cache(hip, rng, R.BF16, [0] * 5, [1600, 0, 59, 61, 1100], 2, 64, 16, table_extra=2 + extra,
+                    bad=[(0, 7), (0, 99), (4, 0)])
+    cache.w = np.where(rng.random(cache.w.shape) < 0.3, np.float32(0.25), cache.w)       # ties
+    cache.w.flat[::97] = -np.inf
+    cache.w.flat[::89] = np.inf
+    cache.w.flat[::83] = np.nan
+    cache.dw.set(cache.w)
+    say(f"evict: keep {keep} sink {sink} recent {recent}, {extra} spare table entries")
+    evict(eng, hip, cache, keep, sink, recent, 32, False)
+
+
+@pytest.mark.parametrize("ctx,keep", [([2047], 1000), ([4080, 30], 2000), ([8176], 3001), ([8193], 3001)])
+def test_evict_at_the_ends_of_the_ranges(eng, hip, ctx, keep):
+    rng = np.random.default_rng(keep)
+    cache = R.Cache(hip, rng, R.F16, [0] * len(ctx), ctx, 1, 64, 16, table_extra=0)
+    say(f"evict: {ctx} rows to {keep}")
+    evict(eng, hip, cache, keep, 4, 32, 64, False)
