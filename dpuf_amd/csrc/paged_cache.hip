@@ -472,12 +472,25 @@ struct EvArgs {
     DpufAmdBatch b;
     DpufAmdPages p, d;
     int shift, dshift;
-    int keep, sink, recent;
+    int keep;
     const int* dtable;
     int dstride;
-    int* kept;
-    int* new_len;
-    int lds_keys;
+    const int* kept;
+};
+// What the selection reads: below 112 bytes of arguments a launch takes the
+// host 2.7 us, above 3.7.
+struct PickArgs {
+    const int *ctx_len, *table;
+    const float* w;
+    int *kept, *new_len;
+    int table_stride, shift, n_pages, nkv;
+    int keep, sink, recent, lds_keys;
+    DEV int ctx(int s) const { return min(max(ctx_len[s], 0), table_stride << shift); }
+    DEV int page(int s, int i) const { return table[(size_t)s * table_stride + (i >> shift)]; }
+    // weight of cached row i of kv head h, on page p of the pool
+    DEV float weight(int p, int h, int i) const {
+        return w[((((size_t)p * nkv + h) << shift) | (unsigned)(i & ((1 << shift) - 1)))];
+    }
 };
 
 // Larger weight, larger integer; NaN and absent rows are 0, below every
@@ -515,7 +528,7 @@ DEV void scan2(int& x, int& y, int& tx, int& ty, int (*sums)[2]) {
 
 // Longer rows: keys in LDS, or read again in every pass where it does not hold
 // them (17 us for eight sequences of up to 9 000 rows).
-__global__ __launch_bounds__(EV_T) void k_ev_pick_long(EvArgs a) {
+__global__ __launch_bounds__(EV_T) void k_ev_pick_long(PickArgs a) {
     extern __shared__ __align__(16) uint32_t keys[];
     __shared__ int hist[EV_T];
     __shared__ int sums[EV_T / 64][2];
@@ -523,9 +536,9 @@ __global__ __launch_bounds__(EV_T) void k_ev_pick_long(EvArgs a) {
     __shared__ uint32_t sh_digit;
     __shared__ int sh_need;
     const int kvh = blockIdx.x, s = blockIdx.y, t = threadIdx.x;
-    const int c = pg_ctx(a.b, a.shift, s), n = min(c, a.keep);
+    const int c = a.ctx(s), n = min(c, a.keep);
     if (kvh == 0 && t == 0) a.new_len[s] = n;
-    int* kept = a.kept + ((size_t)s * a.p.n_kv_heads + kvh) * a.keep;
+    int* kept = a.kept + ((size_t)s * a.nkv + kvh) * a.keep;
     if (c <= a.keep) {
         for (int i = t; i < n; i += EV_T) kept[i] = i;
         return;
@@ -534,9 +547,9 @@ __global__ __launch_bounds__(EV_T) void k_ev_pick_long(EvArgs a) {
     const int mid = hi - lo;
     const bool staged = mid <= a.lds_keys;
     auto fetch = [&](int i) -> uint32_t {
-        const int slot = lo + i, page = pg_page(a.b, a.shift, s, slot);
-        if ((unsigned)page >= (unsigned)a.p.n_pages) return 0;
-        return weight_key(a.p.w[((size_t)page * a.p.n_kv_heads + kvh) * a.p.page_size + (slot & (a.p.page_size - 1))]);
+        const int slot = lo + i, page = a.page(s, slot);
+        if ((unsigned)page >= (unsigned)a.n_pages) return 0;
+        return weight_key(a.weight(page, kvh, slot));
     };
     // the bits in which keys differ, and with a row that fits the keys in LDS
     uint32_t any = 0, all = ~0u;
@@ -546,13 +559,12 @@ __global__ __launch_bounds__(EV_T) void k_ev_pick_long(EvArgs a) {
         float w[AT];
 #pragma unroll
         for (int u = 0; u < AT; u++)
-            if (i0 + u * EV_T < mid) pg[u] = pg_page(a.b, a.shift, s, lo + min(i0 + u * EV_T + t, mid - 1));
+            if (i0 + u * EV_T < mid) pg[u] = a.page(s, lo + min(i0 + u * EV_T + t, mid - 1));
 #pragma unroll
         for (int u = 0; u < AT; u++)
             if (i0 + u * EV_T < mid) {
-                const int in_page = (lo + min(i0 + u * EV_T + t, mid - 1)) & (a.p.page_size - 1);
-                const bool in = (unsigned)pg[u] < (unsigned)a.p.n_pages;
-                w[u] = a.p.w[((size_t)(in ? pg[u] : 0) * a.p.n_kv_heads + kvh) * a.p.page_size + in_page];
+                const bool in = (unsigned)pg[u] < (unsigned)a.n_pages;
+                w[u] = a.weight(in ? pg[u] : 0, kvh, lo + min(i0 + u * EV_T + t, mid - 1));
                 if (!in) pg[u] = -1;
             }
 #pragma unroll
@@ -635,7 +647,7 @@ __global__ __launch_bounds__(EV_T) void k_ev_pick_long(EvArgs a) {
 // Rows of at most NT AT keys: they stay in registers, key u NT + t of the middle
 // with thread t, and the places of the rows that stay follow from ballots, in
 // row order.
-template <int NT, int AT> __global__ __launch_bounds__(NT) void k_ev_pick(EvArgs a) {
+template <int NT, int AT> __global__ __launch_bounds__(NT) void k_ev_pick(PickArgs a) {
     constexpr int BINS = 1024, OWN = BINS / NT, NW = NT / 64, CELLS = AT * NW, LC = (CELLS + 63) / 64;
     __shared__ int hist[BINS];
     __shared__ int sums[NW];
@@ -644,9 +656,9 @@ template <int NT, int AT> __global__ __launch_bounds__(NT) void k_ev_pick(EvArgs
     __shared__ int sh_need;
     __shared__ int cells[2][64 * LC];      // rows above the cut, equal to it, of 64 consecutive ones
     const int kvh = blockIdx.x, s = blockIdx.y, t = threadIdx.x, lane = t & 63, wave = t >> 6;
-    const int c = pg_ctx(a.b, a.shift, s), n = min(c, a.keep);
+    const int c = a.ctx(s), n = min(c, a.keep);
     if (kvh == 0 && t == 0) a.new_len[s] = n;
-    int* kept = a.kept + ((size_t)s * a.p.n_kv_heads + kvh) * a.keep;
+    int* kept = a.kept + ((size_t)s * a.nkv + kvh) * a.keep;
     if (c <= a.keep) {
         for (int i = t; i < n; i += NT) kept[i] = i;
         return;
@@ -656,13 +668,12 @@ template <int NT, int AT> __global__ __launch_bounds__(NT) void k_ev_pick(EvArgs
     uint32_t k[AT];
 #pragma unroll
     for (int u = 0; u < AT; u++)
-        if (u * NT < mid) pg[u] = pg_page(a.b, a.shift, s, lo + min(u * NT + t, mid - 1));
+        if (u * NT < mid) pg[u] = a.page(s, lo + min(u * NT + t, mid - 1));
 #pragma unroll
     for (int u = 0; u < AT; u++) {
         if (u * NT >= mid) continue;
-        const int in_page = (lo + min(u * NT + t, mid - 1)) & (a.p.page_size - 1);
-        const bool in = (unsigned)pg[u] < (unsigned)a.p.n_pages;
-        const float w = a.p.w[((size_t)(in ? pg[u] : 0) * a.p.n_kv_heads + kvh) * a.p.page_size + in_page];
+        const bool in = (unsigned)pg[u] < (unsigned)a.n_pages;
+        const float w = a.weight(in ? pg[u] : 0, kvh, lo + min(u * NT + t, mid - 1));
         k[u] = in ? weight_key(w) : 0;
     }
     for (int i = t; i < a.sink; i += NT) kept[i] = i;
@@ -972,23 +983,33 @@ void dpuf_hip_paged_evict(void* s, const DpufAmdBatch* b, const DpufAmdPages* p,
     a.shift = __builtin_ctz(p->page_size);
     a.dshift = __builtin_ctz(d->page_size);
     a.keep = keep;
-    a.sink = sink;
-    a.recent = recent;
     a.dtable = dtable;
     a.dstride = dstride;
     a.kept = kept;
-    a.new_len = new_len;
+    PickArgs k;
+    k.ctx_len = b->ctx_len;
+    k.table = b->page_table;
+    k.w = p->w;
+    k.kept = kept;
+    k.new_len = new_len;
+    k.table_stride = b->table_stride;
+    k.shift = a.shift;
+    k.n_pages = p->n_pages;
+    k.nkv = p->n_kv_heads;
+    k.keep = keep;
+    k.sink = sink;
+    k.recent = recent;
     const int64_t cap = (int64_t)b->table_stride * p->page_size;
     const dim3 gp(p->n_kv_heads, b->n_seqs);
-    a.lds_keys = (int)(cap < 36864 ? cap : 36864);      // 144 KB of the 160
+    k.lds_keys = (int)(cap < 36864 ? cap : 36864);      // 144 KB of the 160
     // what the tables bound the rows by; the whole call, one sequence of 8 kv
     // heads: 1 290 rows 14.4 us by the long rows' kernel, 12.7 by <1024, 4>,
     // 11.6 by <512, 4>; 4 000 rows 17.2 and 14.6; 8 000 rows 23.3, and 21.3 by
     // <1024, 8>; 9 000 rows 24.1, and 25.4 by <1024, 16>
-    if (cap <= 2048) hipLaunchKernelGGL((k_ev_pick<512, 4>), gp, dim3(512), 0, ST(s), a);
-    else if (cap <= 4096) hipLaunchKernelGGL((k_ev_pick<1024, 4>), gp, dim3(1024), 0, ST(s), a);
-    else if (cap <= 8192) hipLaunchKernelGGL((k_ev_pick<1024, 8>), gp, dim3(1024), 0, ST(s), a);
-    else hipLaunchKernelGGL(k_ev_pick_long, gp, dim3(EV_T), (size_t)a.lds_keys * 4, ST(s), a);
+    if (cap <= 2048) hipLaunchKernelGGL((k_ev_pick<512, 4>), gp, dim3(512), 0, ST(s), k);
+    else if (cap <= 4096) hipLaunchKernelGGL((k_ev_pick<1024, 4>), gp, dim3(1024), 0, ST(s), k);
+    else if (cap <= 8192) hipLaunchKernelGGL((k_ev_pick<1024, 8>), gp, dim3(1024), 0, ST(s), k);
+    else hipLaunchKernelGGL(k_ev_pick_long, gp, dim3(EV_T), (size_t)k.lds_keys * 4, ST(s), k);
     const int rows = 4 * 256 / (p->head_dim / 8);
     int z = (keep + rows - 1) / rows;
     if (z > 1024) z = 1024;
