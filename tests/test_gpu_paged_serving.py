@@ -198,3 +198,88 @@ def test_arguments_that_share_memory_are_refused(eng, hip):
         assert sample(**kw) == -1, kw
     hip.sync()
     hip.lib.hipStreamDestroy(st.stream)
+
+
+def test_pools_beyond_32_bits(eng, hip):
+    """Pages 2^27 elements apart, 24 of them: the same bits as side by side."""
+    rng = np.random.default_rng(6)
+    rows, ctx, page = [1, 70, 0, 2], [130, 90, 3, 60], 16
+    c = R.Cache(hip, rng, R.F16, rows, ctx, NKV, 64, page)
+    stride, size = 1 << 27, page * NKV * 64
+    far = []
+    print("far pages", flush=True)
+    for pool in (c.k, c.v):
+        d = C.c_void_p()
+        assert hip.lib.hipMalloc(C.byref(d), c.n * stride * 2) == 0
+        far.append(d.value)
+        for p in range(c.n):
+            assert hip.lib.hipMemcpy(d.value + p * stride * 2, pool[p].ctypes.data, size * 2, R.H2D) == 0
+    assert c.n >= 20
+    dw = hip.put(c.w)
+    near, wide = c.pages(), c.pages(dw=dw)
+    wide.k, wide.v, wide.page_stride = far[0], far[1], stride
+    qkv = hip.put(rng.standard_normal((c.n_rows, (4 + 2 * NKV) * 64)).astype(np.float32))
+    turns = hip.put(1e4 ** (-np.arange(32) / 32) / 6.283185307179586)
+    rope = abi.DpufAmdRope(turns=turns.p, rot_dim=64, interleaved=1, scale=1.0)
+    pos = hip.put(np.arange(c.n_rows, dtype=np.int32))
+    got = []
+    for p in (near, wide):
+        b, w = c.batch(), (4 + 2 * NKV) * 64
+        dq, do = hip.put(np.zeros((c.n_rows, 4, 64), np.uint16)), hip.put(np.zeros((c.n_rows, 4, 64), np.uint16))
+        dl, kept = hip.put(np.zeros((c.n_rows, 4), np.float32)), hip.put(np.zeros((4, NKV, 40), np.int32))
+        new = hip.put(np.zeros(4, np.int32))
+        dst = R.Cache(hip, np.random.default_rng(7), R.F16, [0] * 4, [40] * 4, NKV, 64, page)
+        assert eng.dpuf_amd_rope_append(C.byref(b), C.byref(p), C.byref(rope), pos.p, R.F32, 4, qkv.p, qkv.p + 4 * 256,
+                                        qkv.p + (4 + NKV) * 256, w, w, w, None, None, 0.0, dq.p, None) == 0
+        n = int(eng.dpuf_amd_paged_attn_workspace(C.byref(b), C.byref(p), 4))
+        ws = hip.put(np.zeros(max(n, 16), np.uint8))
+        assert eng.dpuf_amd_paged_attn(C.byref(b), C.byref(p), 4, dq.p, 0.1, R.F16, do.p, dl.p, ws.p, n, None) == 0
+        assert eng.dpuf_amd_paged_attn_weights(C.byref(b), C.byref(p), 4, dq.p, 0.1, dl.p, 0.5, p.w, None) == 0
+        dp = dst.pages()
+        assert eng.dpuf_amd_paged_evict(C.byref(b), C.byref(p), 40, 1, 4, C.byref(dp), dst.d_table.p,
+                                        dst.table.shape[1], kept.p, new.p, None) == 0
+        got.append([x.get().tobytes() for x in (dq, do, dl, kept, new, dst.dk, dst.dv, dst.dw)])
+    assert got[0] == got[1]
+    back = np.empty_like(c.k)
+    for f, d in zip(far, (c.dk, c.dv)):
+        want = d.get()
+        for p in range(c.n):
+            assert hip.lib.hipMemcpy(back[p].ctypes.data, f + p * stride * 2, size * 2, R.D2H) == 0
+        assert np.array_equal(back, want)
+        hip.lib.hipFree(f)
+    assert np.array_equal(dw.get().view(np.uint32), c.dw.get().view(np.uint32))
+
+
+def test_many_sequences(eng, hip):
+    """Hundreds of sequences of none to a few rows and one chunk among them."""
+    rng = np.random.default_rng(8)
+    n = 700
+    ctx = rng.integers(0, 50, n).tolist()
+    rows = [int(rng.integers(0, min(4, c + 1))) for c in ctx]
+    ctx[333], rows[333] = 200, 150
+    c = R.Cache(hip, rng, R.BF16, rows, ctx, 1, 64, 16)
+    q = R.to_type(rng.standard_normal((c.n_rows, 4, 64)), R.BF16)
+    dq, do = hip.put(q), hip.put(np.zeros((c.n_rows, 4, 64), np.float32))
+    dl = hip.put(np.zeros((c.n_rows, 4), np.float32))
+    ref, rl, A, S, vmax, fresh = R.attention(c, R.from_type(q, R.BF16), float(np.float32(0.1)), 4)
+    bound = R.attention_bound(R.BF16, R.F32, ref, A, S, vmax, 64, 200)
+    seen = np.isfinite(rl)
+    for max_ctx in (50, 3000):
+        print(f"{n} sequences, max_ctx {max_ctx}", flush=True)
+        b, p = c.batch(max_ctx=max_ctx), c.pages()
+        b.table_stride = c.table.shape[1]
+        ws_n = int(eng.dpuf_amd_paged_attn_workspace(C.byref(b), C.byref(p), 4))
+        ws = hip.put(np.full(max(ws_n, 16), 0xFF, np.uint8))
+        assert eng.dpuf_amd_paged_attn(C.byref(b), C.byref(p), 4, dq.p, 0.1, R.F32, do.p, dl.p, ws.p, ws_n, None) == 0
+        out, lse = do.get(), dl.get()
+        assert np.all(np.abs(out - ref) <= bound)
+        assert np.array_equal(np.isneginf(lse), ~seen)
+        c.dw.set(c.w)
+        assert eng.dpuf_amd_paged_attn_weights(C.byref(b), C.byref(p), 4, dq.p, 0.1, dl.p, 1.0, None, None) == 0
+        w = c.dw.get()
+        # as the weights' own tests: two score errors, the log sum's rounding, sums of every row's share
+        rel = 2 * R.score_error(S.max(), 64) + np.abs(rl[seen]).max() * 2.0 ** -22 + 2.0 ** -20 + 640 * 2.0 ** -24
+        for s in range(n):
+            for i in range(ctx[s]):
+                x = w[c.table[s, i // 16], 0, i % 16]
+                assert abs(x - fresh[s][0, i]) <= rel * fresh[s][0, i] + 1e-30, (s, i)
