@@ -117,7 +117,9 @@ template <typename T> DEV f32x4 odd4(const uint16_t* v) {
 // (kv head, sequence and tile of 16 packed rows, key range); its four waves
 // take every fourth tile of 32 keys with sums of their own and meet in LDS at
 // the end, so there is no barrier in the loop and each wave keeps a whole
-// next tile (K and V, 16 KB at 128 columns) in flight in registers.
+// next tile (K and V, 16 KB at 128 columns) in flight in registers.  48 rows of
+// 32 heads, 8 kv heads of 128 over 310 to 6 000 keys: 119 us, 5.2 TB/s; one row
+// of 16 heads over 75 keys 7.4.
 // ---------------------------------------------------------------------------
 template <int HD> struct FewLds {
     static constexpr int PITCH = HD + 16;   // elements of a V row: 4 rows of a transposing read in 4 bank groups
@@ -356,7 +358,10 @@ template <typename T, int HD> DEV void few_rows(const PaArgs& a, FewLds<HD>& sh,
 // of them: while one is computed, the other takes the tile after it from
 // registers, whose loads were issued a tile earlier.  Two workgroups of four
 // waves a CU, whose vector and matrix work overlap, or one of eight, which
-// loads and stores half the tiles for the same rows.
+// loads and stores half the tiles for the same rows.  512 rows of 32 heads, 8
+// kv heads of 128 over 16 384 keys: 150 to 170 us, 800 to 900 TFLOP/s; the
+// reads of K and V from LDS (32 rows a wave use each) take as long as the
+// matrix instructions.
 // ---------------------------------------------------------------------------
 template <int HD> struct ManyLds {
     static constexpr int KT = HD == 256 ? 32 : 64;
@@ -654,7 +659,8 @@ __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void k_pa_mixed(PaArgs a, i
 }
 
 // Joins the key ranges of rows that were split: HD / 4 lanes a (row, head),
-// four ranges' partials in flight.
+// four ranges' partials in flight: 512 rows of 32 heads in four ranges 7.6 us,
+// 4.7 TB/s.
 template <typename T, int HD>
 __global__ __launch_bounds__(256) void k_pa_join(PaArgs a) {
     constexpr int LPR = HD / 4, PER = 256 / LPR;
