@@ -658,48 +658,62 @@ __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void k_pa_mixed(PaArgs a, i
     }
 }
 
-// Joins the key ranges of rows that were split: HD / 4 lanes a (row, head),
-// four ranges' partials in flight: 512 rows of 32 heads in four ranges 7.6 us,
-// 4.7 TB/s.
-template <typename T, int HD>
+// Joins the key ranges of rows that were split: HD / 4 lanes a (row, head) and
+// ZG groups of them, each with every ZG-th range, four of a group's in flight,
+// their sums joined in LDS: 512 rows of 32 heads in four ranges 7.6 us, 4.7 TB/s.
+template <typename T, int HD, int ZG>
 __global__ __launch_bounds__(256) void k_pa_join(PaArgs a) {
-    constexpr int LPR = HD / 4, PER = 256 / LPR;
-    const int lane = threadIdx.x & 63, row = blockIdx.x;
-    const int head = blockIdx.y * PER + threadIdx.x / LPR, d = 4 * (threadIdx.x % LPR);
+    constexpr int LPR = HD / 4, PER = 256 / LPR / ZG;
+    __shared__ float2 sml[ZG][PER];
+    __shared__ f32x4 so[ZG > 1 ? ZG : 1][PER * LPR];
+    const int lane = threadIdx.x & 63, row = blockIdx.x, unit = threadIdx.x / LPR, zg = unit / PER;
+    const int head = blockIdx.y * PER + unit % PER, d = 4 * (threadIdx.x % LPR);
     const int s = pg_seq_of_row(a.b, row, lane);
     if (s < 0) return;
     const PgSeq sq = pg_seq(a.b, a.shift, s);
     const bool few = a.only == PA_FEW || (a.only == PA_BOTH && sq.n * a.G <= a.few);
     const int per = range_keys(sq.ctx, few ? a.chunk_few : a.chunk_many, few ? a.nz_few : a.nz_many);
     const int ranges = sq.ctx > per ? (sq.ctx + per - 1) / per : 1;
-    if (ranges == 1 || row >= sq.r0 + sq.n || head >= a.nq) return;
-    const int kvh = head / a.G;
-    const size_t at = (size_t)row * a.nq + head, total = (size_t)a.b.n_rows * a.nq;
-    const size_t first = few ? few_at(a, 0, s, kvh, (row - sq.r0) * a.G + head - kvh * a.G, at) : at;
+    if (ranges == 1 || row >= sq.r0 + sq.n) return;
+    const bool live = head < a.nq;
+    const int hd = live ? head : a.nq - 1, kvh = hd / a.G;
+    const size_t at = (size_t)row * a.nq + hd, total = (size_t)a.b.n_rows * a.nq;
+    const size_t first = few ? few_at(a, 0, s, kvh, (row - sq.r0) * a.G + hd - kvh * a.G, at) : at;
     const size_t step = few && a.only == PA_BOTH ? (size_t)a.b.n_seqs * a.p.n_kv_heads * a.few : total;
     const float2* mls = (few ? a.few_ml : a.many_ml) + first;
     const float* os = (few ? a.few_o : a.many_o) + first * HD + d;
     float M = NEG_INF, L = 0.0f;
     f32x4 o = {0.f, 0.f, 0.f, 0.f};
-    for (int z0 = 0; z0 < ranges; z0 += 4) {
+    auto add = [&](float m, float l, f32x4 p) {
+        const float mn = fmaxf(M, m), ms = mn == NEG_INF ? 0.0f : mn;
+        const float f0 = __builtin_amdgcn_exp2f(M - ms), f1 = __builtin_amdgcn_exp2f(m - ms);
+        L = L * f0 + l * f1;
+        o = o * f0 + p * f1;
+        M = mn;
+    };
+    for (int z0 = zg; z0 < ranges; z0 += 4 * ZG) {
         float2 ml[4];
         f32x4 po[4];
 #pragma unroll
         for (int e = 0; e < 4; e++) {
-            const size_t z = min(z0 + e, ranges - 1) * step;
+            const size_t z = min(z0 + e * ZG, ranges - 1) * step;
             ml[e] = mls[z];
             po[e] = *(const f32x4*)(os + z * HD);
         }
 #pragma unroll
-        for (int e = 0; e < 4; e++) {
-            if (z0 + e >= ranges) break;
-            const float mn = fmaxf(M, ml[e].x), ms = mn == NEG_INF ? 0.0f : mn;
-            const float f0 = __builtin_amdgcn_exp2f(M - ms), f1 = __builtin_amdgcn_exp2f(ml[e].x - ms);
-            L = L * f0 + ml[e].y * f1;
-            o = o * f0 + po[e] * f1;
-            M = mn;
-        }
+        for (int e = 0; e < 4; e++)
+            if (z0 + e * ZG < ranges) add(ml[e].x, ml[e].y, po[e]);
     }
+    if constexpr (ZG > 1) {
+        const int own = threadIdx.x % (PER * LPR);
+        if (d == 0) sml[zg][unit % PER] = make_float2(M, L);
+        so[zg][own] = o;
+        __syncthreads();
+        if (zg > 0) return;
+#pragma unroll
+        for (int z = 1; z < ZG; z++) add(sml[z][unit % PER].x, sml[z][unit % PER].y, so[z][own]);
+    }
+    if (!live) return;
     const float inv = L > 0.0f ? 1.0f / L : L == 0.0f ? 0.0f : L;
     const float ov[4] = {o[0], o[1], o[2], o[3]};
     put4<T>(a, at * HD + d, ov, inv);
@@ -727,12 +741,13 @@ int range_of(int64_t ctx, double times) { return ((int)(times * sqrt((double)ctx
 // packed rows (a tile of 16; two where a single row has more than 16 query
 // heads per kv head) or more.
 //
-// How many ranges the keys are split into: enough to fill the card, but a
-// range costs its workgroup's start and a partial result, so that the best
-// length grows like the square root of the context.  One row of 32 heads, 8
-// kv heads: over 1 500 keys 22 us in ranges of 1 024, 15.5 in 512, 13.4 in
-// 256, 13.7 in 128; over 4 096 23, 18.0, 18.1, 21; over 16 384 28.7, 30, 41,
-// 64; over 300 10.0 in one, 11.8 in two.
+// Key ranges of decoding sequences: of 128 keys or more, such that every CU has
+// one, but not so long that a batch's shorter sequences leave them idle.  One
+// row of 32 heads, 8 kv heads of 128: over 1 500 keys 22.3 us in ranges of
+// 1 024, 15.9 in 512, 12.6 in 256, 10.7 in 128; over 4 096 22.6, 15.7, 12.6,
+// 10.6; over 16 384 23.9, 19.8, 20.9, 20.8; over 300 10.7 in one, 9.8 in three.
+// 16 rows over 500 to 8 000 keys 56.2, 53.7, 53.4, 61.6; 48 rows 160.5, 164,
+// 164, 172.
 PaPlan plan(const DpufAmdBatch& b, const DpufAmdPages& p, int nq) {
     const int G = nq / p.n_kv_heads;
     PaPlan r;
@@ -747,12 +762,14 @@ PaPlan plan(const DpufAmdBatch& b, const DpufAmdPages& p, int nq) {
     r.y_few = r.only >= PA_MANY ? 0 : b.n_seqs * ((r.few + 15) / 16);
     r.y_many = r.only == PA_FEW ? 0 : r.only == PA_BOTH ? (int)(packed / 128 + (most < b.n_seqs ? most : b.n_seqs))
                                                         : ceil_div(packed, tr);
-    r.chunk_few = ctx <= 512 ? 512 : range_of(ctx, 8.0);
+        const int64_t units = (int64_t)b.n_seqs * p.n_kv_heads;
+    const int64_t even = (ctx * units / 256 + 127) & ~127, long_few = units >= 256 ? 1024 : 512;
+    r.chunk_few = ctx <= 512 || even > long_few ? (int)long_few : even < 128 ? 128 : (int)even;
     r.nz_few = ceil_div(ctx, r.chunk_few);
     if (r.nz_few > 64) r.nz_few = 64;
     // (kv heads x sequences) that fill the card by themselves need no ranges,
     // and the partial sums stay below 16 384 x `few` rows
-    const int64_t cap_z = 16384 / ((int64_t)b.n_seqs * p.n_kv_heads);
+    const int64_t cap_z = 16384 / units;
     if (r.nz_few > cap_z) r.nz_few = cap_z < 1 ? 1 : (int)cap_z;
     // as many ranges of a chunk's keys as fit on the card beside its tiles at
     // once: two workgroups of 128 rows a CU, or one of 256.  Beside decoding
@@ -787,8 +804,19 @@ void launch(const PaArgs& a, const PaPlan& pl, hipStream_t st) {
     } else
         hipLaunchKernelGGL((k_pa_mixed<T, HD>), dim3(nkv * (pl.y_many * pl.nz_many + pl.y_few * pl.nz_few)), dim3(256),
                            0, st, a, pl.y_many, pl.y_few);
-    if (pl.few_rows + pl.many_rows > 0)
-        hipLaunchKernelGGL((k_pa_join<T, HD>), dim3(a.b.n_rows, ceil_div(a.nq, 256 / (HD / 4))), dim3(256), 0, st, a);
+    if (pl.few_rows + pl.many_rows > 0) {
+        constexpr int ZG = HD == 256 ? 4 : 8;
+        const int nz = pl.nz_few > pl.nz_many ? pl.nz_few : pl.nz_many;
+        // few rows of many ranges wait for their loads (one row over 65 536
+        // keys in 64 ranges 52 us, 58 by one group), many are bound by bytes
+        // (a mixed batch of 269 rows of 32 heads, 7 ranges: 60.8 and 53)
+        if (nz > 4 && (int64_t)a.b.n_rows * a.nq <= 4096)
+            hipLaunchKernelGGL((k_pa_join<T, HD, ZG>), dim3(a.b.n_rows, ceil_div(a.nq, 256 / (HD / 4) / ZG)), dim3(256),
+                               0, st, a);
+        else
+            hipLaunchKernelGGL((k_pa_join<T, HD, 1>), dim3(a.b.n_rows, ceil_div(a.nq, 256 / (HD / 4))), dim3(256), 0, st,
+                               a);
+    }
     LAUNCHED("k_pa");
 }
 
