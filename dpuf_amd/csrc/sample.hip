@@ -56,7 +56,17 @@ constexpr int MAX_CHUNKS = 64;   // a wave's lanes take a row's chunks
 
 enum { SM_DONE = 0, SM_PLAIN, SM_LIST, SM_BINS, SM_SPLIT };
 
+// A row's settings.
+struct Settings {
+    float M;                     // the largest logit; 0 where that is infinite (then only its like are left)
+    float bins;                  // bins per logit
+    int inf, k, by_k, by_p, by_m;
+    double invT, p_goal;
+    double min_w, edge;          // 2^S min_p (0: off) and -T ln min_p
+};
+
 struct SmState {
+    Settings set;
     unsigned tick[2], n_list;
     int mode;
     int by_k, by_p, by_m;        // settings that cut something
@@ -171,17 +181,10 @@ template <typename L, int N = NT, typename F> DEV void each(const void* p, int v
     for (int i = done + t; i < hi; i += N) f(i, L::one(p, i));
 }
 
-// A row with its settings.
-template <typename L> struct Row {
+template <typename L> struct Row : Settings {
     const void* p;
     const double* table;         // SIXTEENTHS in LDS
     int V, S, vec;
-    float M;                     // the largest logit; 0 where that is infinite (then only its like are left)
-    bool inf;
-    double invT, p_goal;
-    float bins;                  // bins per logit
-    int k, by_k, by_p, by_m;
-    double min_w, edge;          // 2^S min_p (0: off) and -T ln min_p
 
     DEV double below(float x) const {      // the largest logit less x
         if (inf) x = x == __builtin_huge_valf() ? 0.0f : -__builtin_huge_valf();
@@ -563,6 +566,7 @@ template <typename L> __global__ __launch_bounds__(NT) void k_smp_hist(SmArgs a)
         }
         return;
     }
+    if (c == 0 && t == 0) st->set = row;
     const int lo = c * a.chunk, hi = min(a.V, lo + a.chunk);
     if (!row.by_k && !row.by_p) {
         // a sum for each wave's quarter of the chunk
@@ -971,9 +975,7 @@ template <typename L> __global__ __launch_bounds__(NT) void k_smp_pick(SmArgs a)
     Row<L> row;
     row.open(a, r, sh.table);
     load_table(sh.table);
-    float least;
-    const uint64_t best = row_best(a, r, &least);
-    row.set(a, r, best, least);
+    (Settings&)row = sp->set;
     if (t == 0) sh.n_list = 0;
     __syncthreads();
     if (mode == SM_PLAIN) {
