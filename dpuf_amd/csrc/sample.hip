@@ -1070,6 +1070,7 @@ template <typename L> __global__ __launch_bounds__(NT) void k_smp_pick(SmArgs a)
         uint64_t s;
         const int at = select(sh, n, Want{BY_GOAL, 0, row.goal(sum)}, 0, st.wp, comp,
                               [&](int i) {
+                                  if (!st.by_k && !st.by_m) return true;     // a list of top-p's bins alone
                                   const int b = bin_of(i);
                                   return b >= st.pl && b <= st.ph;
                               },
@@ -1078,7 +1079,7 @@ template <typename L> __global__ __launch_bounds__(NT) void k_smp_pick(SmArgs a)
     }
     // what stays of the list
     for (int i = t; i < n; i += NT)
-        if (sh.list[i] < cut || row.weight_min(logit_of(sh.list[i])) == 0) sh.lw[i] = 0;
+        if (sh.list[i] < cut || (st.by_m && row.weight_min(logit_of(sh.list[i])) == 0)) sh.lw[i] = 0;
     __syncthreads();
     // the chunks' sums: the bins above the highest border, and what stays of
     // the list from there on
