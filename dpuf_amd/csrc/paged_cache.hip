@@ -529,7 +529,7 @@ DEV void scan2(int& x, int& y, int& tx, int& ty, int (*sums)[2]) {
 }
 
 // Longer rows: keys in LDS, or read again in every pass where it does not hold
-// them (17 us for eight sequences of up to 9 000 rows).
+// them (30 000 rows of one sequence to 4 096: 43 us with the move).
 __global__ __launch_bounds__(EV_T) void k_ev_pick_long(PickArgs a) {
     extern __shared__ __align__(16) uint32_t keys[];
     __shared__ int hist[EV_T];
@@ -761,44 +761,38 @@ template <int NT, int AT> __global__ __launch_bounds__(NT) void k_ev_pick(PickAr
         }
     }
     __syncthreads();
-    int ca[LC], ce[LC], sa = 0, se = 0;      // of the lane's cells, before which the lower lanes' lie
+    if (wave == 0) {         // the cells' counts become those of the cells before them
+        int ca[LC], ce[LC], sa = 0, se = 0;
 #pragma unroll
-    for (int e = 0; e < LC; e++) {
-        ca[e] = cells[0][LC * lane + e];
-        ce[e] = cells[1][LC * lane + e];
-        sa += ca[e];
-        se += ce[e];
-    }
-    int xa = sa, xe = se;
+        for (int e = 0; e < LC; e++) {
+            ca[e] = cells[0][LC * lane + e];
+            ce[e] = cells[1][LC * lane + e];
+            sa += ca[e];
+            se += ce[e];
+        }
+        int xa = sa, xe = se;
 #pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-        const int oa = __shfl_up(xa, d), oe = __shfl_up(xe, d);
-        if (lane >= d) xa += oa, xe += oe;
-    }
-    xa -= sa;
-    xe -= se;
+        for (int d = 1; d < 64; d <<= 1) {
+            const int oa = __shfl_up(xa, d), oe = __shfl_up(xe, d);
+            if (lane >= d) xa += oa, xe += oe;
+        }
+        xa -= sa;
+        xe -= se;
 #pragma unroll
-    for (int e = 0; e < LC; e++) {
-        const int na = ca[e], ne = ce[e];
-        ca[e] = xa;
-        ce[e] = xe;
-        xa += na;
-        xe += ne;
+        for (int e = 0; e < LC; e++) {
+            cells[0][LC * lane + e] = xa;
+            cells[1][LC * lane + e] = xe;
+            xa += ca[e];
+            xe += ce[e];
+        }
     }
+    __syncthreads();
     const uint64_t below = (1ull << lane) - 1;
 #pragma unroll
     for (int u = 0; u < AT; u++) {
         if (u * NT >= mid) continue;
-        const int cell = u * NW + wave;
-        int ba = 0, be = 0;
-#pragma unroll
-        for (int e = 0; e < LC; e++)
-            if (cell % LC == e) {
-                ba = __shfl(ca[e], cell / LC);
-                be = __shfl(ce[e], cell / LC);
-            }
-        ba += __popcll(above[u] & below);
-        be += __popcll(equal[u] & below);
+        const int ba = cells[0][u * NW + wave] + __popcll(above[u] & below);
+        const int be = cells[1][u * NW + wave] + __popcll(equal[u] & below);
         if (u * NT + t < mid && (k[u] > cut || (k[u] == cut && be < ties)))
             kept[a.sink + ba + min(be, ties)] = lo + u * NT + t;
     }
@@ -1006,11 +1000,14 @@ void dpuf_hip_paged_evict(void* s, const DpufAmdBatch* b, const DpufAmdPages* p,
     k.lds_keys = (int)(cap < 36864 ? cap : 36864);      // 144 KB of the 160
     // what the tables bound the rows by; the whole call, one sequence of 8 kv
     // heads: 1 290 rows 14.4 us by the long rows' kernel, 12.7 by <1024, 4>,
-    // 11.6 by <512, 4>; 4 000 rows 17.2 and 14.6; 8 000 rows 23.3, and 21.3 by
-    // <1024, 8>; 9 000 rows 24.1, and 25.4 by <1024, 16>
+    // 11.6 by <512, 4>; 4 000 rows 17.2 and 14.6; 8 000 rows 23.3, and 20 by
+    // <1024, 8>; 9 000 rows 23.5, and 22 by <1024, 12>; 16 000 rows 32.4, and
+    // 28.6 by <1024, 16>
     if (cap <= 2048) hipLaunchKernelGGL((k_ev_pick<512, 4>), gp, dim3(512), 0, ST(s), k);
     else if (cap <= 4096) hipLaunchKernelGGL((k_ev_pick<1024, 4>), gp, dim3(1024), 0, ST(s), k);
     else if (cap <= 8192) hipLaunchKernelGGL((k_ev_pick<1024, 8>), gp, dim3(1024), 0, ST(s), k);
+    else if (cap <= 12288) hipLaunchKernelGGL((k_ev_pick<1024, 12>), gp, dim3(1024), 0, ST(s), k);
+    else if (cap <= 16384) hipLaunchKernelGGL((k_ev_pick<1024, 16>), gp, dim3(1024), 0, ST(s), k);
     else hipLaunchKernelGGL(k_ev_pick_long, gp, dim3(EV_T), (size_t)k.lds_keys * 4, ST(s), k);
     const int rows = 4 * 256 / (p->head_dim / 8);
     int z = (keep + rows - 1) / rows;

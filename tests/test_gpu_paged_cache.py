@@ -248,3 +248,21 @@ def test_evict_at_the_ends_of_the_ranges(eng, hip, ctx, keep):
     cache = R.Cache(hip, rng, R.F16, [0] * len(ctx), ctx, 1, 64, 16, table_extra=0)
     say(f"evict: {ctx} rows to {keep}")
     evict(eng, hip, cache, keep, 4, 32, 64, False)
+
+
+@pytest.mark.parametrize("extra", [600, 1200])
+def test_evict_under_much_longer_tables(eng, hip, extra):
+    rng = np.random.default_rng(extra)
+    cache = R.Cache(hip, rng, R.F16, [0] * 3, [1600, 70, 1100], 2, 64, 16, table_extra=2 + extra, bad=[(0, 9)])
+    cache.w = np.where(rng.random(cache.w.shape) < 0.3, np.float32(0.25), cache.w)
+    cache.dw.set(cache.w)
+    say(f"evict: {extra} spare table entries")
+    evict(eng, hip, cache, 700, 4, 16, 32, True)
+
+
+@pytest.mark.parametrize("ctx,keep", [([12288], 5000), ([16384], 4097), ([16385, 5], 4097)])
+def test_evict_at_the_ends_of_the_longer_ranges(eng, hip, ctx, keep):
+    rng = np.random.default_rng(keep)
+    cache = R.Cache(hip, rng, R.BF16, [0] * len(ctx), ctx, 1, 64, 64, table_extra=0)
+    say(f"evict: {ctx} rows to {keep}")
+    evict(eng, hip, cache, keep, 0, 100, 64, False)
