@@ -1084,25 +1084,29 @@ template <typename L> __global__ __launch_bounds__(NT) void k_smp_pick(SmArgs a)
     // the chunks' sums: the bins above the highest border, and what stays of
     // the list from there on
     const int cb = min(cut ? row.bin_of(cut) : NB, st.by_m ? st.ml : NB), g = cb / GB;
-    // (a chunk a wave, eight chunks' loads at a time)
-    for (int k0 = wave; k0 < MAX_CHUNKS; k0 += 8 * NW) {
-        uint64_t s[8];
+    if (a.chunks == 1) {
+        uint64_t own = 0;
+        if (wave == 0)
+            for (int b = lane; b < cb; b += 64) own += a.wsum[(size_t)r * NB + b];
+        own = wave_scan64(own);
+        if (t == 63) sh.wsum[0] = own;
+    } else {
+        // a chunk a wave, the loads of CS at a time, all of them before any is waited for
+        constexpr int CS = 12;
+        const int fine = min(g * GB + (lane & (GB - 1)), NB - 1);
+        for (int k0 = wave; k0 < a.chunks; k0 += CS * NW) {
+            uint64_t sg[CS], sf[CS];
 #pragma unroll
-        for (int e = 0; e < 8; e++) {
-            const size_t at = (size_t)r * a.chunks + min(k0 + e * NW, a.chunks - 1);
-            s[e] = 0;
-            if (a.chunks == 1) {
-                if (k0 + e == 0)
-                    for (int b = lane; b < cb; b += 64) s[e] += a.wsum[at * NB + b];
-            } else {
-                if (lane < g) s[e] = get_agent(a.gsum + 2 * (at * NG + lane));
-                if (lane < cb - g * GB) s[e] += get_agent(a.wsum + at * NB + g * GB + lane);
+            for (int e = 0; e < CS; e++) {
+                const size_t at = (size_t)r * a.chunks + min(k0 + e * NW, a.chunks - 1);
+                sg[e] = get_agent(a.gsum + 2 * (at * NG + lane));
+                sf[e] = get_agent(a.wsum + at * NB + fine);
             }
-        }
 #pragma unroll
-        for (int e = 0; e < 8; e++) {
-            s[e] = wave_scan64(s[e]);
-            if (lane == 63) sh.wsum[k0 + e * NW] = k0 + e * NW < a.chunks ? s[e] : 0;
+            for (int e = 0; e < CS; e++) {
+                const uint64_t own = wave_scan64((lane < g ? sg[e] : 0) + (lane < cb - g * GB ? sf[e] : 0));
+                if (lane == 63 && k0 + e * NW < a.chunks) sh.wsum[k0 + e * NW] = own;
+            }
         }
     }
     __syncthreads();
