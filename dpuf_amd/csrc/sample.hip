@@ -20,7 +20,7 @@
 //               workgroup that ends last adds the chunks' bins up, groups of
 //               16 first, and finds the bins in which the prefixes end;
 //   k_smp_pick  collects the tokens that decide: all of the prefix's where
-//               they are at most one a thread, else those of the bins the
+//               they are at most LISTED, else those of the bins the
 //               borders lie in; the workgroup that ends last finds the borders
 //               among them and draws, from the list or, in index order, from
 //               the chunk in which the running sum passes the draw.
@@ -51,6 +51,7 @@ constexpr int FULL = 1000;       // of them for the tokens that surely have a we
 constexpr int GB = 16;           // bins of a group
 constexpr int NG = NB / GB;      // groups: a wave's lanes
 constexpr int CAP = 2048;        // tokens listed in LDS
+constexpr int LISTED = 128;      // tokens ranked as they are
 constexpr int ROWS = 1024;       // rows of one set of launches
 constexpr int MAX_CHUNKS = 64;   // a wave's lanes take a row's chunks
 
@@ -499,7 +500,7 @@ template <typename L> DEV void find_borders(const SmArgs& a, HistShared& sh, con
         } else {
             gk = sh.gc[last];
         }
-        if (n + gk <= NT) {
+        if (n + gk <= LISTED) {
             if (t == 0) {
                 st->by_k = g >= 0;
                 st->by_p = row.by_p;
@@ -544,7 +545,7 @@ template <typename L> DEV void find_borders(const SmArgs& a, HistShared& sh, con
         st->wk = k.w;
         st->wp = p0.w;
         st->total = tw;
-        st->mode = upto <= NT ? SM_LIST : in_s <= CAP ? SM_BINS : SM_SPLIT;
+        st->mode = upto <= LISTED ? SM_LIST : in_s <= CAP ? SM_BINS : SM_SPLIT;
     }
 }
 
@@ -920,30 +921,44 @@ template <typename L> DEV void split_row(const SmArgs& a, PickShared& sh, const 
     draw_range(a, sh, row, r, 0, row.V, 0, aim_of(a.u[r], total), total, kept);
 }
 
-// A list of at most a token a thread needs no selection: each thread adds up
-// what lies above its token and then what lies before it in two passes over
-// the list, which are shorter than selection's barriers (50 tokens of one row
-// of 151 936: 11.8 us for the launch against 14; up to a list's full length
-// selection, and then the draw from a chunk by bins, is the shorter: top-p 0.9
-// of one row 19.5 us against 28.9).
+// A list of at most LISTED tokens needs no selection: what lies above each
+// token, and then what lies before it, is added up in two passes over the list,
+// a quarter of it by each wave for two tokens a lane (50 to 100 tokens of one
+// row of 151 936: PICK us for the launch against 14 by selection; with 256
+// tokens by a thread each 26, selection and the draw from a chunk 16).
 template <typename L>
 DEV void answer_few(const SmArgs& a, PickShared& sh, const Row<L>& row, const SmState& st, int r, int n) {
-    const int t = threadIdx.x;
-    const uint64_t c = t < n ? sh.list[t] : 0, w = t < n ? sh.lw[t] : 0;
-    unsigned above = 0;
-    uint64_t before = 0;
-#pragma unroll 8
-    for (int j = 0; j < n; j++) {
-        const bool up = sh.list[j] > c;
-        above += up;
-        before += up ? sh.lw[j] : 0;
+    const int t = threadIdx.x, lane = t & 63, part = t >> 6;
+    static_assert(LISTED == 128 && NW == 4 && CAP >= LISTED + 8 * LISTED, "two tokens a lane, the parts behind the list");
+    uint64_t* parts = sh.list + LISTED;                  // [2][NW][LISTED]
+    const uint64_t c0 = sh.list[lane], c1 = sh.list[lane + 64];     // behind the list's end: not looked at
+    uint64_t n0 = 0, n1 = 0, w0 = 0, w1 = 0;
+#pragma unroll 4
+    for (int j = part; j < n; j += NW) {
+        const uint64_t cj = sh.list[j], wj = sh.lw[j];
+        n0 += cj > c0;
+        n1 += cj > c1;
+        w0 += cj > c0 ? wj : 0;
+        w1 += cj > c1 ? wj : 0;
     }
+    parts[part * LISTED + lane] = n0;
+    parts[part * LISTED + lane + 64] = n1;
+    parts[(NW + part) * LISTED + lane] = w0;
+    parts[(NW + part) * LISTED + lane + 64] = w1;
     if (t == 0) {
         sh.b0 = sh.b1 = 0;
         sh.red[0] = st.total;
     }
     __syncthreads();
-    if (st.by_k && t < n && above == (unsigned)row.k - 1) {
+    const uint64_t c = t < n ? sh.list[t] : 0, w = t < n ? sh.lw[t] : 0;
+    uint64_t above = 0, before = 0;
+    if (t < n)
+#pragma unroll
+        for (int e = 0; e < NW; e++) {
+            above += parts[e * LISTED + t];
+            before += parts[(NW + e) * LISTED + t];
+        }
+    if (st.by_k && t < n && above == (uint64_t)row.k - 1) {
         sh.b0 = c;
         sh.red[0] = before + w;
     }
@@ -952,15 +967,29 @@ DEV void answer_few(const SmArgs& a, PickShared& sh, const Row<L>& row, const Sm
     if (st.by_p && t < n && (double)before < goal && (double)(before + w) >= goal) sh.b1 = c;
     __syncthreads();
     const uint64_t cut = sh.b1 > sh.b0 ? sh.b1 : sh.b0;
-    const uint64_t left = c >= cut && t < n && row.weight_min(logit_of(c)) ? w : 0;
+    const uint64_t left = c >= cut && t < n && (!st.by_m || row.weight_min(logit_of(c))) ? w : 0;
     if (t < n) sh.lw[t] = left;
     __syncthreads();
     uint64_t total = 0;
-    before = 0;
-#pragma unroll 8
-    for (int j = 0; j < n; j++) {
-        total += sh.lw[j];
-        before += (uint32_t)sh.list[j] > (uint32_t)c ? sh.lw[j] : 0;     // a lower index
+    w0 = w1 = 0;
+#pragma unroll 4
+    for (int j = part; j < n; j += NW) {
+        const uint32_t ij = (uint32_t)sh.list[j];        // larger: a lower index
+        const uint64_t wj = sh.lw[j];
+        total += wj;
+        w0 += ij > (uint32_t)c0 ? wj : 0;
+        w1 += ij > (uint32_t)c1 ? wj : 0;
+    }
+    parts[part * LISTED + lane] = w0;
+    parts[part * LISTED + lane + 64] = w1;
+    if (lane == 0) sh.red[part] = total;
+    __syncthreads();
+    if (t >= n) return;
+    total = before = 0;
+#pragma unroll
+    for (int e = 0; e < NW; e++) {
+        total += sh.red[e];
+        before += parts[e * LISTED + t];
     }
     const uint64_t aim = aim_of(a.u[r], total);
     if (before <= aim && aim < before + left) answer(a, row, r, index_of(c), logit_of(c), total);
