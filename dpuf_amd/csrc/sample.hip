@@ -51,7 +51,7 @@ constexpr int FULL = 1000;       // of them for the tokens that surely have a we
 constexpr int GB = 16;           // bins of a group
 constexpr int NG = NB / GB;      // groups: a wave's lanes
 constexpr int CAP = 2048;        // tokens listed in LDS
-constexpr int LISTED = 128;      // tokens ranked as they are
+constexpr int LISTED = 256;      // tokens ranked as they are
 constexpr int ROWS = 1024;       // rows of one set of launches
 constexpr int MAX_CHUNKS = 64;   // a wave's lanes take a row's chunks
 
@@ -921,78 +921,94 @@ template <typename L> DEV void split_row(const SmArgs& a, PickShared& sh, const 
     draw_range(a, sh, row, r, 0, row.V, 0, aim_of(a.u[r], total), total, kept);
 }
 
-// A list of at most LISTED tokens needs no selection: what lies above each
-// token, and then what lies before it, is added up in two passes over the list,
-// a quarter of it by each wave for two tokens a lane (50 to 100 tokens of one
-// row of 151 936: PICK us for the launch against 14 by selection; with 256
-// tokens by a thread each 26, selection and the draw from a chunk 16).
-template <typename L>
-DEV void answer_few(const SmArgs& a, PickShared& sh, const Row<L>& row, const SmState& st, int r, int n) {
+// Of a list of at most LISTED tokens, for token t < n of sh.list: how many lie
+// above it (kABOVE: in descending order of composites, else in index order)
+// and their weight.  A quarter of the list by each wave for E tokens a lane, n
+// at most 64 E; *total gets the whole list's weight.
+template <bool kABOVE, int E>
+DEV void ranks_of(PickShared& sh, int n, uint64_t* above, uint64_t* before, uint64_t* total) {
+    static_assert(64 * E <= LISTED && CAP >= LISTED + NW * LISTED, "the parts lie behind the list");
     const int t = threadIdx.x, lane = t & 63, part = t >> 6;
-    static_assert(LISTED == 128 && NW == 4 && CAP >= LISTED + 8 * LISTED, "two tokens a lane, the parts behind the list");
-    uint64_t* parts = sh.list + LISTED;                  // [2][NW][LISTED]
-    const uint64_t c0 = sh.list[lane], c1 = sh.list[lane + 64];     // behind the list's end: not looked at
-    uint64_t n0 = 0, n1 = 0, w0 = 0, w1 = 0;
+    uint64_t *pn = sh.list + LISTED, *pw = sh.lw + LISTED;       // [NW][LISTED]
+    uint64_t c[E], na[E] = {}, wa[E] = {}, sum = 0;
+#pragma unroll
+    for (int e = 0; e < E; e++) c[e] = sh.list[lane + 64 * e];   // behind the list's end: not looked at
 #pragma unroll 4
     for (int j = part; j < n; j += NW) {
         const uint64_t cj = sh.list[j], wj = sh.lw[j];
-        n0 += cj > c0;
-        n1 += cj > c1;
-        w0 += cj > c0 ? wj : 0;
-        w1 += cj > c1 ? wj : 0;
+        sum += wj;
+#pragma unroll
+        for (int e = 0; e < E; e++) {
+            const bool up = kABOVE ? cj > c[e] : (uint32_t)cj > (uint32_t)c[e];      // larger: a lower index
+            if (kABOVE) na[e] += up;
+            wa[e] += up ? wj : 0;
+        }
     }
-    parts[part * LISTED + lane] = n0;
-    parts[part * LISTED + lane + 64] = n1;
-    parts[(NW + part) * LISTED + lane] = w0;
-    parts[(NW + part) * LISTED + lane + 64] = w1;
+#pragma unroll
+    for (int e = 0; e < E; e++) {
+        if (kABOVE) pn[part * LISTED + lane + 64 * e] = na[e];
+        pw[part * LISTED + lane + 64 * e] = wa[e];
+    }
+    if (lane == 0) sh.red[part] = sum;
+    __syncthreads();
+    *above = *before = *total = 0;
+#pragma unroll
+    for (int e = 0; e < NW; e++) {
+        *total += sh.red[e];
+        if (t < n) {
+            if (kABOVE) *above += pn[e * LISTED + t];
+            *before += pw[e * LISTED + t];
+        }
+    }
+    __syncthreads();
+}
+
+template <bool kABOVE> DEV void ranks(PickShared& sh, int n, uint64_t* above, uint64_t* before, uint64_t* total) {
+    if (n <= 128) ranks_of<kABOVE, 2>(sh, n, above, before, total);
+    else ranks_of<kABOVE, LISTED / 64>(sh, n, above, before, total);
+}
+
+// The draw from such a list that holds the whole prefix, without selection (50
+// to 100 tokens of one row of 151 936: 7.7 us for the launch, 14 by selection).
+template <typename L>
+DEV void answer_few(const SmArgs& a, PickShared& sh, const Row<L>& row, const SmState& st, int r, int n) {
+    const int t = threadIdx.x;
+    const uint64_t c = t < n ? sh.list[t] : 0, w = t < n ? sh.lw[t] : 0;
+    uint64_t above, before, total;
     if (t == 0) {
         sh.b0 = sh.b1 = 0;
-        sh.red[0] = st.total;
+        sh.red[NW] = st.total;
     }
-    __syncthreads();
-    const uint64_t c = t < n ? sh.list[t] : 0, w = t < n ? sh.lw[t] : 0;
-    uint64_t above = 0, before = 0;
-    if (t < n)
-#pragma unroll
-        for (int e = 0; e < NW; e++) {
-            above += parts[e * LISTED + t];
-            before += parts[(NW + e) * LISTED + t];
-        }
+    ranks<true>(sh, n, &above, &before, &total);
     if (st.by_k && t < n && above == (uint64_t)row.k - 1) {
         sh.b0 = c;
-        sh.red[0] = before + w;
+        sh.red[NW] = before + w;
     }
     __syncthreads();
-    const double goal = row.goal(sh.red[0]);
+    const double goal = row.goal(sh.red[NW]);
     if (st.by_p && t < n && (double)before < goal && (double)(before + w) >= goal) sh.b1 = c;
     __syncthreads();
     const uint64_t cut = sh.b1 > sh.b0 ? sh.b1 : sh.b0;
     const uint64_t left = c >= cut && t < n && (!st.by_m || row.weight_min(logit_of(c))) ? w : 0;
     if (t < n) sh.lw[t] = left;
     __syncthreads();
-    uint64_t total = 0;
-    w0 = w1 = 0;
-#pragma unroll 4
-    for (int j = part; j < n; j += NW) {
-        const uint32_t ij = (uint32_t)sh.list[j];        // larger: a lower index
-        const uint64_t wj = sh.lw[j];
-        total += wj;
-        w0 += ij > (uint32_t)c0 ? wj : 0;
-        w1 += ij > (uint32_t)c1 ? wj : 0;
-    }
-    parts[part * LISTED + lane] = w0;
-    parts[part * LISTED + lane + 64] = w1;
-    if (lane == 0) sh.red[part] = total;
-    __syncthreads();
-    if (t >= n) return;
-    total = before = 0;
-#pragma unroll
-    for (int e = 0; e < NW; e++) {
-        total += sh.red[e];
-        before += parts[e * LISTED + t];
-    }
+    ranks<false>(sh, n, &above, &before, &total);
     const uint64_t aim = aim_of(a.u[r], total);
-    if (before <= aim && aim < before + left) answer(a, row, r, index_of(c), logit_of(c), total);
+    if (t < n && before <= aim && aim < before + left) answer(a, row, r, index_of(c), logit_of(c), total);
+}
+// The border in such a list of top-k's or of top-p's bins alone, the rest of
+// the prefix above them.
+template <typename L> DEV uint64_t cut_few(PickShared& sh, const Row<L>& row, const SmState& st, int n) {
+    const int t = threadIdx.x;
+    const uint64_t c = t < n ? sh.list[t] : 0, w = t < n ? sh.lw[t] : 0;
+    uint64_t above, before, total;
+    if (t == 0) sh.b1 = 0;
+    ranks<true>(sh, n, &above, &before, &total);
+    before += st.wp;
+    const double goal = row.goal(st.total);
+    if (t < n && (st.by_k ? above + 1 == st.rk : (double)before < goal && (double)(before + w) >= goal)) sh.b1 = c;
+    __syncthreads();
+    return sh.b1;
 }
 
 template <typename L> __global__ __launch_bounds__(NT) void k_smp_pick(SmArgs a) {
@@ -1090,12 +1106,14 @@ template <typename L> __global__ __launch_bounds__(NT) void k_smp_pick(SmArgs a)
     auto comp = [&](int i) { return sh.list[i]; };
     auto bin_of = [&](int i) { return row.bin_of(sh.list[i]); };
     uint64_t sum = st.total, cut = 0;      // composites below cut are out
-    if (st.by_k) {
+    const bool few = n <= LISTED && !st.by_m && st.by_k + st.by_p == 1;
+    if (few) cut = cut_few(sh, row, st, n);
+    if (!few && st.by_k) {
         const int at = select(sh, n, Want{BY_COUNT, st.rk, 0.0}, 0, st.wk, comp,
                               [&](int i) { return bin_of(i) == st.bk; }, &sum);
         if (at >= 0) cut = sh.list[at];
     }
-    if (st.by_p) {
+    if (!few && st.by_p) {
         uint64_t s;
         const int at = select(sh, n, Want{BY_GOAL, 0, row.goal(sum)}, 0, st.wp, comp,
                               [&](int i) {

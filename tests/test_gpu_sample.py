@@ -177,3 +177,24 @@ def test_large_vocabulary_and_many_rows(eng, hip):
            top_k=np.array([0, 70000], np.int32), top_p=[0.5, 0.9], u=[0.3, 0.8])
     say("sample: 700 rows")
     sample(eng, hip, logits(rng, 700, 300), R.F16, temp=[0.9] * 700, top_p=[0.9] * 700, u=rng.random(700))
+
+
+@pytest.mark.parametrize("spread", [0.3, 2.5])
+def test_prefixes_around_the_list_lengths(eng, hip, spread):
+    """Top-k around 64, 128 and 256 tokens, alone and with top-p and min-p, and
+    top-p that keeps such numbers: what is ranked as it is, what is selected."""
+    rng = np.random.default_rng(int(10 * spread))
+    ks = [1, 2, 63, 64, 65, 100, 127, 128, 129, 150, 191, 192, 193, 200, 254, 255, 256, 257, 258, 300, 400]
+    V = 20000
+    x = logits(rng, 3 * len(ks), V, spread)
+    top_k = np.array(ks * 3)
+    top_p = np.repeat([1.0, 0.9, 0.97], len(ks))
+    min_p = np.repeat([0.0, 0.0, 0.01], len(ks))
+    u = rng.random(len(x))
+    say(f"list lengths, spread {spread}: top-k")
+    sample(eng, hip, x, R.F32, None, top_k, top_p, min_p, u)
+    # top-p of the weight of the k largest, so that about k stay
+    w = -np.sort(-np.exp((x[:len(ks)] - x[:len(ks)].max(1, keepdims=True)).astype(np.float64)), 1)
+    p = np.array([w[i, :k].sum() / w[i].sum() for i, k in enumerate(ks)]) * (1 - 1e-5)
+    say(f"list lengths, spread {spread}: top-p")
+    sample(eng, hip, x[:len(ks)], R.F32, None, None, p, None, u[:len(ks)])
