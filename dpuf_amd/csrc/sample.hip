@@ -27,10 +27,10 @@
 // Rows whose border bin alone holds more tokens than the list (long runs of
 // equal logits) are left to one workgroup that splits the bin further.
 //
-// 64 rows of 151 936 fp32 logits with settings of every kind: 9.3, 22 and 30 us
+// 64 rows of 151 936 fp32 logits with settings of every kind: 9.1, 21 and 25 us
 // (bytes; 64-bit exponentials and LDS atomics; one more read, then the slowest
 // row's last workgroup, about 15 us of dependent steps); one row with top-k 50
-// and top-p 0.95: 3.3, 9.2 and 11, all latency, most of it loads of what other
+// and top-p 0.95: 3.3, 9 and 7.7, all latency, most of it loads of what other
 // XCDs stored.
 //
 // The last workgroup is found with a counter per row; what it reads from the
