@@ -996,19 +996,36 @@ DEV void answer_few(const SmArgs& a, PickShared& sh, const Row<L>& row, const Sm
     const uint64_t aim = aim_of(a.u[r], total);
     if (t < n && before <= aim && aim < before + left) answer(a, row, r, index_of(c), logit_of(c), total);
 }
-// The border in such a list of top-k's or of top-p's bins alone, the rest of
-// the prefix above them.
+// The borders in such a list of bins: what of it lies above a border's first
+// bin is above all of that bin's tokens.
 template <typename L> DEV uint64_t cut_few(PickShared& sh, const Row<L>& row, const SmState& st, int n) {
     const int t = threadIdx.x;
     const uint64_t c = t < n ? sh.list[t] : 0, w = t < n ? sh.lw[t] : 0;
+    const int b = t < n ? row.bin_of(c) : NB;
     uint64_t above, before, total;
-    if (t == 0) sh.b1 = 0;
-    ranks<true>(sh, n, &above, &before, &total);
-    before += st.wp;
-    const double goal = row.goal(st.total);
-    if (t < n && (st.by_k ? above + 1 == st.rk : (double)before < goal && (double)(before + w) >= goal)) sh.b1 = c;
+    if (t == 0) {
+        sh.b0 = sh.b1 = 0;
+        sh.red[NW] = st.total;
+        sh.count[0] = 0;
+        sh.wsum[0] = sh.wsum[1] = 0;
+    }
     __syncthreads();
-    return sh.b1;
+    if (st.by_k && b < st.bk) {
+        atomicAdd(&sh.count[0], 1u);
+        atomicAdd(&sh.wsum[0], (unsigned long long)w);
+    }
+    if (st.by_p && b < st.pl) atomicAdd(&sh.wsum[1], (unsigned long long)w);
+    ranks<true>(sh, n, &above, &before, &total);
+    if (st.by_k && b == st.bk && above - sh.count[0] + 1 == st.rk) {
+        sh.b0 = c;
+        sh.red[NW] = st.wk + before - sh.wsum[0] + w;
+    }
+    __syncthreads();
+    const double goal = row.goal(sh.red[NW]);
+    before += st.wp - sh.wsum[1];
+    if (st.by_p && b >= st.pl && b <= st.ph && (double)before < goal && (double)(before + w) >= goal) sh.b1 = c;
+    __syncthreads();
+    return sh.b1 > sh.b0 ? sh.b1 : sh.b0;
 }
 
 template <typename L> __global__ __launch_bounds__(NT) void k_smp_pick(SmArgs a) {
@@ -1106,7 +1123,7 @@ template <typename L> __global__ __launch_bounds__(NT) void k_smp_pick(SmArgs a)
     auto comp = [&](int i) { return sh.list[i]; };
     auto bin_of = [&](int i) { return row.bin_of(sh.list[i]); };
     uint64_t sum = st.total, cut = 0;      // composites below cut are out
-    const bool few = n <= LISTED && !st.by_m && st.by_k + st.by_p == 1;
+    const bool few = n <= LISTED;
     if (few) cut = cut_few(sh, row, st, n);
     if (!few && st.by_k) {
         const int at = select(sh, n, Want{BY_COUNT, st.rk, 0.0}, 0, st.wk, comp,
