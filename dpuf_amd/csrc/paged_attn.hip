@@ -138,6 +138,11 @@ template <typename T, int HD> DEV void few_rows(const PaArgs& a, FewLds<HD>& sh,
     const int col = lane & 15, g4 = lane >> 4;
     const int tiles = (a.few + 15) >> 4;
     const int s = y / tiles;
+    const int* table = a.b.page_table + (size_t)s * a.b.table_stride;
+    // the first range's first pages, beside the lengths
+    int early[2];
+#pragma unroll
+    for (int u = 0; u < 2; u++) early[u] = table[min((32 * wave + 16 * u) >> a.shift, a.b.table_stride - 1)];
     const PgSeq sq = pg_seq(a.b, a.shift, s);
     const int rows = sq.n * a.G;
     if (rows > a.few && a.only == PA_BOTH) return;
@@ -168,7 +173,6 @@ template <typename T, int HD> DEV void few_rows(const PaArgs& a, FewLds<HD>& sh,
 
         const uint16_t* kp = (const uint16_t*)a.p.k + (size_t)kvh * a.p.head_stride + 8 * g4;
         const uint16_t* vp = (const uint16_t*)a.p.v + (size_t)kvh * a.p.head_stride + 8 * g4;
-        const int* table = a.b.page_table + (size_t)s * a.b.table_stride;
         const int top = sq.ctx > 0 ? (sq.ctx - 1) >> a.shift : 0;
         uint16_t* lv = sh.v[wave];
 
@@ -202,7 +206,12 @@ template <typename T, int HD> DEV void few_rows(const PaArgs& a, FewLds<HD>& sh,
         uint32_t odd = 0;
         int base = k0 + 32 * wave;
         if (base < kend) {
-            pages(base, pg);
+            if (z == 0) {
+                pg[0] = early[0];
+                pg[1] = base + 16 < sq.ctx ? early[1] : early[0];
+            } else {
+                pages(base, pg);
+            }
             load(base, pg);
             pages(base + 128, pn);
         }
