@@ -522,10 +522,15 @@ template <typename L> DEV void find_borders(const SmArgs& a, HistShared& sh, con
         p1 = by_k ? find_border(a, sh, r, Want{BY_GOAL, 0, row.goal(k.w + k.w_in)}, &loaded) : p0;
     }
     const bool by_p = p0.bin >= 0 && p1.bin >= 0;
-    const int ml = row.by_m ? row.bin(row.edge * (1.0 - 1e-6)) : -1, mh = row.by_m ? row.bin(row.edge * (1.0 + 1e-6)) : -1;
+    const int last = by_k ? k.bin : by_p ? p1.bin : NB - 1;
     const uint64_t upto = by_k ? k.n + k.n_in : by_p ? p1.n + p1.n_in : tn;
+    // min-p's border cuts something only where it lies within top-k's and
+    // top-p's prefix: behind `last` its bins, however many tokens they hold,
+    // are not listed.  So a list has at most in_s tokens, and at most upto
+    const int ml = row.by_m ? row.bin(row.edge * (1.0 - 1e-6)) : NB;
+    const int mh = row.by_m ? min(row.bin(row.edge * (1.0 + 1e-6)), last) : -1;
     uint64_t in_s = (by_k ? k.n_in : 0) + (by_p ? p1.n + p1.n_in - p0.n : 0);
-    if (row.by_m && upto > CAP)
+    if (upto > CAP)
         for (int b = ml; b <= mh; b++) {
             if (loaded != b / GB) load_group(a, sh, r, b / GB);
             loaded = b / GB;
@@ -534,8 +539,8 @@ template <typename L> DEV void find_borders(const SmArgs& a, HistShared& sh, con
     if (t == 0) {
         st->by_k = by_k;
         st->by_p = by_p;
-        st->by_m = row.by_m;
-        st->last = by_k ? k.bin : by_p ? p1.bin : NB - 1;
+        st->by_m = ml <= last;
+        st->last = last;
         st->bk = k.bin;
         st->pl = p0.bin;
         st->ph = p1.bin;
@@ -545,7 +550,7 @@ template <typename L> DEV void find_borders(const SmArgs& a, HistShared& sh, con
         st->wk = k.w;
         st->wp = p0.w;
         st->total = tw;
-        st->mode = upto <= LISTED ? SM_LIST : in_s <= CAP ? SM_BINS : SM_SPLIT;
+        st->mode = upto <= LISTED ? SM_LIST : in_s <= CAP || upto <= CAP ? SM_BINS : SM_SPLIT;
     }
 }
 

@@ -198,3 +198,59 @@ def test_prefixes_around_the_list_lengths(eng, hip, spread):
     p = np.array([w[i, :k].sum() / w[i].sum() for i, k in enumerate(ks)]) * (1 - 1e-5)
     say(f"list lengths, spread {spread}: top-p")
     sample(eng, hip, x[:len(ks)], R.F32, None, None, p, None, u[:len(ks)])
+
+
+def both_calls(eng, hip, x, t, **kw):
+    """The same call twice: the same tokens (each checked against float64)."""
+    a, b = (sample(eng, hip, x, t, **kw) for _ in range(2))
+    assert np.array_equal(a, b)
+
+
+def settled(n, temp, k, p, mp):
+    return dict(temp=[temp] * n, top_k=np.full(n, k, np.int32), top_p=[p] * n, min_p=[mp] * n)
+
+
+@pytest.mark.parametrize("k,about", [(1000, 0), (0, 300), (0, 1000), (0, 2000), (1500, 1000)])
+def test_min_p_border_in_a_crowd_behind_the_prefix(eng, hip, k, about):
+    """One likely token over a narrow bell: min-p's border lies in the bell,
+    among more tokens than a list holds, behind the last token that top-k, or
+    top-p (about so many tokens), leaves."""
+    rng = np.random.default_rng(k + about)
+    n = 6
+    row = (rng.standard_normal(151936) * 0.1).astype(np.float32)
+    row[777] = 8.0
+    w = np.exp(np.sort(row.astype(np.float64))[::-1] - 8.0)
+    p = float(w[:about].sum() / (w[:k].sum() if k else w.sum())) if about else 1.0
+    say(f"crowd behind the prefix: top-k {k}, top-p {p:.4f}")
+    both_calls(eng, hip, np.repeat(row[None], n, 0), R.F32, u=(np.arange(n) + rng.random(n)) / n,
+               **settled(n, 1.0, k, p, np.exp(-8.0)))
+
+
+@pytest.mark.parametrize("t", [R.BF16, R.F16])
+@pytest.mark.parametrize("k", [257, 300, 500, 2000])
+def test_min_p_border_among_coarse_values(eng, hip, k, t):
+    """16-bit logits of such size that thousands of tokens share a value."""
+    rng = np.random.default_rng(k)
+    n = 4
+    row = (rng.standard_normal(151936) * 2.2 + 20).astype(np.float32)
+    say(f"coarse values: top-k {k}, type {t}")
+    both_calls(eng, hip, np.repeat(row[None], n, 0), t, u=(np.arange(n) + rng.random(n)) / n,
+               **settled(n, 1.5, k, 1.0, 0.0015))
+
+
+@pytest.mark.parametrize("side", [-1, 0, 1])
+@pytest.mark.parametrize("V,loose,k,p", [(4000, 700, 300, 1.0), (4000, 700, 0, 0.9), (4000, 700, 650, 0.99),
+                                         (8000, 1000, 500, 1.0), (8000, 1000, 2000, 1.0), (60000, 2100, 2000, 1.0)])
+def test_min_p_border_on_a_run_of_equal_logits(eng, hip, V, loose, k, p, side):
+    """`loose` tokens between 5 and 10, the others all 0, and min-p a little
+    below, about and above e^-10: one chunk and many, the run behind the prefix
+    and (top-k 2 000 of 1 000 loose ones) within it."""
+    rng = np.random.default_rng(V + k)
+    n = 5
+    row = np.zeros(V, np.float32)
+    at = rng.permutation(V)[:loose]
+    row[at] = 5 + 5 * rng.random(loose)
+    row[at[0]] = 10.0
+    say(f"run at min-p's border: V {V}, top-k {k}, top-p {p}, side {side}")
+    both_calls(eng, hip, np.repeat(row[None], n, 0), R.F32, u=(np.arange(n) + rng.random(n)) / n,
+               **settled(n, 1.0, k, p, np.exp(-10.0) * (1 + 1e-3 * side) + (0 if side else 1e-12)))
