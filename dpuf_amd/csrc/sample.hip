@@ -63,7 +63,7 @@ struct Settings {
     float bins;                  // bins per logit
     int inf, k, by_k, by_p, by_m;
     double invT, p_goal;
-    double min_w, edge;          // 2^S min_p (0: off) and -T ln min_p
+    double min_w, edge, blur;    // 2^S min_p (0: off), -T ln min_p, 2^-48 T
 };
 
 struct SmState {
@@ -231,7 +231,8 @@ template <typename L> struct Row : Settings {
         const double min_p = mp > 1.0f ? 1.0 : mp > 0.0f ? (double)mp : 0.0;
         edge = min_p > 0.0 ? -log(min_p) : 0.0;
         by_m = min_p > 0.0 && edge < (S + 1) * 0.69314718055994530942;
-        edge *= (double)T;
+        edge = edge > 0.0 ? edge * (double)T : 0.0;      // (an infinite T among them)
+        blur = 0x1p-48 * (double)T;
         min_w = by_m ? ldexp(min_p, S) : 0.0;
         return true;
     }
@@ -527,8 +528,10 @@ template <typename L> DEV void find_borders(const SmArgs& a, HistShared& sh, con
     // min-p's border cuts something only where it lies within top-k's and
     // top-p's prefix: behind `last` its bins, however many tokens they hold,
     // are not listed.  So a list has at most in_s tokens, and at most upto
-    const int ml = row.by_m ? row.bin(row.edge * (1.0 - 1e-6)) : NB;
-    const int mh = row.by_m ? min(row.bin(row.edge * (1.0 + 1e-6)), last) : -1;
+    // (of the border's distance 1e-6 on either side, and 2^-48 temperatures:
+    // what rounding moves a weight's distance by)
+    const int ml = row.by_m ? row.bin(fmax(row.edge * (1.0 - 1e-6) - row.blur, 0.0)) : NB;
+    const int mh = row.by_m ? min(row.bin(row.edge * (1.0 + 1e-6) + row.blur), last) : -1;
     uint64_t in_s = (by_k ? k.n_in : 0) + (by_p ? p1.n + p1.n_in - p0.n : 0);
     if (upto > CAP)
         for (int b = ml; b <= mh; b++) {

@@ -254,3 +254,15 @@ def test_min_p_border_on_a_run_of_equal_logits(eng, hip, V, loose, k, p, side):
     say(f"run at min-p's border: V {V}, top-k {k}, top-p {p}, side {side}")
     both_calls(eng, hip, np.repeat(row[None], n, 0), R.F32, u=(np.arange(n) + rng.random(n)) / n,
                **settled(n, 1.0, k, p, np.exp(-10.0) * (1 + 1e-3 * side) + (0 if side else 1e-12)))
+
+
+@pytest.mark.parametrize("temp", [1e22, 3e38, np.inf])
+def test_min_p_at_temperatures_that_make_all_weights_equal(eng, hip, temp):
+    """d / temperature below 2^-60: every weight is 1 in 64 bits, and min-p of
+    1 keeps them all, whatever bin they lie in."""
+    rng = np.random.default_rng(3)
+    n = 6
+    x = logits(rng, n, 20000)
+    for k, p, mp in ((1000, 1.0, 1.0), (0, 0.05, 1.0), (3000, 0.9, 0.999), (0, 1.0, 1.0), (100, 1.0, 1.0)):
+        say(f"temperature {temp}: top-k {k}, top-p {p}, min-p {mp}")
+        both_calls(eng, hip, x, R.F32, u=(np.arange(n) + rng.random(n)) / n, **settled(n, temp, k, p, mp))
