@@ -1316,7 +1316,8 @@ static int32_t forward_common(Engine* e, int32_t n_tokens, const int32_t* token_
     int32_t has_early = env_int("DPUF_EARLY_TILES", &early);
     const char* em = getenv("DPUF_EARLY_MARGIN");
     float margin = em ? (float)atof(em) : 1.25f;
-    if (!has_early) early = 0;
+    /* the early exit vouches for the largest logit alone, not for a draw */
+    if (!has_early || smp) early = 0;
     else if (early <= 0) early = 1; /* env set: the zone is at least 256 tiles */
 
     /* the embedding kernel reads ids and pos0 from h_io (no copy) */

@@ -339,8 +339,9 @@ typedef struct {
 
 /* dpuf_amd_engine_forward_argmax with the last row's token drawn by
  * dpuf_amd_sample (one entry of each setting) instead of its largest logit;
- * logprob_out (or NULL) its logarithmic share.  Same return codes, -1 also
- * without sampling->u. */
+ * logprob_out (or NULL) its logarithmic share.  No Zone-A early exit, which
+ * vouches for the largest logit alone.  Same return codes, -1 also without
+ * sampling->u. */
 DPUF_EXPORT int32_t dpuf_amd_engine_forward_sample(void* handle, int32_t n_tokens, const int32_t* token_ids,
                                                    int32_t pos0, const float* embeds_in, int32_t use_graph,
                                                    const DpufAmdSampling* sampling, int32_t* token_out,

@@ -375,3 +375,43 @@ def test_engine_refusals(eng):
     assert eng.dpuf_amd_engine_forward_slots_sample(h, 1, M.ptr(i32(0)), M.ptr(i32(1)), M.ptr(i32(0)), C.byref(some),
                                                     None, None, None) == -1
     eng.dpuf_engine_destroy(h)
+
+
+def test_sampled_steps_do_not_exit_early(eng, monkeypatch):
+    """The LM head's early exit vouches for the largest logit alone: with it on
+    (and firing for the greedy call) a sampled step has the whole vocabulary's
+    logits, and draws from them."""
+    n = 40960
+    shape = dict(hidden_size=256, intermediate_size=512, num_layers=2, num_q_heads=4, num_kv_heads=2, head_dim=64,
+                 vocab_size=n, tie_word_embeddings=1)
+    m = M.Model.build(shape, max_seq_len=32, seed=9)
+    h = eng.dpuf_engine_create(*m.create_args())
+    ids = np.random.default_rng(3).integers(0, n, 6).astype(np.int32)
+    monkeypatch.delenv("DPUF_EARLY_TILES", raising=False)
+    tok, lp, g = np.zeros(1, np.int32), np.zeros(1, np.float32), np.zeros(1, np.int32)
+    full, lg, zone = np.zeros(n, np.float32), np.zeros(n, np.float32), np.zeros(n, np.float32)
+    col = lambda v, t: np.array([v], t)
+    beyond = 0
+    for count, pos in ((6, 0), (1, 6), (1, 7)):
+        monkeypatch.delenv("DPUF_EARLY_TILES", raising=False)
+        assert eng.dpuf_amd_engine_forward_argmax(h, count, M.ptr(ids), pos, None, 1, M.ptr(g), M.ptr(full)) == 0
+        monkeypatch.setenv("DPUF_EARLY_TILES", "300")
+        monkeypatch.setenv("DPUF_EARLY_MARGIN", "1e-7")
+        assert eng.dpuf_amd_engine_forward_argmax(h, count, M.ptr(ids), pos, None, 1, M.ptr(g), M.ptr(zone)) == 0
+        assert np.all(zone[300 * 16:] == -1e9)
+        exits = eng.dpuf_amd_engine_early_exit_count(h)
+        for graph in (0, 1, 1):
+            for u, t in ((0.1, 1.0), (0.6, 0.7), (0.95, 1.5), (0.5, 0.0)):
+                a = dict(temperature=col(t, np.float32), top_k=col(0, np.int32), top_p=col(1.0, np.float32),
+                         min_p=col(0.0, np.float32), u=col(u, np.float32))
+                s = abi.DpufAmdSampling(**{k: v.ctypes.data for k, v in a.items()})
+                lg[:] = 0
+                assert eng.dpuf_amd_engine_forward_sample(h, count, M.ptr(ids), pos, None, graph, C.byref(s),
+                                                          M.ptr(tok), M.ptr(lp), M.ptr(lg)) == 0
+                assert np.array_equal(lg.view(np.uint32), full.view(np.uint32))
+                want, wl = drawn(a, 0, full)
+                assert tok[0] == want and abs(lp[0] - wl) <= abs(wl) * 2.0 ** -23 + n * 2.0 ** -38 + 2.0 ** -30
+                beyond += int(tok[0]) >= 300 * 16
+        assert eng.dpuf_amd_engine_early_exit_count(h) == exits
+    assert beyond > 0
+    eng.dpuf_engine_destroy(h)
