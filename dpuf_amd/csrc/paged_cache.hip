@@ -296,18 +296,24 @@ __global__ __launch_bounds__(64 * KG * RG) void k_pa_weights(PwArgs a) {
                 __syncthreads();
                 take(buf ^ 1);
             }
-            // keys that the step's first row does not see: row by row
-            if (base + 32 * KB - 1 > sq.ctx - sq.n + by_g(r0)) {
+            // keys that the step's first row does not see, and lanes without a
+            // row, key by key: whatever an infinity or NaN in K, or a row's
+            // lse of NaN, makes of the others' exponentials, they give nothing
+            if (base + 32 * KB - 1 > sq.ctx - sq.n + by_g(r0) || r0 + 32 > rows) {
+#pragma unroll
+                for (int b = 0; b < KB; b++)
+#pragma unroll
+                    for (int i = 0; i < 16; i++) {
+                        const float e = __builtin_amdgcn_exp2f(fmaf(sc[b][i], a.c2, -l2));
+                        acc[b][i] += base + 32 * b + 8 * (i >> 2) + 4 * h + (i & 3) <= limit ? e : 0.0f;
+                    }
+            } else {
 #pragma unroll
                 for (int b = 0; b < KB; b++)
 #pragma unroll
                     for (int i = 0; i < 16; i++)
-                        if (base + 32 * b + 8 * (i >> 2) + 4 * h + (i & 3) > limit) sc[b][i] = NEG_INF;
+                        acc[b][i] += __builtin_amdgcn_exp2f(fmaf(sc[b][i], a.c2, -l2));
             }
-#pragma unroll
-            for (int b = 0; b < KB; b++)
-#pragma unroll
-                for (int i = 0; i < 16; i++) acc[b][i] += __builtin_amdgcn_exp2f(fmaf(sc[b][i], a.c2, -l2));
         }
         // over the 32 lanes of each half: entries i and i + 8 of the lower and
         // the upper 16 lanes are exchanged, so each 16 add up 8 entries of all

@@ -336,3 +336,64 @@ def test_host_memory_is_refused(eng, hip):
     p.k = host.ctypes.data & ~15
     assert ok() == -1
     hip.sync()
+
+
+def weights_of(eng, hip, cache, nq, q, scale, max_ctx=None):
+    """pages->w of one call from nothing, [page][kv head][row]."""
+    _, lse, dq, dl, _ = call(eng, hip, cache, nq, q, scale)
+    dst = hip.put(np.full_like(cache.w, -3.0))
+    b, p = cache.batch(max_ctx=max_ctx), cache.pages(dw=dst)
+    assert eng.dpuf_amd_paged_attn_weights(C.byref(b), C.byref(p), nq, dq.p, scale, dl.p, 1.0, None, None) == 0
+    return dst.get()
+
+
+# batches for the few-row kernel, the other, and both, and max_ctx for its tiles of 128, 64 and 32 keys
+ODD = [([1, 3, 1], [200, 90, 40], None), ([70], [300], 30000), ([70], [300], 6000), ([70], [300], 300),
+       ([90, 1, 1, 1], [333, 250, 40, 33], 100000)]
+
+
+@pytest.mark.parametrize("hd", [64, 128, 256])
+@pytest.mark.parametrize("rows,ctx,max_ctx", ODD)
+def test_weights_of_keys_that_score_minus_infinity(eng, hip, rows, ctx, max_ctx, hd):
+    """An infinite element of a key that every query has with the other sign:
+    each row gives that key nothing, and the others what they get without it."""
+    rng = np.random.default_rng(hd + len(rows))
+    nq = 10
+    cache = R.Cache(hip, rng, R.BF16, rows, ctx, 2, hd, 16, table_extra=6300)
+    q = R.to_type(rng.standard_normal((cache.n_rows, nq, hd)), R.BF16)
+    q[..., 5] = R.to_type(-0.5, R.BF16)
+    for s, i in ((0, 0), (0, 17), (0, ctx[0] - rows[0] - 1)):
+        cache.k[cache.table[s, i // 16], :, i % 16, 5] = R.to_type([np.inf], R.BF16)[0]
+    cache.dk.set(cache.k)
+    say(f"scores of -infinity: rows {rows}, contexts {ctx}, max_ctx {max_ctx}, hd {hd}")
+    got = weights_of(eng, hip, cache, nq, q, 0.1, max_ctx)
+    with np.errstate(all="ignore"):
+        _, rl, _, _, _, fresh = R.attention(cache, R.from_type(q, R.BF16), float(np.float32(0.1)), nq)
+    # |q| and |k| below 6 (standard normal): as the weights' own tests
+    rel = 2 * R.score_error(36.0 * hd * 0.1, hd) + np.abs(rl[np.isfinite(rl)]).max() * 2.0 ** -22 + 2.0 ** -20
+    rel += (max(rows) * nq // 2 + 40) * 2.0 ** -24
+    for s, c in enumerate(ctx):
+        for i in range(c):
+            w = got[cache.table[s, i // 16], :, i % 16]
+            assert np.all(np.abs(w - fresh[s][:, i]) <= rel * fresh[s][:, i] + 1e-30), (s, i, w, fresh[s][:, i])
+
+
+@pytest.mark.parametrize("hd", [64, 128, 256])
+@pytest.mark.parametrize("rows,ctx,max_ctx", ODD)
+def test_weights_of_keys_behind_a_row_without_a_number(eng, hip, rows, ctx, max_ctx, hd):
+    """A query with NaN gives NaN to the keys that its row sees, and to no
+    others: those keep the bits that they have with another query there."""
+    rng = np.random.default_rng(2 * hd + len(rows))
+    nq, row, head = 10, max(rows) // 2, 7
+    s = int(np.argmax(rows))
+    cache = R.Cache(hip, rng, R.F16, rows, ctx, 2, hd, 16, table_extra=6300)
+    q = R.to_type(rng.standard_normal((cache.n_rows, nq, hd)), R.F16)
+    want = weights_of(eng, hip, cache, nq, q, 0.1, max_ctx)
+    q[cache.starts[s] + row, head, 3] = R.to_type([np.nan], R.F16)[0]
+    say(f"a row of NaN: rows {rows}, contexts {ctx}, max_ctx {max_ctx}, hd {hd}")
+    got = weights_of(eng, hip, cache, nq, q, 0.1, max_ctx)
+    for i in range(ctx[s] - rows[s] + row + 1):
+        at = cache.table[s, i // 16], head // (nq // 2), i % 16
+        assert np.isnan(got[at]), i
+        got[at] = want[at]
+    assert np.array_equal(got.view(np.uint32), want.view(np.uint32))
