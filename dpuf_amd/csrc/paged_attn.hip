@@ -20,11 +20,16 @@
 // The running maximum need not be the largest score so far, only near it: m is
 // moved (and l and o multiplied, a product per sum) when a score passes it by
 // more than 2^SLACK, so that most tiles move nothing; p is at most 2^SLACK
-// then, far inside fp16's range.
+// then.
 //
 // Exponentials are of base 2 with the scale folded in (one fma each); p is
 // rounded to the pages' type for the product with V (a relative half step,
-// 2^-8 in bf16 and 2^-11 in fp16, of each term), every sum is fp32.
+// 2^-8 in bf16 and 2^-11 in fp16, of each term), every sum is fp32.  fp16 has
+// few exponents: below 2^-14 of the largest, terms would lose their bits, and
+// below 2^-25 vanish, however many there are.  So there m is LIFT = 9 below the
+// maximum: p is at most 2^(9 + SLACK) = 2^15, and whole down to 2^-23 of the
+// largest.  The maximum is then rounded up to an integer, which keeps m + LIFT
+// and the factors that l and o are moved by exact.
 #include <hip/hip_runtime.h>
 #include <math.h>
 #include <stdint.h>
@@ -86,7 +91,13 @@ DEV void put4(const PaArgs& a, size_t at, const float* o, float inv) {
     }
 }
 
-DEV float lse_of(float m2, float l) { return l == 0.0f ? NEG_INF : (m2 + __log2f(l)) * 0.69314718055994531f; }
+// What m is set to for a maximum, and the log sum of (m, l).
+template <typename T> DEV float lowered(float top) { return T::LIFT == 0.0f ? top : ceilf(top) - T::LIFT; }
+template <typename T> DEV float lse_of(float m2, float l) {
+    constexpr float DOWN = T::LIFT == 0.0f ? 1.0f : 0x1p-9f;
+    static_assert(T::LIFT == 0.0f || T::LIFT == 9.0f, "2^-LIFT");
+    return l == 0.0f ? NEG_INF : (m2 + T::LIFT + __log2f(l * DOWN)) * 0.69314718055994531f;
+}
 
 // Infinities and NaN in V.  A row that does not see a key has p = 0 there, and
 // 0 * inf would reach its sums all the same.  So in a tile that some row does
@@ -257,8 +268,8 @@ template <typename T, int HD> DEV void few_rows(const PaArgs& a, FewLds<HD>& sh,
                              fmaxf(fmaxf(sc[1][0], sc[1][1]), fmaxf(sc[1][2], sc[1][3])));
             mt = max_xor32(max_xor16(mt)) * a.c2;
             // m follows the maximum only when it is behind by more than 2^SLACK
-            if (__any(mt > m + SLACK)) {
-                const float mn = fmaxf(m, mt), f = __builtin_amdgcn_exp2f(m - (mn == NEG_INF ? 0.0f : mn));
+            if (__any(mt > m + (T::LIFT + SLACK))) {
+                const float mn = fmaxf(m, lowered<T>(mt)), f = __builtin_amdgcn_exp2f(m - (mn == NEG_INF ? 0.0f : mn));
                 l *= f;
 #pragma unroll
                 for (int d = 0; d < ND; d++) o[d] *= f;
@@ -355,7 +366,7 @@ template <typename T, int HD> DEV void few_rows(const PaArgs& a, FewLds<HD>& sh,
         }
         if (threadIdx.x < 16 && live) {
             if (ranges > 1) a.few_ml[few_at(a, z, s, kvh, r, row)] = make_float2(M, L);
-            else if (a.lse) a.lse[row] = lse_of(M, L);
+            else if (a.lse) a.lse[row] = lse_of<T>(M, L);
         }
     }
 }
@@ -551,8 +562,8 @@ DEV void many_rows(const PaArgs& a, ManyLds<HD>& sh, int kvh, int tile, int z) {
             for (int i = 0; i < 16; i++) mt = fmaxf(mt, sc[b][i]);
         mt = max_xor32(mt) * a.c2;
         // m follows the maximum only when it is behind by more than 2^SLACK
-        if (__any(mt > m + SLACK)) {
-            const float mn = fmaxf(m, mt), f = __builtin_amdgcn_exp2f(m - (mn == NEG_INF ? 0.0f : mn));
+        if (__any(mt > m + (T::LIFT + SLACK))) {
+            const float mn = fmaxf(m, lowered<T>(mt)), f = __builtin_amdgcn_exp2f(m - (mn == NEG_INF ? 0.0f : mn));
             l *= f;
 #pragma unroll
             for (int d = 0; d < ND; d++) o[d] *= f;
@@ -628,7 +639,7 @@ DEV void many_rows(const PaArgs& a, ManyLds<HD>& sh, int kvh, int tile, int z) {
                 const float ov[4] = {o[d][i], o[d][i + 1], o[d][i + 2], o[d][i + 3]};
                 put4<T>(a, row * HD + 32 * d + 2 * i + 4 * h, ov, inv);
             }
-        if (h == 0 && a.lse) a.lse[row] = lse_of(m, l);
+        if (h == 0 && a.lse) a.lse[row] = lse_of<T>(m, l);
     }
 }
 
@@ -726,7 +737,7 @@ __global__ __launch_bounds__(256) void k_pa_join(PaArgs a) {
     const float inv = L > 0.0f ? 1.0f / L : L == 0.0f ? 0.0f : L;
     const float ov[4] = {o[0], o[1], o[2], o[3]};
     put4<T>(a, at * HD + d, ov, inv);
-    if (d == 0 && a.lse) a.lse[at] = lse_of(M, L);
+    if (d == 0 && a.lse) a.lse[at] = lse_of<T>(M, L);
 }
 
 struct PaPlan {

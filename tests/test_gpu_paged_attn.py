@@ -397,3 +397,44 @@ def test_weights_of_keys_behind_a_row_without_a_number(eng, hip, rows, ctx, max_
         assert np.isnan(got[at]), i
         got[at] = want[at]
     assert np.array_equal(got.view(np.uint32), want.view(np.uint32))
+
+
+@pytest.mark.parametrize("hd", [64, 128, 256])
+@pytest.mark.parametrize("rows,ctx,max_ctx", [([1, 1], [400, 3], None), ([1], [2000], None), ([40], [700], 300),
+                                              ([97], [2300], None), ([1, 70], [400, 500], 500)])
+def test_fp16_probabilities_far_below_the_largest(eng, hip, rows, ctx, max_ctx, hd):
+    """One key 2^20 times as likely as the others, with nothing in its value:
+    the others' probabilities, all below fp16's normal numbers, are what there
+    is, and keep a relative half step each."""
+    rng = np.random.default_rng(hd)
+    nq, scale = 4, 0.125
+    cache = R.Cache(hip, rng, R.F16, rows, ctx, 1, hd, 16, table_extra=150)
+    n = cache.n_rows
+    # score of key 0: scale * 8 * x, of the others 0; x so that exp(score) is
+    # 2^24 / 16.5: halfway between two of fp16's subnormal numbers
+    q = np.zeros((n, nq, hd))
+    q[..., 0], q[..., 1] = 8.0, 2.0 ** -10
+    score = np.log(2.0 ** 24 / 16.5)
+    hi = float(np.float16(score))
+    lo = float(np.float16((score - hi) * 2.0 ** 13))
+    for s, c in enumerate(ctx):
+        for i in range(c):
+            pg, r = cache.table[s, i // 16], i % 16
+            cache.k[pg, :, r] = 0
+            cache.v[pg, :, r] = R.to_type(1 + 0.1 * rng.standard_normal(hd), R.F16)
+            if i == 0:
+                cache.k[pg, 0, r, :2] = R.to_type([hi, lo], R.F16)
+                cache.v[pg, :, r] = 0
+    cache.dk.set(cache.k)
+    cache.dv.set(cache.v)
+    q = R.to_type(q, R.F16)
+    say(f"far below the largest: rows {rows}, contexts {ctx}, max_ctx {max_ctx}, hd {hd}")
+    out, lse, *_ = call(eng, hip, cache, nq, q, scale, out_t=R.F32, max_ctx=max_ctx)
+    ref, rl, A, S, _, _ = R.attention(cache, R.from_type(q, R.F16), scale, nq)
+    # attention_bound without the share of rounded-off terms: 2^-20 of the largest times 2^9 is a normal number
+    d = R.score_error(S, hd)[..., None]
+    bound = A * (R.HALF_STEP[R.F16] + 2 * d + (max(ctx) + 64) * 2.0 ** -24) * 1.01 + 1e-30
+    err = np.abs(out - ref)
+    say(f"  worst error {float((err / bound).max()):.3f} of the bound")
+    assert np.all(err <= bound)
+    assert np.all(np.abs(lse - rl) <= R.score_error(S, hd) + np.abs(rl) * 2.0 ** -22 + 2.0 ** -20)
