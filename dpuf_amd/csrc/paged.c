@@ -29,10 +29,31 @@ static int32_t device_of(const void* const* p, int n) {
     return dev;
 }
 
-static int overlap(const void* a, uint64_t an, const void* b, uint64_t bn) {
-    const uintptr_t x = (uintptr_t)a, y = (uintptr_t)b;
-    return a && b && an && bn && x < y + bn && y < x + an;
+/* Memory that a call reads or writes. */
+typedef struct {
+    const void* p;
+    uint64_t n;
+} Span;
+
+static int overlap(Span a, Span b) {
+    const uintptr_t x = (uintptr_t)a.p, y = (uintptr_t)b.p;
+    return a.p && b.p && a.n && b.n && x < y + b.n && y < x + a.n;
 }
+
+/* Whether any of the n spans at a shares memory with any of the m at b. */
+static int any_overlap(const Span* a, int n, const Span* b, int m) {
+    for (int i = 0; i < n; i++)
+        for (int j = 0; j < m; j++)
+            if (overlap(a[i], b[j])) return 1;
+    return 0;
+}
+/* Whether any two of the n spans do. */
+static int overlap_within(const Span* a, int n) {
+    for (int i = 1; i < n; i++)
+        if (any_overlap(a + i, 1, a, i)) return 1;
+    return 0;
+}
+#define COUNT(a) ((int)(sizeof(a) / sizeof((a)[0])))
 
 static int32_t check_pages(const DpufAmdPages* p) {
     if (!p) return -1;
@@ -60,12 +81,38 @@ static int32_t check_heads(const DpufAmdPages* p, int32_t nq) {
     return nq < 1 || nq % p->n_kv_heads != 0 || nq / p->n_kv_heads > 32 ? -2 : 0;
 }
 
-/* Bytes that the rows of an n-row operand of `cols` columns span. */
-static uint64_t span(int64_t n, int64_t stride, int64_t cols, int64_t size) {
-    return n > 0 ? (uint64_t)((n - 1) * stride + cols) * (uint64_t)size : 0;
-}
-
 static int64_t type_size(int32_t t) { return t == DPUF_AMD_F32 ? 4 : 2; }
+
+/* n elements of `size` bytes, n rows of `cols` of them, and what strides of any
+ * size span: more than an address space holds counts as all of it. */
+static Span run(const void* p, int64_t n, int64_t size) {
+    const Span s = {p, (uint64_t)(n * size)};
+    return s;
+}
+static Span bounded(const void* p, unsigned __int128 n, int64_t size) {
+    const uint64_t most = UINT64_MAX / 2 - (uintptr_t)p / 2;
+    const Span s = {p, n > most / (uint64_t)size ? most : (uint64_t)n * (uint64_t)size};
+    return s;
+}
+static Span rows_of(const void* p, int64_t n, int64_t stride, int64_t cols, int64_t size) {
+    return bounded(p, n > 0 ? (unsigned __int128)(n - 1) * (uint64_t)stride + (uint64_t)cols : 0, size);
+}
+/* The batch's three arrays. */
+static void batch_spans(const DpufAmdBatch* b, Span* s) {
+    s[0] = run(b->row_start, b->n_seqs + 1, 4);
+    s[1] = run(b->ctx_len, b->n_seqs, 4);
+    s[2] = run(b->page_table, (int64_t)b->n_seqs * b->table_stride, 4);
+}
+/* The pages' k or v from its first row to its last, and w. */
+static Span pool_span(const DpufAmdPages* p, const void* at) {
+    const unsigned __int128 n = (unsigned __int128)(p->n_pages - 1) * (uint64_t)p->page_stride +
+                                (unsigned __int128)(p->n_kv_heads - 1) * (uint64_t)p->head_stride +
+                                (unsigned __int128)(p->page_size - 1) * (uint64_t)p->row_stride + (uint64_t)p->head_dim;
+    return bounded(at, n, 2);
+}
+static Span weight_span(const DpufAmdPages* p, const void* at) {
+    return run(at, (int64_t)p->n_pages * p->n_kv_heads * p->page_size, 4);
+}
 
 /* Runs `call` with the pointers' device current. */
 #define ON_DEVICE(dev, call)                               \
@@ -138,11 +185,17 @@ DPUF_EXPORT int32_t dpuf_amd_rope_append(const DpufAmdBatch* batch, const DpufAm
     const int64_t st[3] = {q_stride, k_stride, v_stride}, need[3] = {n_q_heads * hd, nkv * hd, nkv * hd};
     for (int i = n_q_heads ? 0 : 1; i < 3; i++)
         if (st[i] < need[i] || st[i] % 8 != 0) return -4;
-    const uint64_t out_n = (uint64_t)batch->n_rows * (uint64_t)need[0] * 2u;
     const int in_place = d_q && d_q_out == d_q && in_type == pages->type && q_stride == need[0];
-    if ((!in_place && overlap(d_q_out, out_n, d_q, span(batch->n_rows, q_stride, need[0], es))) ||
-        overlap(d_q_out, out_n, d_k, span(batch->n_rows, k_stride, need[1], es)) ||
-        overlap(d_q_out, out_n, d_v, span(batch->n_rows, v_stride, need[2], es)))
+    Span in[9] = {rows_of(d_k, batch->n_rows, k_stride, need[1], es), rows_of(d_v, batch->n_rows, v_stride, need[2], es),
+                  run(d_positions, batch->n_rows, 4), run(rope->turns, rope->rot_dim / 2, 8), run(d_q_norm, hd, 4),
+                  run(d_k_norm, hd, 4)};
+    batch_spans(batch, in + 6);
+    const Span q = rows_of(d_q, batch->n_rows, q_stride, need[0], es);
+    /* k and v may lie interleaved in one allocation */
+    const Span out[] = {run(d_q_out, batch->n_rows * need[0], 2), pool_span(pages, pages->k), pool_span(pages, pages->v),
+                        weight_span(pages, pages->w)};
+    if (any_overlap(out, 4, in, COUNT(in)) || any_overlap(out + 1, 3, &q, 1) || (!in_place && overlap(out[0], q)) ||
+        any_overlap(out, 1, out + 1, 3) || any_overlap(out + 1, 2, out + 3, 1))
         return -1;
     const void* ps[] = {pages->k, pages->v, pages->w, batch->row_start, batch->ctx_len, batch->page_table, rope->turns,
                         d_positions, d_q, d_k, d_v, d_q_norm, d_k_norm, d_q_out};
@@ -170,15 +223,14 @@ DPUF_EXPORT int32_t dpuf_amd_paged_attn(const DpufAmdBatch* batch, const DpufAmd
     if (!(scale > 0.0f) || !isfinite(scale)) return -2;
     if (batch->n_rows == 0) return 0;
     if (!aligned(d_q, 16) || !aligned(d_out, 16) || (d_lse && !aligned(d_lse, 4))) return -1;
-    const uint64_t n = (uint64_t)batch->n_rows * (uint64_t)n_q_heads * (uint64_t)pages->head_dim;
-    if (overlap(d_q, n * 2u, d_out, n * (uint64_t)type_size(out_type))) return -1;
     const size_t ws = dpuf_hip_paged_attn_workspace(batch, pages, n_q_heads);
     if (ws > 0 && !aligned(d_workspace, 16)) return -1;
     if (workspace_bytes < ws) return -7;
-    const uint64_t nl = (uint64_t)batch->n_rows * (uint64_t)n_q_heads * 4u, no = n * (uint64_t)type_size(out_type);
-    if (overlap(d_lse, nl, d_q, n * 2u) || overlap(d_lse, nl, d_out, no) || overlap(d_workspace, ws, d_q, n * 2u) ||
-        overlap(d_workspace, ws, d_out, no) || overlap(d_workspace, ws, d_lse, nl))
-        return -1;
+    const int64_t nr = (int64_t)batch->n_rows * n_q_heads, n = nr * pages->head_dim;
+    Span in[6] = {run(d_q, n, 2), pool_span(pages, pages->k), pool_span(pages, pages->v)};
+    batch_spans(batch, in + 3);
+    const Span out[] = {run(d_out, n, type_size(out_type)), run(d_lse, nr, 4), run(d_workspace, (int64_t)ws, 1)};
+    if (any_overlap(out, 3, in, COUNT(in)) || overlap_within(out, 3)) return -1;
     const void* ps[] = {pages->k, pages->v, batch->row_start, batch->ctx_len, batch->page_table, d_q, d_out, d_lse,
                         ws > 0 ? d_workspace : NULL};
     const int32_t dev = device_of(ps, (int)(sizeof ps / sizeof ps[0]));
@@ -198,10 +250,11 @@ DPUF_EXPORT int32_t dpuf_amd_paged_attn_weights(const DpufAmdBatch* batch, const
     if (!(scale > 0.0f) || !isfinite(scale) || !isfinite(decay)) return -2;
     if (!aligned(pages->w, 4) || (d_w_in && !aligned(d_w_in, 4))) return -1;
     if (batch->n_rows > 0 && (!aligned(d_q, 16) || !aligned(d_lse, 4))) return -1;
-    const uint64_t n = (uint64_t)pages->n_pages * (uint64_t)pages->n_kv_heads * (uint64_t)pages->page_size * 4u;
-    if (d_w_in != pages->w && overlap(d_w_in, n, pages->w, n)) return -1;
-    const uint64_t nl = (uint64_t)batch->n_rows * (uint64_t)n_q_heads * 4u;
-    if (overlap(d_lse, nl, pages->w, n)) return -1;
+    const int64_t nr = (int64_t)batch->n_rows * n_q_heads;
+    Span in[6] = {run(d_q, nr * pages->head_dim, 2), run(d_lse, nr, 4), pool_span(pages, pages->k)};
+    batch_spans(batch, in + 3);
+    const Span w = weight_span(pages, pages->w), w_in = weight_span(pages, d_w_in);
+    if (any_overlap(&w, 1, in, COUNT(in)) || (d_w_in != pages->w && overlap(w, w_in))) return -1;
     const void* ps[] = {pages->k, pages->w, batch->row_start, batch->ctx_len, batch->page_table, d_w_in,
                         batch->n_rows > 0 ? d_q : NULL, batch->n_rows > 0 ? (const void*)d_lse : NULL};
     const int32_t dev = device_of(ps, (int)(sizeof ps / sizeof ps[0]));
@@ -232,12 +285,16 @@ DPUF_EXPORT int32_t dpuf_amd_paged_evict(const DpufAmdBatch* batch, const DpufAm
     if (!aligned(pages->w, 4) || !aligned(dst->w, 4) || !aligned(d_dst_table, 4) || !aligned(d_kept, 4) ||
         !aligned(d_new_len, 4))
         return -1;
-    const uint64_t ns = (uint64_t)batch->n_seqs * 4u, nk = ns * (uint64_t)pages->n_kv_heads * (uint64_t)keep;
-    const uint64_t nt = ns * (uint64_t)batch->table_stride, nd = ns * (uint64_t)dst_table_stride;
-    if (overlap(d_new_len, ns, batch->ctx_len, ns) || overlap(d_new_len, ns, batch->page_table, nt) ||
-        overlap(d_kept, nk, batch->ctx_len, ns) || overlap(d_kept, nk, batch->page_table, nt) ||
-        overlap(d_new_len, ns, d_dst_table, nd) || overlap(d_kept, nk, d_dst_table, nd) ||
-        overlap(d_new_len, ns, d_kept, nk))
+    const int64_t ns = batch->n_seqs;
+    const Span in[] = {run(batch->ctx_len, ns, 4), run(batch->page_table, ns * batch->table_stride, 4),
+                       run(d_dst_table, ns * dst_table_stride, 4)};
+    const Span lists[] = {run(d_kept, ns * pages->n_kv_heads * keep, 4), run(d_new_len, ns, 4)};
+    /* dst may be other pages of the same pool */
+    const Span from[] = {pool_span(pages, pages->k), pool_span(pages, pages->v), weight_span(pages, pages->w)};
+    const Span to[] = {pool_span(dst, dst->k), pool_span(dst, dst->v), weight_span(dst, dst->w)};
+    if (any_overlap(lists, 2, in, 3) || overlap(lists[0], lists[1]) || any_overlap(lists, 2, from, 3) ||
+        any_overlap(lists, 2, to, 3) || any_overlap(to, 3, in, 3) || any_overlap(to, 2, from + 2, 1) ||
+        any_overlap(to + 2, 1, from, 2) || any_overlap(to, 2, to + 2, 1))
         return -1;
     const void* ps[] = {pages->k, pages->v, pages->w, dst->k, dst->v, dst->w, batch->ctx_len, batch->page_table,
                         d_dst_table, d_kept, d_new_len};
@@ -264,21 +321,13 @@ DPUF_EXPORT int32_t dpuf_amd_sample(int32_t type, int32_t n, int32_t V, int64_t 
     const void* opt[] = {d_temperature, d_top_k, d_top_p, d_min_p, d_logprobs};
     for (int i = 0; i < 5; i++)
         if (opt[i] && !aligned(opt[i], 4)) return -1;
-    const uint64_t nb = (uint64_t)n * 4u, nx = span(n, row_stride, V, type_size(type));
-    if (overlap(d_tokens, nb, d_logprobs, nb) || overlap(d_tokens, nb, d_logits, nx) ||
-        overlap(d_logprobs, nb, d_logits, nx))
-        return -1;
-    const void* in[] = {d_temperature, d_top_k, d_top_p, d_min_p, d_u};
-    for (int i = 0; i < 5; i++)
-        if (overlap(d_tokens, nb, in[i], nb) || overlap(d_logprobs, nb, in[i], nb)) return -1;
     const size_t ws = dpuf_hip_sample_workspace(n, V);
     if (ws > 0 && !aligned(d_workspace, 16)) return -1;
     if (workspace_bytes < ws) return -7;
-    if (overlap(d_workspace, ws, d_logits, nx) || overlap(d_workspace, ws, d_tokens, nb) ||
-        overlap(d_workspace, ws, d_logprobs, nb))
-        return -1;
-    for (int i = 0; i < 5; i++)
-        if (overlap(d_workspace, ws, in[i], nb)) return -1;
+    const Span in[] = {rows_of(d_logits, n, row_stride, V, type_size(type)), run(d_temperature, n, 4), run(d_top_k, n, 4),
+                       run(d_top_p, n, 4), run(d_min_p, n, 4), run(d_u, n, 4)};
+    const Span out[] = {run(d_tokens, n, 4), run(d_logprobs, n, 4), run(d_workspace, (int64_t)ws, 1)};
+    if (any_overlap(out, 3, in, COUNT(in)) || overlap_within(out, 3)) return -1;
     const void* ps[] = {d_logits, d_temperature, d_top_k, d_top_p, d_min_p, d_u, d_tokens, d_logprobs,
                         ws > 0 ? d_workspace : NULL};
     const int32_t dev = device_of(ps, (int)(sizeof ps / sizeof ps[0]));

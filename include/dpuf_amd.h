@@ -164,8 +164,11 @@ DPUF_EXPORT int32_t dpuf_amd_verify_tiles_device(int32_t mode, int32_t n_tiles, 
  * not overlap.  No counterparts in the reference.
  *
  * Return codes: 0 enqueued; -1 NULL or misaligned pointer, host memory where
- * device memory is needed, pointers of different devices, or overlapping
- * arguments; -2 a size or setting out of range; -4 a stride that is not a
+ * device memory is needed, pointers of different devices, or an output or
+ * workspace that shares memory with anything else that the call reads or
+ * writes (pools count from their first row to their last; k and v of one
+ * allocation may interleave, and an operator says where it works in place);
+ * -2 a size or setting out of range; -4 a stride that is not a
  * multiple of 8 elements or too small; -5 a type or head dim that is not
  * built; -6 device error (dpuf_amd_last_error); -7 workspace too small. */
 

@@ -283,3 +283,138 @@ def test_many_sequences(eng, hip):
             for i in range(ctx[s]):
                 x = w[c.table[s, i // 16], 0, i % 16]
                 assert abs(x - fresh[s][0, i]) <= rel * fresh[s][0, i] + 1e-30, (s, i)
+
+
+def test_outputs_in_memory_that_a_call_reads_are_refused(eng, hip):
+    """Every output and workspace of every operator, laid into each of the
+    inputs, tables and pools that the call reads or also writes: refused, and
+    nothing of the call is done."""
+    st = Step(eng, hip, 5, [1, 1, 2], [900, 1500, 40])
+    st.enter(0)
+    e, r, c = eng, C.byref, st.cache
+    assert st.ws_n > 0
+    width = (NQ + 2 * NKV) * HD
+    scratch = hip.put(np.zeros(1 << 20, np.uint8))
+    tables = dict(starts=c.d_starts.p, ctx=c.d_ctx.p, table=c.d_table.p)
+    pools = dict(k=c.dk.p + 4096, v=c.dv.p + 4096, w=c.dw.p + 64)
+
+    def pages(w=None, k=None, v=None):
+        p = c.pages()
+        p.w, p.k, p.v = w or p.w, k or p.k, v or p.v
+        return p
+
+    at = st.qkv.p
+    ok_rope = dict(q=at, k=at + NQ * HD * 4, v=at + (NQ + NKV) * HD * 4, pos=st.pos.p, out=st.q.p, turns=st.rope.turns,
+                   norm=scratch.p, p=pages())
+
+    def rope(**kw):
+        a = dict(ok_rope, **kw)
+        s = abi.DpufAmdRope(turns=a["turns"], rot_dim=HD, interleaved=0, scale=1.0)
+        return e.dpuf_amd_rope_append(r(st.b), r(a["p"]), r(s), a["pos"], R.F32, NQ, a["q"], a["k"], a["v"], width,
+                                      width, width, a["norm"], None, 1e-6, a["out"], st.stream)
+
+    def attn(**kw):
+        a = dict(dict(q=st.q.p, out=st.out.p, lse=st.lse.p, ws=st.ws.p), **kw)
+        return e.dpuf_amd_paged_attn(r(st.b), r(st.p), NQ, a["q"], 0.09, R.F32, a["out"], a["lse"], a["ws"], st.ws_n,
+                                     st.stream)
+
+    def weights(**kw):
+        a = dict(dict(p=pages(), q=st.q.p, lse=st.lse.p, w_in=None), **kw)
+        return e.dpuf_amd_paged_attn_weights(r(st.b), r(a["p"]), NQ, a["q"], 0.09, a["lse"], 0.9, a["w_in"], st.stream)
+
+    def evict(**kw):
+        a = dict(dict(p=pages(), dp=st.dp, dt=st.dst.d_table.p, kept=st.kept.p, new=st.new_len.p), **kw)
+        return e.dpuf_amd_paged_evict(r(st.b), r(a["p"]), KEEP, 2, 8, r(a["dp"]), a["dt"], st.dst.table.shape[1],
+                                      a["kept"], a["new"], st.stream)
+
+    # what stays allowed, weights in place among it
+    for call in (rope, attn, weights, evict):
+        assert call() == 0
+    assert weights(w_in=c.dw.p) == 0
+    hip.sync()
+    before = [x.get().tobytes() for x in (st.q, st.out, st.lse, st.kept, st.new_len, c.dk, c.dv, c.dw, c.d_starts,
+                                          c.d_ctx, c.d_table, st.qkv, st.dst.dk, st.dst.dv, st.dst.dw, st.dst.d_table)]
+    bad = []
+    for name, x in {**tables, **pools, "pos": st.pos.p, "turns": st.rope.turns, "norm": scratch.p}.items():
+        bad.append((f"rope: out in {name}", lambda x=x: rope(out=x & ~15)))
+    for name in ("q", "k", "v", "pos", "turns"):
+        for pool, x in pools.items():
+            bad.append((f"rope: {name} in {pool}", lambda x=x, name=name: rope(**{name: x})))
+    bad += [("rope: w in k", lambda: rope(p=pages(w=pools["k"]))), ("rope: w in v", lambda: rope(p=pages(w=pools["v"]))),
+            ("rope: w in the table", lambda: rope(p=pages(w=c.d_table.p)))]
+    for name, x in {**tables, "k": pools["k"], "v": pools["v"], "q": st.q.p}.items():
+        for what in ("out", "lse", "ws"):
+            bad.append((f"attention: {what} in {name}", lambda x=x, what=what: attn(**{what: x & ~15})))
+        if name != "v":
+            bad.append((f"weights: w in {name}", lambda x=x: weights(p=pages(w=x))))
+    bad += [("weights: w in lse", lambda: weights(p=pages(w=st.lse.p))),
+            ("weights: w_in beside w", lambda: weights(w_in=c.dw.p + 4))]
+    dst = dict(dst_k=st.dst.dk.p, dst_v=st.dst.dv.p, dst_w=st.dst.dw.p, dst_table=st.dst.d_table.p)
+    for name, x in {**tables, **pools, **dst}.items():
+        for what in ("kept", "new"):
+            if name != "starts":
+                bad.append((f"evict: {what} in {name}", lambda x=x, what=what: evict(**{what: x})))
+
+    def dst_pages(**kw):
+        p = st.dst.pages()
+        for k, x in kw.items():
+            setattr(p, k, x)
+        return p
+
+    for kw in (dict(w=pools["k"]), dict(w=pools["v"]), dict(w=c.d_table.p), dict(w=st.dst.dk.p), dict(k=c.dw.p),
+               dict(v=c.dw.p), dict(k=c.d_table.p & ~15), dict(w=st.dst.d_table.p), dict(v=st.dst.d_table.p & ~15)):
+        bad.append((f"evict: destination {list(kw)}", lambda kw=kw: evict(dp=dst_pages(**kw))))
+    print(f"{len(bad)} calls with shared memory", flush=True)
+    for name, call in bad:
+        assert call() == -1, name
+    hip.sync()
+    after = [x.get().tobytes() for x in (st.q, st.out, st.lse, st.kept, st.new_len, c.dk, c.dv, c.dw, c.d_starts,
+                                         c.d_ctx, c.d_table, st.qkv, st.dst.dk, st.dst.dv, st.dst.dw, st.dst.d_table)]
+    assert before == after
+    hip.lib.hipStreamDestroy(st.stream)
+
+
+def test_keys_and_values_in_one_allocation(eng, hip):
+    """K and V rows interleaved page by page, and eviction into other pages of
+    the same pool: the same bits as in pools of their own."""
+    rng = np.random.default_rng(21)
+    page, n = 16, 24
+    size = NKV * page * HD
+    kv = R.to_type(rng.standard_normal((n, 2, NKV, page, HD)), R.BF16)
+    w = np.exp(rng.standard_normal((n, NKV, page))).astype(np.float32)
+    table = np.array([[3, 9, 1, 20], [7, 0, -1, -1]], np.int32)
+    dst_table = np.array([[4, 5], [6, 8]], np.int32)
+    ctx, starts = np.array([60, 20], np.int32), np.array([0, 2, 3], np.int32)
+    qkv = rng.standard_normal((3, (NQ + 2 * NKV) * HD)).astype(np.float32)
+    turns, pos = 1e4 ** (-np.arange(64) / 64) / 6.283185307179586, np.array([100, 101, 30], np.int32)
+    got = []
+    print("interleaved pages", flush=True)
+    for together in (0, 1):
+        if together:
+            d = hip.put(kv)
+            k, v, stride = d.p, d.p + 2 * size, 2 * size
+        else:
+            d = [hip.put(np.ascontiguousarray(kv[:, i])) for i in range(2)]
+            k, v, stride = d[0].p, d[1].p, size
+        put = hip.put
+        dw, dt, dd, dc, ds = put(w), put(table), put(dst_table), put(ctx), put(starts)
+        p = abi.DpufAmdPages(type=R.BF16, n_pages=n, page_size=page, n_kv_heads=NKV, head_dim=HD, page_stride=stride,
+                             head_stride=page * HD, row_stride=HD, k=k, v=v, w=dw.p)
+        b = abi.DpufAmdBatch(n_seqs=2, n_rows=3, table_stride=4, max_ctx=60, row_start=ds.p, ctx_len=dc.p,
+                             page_table=dt.p)
+        dq = put(qkv)
+        q, out, lse = (put(np.zeros(s, t)) for s, t in (((3, NQ, HD), np.uint16), ((3, NQ, HD), np.float32),
+                                                        ((3, NQ), np.float32)))
+        kept, new, dp = put(np.zeros((2, NKV, 32), np.int32)), put(np.zeros(2, np.int32)), put(pos)
+        rope = abi.DpufAmdRope(turns=put(turns).p, rot_dim=HD, interleaved=0, scale=1.0)
+        wid = (NQ + 2 * NKV) * HD
+        assert eng.dpuf_amd_rope_append(C.byref(b), C.byref(p), C.byref(rope), dp.p, R.F32, NQ, dq.p, dq.p + NQ * HD * 4,
+                                        dq.p + (NQ + NKV) * HD * 4, wid, wid, wid, None, None, 0.0, q.p, None) == 0
+        ws_n = int(eng.dpuf_amd_paged_attn_workspace(C.byref(b), C.byref(p), NQ))
+        ws = put(np.zeros(max(16, ws_n), np.uint8))
+        assert eng.dpuf_amd_paged_attn(C.byref(b), C.byref(p), NQ, q.p, 0.09, R.F32, out.p, lse.p, ws.p, ws_n, None) == 0
+        assert eng.dpuf_amd_paged_attn_weights(C.byref(b), C.byref(p), NQ, q.p, 0.09, lse.p, 0.9, dw.p, None) == 0
+        assert eng.dpuf_amd_paged_evict(C.byref(b), C.byref(p), 32, 2, 4, C.byref(p), dd.p, 2, kept.p, new.p, None) == 0
+        pools = [d.get()[:, i] for i in range(2)] if together else [x.get() for x in d]
+        got.append([x.tobytes() for x in (q.get(), out.get(), lse.get(), kept.get(), new.get(), dw.get(), *pools)])
+    assert got[0] == got[1]
