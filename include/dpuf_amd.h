@@ -272,7 +272,11 @@ DPUF_EXPORT int32_t dpuf_amd_rope_append(const DpufAmdBatch* batch, const DpufAm
  * cached row to attend to gives 0 and -infinity; rows behind the last
  * sequence's are left as they were.  Probabilities are rounded to the pages'
  * type before the product with V, sums are fp32.  d_workspace of at least
- * dpuf_amd_paged_attn_workspace bytes, on 16 bytes (NULL when that is 0). */
+ * dpuf_amd_paged_attn_workspace bytes, on 16 bytes (NULL when that is 0).  That
+ * is the need of these very arguments: fewer rows, sequences or keys are split
+ * otherwise and may need more, so a program that keeps one workspace takes the
+ * largest over the batches it makes, or asks before each call (the host's
+ * arithmetic alone). */
 DPUF_EXPORT size_t dpuf_amd_paged_attn_workspace(const DpufAmdBatch* batch, const DpufAmdPages* pages,
                                                  int32_t n_q_heads);
 DPUF_EXPORT int32_t dpuf_amd_paged_attn(const DpufAmdBatch* batch, const DpufAmdPages* pages, int32_t n_q_heads,
@@ -319,7 +323,8 @@ DPUF_EXPORT int32_t dpuf_amd_paged_evict(const DpufAmdBatch* batch, const DpufAm
  * logarithmic share of that sum goes to d_logprobs (or NULL).  temperature 0
  * or less (or NaN): the first largest logit, and 0.  A row with no logit above
  * -infinity: -1, and -infinity.  Weights are held as integers of at least
- * 2^-38 of the largest, so sums do not depend on any order. */
+ * 2^-38 of the largest, so sums do not depend on any order.  The workspace is
+ * that of n rows of V: fewer rows are cut into more chunks and may need more. */
 #define DPUF_AMD_SAMPLE_MAX_VOCAB (1 << 24)
 DPUF_EXPORT size_t dpuf_amd_sample_workspace(int32_t n, int32_t V);
 DPUF_EXPORT int32_t dpuf_amd_sample(int32_t type, int32_t n, int32_t V, int64_t row_stride, const void* d_logits,

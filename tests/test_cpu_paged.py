@@ -194,3 +194,26 @@ def test_null_descriptors(lib):
 def test_structure_sizes():
     assert C.sizeof(abi.DpufAmdPages) == 72 and C.sizeof(abi.DpufAmdBatch) == 40
     assert C.sizeof(abi.DpufAmdRopeSpec) == 36 and C.sizeof(abi.DpufAmdRope) == 24
+
+
+def test_workspaces_are_those_of_the_arguments(lib):
+    """A workspace of the size given for a call's own arguments is enough, one
+    byte less is not, and a smaller call may need a larger one."""
+    V, sizes = 151936, []
+    for n in (1, 2, 7, 56, 57, 1024, 5000):
+        need = lib.dpuf_amd_sample_workspace(n, V)
+        run = lambda size: lib.dpuf_amd_sample(0, n, V, V, A, None, None, None, None, LSE + (1 << 40), OUT + (1 << 41), None,
+                                               WS + (1 << 42), size, None)
+        assert run(need - 1) == -7 and run(need) == -1      # -1: no device memory
+        sizes.append(need)
+    assert sizes[3] > sizes[4]
+    p, nq, sizes = pages(n_kv_heads=8, page_stride=8 * 16 * 64), 32, []
+    for seqs, rows, ctx in ((1, 1, 4096), (1, 512, 4096), (4, 512, 4096), (64, 64, 4096), (512, 512, 4096),
+                            (2048, 2048, 4096)):
+        b = batch(n_seqs=seqs, n_rows=rows, table_stride=1 << 10, max_ctx=ctx)
+        need = lib.dpuf_amd_paged_attn_workspace(C.byref(b), C.byref(p), nq)
+        if need:
+            assert attn(lib, b=b, p=p, nq=nq, n=need - 1) == -7
+        assert attn(lib, b=b, p=p, nq=nq, n=need) == -1
+        sizes.append(need)
+    assert max(sizes[:-1]) > sizes[-1]
