@@ -765,9 +765,15 @@ int range_of(int64_t ctx, double times) { return ((int)(times * sqrt((double)ctx
 // one, but not so long that a batch's shorter sequences leave them idle.  One
 // row of 32 heads, 8 kv heads of 128: over 1 500 keys 22.3 us in ranges of
 // 1 024, 15.9 in 512, 12.6 in 256, 10.7 in 128; over 4 096 22.6, 15.7, 12.6,
-// 10.6; over 16 384 23.9, 19.8, 20.9, 20.8; over 300 10.7 in one, 9.8 in three.
-// 16 rows over 500 to 8 000 keys 56.2, 53.7, 53.4, 61.6; 48 rows 160.5, 164,
-// 164, 172.
+// 10.6; over 16 384 23.9, 19.8, 20.9, 20.8.  16 rows over 500 to 8 000 keys
+// 56.2, 53.7, 53.4, 61.6; 48 rows 160.5, 164, 164, 172.
+//
+// Short contexts are one range, since the join is a launch more: one row over
+// 200 keys 8.7 us in one, 9.4 in two, over 150 8.2 and 8.8.  From 257 keys on
+// they are split where all ranges of 128 fit on the card at once, four of
+// them from up to 64 (sequence, kv head): one row over 300 keys 10.2 in one,
+// 9.3 in three, over 512 11.7 and 9.2; 8 rows 10.4 and 9.6, 12.5 and 10.8; but
+// 12 rows 11.0 and 12.5, 12.7 and 12.9, 16 rows 11.6 and 12.1, 12.8 and 14.0.
 PaPlan plan(const DpufAmdBatch& b, const DpufAmdPages& p, int nq) {
     const int G = nq / p.n_kv_heads;
     PaPlan r;
@@ -782,9 +788,10 @@ PaPlan plan(const DpufAmdBatch& b, const DpufAmdPages& p, int nq) {
     r.y_few = r.only >= PA_MANY ? 0 : b.n_seqs * ((r.few + 15) / 16);
     r.y_many = r.only == PA_FEW ? 0 : r.only == PA_BOTH ? (int)(packed / 128 + (most < b.n_seqs ? most : b.n_seqs))
                                                         : ceil_div(packed, tr);
-        const int64_t units = (int64_t)b.n_seqs * p.n_kv_heads;
+    const int64_t units = (int64_t)b.n_seqs * p.n_kv_heads;
     const int64_t even = (ctx * units / 256 + 127) & ~127, long_few = units >= 256 ? 1024 : 512;
-    r.chunk_few = ctx <= 512 || even > long_few ? (int)long_few : even < 128 ? 128 : (int)even;
+    const bool whole = ctx <= (units <= 64 ? 256 : 512);
+    r.chunk_few = whole || even > long_few ? (int)long_few : even < 128 ? 128 : (int)even;
     r.nz_few = ceil_div(ctx, r.chunk_few);
     if (r.nz_few > 64) r.nz_few = 64;
     // (kv heads x sequences) that fill the card by themselves need no ranges,

@@ -438,3 +438,17 @@ def test_fp16_probabilities_far_below_the_largest(eng, hip, rows, ctx, max_ctx, 
     say(f"  worst error {float((err / bound).max()):.3f} of the bound")
     assert np.all(err <= bound)
     assert np.all(np.abs(lse - rl) <= R.score_error(S, hd) + np.abs(rl) * 2.0 ** -22 + 2.0 ** -20)
+
+
+@pytest.mark.parametrize("nkv,seqs", [(2, 1), (8, 8), (8, 9)])
+@pytest.mark.parametrize("ctx", [255, 256, 257, 300, 511, 512, 513])
+def test_short_contexts(eng, hip, ctx, nkv, seqs):
+    """One range of keys and a few, at the lengths where that changes."""
+    rng = np.random.default_rng(ctx + seqs)
+    cache = R.Cache(hip, rng, R.BF16, [1] * seqs, [ctx] + [7] * (seqs - 1), nkv, 64, 16)
+    nq = 2 * nkv
+    q = R.to_type(rng.standard_normal((cache.n_rows, nq, 64)) * 1.5, R.BF16)
+    say(f"short contexts: {ctx} keys, {seqs} sequences of {nkv} kv heads")
+    out, lse, *_, ws = call(eng, hip, cache, nq, q, 0.125)
+    assert (ws > 0) == (ctx > (256 if seqs * nkv <= 64 else 512))
+    check(cache, nq, q, 0.125, out, lse, R.BF16)
