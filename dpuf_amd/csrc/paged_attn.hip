@@ -129,8 +129,8 @@ template <typename T> DEV f32x4 odd4(const uint16_t* v) {
 // take every fourth tile of 32 keys with sums of their own and meet in LDS at
 // the end, so there is no barrier in the loop and each wave keeps a whole
 // next tile (K and V, 16 KB at 128 columns) in flight in registers.  48 rows of
-// 32 heads, 8 kv heads of 128 over 310 to 6 000 keys: 119 us, 5.2 TB/s; one row
-// of 16 heads over 75 keys 7.4.
+// 32 heads, 8 kv heads of 128 over 310 to 6 000 keys: 122 us, 5.1 TB/s; one row
+// of 16 heads over 75 keys 7.7.
 // ---------------------------------------------------------------------------
 template <int HD> struct FewLds {
     static constexpr int PITCH = HD + 16;   // elements of a V row: 4 rows of a transposing read in 4 bank groups
@@ -804,7 +804,12 @@ PaPlan plan(const DpufAmdBatch& b, const DpufAmdPages& p, int nq) {
     // time (a chunk of 256 rows and 31 single rows over 500 to 6 000 keys: 122
     // us with room for 400, 134 for 512, 140 for 768), unless the chunks are
     // nearly all of the work: then more, since the shorter contexts end sooner
-    // (three of 128 rows and a single one over 4 096 to 16 384: 201, 157, 119)
+    // (three of 128 rows and a single one over 4 096 to 16 384: 201, 157, 119).
+    // Two values for what varies with tiles, single rows and contexts: of 54
+    // batches of 1 to 4 chunks of 64 to 256 rows beside 1, 7 or 31 single rows,
+    // 39 are within 10 % of the best of 256 to 1 024, 7 % in the middle; the
+    // farthest is four of 64 and a single one over 4 096 to 16 384, 131 with
+    // 400 and 85 with 768
     const bool chunks = (int64_t)(b.n_rows - b.n_seqs) * G > 220 * (int64_t)b.n_seqs;
     const int64_t room = r.only == PA_WIDE ? 256 : r.only == PA_MANY ? 512 : chunks ? 768 : 400;
     const int64_t wgs = (packed + tr - 1) / tr * p.n_kv_heads;

@@ -155,7 +155,7 @@ __global__ __launch_bounds__(256) void k_rope_append(RaArgs a) {
 // step ahead, so that each is read from memory once for all its keys (as the
 // matrix operand straight from the L1, 32 bytes of a row a load, it was that
 // which took the time: 256 rows of 4 heads, 8 kv heads over 4 096 keys 24.3 us
-// against 20.2).  Bound then by the matrix instructions and, of about the same
+// against 20.4).  Bound then by the matrix instructions and, of about the same
 // length, the exponentials and the queries' way through LDS.
 // ---------------------------------------------------------------------------
 struct PwArgs {
@@ -363,7 +363,7 @@ __global__ __launch_bounds__(64 * KG * RG) void k_pa_weights(PwArgs a) {
 // operand of 16 x 16 steps, so that a load of the wave takes 64 consecutive
 // bytes of 16 rows (of 32 rows 32 bytes, as above, it reached 3.8 TB/s); NB
 // blocks a wave, and the next ones in flight.  24 rows of 32 heads, 8 kv heads of
-// 128 over 900 to 4 096 keys: 27 us, 4.7 TB/s.
+// 128 over 900 to 4 096 keys: 27.6 us, 4.6 TB/s.
 template <typename T, int HD>
 __global__ __launch_bounds__(256) void k_pa_weights_few(PwArgs a) {
     constexpr int NC = HD / 32, NB = HD == 256 ? 2 : 4, WK = 16 * NB;
@@ -870,7 +870,7 @@ void weights_many(const PwArgs& a, int64_t ctx, int64_t rows_of_tiles, hipStream
 // steps are latency rather than work while the card is not full: 256 rows of 8
 // heads, 2 kv heads of 64 columns over 4 096 keys 10.5 us with 32 keys (256
 // tiles), 14.5 with 64, 22 with 128; 256 rows of 4 heads, 8 kv heads of 128
-// over 2 000 19.7, 12.6, 18.5 (500, 250, 125 tiles); over 4 096 39, 24.5, 20.2.
+// over 2 000 19.7, 12.6, 18.5 (500, 250, 125 tiles); over 4 096 39, 24.5, 20.4.
 constexpr int LIM = 128;
 template <typename T, int HD> void weights_hd(PwArgs a, int64_t ctx, hipStream_t st) {
     const int64_t G = a.G, nkv = a.p.n_kv_heads, n = a.b.n_seqs, packed = a.b.n_rows * G, cus = dpuf_hip_cu_count();
