@@ -21,6 +21,7 @@ typedef s16x4 __attribute__((address_space(3))) * lds_s16x4;
 struct Bf16 {
     static constexpr uint32_t EXP = 0x7f80;     // exponent bits
     static constexpr float LIFT = 0.0f;
+    static constexpr bool REST = true;          // probabilities of few rows as two terms: 8 bits are few
     typedef __bf16 e;
     typedef __bf16 v8 __attribute__((ext_vector_type(8)));
     typedef __bf16 v4 __attribute__((ext_vector_type(4)));
@@ -32,6 +33,7 @@ struct Fp16 {
     static constexpr uint32_t EXP = 0x7c00;
     // Probabilities are 2^LIFT times as large: fp16's normal numbers end at 2^-14
     static constexpr float LIFT = 9.0f;
+    static constexpr bool REST = false;
     typedef _Float16 e;
     typedef _Float16 v8 __attribute__((ext_vector_type(8)));
     typedef _Float16 v4 __attribute__((ext_vector_type(4)));

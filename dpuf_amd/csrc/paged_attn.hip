@@ -22,14 +22,20 @@
 // more than 2^SLACK, so that most tiles move nothing; p is at most 2^SLACK
 // then.
 //
-// Exponentials are of base 2 with the scale folded in (one fma each); p is
-// rounded to the pages' type for the product with V (a relative half step,
-// 2^-8 in bf16 and 2^-11 in fp16, of each term), every sum is fp32.  fp16 has
-// few exponents: below 2^-14 of the largest, terms would lose their bits, and
-// below 2^-25 vanish, however many there are.  So there m is LIFT = 9 below the
-// maximum: p is at most 2^(9 + SLACK) = 2^15, and whole down to 2^-23 of the
-// largest.  The maximum is then rounded up to an integer, which keeps m + LIFT
-// and the factors that l and o are moved by exact.
+// Exponentials are of base 2 with the scale folded in (one fma each), every sum
+// is fp32.  The 16-bit matrix instructions take p rounded to the pages' type (a
+// relative half step, 2^-8 in bf16 and 2^-11 in fp16, of each term).  In bf16
+// few rows, which wait for memory, add what that takes off by a second product
+// (48 rows over 310 to 6 000 keys 125.4 us without, 125.8 with; the outputs are
+// off from 64 bits by 2.2e-3 and 1.7e-3, nearly all of the latter their own
+// rounding).  Many rows do not: 512 over 16 384 keys would take 213 us instead
+// of 169, for 1.7e-3 instead of 2.3e-3.
+//
+// fp16 has few exponents: below 2^-14 of the largest, terms would lose their
+// bits, and below 2^-25 vanish, however many there are.  So there m is LIFT = 9
+// below the maximum: p is at most 2^(9 + SLACK) = 2^15, and whole down to 2^-23
+// of the largest.  The maximum is then rounded up to an integer, which keeps
+// m + LIFT and the factors that l and o are moved by exact.
 #include <hip/hip_runtime.h>
 #include <math.h>
 #include <stdint.h>
@@ -121,6 +127,29 @@ template <typename T> DEV f32x4 odd4(const uint16_t* v) {
     const uint2 w = *(const uint2*)v;
     return __builtin_convertvector(
         __builtin_bit_cast(typename T::v4, make_uint2(w.x & odd_mask<T>(w.x), w.y & odd_mask<T>(w.y))), f32x4);
+}
+
+// Eight probabilities as an operand of the product with V, and, with T::REST,
+// what that leaves of them as another.  The first is cut off rather than
+// rounded, and the rest at least 2^-30 of p, so that neither is negative, nor 0
+// where p is not: an infinity in V stays what it is.
+template <typename T> DEV void split8(float* p, typename T::v8& hi, typename T::v8& rest) {
+    u32x4 h, r;
+    if constexpr (T::REST) {
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            h[i] = __builtin_amdgcn_perm(__float_as_uint(p[2 * i + 1]), __float_as_uint(p[2 * i]), 0x07060302);
+#pragma unroll
+            for (int e = 2 * i; e < 2 * i + 2; e++)
+                p[e] = fmaxf(p[e] - __uint_as_float(__float_as_uint(p[e]) & 0xffff0000u), p[e] * 0x1p-30f);
+            r[i] = pack2<T>(p[2 * i], p[2 * i + 1]);
+        }
+        rest = vec_of<typename T::v8>(r);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; i++) h[i] = pack2<T>(p[2 * i], p[2 * i + 1]);
+    }
+    hi = vec_of<typename T::v8>(h);
 }
 
 // ---------------------------------------------------------------------------
@@ -284,16 +313,17 @@ template <typename T, int HD> DEV void few_rows(const PaArgs& a, FewLds<HD>& sh,
                     pr[4 * u + i] = __builtin_amdgcn_exp2f(fmaf(sc[u][i], a.c2, -ms));
                     l += pr[4 * u + i];
                 }
-            const u32x4 pw = {pack2<T>(pr[0], pr[1]), pack2<T>(pr[2], pr[3]), pack2<T>(pr[4], pr[5]),
-                              pack2<T>(pr[6], pr[7])};
-            const v8 pf = vec_of<v8>(pw);
+            v8 pf, rf;
+            split8<T>(pr, pf, rf);
             lds_order();
             const uint16_t* tr = lv + (4 * g4 + (col >> 2)) * PITCH + 4 * (col & 3);
 #pragma unroll
             for (int d = 0; d < ND; d++) {
                 const s16x4 lo = lds_tr4(tr + 16 * d), hi = lds_tr4(tr + 16 * PITCH + 16 * d);
                 const uint2 a0 = __builtin_bit_cast(uint2, lo), a1 = __builtin_bit_cast(uint2, hi);
-                o[d] = T::mma16(vec_of<v8>(u32x4{a0.x, a0.y, a1.x, a1.y}), pf, o[d]);
+                const v8 vt = vec_of<v8>(u32x4{a0.x, a0.y, a1.x, a1.y});
+                o[d] = T::mma16(vt, pf, o[d]);
+                if (T::REST) o[d] = T::mma16(vt, rf, o[d]);
             }
         }
 

@@ -270,9 +270,11 @@ DPUF_EXPORT int32_t dpuf_amd_rope_append(const DpufAmdBatch* batch, const DpufAm
  * same shape, out_type that type or DPUF_AMD_F32; d_lse [n_rows][n_q_heads]
  * (or NULL) the logarithm of each row's sum of exp(scale q.k).  A row with no
  * cached row to attend to gives 0 and -infinity; rows behind the last
- * sequence's are left as they were.  Probabilities are rounded to the pages'
- * type before the product with V, sums are fp32.  d_workspace of at least
- * dpuf_amd_paged_attn_workspace bytes, on 16 bytes (NULL when that is 0).  That
+ * sequence's are left as they were.  Sums are fp32; probabilities enter the
+ * product with V rounded to the pages' type, and in bf16 those of decoding
+ * sequences (up to 16 new rows times query heads per kv head, 32 where a row
+ * alone has more than 16) with the remainder beside them.  d_workspace of at
+ * least dpuf_amd_paged_attn_workspace bytes, on 16 bytes (NULL when that is 0).  That
  * is the need of these very arguments: fewer rows, sequences or keys are split
  * otherwise and may need more, so a program that keeps one workspace takes the
  * largest over the batches it makes, or asks before each call (the host's

@@ -452,3 +452,83 @@ def test_short_contexts(eng, hip, ctx, nkv, seqs):
     out, lse, *_, ws = call(eng, hip, cache, nq, q, 0.125)
     assert (ws > 0) == (ctx > (256 if seqs * nkv <= 64 else 512))
     check(cache, nq, q, 0.125, out, lse, R.BF16)
+
+
+DECODE = [([1], [75]), ([1, 1, 1], [900, 3, 2111]), ([1, 70, 1, 1], [700, 90, 33, 400]), ([0, 3, 0, 1], [5, 50, 0, 300])]
+
+
+@pytest.mark.parametrize("hd", [64, 128, 256])
+@pytest.mark.parametrize("rows,ctx", DECODE)
+def test_decoding_rows_keep_their_probabilities(eng, hip, rows, ctx, hd):
+    """bf16 pages, outputs in fp32: decoding sequences' probabilities are held
+    in two terms, so that their outputs are off by far less than bf16's step."""
+    rng = np.random.default_rng(hd + sum(ctx))
+    nq, nkv = 8, 2
+    cache = R.Cache(hip, rng, R.BF16, rows, ctx, nkv, hd, 16)
+    q = R.to_type(rng.standard_normal((cache.n_rows, nq, hd)) * 1.5, R.BF16)
+    say(f"two terms: rows {rows}, contexts {ctx}, hd {hd}")
+    out, lse, *_ = call(eng, hip, cache, nq, q, 0.1, out_t=R.F32)
+    ref, rl, A, S, _, _ = R.attention(cache, R.from_type(q, R.BF16), float(np.float32(0.1)), nq)
+    # what the first term leaves is at most 2^-7 of a probability, and rounded by 2^-8 of that; the rest as in
+    # attention_bound
+    d = R.score_error(S, hd)[..., None]
+    bound = A * (2.0 ** -15 + 2.0 ** -24 + 2 * d + (max(ctx) + 64) * 2.0 ** -24) * 1.01 + 1e-30
+    for s, (r, c) in enumerate(zip(rows, ctx)):
+        if r * nq // nkv > 16 and sum(rows) > len(rows):      # a chunk: rounded once
+            continue
+        at = slice(cache.starts[s], cache.starts[s + 1])
+        assert np.all(np.abs(out[at] - ref[at]) <= bound[at]), s
+
+
+@pytest.mark.parametrize("t", [R.BF16, R.F16])
+@pytest.mark.parametrize("hd", [64, 128, 256])
+@pytest.mark.parametrize("rows,ctx,max_ctx", [([1, 1], [400, 90], None), ([1], [3000], None), ([40], [700], None),
+                                              ([97], [2300], None), ([1, 70], [400, 500], None)])
+def test_infinities_that_all_rows_see(eng, hip, rows, ctx, max_ctx, hd, t):
+    """Infinities and NaN in values of old keys, in tiles that every row sees
+    whole: infinite of their sign, NaN where both meet."""
+    rng = np.random.default_rng(hd + t)
+    nq, nkv = 8, 2
+    cache = R.Cache(hip, rng, t, rows, ctx, nkv, hd, 16)
+    inf, nan = R.to_type([np.inf, -np.inf, np.nan], t)[:2], R.to_type([np.nan], t)[0]
+    for s in range(len(ctx)):
+        for i, col, x in ((0, 1, inf[0]), (9, 2, inf[1]), (20, 3, inf[0]), (21, 3, inf[1]), (16, 4, nan), (5, 6, inf[0]),
+                          (17, 6, inf[0])):
+            cache.row(cache.v, cache.table[s, i // 16], i % 16)[:, col] = x
+    cache.dv.set(cache.v)
+    q = R.to_type(rng.standard_normal((cache.n_rows, nq, hd)) * 0.5, t)
+    say(f"infinities: rows {rows}, contexts {ctx}, hd {hd}, type {t}")
+    out, lse, *_ = call(eng, hip, cache, nq, q, 0.1, out_t=R.F32, max_ctx=max_ctx)
+    with np.errstate(all="ignore"):
+        ref, rl, A, S, _, _ = R.attention(cache, R.from_type(q, t), float(np.float32(0.1)), nq)
+    assert np.isposinf(ref).any() and np.isneginf(ref).any() and np.isnan(ref).any()
+    for kind in (np.isnan, np.isposinf, np.isneginf):
+        assert np.array_equal(kind(out), kind(ref))
+    # finite values are below 10 (standard normal)
+    ok = np.isfinite(ref)
+    with np.errstate(all="ignore"):
+        bound = R.attention_bound(t, R.F32, ref, A, S, np.full(S.shape, 10.0), hd, max(ctx))
+    assert np.all(np.abs(out[ok] - ref[ok]) <= bound[ok])
+
+
+def test_huge_values_that_a_row_does_not_see(eng, hip):
+    """bf16's largest numbers behind a row's last key, and in absent pages,
+    reach it by no share of them, however small."""
+    rng = np.random.default_rng(5)
+    for rows, ctx in (([1, 3, 0, 1], [33, 20, 4, 100]), ([30], [70])):
+        cache = R.Cache(hip, rng, R.BF16, rows, ctx, 2, 128, 16, bad=[(0, 1)])
+        q = R.to_type(rng.standard_normal((cache.n_rows, 8, 128)), R.BF16)
+        outs = []
+        for huge in (False, True):
+            if huge:
+                seen = np.zeros(cache.v.shape, bool)
+                for s, (r, c) in enumerate(zip(rows, ctx)):
+                    for i in range(c - r + 1 if r else 0):
+                        if cache.ok(s, i):
+                            seen[cache.table[s, i // 16], :, i % 16] = True
+                cache.v = np.where(seen, cache.v, R.to_type([3.3e38], R.BF16)[0])
+                cache.dv.set(cache.v)
+            say(f"huge values {huge}: rows {rows}")
+            out, lse, *_ = call(eng, hip, cache, 8, q, 0.1, out_t=R.F32)
+            outs.append(out[[int(cache.starts[s]) for s in range(len(rows)) if rows[s]]])
+        assert np.array_equal(outs[0], outs[1])
