@@ -148,6 +148,8 @@ typedef struct {
     size_t pg_ws_bytes;
     int32_t *h_pg, *d_pg;
     size_t pg_ints;
+    int32_t* pg_kept;    /* rows that an eviction keeps, layer by layer */
+    size_t pg_kept_ints;
     DpufAmdBatch pg_b;   /* of the call at work; n_seqs 0: the layers run over slots */
     int32_t* pg_pos;
     float pg_decay;
@@ -503,7 +505,7 @@ static void prefix_copy(Engine* e, int32_t s, int32_t p, int32_t len, int to_pre
 }
 
 static void pages_free(Engine* e) {
-    void* const d[] = {e->pg_k, e->pg_v, e->pg_w, e->pg_q, e->pg_lse, e->pg_turns, e->pg_ws, e->d_pg};
+    void* const d[] = {e->pg_k, e->pg_v, e->pg_w, e->pg_q, e->pg_lse, e->pg_turns, e->pg_ws, e->d_pg, e->pg_kept};
     for (size_t i = 0; i < sizeof d / sizeof d[0]; i++) dpuf_hip_free(d[i]);
     dpuf_hip_host_free(e->h_pg);
     e->pg_k = e->pg_v = e->pg_q = NULL;
@@ -511,7 +513,8 @@ static void pages_free(Engine* e) {
     e->pg_turns = NULL;
     e->pg_ws = NULL;
     e->h_pg = e->d_pg = NULL;
-    e->pg_ws_bytes = e->pg_ints = 0;
+    e->pg_kept = NULL;
+    e->pg_ws_bytes = e->pg_ints = e->pg_kept_ints = 0;
     e->pg_n = 0;
 }
 
@@ -1747,7 +1750,12 @@ DPUF_EXPORT int32_t dpuf_amd_engine_evict_pages(void* handle, int32_t n, const i
     int32_t rc = len && uses && dst_uses ? 0 : -2;
     if (rc == 0) rc = check_tables(e, n, ctx_len, page_table, table_stride, 0, uses);
     if (rc == 0) {
-        for (int32_t i = 0; i < n; i++) len[i] = ctx_len[i] < keep ? ctx_len[i] : keep;
+        int32_t longest = 1;
+        for (int32_t i = 0; i < n; i++) {
+            len[i] = ctx_len[i] < keep ? ctx_len[i] : keep;
+            if (ctx_len[i] > longest) longest = ctx_len[i];
+        }
+        if (keep > longest) keep = longest;      /* every row stays: sink and recent say nothing */
         rc = check_tables(e, n, len, dst_table, dst_stride, 0, dst_uses);
     }
     for (int32_t p = 0; p < e->pg_n && rc == 0; p++)
@@ -1760,9 +1768,13 @@ DPUF_EXPORT int32_t dpuf_amd_engine_evict_pages(void* handle, int32_t n, const i
     }
     begin_call(e);
     const size_t ints = (size_t)2 * n + (size_t)n * table_stride + (size_t)n * dst_stride;
-    int32_t* kept = (int32_t*)dpuf_hip_malloc((size_t)n * e->nkv * keep * 4);
-    if (!kept || !pages_staging(e, ints)) {
-        dpuf_hip_free(kept);
+    const size_t list = (size_t)n * e->nkv * keep;
+    if (list > e->pg_kept_ints) {
+        dpuf_hip_free(e->pg_kept);
+        e->pg_kept = (int32_t*)dpuf_hip_malloc(list * 4);
+        e->pg_kept_ints = e->pg_kept ? list : 0;
+    }
+    if (!e->pg_kept || !pages_staging(e, ints)) {
         free(len);
         return -2;
     }
@@ -1781,10 +1793,10 @@ DPUF_EXPORT int32_t dpuf_amd_engine_evict_pages(void* handle, int32_t n, const i
     b.page_table = e->d_pg + (ht - hc);
     for (int32_t l = 0; l < e->L; l++) {
         const DpufAmdPages p = pages_of(e, l);
-        dpuf_hip_paged_evict(e->stream, &b, &p, keep, sink, recent, &p, e->d_pg + (hd - hc), dst_stride, kept, d_len);
+        dpuf_hip_paged_evict(e->stream, &b, &p, keep, sink, recent, &p, e->d_pg + (hd - hc), dst_stride, e->pg_kept,
+                             d_len);
     }
     rc = dpuf_hip_sync(e->stream) == 0 && dpuf_hip_ok() ? 0 : -6;
-    dpuf_hip_free(kept);
     if (rc == 0) memcpy(new_len, len, (size_t)n * 4);
     free(len);
     return rc;

@@ -415,3 +415,37 @@ def test_sampled_steps_do_not_exit_early(eng, monkeypatch):
         assert eng.dpuf_amd_engine_early_exit_count(h) == exits
     assert beyond > 0
     eng.dpuf_engine_destroy(h)
+
+
+def test_eviction_that_keeps_all(eng, hip):
+    """keep far beyond every length: all rows move to the other pages, whatever
+    sink and recent are, and the list of rows that stay is as long as the
+    sequences, not as keep (20 x 2 x 2^30 entries would not fit the card)."""
+    m, h = _engine(eng)
+    n, page = 20, 1024
+    assert eng.dpuf_amd_engine_pages_create(h, 2 * n, page, R.BF16) == 0
+    rng = np.random.default_rng(11)
+    rows = np.array([1 + i % 7 for i in range(n)], np.int32)
+    table = np.arange(n, dtype=np.int32)[:, None].copy()
+    ids, pos = rng.integers(0, V, rows.sum()).astype(np.int32), np.concatenate([np.arange(r) for r in rows]).astype(np.int32)
+    lg = np.zeros((n, V), np.float32)
+    assert eng.dpuf_amd_engine_forward_pages(h, n, M.ptr(rows), M.ptr(rows), M.ptr(table), 1, M.ptr(ids), M.ptr(pos), 1.0,
+                                             None, M.ptr(lg), None, None) == 0
+    stride = 1 << 20
+    dst = np.full((n, stride), -1, np.int32)
+    dst[:, 0] = n + rng.permutation(n)
+    new = np.zeros(n, np.int32)
+    say(f"keep {page * stride} of up to 7 rows")
+    assert eng.dpuf_amd_engine_evict_pages(h, n, M.ptr(rows), M.ptr(table), 1, page * stride, 5, 9, M.ptr(dst), stride,
+                                           M.ptr(new)) == 0, eng.dpuf_amd_last_error()
+    assert np.array_equal(new, rows)
+    for l in range(2):
+        p = abi.DpufAmdPages()
+        assert eng.dpuf_amd_engine_pages(h, l, C.byref(p)) == 0
+        for at, width, t in ((p.k, 64, np.uint16), (p.v, 64, np.uint16), (p.w, 1, np.float32)):
+            got = np.empty((2 * n, 2, page, width), t)
+            assert hip.lib.hipMemcpy(M.ptr(got), at, got.nbytes, R.D2H) == 0
+            for i in range(n):
+                assert got[i, :, :rows[i]].any()
+                assert np.array_equal(got[i, :, :rows[i]], got[dst[i, 0], :, :rows[i]])
+    eng.dpuf_engine_destroy(h)
