@@ -168,9 +168,9 @@ DPUF_EXPORT int32_t dpuf_amd_verify_tiles_device(int32_t mode, int32_t n_tiles, 
  * workspace that shares memory with anything else that the call reads or
  * writes (pools count from their first row to their last; k and v of one
  * allocation may interleave, and an operator says where it works in place);
- * -2 a size or setting out of range; -4 a stride that is not a
- * multiple of 8 elements or too small; -5 a type or head dim that is not
- * built; -6 device error (dpuf_amd_last_error); -7 workspace too small. */
+ * -2 a size or setting out of range; -4 a stride that is not a multiple of 8
+ * elements or too small; -5 a type or head dim that is not built; -6 device
+ * error (dpuf_amd_last_error); -7 workspace too small. */
 
 /* Element types. */
 enum {
@@ -274,11 +274,11 @@ DPUF_EXPORT int32_t dpuf_amd_rope_append(const DpufAmdBatch* batch, const DpufAm
  * product with V rounded to the pages' type, and in bf16 those of decoding
  * sequences (up to 16 new rows times query heads per kv head, 32 where a row
  * alone has more than 16) with the remainder beside them.  d_workspace of at
- * least dpuf_amd_paged_attn_workspace bytes, on 16 bytes (NULL when that is 0).  That
- * is the need of these very arguments: fewer rows, sequences or keys are split
- * otherwise and may need more, so a program that keeps one workspace takes the
- * largest over the batches it makes, or asks before each call (the host's
- * arithmetic alone). */
+ * least dpuf_amd_paged_attn_workspace bytes, on 16 bytes (NULL when that is 0).
+ * That is the need of these very arguments: fewer rows, sequences or keys are
+ * split otherwise and may need more, so a program that keeps one workspace
+ * takes the largest over the batches it makes, or asks before each call (the
+ * host's arithmetic alone). */
 DPUF_EXPORT size_t dpuf_amd_paged_attn_workspace(const DpufAmdBatch* batch, const DpufAmdPages* pages,
                                                  int32_t n_q_heads);
 DPUF_EXPORT int32_t dpuf_amd_paged_attn(const DpufAmdBatch* batch, const DpufAmdPages* pages, int32_t n_q_heads,
