@@ -145,6 +145,15 @@ class DpufAmdRope(C.Structure):
     ]
 
 
+class DpufAmdRopeAxes(C.Structure):
+    """Position axes of a rotation's pairs (include/dpuf_amd.h)."""
+    _fields_ = [
+        ("n_axes", C.c_int32),
+        ("sections", C.c_int32 * 4),
+        ("in_turn", C.c_int32),
+    ]
+
+
 class DpufAmdSampling(C.Structure):
     """Host arrays of an engine call's sampling settings (include/dpuf_amd.h)."""
     _fields_ = [
@@ -294,10 +303,16 @@ def load_engine():
                                             P, P, F32, P, P])
     _sig(lib, "dpuf_amd_paged_attn_workspace", C.c_size_t, [batch, pages, I32])
     _sig(lib, "dpuf_amd_paged_attn", I32, [batch, pages, I32, P, F32, I32, P, P, P, C.c_size_t, P])
+    _sig(lib, "dpuf_amd_rope_append_axes", I32, [batch, pages, C.POINTER(DpufAmdRope), C.POINTER(DpufAmdRopeAxes), P,
+                                                 I64, I32, I32, P, P, P, I64, I64, I64, P, P, F32, P, P])
+    _sig(lib, "dpuf_amd_paged_attn_window_workspace", C.c_size_t, [batch, pages, I32, I32, I32])
+    _sig(lib, "dpuf_amd_paged_attn_window", I32, [batch, pages, I32, P, F32, I32, I32, I32, P, P, P, C.c_size_t, P])
     _sig(lib, "dpuf_amd_paged_attn_weights", I32, [batch, pages, I32, P, F32, P, F32, P, P])
     _sig(lib, "dpuf_amd_paged_evict", I32, [batch, pages, I32, I32, I32, pages, P, I32, P, P, P])
     _sig(lib, "dpuf_amd_sample_workspace", C.c_size_t, [I32, I32])
     _sig(lib, "dpuf_amd_sample", I32, [I32, I32, I32, I64, P, P, P, P, P, P, P, P, P, C.c_size_t, P])
+    _sig(lib, "dpuf_amd_logprobs_workspace", C.c_size_t, [I32, I32, I32])
+    _sig(lib, "dpuf_amd_logprobs", I32, [I32, I32, I32, I64, P, I32, P, I32, P, P, P, P, P, C.c_size_t, P])
     smp = C.POINTER(DpufAmdSampling)
     _sig(lib, "dpuf_amd_engine_forward_sample", I32, [P, I32, P, I32, P, I32, smp, P, P, P])
     _sig(lib, "dpuf_amd_engine_forward_slots_sample", I32, [P, I32, P, P, P, smp, P, P, P])

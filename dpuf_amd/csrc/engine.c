@@ -1021,9 +1021,9 @@ static DpufAmdPages pages_of(const Engine* e, int32_t l) {
 static void enqueue_paged_attention(Engine* e, int32_t l, float scale, float eps) {
     void* s = e->stream;
     const DpufAmdPages p = pages_of(e, l);
-    dpuf_hip_rope_append(s, &e->pg_b, &p, &e->pg_rope, e->pg_pos, DPUF_AMD_F32, e->nq, e->q, e->k, e->v, e->qd, e->kvd,
+    dpuf_hip_rope_append(s, &e->pg_b, &p, &e->pg_rope, NULL, e->pg_pos, 0, DPUF_AMD_F32, e->nq, e->q, e->k, e->v, e->qd, e->kvd,
                          e->kvd, e->d_norm[4 * l + 1], e->d_norm[4 * l + 2], eps, e->pg_q);
-    dpuf_hip_paged_attn(s, &e->pg_b, &p, e->nq, e->pg_q, scale, 1, e->ao, e->pg_lse, e->pg_ws);
+    dpuf_hip_paged_attn(s, &e->pg_b, &p, e->nq, e->pg_q, scale, 0, 0, 1, e->ao, e->pg_lse, e->pg_ws);
     if (e->pg_decay >= 0.0f)
         dpuf_hip_paged_attn_weights(s, &e->pg_b, &p, e->nq, e->pg_q, scale, e->pg_lse, e->pg_decay, p.w);
 }
@@ -1687,7 +1687,7 @@ DPUF_EXPORT int32_t dpuf_amd_engine_forward_pages(void* handle, int32_t n, const
     b.ctx_len = e->d_pg + (hc - hs);
     b.page_table = e->d_pg + (ht - hs);
     const DpufAmdPages p0 = pages_of(e, 0);
-    const size_t ws = dpuf_hip_paged_attn_workspace(&b, &p0, e->nq);
+    const size_t ws = dpuf_hip_paged_attn_workspace(&b, &p0, e->nq, 0, 0);
     if (ws > e->pg_ws_bytes) {
         dpuf_hip_free(e->pg_ws);
         e->pg_ws = dpuf_hip_malloc(ws);

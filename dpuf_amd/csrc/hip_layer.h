@@ -304,13 +304,16 @@ void dpuf_hip_device_leave(int32_t back);
 
 /* The paged-serving operators behind include/dpuf_amd.h's entry points of the
  * same names, whose arguments have been checked. */
+/* x NULL: one axis. */
 void dpuf_hip_rope_append(void* s, const DpufAmdBatch* b, const DpufAmdPages* p, const DpufAmdRope* r,
-                          const int32_t* pos, int32_t in_type, int32_t nq, const void* q, const void* k, const void* v,
+                          const DpufAmdRopeAxes* x, const int32_t* pos, int64_t pos_stride, int32_t in_type, int32_t nq, const void* q, const void* k, const void* v,
                           int64_t qs, int64_t ks, int64_t vs, const float* qn, const float* kn, float eps,
                           void* q_out);
-size_t dpuf_hip_paged_attn_workspace(const DpufAmdBatch* b, const DpufAmdPages* p, int32_t nq);
+/* window 0: none (sink then says nothing). */
+size_t dpuf_hip_paged_attn_workspace(const DpufAmdBatch* b, const DpufAmdPages* p, int32_t nq, int32_t window,
+                                     int32_t sink);
 void dpuf_hip_paged_attn(void* s, const DpufAmdBatch* b, const DpufAmdPages* p, int32_t nq, const void* q, float scale,
-                         int32_t out_f32, void* out, float* lse, void* ws);
+                         int32_t window, int32_t sink, int32_t out_f32, void* out, float* lse, void* ws);
 void dpuf_hip_paged_attn_weights(void* s, const DpufAmdBatch* b, const DpufAmdPages* p, int32_t nq, const void* q,
                                  float scale, const float* lse, float decay, const float* w_in);
 void dpuf_hip_paged_evict(void* s, const DpufAmdBatch* b, const DpufAmdPages* p, int32_t keep, int32_t sink,
@@ -320,6 +323,10 @@ size_t dpuf_hip_sample_workspace(int32_t n, int32_t V);
 void dpuf_hip_sample(void* s, int32_t type, int32_t n, int32_t V, int64_t stride, const void* x, const float* temp,
                      const int32_t* top_k, const float* top_p, const float* min_p, const float* u, int32_t* tok,
                      float* logp, void* ws);
+size_t dpuf_hip_logprobs_workspace(int32_t n, int32_t V, int32_t n_top);
+void dpuf_hip_logprobs(void* s, int32_t type, int32_t n, int32_t V, int64_t stride, const void* x, int32_t n_targets,
+                       const int32_t* targets, int32_t n_top, float* logp, float* entropy, int32_t* top,
+                       float* top_logp, void* ws);
 
 #ifdef __cplusplus
 }

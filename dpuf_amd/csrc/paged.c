@@ -161,12 +161,25 @@ DPUF_EXPORT int32_t dpuf_amd_rope_turns(const DpufAmdRopeSpec* spec, double* tur
     return 0;
 }
 
-DPUF_EXPORT int32_t dpuf_amd_rope_append(const DpufAmdBatch* batch, const DpufAmdPages* pages,
-                                         const DpufAmdRope* rope, const int32_t* d_positions, int32_t in_type,
-                                         int32_t n_q_heads, const void* d_q, const void* d_k, const void* d_v,
-                                         int64_t q_stride, int64_t k_stride, int64_t v_stride,
-                                         const float* d_q_norm, const float* d_k_norm, float eps, void* d_q_out,
-                                         void* hip_stream) {
+/* Axis a > 0 takes pairs a, a + n, ... of `pairs` in turn, as many as it says. */
+static int32_t check_axes(const DpufAmdRopeAxes* x, int32_t pairs) {
+    if (!x) return -1;
+    if (x->n_axes < 1 || x->n_axes > 4) return -2;
+    int64_t sum = 0;
+    for (int32_t a = 0; a < x->n_axes; a++) {
+        if (x->sections[a] < 0 || x->sections[a] > pairs) return -2;
+        if (x->in_turn && a > 0 && x->sections[a] > 0 && a + x->n_axes * (x->sections[a] - 1) >= pairs) return -2;
+        sum += x->sections[a];
+    }
+    return sum == pairs ? 0 : -2;
+}
+
+/* axes NULL: one axis. */
+static int32_t rope_append(const DpufAmdBatch* batch, const DpufAmdPages* pages, const DpufAmdRope* rope,
+                           const DpufAmdRopeAxes* axes, const int32_t* d_positions, int64_t pos_stride,
+                           int32_t in_type, int32_t n_q_heads, const void* d_q, const void* d_k, const void* d_v,
+                           int64_t q_stride, int64_t k_stride, int64_t v_stride, const float* d_q_norm,
+                           const float* d_k_norm, float eps, void* d_q_out, void* hip_stream) {
     dpuf_hip_clear_error();
     int32_t rc = check_pages(pages);
     if (rc == 0) rc = check_batch(batch, pages);
@@ -175,6 +188,10 @@ DPUF_EXPORT int32_t dpuf_amd_rope_append(const DpufAmdBatch* batch, const DpufAm
     if (!rope || !aligned(rope->turns, 8)) return -1;
     const int64_t hd = pages->head_dim, nkv = pages->n_kv_heads, es = type_size(in_type);
     if (rope->rot_dim < 2 || (rope->rot_dim & 1) || rope->rot_dim > hd || !isfinite(rope->scale)) return -2;
+    const int32_t n_axes = axes ? axes->n_axes : 1;
+    rc = axes ? check_axes(axes, rope->rot_dim / 2) : 0;
+    if (rc != 0) return rc;
+    if (n_axes > 1 && pos_stride < batch->n_rows) return -4;
     if (n_q_heads < 0 || n_q_heads > 32 * nkv) return -2;
     if ((n_q_heads == 0) != (d_q == NULL) || (n_q_heads == 0) != (d_q_out == NULL)) return -1;
     if (batch->n_rows == 0) return 0;
@@ -187,7 +204,7 @@ DPUF_EXPORT int32_t dpuf_amd_rope_append(const DpufAmdBatch* batch, const DpufAm
         if (st[i] < need[i] || st[i] % 8 != 0) return -4;
     const int in_place = d_q && d_q_out == d_q && in_type == pages->type && q_stride == need[0];
     Span in[9] = {rows_of(d_k, batch->n_rows, k_stride, need[1], es), rows_of(d_v, batch->n_rows, v_stride, need[2], es),
-                  run(d_positions, batch->n_rows, 4), run(rope->turns, rope->rot_dim / 2, 8), run(d_q_norm, hd, 4),
+                  rows_of(d_positions, n_axes, n_axes > 1 ? pos_stride : 0, batch->n_rows, 4), run(rope->turns, rope->rot_dim / 2, 8), run(d_q_norm, hd, 4),
                   run(d_k_norm, hd, 4)};
     batch_spans(batch, in + 6);
     const Span q = rows_of(d_q, batch->n_rows, q_stride, need[0], es);
@@ -201,19 +218,55 @@ DPUF_EXPORT int32_t dpuf_amd_rope_append(const DpufAmdBatch* batch, const DpufAm
                         d_positions, d_q, d_k, d_v, d_q_norm, d_k_norm, d_q_out};
     const int32_t dev = device_of(ps, (int)(sizeof ps / sizeof ps[0]));
     if (dev < 0) return -1;
-    ON_DEVICE(dev, dpuf_hip_rope_append(hip_stream, batch, pages, rope, d_positions, in_type, n_q_heads, d_q, d_k, d_v,
-                                        q_stride, k_stride, v_stride, d_q_norm, d_k_norm, eps, d_q_out));
+    ON_DEVICE(dev, dpuf_hip_rope_append(hip_stream, batch, pages, rope, axes, d_positions, pos_stride, in_type,
+                                        n_q_heads, d_q, d_k, d_v, q_stride, k_stride, v_stride, d_q_norm, d_k_norm, eps,
+                                        d_q_out));
+}
+
+DPUF_EXPORT int32_t dpuf_amd_rope_append(const DpufAmdBatch* batch, const DpufAmdPages* pages,
+                                         const DpufAmdRope* rope, const int32_t* d_positions, int32_t in_type,
+                                         int32_t n_q_heads, const void* d_q, const void* d_k, const void* d_v,
+                                         int64_t q_stride, int64_t k_stride, int64_t v_stride,
+                                         const float* d_q_norm, const float* d_k_norm, float eps, void* d_q_out,
+                                         void* hip_stream) {
+    return rope_append(batch, pages, rope, NULL, d_positions, 0, in_type, n_q_heads, d_q, d_k, d_v, q_stride, k_stride,
+                       v_stride, d_q_norm, d_k_norm, eps, d_q_out, hip_stream);
+}
+
+DPUF_EXPORT int32_t dpuf_amd_rope_append_axes(const DpufAmdBatch* batch, const DpufAmdPages* pages,
+                                              const DpufAmdRope* rope, const DpufAmdRopeAxes* axes,
+                                              const int32_t* d_positions, int64_t pos_stride, int32_t in_type,
+                                              int32_t n_q_heads, const void* d_q, const void* d_k, const void* d_v,
+                                              int64_t q_stride, int64_t k_stride, int64_t v_stride,
+                                              const float* d_q_norm, const float* d_k_norm, float eps, void* d_q_out,
+                                              void* hip_stream) {
+    if (!axes) return -1;
+    return rope_append(batch, pages, rope, axes, d_positions, pos_stride, in_type, n_q_heads, d_q, d_k, d_v, q_stride,
+                       k_stride, v_stride, d_q_norm, d_k_norm, eps, d_q_out, hip_stream);
 }
 
 DPUF_EXPORT size_t dpuf_amd_paged_attn_workspace(const DpufAmdBatch* batch, const DpufAmdPages* pages,
                                                  int32_t n_q_heads) {
     if (check_pages(pages) != 0 || check_batch(batch, pages) != 0 || check_heads(pages, n_q_heads) != 0) return 0;
-    return dpuf_hip_paged_attn_workspace(batch, pages, n_q_heads);
+    return dpuf_hip_paged_attn_workspace(batch, pages, n_q_heads, 0, 0);
 }
 
-DPUF_EXPORT int32_t dpuf_amd_paged_attn(const DpufAmdBatch* batch, const DpufAmdPages* pages, int32_t n_q_heads,
-                                        const void* d_q, float scale, int32_t out_type, void* d_out, float* d_lse,
-                                        void* d_workspace, size_t workspace_bytes, void* hip_stream) {
+static int window_ok(int32_t window, int32_t sink) {
+    return window >= 1 && window <= 1 << 30 && sink >= 0 && sink <= 1 << 30;
+}
+
+DPUF_EXPORT size_t dpuf_amd_paged_attn_window_workspace(const DpufAmdBatch* batch, const DpufAmdPages* pages,
+                                                        int32_t n_q_heads, int32_t window, int32_t sink) {
+    if (check_pages(pages) != 0 || check_batch(batch, pages) != 0 || check_heads(pages, n_q_heads) != 0 ||
+        !window_ok(window, sink))
+        return 0;
+    return dpuf_hip_paged_attn_workspace(batch, pages, n_q_heads, window, sink);
+}
+
+/* window 0: none. */
+static int32_t paged_attn(const DpufAmdBatch* batch, const DpufAmdPages* pages, int32_t n_q_heads, const void* d_q,
+                          float scale, int32_t window, int32_t sink, int32_t out_type, void* d_out, float* d_lse,
+                          void* d_workspace, size_t workspace_bytes, void* hip_stream) {
     dpuf_hip_clear_error();
     int32_t rc = check_pages(pages);
     if (rc == 0) rc = check_batch(batch, pages);
@@ -223,7 +276,7 @@ DPUF_EXPORT int32_t dpuf_amd_paged_attn(const DpufAmdBatch* batch, const DpufAmd
     if (!(scale > 0.0f) || !isfinite(scale)) return -2;
     if (batch->n_rows == 0) return 0;
     if (!aligned(d_q, 16) || !aligned(d_out, 16) || (d_lse && !aligned(d_lse, 4))) return -1;
-    const size_t ws = dpuf_hip_paged_attn_workspace(batch, pages, n_q_heads);
+    const size_t ws = dpuf_hip_paged_attn_workspace(batch, pages, n_q_heads, window, sink);
     if (ws > 0 && !aligned(d_workspace, 16)) return -1;
     if (workspace_bytes < ws) return -7;
     const int64_t nr = (int64_t)batch->n_rows * n_q_heads, n = nr * pages->head_dim;
@@ -235,8 +288,24 @@ DPUF_EXPORT int32_t dpuf_amd_paged_attn(const DpufAmdBatch* batch, const DpufAmd
                         ws > 0 ? d_workspace : NULL};
     const int32_t dev = device_of(ps, (int)(sizeof ps / sizeof ps[0]));
     if (dev < 0) return -1;
-    ON_DEVICE(dev, dpuf_hip_paged_attn(hip_stream, batch, pages, n_q_heads, d_q, scale, out_type == DPUF_AMD_F32,
-                                       d_out, d_lse, ws > 0 ? d_workspace : NULL));
+    ON_DEVICE(dev, dpuf_hip_paged_attn(hip_stream, batch, pages, n_q_heads, d_q, scale, window, sink,
+                                       out_type == DPUF_AMD_F32, d_out, d_lse, ws > 0 ? d_workspace : NULL));
+}
+
+DPUF_EXPORT int32_t dpuf_amd_paged_attn(const DpufAmdBatch* batch, const DpufAmdPages* pages, int32_t n_q_heads,
+                                        const void* d_q, float scale, int32_t out_type, void* d_out, float* d_lse,
+                                        void* d_workspace, size_t workspace_bytes, void* hip_stream) {
+    return paged_attn(batch, pages, n_q_heads, d_q, scale, 0, 0, out_type, d_out, d_lse, d_workspace, workspace_bytes,
+                      hip_stream);
+}
+
+DPUF_EXPORT int32_t dpuf_amd_paged_attn_window(const DpufAmdBatch* batch, const DpufAmdPages* pages, int32_t n_q_heads,
+                                               const void* d_q, float scale, int32_t window, int32_t sink,
+                                               int32_t out_type, void* d_out, float* d_lse, void* d_workspace,
+                                               size_t workspace_bytes, void* hip_stream) {
+    if (!window_ok(window, sink)) return -2;
+    return paged_attn(batch, pages, n_q_heads, d_q, scale, window, sink, out_type, d_out, d_lse, d_workspace,
+                      workspace_bytes, hip_stream);
 }
 
 DPUF_EXPORT int32_t dpuf_amd_paged_attn_weights(const DpufAmdBatch* batch, const DpufAmdPages* pages,
@@ -334,4 +403,44 @@ DPUF_EXPORT int32_t dpuf_amd_sample(int32_t type, int32_t n, int32_t V, int64_t 
     if (dev < 0) return -1;
     ON_DEVICE(dev, dpuf_hip_sample(hip_stream, type, n, V, row_stride, d_logits, d_temperature, d_top_k, d_top_p,
                                    d_min_p, d_u, d_tokens, d_logprobs, d_workspace));
+}
+
+DPUF_EXPORT size_t dpuf_amd_logprobs_workspace(int32_t n, int32_t V, int32_t n_top) {
+    if (n < 1 || n > MAX_ROWS || V < 1 || V > DPUF_AMD_SAMPLE_MAX_VOCAB || n_top < 0 || n_top > DPUF_AMD_LOGPROBS_MAX_TOP)
+        return 0;
+    return dpuf_hip_logprobs_workspace(n, V, n_top);
+}
+
+DPUF_EXPORT int32_t dpuf_amd_logprobs(int32_t type, int32_t n, int32_t V, int64_t row_stride, const void* d_logits,
+                                      int32_t n_targets, const int32_t* d_targets, int32_t n_top, float* d_logprobs,
+                                      float* d_entropy, int32_t* d_top_tokens, float* d_top_logprobs,
+                                      void* d_workspace, size_t workspace_bytes, void* hip_stream) {
+    dpuf_hip_clear_error();
+    if (type != DPUF_AMD_F32 && type != DPUF_AMD_BF16 && type != DPUF_AMD_F16) return -5;
+    if (n < 1 || n > MAX_ROWS || V < 1 || V > DPUF_AMD_SAMPLE_MAX_VOCAB || n_targets < 0 ||
+        n_targets > DPUF_AMD_LOGPROBS_MAX_TARGETS || n_top < 0 || n_top > DPUF_AMD_LOGPROBS_MAX_TOP)
+        return -2;
+    if (row_stride < V) return -4;
+    if ((n_targets == 0) != (d_targets == NULL) || (n_targets == 0) != (d_logprobs == NULL) ||
+        (n_top == 0) != (d_top_tokens == NULL) || (n_top == 0) != (d_top_logprobs == NULL) ||
+        (n_targets == 0 && n_top == 0 && !d_entropy))
+        return -1;
+    if (!aligned(d_logits, (uintptr_t)type_size(type))) return -1;
+    const void* opt[] = {d_targets, d_logprobs, d_entropy, d_top_tokens, d_top_logprobs};
+    for (int i = 0; i < COUNT(opt); i++)
+        if (opt[i] && !aligned(opt[i], 4)) return -1;
+    const size_t ws = dpuf_hip_logprobs_workspace(n, V, n_top);
+    if (ws > 0 && !aligned(d_workspace, 16)) return -1;
+    if (workspace_bytes < ws) return -7;
+    const Span in[] = {rows_of(d_logits, n, row_stride, V, type_size(type)), run(d_targets, (int64_t)n * n_targets, 4)};
+    const Span out[] = {run(d_logprobs, (int64_t)n * n_targets, 4), run(d_entropy, n, 4),
+                        run(d_top_tokens, (int64_t)n * n_top, 4), run(d_top_logprobs, (int64_t)n * n_top, 4),
+                        run(d_workspace, (int64_t)ws, 1)};
+    if (any_overlap(out, COUNT(out), in, COUNT(in)) || overlap_within(out, COUNT(out))) return -1;
+    const void* ps[] = {d_logits, d_targets, d_logprobs, d_entropy, d_top_tokens, d_top_logprobs,
+                        ws > 0 ? d_workspace : NULL};
+    const int32_t dev = device_of(ps, COUNT(ps));
+    if (dev < 0) return -1;
+    ON_DEVICE(dev, dpuf_hip_logprobs(hip_stream, type, n, V, row_stride, d_logits, n_targets, d_targets, n_top,
+                                     d_logprobs, d_entropy, d_top_tokens, d_top_logprobs, ws > 0 ? d_workspace : NULL));
 }

@@ -28,6 +28,10 @@ struct Bf16 {
     typedef __bf16 v2 __attribute__((ext_vector_type(2)));
     static DEV f32x4 mma16(v8 a, v8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
     static DEV f32x16 mma32(v8 a, v8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
+    // c + both halves of w, in fp32 (denormals kept)
+    static DEV float add2(uint32_t w, float c) {
+        return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(v2, w), __builtin_bit_cast(v2, 0x3f803f80u), c, false);
+    }
 };
 struct Fp16 {
     static constexpr uint32_t EXP = 0x7c00;
@@ -40,6 +44,9 @@ struct Fp16 {
     typedef _Float16 v2 __attribute__((ext_vector_type(2)));
     static DEV f32x4 mma16(v8 a, v8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
     static DEV f32x16 mma32(v8 a, v8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
+    static DEV float add2(uint32_t w, float c) {
+        return __builtin_amdgcn_fdot2(__builtin_bit_cast(v2, w), __builtin_bit_cast(v2, 0x3c003c00u), c, false);
+    }
 };
 
 // Two floats rounded (to nearest even) into one 32-bit word of T.

@@ -36,9 +36,23 @@
 // below the maximum: p is at most 2^(9 + SLACK) = 2^15, and whole down to 2^-23
 // of the largest.  The maximum is then rounded up to an integer, which keeps
 // m + LIFT and the factors that l and o are moved by exact.
+//
+// With a window and sinks (W), a row at place p of its sequence sees the keys t
+// <= p with t > p - window or t < sink.  What a tile of rows sees is then two
+// runs of keys, the first few and those from its first row's window on.  Both
+// begin and end at whole tiles of keys here, so that the kernels walk them as
+// one run, in which a key behind the first ones is `gap` before its place; the
+// keys of those tiles that a row does not see are masked like those behind its
+// last.  A sequence's keys are split by that run's length, not by its context.
+//
+// A window may hold few keys, one of which has most of the weight, and then o is
+// nearly that key's v, but for the rounding of its p.  So where p is rounded once
+// the W kernels add up the rounded p too and multiply o by l over that sum: what
+// is left of the errors e_t of p_t is sum e_t (v_t - o), not sum e_t v_t.
 #include <hip/hip_runtime.h>
 #include <math.h>
 #include <stdint.h>
+#include <type_traits>
 
 #include "hip_internal.h"
 #include "paged.h"
@@ -61,6 +75,8 @@ struct PaArgs {
     int only;           // PA_BOTH, or the kernel that takes every sequence
     int nz_few, nz_many; // key ranges a sequence is split into at most
     int chunk_few, chunk_many;
+    int window, sink;    // of the W kernels
+    int reach_few, reach_many;  // keys that a tile of rows sees at most, whole tiles of them
     int out_f32;
     void* out;
     float* lse;
@@ -76,6 +92,28 @@ struct PaArgs {
 DEV int range_keys(int ctx, int chunk, int nz) {
     const int need = (ctx + nz - 1) / nz;
     return need <= chunk ? chunk : (need + 127) & ~127;
+}
+
+// The keys that a tile of rows walks: its rows' places begin at `first` and end
+// before kend; KT keys a step.
+template <bool W, int KT> struct Run {
+    int gap, head;       // keys [0, head) are where they are, those behind it `gap` later
+    DEV Run(const PaArgs& a, int first, int kend) {
+        gap = head = 0;
+        if constexpr (W) {
+            head = (min(a.sink, max(0, kend)) + KT - 1) & -KT;
+            gap = max(0, (max(0, first - a.window + 1) & -KT) - head);
+        }
+    }
+    DEV int key(int at) const { return W && at >= head ? at + gap : at; }
+};
+// Whether a row at place p sees all of the keys [t, t + n) as far as its window says.
+template <bool W> DEV bool in_window(const PaArgs& a, int t, int n, int p) {
+    return !W || t > p - a.window || t + n <= a.sink;
+}
+// Keys of a sequence as its ranges count them.
+template <bool W> DEV int span_of(const PaArgs& a, int ctx, bool few) {
+    return W ? min(ctx, few ? a.reach_few : a.reach_many) : ctx;
 }
 
 // Partial of a few-row sequence's packed row r (row: its place in the output).
@@ -168,7 +206,7 @@ template <int HD> struct FewLds {
     int odd[4];
 };
 
-template <typename T, int HD> DEV void few_rows(const PaArgs& a, FewLds<HD>& sh, int kvh, int y, int z) {
+template <typename T, int HD, bool W> DEV void few_rows(const PaArgs& a, FewLds<HD>& sh, int kvh, int y, int z) {
     constexpr int NC = HD / 32;          // 32-column steps of a key
     constexpr int ND = HD / 16;          // 16-column tiles of the output
     constexpr int PITCH = FewLds<HD>::PITCH;
@@ -179,15 +217,17 @@ template <typename T, int HD> DEV void few_rows(const PaArgs& a, FewLds<HD>& sh,
     const int tiles = (a.few + 15) >> 4;
     const int s = y / tiles;
     const int* table = a.b.page_table + (size_t)s * a.b.table_stride;
-    // the first range's first pages, beside the lengths
+    // the first range's first pages, beside the lengths (which say where a window begins)
     int early[2];
+    if (!W)
 #pragma unroll
     for (int u = 0; u < 2; u++) early[u] = table[min((32 * wave + 16 * u) >> a.shift, a.b.table_stride - 1)];
     const PgSeq sq = pg_seq(a.b, a.shift, s);
     const int rows = sq.n * a.G;
     if (rows > a.few && a.only == PA_BOTH) return;
-    const int per = range_keys(sq.ctx, a.chunk_few, a.nz_few);
-    const int ranges = sq.ctx > per ? (sq.ctx + per - 1) / per : 1;
+    const int span = span_of<W>(a, sq.ctx, true);
+    const int per = range_keys(span, a.chunk_few, a.nz_few);
+    const int ranges = span > per ? (span + per - 1) / per : 1;
     if (z >= ranges) return;
 
     // one tile of rows, unless a sequence has more than the others' few
@@ -199,7 +239,9 @@ template <typename T, int HD> DEV void few_rows(const PaArgs& a, FewLds<HD>& sh,
         const int limit = live ? sq.ctx - sq.n + qi : -1;             // last key this row sees
         const int last = min(rows, 16 * tile + 16) - 1;
         const int first_limit = sq.ctx - sq.n + 16 * tile / a.G;      // of the tile's first row
-        const int k0 = z * per, kend = min(min(sq.ctx - sq.n + last / a.G + 1, sq.ctx), k0 + per);
+        const int all = min(sq.ctx - sq.n + last / a.G + 1, sq.ctx);  // keys up to the last row's last
+        const Run<W, 32> run(a, first_limit, all);
+        const int k0 = z * per, kend = min(all - run.gap, k0 + per);
 
         v8 qf[NC];
 #pragma unroll
@@ -209,7 +251,8 @@ template <typename T, int HD> DEV void few_rows(const PaArgs& a, FewLds<HD>& sh,
         f32x4 o[ND];
 #pragma unroll
         for (int d = 0; d < ND; d++) o[d] = f32x4{0.f, 0.f, 0.f, 0.f};
-        float m = NEG_INF, l = 0.0f;
+        float m = NEG_INF, l = 0.0f, lp = 0.0f;      // lp: l of the rounded p, where that is kept
+        constexpr bool LP = W && !T::REST;
 
         const uint16_t* kp = (const uint16_t*)a.p.k + (size_t)kvh * a.p.head_stride + 8 * g4;
         const uint16_t* vp = (const uint16_t*)a.p.v + (size_t)kvh * a.p.head_stride + 8 * g4;
@@ -223,12 +266,12 @@ template <typename T, int HD> DEV void few_rows(const PaArgs& a, FewLds<HD>& sh,
         // page 0: both are masked below.
         auto pages = [&](int base, int* out) {
 #pragma unroll
-            for (int u = 0; u < 2; u++) out[u] = table[min((base + 16 * u) >> a.shift, top)];
+            for (int u = 0; u < 2; u++) out[u] = table[min((run.key(base) + 16 * u) >> a.shift, top)];
         };
         auto load = [&](int base, const int* pid) {
 #pragma unroll
             for (int u = 0; u < 2; u++) {
-                const int key = base + 16 * u + col;
+                const int key = run.key(base) + 16 * u + col;
                 const bool in = (unsigned)pid[u] < (unsigned)a.p.n_pages;
                 const size_t off = (size_t)(in ? pid[u] : 0) * a.p.page_stride +
                                    (size_t)(key & (a.p.page_size - 1)) * a.p.row_stride;
@@ -240,13 +283,13 @@ template <typename T, int HD> DEV void few_rows(const PaArgs& a, FewLds<HD>& sh,
         };
 
         auto whole_at = [&](int base, const int* pid) {
-            return base + 32 <= min(kend, first_limit + 1) && (unsigned)pid[0] < (unsigned)a.p.n_pages &&
-                   (unsigned)pid[1] < (unsigned)a.p.n_pages;
+            return base + 32 <= min(kend, first_limit + 1 - run.gap) && (unsigned)pid[0] < (unsigned)a.p.n_pages &&
+                   (unsigned)pid[1] < (unsigned)a.p.n_pages && in_window<W>(a, run.key(base), 32, all - 1);
         };
         uint32_t odd = 0;
         int base = k0 + 32 * wave;
         if (base < kend) {
-            if (z == 0) {
+            if (z == 0 && !W) {
                 pg[0] = early[0];
                 pg[1] = base + 16 < sq.ctx ? early[1] : early[0];
             } else {
@@ -277,7 +320,7 @@ template <typename T, int HD> DEV void few_rows(const PaArgs& a, FewLds<HD>& sh,
             for (int c = 0; c < NC; c++)
 #pragma unroll
                 for (int u = 0; u < 2; u++) sc[u] = T::mma16(vec_of<v8>(kf[u][c]), qf[c], sc[u]);
-            const int here = base;
+            const int here = run.key(base);
             const bool ok[2] = {(unsigned)pg[0] < (unsigned)a.p.n_pages, (unsigned)pg[1] < (unsigned)a.p.n_pages};
             if (base + 128 < kend) {
                 pg[0] = pn[0];
@@ -291,7 +334,9 @@ template <typename T, int HD> DEV void few_rows(const PaArgs& a, FewLds<HD>& sh,
                 for (int u = 0; u < 2; u++)
 #pragma unroll
                     for (int i = 0; i < 4; i++)
-                        if (!ok[u] || here + 16 * u + 4 * g4 + i > limit) sc[u][i] = NEG_INF;
+                        if (!ok[u] || here + 16 * u + 4 * g4 + i > limit ||
+                            !in_window<W>(a, here + 16 * u + 4 * g4 + i, 1, limit))
+                            sc[u][i] = NEG_INF;
             }
             float mt = fmaxf(fmaxf(fmaxf(sc[0][0], sc[0][1]), fmaxf(sc[0][2], sc[0][3])),
                              fmaxf(fmaxf(sc[1][0], sc[1][1]), fmaxf(sc[1][2], sc[1][3])));
@@ -300,6 +345,7 @@ template <typename T, int HD> DEV void few_rows(const PaArgs& a, FewLds<HD>& sh,
             if (__any(mt > m + (T::LIFT + SLACK))) {
                 const float mn = fmaxf(m, lowered<T>(mt)), f = __builtin_amdgcn_exp2f(m - (mn == NEG_INF ? 0.0f : mn));
                 l *= f;
+                if (LP) lp *= f;
 #pragma unroll
                 for (int d = 0; d < ND; d++) o[d] *= f;
                 m = mn;
@@ -315,6 +361,9 @@ template <typename T, int HD> DEV void few_rows(const PaArgs& a, FewLds<HD>& sh,
                 }
             v8 pf, rf;
             split8<T>(pr, pf, rf);
+            if (LP)
+#pragma unroll
+                for (int i = 0; i < 4; i++) lp = T::add2(__builtin_bit_cast(u32x4, pf)[i], lp);
             lds_order();
             const uint16_t* tr = lv + (4 * g4 + (col >> 2)) * PITCH + 4 * (col & 3);
 #pragma unroll
@@ -329,6 +378,7 @@ template <typename T, int HD> DEV void few_rows(const PaArgs& a, FewLds<HD>& sh,
 
         // join the four waves: m, l of the 16 rows, then O by output column
         l = add_xor32(add_xor16(l));
+        if (LP) lp = add_xor32(add_xor16(lp));
         if (lane < 16) sh.ml[wave][lane] = make_float2(m, l);
         const bool my_odd = __any(odd != 0);
         if (lane == 0) sh.odd[wave] = my_odd;
@@ -340,7 +390,7 @@ template <typename T, int HD> DEV void few_rows(const PaArgs& a, FewLds<HD>& sh,
         const float Ms = M == NEG_INF ? 0.0f : M;
 #pragma unroll
         for (int w = 0; w < 4; w++) L += sh.ml[w][col].y * __builtin_amdgcn_exp2f(sh.ml[w][col].x - Ms);
-        const float f = __builtin_amdgcn_exp2f(m - Ms);
+        const float f = __builtin_amdgcn_exp2f(m - Ms) * (LP && lp > 0.0f ? l / lp : 1.0f);
         // [wave][16 rows][HD + 4] floats over the V tiles, a half of the columns
         // at a time (16 * (HD / 2 + 4) floats fit a wave's 32 * (HD + 16) halves)
         constexpr int OP = HD / 2 + 4;
@@ -367,7 +417,9 @@ template <typename T, int HD> DEV void few_rows(const PaArgs& a, FewLds<HD>& sh,
                             int pid[2];
                             pages(t0, pid);
                             if (whole_at(t0, pid)) continue;
-                            for (int t = t0; t < t0 + 32 && t <= sq.ctx - sq.n + i; t++) {
+                            const int t1 = run.key(t0), place = sq.ctx - sq.n + i;
+                            for (int t = t1; t < t1 + 32 && t <= place; t++) {
+                                if (!in_window<W>(a, t, 1, place)) continue;
                                 const int p = pid[(t >> 4) & 1];
                                 if ((unsigned)p < (unsigned)a.p.n_pages)
                                     v += odd4<T>((const uint16_t*)a.p.v + (size_t)kvh * a.p.head_stride +
@@ -422,7 +474,7 @@ template <int HD> struct ManyLds {
     int odd;
 };
 
-template <typename T, int HD, int WAVES>
+template <typename T, int HD, int WAVES, bool W>
 DEV void many_rows(const PaArgs& a, ManyLds<HD>& sh, int kvh, int tile, int z) {
     constexpr int KT = ManyLds<HD>::KT, KP = ManyLds<HD>::KP, VP = ManyLds<HD>::VP;
     constexpr int NC = HD / 16;          // 16-column steps of a key
@@ -466,8 +518,9 @@ DEV void many_rows(const PaArgs& a, ManyLds<HD>& sh, int kvh, int tile, int z) {
     if (s < 0) return;
     const PgSeq sq = pg_seq(a.b, a.shift, s);
     const int rows = sq.n * a.G;
-    const int per = range_keys(sq.ctx, a.chunk_many, a.nz_many);
-    const int ranges = sq.ctx > per ? (sq.ctx + per - 1) / per : 1;
+    const int span = span_of<W>(a, sq.ctx, false);
+    const int per = range_keys(span, a.chunk_many, a.nz_many);
+    const int ranges = span > per ? (span + per - 1) / per : 1;
     if (z >= ranges) return;
 
     const int r = TR * tile + 32 * wave + col;
@@ -479,9 +532,11 @@ DEV void many_rows(const PaArgs& a, ManyLds<HD>& sh, int kvh, int tile, int z) {
     // workgroup's by all
     const int wl = min(rows, TR * tile + 32 * wave + 32) - 1, gl = min(rows, TR * tile + TR) - 1;
     const int first_limit = sq.ctx - sq.n + (TR * tile + 32 * wave) / a.G;
+    const int all = min(sq.ctx - sq.n + gl / a.G + 1, sq.ctx), w_last = sq.ctx - sq.n + wl / a.G;
+    const Run<W, KT> run(a, sq.ctx - sq.n + TR * tile / a.G, all);
     const int k0 = z * per;
-    const int wend = TR * tile + 32 * wave < rows ? min(sq.ctx - sq.n + wl / a.G + 1, k0 + per) : 0;
-    const int kend = min(min(sq.ctx - sq.n + gl / a.G + 1, sq.ctx), k0 + per);
+    const int wend = TR * tile + 32 * wave < rows ? min(w_last + 1 - run.gap, k0 + per) : 0;
+    const int kend = min(all - run.gap, k0 + per);
 
     v8 qf[NC];
 #pragma unroll
@@ -492,7 +547,7 @@ DEV void many_rows(const PaArgs& a, ManyLds<HD>& sh, int kvh, int tile, int z) {
     for (int d = 0; d < ND; d++)
 #pragma unroll
         for (int i = 0; i < 16; i++) o[d][i] = 0.0f;
-    float m = NEG_INF, l = 0.0f;
+    float m = NEG_INF, l = 0.0f, lp = 0.0f;
 
     // A tile's pages, one for each 16 keys (pages hold a multiple of 16 rows),
     // are the same for all lanes: a thread's address is its own offset within
@@ -508,13 +563,16 @@ DEV void many_rows(const PaArgs& a, ManyLds<HD>& sh, int kvh, int tile, int z) {
     u32x4 kf[NP], vf[NP];
     int pn[NG];              // pages of the tile to be loaded next
     uint32_t odd = 0;
-    const int seen = min(kend, sq.ctx - sq.n + TR * tile / a.G + 1);     // keys before it: by all rows
+    // keys before it (with a window, of those that all have in theirs): by all rows
+    const int seen = min(kend, sq.ctx - sq.n + TR * tile / a.G + 1 - run.gap);
+    auto by_all = [&](int base) { return base + KT <= seen && in_window<W>(a, run.key(base), KT, all - 1); };
     uint32_t bad1 = 0, bad2 = 0;   // of the tile in kf / vf (one bit per 16 keys: outside the pool), and of the next
     auto pages = [&](int base) {
 #pragma unroll
-        for (int g = 0; g < NG; g++) pn[g] = table[min((base + 16 * g) >> a.shift, top)];
+        for (int g = 0; g < NG; g++) pn[g] = table[min((run.key(base) + 16 * g) >> a.shift, top)];
     };
     auto load = [&](int base) {
+        const int key = run.key(base);
         bad2 = 0;
 #pragma unroll
         for (int g = 0; g < NG; g++) bad2 |= ((unsigned)pn[g] >= (unsigned)a.p.n_pages) << g;
@@ -526,12 +584,12 @@ DEV void many_rows(const PaArgs& a, ManyLds<HD>& sh, int kvh, int tile, int z) {
             for (int e = 1; e < RP / 16; e++) pg = wr == e ? pn[(u * RP / 16 + e) % NG] : pg;
             if ((bad2 >> g) & 1) pg = 0;
             const size_t at = (size_t)pg * a.p.page_stride +
-                              (size_t)((base + 16 * g) & (a.p.page_size - 1)) * a.p.row_stride +
+                              (size_t)((key + 16 * g) & (a.p.page_size - 1)) * a.p.row_stride +
                               (RP == 8 ? (size_t)(u & 1) * 8 * a.p.row_stride : 0);
             kf[u] = *(const u32x4*)(kp + at + lo);
             vf[u] = *(const u32x4*)(vp + at + lo);
         }
-        if (bad2 || base + KT > seen)
+        if (bad2 || !by_all(base))
 #pragma unroll
             for (int u = 0; u < NP; u++) odd |= take_odd<T>(vf[u]);
     };
@@ -566,6 +624,9 @@ DEV void many_rows(const PaArgs& a, ManyLds<HD>& sh, int kvh, int tile, int z) {
             pages(base + 3 * KT);
         }
         if (base >= wend) continue;
+        const int here = run.key(base);
+        // nothing that the wave's rows see
+        if (W && here >= a.sink && here + KT <= first_limit - a.window + 1) continue;
         const f32x16 zero = {};
         f32x16 sc[NB];
 #pragma unroll
@@ -576,13 +637,14 @@ DEV void many_rows(const PaArgs& a, ManyLds<HD>& sh, int kvh, int tile, int z) {
                 sc[b] = T::mma32(kv, qf[c], c ? sc[b] : zero);
             }
         // sc[b][i]: key 32 b + 8 (i / 4) + 4 h + i % 4
-        if (base + KT > min(wend, first_limit + 1) || bad) {
+        if (base + KT > min(wend, first_limit + 1 - run.gap) || bad || !in_window<W>(a, here, KT, w_last)) {
 #pragma unroll
             for (int b = 0; b < NB; b++)
 #pragma unroll
                 for (int i = 0; i < 16; i++) {
                     const int key = 32 * b + 8 * (i >> 2) + 4 * h + (i & 3);
-                    if (base + key > limit || ((bad >> (key >> 4)) & 1)) sc[b][i] = NEG_INF;
+                    if (here + key > limit || ((bad >> (key >> 4)) & 1) || !in_window<W>(a, here + key, 1, limit))
+                        sc[b][i] = NEG_INF;
                 }
         }
         float mt = NEG_INF;
@@ -595,6 +657,7 @@ DEV void many_rows(const PaArgs& a, ManyLds<HD>& sh, int kvh, int tile, int z) {
         if (__any(mt > m + (T::LIFT + SLACK))) {
             const float mn = fmaxf(m, lowered<T>(mt)), f = __builtin_amdgcn_exp2f(m - (mn == NEG_INF ? 0.0f : mn));
             l *= f;
+            if (W) lp *= f;
 #pragma unroll
             for (int d = 0; d < ND; d++) o[d] *= f;
             m = mn;
@@ -612,6 +675,9 @@ DEV void many_rows(const PaArgs& a, ManyLds<HD>& sh, int kvh, int tile, int z) {
                 }
                 const u32x4 pw = {pack2<T>(pr[0], pr[1]), pack2<T>(pr[2], pr[3]), pack2<T>(pr[4], pr[5]),
                                   pack2<T>(pr[6], pr[7])};
+                if (W)
+#pragma unroll
+                    for (int i = 0; i < 4; i++) lp = T::add2(pw[i], lp);
                 const v8 pf = vec_of<v8>(pw);
                 // keys 4 h .. + 3 and 8 + 4 h .. + 3 of the 16, columns 16 * (lane / 16 % 2) + lane % 16
                 const uint16_t* tr = lv[buf] + (32 * b + 16 * k + 4 * h + ((lane & 15) >> 2)) * VP +
@@ -624,19 +690,27 @@ DEV void many_rows(const PaArgs& a, ManyLds<HD>& sh, int kvh, int tile, int z) {
                 }
             }
     }
+    l = add_xor32(l);
+    if (W) {
+        lp = add_xor32(lp);
+        const float f = lp > 0.0f ? l / lp : 1.0f;
+#pragma unroll
+        for (int d = 0; d < ND; d++) o[d] *= f;
+    }
     __syncthreads();
     if (__any(odd != 0) && lane == 0) sh.odd = 1;
     __syncthreads();
     if (sh.odd)
         for (int base = k0; base < kend; base += 16) {
-            const int pg = table[min(base >> a.shift, top)], t0 = base & ~(KT - 1);
+            const int here = run.key(base);
+            const int pg = table[min(here >> a.shift, top)], t0 = base & ~(KT - 1);
             if ((unsigned)pg >= (unsigned)a.p.n_pages) continue;
-            bool whole = t0 + KT <= seen;
+            bool whole = by_all(t0);
             for (int g = 0; g < NG; g++)
-                whole = whole && (unsigned)table[min((t0 + 16 * g) >> a.shift, top)] < (unsigned)a.p.n_pages;
+                whole = whole && (unsigned)table[min((run.key(t0) + 16 * g) >> a.shift, top)] < (unsigned)a.p.n_pages;
             if (whole) continue;
 #pragma unroll 1
-            for (int key = base; key < base + 16; key++) {
+            for (int key = here; key < here + 16; key++) {
                 const uint16_t* v = vp + (size_t)pg * a.p.page_stride +
                                     (size_t)(key & (a.p.page_size - 1)) * a.p.row_stride + 4 * h;
 #pragma unroll
@@ -645,11 +719,10 @@ DEV void many_rows(const PaArgs& a, ManyLds<HD>& sh, int kvh, int tile, int z) {
                     for (int i = 0; i < 16; i += 4) {
                         const f32x4 x = odd4<T>(v + 32 * d + 2 * i);
 #pragma unroll
-                        for (int e = 0; e < 4; e++) o[d][i + e] += key <= limit ? x[e] : 0.0f;
+                        for (int e = 0; e < 4; e++) o[d][i + e] += key <= limit && in_window<W>(a, key, 1, limit) ? x[e] : 0.0f;
                     }
             }
         }
-    l = add_xor32(l);
     if (!live) return;
     // o[d][i]: column 32 d + 8 (i / 4) + 4 h + i % 4
     if (ranges > 1) {
@@ -676,21 +749,21 @@ DEV void many_rows(const PaArgs& a, ManyLds<HD>& sh, int kvh, int tile, int z) {
 // Blocks of the three kernels: kv heads fastest, so that the workgroups that
 // read the same keys run on the same XCDs (8 kv heads: one XCD each) and share
 // their L2.
-template <typename T, int HD> __global__ __launch_bounds__(256, HD == 256 ? 1 : 3) void k_pa_few(PaArgs a) {
+template <typename T, int HD, bool W> __global__ __launch_bounds__(256, HD == 256 ? 1 : 3) void k_pa_few(PaArgs a) {
     __shared__ __align__(16) FewLds<HD> sh;
-    few_rows<T, HD>(a, sh, blockIdx.x, blockIdx.y, blockIdx.z);
+    few_rows<T, HD, W>(a, sh, blockIdx.x, blockIdx.y, blockIdx.z);
 }
-template <typename T, int HD> __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void k_pa_many(PaArgs a) {
+template <typename T, int HD, bool W> __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void k_pa_many(PaArgs a) {
     __shared__ __align__(16) ManyLds<HD> sh;
-    many_rows<T, HD, 4>(a, sh, blockIdx.x, blockIdx.y, blockIdx.z);
+    many_rows<T, HD, 4, W>(a, sh, blockIdx.x, blockIdx.y, blockIdx.z);
 }
-template <typename T, int HD> __global__ __launch_bounds__(512, 2) void k_pa_wide(PaArgs a) {
+template <typename T, int HD, bool W> __global__ __launch_bounds__(512, 2) void k_pa_wide(PaArgs a) {
     __shared__ __align__(16) ManyLds<HD> sh;
-    many_rows<T, HD, 8>(a, sh, blockIdx.x, blockIdx.y, blockIdx.z);
+    many_rows<T, HD, 8, W>(a, sh, blockIdx.x, blockIdx.y, blockIdx.z);
 }
 // Chunks and decoding sequences in one call: the chunks' workgroups, which are
 // bound by arithmetic, first, and beside them those that are bound by memory.
-template <typename T, int HD>
+template <typename T, int HD, bool W>
 __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void k_pa_mixed(PaArgs a, int y_many, int y_few) {
     __shared__ __align__(16) char raw[sizeof(ManyLds<HD>) > sizeof(FewLds<HD>) ? sizeof(ManyLds<HD>)
                                                                                : sizeof(FewLds<HD>)];
@@ -699,19 +772,19 @@ __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void k_pa_mixed(PaArgs a, i
     if (b < many) {
         const int kvh = b % nkv;
         b /= nkv;
-        many_rows<T, HD, 4>(a, *(ManyLds<HD>*)raw, kvh, b % y_many, b / y_many);
+        many_rows<T, HD, 4, W>(a, *(ManyLds<HD>*)raw, kvh, b % y_many, b / y_many);
     } else {
         b -= many;
         const int kvh = b % nkv;
         b /= nkv;
-        few_rows<T, HD>(a, *(FewLds<HD>*)raw, kvh, b % y_few, b / y_few);
+        few_rows<T, HD, W>(a, *(FewLds<HD>*)raw, kvh, b % y_few, b / y_few);
     }
 }
 
 // Joins the key ranges of rows that were split: HD / 4 lanes a (row, head) and
 // ZG groups of them, each with every ZG-th range, four of a group's in flight,
 // their sums joined in LDS: 512 rows of 32 heads in four ranges 7.6 us, 4.7 TB/s.
-template <typename T, int HD, int ZG>
+template <typename T, int HD, int ZG, bool W>
 __global__ __launch_bounds__(256) void k_pa_join(PaArgs a) {
     constexpr int LPR = HD / 4, PER = 256 / LPR / ZG;
     __shared__ float2 sml[ZG][PER];
@@ -722,8 +795,9 @@ __global__ __launch_bounds__(256) void k_pa_join(PaArgs a) {
     if (s < 0) return;
     const PgSeq sq = pg_seq(a.b, a.shift, s);
     const bool few = a.only == PA_FEW || (a.only == PA_BOTH && sq.n * a.G <= a.few);
-    const int per = range_keys(sq.ctx, few ? a.chunk_few : a.chunk_many, few ? a.nz_few : a.nz_many);
-    const int ranges = sq.ctx > per ? (sq.ctx + per - 1) / per : 1;
+    const int span = span_of<W>(a, sq.ctx, few);
+    const int per = range_keys(span, few ? a.chunk_few : a.chunk_many, few ? a.nz_few : a.nz_many);
+    const int ranges = span > per ? (span + per - 1) / per : 1;
     if (ranges == 1 || row >= sq.r0 + sq.n) return;
     const bool live = head < a.nq;
     const int hd = live ? head : a.nq - 1, kvh = hd / a.G;
@@ -771,6 +845,7 @@ __global__ __launch_bounds__(256) void k_pa_join(PaArgs a) {
 }
 
 struct PaPlan {
+    int window, sink, reach_few, reach_many;
     int only, few, nz_few, nz_many, chunk_few, chunk_many, y_few, y_many;
     size_t few_rows, many_rows;   // partial sums in the workspace
 };
@@ -804,12 +879,23 @@ int range_of(int64_t ctx, double times) { return ((int)(times * sqrt((double)ctx
 // them from up to 64 (sequence, kv head): one row over 300 keys 10.2 in one,
 // 9.3 in three, over 512 11.7 and 9.2; 8 rows 10.4 and 9.6, 12.5 and 10.8; but
 // 12 rows 11.0 and 12.5, 12.7 and 12.9, 16 rows 11.6 and 12.1, 12.8 and 14.0.
-PaPlan plan(const DpufAmdBatch& b, const DpufAmdPages& p, int nq) {
+//
+// With a window the same, by the keys that a tile of rows sees: the first ones,
+// the window and as many more as the tile's rows are apart, in whole tiles of
+// keys.  (A window of 0 here is none.)
+PaPlan plan(const DpufAmdBatch& b, const DpufAmdPages& p, int nq, int window, int sink) {
     const int G = nq / p.n_kv_heads;
     PaPlan r;
     r.few = G > 16 ? 32 : 16;
     const int64_t cap = (int64_t)b.table_stride * p.page_size;
-    const int64_t ctx = b.max_ctx < 1 ? 1 : b.max_ctx < cap ? b.max_ctx : cap;
+    int64_t ctx = b.max_ctx < 1 ? 1 : b.max_ctx < cap ? b.max_ctx : cap;
+    // what reaches every key of the table needs no more than that
+    r.window = window < cap && sink < cap ? window : (int)cap;
+    r.sink = r.window < cap ? sink : 0;
+    const int64_t near = (int64_t)r.window + (r.sink + 63) / 64 * 64 + 64;
+    r.reach_few = (int)(near + 16 / G + 1 < cap ? near + 16 / G + 1 : cap);
+    r.reach_many = (int)(near + 256 / G + 1 < cap ? near + 256 / G + 1 : cap);
+    if (window && ctx > r.reach_few) ctx = r.reach_few;
     const int64_t packed = (int64_t)b.n_rows * G;
     r.only = b.n_rows <= b.n_seqs || packed <= r.few ? PA_FEW : b.n_seqs > 1 ? PA_BOTH
              : packed >= 384 && ctx >= 2048 && p.head_dim <= 128 ? PA_WIDE : PA_MANY;
@@ -853,18 +939,18 @@ PaPlan plan(const DpufAmdBatch& b, const DpufAmdPages& p, int nq) {
     return r;
 }
 
-template <typename T, int HD>
+template <typename T, int HD, bool W>
 void launch(const PaArgs& a, const PaPlan& pl, hipStream_t st) {
     const int nkv = a.p.n_kv_heads;
     if (pl.only == PA_FEW)
-        hipLaunchKernelGGL((k_pa_few<T, HD>), dim3(nkv, pl.y_few, pl.nz_few), dim3(256), 0, st, a);
+        hipLaunchKernelGGL((k_pa_few<T, HD, W>), dim3(nkv, pl.y_few, pl.nz_few), dim3(256), 0, st, a);
     else if (pl.only == PA_MANY)
-        hipLaunchKernelGGL((k_pa_many<T, HD>), dim3(nkv, pl.y_many, pl.nz_many), dim3(256), 0, st, a);
+        hipLaunchKernelGGL((k_pa_many<T, HD, W>), dim3(nkv, pl.y_many, pl.nz_many), dim3(256), 0, st, a);
     else if (pl.only == PA_WIDE) {
         if constexpr (HD <= 128)
-            hipLaunchKernelGGL((k_pa_wide<T, HD>), dim3(nkv, pl.y_many, pl.nz_many), dim3(512), 0, st, a);
+            hipLaunchKernelGGL((k_pa_wide<T, HD, W>), dim3(nkv, pl.y_many, pl.nz_many), dim3(512), 0, st, a);
     } else
-        hipLaunchKernelGGL((k_pa_mixed<T, HD>), dim3(nkv * (pl.y_many * pl.nz_many + pl.y_few * pl.nz_few)), dim3(256),
+        hipLaunchKernelGGL((k_pa_mixed<T, HD, W>), dim3(nkv * (pl.y_many * pl.nz_many + pl.y_few * pl.nz_few)), dim3(256),
                            0, st, a, pl.y_many, pl.y_few);
     if (pl.few_rows + pl.many_rows > 0) {
         constexpr int ZG = HD == 256 ? 4 : 8;
@@ -873,10 +959,10 @@ void launch(const PaArgs& a, const PaPlan& pl, hipStream_t st) {
         // keys in 64 ranges 52 us, 58 by one group), many are bound by bytes
         // (a mixed batch of 269 rows of 32 heads, 7 ranges: 60.8 and 53)
         if (nz > 4 && (int64_t)a.b.n_rows * a.nq <= 4096)
-            hipLaunchKernelGGL((k_pa_join<T, HD, ZG>), dim3(a.b.n_rows, ceil_div(a.nq, 256 / (HD / 4) / ZG)), dim3(256),
+            hipLaunchKernelGGL((k_pa_join<T, HD, ZG, W>), dim3(a.b.n_rows, ceil_div(a.nq, 256 / (HD / 4) / ZG)), dim3(256),
                                0, st, a);
         else
-            hipLaunchKernelGGL((k_pa_join<T, HD, 1>), dim3(a.b.n_rows, ceil_div(a.nq, 256 / (HD / 4))), dim3(256), 0, st,
+            hipLaunchKernelGGL((k_pa_join<T, HD, 1, W>), dim3(a.b.n_rows, ceil_div(a.nq, 256 / (HD / 4))), dim3(256), 0, st,
                                a);
     }
     LAUNCHED("k_pa");
@@ -886,14 +972,15 @@ void launch(const PaArgs& a, const PaPlan& pl, hipStream_t st) {
 
 extern "C" {
 
-size_t dpuf_hip_paged_attn_workspace(const DpufAmdBatch* b, const DpufAmdPages* p, int32_t nq) {
-    const PaPlan pl = plan(*b, *p, nq);
+size_t dpuf_hip_paged_attn_workspace(const DpufAmdBatch* b, const DpufAmdPages* p, int32_t nq, int32_t window,
+                                     int32_t sink) {
+    const PaPlan pl = plan(*b, *p, nq, window, sink);
     return (pl.few_rows + pl.many_rows) * ((size_t)p->head_dim * 4 + 8);
 }
 
 void dpuf_hip_paged_attn(void* s, const DpufAmdBatch* b, const DpufAmdPages* p, int32_t nq, const void* q, float scale,
-                         int32_t out_f32, void* out, float* lse, void* ws) {
-    const PaPlan pl = plan(*b, *p, nq);
+                         int32_t window, int32_t sink, int32_t out_f32, void* out, float* lse, void* ws) {
+    const PaPlan pl = plan(*b, *p, nq, window, sink);
     PaArgs a;
     a.b = *b;
     a.p = *p;
@@ -908,6 +995,10 @@ void dpuf_hip_paged_attn(void* s, const DpufAmdBatch* b, const DpufAmdPages* p, 
     a.nz_many = pl.nz_many;
     a.chunk_few = pl.chunk_few;
     a.chunk_many = pl.chunk_many;
+    a.window = pl.window;
+    a.sink = pl.sink;
+    a.reach_few = pl.reach_few;
+    a.reach_many = pl.reach_many;
     a.out_f32 = out_f32;
     a.out = out;
     a.lse = lse;
@@ -915,12 +1006,18 @@ void dpuf_hip_paged_attn(void* s, const DpufAmdBatch* b, const DpufAmdPages* p, 
     a.many_o = a.few_o + pl.few_rows * p->head_dim;
     a.few_ml = (float2*)(a.many_o + pl.many_rows * p->head_dim);
     a.many_ml = a.few_ml + pl.few_rows;
+    auto go = [&](auto type, auto windowed) {
+        typedef decltype(type) T;
+        constexpr bool W = decltype(windowed)::value;
+        switch (p->head_dim) {
+            case 64: launch<T, 64, W>(a, pl, ST(s)); break;
+            case 128: launch<T, 128, W>(a, pl, ST(s)); break;
+            default: launch<T, 256, W>(a, pl, ST(s)); break;
+        }
+    };
     const bool bf = p->type == DPUF_AMD_BF16;
-    switch (p->head_dim) {
-        case 64: bf ? launch<Bf16, 64>(a, pl, ST(s)) : launch<Fp16, 64>(a, pl, ST(s)); break;
-        case 128: bf ? launch<Bf16, 128>(a, pl, ST(s)) : launch<Fp16, 128>(a, pl, ST(s)); break;
-        default: bf ? launch<Bf16, 256>(a, pl, ST(s)) : launch<Fp16, 256>(a, pl, ST(s)); break;
-    }
+    if (window) bf ? go(Bf16(), std::true_type()) : go(Fp16(), std::true_type());
+    else bf ? go(Bf16(), std::false_type()) : go(Fp16(), std::false_type());
 }
 
 }  // extern "C"

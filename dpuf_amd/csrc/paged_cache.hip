@@ -33,25 +33,65 @@ struct RaArgs {
     uint16_t* q_out;
 };
 
-template <bool F32, typename T> DEV void load8(const void* base, int64_t at, float* x) {
-    if (F32) {
-        const float4 a = *(const float4*)((const float*)base + at), b = *(const float4*)((const float*)base + at + 4);
-        x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w;
-        x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
-    } else {
-        const typename T::v8 a = vec_of<typename T::v8>(*(const u32x4*)((const uint16_t*)base + at));
-#pragma unroll
-        for (int i = 0; i < 8; i++) x[i] = (float)a[i];
-    }
+// Position axes: pair j's axis, by the sections' ends or in turn.
+struct AxArgs {
+    int n, in_turn;
+    int end[3];         // pairs of the axes up to this one; in turn: past the axis's last pair (of axes 1 to 3)
+    uint32_t inv;       // 2^16 / n, rounded up: j / n of j below 256
+    int64_t stride;
+};
+DEV int axis_of(const AxArgs& x, int j) {
+    if (!x.in_turn) return (j >= x.end[0]) + (j >= x.end[1]) + (j >= x.end[2]);
+    const int a = j - (int)((uint32_t)j * x.inv >> 16) * x.n;
+    return a > 0 && j < (a == 1 ? x.end[0] : a == 2 ? x.end[1] : x.end[2]) ? a : 0;
 }
 
-template <typename TI, bool F32, typename T, int HD>
-__global__ __launch_bounds__(256) void k_rope_append(RaArgs a) {
+template <bool F32, typename T> struct Raw8 {
+    u32x4 w[F32 ? 2 : 1];
+    DEV void load(const void* base, int64_t at) {
+        const u32x4* p = (const u32x4*)((const char*)base + at * (F32 ? 4 : 2));
+        w[0] = p[0];
+        if (F32) w[F32 ? 1 : 0] = p[1];
+    }
+    DEV void get(float* x) const {
+        if constexpr (F32) {
+#pragma unroll
+            for (int i = 0; i < 8; i++) x[i] = __uint_as_float(w[i >> 2][i & 3]);
+        } else {
+            const typename T::v8 a = vec_of<typename T::v8>(w[0]);
+#pragma unroll
+            for (int i = 0; i < 8; i++) x[i] = (float)a[i];
+        }
+    }
+};
+
+template <typename TI, bool F32, typename T, int HD, bool AX> DEV void rope_row(const RaArgs& a, const AxArgs& ax) {
     constexpr int LH = HD / 8;                 // lanes of a head
     constexpr int GROUPS = 256 / LH;
     __shared__ float xs[256 * 8];
     const int lane = threadIdx.x & 63;
     const int row = blockIdx.x;
+    const int sub = threadIdx.x % LH, grp = threadIdx.x / LH;
+    const int c0 = 8 * sub, half = a.rot >> 1;
+    const int nkv = a.p.n_kv_heads, heads = a.nq + 2 * nkv;
+    // the first heads' columns, whose place is known, before the row's
+    // sequence is looked for; later ones a turn ahead
+    auto fetch = [&](int h0) {
+        Raw8<F32, TI> r = {};
+        const int hh = h0 + grp;
+        if (hh < a.nq) r.load(a.q, row * a.qs + (int64_t)hh * HD + c0);
+        else if (hh < a.nq + nkv) r.load(a.k, row * a.ks + (int64_t)(hh - a.nq) * HD + c0);
+        else if (hh < heads) r.load(a.v, row * a.vs + (int64_t)(hh - a.nq - nkv) * HD + c0);
+        return r;
+    };
+    Raw8<F32, TI> next = fetch(GROUPS * blockIdx.y);
+    const double pos = (double)a.pos[row];
+    double pos1 = 0.0, pos2 = 0.0, pos3 = 0.0;
+    if constexpr (AX) {
+        pos1 = ax.n > 1 ? (double)a.pos[row + ax.stride] : 0.0;
+        pos2 = ax.n > 2 ? (double)a.pos[row + 2 * ax.stride] : 0.0;
+        pos3 = ax.n > 3 ? (double)a.pos[row + 3 * ax.stride] : 0.0;
+    }
     const int s = pg_seq_of_row(a.b, row, lane);
     if (s < 0) return;
     const PgSeq sq = pg_seq(a.b, a.shift, s);
@@ -62,9 +102,6 @@ __global__ __launch_bounds__(256) void k_rope_append(RaArgs a) {
     const bool put = (unsigned)page < (unsigned)a.p.n_pages;
     const int in_page = slot & (a.p.page_size - 1);
 
-    const int sub = threadIdx.x % LH, grp = threadIdx.x / LH;
-    const int c0 = 8 * sub, half = a.rot >> 1;
-    const double pos = (double)a.pos[row];
     float cs[8], sn[8];
 #pragma unroll
     for (int e = 0; e < 8; e++) {
@@ -72,7 +109,13 @@ __global__ __launch_bounds__(256) void k_rope_append(RaArgs a) {
         cs[e] = 1.0f;
         sn[e] = 0.0f;
         if (c < a.rot) {
-            const double t = pos * a.turns[a.inter ? c >> 1 : (c < half ? c : c - half)];
+            const int j = a.inter ? c >> 1 : (c < half ? c : c - half);
+            double at = pos;
+            if constexpr (AX) {
+                const int axis = axis_of(ax, j);
+                at = axis == 0 ? pos : axis == 1 ? pos1 : axis == 2 ? pos2 : pos3;
+            }
+            const double t = at * a.turns[j];
             const float f = (float)(t - rint(t));
             float si, co;
             sincospif(2.0f * f, &si, &co);
@@ -81,18 +124,14 @@ __global__ __launch_bounds__(256) void k_rope_append(RaArgs a) {
             sn[e] = (second ? si : -si) * a.mscale;
         }
     }
-    const int nkv = a.p.n_kv_heads, heads = a.nq + 2 * nkv;
     for (int h0 = GROUPS * blockIdx.y; h0 < heads; h0 += GROUPS * gridDim.y) {
         const int hh = h0 + grp;
         const bool on = hh < heads;
         const int kind = hh < a.nq ? 0 : hh < a.nq + nkv ? 1 : 2;    // q, k, v
         const int kh = kind == 0 ? 0 : kind == 1 ? hh - a.nq : hh - a.nq - nkv;
-        float x[8] = {};
-        if (on) {
-            if (kind == 0) load8<F32, TI>(a.q, row * a.qs + (int64_t)hh * HD + c0, x);
-            else if (kind == 1) load8<F32, TI>(a.k, row * a.ks + (int64_t)kh * HD + c0, x);
-            else load8<F32, TI>(a.v, row * a.vs + (int64_t)kh * HD + c0, x);
-        }
+        float x[8];
+        next.get(x);
+        if (h0 + GROUPS * gridDim.y < heads) next = fetch(h0 + GROUPS * gridDim.y);
         const float* nw = kind == 0 ? a.qn : kind == 1 ? a.kn : nullptr;
         if (a.qn || a.kn) {
             float ss = 0.0f;
@@ -142,6 +181,14 @@ __global__ __launch_bounds__(256) void k_rope_append(RaArgs a) {
                 a.p.w[((size_t)page * nkv + kh) * a.p.page_size + in_page] = 0.0f;
         }
     }
+}
+
+template <typename TI, bool F32, typename T, int HD> __global__ __launch_bounds__(256) void k_rope_append(RaArgs a) {
+    rope_row<TI, F32, T, HD, false>(a, AxArgs());
+}
+template <typename TI, bool F32, typename T, int HD>
+__global__ __launch_bounds__(256) void k_rope_append_axes(RaArgs a, AxArgs ax) {
+    rope_row<TI, F32, T, HD, true>(a, ax);
 }
 
 // ---------------------------------------------------------------------------
@@ -899,17 +946,22 @@ template <typename T, int HD> void weights_hd(PwArgs a, int64_t ctx, hipStream_t
     const dim3 g((unsigned)nkv, (unsigned)n, (unsigned)z);
     hipLaunchKernelGGL((k_pa_weights_few<T, HD>), g, dim3(256), 0, st, a);
 }
-template <typename TI, bool F32, typename T> void rope_hd(const RaArgs& a, dim3 g, hipStream_t st) {
+template <typename TI, bool F32, typename T, int HD>
+void rope_go(const RaArgs& a, const AxArgs* ax, dim3 g, hipStream_t st) {
+    if (ax) hipLaunchKernelGGL((k_rope_append_axes<TI, F32, T, HD>), g, dim3(256), 0, st, a, *ax);
+    else hipLaunchKernelGGL((k_rope_append<TI, F32, T, HD>), g, dim3(256), 0, st, a);
+}
+template <typename TI, bool F32, typename T> void rope_hd(const RaArgs& a, const AxArgs* ax, dim3 g, hipStream_t st) {
     switch (a.p.head_dim) {
-        case 64: hipLaunchKernelGGL((k_rope_append<TI, F32, T, 64>), g, dim3(256), 0, st, a); break;
-        case 128: hipLaunchKernelGGL((k_rope_append<TI, F32, T, 128>), g, dim3(256), 0, st, a); break;
-        default: hipLaunchKernelGGL((k_rope_append<TI, F32, T, 256>), g, dim3(256), 0, st, a); break;
+        case 64: rope_go<TI, F32, T, 64>(a, ax, g, st); break;
+        case 128: rope_go<TI, F32, T, 128>(a, ax, g, st); break;
+        default: rope_go<TI, F32, T, 256>(a, ax, g, st); break;
     }
 }
-template <typename T> void rope_in(const RaArgs& a, int in_type, dim3 g, hipStream_t st) {
-    if (in_type == DPUF_AMD_F32) rope_hd<Bf16, true, T>(a, g, st);
-    else if (in_type == DPUF_AMD_BF16) rope_hd<Bf16, false, T>(a, g, st);
-    else rope_hd<Fp16, false, T>(a, g, st);
+template <typename T> void rope_in(const RaArgs& a, const AxArgs* ax, int in_type, dim3 g, hipStream_t st) {
+    if (in_type == DPUF_AMD_F32) rope_hd<Bf16, true, T>(a, ax, g, st);
+    else if (in_type == DPUF_AMD_BF16) rope_hd<Bf16, false, T>(a, ax, g, st);
+    else rope_hd<Fp16, false, T>(a, ax, g, st);
 }
 
 }  // namespace
@@ -917,9 +969,9 @@ template <typename T> void rope_in(const RaArgs& a, int in_type, dim3 g, hipStre
 extern "C" {
 
 void dpuf_hip_rope_append(void* s, const DpufAmdBatch* b, const DpufAmdPages* p, const DpufAmdRope* r,
-                          const int32_t* pos, int32_t in_type, int32_t nq, const void* q, const void* k, const void* v,
-                          int64_t qs, int64_t ks, int64_t vs, const float* qn, const float* kn, float eps,
-                          void* q_out) {
+                          const DpufAmdRopeAxes* x, const int32_t* pos, int64_t pos_stride, int32_t in_type, int32_t nq,
+                          const void* q, const void* k, const void* v, int64_t qs, int64_t ks, int64_t vs,
+                          const float* qn, const float* kn, float eps, void* q_out) {
     RaArgs a;
     a.b = *b;
     a.p = *p;
@@ -946,8 +998,19 @@ void dpuf_hip_rope_append(void* s, const DpufAmdBatch* b, const DpufAmdPages* p,
     int y = (dpuf_hip_cu_count() + b->n_rows - 1) / b->n_rows;
     if (y > turns) y = turns;
     const dim3 g(b->n_rows, y);
-    if (p->type == DPUF_AMD_BF16) rope_in<Bf16>(a, in_type, g, ST(s));
-    else rope_in<Fp16>(a, in_type, g, ST(s));
+    AxArgs ax = {};
+    if (x) {
+        ax.n = x->n_axes;
+        ax.in_turn = x->in_turn != 0;
+        for (int i = 0, end = 0; i < 3; i++) {
+            end += i < ax.n ? x->sections[i] : 0;
+            ax.end[i] = !ax.in_turn ? end : i + 1 < ax.n ? ax.n * x->sections[i + 1] : 0;
+        }
+        ax.inv = 65536 / ax.n + 1;
+        ax.stride = pos_stride;
+    }
+    if (p->type == DPUF_AMD_BF16) rope_in<Bf16>(a, x ? &ax : nullptr, in_type, g, ST(s));
+    else rope_in<Fp16>(a, x ? &ax : nullptr, in_type, g, ST(s));
     LAUNCHED("k_rope_append");
 }
 

@@ -263,6 +263,30 @@ DPUF_EXPORT int32_t dpuf_amd_rope_append(const DpufAmdBatch* batch, const DpufAm
                                          const float* d_q_norm, const float* d_k_norm, float eps, void* d_q_out,
                                          void* hip_stream);
 
+/* Positions of several axes (time, height and width of a picture's or film's
+ * patches; text has the same on all): pair j of the rotated columns turns by
+ * the position on its axis.  Axes take sections[0], sections[1], ... pairs one
+ * after the other, or in turn: axis a > 0 the pairs a, a + n_axes, ... as many
+ * as its section says, axis 0 all others.  n_axes 1 to 4; sections 0 or more,
+ * rot_dim / 2 together (entries past n_axes are not read), and in turn no more
+ * than there are such pairs. */
+typedef struct {
+    int32_t n_axes;
+    int32_t sections[4];
+    int32_t in_turn;
+} DpufAmdRopeAxes;
+
+/* dpuf_amd_rope_append with a position on each axis: row's on axis a is
+ * d_positions[a * pos_stride + row], pos_stride at least n_rows (with one axis
+ * it is not read).  Everything else as above. */
+DPUF_EXPORT int32_t dpuf_amd_rope_append_axes(const DpufAmdBatch* batch, const DpufAmdPages* pages,
+                                              const DpufAmdRope* rope, const DpufAmdRopeAxes* axes,
+                                              const int32_t* d_positions, int64_t pos_stride, int32_t in_type,
+                                              int32_t n_q_heads, const void* d_q, const void* d_k, const void* d_v,
+                                              int64_t q_stride, int64_t k_stride, int64_t v_stride,
+                                              const float* d_q_norm, const float* d_k_norm, float eps, void* d_q_out,
+                                              void* hip_stream);
+
 /* Attention of the new rows over the pages: row i of a sequence's n attends
  * to cached rows 0 .. ctx_len - n + i; query head j to kv head
  * j / (n_q_heads / n_kv_heads), at most 32 query heads per kv head.  d_q
@@ -284,6 +308,20 @@ DPUF_EXPORT size_t dpuf_amd_paged_attn_workspace(const DpufAmdBatch* batch, cons
 DPUF_EXPORT int32_t dpuf_amd_paged_attn(const DpufAmdBatch* batch, const DpufAmdPages* pages, int32_t n_q_heads,
                                         const void* d_q, float scale, int32_t out_type, void* d_out, float* d_lse,
                                         void* d_workspace, size_t workspace_bytes, void* hip_stream);
+
+/* dpuf_amd_paged_attn with a sliding window and first tokens that stay visible:
+ * the row at place p of its sequence (p = ctx_len - n + i) attends to cached
+ * rows t <= p with t > p - window or t < sink.  window 1 to 2^30, itself
+ * included; sink 0 to 2^30.  Table entries of pages with no row that a new row
+ * attends to are not read as pages: they may hold anything, and the pages may
+ * be other sequences' by now.  The workspace is that of these arguments, window
+ * and sink among them.  Everything else as above. */
+DPUF_EXPORT size_t dpuf_amd_paged_attn_window_workspace(const DpufAmdBatch* batch, const DpufAmdPages* pages,
+                                                        int32_t n_q_heads, int32_t window, int32_t sink);
+DPUF_EXPORT int32_t dpuf_amd_paged_attn_window(const DpufAmdBatch* batch, const DpufAmdPages* pages, int32_t n_q_heads,
+                                               const void* d_q, float scale, int32_t window, int32_t sink,
+                                               int32_t out_type, void* d_out, float* d_lse, void* d_workspace,
+                                               size_t workspace_bytes, void* hip_stream);
 
 /* pages->w[row] = decay * d_w_in[row] + the probabilities exp(scale q.k - lse)
  * that the new rows of the row's sequence give it, summed over rows and over
@@ -333,6 +371,28 @@ DPUF_EXPORT int32_t dpuf_amd_sample(int32_t type, int32_t n, int32_t V, int64_t 
                                     const float* d_temperature, const int32_t* d_top_k, const float* d_top_p,
                                     const float* d_min_p, const float* d_u, int32_t* d_tokens, float* d_logprobs,
                                     void* d_workspace, size_t workspace_bytes, void* hip_stream);
+
+/* Scores of n rows (1 to 65536) of V logits (1 to DPUF_AMD_SAMPLE_MAX_VOCAB;
+ * rows row_stride elements apart) as they are, at temperature 1, with
+ * p = exp(x) / sum exp(x): NaN logits count as -infinity, +infinity leaves only
+ * its like.  d_logprobs [n][n_targets] gets ln p of row i's tokens
+ * d_targets[i * n_targets ...] (0 to DPUF_AMD_LOGPROBS_MAX_TARGETS of them; the
+ * same one may be there twice; one outside [0, V) gets -infinity), d_entropy
+ * [n] -sum p ln p, d_top_tokens and d_top_logprobs [n][n_top] the n_top (0 to
+ * DPUF_AMD_LOGPROBS_MAX_TOP) largest logits' tokens (ties: the lowest indices)
+ * and ln p, in that order.  Fewer logits above -infinity than that leave -1 and
+ * -infinity; a row without any gives -infinity and an entropy of 0.  d_targets
+ * and d_logprobs may be NULL (n_targets 0), as may d_entropy, and d_top_tokens
+ * and d_top_logprobs (n_top 0), not all three outputs.  Sums are fp32.  The
+ * same inputs give the same bits.  The workspace (on 16 bytes) is that of n
+ * rows of V: fewer rows are cut into more chunks and may need more. */
+#define DPUF_AMD_LOGPROBS_MAX_TARGETS 1024
+#define DPUF_AMD_LOGPROBS_MAX_TOP 64
+DPUF_EXPORT size_t dpuf_amd_logprobs_workspace(int32_t n, int32_t V, int32_t n_top);
+DPUF_EXPORT int32_t dpuf_amd_logprobs(int32_t type, int32_t n, int32_t V, int64_t row_stride, const void* d_logits,
+                                      int32_t n_targets, const int32_t* d_targets, int32_t n_top, float* d_logprobs,
+                                      float* d_entropy, int32_t* d_top_tokens, float* d_top_logprobs,
+                                      void* d_workspace, size_t workspace_bytes, void* hip_stream);
 
 /* ---- The engine over pages and with sampling ----------------------------- */
 
