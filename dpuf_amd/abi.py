@@ -319,6 +319,8 @@ def load_engine():
     _sig(lib, "dpuf_amd_engine_pages_create", I32, [P, I32, I32, I32])
     _sig(lib, "dpuf_amd_engine_pages", I32, [P, I32, pages])
     _sig(lib, "dpuf_amd_engine_forward_pages", I32, [P, I32, P, P, P, I32, P, P, F32, smp, P, P, P])
+    _sig(lib, "dpuf_amd_engine_pages_window", I32, [P, P, I32])
+    _sig(lib, "dpuf_amd_engine_score_pages", I32, [P, I32, P, P, P, I32, P, P, I32, P, I32, P, P, P, P])
     _sig(lib, "dpuf_amd_engine_evict_pages", I32, [P, I32, P, P, I32, I32, I32, I32, P, I32, P])
     _engine = lib
     return lib

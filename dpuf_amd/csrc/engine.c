@@ -153,6 +153,14 @@ typedef struct {
     DpufAmdBatch pg_b;   /* of the call at work; n_seqs 0: the layers run over slots */
     int32_t* pg_pos;
     float pg_decay;
+    /* the layers' windows (NULL: none) and their first tokens that stay visible */
+    int32_t* pg_window;
+    int32_t pg_sink;
+    /* scores (dpuf_amd_engine_score_pages): targets and results through pinned staging */
+    int32_t *h_score, *d_score;
+    size_t score_ints;
+    void* d_score_ws;
+    size_t score_ws;
 } Engine;
 
 #define IO_POS DPUF_AMD_MAX_BATCH
@@ -523,6 +531,10 @@ static void engine_free(Engine* e) {
     dpuf_hip_bind_error_word(NULL);
     if (e->stream) dpuf_hip_sync(e->stream);
     pages_free(e);
+    free(e->pg_window);
+    dpuf_hip_host_free(e->h_score);
+    dpuf_hip_free(e->d_score);
+    dpuf_hip_free(e->d_score_ws);
     dpuf_hip_host_free(e->h_smp);
     dpuf_hip_free(e->d_smp);
     dpuf_hip_free(e->d_smp_ws);
@@ -1016,6 +1028,9 @@ static DpufAmdPages pages_of(const Engine* e, int32_t l) {
     return p;
 }
 
+/* Layer l's window (0: none). */
+static int32_t window_of(const Engine* e, int32_t l) { return e->pg_window ? e->pg_window[l] : 0; }
+
 /* QK-norm, RoPE, the append to layer l's pages and the attention of the
  * call's rows over them, into e->ao; with pg_decay >= 0 the weights too. */
 static void enqueue_paged_attention(Engine* e, int32_t l, float scale, float eps) {
@@ -1023,7 +1038,8 @@ static void enqueue_paged_attention(Engine* e, int32_t l, float scale, float eps
     const DpufAmdPages p = pages_of(e, l);
     dpuf_hip_rope_append(s, &e->pg_b, &p, &e->pg_rope, NULL, e->pg_pos, 0, DPUF_AMD_F32, e->nq, e->q, e->k, e->v, e->qd, e->kvd,
                          e->kvd, e->d_norm[4 * l + 1], e->d_norm[4 * l + 2], eps, e->pg_q);
-    dpuf_hip_paged_attn(s, &e->pg_b, &p, e->nq, e->pg_q, scale, 0, 0, 1, e->ao, e->pg_lse, e->pg_ws);
+    dpuf_hip_paged_attn(s, &e->pg_b, &p, e->nq, e->pg_q, scale, window_of(e, l), e->pg_sink, 1, e->ao, e->pg_lse,
+                        e->pg_ws);
     if (e->pg_decay >= 0.0f)
         dpuf_hip_paged_attn_weights(s, &e->pg_b, &p, e->nq, e->pg_q, scale, e->pg_lse, e->pg_decay, p.w);
 }
@@ -1588,34 +1604,69 @@ DPUF_EXPORT int32_t dpuf_amd_engine_pages(void* handle, int32_t layer, DpufAmdPa
     return 0;
 }
 
-/* Staging of `ints` table entries, host and device; grown when needed (no
- * call is in flight: every one ends with its stream drained). */
-static int pages_staging(Engine* e, size_t ints) {
-    if (ints <= e->pg_ints) return 1;
-    dpuf_hip_host_free(e->h_pg);
-    dpuf_hip_free(e->d_pg);
-    e->pg_ints = 0;
-    e->h_pg = (int32_t*)dpuf_hip_host_alloc(ints * 4);
-    e->d_pg = (int32_t*)dpuf_hip_malloc(ints * 4);
-    if (!e->h_pg || !e->d_pg) {
-        dpuf_hip_host_free(e->h_pg);
-        dpuf_hip_free(e->d_pg);
-        e->h_pg = e->d_pg = NULL;
+DPUF_EXPORT int32_t dpuf_amd_engine_pages_window(void* handle, const int32_t* window, int32_t sink) {
+    Engine* e = (Engine*)handle;
+    if (!e) return -1;
+    if (sink < 0 || sink > 1 << 30) return -2;
+    int some = 0;
+    for (int32_t l = 0; window && l < e->L; l++) {
+        if (window[l] < 0 || window[l] > 1 << 30) return -2;
+        some |= window[l] > 0;
+    }
+    int32_t* w = NULL;
+    if (some) {
+        w = (int32_t*)malloc((size_t)e->L * 4);
+        if (!w) return -2;
+        memcpy(w, window, (size_t)e->L * 4);
+    }
+    free(e->pg_window);
+    e->pg_window = w;
+    e->pg_sink = sink;
+    return 0;
+}
+
+/* Staging of `ints` words, host and device; grown when needed (no call is in
+ * flight: every one ends with its stream drained). */
+static int staging(int32_t** h, int32_t** d, size_t* have, size_t ints) {
+    if (ints <= *have) return 1;
+    dpuf_hip_host_free(*h);
+    dpuf_hip_free(*d);
+    *have = 0;
+    *h = (int32_t*)dpuf_hip_host_alloc(ints * 4);
+    *d = (int32_t*)dpuf_hip_malloc(ints * 4);
+    if (!*h || !*d) {
+        dpuf_hip_host_free(*h);
+        dpuf_hip_free(*d);
+        *h = *d = NULL;
         return 0;
     }
-    e->pg_ints = ints;
+    *have = ints;
     return 1;
+}
+static int pages_staging(Engine* e, size_t ints) { return staging(&e->h_pg, &e->d_pg, &e->pg_ints, ints); }
+
+/* Device memory of at least n bytes at *p. */
+static int grown(void** p, size_t* have, size_t n) {
+    if (n <= *have) return 1;
+    dpuf_hip_free(*p);
+    *p = dpuf_hip_malloc(n);
+    *have = *p ? n : 0;
+    return *p != NULL;
 }
 
 /* Lengths and tables of n sequences: every length fits its row of the table
  * and every page it needs is in the pool.  uses (pg_n counters, zeroed) counts
- * each page's sequences. */
+ * each page's sequences.  rows (or NULL): its new rows, which see no more than
+ * the layers' windows (`reach`, if every layer has one, and pg_sink) leave. */
 static int32_t check_tables(const Engine* e, int32_t n, const int32_t* len, const int32_t* table, int32_t stride,
-                            int32_t least, uint8_t* uses) {
+                            int32_t least, uint8_t* uses, const int32_t* rows, int32_t reach) {
     for (int32_t i = 0; i < n; i++) {
         if (len[i] < least || (int64_t)len[i] > (int64_t)stride * e->pg_size) return -3;
         const int32_t np = (len[i] + e->pg_size - 1) / e->pg_size;
+        const int32_t lo = rows && reach ? len[i] - rows[i] - reach + 1 : 0;
         for (int32_t j = 0; j < np; j++) {
+            const int64_t at = (int64_t)j * e->pg_size;
+            if (at + e->pg_size <= lo && at >= e->pg_sink) continue;
             const int32_t p = table[(size_t)i * stride + j];
             if (p < 0 || p >= e->pg_n) return -3;
             if (uses[p] < 2) uses[p]++;
@@ -1624,16 +1675,57 @@ static int32_t check_tables(const Engine* e, int32_t n, const int32_t* len, cons
     return 0;
 }
 
-DPUF_EXPORT int32_t dpuf_amd_engine_forward_pages(void* handle, int32_t n, const int32_t* rows,
-                                                  const int32_t* ctx_len, const int32_t* page_table,
-                                                  int32_t table_stride, const int32_t* token_ids,
-                                                  const int32_t* positions, float weight_decay,
-                                                  const DpufAmdSampling* sampling, float* logits_out,
-                                                  int32_t* tokens_out, float* logprobs_out) {
-    Engine* e = (Engine*)handle;
+/* What a pass is scored by (dpuf_amd_engine_score_pages). */
+typedef struct {
+    int32_t n_targets, n_top;
+    const int32_t* targets;
+    float *logprobs, *entropy, *top_logprobs;
+    int32_t* top_tokens;
+} Score;
+
+/* Memory for the scores of M rows, with the targets on their way to the device. */
+static int score_begin(Engine* e, int32_t M, const Score* sc) {
+    const size_t nt = (size_t)M * sc->n_targets, k = (size_t)M * sc->n_top;
+    if (!staging(&e->h_score, &e->d_score, &e->score_ints, 2 * nt + 2 * k + M) ||
+        !grown(&e->d_score_ws, &e->score_ws, dpuf_hip_logprobs_workspace(M, e->V, sc->n_top)))
+        return 0;
+    if (nt) {
+        memcpy(e->h_score, sc->targets, nt * 4);
+        dpuf_hip_h2d(e->d_score, e->h_score, nt * 4, e->stream);
+    }
+    return 1;
+}
+
+/* Scores of e->logits' first M rows into h_score: [M] entropies, [M][n_targets]
+ * and [M][n_top] log probabilities and [M][n_top] tokens behind the targets,
+ * valid once the stream has drained. */
+static void enqueue_score(Engine* e, int32_t M, const Score* sc) {
+    const size_t nt = (size_t)M * sc->n_targets, k = (size_t)M * sc->n_top;
+    float *en = (float*)e->d_score + nt, *lp = en + M, *tl = lp + nt;
+    dpuf_hip_logprobs(e->stream, DPUF_AMD_F32, M, e->V, e->V, e->logits, sc->n_targets, nt ? e->d_score : NULL,
+                      sc->n_top, nt ? lp : NULL, en, k ? (int32_t*)(tl + k) : NULL, k ? tl : NULL, e->d_score_ws);
+    dpuf_hip_d2h(e->h_score + nt, en, (M + nt + 2 * k) * 4, e->stream);
+}
+static void score_end(const Engine* e, int32_t M, const Score* sc) {
+    const size_t nt = (size_t)M * sc->n_targets, k = (size_t)M * sc->n_top;
+    const int32_t* en = e->h_score + nt;
+    if (sc->entropy) memcpy(sc->entropy, en, (size_t)M * 4);
+    if (nt) memcpy(sc->logprobs, en + M, nt * 4);
+    if (k) {
+        memcpy(sc->top_logprobs, en + M + nt, k * 4);
+        memcpy(sc->top_tokens, en + M + nt + k, k * 4);
+    }
+}
+
+/* score (or NULL) instead of everything else that a pass gives out. */
+static int32_t forward_pages(Engine* e, int32_t n, const int32_t* rows, const int32_t* ctx_len,
+                             const int32_t* page_table, int32_t table_stride, const int32_t* token_ids,
+                             const int32_t* positions, float weight_decay, const DpufAmdSampling* sampling,
+                             float* logits_out, int32_t* tokens_out, float* logprobs_out, const Score* score) {
     if (!e || e->pg_n == 0 || !rows || !ctx_len || !page_table || !token_ids || !positions ||
-        (!logits_out && !tokens_out) || (sampling && (!tokens_out || !sampling_ok(e, sampling))) ||
-        (logprobs_out && !sampling) || !(weight_decay == weight_decay) || isinf(weight_decay))
+        (!logits_out && !tokens_out && !score) || (sampling && (!tokens_out || !sampling_ok(e, sampling))) ||
+        (logprobs_out && !sampling) || !(weight_decay == weight_decay) || isinf(weight_decay) ||
+        (weight_decay >= 0.0f && e->pg_window))
         return -1;
     if (n < 1 || n > DPUF_AMD_MAX_BATCH || table_stride < 1 || (int64_t)table_stride * e->pg_size > (int64_t)1 << 30)
         return -2;
@@ -1650,7 +1742,13 @@ DPUF_EXPORT int32_t dpuf_amd_engine_forward_pages(void* handle, int32_t n, const
     }
     uint8_t* uses = (uint8_t*)calloc((size_t)e->pg_n, 1);
     if (!uses) return -2;
-    int32_t rc = check_tables(e, n, ctx_len, page_table, table_stride, 1, uses);
+    /* what the layer that reaches furthest back sees; 0 where one sees all */
+    int32_t reach = 0;
+    for (int32_t l = 0; l < e->L; l++) {
+        const int32_t w = window_of(e, l);
+        reach = w && (reach || l == 0) ? (w > reach ? w : reach) : 0;
+    }
+    int32_t rc = check_tables(e, n, ctx_len, page_table, table_stride, 1, uses, rows, reach);
     for (int32_t i = 0; i < n && rc == 0; i++) {
         /* pages that new rows go into, and with weights kept all pages, are
          * this sequence's alone */
@@ -1687,13 +1785,12 @@ DPUF_EXPORT int32_t dpuf_amd_engine_forward_pages(void* handle, int32_t n, const
     b.ctx_len = e->d_pg + (hc - hs);
     b.page_table = e->d_pg + (ht - hs);
     const DpufAmdPages p0 = pages_of(e, 0);
-    const size_t ws = dpuf_hip_paged_attn_workspace(&b, &p0, e->nq, 0, 0);
-    if (ws > e->pg_ws_bytes) {
-        dpuf_hip_free(e->pg_ws);
-        e->pg_ws = dpuf_hip_malloc(ws);
-        e->pg_ws_bytes = e->pg_ws ? ws : 0;
-        if (!e->pg_ws) return -2;
+    size_t ws = 0;
+    for (int32_t l = 0; l < (e->pg_window ? e->L : 1); l++) {
+        const size_t w = dpuf_hip_paged_attn_workspace(&b, &p0, e->nq, window_of(e, l), e->pg_sink);
+        if (w > ws) ws = w;
     }
+    if (!grown(&e->pg_ws, &e->pg_ws_bytes, ws) || (score && !score_begin(e, M, score))) return -2;
     dpuf_hip_h2d(e->d_pg, e->h_pg, ints * 4, e->stream);
     /* the decode setting when every sequence appends one token, as for
      * sessions; the prefill setting with a prompt among them */
@@ -1710,14 +1807,18 @@ DPUF_EXPORT int32_t dpuf_amd_engine_forward_pages(void* handle, int32_t n, const
     e->pg_decay = weight_decay;
     enqueue_layers(e, M, keep);
     e->pg_b.n_seqs = 0;
-    /* the sequences' last rows, one after the other, then the head over them */
+    /* the sequences' last rows, one after the other (for scores all rows, as
+     * they are), then the head over them */
+    const int32_t out_rows = score ? M : n;
     float* hx = h_other(e);
-    dpuf_hip_gather_sum(e->stream, n, e->H, e->d_pg + (hl - hs), e->hcur, e->L > 0 ? e->hn : NULL, hx);
     const uint8_t* ps[1] = {e->lm.sign};
-    dpuf_hip_resnorm_prep(e->stream, n, e->H, hx, NULL, NULL, e->d_out_norm, e->cfg.rms_eps, 1, ps, e->prep, NULL);
+    if (!score) dpuf_hip_gather_sum(e->stream, n, e->H, e->d_pg + (hl - hs), e->hcur, e->L > 0 ? e->hn : NULL, hx);
+    dpuf_hip_resnorm_prep(e->stream, out_rows, e->H, score ? e->hcur : hx, score && e->L > 0 ? e->hn : NULL,
+                          score && e->L > 0 ? hx : NULL, e->d_out_norm, e->cfg.rms_eps, 1, ps, e->prep, NULL);
     const DpufGemvJob j = job(&e->lm, 0, n_tiles_of(&e->lm), e->prep[0], e->logits, e->V);
-    dpuf_hip_gemv(e->stream, n, 1, &j, NULL, 0.0f);
-    if (sampling) enqueue_sample(e, n, NULL, sampling);
+    dpuf_hip_gemv(e->stream, out_rows, 1, &j, NULL, 0.0f);
+    if (score) enqueue_score(e, M, score);
+    else if (sampling) enqueue_sample(e, n, NULL, sampling);
     else if (tokens_out) dpuf_hip_argmax_rows(e->stream, e->logits, e->V, n, e->d_ms_tok, e->h_tok, e->d_lmred);
     dpuf_hip_publish(e->stream, e->d_flag, 0, e->h_io + IO_OUT);
     tm_end(e, tm);
@@ -1731,7 +1832,36 @@ DPUF_EXPORT int32_t dpuf_amd_engine_forward_pages(void* handle, int32_t n, const
                                      : ((volatile int32_t*)e->h_tok)[i];
         if (logprobs_out) memcpy(logprobs_out, e->h_smp + 6 * DPUF_AMD_MAX_BATCH, (size_t)n * 4);
     }
+    if (rc == 0 && score) score_end(e, M, score);
     return rc;
+}
+
+DPUF_EXPORT int32_t dpuf_amd_engine_forward_pages(void* handle, int32_t n, const int32_t* rows,
+                                                  const int32_t* ctx_len, const int32_t* page_table,
+                                                  int32_t table_stride, const int32_t* token_ids,
+                                                  const int32_t* positions, float weight_decay,
+                                                  const DpufAmdSampling* sampling, float* logits_out,
+                                                  int32_t* tokens_out, float* logprobs_out) {
+    return forward_pages((Engine*)handle, n, rows, ctx_len, page_table, table_stride, token_ids, positions,
+                         weight_decay, sampling, logits_out, tokens_out, logprobs_out, NULL);
+}
+
+DPUF_EXPORT int32_t dpuf_amd_engine_score_pages(void* handle, int32_t n, const int32_t* rows, const int32_t* ctx_len,
+                                                const int32_t* page_table, int32_t table_stride,
+                                                const int32_t* token_ids, const int32_t* positions, int32_t n_targets,
+                                                const int32_t* targets, int32_t n_top, float* logprobs_out,
+                                                float* entropy_out, int32_t* top_tokens_out, float* top_logprobs_out) {
+    Engine* e = (Engine*)handle;
+    if (!e || (n_targets > 0) != (targets != NULL) || (n_targets > 0) != (logprobs_out != NULL) ||
+        (n_top > 0) != (top_tokens_out != NULL) || (n_top > 0) != (top_logprobs_out != NULL) ||
+        (!logprobs_out && !entropy_out && !top_tokens_out))
+        return -1;
+    if (n_targets < 0 || n_targets > DPUF_AMD_LOGPROBS_MAX_TARGETS || n_top < 0 || n_top > DPUF_AMD_LOGPROBS_MAX_TOP ||
+        e->V > DPUF_AMD_SAMPLE_MAX_VOCAB)
+        return -2;
+    const Score sc = {n_targets, n_top, targets, logprobs_out, entropy_out, top_logprobs_out, top_tokens_out};
+    return forward_pages(e, n, rows, ctx_len, page_table, table_stride, token_ids, positions, -1.0f, NULL, NULL, NULL,
+                         NULL, &sc);
 }
 
 DPUF_EXPORT int32_t dpuf_amd_engine_evict_pages(void* handle, int32_t n, const int32_t* ctx_len,
@@ -1748,7 +1878,7 @@ DPUF_EXPORT int32_t dpuf_amd_engine_evict_pages(void* handle, int32_t n, const i
     uint8_t* uses = (uint8_t*)calloc((size_t)e->pg_n, 1);
     uint8_t* dst_uses = (uint8_t*)calloc((size_t)e->pg_n, 1);
     int32_t rc = len && uses && dst_uses ? 0 : -2;
-    if (rc == 0) rc = check_tables(e, n, ctx_len, page_table, table_stride, 0, uses);
+    if (rc == 0) rc = check_tables(e, n, ctx_len, page_table, table_stride, 0, uses, NULL, 0);
     if (rc == 0) {
         int32_t longest = 1;
         for (int32_t i = 0; i < n; i++) {
@@ -1756,7 +1886,7 @@ DPUF_EXPORT int32_t dpuf_amd_engine_evict_pages(void* handle, int32_t n, const i
             if (ctx_len[i] > longest) longest = ctx_len[i];
         }
         if (keep > longest) keep = longest;      /* every row stays: sink and recent say nothing */
-        rc = check_tables(e, n, len, dst_table, dst_stride, 0, dst_uses);
+        rc = check_tables(e, n, len, dst_table, dst_stride, 0, dst_uses, NULL, 0);
     }
     for (int32_t p = 0; p < e->pg_n && rc == 0; p++)
         if (dst_uses[p] > 1 || (dst_uses[p] && uses[p])) rc = -1;

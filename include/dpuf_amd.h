@@ -462,6 +462,26 @@ DPUF_EXPORT int32_t dpuf_amd_engine_forward_pages(void* handle, int32_t n, const
                                                   const DpufAmdSampling* sampling, float* logits_out,
                                                   int32_t* tokens_out, float* logprobs_out);
 
+/* The layers' sliding windows in dpuf_amd_engine_forward_pages and _score_pages
+ * from now on, as in dpuf_amd_paged_attn_window: window [num_layers] (host), 0
+ * for a layer that sees every cached row; NULL, or all 0, for none.  While any
+ * layer has one, weight_decay has to be below 0, and where all have one, table
+ * entries of pages that no new row sees in any layer may be anything.  0 ok; -1
+ * NULL handle, -2 a window or sink outside 0 to 2^30. */
+DPUF_EXPORT int32_t dpuf_amd_engine_pages_window(void* handle, const int32_t* window, int32_t sink);
+
+/* dpuf_amd_engine_forward_pages whose every new row's logits are scored as
+ * dpuf_amd_logprobs does, in the order of token_ids: with M rows in all, targets
+ * [M][n_targets] (a prompt's next tokens, say) and logprobs_out of that size,
+ * entropy_out [M], top_tokens_out and top_logprobs_out [M][n_top]; each may be
+ * NULL (with a count of 0), not all three.  The cached rows' weights stay as they
+ * are.  Codes as for dpuf_amd_engine_forward_pages, -2 also for the counts. */
+DPUF_EXPORT int32_t dpuf_amd_engine_score_pages(void* handle, int32_t n, const int32_t* rows, const int32_t* ctx_len,
+                                                const int32_t* page_table, int32_t table_stride,
+                                                const int32_t* token_ids, const int32_t* positions, int32_t n_targets,
+                                                const int32_t* targets, int32_t n_top, float* logprobs_out,
+                                                float* entropy_out, int32_t* top_tokens_out, float* top_logprobs_out);
+
 /* dpuf_amd_paged_evict on every layer of n sequences of the engine's pages
  * (host pointers): sequence i's min(ctx_len[i], keep) rows that stay go to the
  * pages dst_table[i * dst_stride ...], none of which any of the sequences
