@@ -1,11 +1,14 @@
 // logprobs.hip -- log probabilities of given tokens, entropy and the largest
 // alternatives of rows of logits.
 //
-// With any m near a row's largest logit,
-//     l = sum exp(x_i - m),  u = sum exp(x_i - m) (x_i - m),
-//     ln p_t = x_t - m - ln l,  -sum p ln p = ln l - u / l.
-// Partial sums (m, l, u) move to another m' by d = m' - m: l' = exp(-d) l, u' =
-// exp(-d) (u - d l).
+// With s_i = x_i log2 e - r (one fma, so that r's own rounding cancels) and any r
+// near a row's largest x_i log2 e,
+//     l = sum 2^s_i,  u = sum 2^s_i s_i,
+//     ln p_t = (s_t - log2 l) ln 2,  -sum p ln p = (log2 l - u / l) ln 2.
+// Partial sums (r, l, u) move to another r' by d = r' - r: l' = 2^-d l, u' =
+// 2^-d (u - d l).  Rows whose largest logit is 2^20 or more away from 0, where r
+// would be off by much of a unit, and +infinity, are summed up again, by
+// differences of logits.
 //
 // The k largest logits, in the order "larger first, then lower index": cut the
 // row into groups of neighbouring tokens and order the groups by their largest
@@ -14,9 +17,10 @@
 // or as large and further to the front.  So one pass over the row leaves the
 // groups' largest, and what is read again is k groups.
 //
-//   k_lp_part  a workgroup per chunk of a row: (m, l, u) and the groups' largest;
-//   k_lp_row   a workgroup per row: joins the chunks, picks the k groups, the k
-//              tokens among theirs, and writes.
+//   k_lp_part   a workgroup per chunk of a row: (r, l, u) and the groups' largest;
+//   k_lp_row    a workgroup per row: joins the chunks, picks the k groups, the k
+//               tokens among theirs, and writes;
+//   k_lp_whole  both, a workgroup per row, where there are many rows.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
@@ -28,13 +32,15 @@ namespace {
 constexpr int NT = 256;              // threads of a workgroup
 constexpr int NW = NT / 64;
 constexpr int GL = 16;               // lanes of a group: a row of the wave
-constexpr int DIRECT = 8192;         // groups that are picked from as they are
+constexpr int FEW = 10, MOST = 32;   // groups a thread picks from
+constexpr int DIRECT = NT * MOST;    // groups that are picked from as they are
 constexpr int OVER = 64;             // groups of a bundle, where there are more
 constexpr int LISTED = 1024;         // candidates that are ranked
 constexpr int MAX_TOP = DPUF_AMD_LOGPROBS_MAX_TOP;
-constexpr float LOG2E = 1.4426950408889634f;
-constexpr float SLACK = 6.0f;        // m stays while no logit is larger by more
-const float NEG_INF = -__builtin_huge_valf(), POS_INF = __builtin_huge_valf();
+constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.69314718055994531f;
+constexpr float SLACK = 8.0f;        // r stays while no s is larger
+constexpr float FAR = 0x1p20f;
+const float NEG_INF = -__builtin_huge_valf();
 
 struct LpArgs {
     const void* x;
@@ -44,34 +50,55 @@ struct LpArgs {
     const int* targets;
     float *logp, *entropy, *top_logp;
     int* top;
-    float4* part;                    // [row][chunk]: m, l, u, the largest logit
+    float4* part;                    // [row][chunk]: r, l, u, the largest logit
     uint32_t* most;                  // [row][group]: order_bits of the group's largest logit
 };
 
+// Logits as they lie in memory, 16 bytes a lane, at any place.
+struct __attribute__((packed, aligned(2))) Lines2 { uint32_t w[4]; };
+struct __attribute__((packed, aligned(4))) Lines4 { uint32_t w[4]; };
 struct F32L {
-    static constexpr int VE = 4;
+    static constexpr int VE = 4, U = 4;      // logits of a load; loads of a lane at a time
     typedef float e;
+    static constexpr uint32_t NONE = 0xff800000u;       // -infinity
     static DEV float one(const void* p, int64_t i) { return ((const float*)p)[i]; }
-    // 4 logits at any place
-    static DEV void many(const void* p, int64_t i, float* o) {
-        struct __attribute__((packed, aligned(4))) V4 { float f[4]; };
-        const V4 v = *(const V4*)((const float*)p + i);
+    static DEV u32x4 raw(const void* p, int64_t i) {
+        const Lines4 v = *(const Lines4*)((const float*)p + i);
+        return u32x4{v.w[0], v.w[1], v.w[2], v.w[3]};
+    }
+    static DEV void get(u32x4 v, float* o) {
 #pragma unroll
-        for (int e = 0; e < 4; e++) o[e] = v.f[e];
+        for (int e = 0; e < 4; e++) o[e] = __uint_as_float(v[e]);
     }
 };
 template <typename T> struct H16L {
-    static constexpr int VE = 8;
+    static constexpr int VE = 8, U = 2;
     typedef typename T::e e;
+    static constexpr uint32_t NONE = 0x80008000u | T::EXP | T::EXP << 16;
     static DEV float one(const void* p, int64_t i) { return (float)((const typename T::e*)p)[i]; }
-    static DEV void many(const void* p, int64_t i, float* o) {
-        struct __attribute__((packed, aligned(2))) V8 { uint32_t w[4]; };
-        const V8 w = *(const V8*)((const uint16_t*)p + i);
-        const typename T::v8 v = vec_of<typename T::v8>(u32x4{w.w[0], w.w[1], w.w[2], w.w[3]});
+    static DEV u32x4 raw(const void* p, int64_t i) {
+        const Lines2 v = *(const Lines2*)((const uint16_t*)p + i);
+        return u32x4{v.w[0], v.w[1], v.w[2], v.w[3]};
+    }
+    static DEV void get(u32x4 w, float* o) {
+        const typename T::v8 v = vec_of<typename T::v8>(w);
 #pragma unroll
         for (int e = 0; e < 8; e++) o[e] = (float)v[e];
     }
 };
+// The VE logits from i on, those from hi on -infinity.
+template <typename L> DEV u32x4 load(const void* p, int i, int hi) {
+    if (i + L::VE <= hi) return L::raw(p, i);
+    u32x4 v = {L::NONE, L::NONE, L::NONE, L::NONE};
+    constexpr int PER = L::VE / 4;       // logits of a word
+#pragma unroll
+    for (int e = 0; e < L::VE; e++)
+        if (i + e < hi) {
+            uint32_t x = PER == 1 ? ((const uint32_t*)p)[i + e] : ((const uint16_t*)p)[i + e];
+            v[e / PER] = PER == 1 ? x : (v[e / PER] & ~(0xffffu << (e % PER * 16))) | x << (e % PER * 16);
+        }
+    return v;
+}
 
 // Larger logit, larger integer; -infinity and NaN are 0, both zeros one value.
 DEV uint32_t order_bits(float x) {
@@ -80,154 +107,186 @@ DEV uint32_t order_bits(float x) {
     return x > NEG_INF ? k : 0;
 }
 DEV float from_bits(uint32_t k) { return __uint_as_float(k & 0x80000000u ? k & 0x7fffffffu : ~k); }
-DEV uint64_t comp_of(uint32_t bits, uint32_t i) { return (uint64_t)bits << 32 | (0xffffffffu - i); }
+DEV uint64_t comp_of(uint32_t bits, uint32_t i) { return bits ? (uint64_t)bits << 32 | (0xffffffffu - i) : 0; }
 DEV uint32_t index_of(uint64_t c) { return 0xffffffffu - (uint32_t)c; }
+DEV uint64_t max64(uint64_t a, uint64_t b) { return a > b ? a : b; }
+
+template <int CTRL> DEV uint32_t dpp(uint32_t v) {
+    return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, 0xF, 0xF, false);
+}
+template <int CTRL> DEV float dppf(float v) { return __uint_as_float(dpp<CTRL>(__float_as_uint(v))); }
+// Over the wave, in every lane (of sums, the same bits only from run to run).
+DEV float wave_max(float v) {
+    v = fmaxf(v, dppf<0x128>(v));
+    v = fmaxf(v, dppf<0x124>(v));
+    v = fmaxf(v, dppf<0x122>(v));
+    v = fmaxf(v, dppf<0x121>(v));
+    return max_xor32(max_xor16(v));
+}
+DEV float wave_add(float v) {
+    v += dppf<0x128>(v);
+    v += dppf<0x124>(v);
+    v += dppf<0x122>(v);
+    v += dppf<0x121>(v);
+    return add_xor32(add_xor16(v));
+}
 
 struct Sum {
-    float m, l, u;       // of nothing: l 0
-    // to m' >= m.  Past 1 000 nothing is left, and no product of it is NaN.
+    float r, l, u;       // of nothing: l 0
+    // to r' >= r.  Past 1 000 nothing is left, and no product of it is NaN.
     DEV void move(float to) {
-        const float d = l == 0.0f ? 0.0f : fminf(to - m, 1000.0f), f = __builtin_amdgcn_exp2f(-d * LOG2E);
+        const float d = l == 0.0f ? 0.0f : fminf(to - r, 1000.0f), f = __builtin_amdgcn_exp2f(-d);
         u = f * fmaf(-d, l, u);
         l *= f;
-        m = to;
+        r = to;
     }
     DEV void add(Sum o) {
-        const float to = l == 0.0f ? o.m : o.l == 0.0f ? m : fmaxf(m, o.m);
+        const float to = l == 0.0f ? o.r : o.l == 0.0f ? r : fmaxf(r, o.r);
         move(to);
         o.move(to);
         l += o.l;
         u += o.u;
     }
 };
-// The same sum in every lane of the wave, in one order.
 DEV Sum wave_sum(Sum s) {
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-        const Sum o = {__shfl_xor(s.m, d), __shfl_xor(s.l, d), __shfl_xor(s.u, d)};
-        // both lanes of a pair add in the same order
-        const bool low = (threadIdx.x & d) == 0;
-        Sum a = low ? s : o;
-        a.add(low ? o : s);
-        s = a;
-    }
-    return s;
-}
-
-template <typename L, bool TOP> __global__ __launch_bounds__(NT) void k_lp_part(LpArgs a) {
-    constexpr int VE = L::VE, U = 4, STEP = 64 * VE;       // tokens a wave loads at once
-    __shared__ Sum ss[NW];
-    __shared__ float sm[NW];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int row = blockIdx.x / a.chunks, c = blockIdx.x - row * a.chunks;
-    const void* p = (const typename L::e*)a.x + row * a.stride;
-    const int lo = c * a.chunk, hi = min(a.V, lo + a.chunk);
-    Sum s = {NEG_INF, 0.0f, 0.0f};
-    float top = NEG_INF;
-    for (int w0 = lo + wave * STEP; w0 < hi; w0 += NW * STEP * U) {
-        float x[U][VE];
-#pragma unroll
-        for (int u = 0; u < U; u++) {
-            const int i = w0 + u * NW * STEP + lane * VE;
-            if (i + VE <= hi) {
-                L::many(p, i, x[u]);
-            } else {
-#pragma unroll
-                for (int e = 0; e < VE; e++) x[u][e] = i + e < hi ? L::one(p, i + e) : NEG_INF;
-            }
-        }
-#pragma unroll
-        for (int u = 0; u < U; u++) {
-            const int at = w0 + u * NW * STEP;
-            if (at >= hi) break;
-            float mx = NEG_INF;
-#pragma unroll
-            for (int e = 0; e < VE; e++) mx = fmaxf(mx, __builtin_canonicalizef(x[u][e]));   // (a maximum keeps a signalling NaN)
-            top = fmaxf(top, mx);
-            if (TOP) {
-                uint32_t k = order_bits(mx);
-#define LP_ROR(n) k = max(k, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)k, 0x120 + n, 0xF, 0xF, false))
-                LP_ROR(8);
-                LP_ROR(4);
-                LP_ROR(2);
-                LP_ROR(1);
-#undef LP_ROR
-                const int g = at / (GL * VE) + lane / GL;
-                if (lane % GL == 0 && g < a.groups) a.most[(size_t)row * a.groups + g] = k;
-            }
-            // m follows the largest logit only when it is behind by more than SLACK
-            if (mx > s.m + SLACK) s.move(mx);
-#pragma unroll
-            for (int e = 0; e < VE; e++) {
-                const float d = fmaxf(x[u][e] - s.m, -1000.0f);     // NaN and -infinity: -1000, and so 0
-                const float q = __builtin_amdgcn_exp2f(d * LOG2E);
-                s.l += q;
-                s.u = fmaf(q, d, s.u);
-            }
-        }
-    }
-    s = wave_sum(s);
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) top = fmaxf(top, __shfl_xor(top, d));
-    if (lane == 0) {
-        ss[wave] = s;
-        sm[wave] = top;
-    }
-    __syncthreads();
-    if (threadIdx.x == 0) {
-#pragma unroll
-        for (int w = 1; w < NW; w++) {
-            s.add(ss[w]);
-            top = fmaxf(top, sm[w]);
-        }
-        a.part[blockIdx.x] = make_float4(s.m, s.l, s.u, top);
-    }
+    s.move(wave_max(s.l == 0.0f ? NEG_INF : s.r));
+    return Sum{s.r, wave_add(s.l), wave_add(s.u)};
 }
 
 struct RowLds {
     Sum ss[NW];
     float sm[NW];
-    int count[NW];
     unsigned n;
-    uint64_t quad[64], best[NW], list[LISTED];
+    uint64_t __attribute__((aligned(16))) quad[64];
+    uint64_t best[NW], list[LISTED];
     uint64_t groups[MAX_TOP], tokens[MAX_TOP];
-    uint32_t bundle[(1 << 24) / (GL * 4) / OVER];
 };
 
-DEV uint64_t max64(uint64_t a, uint64_t b) { return a > b ? a : b; }
+// The workgroup's sum and largest logit, in every thread.
+DEV void join(RowLds& sh, Sum& s, float& top) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    s = wave_sum(s);
+    top = wave_max(top);
+    if (lane == 0) {
+        sh.ss[wave] = s;
+        sh.sm[wave] = top;
+    }
+    __syncthreads();
+    s = sh.ss[0];
+    top = sh.sm[0];
+#pragma unroll
+    for (int w = 1; w < NW; w++) {
+        s.add(sh.ss[w]);
+        top = fmaxf(top, sh.sm[w]);
+    }
+}
 
-// The K largest of key(0) .. key(n - 1), largest first, into out; keys other
-// than 0 are distinct, and 0 is nothing.  Returns how many there are, K at most.
-// A bound first: the K-th largest of the largest ones of 64 quads of threads,
-// which at least K keys reach; those that do are listed and ranked.
-template <typename F> DEV int pick(RowLds& sh, int n, int K, F key, uint64_t* out) {
+// (r, l, u) and the largest of tokens [lo, hi), a thread's share; put(g, bits)
+// the groups' largest, by the first lane of each.
+template <typename L, bool TOP, typename F> DEV void scan(const void* p, int lo, int hi, Sum& s, float& top, F put) {
+    constexpr int VE = L::VE, U = L::U, STEP = 64 * VE;       // tokens a wave loads at once
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    s = Sum{-2.0f * FAR, 0.0f, 0.0f};    // logits far below that are nothing (a mask), or the row is summed up again
+    top = NEG_INF;
+    // the next U loads of a lane are on their way while these are worked on
+    u32x4 now[U], next[U];
+    auto fetch = [&](int w0) {
+#pragma unroll
+        for (int u = 0; u < U; u++) next[u] = load<L>(p, w0 + u * NW * STEP + lane * VE, hi);
+    };
+    fetch(lo + wave * STEP);
+    for (int w0 = lo + wave * STEP; w0 < hi; w0 += NW * STEP * U) {
+#pragma unroll
+        for (int u = 0; u < U; u++) now[u] = next[u];
+        if (w0 + NW * STEP * U < hi) fetch(w0 + NW * STEP * U);
+        float x[U][VE];
+#pragma unroll
+        for (int u = 0; u < U; u++) L::get(now[u], x[u]);
+        float most = NEG_INF;
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            float mx = NEG_INF;
+#pragma unroll
+            for (int e = 0; e < VE; e++) mx = fmaxf(mx, __builtin_canonicalizef(x[u][e]));   // (a maximum keeps a signalling NaN)
+            most = fmaxf(most, mx);
+            if (TOP) {
+                uint32_t k = order_bits(mx);
+                k = max(k, dpp<0x128>(k));
+                k = max(k, dpp<0x124>(k));
+                k = max(k, dpp<0x122>(k));
+                k = max(k, dpp<0x121>(k));
+                const int i = w0 + u * NW * STEP + lane * VE;
+                if (lane % GL == 0 && i < hi) put(i / (GL * VE), k);
+            }
+        }
+        // r follows the largest logit only when it is behind by more than SLACK
+        top = fmaxf(top, most);
+        const float m2 = most * LOG2E;
+        if (m2 > s.r + SLACK) s.move(m2);
+        float l = 0.0f, v = 0.0f;
+#pragma unroll
+        for (int u = 0; u < U; u++)
+#pragma unroll
+            for (int e = 0; e < VE; e++) {
+                const float t = fmaxf(fmaf(x[u][e], LOG2E, -s.r), -1000.0f);     // NaN and -infinity: -1000, and so 0
+                const float q = __builtin_amdgcn_exp2f(t);
+                l += q;
+                v = fmaf(q, t, v);
+            }
+        s.l += l;
+        s.u += v;
+    }
+}
+
+// The K largest of the threads' keys, key(0) .. key(n - 1) each (R of them, in
+// registers, or with R 0 n, wherever they are), largest first, into out; keys other than 0 are distinct, and 0 is nothing.  Returns how
+// many there are, K at most.  A bound first: the K-th largest of the largest ones
+// of 64 quads of threads, which at least K keys reach; those that do are listed
+// and ranked.
+template <int R, typename F> DEV int pick(RowLds& sh, int n, int K, F key, uint64_t* out) {
     const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
+    // f(key) of a thread's keys
+    auto each = [&](auto f) {
+        if constexpr (R > 0) {
+#pragma unroll
+            for (int i = 0; i < R; i++) f(key(i));
+        } else {
+            for (int i = 0; i < n; i++) f(key(i));
+        }
+    };
     uint64_t b = 0;
-    for (int i = t; i < n; i += NT) b = max64(b, key(i));
-    b = max64(b, __shfl_xor((unsigned long long)b, 1));
-    b = max64(b, __shfl_xor((unsigned long long)b, 2));
+    each([&](uint64_t k) { b = max64(b, k); });
+    b = max64(b, (uint64_t)dpp<0xB1>((uint32_t)(b >> 32)) << 32 | dpp<0xB1>((uint32_t)b));      // lanes 1 0 3 2
+    b = max64(b, (uint64_t)dpp<0x4E>((uint32_t)(b >> 32)) << 32 | dpp<0x4E>((uint32_t)b));      // lanes 2 3 0 1
     if ((t & 3) == 0) sh.quad[t >> 2] = b;
     if (t == 0) sh.n = 0;
     __syncthreads();
     const uint64_t mine = sh.quad[lane];
     int above = 0;
-#pragma unroll 8
-    for (int i = 0; i < 64; i++) above += sh.quad[i] > mine;
-    const uint64_t at = __ballot(above == K - 1 && mine != 0);
-    const uint64_t bound = at ? __shfl((unsigned long long)mine, __ffsll((unsigned long long)at) - 1) : 1;
-    for (int i = t; i < n; i += NT) {
-        const uint64_t k = key(i);
-        if (k >= bound) {
-            const unsigned e = atomicAdd(&sh.n, 1u);
-            if (e < LISTED) sh.list[e] = k;
-        }
+#pragma unroll
+    for (int i = 0; i < 64; i += 2) {
+        const ulonglong2 q = *(const ulonglong2*)&sh.quad[i];
+        above += (q.x > mine) + (q.y > mine);
     }
+    const uint64_t at = __ballot(above == K - 1 && mine != 0);
+    uint64_t bound = 1;
+    if (at) {
+        const int l = __ffsll((unsigned long long)at) - 1;
+        bound = (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(mine >> 32), l) << 32 |
+                (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)mine, l);
+    }
+    each([&](uint64_t k) {
+        if (k < bound) return;
+        const unsigned e = atomicAdd(&sh.n, 1u);
+        if (e < LISTED) sh.list[e] = k;
+    });
     __syncthreads();
-    const int found = min((int)sh.n, K), listed = sh.n;
+    const int listed = sh.n, found = min(listed, K);
     if (listed <= LISTED) {
         for (int i = t; i < listed; i += NT) {
             const uint64_t k = sh.list[i];
             int r = 0;
+#pragma unroll 8
             for (int e = 0; e < listed; e++) r += sh.list[e] > k;
             if (r < K) out[r] = k;
         }
@@ -236,10 +295,7 @@ template <typename F> DEV int pick(RowLds& sh, int n, int K, F key, uint64_t* ou
         uint64_t last = ~0ull;
         for (int r = 0; r < K; r++) {
             uint64_t m = 0;
-            for (int i = t; i < n; i += NT) {
-                const uint64_t k = key(i);
-                if (k < last) m = max64(m, k);
-            }
+            each([&](uint64_t k) { m = k < last ? max64(m, k) : m; });
 #pragma unroll
             for (int d = 1; d < 64; d <<= 1) m = max64(m, __shfl_xor((unsigned long long)m, d));
             if (lane == 0) sh.best[wave] = m;
@@ -253,124 +309,218 @@ template <typename F> DEV int pick(RowLds& sh, int n, int K, F key, uint64_t* ou
     return found;
 }
 
-template <typename L, bool TOP> __global__ __launch_bounds__(NT) void k_lp_row(LpArgs a) {
-    constexpr int GS = GL * L::VE;       // tokens of a group
-    __shared__ RowLds sh;
-    const int t = threadIdx.x, lane = t & 63, wave = t >> 6, row = blockIdx.x;
-    const void* p = (const typename L::e*)a.x + row * a.stride;
-    Sum s = {NEG_INF, 0.0f, 0.0f};
-    float top = NEG_INF;
-    for (int c = t; c < a.chunks; c += NT) {
-        const float4 v = a.part[(size_t)row * a.chunks + c];
-        s.add(Sum{v.x, v.y, v.z});
-        top = fmaxf(top, v.w);
-    }
-    s = wave_sum(s);
+// The groups' largest: in memory, a thread's first ones on their way before the
+// row's sum is known, or in LDS.
+struct Stored {
+    const uint32_t* p;
+    uint32_t early[FEW];
+    DEV Stored(const uint32_t* at, int n) : p(at) {
 #pragma unroll
-    for (int d = 1; d < 64; d <<= 1) top = fmaxf(top, __shfl_xor(top, d));
-    if (lane == 0) {
-        sh.ss[wave] = s;
-        sh.sm[wave] = top;
+        for (int i = 0; i < FEW; i++) early[i] = at[min(i * NT + (int)threadIdx.x, n - 1)];
     }
-    __syncthreads();
-    s = sh.ss[0];
-    top = sh.sm[0];
+    DEV uint32_t at(int g) const { return p[g]; }
+};
+struct Kept {
+    const uint32_t* p;
+    DEV uint32_t at(int g) const { return p[g]; }
+};
+template <int R> DEV int pick_stored(RowLds& sh, int n, int K, const Stored& most, uint64_t* out) {
+    uint32_t v[R];
 #pragma unroll
-    for (int w = 1; w < NW; w++) {
-        s.add(sh.ss[w]);
-        top = fmaxf(top, sh.sm[w]);
+    for (int i = 0; i < R; i++) {
+        const int g = i * NT + threadIdx.x;
+        v[i] = R <= FEW ? most.early[i % FEW] : most.p[min(g, n - 1)];
+        if (g >= n) v[i] = 0;
     }
-    if (top == POS_INF) {                // its like alone, all as likely
-        int n = 0;
-        for (int i = t; i < a.V; i += NT) n += L::one(p, i) == POS_INF;
+    return pick<R>(sh, R, K, [&](int i) { return comp_of(v[i], i * NT + threadIdx.x); }, out);
+}
+DEV int pick_groups(RowLds& sh, int n, int K, const Stored& most, uint64_t* out) {
+    return n <= NT * FEW / 2 ? pick_stored<FEW / 2>(sh, n, K, most, out)
+           : n <= NT * FEW   ? pick_stored<FEW>(sh, n, K, most, out)
+                             : pick_stored<MOST>(sh, n, K, most, out);
+}
+DEV int pick_groups(RowLds& sh, int n, int K, const Kept& most, uint64_t* out) {
+    return pick<0>(sh, (n + NT - 1) / NT, K,
+                   [&](int i) {
+                       const int g = i * NT + threadIdx.x;
+                       return g < n ? comp_of(most.p[g], g) : 0;
+                   },
+                   out);
+}
+
+// The n groups' tokens, a lane's load of a group at a time, R of them a thread.
+template <typename L, int R> DEV int pick_tokens(const LpArgs& a, RowLds& sh, int n, const void* p) {
+    constexpr int VE = L::VE;
+    uint32_t v[R][VE];
+    int tok[R];
 #pragma unroll
-        for (int d = 1; d < 64; d <<= 1) n += __shfl_xor(n, d);
-        if (lane == 0) sh.count[wave] = n;
+    for (int i = 0; i < R; i++) {
+        const int e = i * NT + threadIdx.x;
+        tok[i] = e < n * GL ? (int)index_of(sh.groups[e / GL]) * GL * VE + e % GL * VE : a.V;
+        float x[VE];
+        L::get(load<L>(p, tok[i], a.V), x);
+#pragma unroll
+        for (int j = 0; j < VE; j++) v[i][j] = order_bits(x[j]);
+    }
+    return pick<R * VE>(sh, R * VE, a.n_top, [&](int i) { return comp_of(v[i / VE][i % VE], tok[i / VE] + i % VE); }, sh.tokens);
+}
+
+// Everything about a row, once its sum and its groups' largest are known.
+// Its thread's first target was read before: tok0.
+template <typename L, bool TOP, typename M>
+DEV void finish(const LpArgs& a, RowLds& sh, int row, const void* p, Sum s, float top, int tok0, const M& most) {
+    const int t = threadIdx.x;
+    auto logit = [&](int tok) { return (unsigned)tok < (unsigned)a.V ? L::one(p, tok) : NEG_INF; };
+    const float x0 = logit(tok0);
+    const bool far = fabsf(top) >= FAR && top > NEG_INF;
+    // difference to the largest, of far rows
+    auto below = [&](float x) { return x == top ? 0.0f : fmaxf((x - top) * LOG2E, -1000.0f); };
+    if (far) {
+        s = Sum{0.0f, 0.0f, 0.0f};
+        for (int i0 = 0; i0 < a.V; i0 += 32 * NT) {
+            float l = 0.0f, u = 0.0f;
+            for (int i = i0 + t; i < min(a.V, i0 + 32 * NT); i += NT) {
+                const float d = below(L::one(p, i)), q = __builtin_amdgcn_exp2f(d);
+                l += q;
+                u = fmaf(q, d, u);
+            }
+            s.l += l;
+            s.u += u;
+        }
+        float same = 0.0f;
         __syncthreads();
-        s = Sum{0.0f, (float)(sh.count[0] + sh.count[1] + sh.count[2] + sh.count[3]), 0.0f};
+        join(sh, s, same);
     }
-    const float log_l = logf(s.l);
+    const float log_l = log2f(s.l);
     auto logp = [&](float x) {
-        if (top == POS_INF) return x == POS_INF ? -log_l : NEG_INF;
-        return x > NEG_INF ? x - s.m - log_l : NEG_INF;
+        if (!(x > NEG_INF)) return NEG_INF;
+        if (far) return (x == top ? 0.0f : x - top) - log_l * LN2;
+        const float d = fmaf(x, LOG2E, -s.r);
+        return d > -1e30f ? (d - log_l) * LN2 : x - top;
     };
-    if (t == 0 && a.entropy) a.entropy[row] = top > NEG_INF ? fmaxf(log_l - s.u / s.l, 0.0f) : 0.0f;
-    for (int i = t; i < a.n_targets; i += NT) {
-        const int64_t at = (int64_t)row * a.n_targets + i;
-        const int tok = a.targets[at];
-        a.logp[at] = (unsigned)tok < (unsigned)a.V ? logp(L::one(p, tok)) : NEG_INF;
-    }
+    if (t == 0 && a.entropy) a.entropy[row] = top > NEG_INF ? fmaxf((log_l - s.u / s.l) * LN2, 0.0f) : 0.0f;
     if constexpr (TOP) {
-        const uint32_t* most = a.most + (size_t)row * a.groups;
-        auto group = [&](int g) -> uint64_t {
-            const uint32_t k = g < a.groups ? most[g] : 0;
-            return k ? comp_of(k, g) : 0;
-        };
+        const int K = a.n_top;
         int n;
         if (a.groups <= DIRECT) {
-            n = pick(sh, a.groups, a.n_top, group, sh.groups);
+            n = pick_groups(sh, a.groups, K, most, sh.groups);
         } else {
-            // bundles of OVER groups first, by the same argument
+            // bundles of OVER groups first, by the same argument; 4 096 of them at most
             const int bundles = (a.groups + OVER - 1) / OVER;
-            for (int b = wave; b < bundles; b += NW) {
-                const int g = b * OVER + lane;
-                uint32_t k = g < a.groups ? most[g] : 0;
-#pragma unroll
-                for (int d = 1; d < 64; d <<= 1) k = max(k, __shfl_xor(k, d));
-                if (lane == 0) sh.bundle[b] = k;
+            uint64_t b[16];
+#pragma unroll 1
+            for (int i = 0; i < 16; i++) {
+                const int at = i * NT + t;
+                uint32_t k = 0;
+                for (int g = at * OVER; g < min(a.groups, (at + 1) * OVER); g++) k = max(k, most.at(g));
+                b[i] = at < bundles ? comp_of(k, at) : 0;
             }
-            __syncthreads();
-            n = pick(sh, bundles, a.n_top, [&](int b) -> uint64_t { return sh.bundle[b] ? comp_of(sh.bundle[b], b) : 0; },
-                     sh.tokens);
-            n = pick(sh, n * OVER, a.n_top,
-                     [&](int i) { return group((int)index_of(sh.tokens[i / OVER]) * OVER + i % OVER); }, sh.groups);
+            n = pick<16>(sh, 16, K, [&](int i) { return b[i]; }, sh.tokens);
+            uint64_t v[MAX_TOP * OVER / NT];
+#pragma unroll
+            for (int i = 0; i < MAX_TOP * OVER / NT; i++) {
+                const int e = i * NT + t, g = e < n * OVER ? (int)index_of(sh.tokens[e / OVER]) * OVER + e % OVER : a.groups;
+                v[i] = g < a.groups ? comp_of(most.at(g), g) : 0;
+            }
+            n = pick<MAX_TOP * OVER / NT>(sh, MAX_TOP * OVER / NT, K, [&](int i) { return v[i]; }, sh.groups);
         }
-        n = pick(sh, n * GS, a.n_top,
-                 [&](int i) -> uint64_t {
-                     const int tok = (int)index_of(sh.groups[i / GS]) * GS + i % GS;
-                     const uint32_t k = tok < a.V ? order_bits(L::one(p, tok)) : 0;
-                     return k ? comp_of(k, tok) : 0;
-                 },
-                 sh.tokens);
-        for (int i = t; i < a.n_top; i += NT) {
-            const int64_t at = (int64_t)row * a.n_top + i;
+        constexpr int LOADS = MAX_TOP * GL / NT;       // of a thread, for that many groups
+        static_assert(LOADS == 4, "as chosen from");
+        n = K <= MAX_TOP / 4   ? pick_tokens<L, 1>(a, sh, n, p)
+            : K <= MAX_TOP / 2 ? pick_tokens<L, 2>(a, sh, n, p)
+                               : pick_tokens<L, 4>(a, sh, n, p);
+        for (int i = t; i < K; i += NT) {
+            const int64_t at = (int64_t)row * K + i;
             a.top[at] = i < n ? (int)index_of(sh.tokens[i]) : -1;
             a.top_logp[at] = i < n ? logp(from_bits((uint32_t)(sh.tokens[i] >> 32))) : NEG_INF;
         }
     }
+    for (int i = t; i < a.n_targets; i += NT) {
+        const int64_t at = (int64_t)row * a.n_targets + i;
+        a.logp[at] = logp(i == t ? x0 : logit(a.targets[at]));
+    }
+}
+
+template <typename L, bool TOP> __global__ __launch_bounds__(NT) void k_lp_part(LpArgs a) {
+    __shared__ RowLds sh;
+    const int row = blockIdx.x / a.chunks, lo = (blockIdx.x - row * a.chunks) * a.chunk;
+    Sum s;
+    float top;
+    scan<L, TOP>((const typename L::e*)a.x + row * a.stride, lo, min(a.V, lo + a.chunk), s, top,
+                 [&](int g, uint32_t k) { a.most[(size_t)row * a.groups + g] = k; });
+    join(sh, s, top);
+    if (threadIdx.x == 0) a.part[blockIdx.x] = make_float4(s.r, s.l, s.u, top);
+}
+
+// A thread's first target of a row, or -1.
+DEV int first_target(const LpArgs& a, int row) {
+    const int t = threadIdx.x;
+    return t < a.n_targets ? a.targets[(int64_t)row * a.n_targets + t] : -1;
+}
+
+template <typename L, bool TOP> __global__ __launch_bounds__(NT) void k_lp_row(LpArgs a) {
+    __shared__ RowLds sh;
+    const int row = blockIdx.x, tok = first_target(a, row);
+    const Stored most(TOP ? a.most + (size_t)row * a.groups : (const uint32_t*)a.part, TOP ? a.groups : 1);
+    Sum s = {NEG_INF, 0.0f, 0.0f};
+    float top = NEG_INF;
+    for (int c = threadIdx.x; c < a.chunks; c += NT) {
+        const float4 v = a.part[(size_t)row * a.chunks + c];
+        s.add(Sum{v.x, v.y, v.z});
+        top = fmaxf(top, v.w);
+    }
+    join(sh, s, top);
+    finish<L, TOP>(a, sh, row, (const typename L::e*)a.x + row * a.stride, s, top, tok, most);
+}
+
+template <typename L, bool TOP> __global__ __launch_bounds__(NT, 8) void k_lp_whole(LpArgs a) {
+    __shared__ RowLds sh;
+    extern __shared__ uint32_t most[];
+    const int row = blockIdx.x, tok = first_target(a, row);
+    const void* p = (const typename L::e*)a.x + row * a.stride;
+    Sum s;
+    float top;
+    scan<L, TOP>(p, 0, a.V, s, top, [&](int g, uint32_t k) { most[g] = k; });
+    join(sh, s, top);
+    finish<L, TOP>(a, sh, row, p, s, top, tok, Kept{most});
 }
 
 struct LpPlan {
-    int chunk, chunks, groups;
+    int whole, chunk, chunks, groups;
     size_t most, bytes;
 };
 
-// Chunks of whole loads of a workgroup, as many as give the card about 2 048
-// workgroups; at most 32 768 tokens, so that a thread adds up no more than 128
-// before sums meet in pairs.
+// One workgroup a row where rows are short (12 000 fp32 logits: one row 8.6 us
+// against 9.7 in two launches, 64 rows 9.1 and 10.2; 20 000: 10.3 and 9.6) or
+// give every CU one or more: 256 rows of 64 000 20.5 and 22.4 (128: 20.0 and
+// 17.1), 384 of 151 936 49 and 60 (bf16 41 and 36; 512: 43 and 45), 256 of them
+// 42 and 40.  Up to 2^19 tokens: a thread adds up 16 at a time, and then 128 such
+// sums, before sums meet in pairs.
+//
+// Otherwise chunks of whole loads of a workgroup, as many as give the card about
+// 2 048 workgroups, of at most 32 768 tokens.  64 rows of 151 936: 17.6 us, in
+// chunks of any multiple of 1 024 tokens, the last load part empty, 20.4.
 LpPlan plan(int n, int V, int n_top, int VE) {
     LpPlan p;
-    const int unit = NT * VE;
+    p.groups = n_top ? (V + GL * VE - 1) / (GL * VE) : 0;
+    p.whole = V <= 16384 || (V <= 1 << 19 && n >= (V <= 65536 ? 256 : 384));
     int c = (2048 + n - 1) / n;
     if (c < (V + 32767) / 32768) c = (V + 32767) / 32768;
-    p.chunk = ((V + c - 1) / c + unit - 1) / unit * unit;
+    p.chunk = ((V + c - 1) / c + 4095) / 4096 * 4096;
     p.chunks = (V + p.chunk - 1) / p.chunk;
-    p.groups = n_top ? (V + GL * VE - 1) / (GL * VE) : 0;
     p.most = (size_t)n * p.chunks * sizeof(float4);
-    p.bytes = p.most + (size_t)n * p.groups * 4;
+    p.bytes = p.whole ? 0 : p.most + (size_t)n * p.groups * 4;
     return p;
 }
 
-template <typename L> void launch(const LpArgs& a, int n, hipStream_t st) {
-    const dim3 g((unsigned)n * a.chunks);
-    if (a.n_top) {
-        hipLaunchKernelGGL((k_lp_part<L, true>), g, dim3(NT), 0, st, a);
-        hipLaunchKernelGGL((k_lp_row<L, true>), dim3(n), dim3(NT), 0, st, a);
+template <typename L, bool TOP> void launch(const LpArgs& a, const LpPlan& pl, int n, hipStream_t st) {
+    if (pl.whole) {
+        hipLaunchKernelGGL((k_lp_whole<L, TOP>), dim3(n), dim3(NT), pl.groups * 4, st, a);
     } else {
-        hipLaunchKernelGGL((k_lp_part<L, false>), g, dim3(NT), 0, st, a);
-        hipLaunchKernelGGL((k_lp_row<L, false>), dim3(n), dim3(NT), 0, st, a);
+        hipLaunchKernelGGL((k_lp_part<L, TOP>), dim3((unsigned)n * a.chunks), dim3(NT), 0, st, a);
+        hipLaunchKernelGGL((k_lp_row<L, TOP>), dim3(n), dim3(NT), 0, st, a);
     }
-    LAUNCHED("k_lp_part/row");
+    LAUNCHED("k_lp");
 }
 
 }  // namespace
@@ -403,9 +553,13 @@ void dpuf_hip_logprobs(void* s, int32_t type, int32_t n, int32_t V, int64_t stri
     a.top = top;
     a.part = (float4*)ws;
     a.most = (uint32_t*)((char*)ws + pl.most);
-    if (type == DPUF_AMD_F32) launch<F32L>(a, n, ST(s));
-    else if (type == DPUF_AMD_BF16) launch<H16L<Bf16>>(a, n, ST(s));
-    else launch<H16L<Fp16>>(a, n, ST(s));
+    auto go = [&](auto type_) {
+        typedef decltype(type_) L;
+        n_top ? launch<L, true>(a, pl, n, ST(s)) : launch<L, false>(a, pl, n, ST(s));
+    };
+    if (type == DPUF_AMD_F32) go(F32L());
+    else if (type == DPUF_AMD_BF16) go(H16L<Bf16>());
+    else go(H16L<Fp16>());
 }
 
 }  // extern "C"

@@ -92,7 +92,7 @@ def test_axes_pages_refused(lib, over, code):
     assert axes(lib, p=pages(**over)) == code
 
 
-def logprobs(lib, t=0, n=3, V=100, stride=100, x=A, nt=2, tg=Q, k=5, lp=OUT, en=LSE, top=OUT + 4096, tl=OUT + 8192, ws=WS,
+def logprobs(lib, t=0, n=3, V=20000, stride=20000, x=A, nt=2, tg=Q, k=5, lp=OUT, en=LSE, top=OUT + 4096, tl=OUT + 8192, ws=WS,
              size=None):
     if size is None:
         size = lib.dpuf_amd_logprobs_workspace(max(1, min(n, 65536)), max(1, min(V, 1 << 24)), max(0, min(k, 64)))
@@ -101,12 +101,12 @@ def logprobs(lib, t=0, n=3, V=100, stride=100, x=A, nt=2, tg=Q, k=5, lp=OUT, en=
 
 @pytest.mark.parametrize("kw,code", [
     (dict(t=3), -5), (dict(t=-1), -5), (dict(n=0), -2), (dict(n=65537), -2), (dict(V=0), -2), (dict(V=(1 << 24) + 1), -2),
-    (dict(nt=-1), -2), (dict(nt=1025), -2), (dict(k=-1), -2), (dict(k=65), -2), (dict(stride=99), -4), (dict(x=None), -1),
+    (dict(nt=-1), -2), (dict(nt=1025), -2), (dict(k=-1), -2), (dict(k=65), -2), (dict(stride=19999), -4), (dict(x=None), -1),
     (dict(x=A + 2), -1), (dict(t=1, x=A + 1), -1), (dict(tg=None), -1), (dict(lp=None), -1), (dict(nt=0), -1),
     (dict(nt=0, tg=None), -1), (dict(k=0), -1), (dict(top=None), -1), (dict(tl=None), -1),
     (dict(nt=0, tg=None, lp=None, k=0, top=None, tl=None, en=None), -1), (dict(tg=Q + 2), -1), (dict(en=LSE + 1), -1),
     (dict(lp=A + 400), -1), (dict(en=Q + 4), -1), (dict(en=OUT + 4), -1), (dict(tl=OUT + 4096 + 4), -1),
-    (dict(ws=None), -1), (dict(ws=WS + 8), -1), (dict(ws=OUT), -1), (dict(size=0), -7),
+    (dict(ws=None), -1), (dict(ws=WS + 8), -1), (dict(n=1, ws=WS + 8), -1), (dict(ws=OUT), -1), (dict(size=0), -7),
     (dict(), -1)])
 def test_logprobs_refused(lib, kw, code):
     """The last of them is in order but for the memory."""
@@ -119,7 +119,8 @@ def test_logprobs_workspace(lib):
     for n, V, k in ((1, 1, 0), (1, 151936, 20), (512, 151936, 0), (2048, 151936, 20), (7, 1 << 24, 64), (65536, 5, 2)):
         need = size(n, V, k)
         over = dict(n=n, V=V, stride=V, k=k, **({} if k else dict(top=None, tl=None)))
-        assert need > 0 and logprobs(lib, size=need - 1, **over) == -7 and logprobs(lib, size=need, **over) == -1
+        assert logprobs(lib, size=need, **over) == -1
+        assert need == 0 or (logprobs(lib, size=need - 1, **over) == -7 and logprobs(lib, ws=None, **over) == -1)
         assert need <= n * V // 8 + 32 * (n + 4096)       # a fraction of the logits
 
 
