@@ -101,8 +101,8 @@ template <bool W, int KT> struct Run {
     DEV Run(const PaArgs& a, int first, int kend) {
         gap = head = 0;
         if constexpr (W) {
-            head = (min(a.sink, max(0, kend)) + KT - 1) & -KT;
-            gap = max(0, (max(0, first - a.window + 1) & -KT) - head);
+            head = __builtin_amdgcn_readfirstlane((min(a.sink, max(0, kend)) + KT - 1) & -KT);
+            gap = __builtin_amdgcn_readfirstlane(max(0, (max(0, first - a.window + 1) & -KT) - head));
         }
     }
     DEV int key(int at) const { return W && at >= head ? at + gap : at; }
@@ -110,6 +110,16 @@ template <bool W, int KT> struct Run {
 // Whether a row at place p sees all of the keys [t, t + n) as far as its window says.
 template <bool W> DEV bool in_window(const PaArgs& a, int t, int n, int p) {
     return !W || t > p - a.window || t + n <= a.sink;
+}
+// Of a lane's keys 0 .. 3, 8 .. 11, 16 .. 19, ..., a bit each, those below n.
+DEV uint32_t first_keys(int n) {
+    const int c = max(n, 0), e = min(4 * (c >> 3) + min(c & 7, 4), 32);
+    return (uint32_t)((1ull << e) - 1);
+}
+// A sequence's rows and length, the same in every lane, in scalar registers.
+DEV PgSeq scalar(PgSeq q) {
+    return PgSeq{__builtin_amdgcn_readfirstlane(q.r0), __builtin_amdgcn_readfirstlane(q.n),
+                 __builtin_amdgcn_readfirstlane(q.ctx)};
 }
 // Keys of a sequence as its ranges count them.
 template <bool W> DEV int span_of(const PaArgs& a, int ctx, bool few) {
@@ -159,6 +169,11 @@ template <typename T> DEV uint32_t take_odd(u32x4& v) {
         v[i] &= ~m;
     }
     return any;
+}
+// Not 0 where v holds an infinity or NaN: adding one to the exponent carries.
+template <typename T> DEV uint32_t odd_hint(u32x4 v) {
+    constexpr uint32_t E = T::EXP | T::EXP << 16, ONE = (0x8000 - T::EXP) * 0x10001u;
+    return (((v[0] & E) + ONE) | ((v[1] & E) + ONE) | ((v[2] & E) + ONE) | ((v[3] & E) + ONE)) & 0x80008000u;
 }
 // The infinities and NaN of the four elements at v, 0 for the others.
 template <typename T> DEV f32x4 odd4(const uint16_t* v) {
@@ -334,9 +349,14 @@ template <typename T, int HD, bool W> DEV void few_rows(const PaArgs& a, FewLds<
                 for (int u = 0; u < 2; u++)
 #pragma unroll
                     for (int i = 0; i < 4; i++)
-                        if (!ok[u] || here + 16 * u + 4 * g4 + i > limit ||
-                            !in_window<W>(a, here + 16 * u + 4 * g4 + i, 1, limit))
+                        if (W) {
+                            const int key = here + 16 * u + 4 * g4 + i;
+                            const bool see = ((unsigned)(limit - key) < (unsigned)a.window) |
+                                             ((key < a.sink) & (key <= limit));
+                            sc[u][i] = (see & ok[u]) ? sc[u][i] : NEG_INF;
+                        } else if (!ok[u] || here + 16 * u + 4 * g4 + i > limit) {
                             sc[u][i] = NEG_INF;
+                        }
             }
             float mt = fmaxf(fmaxf(fmaxf(sc[0][0], sc[0][1]), fmaxf(sc[0][2], sc[0][3])),
                              fmaxf(fmaxf(sc[1][0], sc[1][1]), fmaxf(sc[1][2], sc[1][3])));
@@ -516,7 +536,7 @@ DEV void many_rows(const PaArgs& a, ManyLds<HD>& sh, int kvh, int tile, int z) {
     s = __builtin_amdgcn_readfirstlane(s);
     tile = __builtin_amdgcn_readfirstlane(tile);
     if (s < 0) return;
-    const PgSeq sq = pg_seq(a.b, a.shift, s);
+    const PgSeq sq = scalar(pg_seq(a.b, a.shift, s));
     const int rows = sq.n * a.G;
     const int span = span_of<W>(a, sq.ctx, false);
     const int per = range_keys(span, a.chunk_many, a.nz_many);
@@ -563,6 +583,7 @@ DEV void many_rows(const PaArgs& a, ManyLds<HD>& sh, int kvh, int tile, int z) {
     u32x4 kf[NP], vf[NP];
     int pn[NG];              // pages of the tile to be loaded next
     uint32_t odd = 0;
+    bool part = false;       // of the tile in kf / vf: some row does not see it whole
     // keys before it (with a window, of those that all have in theirs): by all rows
     const int seen = min(kend, sq.ctx - sq.n + TR * tile / a.G + 1 - run.gap);
     auto by_all = [&](int base) { return base + KT <= seen && in_window<W>(a, run.key(base), KT, all - 1); };
@@ -573,27 +594,38 @@ DEV void many_rows(const PaArgs& a, ManyLds<HD>& sh, int kvh, int tile, int z) {
     };
     auto load = [&](int base) {
         const int key = run.key(base);
+        int id[NG];          // scalar, and with them a thread's bases
         bad2 = 0;
 #pragma unroll
-        for (int g = 0; g < NG; g++) bad2 |= ((unsigned)pn[g] >= (unsigned)a.p.n_pages) << g;
+        for (int g = 0; g < NG; g++) {
+            id[g] = __builtin_amdgcn_readfirstlane(pn[g]);
+            const bool in = (unsigned)id[g] < (unsigned)a.p.n_pages;
+            bad2 |= (uint32_t)!in << g;
+            if (!in) id[g] = 0;
+        }
 #pragma unroll
         for (int u = 0; u < NP; u++) {
             const int g = u * RP / 16 + (RP > 16 ? wr : 0);
-            int pg = pn[u * RP / 16 % NG];
+            int pg = id[u * RP / 16 % NG];
 #pragma unroll
-            for (int e = 1; e < RP / 16; e++) pg = wr == e ? pn[(u * RP / 16 + e) % NG] : pg;
-            if ((bad2 >> g) & 1) pg = 0;
+            for (int e = 1; e < RP / 16; e++) pg = wr == e ? id[(u * RP / 16 + e) % NG] : pg;
             const size_t at = (size_t)pg * a.p.page_stride +
                               (size_t)((key + 16 * g) & (a.p.page_size - 1)) * a.p.row_stride +
                               (RP == 8 ? (size_t)(u & 1) * 8 * a.p.row_stride : 0);
             kf[u] = *(const u32x4*)(kp + at + lo);
             vf[u] = *(const u32x4*)(vp + at + lo);
         }
-        if (bad2 || !by_all(base))
-#pragma unroll
-            for (int u = 0; u < NP; u++) odd |= take_odd<T>(vf[u]);
+        part = bad2 || !by_all(base);
     };
     auto store = [&](int buf) {
+        if (part) {
+            uint32_t some = 0;
+#pragma unroll
+            for (int u = 0; u < NP; u++) some |= odd_hint<T>(vf[u]);
+            if (some)
+#pragma unroll
+                for (int u = 0; u < NP; u++) odd |= take_odd<T>(vf[u]);
+        }
 #pragma unroll
         for (int u = 0; u < NP; u++) {
             *(u32x4*)(lk[buf] + (u * RP + lr) * KP + lc) = kf[u];
@@ -637,14 +669,24 @@ DEV void many_rows(const PaArgs& a, ManyLds<HD>& sh, int kvh, int tile, int z) {
                 sc[b] = T::mma32(kv, qf[c], c ? sc[b] : zero);
             }
         // sc[b][i]: key 32 b + 8 (i / 4) + 4 h + i % 4
+        // A lane's keys of the tile, in their order, are the bits of a word: the
+        // row's last one, its window's first and the first ones' end cut it into
+        // runs, and absent pages are eight keys each.
         if (base + KT > min(wend, first_limit + 1 - run.gap) || bad || !in_window<W>(a, here, KT, w_last)) {
+            const int back = limit - here - 4 * h;
+            uint32_t see = first_keys(back + 1);
+            if (W) {
+                see &= ~first_keys(max(back, -1) + 1 - a.window);
+                if (here < run.head) see |= first_keys(min(back + 1, a.sink - here - 4 * h));
+            }
+#pragma unroll
+            for (int g = 0; g < KT / 16; g++) see &= (bad >> g) & 1 ? ~(0xffu << 8 * g) : ~0u;
 #pragma unroll
             for (int b = 0; b < NB; b++)
 #pragma unroll
                 for (int i = 0; i < 16; i++) {
-                    const int key = 32 * b + 8 * (i >> 2) + 4 * h + (i & 3);
-                    if (here + key > limit || ((bad >> (key >> 4)) & 1) || !in_window<W>(a, here + key, 1, limit))
-                        sc[b][i] = NEG_INF;
+                    const uint32_t on = (int)(see << (31 - 16 * b - i)) >> 31, x = __float_as_uint(sc[b][i]);
+                    sc[b][i] = __uint_as_float((x & on) | (0xff800000u & ~on));
                 }
         }
         float mt = NEG_INF;
