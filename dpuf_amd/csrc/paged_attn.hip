@@ -897,6 +897,38 @@ int ceil_div(int64_t a, int64_t b) { return (int)((a + b - 1) / b); }
 // Keys per range: about `times` sqrt(ctx), in whole 128.
 int range_of(int64_t ctx, double times) { return ((int)(times * sqrt((double)ctx)) + 127) & ~127; }
 
+// Key ranges of chunks with a window of about ctx keys: as many as take the
+// least time of up to 8, counted in steps of 64 keys that a workgroup walks one
+// after the other (0.3 us + 1.7 a 128 columns, a sixth more with two workgroups
+// a CU), the join of the ranges (4.5 us and the partial sums written and read at
+// 4.5 TB/s) and the workgroups of the grid that find no rows (1 us a round);
+// beside decoding sequences not less than those take.  Measured for one, two,
+// three, four and eight ranges: 512 rows of 32 heads, 8 kv heads of 128 with a
+// window of 128 keys 15.0 us, 23.6, 22.4, 22.4, 22.5, of 512 24.6, 27.2, 27.0,
+// 26.6, 35.8, of 2 048 80, 57, 46, 44, 56; 48 rows, 512 keys 24.0, 22.1, 19.3,
+// 19.3, 16.9; 256 rows and 31 single ones, 1 024 keys 53.6, 47.0, 47.5, 50.3, 63.
+void window_ranges(PaPlan& r, const DpufAmdBatch& b, const DpufAmdPages& p, int nq, int64_t ctx) {
+    const int G = nq / p.n_kv_heads, tr = r.only == PA_WIDE ? 256 : 128;
+    const int64_t packed = (int64_t)(r.only == PA_BOTH && b.n_rows > b.n_seqs ? b.n_rows - b.n_seqs : b.n_rows) * G;
+    const int64_t wgs = (packed + tr - 1) / tr * p.n_kv_heads, slots = r.only == PA_WIDE ? 256 : 512;
+    const double step = 0.3 + 1.7 * p.head_dim / 128;
+    const double singles = r.only == PA_BOTH ? 0.6 * b.n_seqs * ctx * p.n_kv_heads * p.head_dim * 4 / 4.9e6 : 0;
+    double best = 0;
+    for (int nz = 1; nz <= 8; nz++) {
+        const int chunk = (ceil_div(ctx, nz) + 63) & ~63;
+        if (nz > 1 && ceil_div(ctx, chunk) < nz) continue;
+        double t = (double)chunk / 64 * step * ((wgs * nz + slots - 1) / slots);
+        if (wgs * nz > 256) t *= 1.15;
+        if (t < singles) t = singles;
+        t += (double)p.n_kv_heads * r.y_many * nz / slots;
+        if (nz > 1) t += 4.5 + (double)b.n_rows * nq * nz * p.head_dim * 8 / 4.5e6;
+        if (nz > 1 && t >= 0.97 * best) continue;
+        best = t;
+        r.chunk_many = chunk;
+        r.nz_many = nz;
+    }
+}
+
 // Which kernel takes which sequences.  Row counts are on the device; what the
 // host knows is their sum and the number of sequences.  No more rows than
 // sequences: a decode step (a sequence that has several rows all the same has
@@ -924,7 +956,7 @@ int range_of(int64_t ctx, double times) { return ((int)(times * sqrt((double)ctx
 //
 // With a window the same, by the keys that a tile of rows sees: the first ones,
 // the window and as many more as the tile's rows are apart, in whole tiles of
-// keys.  (A window of 0 here is none.)
+// keys; but the chunks' ranges by window_ranges.  (A window of 0 here is none.)
 PaPlan plan(const DpufAmdBatch& b, const DpufAmdPages& p, int nq, int window, int sink) {
     const int G = nq / p.n_kv_heads;
     PaPlan r;
@@ -936,12 +968,12 @@ PaPlan plan(const DpufAmdBatch& b, const DpufAmdPages& p, int nq, int window, in
     r.sink = r.window < cap ? sink : 0;
     const int64_t near = (int64_t)r.window + (r.sink + 63) / 64 * 64 + 64;
     r.reach_few = (int)(near + 16 / G + 1 < cap ? near + 16 / G + 1 : cap);
-    r.reach_many = (int)(near + 256 / G + 1 < cap ? near + 256 / G + 1 : cap);
     if (window && ctx > r.reach_few) ctx = r.reach_few;
     const int64_t packed = (int64_t)b.n_rows * G;
     r.only = b.n_rows <= b.n_seqs || packed <= r.few ? PA_FEW : b.n_seqs > 1 ? PA_BOTH
              : packed >= 384 && ctx >= 2048 && p.head_dim <= 128 ? PA_WIDE : PA_MANY;
     const int tr = r.only == PA_WIDE ? 256 : 128;
+    r.reach_many = (int)(near + tr / G + 1 < cap ? near + tr / G + 1 : cap);
     const int64_t most = packed / (r.few + 1);
     r.y_few = r.only >= PA_MANY ? 0 : b.n_seqs * ((r.few + 15) / 16);
     r.y_many = r.only == PA_FEW ? 0 : r.only == PA_BOTH ? (int)(packed / 128 + (most < b.n_seqs ? most : b.n_seqs))
@@ -975,6 +1007,7 @@ PaPlan plan(const DpufAmdBatch& b, const DpufAmdPages& p, int nq, int window, in
     r.chunk_many = (ceil_div(ctx, nz) + 127) & ~127;
     if (r.chunk_many < range_of(ctx, 4.0)) r.chunk_many = range_of(ctx, 4.0);
     r.nz_many = ceil_div(ctx, r.chunk_many);
+    if (window && r.only != PA_FEW) window_ranges(r, b, p, nq, b.max_ctx > r.reach_many ? r.reach_many : ctx);
     const size_t all = (size_t)b.n_rows * nq, some = (size_t)b.n_seqs * p.n_kv_heads * r.few;
     r.few_rows = r.only <= PA_FEW && r.nz_few > 1 ? r.nz_few * (r.only == PA_FEW ? all : some) : 0;
     r.many_rows = r.only != PA_FEW && r.nz_many > 1 ? r.nz_many * all : 0;
