@@ -157,8 +157,9 @@ struct RowLds {
     Sum ss[NW];
     float sm[NW];
     unsigned n;
-    uint64_t __attribute__((aligned(16))) quad[64];
-    uint64_t best[NW], list[LISTED];
+    uint32_t __attribute__((aligned(16))) quad[64];
+    uint64_t __attribute__((aligned(16))) list[LISTED];
+    uint64_t best[NW];
     uint64_t groups[MAX_TOP], tokens[MAX_TOP];
 };
 
@@ -238,64 +239,89 @@ template <typename L, bool TOP, typename F> DEV void scan(const void* p, int lo,
     }
 }
 
-// The K largest of the threads' keys, key(0) .. key(n - 1) each (R of them, in
-// registers, or with R 0 n, wherever they are), largest first, into out; keys other than 0 are distinct, and 0 is nothing.  Returns how
-// many there are, K at most.  A bound first: the K-th largest of the largest ones
-// of 64 quads of threads, which at least K keys reach; those that do are listed
-// and ranked.
-template <int R, typename F> DEV int pick(RowLds& sh, int n, int K, F key, uint64_t* out) {
+// The K largest of the threads' items, first by bits, then by the lower index,
+// largest first, into out (as comp_of).  A thread has n items (R of them, in
+// registers, or with R 0 n, wherever they are): bits(i), 0 for none, of index
+// id(i).  Returns how many there are, K at most.  A bound first: the K-th largest
+// of the largest of 64 quads of threads, which at least K items reach; those that
+// do are listed and ranked.
+// LEAN: in few registers.
+template <int R, bool LEAN = false, typename F, typename G>
+DEV int pick(RowLds& sh, int n, int K, F bits, G id, uint64_t* out) {
     const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
-    // f(key) of a thread's keys
+    // f(bits, i) of a thread's items
     auto each = [&](auto f) {
         if constexpr (R > 0) {
 #pragma unroll
-            for (int i = 0; i < R; i++) f(key(i));
+            for (int i = 0; i < R; i++) f(bits(i), i);
         } else {
-            for (int i = 0; i < n; i++) f(key(i));
+            for (int i = 0; i < n; i++) f(bits(i), i);
         }
     };
-    uint64_t b = 0;
-    each([&](uint64_t k) { b = max64(b, k); });
-    b = max64(b, (uint64_t)dpp<0xB1>((uint32_t)(b >> 32)) << 32 | dpp<0xB1>((uint32_t)b));      // lanes 1 0 3 2
-    b = max64(b, (uint64_t)dpp<0x4E>((uint32_t)(b >> 32)) << 32 | dpp<0x4E>((uint32_t)b));      // lanes 2 3 0 1
+    uint32_t b = 0;
+    each([&](uint32_t k, int) { b = max(b, k); });
+    b = max(b, dpp<0xB1>(b));      // lanes 1 0 3 2
+    b = max(b, dpp<0x4E>(b));      // lanes 2 3 0 1
     if ((t & 3) == 0) sh.quad[t >> 2] = b;
     if (t == 0) sh.n = 0;
     __syncthreads();
-    const uint64_t mine = sh.quad[lane];
+    const uint32_t mine = sh.quad[lane];
     int above = 0;
+    constexpr int AT_ONCE = LEAN ? 16 : 64;
+#pragma unroll 1
+    for (int i0 = 0; i0 < 64; i0 += AT_ONCE)
 #pragma unroll
-    for (int i = 0; i < 64; i += 2) {
-        const ulonglong2 q = *(const ulonglong2*)&sh.quad[i];
-        above += (q.x > mine) + (q.y > mine);
+        for (int i = i0; i < i0 + AT_ONCE; i += 4) {
+            const u32x4 q = *(const u32x4*)&sh.quad[i];
+#pragma unroll
+            for (int e = 0; e < 4; e++) above += q[e] > mine;
+        }
+    uint32_t bound = above < K ? mine : ~0u;       // the least of the K largest
+    bound = min(bound, dpp<0x128>(bound));
+    bound = min(bound, dpp<0x124>(bound));
+    bound = min(bound, dpp<0x122>(bound));
+    bound = min(bound, dpp<0x121>(bound));
+    bound = min(min((uint32_t)__builtin_amdgcn_readlane((int)bound, 0), (uint32_t)__builtin_amdgcn_readlane((int)bound, 16)),
+                min((uint32_t)__builtin_amdgcn_readlane((int)bound, 32), (uint32_t)__builtin_amdgcn_readlane((int)bound, 48)));
+    bound = max(bound, 1u);
+    // a wave's items side by side, each round's by lane
+    int hits = 0;
+    each([&](uint32_t k, int) { hits += __popcll(__ballot(k >= bound)); });
+    if (hits) {
+        int e = lane == 0 ? (int)atomicAdd(&sh.n, (unsigned)hits) : 0;
+        e = __builtin_amdgcn_readfirstlane(e);
+        each([&](uint32_t k, int i) {
+            const uint64_t hit = __ballot(k >= bound);
+            const int at = e + (int)__builtin_amdgcn_mbcnt_hi((uint32_t)(hit >> 32),
+                                                              __builtin_amdgcn_mbcnt_lo((uint32_t)hit, 0));
+            if (k >= bound && at < LISTED) sh.list[at] = comp_of(k, id(i));
+            e += __popcll(hit);
+        });
     }
-    const uint64_t at = __ballot(above == K - 1 && mine != 0);
-    uint64_t bound = 1;
-    if (at) {
-        const int l = __ffsll((unsigned long long)at) - 1;
-        bound = (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(mine >> 32), l) << 32 |
-                (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)mine, l);
-    }
-    each([&](uint64_t k) {
-        if (k < bound) return;
-        const unsigned e = atomicAdd(&sh.n, 1u);
-        if (e < LISTED) sh.list[e] = k;
-    });
     __syncthreads();
     const int listed = sh.n, found = min(listed, K);
     if (listed <= LISTED) {
         for (int i = t; i < listed; i += NT) {
             const uint64_t k = sh.list[i];
-            int r = 0;
-#pragma unroll 8
-            for (int e = 0; e < listed; e++) r += sh.list[e] > k;
+            int r = 0, e = 0;
+            for (; e + 8 <= listed; e += 8)
+#pragma unroll
+                for (int d = 0; d < 8; d += 2) {
+                    const ulonglong2 q = *(const ulonglong2*)&sh.list[e + d];
+                    r += (q.x > k) + (q.y > k);
+                }
+            for (; e < listed; e++) r += sh.list[e] > k;
             if (r < K) out[r] = k;
         }
     } else {
-        // too many reach the bound (they lie with few of the threads): one at a time
+        // too many reach the bound (long runs of equal ones, or all with few of the threads): one at a time
         uint64_t last = ~0ull;
         for (int r = 0; r < K; r++) {
             uint64_t m = 0;
-            each([&](uint64_t k) { m = k < last ? max64(m, k) : m; });
+            each([&](uint32_t k, int i) {
+                const uint64_t c = comp_of(k, id(i));
+                m = c < last ? max64(m, c) : m;
+            });
 #pragma unroll
             for (int d = 1; d < 64; d <<= 1) m = max64(m, __shfl_xor((unsigned long long)m, d));
             if (lane == 0) sh.best[wave] = m;
@@ -312,6 +338,7 @@ template <int R, typename F> DEV int pick(RowLds& sh, int n, int K, F key, uint6
 // The groups' largest: in memory, a thread's first ones on their way before the
 // row's sum is known, or in LDS.
 struct Stored {
+    static constexpr bool LEAN = false;
     const uint32_t* p;
     uint32_t early[FEW];
     DEV Stored(const uint32_t* at, int n) : p(at) {
@@ -321,6 +348,7 @@ struct Stored {
     DEV uint32_t at(int g) const { return p[g]; }
 };
 struct Kept {
+    static constexpr bool LEAN = true;
     const uint32_t* p;
     DEV uint32_t at(int g) const { return p[g]; }
 };
@@ -332,7 +360,7 @@ template <int R> DEV int pick_stored(RowLds& sh, int n, int K, const Stored& mos
         v[i] = R <= FEW ? most.early[i % FEW] : most.p[min(g, n - 1)];
         if (g >= n) v[i] = 0;
     }
-    return pick<R>(sh, R, K, [&](int i) { return comp_of(v[i], i * NT + threadIdx.x); }, out);
+    return pick<R>(sh, R, K, [&](int i) { return v[i]; }, [&](int i) { return i * NT + threadIdx.x; }, out);
 }
 DEV int pick_groups(RowLds& sh, int n, int K, const Stored& most, uint64_t* out) {
     return n <= NT * FEW / 2 ? pick_stored<FEW / 2>(sh, n, K, most, out)
@@ -340,16 +368,16 @@ DEV int pick_groups(RowLds& sh, int n, int K, const Stored& most, uint64_t* out)
                              : pick_stored<MOST>(sh, n, K, most, out);
 }
 DEV int pick_groups(RowLds& sh, int n, int K, const Kept& most, uint64_t* out) {
-    return pick<0>(sh, (n + NT - 1) / NT, K,
+    return pick<0, true>(sh, (n + NT - 1) / NT, K,
                    [&](int i) {
                        const int g = i * NT + threadIdx.x;
-                       return g < n ? comp_of(most.p[g], g) : 0;
+                       return g < n ? most.p[g] : 0;
                    },
-                   out);
+                   [&](int i) { return i * NT + threadIdx.x; }, out);
 }
 
 // The n groups' tokens, a lane's load of a group at a time, R of them a thread.
-template <typename L, int R> DEV int pick_tokens(const LpArgs& a, RowLds& sh, int n, const void* p) {
+template <typename L, int R, bool LEAN> DEV int pick_tokens(const LpArgs& a, RowLds& sh, int n, const void* p) {
     constexpr int VE = L::VE;
     uint32_t v[R][VE];
     int tok[R];
@@ -362,13 +390,21 @@ template <typename L, int R> DEV int pick_tokens(const LpArgs& a, RowLds& sh, in
 #pragma unroll
         for (int j = 0; j < VE; j++) v[i][j] = order_bits(x[j]);
     }
-    return pick<R * VE>(sh, R * VE, a.n_top, [&](int i) { return comp_of(v[i / VE][i % VE], tok[i / VE] + i % VE); }, sh.tokens);
+    return pick<R * VE, LEAN>(sh, R * VE, a.n_top, [&](int i) { return v[i / VE][i % VE]; },
+                        [&](int i) { return tok[i / VE] + i % VE; }, sh.tokens);
+}
+
+// Loads of a thread for the tokens of K groups: 1, 2 or 4.
+__host__ __device__ inline int loads_of(int K) {
+    static_assert(MAX_TOP * GL / NT == 4, "loads of all groups' tokens");
+    return K <= MAX_TOP / 4 ? 1 : K <= MAX_TOP / 2 ? 2 : 4;
 }
 
 // Everything about a row, once its sum and its groups' largest are known.
-// Its thread's first target was read before: tok0.
+// Its thread's first target was read before: tok0.  loads: loads_of(K).
 template <typename L, bool TOP, typename M>
-DEV void finish(const LpArgs& a, RowLds& sh, int row, const void* p, Sum s, float top, int tok0, const M& most) {
+DEV void finish(const LpArgs& a, RowLds& sh, int row, const void* p, Sum s, float top, int tok0, const M& most,
+                int loads) {
     const int t = threadIdx.x;
     auto logit = [&](int tok) { return (unsigned)tok < (unsigned)a.V ? L::one(p, tok) : NEG_INF; };
     const float x0 = logit(tok0);
@@ -407,28 +443,28 @@ DEV void finish(const LpArgs& a, RowLds& sh, int row, const void* p, Sum s, floa
         } else {
             // bundles of OVER groups first, by the same argument; 4 096 of them at most
             const int bundles = (a.groups + OVER - 1) / OVER;
-            uint64_t b[16];
+            uint32_t b[16];
 #pragma unroll 1
             for (int i = 0; i < 16; i++) {
                 const int at = i * NT + t;
                 uint32_t k = 0;
                 for (int g = at * OVER; g < min(a.groups, (at + 1) * OVER); g++) k = max(k, most.at(g));
-                b[i] = at < bundles ? comp_of(k, at) : 0;
+                b[i] = at < bundles ? k : 0;
             }
-            n = pick<16>(sh, 16, K, [&](int i) { return b[i]; }, sh.tokens);
-            uint64_t v[MAX_TOP * OVER / NT];
+            n = pick<16>(sh, 16, K, [&](int i) { return b[i]; }, [&](int i) { return i * NT + t; }, sh.tokens);
+            constexpr int RG = MAX_TOP * OVER / NT;
+            uint32_t v[RG];
+            auto of = [&](int i) {
+                const int e = i * NT + t;
+                return e < n * OVER ? (int)index_of(sh.tokens[e / OVER]) * OVER + e % OVER : a.groups;
+            };
 #pragma unroll
-            for (int i = 0; i < MAX_TOP * OVER / NT; i++) {
-                const int e = i * NT + t, g = e < n * OVER ? (int)index_of(sh.tokens[e / OVER]) * OVER + e % OVER : a.groups;
-                v[i] = g < a.groups ? comp_of(most.at(g), g) : 0;
-            }
-            n = pick<MAX_TOP * OVER / NT>(sh, MAX_TOP * OVER / NT, K, [&](int i) { return v[i]; }, sh.groups);
+            for (int i = 0; i < RG; i++) v[i] = of(i) < a.groups ? most.at(of(i)) : 0;
+            n = pick<RG>(sh, RG, K, [&](int i) { return v[i]; }, of, sh.groups);
         }
-        constexpr int LOADS = MAX_TOP * GL / NT;       // of a thread, for that many groups
-        static_assert(LOADS == 4, "as chosen from");
-        n = K <= MAX_TOP / 4   ? pick_tokens<L, 1>(a, sh, n, p)
-            : K <= MAX_TOP / 2 ? pick_tokens<L, 2>(a, sh, n, p)
-                               : pick_tokens<L, 4>(a, sh, n, p);
+        n = loads == 1   ? pick_tokens<L, 1, M::LEAN>(a, sh, n, p)
+            : loads == 2 ? pick_tokens<L, 2, M::LEAN>(a, sh, n, p)
+                         : pick_tokens<L, 4, M::LEAN>(a, sh, n, p);
         for (int i = t; i < K; i += NT) {
             const int64_t at = (int64_t)row * K + i;
             a.top[at] = i < n ? (int)index_of(sh.tokens[i]) : -1;
@@ -470,10 +506,14 @@ template <typename L, bool TOP> __global__ __launch_bounds__(NT) void k_lp_row(L
         top = fmaxf(top, v.w);
     }
     join(sh, s, top);
-    finish<L, TOP>(a, sh, row, (const typename L::e*)a.x + row * a.stride, s, top, tok, most);
+    finish<L, TOP>(a, sh, row, (const typename L::e*)a.x + row * a.stride, s, top, tok, most, loads_of(a.n_top));
 }
 
-template <typename L, bool TOP> __global__ __launch_bounds__(NT, 8) void k_lp_whole(LpArgs a) {
+// LOADS: loads_of(K), or 0 without alternatives; eight workgroups a CU as long as
+// their registers suffice (2 048 bf16 rows of 151 936 with 20 alternatives 130 us,
+// five a CU 147).
+template <typename L, int LOADS> __global__ __launch_bounds__(NT, LOADS == 4 ? 5 : 8) void k_lp_whole(LpArgs a) {
+    constexpr bool TOP = LOADS > 0;
     __shared__ RowLds sh;
     extern __shared__ uint32_t most[];
     const int row = blockIdx.x, tok = first_target(a, row);
@@ -482,7 +522,7 @@ template <typename L, bool TOP> __global__ __launch_bounds__(NT, 8) void k_lp_wh
     float top;
     scan<L, TOP>(p, 0, a.V, s, top, [&](int g, uint32_t k) { most[g] = k; });
     join(sh, s, top);
-    finish<L, TOP>(a, sh, row, p, s, top, tok, Kept{most});
+    finish<L, TOP>(a, sh, row, p, s, top, tok, Kept{most}, LOADS);
 }
 
 struct LpPlan {
@@ -515,7 +555,11 @@ LpPlan plan(int n, int V, int n_top, int VE) {
 
 template <typename L, bool TOP> void launch(const LpArgs& a, const LpPlan& pl, int n, hipStream_t st) {
     if (pl.whole) {
-        hipLaunchKernelGGL((k_lp_whole<L, TOP>), dim3(n), dim3(NT), pl.groups * 4, st, a);
+        const auto k = !TOP                     ? k_lp_whole<L, 0>
+                       : loads_of(a.n_top) == 1 ? k_lp_whole<L, 1>
+                       : loads_of(a.n_top) == 2 ? k_lp_whole<L, 2>
+                                                : k_lp_whole<L, 4>;
+        hipLaunchKernelGGL(k, dim3(n), dim3(NT), pl.groups * 4, st, a);
     } else {
         hipLaunchKernelGGL((k_lp_part<L, TOP>), dim3((unsigned)n * a.chunks), dim3(NT), 0, st, a);
         hipLaunchKernelGGL((k_lp_row<L, TOP>), dim3(n), dim3(NT), 0, st, a);

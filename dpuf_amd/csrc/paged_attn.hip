@@ -256,6 +256,7 @@ template <typename T, int HD, bool W> DEV void few_rows(const PaArgs& a, FewLds<
         const int first_limit = sq.ctx - sq.n + 16 * tile / a.G;      // of the tile's first row
         const int all = min(sq.ctx - sq.n + last / a.G + 1, sq.ctx);  // keys up to the last row's last
         const Run<W, 32> run(a, first_limit, all);
+        const bool one_place = first_limit + 1 == all;                // of all rows of the tile
         const int k0 = z * per, kend = min(all - run.gap, k0 + per);
 
         v8 qf[NC];
@@ -322,7 +323,18 @@ template <typename T, int HD, bool W> DEV void few_rows(const PaArgs& a, FewLds<
             for (int u = 0; u < 2; u++)
 #pragma unroll
                 for (int c = 0; c < NC; c++) *(u32x4*)(lv + (16 * u + col) * PITCH + 32 * c + 8 * g4) = vf[u][c];
-            if (!whole)
+            if (W && one_place) {
+                // what one row does not see none does: nothing of it is left
+                if (!whole)
+#pragma unroll
+                    for (int u = 0; u < 2; u++) {
+                        const int key = run.key(base) + 16 * u + col;
+                        if (key >= all || !in_window<W>(a, key, 1, all - 1) || (unsigned)pg[u] >= (unsigned)a.p.n_pages)
+#pragma unroll
+                            for (int c = 0; c < NC; c++)
+                                *(u32x4*)(lv + (16 * u + col) * PITCH + 32 * c + 8 * g4) = u32x4{0, 0, 0, 0};
+                    }
+            } else if (!whole) {
 #pragma unroll 1
                 for (int e = 0; e < 2 * NC; e++) {
                     u32x4* at = (u32x4*)(lv + (e / NC * 16 + col) * PITCH + 32 * (e % NC) + 8 * g4);
@@ -330,6 +342,7 @@ template <typename T, int HD, bool W> DEV void few_rows(const PaArgs& a, FewLds<
                     odd |= take_odd<T>(v);
                     *at = v;
                 }
+            }
             f32x4 sc[2] = {f32x4{0.f, 0.f, 0.f, 0.f}, f32x4{0.f, 0.f, 0.f, 0.f}};
 #pragma unroll
             for (int c = 0; c < NC; c++)
@@ -956,7 +969,10 @@ void window_ranges(PaPlan& r, const DpufAmdBatch& b, const DpufAmdPages& p, int 
 //
 // With a window the same, by the keys that a tile of rows sees: the first ones,
 // the window and as many more as the tile's rows are apart, in whole tiles of
-// keys; but the chunks' ranges by window_ranges.  (A window of 0 here is none.)
+// keys; but the chunks' ranges by window_ranges, and one range of up to 512 keys
+// of 64 columns (a window of 256, one row 8.1 us a call against 10.3 in two, of
+// 384 8.8 and 10.1; of 128 columns 10.6 and 10.3, 12.2 and 10.5).  (A window of
+// 0 here is none.)
 PaPlan plan(const DpufAmdBatch& b, const DpufAmdPages& p, int nq, int window, int sink) {
     const int G = nq / p.n_kv_heads;
     PaPlan r;
@@ -966,21 +982,22 @@ PaPlan plan(const DpufAmdBatch& b, const DpufAmdPages& p, int nq, int window, in
     // what reaches every key of the table needs no more than that
     r.window = window < cap && sink < cap ? window : (int)cap;
     r.sink = r.window < cap ? sink : 0;
-    const int64_t near = (int64_t)r.window + (r.sink + 63) / 64 * 64 + 64;
+    const int64_t near = (int64_t)r.window + (r.sink + 31) / 32 * 32 + 32;
     r.reach_few = (int)(near + 16 / G + 1 < cap ? near + 16 / G + 1 : cap);
     if (window && ctx > r.reach_few) ctx = r.reach_few;
     const int64_t packed = (int64_t)b.n_rows * G;
     r.only = b.n_rows <= b.n_seqs || packed <= r.few ? PA_FEW : b.n_seqs > 1 ? PA_BOTH
              : packed >= 384 && ctx >= 2048 && p.head_dim <= 128 ? PA_WIDE : PA_MANY;
     const int tr = r.only == PA_WIDE ? 256 : 128;
-    r.reach_many = (int)(near + tr / G + 1 < cap ? near + tr / G + 1 : cap);
+    const int64_t near_many = (int64_t)r.window + (r.sink + 63) / 64 * 64 + 64 + tr / G + 1;
+    r.reach_many = (int)(near_many < cap ? near_many : cap);
     const int64_t most = packed / (r.few + 1);
     r.y_few = r.only >= PA_MANY ? 0 : b.n_seqs * ((r.few + 15) / 16);
     r.y_many = r.only == PA_FEW ? 0 : r.only == PA_BOTH ? (int)(packed / 128 + (most < b.n_seqs ? most : b.n_seqs))
                                                         : ceil_div(packed, tr);
     const int64_t units = (int64_t)b.n_seqs * p.n_kv_heads;
     const int64_t even = (ctx * units / 256 + 127) & ~127, long_few = units >= 256 ? 1024 : 512;
-    const bool whole = ctx <= (units <= 64 ? 256 : 512);
+    const bool whole = ctx <= (units <= 64 && !(window && p.head_dim == 64) ? 256 : 512);
     r.chunk_few = whole || even > long_few ? (int)long_few : even < 128 ? 128 : (int)even;
     r.nz_few = ceil_div(ctx, r.chunk_few);
     if (r.nz_few > 64) r.nz_few = 64;

@@ -993,9 +993,12 @@ void dpuf_hip_rope_append(void* s, const DpufAmdBatch* b, const DpufAmdPages* p,
     a.eps = eps;
     a.q_out = (uint16_t*)q_out;
     // a row's heads by one workgroup, or spread over several while the rows
-    // alone do not give every CU one
+    // alone do not give every CU two (256 rows of 32 heads and 8 + 8 of 128, three
+    // turns a row: 8.0 us by two workgroups a row against 8.9 by one, 64 6.6 by
+    // three and 8.3, 512 9.8 and 10.3, but bf16 ones without norms 8.3 and 8.0)
     const int groups = 256 / (p->head_dim / 8), turns = (nq + 2 * p->n_kv_heads + groups - 1) / groups;
-    int y = (dpuf_hip_cu_count() + b->n_rows - 1) / b->n_rows;
+    int y = 2 * dpuf_hip_cu_count() / b->n_rows;
+    if (y < 1) y = 1;
     if (y > turns) y = turns;
     const dim3 g(b->n_rows, y);
     AxArgs ax = {};
