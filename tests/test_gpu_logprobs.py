@@ -211,7 +211,7 @@ def test_alternatives_that_crowd(eng, hip, t):
         run(eng, hip, x, t, rng.integers(0, V, (6, 1)), k)
 
 
-@pytest.mark.parametrize("t,V", [(R.F32, (1 << 20) + 3), (R.F16, (1 << 21) + 5), (R.F32, 1 << 24), (R.BF16, 1 << 24)])
+@pytest.mark.parametrize("t,V", [(R.F32, 300001), (R.BF16, 400003), (R.F32, 1 << 19), (R.F32, (1 << 20) + 3), (R.F16, (1 << 21) + 5), (R.F32, 1 << 24), (R.BF16, 1 << 24)])
 def test_large_vocabularies(eng, hip, t, V):
     rng = np.random.default_rng(10)
     x = rng.standard_normal((1, V)).astype(F)
@@ -233,6 +233,23 @@ def test_many_rows(eng, hip, n, V, k):
     p = np.exp((x - x.max(1, keepdims=True)).astype(np.float64))
     lp = np.log(np.take_along_axis(p, targets, 1) / p.sum(1, keepdims=True))
     assert np.all(np.abs(got[0] - lp) < 1e-4)
+
+
+@pytest.mark.parametrize("t,n,V,k", [(R.F32, 300, 20001, 20), (R.BF16, 256, 65536, 64), (R.F16, 384, 70001, 5),
+                                     (R.BF16, 390, 151936, 20), (R.F32, 255, 20001, 33), (R.F32, 383, 70000, 0)])
+def test_rows_that_a_workgroup_each_takes(eng, hip, t, n, V, k):
+    """Around the numbers of rows from which a row is not cut; a thousand
+    targets and more than a workgroup's threads."""
+    rng = np.random.default_rng(n + V)
+    x = (rng.standard_normal((n, V), np.float32) * 3).astype(F)
+    x[1] = -np.inf
+    x[2, ::2] = np.nan
+    x[3] = 1e9
+    say(f"logprobs: {n} rows of {V}, type {t}, {k} alternatives")
+    targets = rng.integers(-1, V + 1, (n, 1024 if n < 300 else 257))
+    got = run(eng, hip, x, t, targets, k, want=False)
+    some = np.unique(np.concatenate([rng.integers(0, n, 8), [0, 1, 2, 3, n - 1]]))
+    check(R.from_type(R.to_type(x[some], t), t).reshape(len(some), V), targets[some], k, [g[some] for g in got])
 
 
 def test_flat_and_sharp_rows(eng, hip):

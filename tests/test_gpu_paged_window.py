@@ -147,6 +147,32 @@ def test_kernels_and_splits(eng, hip, mode, hd):
     check(cache, 8, q, 0.1, out, lse, R.F32 if hd == 256 else t, window, sink)
 
 
+@pytest.mark.parametrize("max_ctx", [1, 600, 100000])
+@pytest.mark.parametrize("mode", ["few, split", "many, split", "wide, split", "mixed", "mixed, split"])
+def test_estimates_of_the_longest_context(eng, hip, mode, max_ctx):
+    """Keys are split by what the windows leave, whatever the caller's estimate
+    of the longest context is."""
+    rows, ctx, _, window, sink = MODES[mode]
+    rng = np.random.default_rng(len(mode) + max_ctx)
+    cache = R.Cache(hip, rng, R.BF16, rows, ctx, 2, 64, 16, table_extra=6000)
+    q = R.to_type(rng.standard_normal((cache.n_rows, 8, 64)) * 1.5, R.BF16)
+    say(f"estimates: {mode}, max_ctx {max_ctx}")
+    out, lse, _ = call(eng, hip, cache, 8, q, 0.1, window, sink, max_ctx=max_ctx, extra=2)
+    check(cache, 8, q, 0.1, out, lse, R.BF16, window, sink)
+
+
+@pytest.mark.parametrize("rows", [1, 3])
+def test_hundreds_of_sequences(eng, hip, rows):
+    rng = np.random.default_rng(rows)
+    n = 300
+    ctx = [int(c) for c in rng.integers(rows, 90, n)]
+    cache = R.Cache(hip, rng, R.BF16, [rows if i % 7 else 0 for i in range(n)], ctx, 1, 64, 16)
+    q = R.to_type(rng.standard_normal((cache.n_rows, 4, 64)) * 1.5, R.BF16)
+    say(f"{n} sequences of {rows} rows")
+    out, lse, _ = call(eng, hip, cache, 4, q, 0.125, 20, 3, extra=5)
+    check(cache, 4, q, 0.125, out, lse, R.BF16, 20, 3)
+
+
 @pytest.mark.parametrize("mode", MODES)
 def test_pages_outside_every_window_may_be_anything(eng, hip, mode):
     """Tables whose other entries are gone, another sequence's or no page at
