@@ -525,10 +525,12 @@ DEV void many_rows(const PaArgs& a, ManyLds<HD>& sh, int kvh, int tile, int z) {
     const int col = lane & 31, h = lane >> 5;
     // sequence of the tile, and its tile there, among the sequences with many rows
     int s = -1;
+    PgSeq sq = {};
     for (int s0 = 0; s0 < a.b.n_seqs && s < 0; s0 += 64) {
         int n = 0;
+        PgSeq t = {};
         if (s0 + lane < a.b.n_seqs) {
-            const PgSeq t = pg_seq(a.b, a.shift, s0 + lane);
+            t = pg_seq(a.b, a.shift, s0 + lane);
             const int rows = t.n * a.G;
             n = rows > a.few || a.only != PA_BOTH ? (rows + TR - 1) / TR : 0;
         }
@@ -542,6 +544,7 @@ DEV void many_rows(const PaArgs& a, ManyLds<HD>& sh, int kvh, int tile, int z) {
             const int at = __ffsll((unsigned long long)past) - 1;
             tile -= __shfl(sum - n, at);
             s = s0 + at;
+            sq = PgSeq{__shfl(t.r0, at), __shfl(t.n, at), __shfl(t.ctx, at)};
         } else {
             tile -= __shfl(sum, 63);
         }
@@ -549,7 +552,7 @@ DEV void many_rows(const PaArgs& a, ManyLds<HD>& sh, int kvh, int tile, int z) {
     s = __builtin_amdgcn_readfirstlane(s);
     tile = __builtin_amdgcn_readfirstlane(tile);
     if (s < 0) return;
-    const PgSeq sq = scalar(pg_seq(a.b, a.shift, s));
+    sq = scalar(sq);
     const int rows = sq.n * a.G;
     const int span = span_of<W>(a, sq.ctx, false);
     const int per = range_keys(span, a.chunk_many, a.nz_many);
