@@ -21,6 +21,12 @@
 //   k_lp_row    a workgroup per row: joins the chunks, picks the k groups, the k
 //               tokens among theirs, and writes;
 //   k_lp_whole  both, a workgroup per row, where there are many rows.
+//
+// Bound by the bytes of the logits, in 16 bits nearly as much by the exponential
+// and ten other instructions of each: 512 rows of 151 936 fp32 logits 54 us, 5.7
+// TB/s, 2 048 in bf16 with 20 alternatives 135 us, 4.6 TB/s.  Few rows are bound
+// by latency: one with 20 alternatives 3.8 us (38 workgroups) and 7.0, of which
+// 1.0 are the first loads, 0.8 the sums, 2.2 each pick and 0.8 what it reads.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
@@ -157,7 +163,8 @@ struct RowLds {
     Sum ss[NW];
     float sm[NW];
     unsigned n;
-    uint32_t __attribute__((aligned(16))) quad[64];
+    uint32_t __attribute__((aligned(16))) most[NT];
+    uint32_t bound;
     uint64_t __attribute__((aligned(16))) list[LISTED];
     uint64_t best[NW];
     uint64_t groups[MAX_TOP], tokens[MAX_TOP];
@@ -239,40 +246,33 @@ template <typename L, bool TOP, typename F> DEV void scan(const void* p, int lo,
     }
 }
 
-// The K largest of the threads' items, first by bits, then by the lower index,
-// largest first, into out (as comp_of).  A thread has n items (R of them, in
-// registers, or with R 0 n, wherever they are): bits(i), 0 for none, of index
-// id(i).  Returns how many there are, K at most.  A bound first: the K-th largest
-// of the largest of 64 quads of threads, which at least K items reach; those that
-// do are listed and ranked.
-// LEAN: in few registers.
-template <int R, bool LEAN = false, typename F, typename G>
-DEV int pick(RowLds& sh, int n, int K, F bits, G id, uint64_t* out) {
-    const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
-    // f(bits, i) of a thread's items
-    auto each = [&](auto f) {
-        if constexpr (R > 0) {
-#pragma unroll
-            for (int i = 0; i < R; i++) f(bits(i), i);
-        } else {
-            for (int i = 0; i < n; i++) f(bits(i), i);
-        }
-    };
+// A number that at least K of the threads' items reach, and not many more: the
+// K-th largest of the largest of 64 quads of threads, or, where MANY may be asked
+// for, of the threads.  f(key) for each item; 0 is none, and 1 the least bound.
+template <bool LEAN, bool MANY, typename F> DEV uint32_t bound_of(RowLds& sh, int K, F each) {
+    const int t = threadIdx.x, lane = t & 63;
     uint32_t b = 0;
     each([&](uint32_t k, int) { b = max(b, k); });
-    b = max(b, dpp<0xB1>(b));      // lanes 1 0 3 2
-    b = max(b, dpp<0x4E>(b));      // lanes 2 3 0 1
-    if ((t & 3) == 0) sh.quad[t >> 2] = b;
-    if (t == 0) sh.n = 0;
+    if (!MANY) {
+        b = max(b, dpp<0xB1>(b));      // lanes 1 0 3 2
+        b = max(b, dpp<0x4E>(b));      // lanes 2 3 0 1
+        if ((t & 3) == 0) sh.most[t >> 2] = b;
+    } else {
+        sh.most[t] = b;
+    }
+    if (t == 0) {
+        sh.n = 0;
+        sh.bound = ~0u;
+    }
     __syncthreads();
-    const uint32_t mine = sh.quad[lane];
+    const uint32_t mine = MANY ? b : sh.most[lane];
     int above = 0;
     constexpr int AT_ONCE = LEAN ? 16 : 64;
 #pragma unroll 1
-    for (int i0 = 0; i0 < 64; i0 += AT_ONCE)
+    for (int i0 = 0; i0 < (MANY ? NT : 64); i0 += AT_ONCE)
 #pragma unroll
         for (int i = i0; i < i0 + AT_ONCE; i += 4) {
-            const u32x4 q = *(const u32x4*)&sh.quad[i];
+            const u32x4 q = *(const u32x4*)&sh.most[i];
 #pragma unroll
             for (int e = 0; e < 4; e++) above += q[e] > mine;
         }
@@ -281,25 +281,67 @@ DEV int pick(RowLds& sh, int n, int K, F bits, G id, uint64_t* out) {
     bound = min(bound, dpp<0x124>(bound));
     bound = min(bound, dpp<0x122>(bound));
     bound = min(bound, dpp<0x121>(bound));
-    bound = min(min((uint32_t)__builtin_amdgcn_readlane((int)bound, 0), (uint32_t)__builtin_amdgcn_readlane((int)bound, 16)),
-                min((uint32_t)__builtin_amdgcn_readlane((int)bound, 32), (uint32_t)__builtin_amdgcn_readlane((int)bound, 48)));
-    bound = max(bound, 1u);
-    // a wave's items side by side, each round's by lane
-    int hits = 0;
-    each([&](uint32_t k, int) { hits += __popcll(__ballot(k >= bound)); });
-    if (hits) {
-        int e = lane == 0 ? (int)atomicAdd(&sh.n, (unsigned)hits) : 0;
-        e = __builtin_amdgcn_readfirstlane(e);
-        each([&](uint32_t k, int i) {
-            const uint64_t hit = __ballot(k >= bound);
-            const int at = e + (int)__builtin_amdgcn_mbcnt_hi((uint32_t)(hit >> 32),
-                                                              __builtin_amdgcn_mbcnt_lo((uint32_t)hit, 0));
-            if (k >= bound && at < LISTED) sh.list[at] = comp_of(k, id(i));
-            e += __popcll(hit);
-        });
+    auto row = [&](int l) { return (uint32_t)__builtin_amdgcn_readlane((int)bound, l); };
+    bound = min(min(row(0), row(16)), min(row(32), row(48)));
+    if (MANY) {
+        if (lane == 0) atomicMin(&sh.bound, bound);
+        __syncthreads();
+        bound = sh.bound;
     }
-    __syncthreads();
-    const int listed = sh.n, found = min(listed, K);
+    return max(bound, 1u);
+}
+
+// The K largest of the threads' items, first by bits, then by the lower index,
+// largest first, into out (as comp_of).  A thread has n items (R of them, in
+// registers, or with R 0 n, wherever they are): bits(i), 0 for none, of index
+// id(i).  Returns how many there are, K at most.  What reaches a bound is listed
+// and ranked.  LEAN: in few registers.  MANY: K may be more than 32.  A row of
+// 151 936 random logits takes 17 us with 64 of them, 11.3 with 20; 64 by the
+// quads' bound 21.7 (bf16 31.7), and 20 by the threads' 11.7.
+template <int R, bool LEAN, bool MANY, typename F, typename G>
+DEV int pick(RowLds& sh, int n, int K, F bits, G id, uint64_t* out) {
+    const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
+    // f(item) of a thread's items
+    auto items = [&](auto f) {
+        if constexpr (R > 0) {
+#pragma unroll
+            for (int i = 0; i < R; i++) f(i);
+        } else {
+            for (int i = 0; i < n; i++) f(i);
+        }
+    };
+    // lists the items whose key reaches the bound, a wave's side by side, each round's by lane
+    auto list = [&](uint32_t bound, auto key) {
+        int hits = 0;
+        items([&](int i) { hits += __popcll(__ballot(key(i) >= bound)); });
+        if (hits) {
+            int e = lane == 0 ? (int)atomicAdd(&sh.n, (unsigned)hits) : 0;
+            e = __builtin_amdgcn_readfirstlane(e);
+            items([&](int i) {
+                const bool in = key(i) >= bound;
+                const uint64_t hit = __ballot(in);
+                const int at = e + (int)__builtin_amdgcn_mbcnt_hi((uint32_t)(hit >> 32),
+                                                                  __builtin_amdgcn_mbcnt_lo((uint32_t)hit, 0));
+                if (in && at < LISTED) sh.list[at] = comp_of(bits(i), id(i));
+                e += __popcll(hit);
+            });
+        }
+        __syncthreads();
+        return (int)sh.n;
+    };
+    const uint32_t bound = bound_of<LEAN, MANY>(sh, K, [&](auto f) { items([&](int i) { f(bits(i), i); }); });
+    int listed = list(bound, bits);
+    const int found = min(listed, K);
+    if (MANY && listed > LISTED) {
+        // long runs of equal ones: of those on the bound the lowest indices
+        auto key = [&](int i) {
+            const uint32_t k = bits(i);
+            return k > bound ? ~0u : k == bound ? ~(uint32_t)id(i) : 0u;
+        };
+        __syncthreads();
+        const uint32_t least = bound_of<LEAN, MANY>(sh, K, [&](auto f) { items([&](int i) { f(key(i), i); }); });
+        listed = list(least, key);
+    }
     if (listed <= LISTED) {
         for (int i = t; i < listed; i += NT) {
             const uint64_t k = sh.list[i];
@@ -314,12 +356,12 @@ DEV int pick(RowLds& sh, int n, int K, F bits, G id, uint64_t* out) {
             if (r < K) out[r] = k;
         }
     } else {
-        // too many reach the bound (long runs of equal ones, or all with few of the threads): one at a time
+        // too many (long runs of equal ones, or they lie with few of the threads): one at a time
         uint64_t last = ~0ull;
         for (int r = 0; r < K; r++) {
             uint64_t m = 0;
-            each([&](uint32_t k, int i) {
-                const uint64_t c = comp_of(k, id(i));
+            items([&](int i) {
+                const uint64_t c = comp_of(bits(i), id(i));
                 m = c < last ? max64(m, c) : m;
             });
 #pragma unroll
@@ -352,7 +394,7 @@ struct Kept {
     const uint32_t* p;
     DEV uint32_t at(int g) const { return p[g]; }
 };
-template <int R> DEV int pick_stored(RowLds& sh, int n, int K, const Stored& most, uint64_t* out) {
+template <int R, bool MANY> DEV int pick_stored(RowLds& sh, int n, int K, const Stored& most, uint64_t* out) {
     uint32_t v[R];
 #pragma unroll
     for (int i = 0; i < R; i++) {
@@ -360,15 +402,15 @@ template <int R> DEV int pick_stored(RowLds& sh, int n, int K, const Stored& mos
         v[i] = R <= FEW ? most.early[i % FEW] : most.p[min(g, n - 1)];
         if (g >= n) v[i] = 0;
     }
-    return pick<R>(sh, R, K, [&](int i) { return v[i]; }, [&](int i) { return i * NT + threadIdx.x; }, out);
+    return pick<R, false, MANY>(sh, R, K, [&](int i) { return v[i]; }, [&](int i) { return i * NT + threadIdx.x; }, out);
 }
-DEV int pick_groups(RowLds& sh, int n, int K, const Stored& most, uint64_t* out) {
-    return n <= NT * FEW / 2 ? pick_stored<FEW / 2>(sh, n, K, most, out)
-           : n <= NT * FEW   ? pick_stored<FEW>(sh, n, K, most, out)
-                             : pick_stored<MOST>(sh, n, K, most, out);
+template <bool MANY> DEV int pick_groups(RowLds& sh, int n, int K, const Stored& most, uint64_t* out) {
+    return n <= NT * FEW / 2 ? pick_stored<FEW / 2, MANY>(sh, n, K, most, out)
+           : n <= NT * FEW   ? pick_stored<FEW, MANY>(sh, n, K, most, out)
+                             : pick_stored<MOST, MANY>(sh, n, K, most, out);
 }
-DEV int pick_groups(RowLds& sh, int n, int K, const Kept& most, uint64_t* out) {
-    return pick<0, true>(sh, (n + NT - 1) / NT, K,
+template <bool MANY> DEV int pick_groups(RowLds& sh, int n, int K, const Kept& most, uint64_t* out) {
+    return pick<0, true, MANY>(sh, (n + NT - 1) / NT, K,
                    [&](int i) {
                        const int g = i * NT + threadIdx.x;
                        return g < n ? most.p[g] : 0;
@@ -390,7 +432,7 @@ template <typename L, int R, bool LEAN> DEV int pick_tokens(const LpArgs& a, Row
 #pragma unroll
         for (int j = 0; j < VE; j++) v[i][j] = order_bits(x[j]);
     }
-    return pick<R * VE, LEAN>(sh, R * VE, a.n_top, [&](int i) { return v[i / VE][i % VE]; },
+    return pick<R * VE, LEAN, (R > 2)>(sh, R * VE, a.n_top, [&](int i) { return v[i / VE][i % VE]; },
                         [&](int i) { return tok[i / VE] + i % VE; }, sh.tokens);
 }
 
@@ -401,10 +443,11 @@ __host__ __device__ inline int loads_of(int K) {
 }
 
 // Everything about a row, once its sum and its groups' largest are known.
-// Its thread's first target was read before: tok0.  loads: loads_of(K).
-template <typename L, bool TOP, typename M>
-DEV void finish(const LpArgs& a, RowLds& sh, int row, const void* p, Sum s, float top, int tok0, const M& most,
-                int loads) {
+// Its thread's first target was read before: tok0.  LOADS: loads_of(K), or 0
+// without alternatives.
+template <typename L, int LOADS, typename M>
+DEV void finish(const LpArgs& a, RowLds& sh, int row, const void* p, Sum s, float top, int tok0, const M& most) {
+    constexpr bool MANY = LOADS == 4;
     const int t = threadIdx.x;
     auto logit = [&](int tok) { return (unsigned)tok < (unsigned)a.V ? L::one(p, tok) : NEG_INF; };
     const float x0 = logit(tok0);
@@ -435,11 +478,11 @@ DEV void finish(const LpArgs& a, RowLds& sh, int row, const void* p, Sum s, floa
         return d > -1e30f ? (d - log_l) * LN2 : x - top;
     };
     if (t == 0 && a.entropy) a.entropy[row] = top > NEG_INF ? fmaxf((log_l - s.u / s.l) * LN2, 0.0f) : 0.0f;
-    if constexpr (TOP) {
+    if constexpr (LOADS > 0) {
         const int K = a.n_top;
         int n;
         if (a.groups <= DIRECT) {
-            n = pick_groups(sh, a.groups, K, most, sh.groups);
+            n = pick_groups<MANY>(sh, a.groups, K, most, sh.groups);
         } else {
             // bundles of OVER groups first, by the same argument; 4 096 of them at most
             const int bundles = (a.groups + OVER - 1) / OVER;
@@ -451,7 +494,7 @@ DEV void finish(const LpArgs& a, RowLds& sh, int row, const void* p, Sum s, floa
                 for (int g = at * OVER; g < min(a.groups, (at + 1) * OVER); g++) k = max(k, most.at(g));
                 b[i] = at < bundles ? k : 0;
             }
-            n = pick<16>(sh, 16, K, [&](int i) { return b[i]; }, [&](int i) { return i * NT + t; }, sh.tokens);
+            n = pick<16, false, MANY>(sh, 16, K, [&](int i) { return b[i]; }, [&](int i) { return i * NT + t; }, sh.tokens);
             constexpr int RG = MAX_TOP * OVER / NT;
             uint32_t v[RG];
             auto of = [&](int i) {
@@ -460,11 +503,9 @@ DEV void finish(const LpArgs& a, RowLds& sh, int row, const void* p, Sum s, floa
             };
 #pragma unroll
             for (int i = 0; i < RG; i++) v[i] = of(i) < a.groups ? most.at(of(i)) : 0;
-            n = pick<RG>(sh, RG, K, [&](int i) { return v[i]; }, of, sh.groups);
+            n = pick<RG, false, MANY>(sh, RG, K, [&](int i) { return v[i]; }, of, sh.groups);
         }
-        n = loads == 1   ? pick_tokens<L, 1, M::LEAN>(a, sh, n, p)
-            : loads == 2 ? pick_tokens<L, 2, M::LEAN>(a, sh, n, p)
-                         : pick_tokens<L, 4, M::LEAN>(a, sh, n, p);
+        n = pick_tokens<L, LOADS, M::LEAN>(a, sh, n, p);
         for (int i = t; i < K; i += NT) {
             const int64_t at = (int64_t)row * K + i;
             a.top[at] = i < n ? (int)index_of(sh.tokens[i]) : -1;
@@ -494,7 +535,8 @@ DEV int first_target(const LpArgs& a, int row) {
     return t < a.n_targets ? a.targets[(int64_t)row * a.n_targets + t] : -1;
 }
 
-template <typename L, bool TOP> __global__ __launch_bounds__(NT) void k_lp_row(LpArgs a) {
+template <typename L, int LOADS> __global__ __launch_bounds__(NT) void k_lp_row(LpArgs a) {
+    constexpr bool TOP = LOADS > 0;
     __shared__ RowLds sh;
     const int row = blockIdx.x, tok = first_target(a, row);
     const Stored most(TOP ? a.most + (size_t)row * a.groups : (const uint32_t*)a.part, TOP ? a.groups : 1);
@@ -506,10 +548,10 @@ template <typename L, bool TOP> __global__ __launch_bounds__(NT) void k_lp_row(L
         top = fmaxf(top, v.w);
     }
     join(sh, s, top);
-    finish<L, TOP>(a, sh, row, (const typename L::e*)a.x + row * a.stride, s, top, tok, most, loads_of(a.n_top));
+    finish<L, LOADS>(a, sh, row, (const typename L::e*)a.x + row * a.stride, s, top, tok, most);
 }
 
-// LOADS: loads_of(K), or 0 without alternatives; eight workgroups a CU as long as
+// Eight workgroups a CU as long as
 // their registers suffice (2 048 bf16 rows of 151 936 with 20 alternatives 130 us,
 // five a CU 147).
 template <typename L, int LOADS> __global__ __launch_bounds__(NT, LOADS == 4 ? 5 : 8) void k_lp_whole(LpArgs a) {
@@ -522,7 +564,7 @@ template <typename L, int LOADS> __global__ __launch_bounds__(NT, LOADS == 4 ? 5
     float top;
     scan<L, TOP>(p, 0, a.V, s, top, [&](int g, uint32_t k) { most[g] = k; });
     join(sh, s, top);
-    finish<L, TOP>(a, sh, row, p, s, top, tok, Kept{most}, LOADS);
+    finish<L, LOADS>(a, sh, row, p, s, top, tok, Kept{most});
 }
 
 struct LpPlan {
@@ -553,16 +595,12 @@ LpPlan plan(int n, int V, int n_top, int VE) {
     return p;
 }
 
-template <typename L, bool TOP> void launch(const LpArgs& a, const LpPlan& pl, int n, hipStream_t st) {
+template <typename L, int LOADS> void launch(const LpArgs& a, const LpPlan& pl, int n, hipStream_t st) {
     if (pl.whole) {
-        const auto k = !TOP                     ? k_lp_whole<L, 0>
-                       : loads_of(a.n_top) == 1 ? k_lp_whole<L, 1>
-                       : loads_of(a.n_top) == 2 ? k_lp_whole<L, 2>
-                                                : k_lp_whole<L, 4>;
-        hipLaunchKernelGGL(k, dim3(n), dim3(NT), pl.groups * 4, st, a);
+        hipLaunchKernelGGL((k_lp_whole<L, LOADS>), dim3(n), dim3(NT), pl.groups * 4, st, a);
     } else {
-        hipLaunchKernelGGL((k_lp_part<L, TOP>), dim3((unsigned)n * a.chunks), dim3(NT), 0, st, a);
-        hipLaunchKernelGGL((k_lp_row<L, TOP>), dim3(n), dim3(NT), 0, st, a);
+        hipLaunchKernelGGL((k_lp_part<L, (LOADS > 0)>), dim3((unsigned)n * a.chunks), dim3(NT), 0, st, a);
+        hipLaunchKernelGGL((k_lp_row<L, LOADS>), dim3(n), dim3(NT), 0, st, a);
     }
     LAUNCHED("k_lp");
 }
@@ -599,7 +637,9 @@ void dpuf_hip_logprobs(void* s, int32_t type, int32_t n, int32_t V, int64_t stri
     a.most = (uint32_t*)((char*)ws + pl.most);
     auto go = [&](auto type_) {
         typedef decltype(type_) L;
-        n_top ? launch<L, true>(a, pl, n, ST(s)) : launch<L, false>(a, pl, n, ST(s));
+        const int loads = n_top ? loads_of(n_top) : 0;
+        const auto f = loads == 0 ? launch<L, 0> : loads == 1 ? launch<L, 1> : loads == 2 ? launch<L, 2> : launch<L, 4>;
+        f(a, pl, n, ST(s));
     };
     if (type == DPUF_AMD_F32) go(F32L());
     else if (type == DPUF_AMD_BF16) go(H16L<Bf16>());

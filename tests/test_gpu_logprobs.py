@@ -143,6 +143,34 @@ def test_ties(eng, hip, V):
             run(eng, hip, x, t, rng.integers(0, V, (8, 2)), k)
 
 
+@pytest.mark.parametrize("k", [32, 33, 64])
+@pytest.mark.parametrize("t", [R.F32, R.BF16])
+def test_long_runs_of_equal_logits(eng, hip, t, k):
+    """More equal ones than a workgroup lists: with fewer larger ones than
+    alternatives, a few distinct values, all that is left after a mask, and what
+    lies with few of the threads; rows cut and not."""
+    rng = np.random.default_rng(k)
+    V = 70001
+    x = np.zeros((8, V), F)
+    x[1, rng.permutation(V)[:k - 1]] = 2 + rng.integers(0, 4, k - 1)
+    x[2] = rng.integers(-2, 3, V)
+    x[3, :V // 2] = -np.inf
+    x[4] = -np.inf
+    x[4, V - 5000:] = 0.5
+    x[5] = np.nan
+    x[5, 4096:4096 + 2000] = -1.0
+    x[6, V - 40:] = 1.0
+    x[7] = np.where(np.arange(V) % 1024 < 64, 3.0, 0.0)
+    targets = rng.integers(0, V, (8, 2))
+    say(f"long runs of equal logits: {k} alternatives, type {t}")
+    run(eng, hip, x, t, targets, k)
+    rows = np.arange(400) % 8
+    got = run(eng, hip, x[rows], t, targets[rows], k, want=False)
+    check(R.from_type(R.to_type(x, t), t).reshape(x.shape), targets, k, [g[:8] for g in got])
+    for g in got:
+        assert np.array_equal(g.view(np.uint32), g[rows].view(np.uint32))
+
+
 def test_masked_and_odd_logits(eng, hip):
     """-infinity (a grammar's mask), NaN, +infinity, rows that leave nothing,
     the lowest finite value as a mask, huge values."""
