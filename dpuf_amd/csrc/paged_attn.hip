@@ -44,6 +44,11 @@
 // one run, in which a key behind the first ones is `gap` before its place; the
 // keys of those tiles that a row does not see are masked like those behind its
 // last.  A sequence's keys are split by that run's length, not by its context.
+// 48 single rows of 32 heads, 8 kv heads of 128 over 310 to 30 000 keys with a
+// window of 2 048: 79 us, 4.9 TB/s; 512 rows over 16 384 with one of 4 096: 57 us,
+// 600 TFLOP/s (of the kernel's 49 to 55 us 40 are steps, the rest the way to the
+// first and from the last); eight chunks of 64 rows with one of 128, 8 heads of 64
+// a kv head: 12 us, all but 4 of them latency around the steps.
 //
 // A window may hold few keys, one of which has most of the weight, and then o is
 // nearly that key's v, but for the rounding of its p.  So where p is rounded once
