@@ -24,7 +24,7 @@
 //
 // Bound by the bytes of the logits, in 16 bits nearly as much by the exponential
 // and ten other instructions of each: 512 rows of 151 936 fp32 logits 54 us, 5.7
-// TB/s, 2 048 in bf16 with 20 alternatives 135 us, 4.6 TB/s.  Few rows are bound
+// TB/s, 2 048 in bf16 with 20 alternatives 127 us, 4.9 TB/s.  Few rows are bound
 // by latency: one with 20 alternatives 3.8 us (38 workgroups) and 7.0, of which
 // 1.0 are the first loads, 0.8 the sums, 2.2 each pick and 0.8 what it reads.
 #include <hip/hip_runtime.h>
@@ -40,6 +40,7 @@ constexpr int NW = NT / 64;
 constexpr int GL = 16;               // lanes of a group: a row of the wave
 constexpr int FEW = 10, MOST = 32;   // groups a thread picks from
 constexpr int DIRECT = NT * MOST;    // groups that are picked from as they are
+constexpr int WHOLE = DIRECT * GL * 4;  // tokens of a row that is not cut, of any type, at most
 constexpr int OVER = 64;             // groups of a bundle, where there are more
 constexpr int LISTED = 1024;         // candidates that are ranked
 constexpr int MAX_TOP = DPUF_AMD_LOGPROBS_MAX_TOP;
@@ -481,7 +482,7 @@ DEV void finish(const LpArgs& a, RowLds& sh, int row, const void* p, Sum s, floa
     if constexpr (LOADS > 0) {
         const int K = a.n_top;
         int n;
-        if (a.groups <= DIRECT) {
+        if (M::LEAN || a.groups <= DIRECT) {
             n = pick_groups<MANY>(sh, a.groups, K, most, sh.groups);
         } else {
             // bundles of OVER groups first, by the same argument; 4 096 of them at most
@@ -551,10 +552,11 @@ template <typename L, int LOADS> __global__ __launch_bounds__(NT) void k_lp_row(
     finish<L, LOADS>(a, sh, row, (const typename L::e*)a.x + row * a.stride, s, top, tok, most);
 }
 
-// Eight workgroups a CU as long as
-// their registers suffice (2 048 bf16 rows of 151 936 with 20 alternatives 130 us,
-// five a CU 147).
-template <typename L, int LOADS> __global__ __launch_bounds__(NT, LOADS == 4 ? 5 : 8) void k_lp_whole(LpArgs a) {
+// Eight workgroups a CU as long as their registers suffice: 2 048 bf16 rows of
+// 151 936 with 20 alternatives 127 us, five a CU 147.  More than 32 alternatives
+// take more of them, and none may go to memory.
+template <typename L, int LOADS>
+__global__ __launch_bounds__(NT, LOADS < 4 ? 8 : L::VE < 8 ? 7 : 4) void k_lp_whole(LpArgs a) {
     constexpr bool TOP = LOADS > 0;
     __shared__ RowLds sh;
     extern __shared__ uint32_t most[];
@@ -585,7 +587,7 @@ struct LpPlan {
 LpPlan plan(int n, int V, int n_top, int VE) {
     LpPlan p;
     p.groups = n_top ? (V + GL * VE - 1) / (GL * VE) : 0;
-    p.whole = V <= 16384 || (V <= 1 << 19 && n >= (V <= 65536 ? 256 : 384));
+    p.whole = V <= 16384 || (V <= WHOLE && n >= (V <= 65536 ? 256 : 384));
     int c = (2048 + n - 1) / n;
     if (c < (V + 32767) / 32768) c = (V + 32767) / 32768;
     p.chunk = ((V + c - 1) / c + 4095) / 4096 * 4096;
