@@ -1036,8 +1036,8 @@ static int32_t window_of(const Engine* e, int32_t l) { return e->pg_window ? e->
 static void enqueue_paged_attention(Engine* e, int32_t l, float scale, float eps) {
     void* s = e->stream;
     const DpufAmdPages p = pages_of(e, l);
-    dpuf_hip_rope_append(s, &e->pg_b, &p, &e->pg_rope, NULL, e->pg_pos, 0, DPUF_AMD_F32, e->nq, e->q, e->k, e->v, e->qd, e->kvd,
-                         e->kvd, e->d_norm[4 * l + 1], e->d_norm[4 * l + 2], eps, e->pg_q);
+    dpuf_hip_rope_append(s, &e->pg_b, &p, &e->pg_rope, NULL, e->pg_pos, 0, DPUF_AMD_F32, e->nq, e->q, e->k, e->v,
+                         e->qd, e->kvd, e->kvd, e->d_norm[4 * l + 1], e->d_norm[4 * l + 2], eps, e->pg_q);
     dpuf_hip_paged_attn(s, &e->pg_b, &p, e->nq, e->pg_q, scale, window_of(e, l), e->pg_sink, 1, e->ao, e->pg_lse,
                         e->pg_ws);
     if (e->pg_decay >= 0.0f)

@@ -303,12 +303,11 @@ int32_t dpuf_hip_device_enter(int32_t dev);
 void dpuf_hip_device_leave(int32_t back);
 
 /* The paged-serving operators behind include/dpuf_amd.h's entry points of the
- * same names, whose arguments have been checked. */
-/* x NULL: one axis. */
+ * same names, whose arguments have been checked.  x NULL: one axis. */
 void dpuf_hip_rope_append(void* s, const DpufAmdBatch* b, const DpufAmdPages* p, const DpufAmdRope* r,
-                          const DpufAmdRopeAxes* x, const int32_t* pos, int64_t pos_stride, int32_t in_type, int32_t nq, const void* q, const void* k, const void* v,
-                          int64_t qs, int64_t ks, int64_t vs, const float* qn, const float* kn, float eps,
-                          void* q_out);
+                          const DpufAmdRopeAxes* x, const int32_t* pos, int64_t pos_stride, int32_t in_type,
+                          int32_t nq, const void* q, const void* k, const void* v, int64_t qs, int64_t ks, int64_t vs,
+                          const float* qn, const float* kn, float eps, void* q_out);
 /* window 0: none (sink then says nothing). */
 size_t dpuf_hip_paged_attn_workspace(const DpufAmdBatch* b, const DpufAmdPages* p, int32_t nq, int32_t window,
                                      int32_t sink);

@@ -216,7 +216,8 @@ template <typename L, bool TOP, typename F> DEV void scan(const void* p, int lo,
         for (int u = 0; u < U; u++) {
             float mx = NEG_INF;
 #pragma unroll
-            for (int e = 0; e < VE; e++) mx = fmaxf(mx, __builtin_canonicalizef(x[u][e]));   // (a maximum keeps a signalling NaN)
+            for (int e = 0; e < VE; e++)     // (of a signalling NaN the maximum would be NaN)
+                mx = fmaxf(mx, __builtin_canonicalizef(x[u][e]));
             most = fmaxf(most, mx);
             if (TOP) {
                 uint32_t k = order_bits(mx);
@@ -403,7 +404,8 @@ template <int R, bool MANY> DEV int pick_stored(RowLds& sh, int n, int K, const 
         v[i] = R <= FEW ? most.early[i % FEW] : most.p[min(g, n - 1)];
         if (g >= n) v[i] = 0;
     }
-    return pick<R, false, MANY>(sh, R, K, [&](int i) { return v[i]; }, [&](int i) { return i * NT + threadIdx.x; }, out);
+    return pick<R, false, MANY>(
+        sh, R, K, [&](int i) { return v[i]; }, [&](int i) { return i * NT + threadIdx.x; }, out);
 }
 template <bool MANY> DEV int pick_groups(RowLds& sh, int n, int K, const Stored& most, uint64_t* out) {
     return n <= NT * FEW / 2 ? pick_stored<FEW / 2, MANY>(sh, n, K, most, out)

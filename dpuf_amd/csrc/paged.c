@@ -204,8 +204,8 @@ static int32_t rope_append(const DpufAmdBatch* batch, const DpufAmdPages* pages,
         if (st[i] < need[i] || st[i] % 8 != 0) return -4;
     const int in_place = d_q && d_q_out == d_q && in_type == pages->type && q_stride == need[0];
     Span in[9] = {rows_of(d_k, batch->n_rows, k_stride, need[1], es), rows_of(d_v, batch->n_rows, v_stride, need[2], es),
-                  rows_of(d_positions, n_axes, n_axes > 1 ? pos_stride : 0, batch->n_rows, 4), run(rope->turns, rope->rot_dim / 2, 8), run(d_q_norm, hd, 4),
-                  run(d_k_norm, hd, 4)};
+                  rows_of(d_positions, n_axes, n_axes > 1 ? pos_stride : 0, batch->n_rows, 4),
+                  run(rope->turns, rope->rot_dim / 2, 8), run(d_q_norm, hd, 4), run(d_k_norm, hd, 4)};
     batch_spans(batch, in + 6);
     const Span q = rows_of(d_q, batch->n_rows, q_stride, need[0], es);
     /* k and v may lie interleaved in one allocation */
@@ -406,7 +406,8 @@ DPUF_EXPORT int32_t dpuf_amd_sample(int32_t type, int32_t n, int32_t V, int64_t 
 }
 
 DPUF_EXPORT size_t dpuf_amd_logprobs_workspace(int32_t n, int32_t V, int32_t n_top) {
-    if (n < 1 || n > MAX_ROWS || V < 1 || V > DPUF_AMD_SAMPLE_MAX_VOCAB || n_top < 0 || n_top > DPUF_AMD_LOGPROBS_MAX_TOP)
+    if (n < 1 || n > MAX_ROWS || V < 1 || V > DPUF_AMD_SAMPLE_MAX_VOCAB || n_top < 0 ||
+        n_top > DPUF_AMD_LOGPROBS_MAX_TOP)
         return 0;
     return dpuf_hip_logprobs_workspace(n, V, n_top);
 }

@@ -918,8 +918,13 @@ int ceil_div(int64_t a, int64_t b) { return (int)((a + b - 1) / b); }
 // Keys per range: about `times` sqrt(ctx), in whole 128.
 int range_of(int64_t ctx, double times) { return ((int)(times * sqrt((double)ctx)) + 127) & ~127; }
 
+// Whether chunks are nearly all of the work of a batch with single rows.
+bool mostly_chunks(const DpufAmdBatch& b, int G) {
+    return (int64_t)(b.n_rows - b.n_seqs) * G > 220 * (int64_t)b.n_seqs;
+}
+
 // Key ranges of chunks with a window of about ctx keys: as many as take the
-// least time of up to 8, counted in steps of 64 keys that a workgroup walks one
+// least time of up to 16, counted in steps of 64 keys that a workgroup walks one
 // after the other (0.3 us + 1.7 a 128 columns, a sixth more with two workgroups
 // a CU), the join of the ranges (4.5 us and the partial sums written and read at
 // 4.5 TB/s) and the workgroups of the grid that find no rows (1 us a round);
@@ -927,15 +932,19 @@ int range_of(int64_t ctx, double times) { return ((int)(times * sqrt((double)ctx
 // three, four and eight ranges: 512 rows of 32 heads, 8 kv heads of 128 with a
 // window of 128 keys 15.0 us, 23.6, 22.4, 22.4, 22.5, of 512 24.6, 27.2, 27.0,
 // 26.6, 35.8, of 2 048 80, 57, 46, 44, 56; 48 rows, 512 keys 24.0, 22.1, 19.3,
-// 19.3, 16.9; 256 rows and 31 single ones, 1 024 keys 53.6, 47.0, 47.5, 50.3, 63.
+// 19.3, 16.9; 256 rows and 31 single ones, 1 024 keys 53.6, 47.0, 47.5, 50.3, 63;
+// 100 rows, 8 192 keys 52.5 in eight, 39.6 in fifteen.  Single rows beside few
+// chunks get room, as without windows: two chunks of 131 rows and 7 single ones,
+// 8 192 keys 99 us with 400 workgroups for chunks, 109 with 512.
 void window_ranges(PaPlan& r, const DpufAmdBatch& b, const DpufAmdPages& p, int nq, int64_t ctx) {
     const int G = nq / p.n_kv_heads, tr = r.only == PA_WIDE ? 256 : 128;
     const int64_t packed = (int64_t)(r.only == PA_BOTH && b.n_rows > b.n_seqs ? b.n_rows - b.n_seqs : b.n_rows) * G;
-    const int64_t wgs = (packed + tr - 1) / tr * p.n_kv_heads, slots = r.only == PA_WIDE ? 256 : 512;
+    const int64_t wgs = (packed + tr - 1) / tr * p.n_kv_heads;
+    const int64_t slots = r.only == PA_WIDE ? 256 : r.only == PA_BOTH && !mostly_chunks(b, G) ? 400 : 512;
     const double step = 0.3 + 1.7 * p.head_dim / 128;
     const double singles = r.only == PA_BOTH ? 0.6 * b.n_seqs * ctx * p.n_kv_heads * p.head_dim * 4 / 4.9e6 : 0;
     double best = 0;
-    for (int nz = 1; nz <= 8; nz++) {
+    for (int nz = 1; nz <= 16; nz++) {
         const int chunk = (ceil_div(ctx, nz) + 63) & ~63;
         if (nz > 1 && ceil_div(ctx, chunk) < nz) continue;
         double t = (double)chunk / 64 * step * ((wgs * nz + slots - 1) / slots);
@@ -979,17 +988,19 @@ void window_ranges(PaPlan& r, const DpufAmdBatch& b, const DpufAmdPages& p, int 
 // the window and as many more as the tile's rows are apart, in whole tiles of
 // keys; but the chunks' ranges by window_ranges, and one range of up to 512 keys
 // of 64 columns (a window of 256, one row 8.1 us a call against 10.3 in two, of
-// 384 8.8 and 10.1; of 128 columns 10.6 and 10.3, 12.2 and 10.5).  (A window of
-// 0 here is none.)
+// 384 8.8 and 10.1; of 128 columns 10.6 and 10.3, 12.2 and 10.5).  A window of
+// 0 here is none, and for the kernels so is one that reaches whatever the table
+// can hold (512 rows over 16 384 keys 157 us instead of 162).
 PaPlan plan(const DpufAmdBatch& b, const DpufAmdPages& p, int nq, int window, int sink) {
     const int G = nq / p.n_kv_heads;
     PaPlan r;
     r.few = G > 16 ? 32 : 16;
     const int64_t cap = (int64_t)b.table_stride * p.page_size;
     int64_t ctx = b.max_ctx < 1 ? 1 : b.max_ctx < cap ? b.max_ctx : cap;
-    // what reaches every key of the table needs no more than that
-    r.window = window < cap && sink < cap ? window : (int)cap;
-    r.sink = r.window < cap ? sink : 0;
+    const bool windowed = window > 0;
+    if (window >= cap || sink >= cap) window = 0;
+    r.window = window;
+    r.sink = window ? sink : 0;
     const int64_t near = (int64_t)r.window + (r.sink + 31) / 32 * 32 + 32;
     r.reach_few = (int)(near + 16 / G + 1 < cap ? near + 16 / G + 1 : cap);
     if (window && ctx > r.reach_few) ctx = r.reach_few;
@@ -1025,14 +1036,14 @@ PaPlan plan(const DpufAmdBatch& b, const DpufAmdPages& p, int nq, int window, in
     // 39 are within 10 % of the best of 256 to 1 024, 7 % in the middle; the
     // farthest is four of 64 and a single one over 4 096 to 16 384, 131 with
     // 400 and 85 with 768
-    const bool chunks = (int64_t)(b.n_rows - b.n_seqs) * G > 220 * (int64_t)b.n_seqs;
-    const int64_t room = r.only == PA_WIDE ? 256 : r.only == PA_MANY ? 512 : chunks ? 768 : 400;
+    const int64_t room = r.only == PA_WIDE ? 256 : r.only == PA_MANY ? 512 : mostly_chunks(b, G) ? 768 : 400;
     const int64_t wgs = (packed + tr - 1) / tr * p.n_kv_heads;
     const int64_t nz = wgs >= room ? 1 : room / (wgs > 0 ? wgs : 1);
     r.chunk_many = (ceil_div(ctx, nz) + 127) & ~127;
     if (r.chunk_many < range_of(ctx, 4.0)) r.chunk_many = range_of(ctx, 4.0);
     r.nz_many = ceil_div(ctx, r.chunk_many);
-    if (window && r.only != PA_FEW) window_ranges(r, b, p, nq, b.max_ctx > r.reach_many ? r.reach_many : ctx);
+    if (windowed && r.only != PA_FEW)
+        window_ranges(r, b, p, nq, window && b.max_ctx > r.reach_many ? r.reach_many : ctx);
     const size_t all = (size_t)b.n_rows * nq, some = (size_t)b.n_seqs * p.n_kv_heads * r.few;
     r.few_rows = r.only <= PA_FEW && r.nz_few > 1 ? r.nz_few * (r.only == PA_FEW ? all : some) : 0;
     r.many_rows = r.only != PA_FEW && r.nz_many > 1 ? r.nz_many * all : 0;
@@ -1116,7 +1127,7 @@ void dpuf_hip_paged_attn(void* s, const DpufAmdBatch* b, const DpufAmdPages* p, 
         }
     };
     const bool bf = p->type == DPUF_AMD_BF16;
-    if (window) bf ? go(Bf16(), std::true_type()) : go(Fp16(), std::true_type());
+    if (pl.window) bf ? go(Bf16(), std::true_type()) : go(Fp16(), std::true_type());
     else bf ? go(Bf16(), std::false_type()) : go(Fp16(), std::false_type());
 }
 

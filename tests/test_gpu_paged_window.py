@@ -161,6 +161,19 @@ def test_estimates_of_the_longest_context(eng, hip, mode, max_ctx):
     check(cache, 8, q, 0.1, out, lse, R.BF16, window, sink)
 
 
+@pytest.mark.parametrize("rows,ctx", [([50], [9000]), ([1, 60, 1, 45], [300, 9000, 4000, 45]), ([30, 20], [8200, 30])])
+@pytest.mark.parametrize("window", [8191, 8200, 9007, 9008, 1 << 30])
+def test_long_windows_of_chunks(eng, hip, rows, ctx, window):
+    """Many ranges of keys, and windows a key less than what the table holds
+    (9 008 rows), as much, and more."""
+    rng = np.random.default_rng(window + len(rows))
+    cache = R.Cache(hip, rng, R.BF16, rows, ctx, 1, 64, 16)
+    q = R.to_type(rng.standard_normal((cache.n_rows, 4, 64)) * 1.5, R.BF16)
+    say(f"long windows: rows {rows} over {ctx}, window {window}, table {cache.table.shape}")
+    out, lse, _ = call(eng, hip, cache, 4, q, 0.125, window, 3, extra=1)
+    check(cache, 4, q, 0.125, out, lse, R.BF16, window, 3)
+
+
 @pytest.mark.parametrize("rows", [1, 3])
 def test_hundreds_of_sequences(eng, hip, rows):
     rng = np.random.default_rng(rows)
