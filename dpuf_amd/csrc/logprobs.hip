@@ -15,18 +15,22 @@
 // logit, then by place.  The first k groups hold the k largest logits: a token
 // of another group has k groups before its own, each with a logit that is larger
 // or as large and further to the front.  So one pass over the row leaves the
-// groups' largest, and what is read again is k groups.
+// groups' largest, and what is read again is k groups; or, without ordering them
+// first, the few more that reach a bound which at least k groups' largest reach
+// (of 151 936 random logits and 20 alternatives 24 groups; one row 9.5 us, 10.7 by
+// the order of the groups), unless those, or their tokens, are many.
 //
 //   k_lp_part   a workgroup per chunk of a row: (r, l, u) and the groups' largest;
-//   k_lp_row    a workgroup per row: joins the chunks, picks the k groups, the k
-//               tokens among theirs, and writes;
+//   k_lp_row    a workgroup per row: joins the chunks, picks groups, the k tokens
+//               among theirs, and writes;
 //   k_lp_whole  both, a workgroup per row, where there are many rows.
 //
 // Bound by the bytes of the logits, in 16 bits nearly as much by the exponential
 // and ten other instructions of each: 512 rows of 151 936 fp32 logits 54 us, 5.7
-// TB/s, 2 048 in bf16 with 20 alternatives 127 us, 4.9 TB/s.  Few rows are bound
-// by latency: one with 20 alternatives 3.8 us (38 workgroups) and 7.0, of which
-// 1.0 are the first loads, 0.8 the sums, 2.2 each pick and 0.8 what it reads.
+// TB/s, 2 048 in bf16 with 20 alternatives 124 us, 5.0 TB/s.  Few rows are bound
+// by latency: one with 20 alternatives 3.8 us (38 workgroups) and 5.6, of which
+// 1.0 are the first loads, 0.8 the sums, 0.8 the groups' tokens and the rest the
+// bound, the lists and the order.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
@@ -43,6 +47,7 @@ constexpr int DIRECT = NT * MOST;    // groups that are picked from as they are
 constexpr int WHOLE = DIRECT * GL * 4;  // tokens of a row that is not cut, of any type, at most
 constexpr int OVER = 64;             // groups of a bundle, where there are more
 constexpr int LISTED = 1024;         // candidates that are ranked
+constexpr int WHICH = 128;           // groups whose tokens may be listed unranked
 constexpr int MAX_TOP = DPUF_AMD_LOGPROBS_MAX_TOP;
 constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.69314718055994531f;
 constexpr float SLACK = 8.0f;        // r stays while no s is larger
@@ -163,8 +168,9 @@ DEV Sum wave_sum(Sum s) {
 struct RowLds {
     Sum ss[NW];
     float sm[NW];
-    unsigned n;
+    unsigned n, n_tokens;
     uint32_t __attribute__((aligned(16))) most[NT];
+    uint32_t which[WHICH];
     uint32_t bound;
     uint64_t __attribute__((aligned(16))) list[LISTED];
     uint64_t best[NW];
@@ -250,7 +256,9 @@ template <typename L, bool TOP, typename F> DEV void scan(const void* p, int lo,
 
 // A number that at least K of the threads' items reach, and not many more: the
 // K-th largest of the largest of 64 quads of threads, or, where MANY may be asked
-// for, of the threads.  f(key) for each item; 0 is none, and 1 the least bound.
+// for, of the threads (64 alternatives of one row of 151 936 16.6 us instead of
+// 20.8, 20 11.1 instead of 10.7).  f(key) for each item; 0 is none, and 1 the
+// least bound.
 template <bool LEAN, bool MANY, typename F> DEV uint32_t bound_of(RowLds& sh, int K, F each) {
     const int t = threadIdx.x, lane = t & 63;
     uint32_t b = 0;
@@ -263,7 +271,7 @@ template <bool LEAN, bool MANY, typename F> DEV uint32_t bound_of(RowLds& sh, in
         sh.most[t] = b;
     }
     if (t == 0) {
-        sh.n = 0;
+        sh.n = sh.n_tokens = 0;
         sh.bound = ~0u;
     }
     __syncthreads();
@@ -293,13 +301,45 @@ template <bool LEAN, bool MANY, typename F> DEV uint32_t bound_of(RowLds& sh, in
     return max(bound, 1u);
 }
 
+// put(place, i) of those of a thread's items that are in, at the next places of a
+// list of *n, a wave's side by side, each round's by lane.
+template <typename I, typename F, typename P> DEV void append(unsigned* n, I items, F in, P put) {
+    int hits = 0;
+    items([&](int i) { hits += __popcll(__ballot(in(i))); });
+    if (!hits) return;
+    int e = (threadIdx.x & 63) == 0 ? (int)atomicAdd(n, (unsigned)hits) : 0;
+    e = __builtin_amdgcn_readfirstlane(e);
+    items([&](int i) {
+        const bool on = in(i);
+        const uint64_t hit = __ballot(on);
+        const int at = e + (int)__builtin_amdgcn_mbcnt_hi((uint32_t)(hit >> 32),
+                                                          __builtin_amdgcn_mbcnt_lo((uint32_t)hit, 0));
+        if (on) put(at, i);
+        e += __popcll(hit);
+    });
+}
+
+// The K largest of the list's n, largest first, into out.
+DEV void rank(const RowLds& sh, int n, int K, uint64_t* out) {
+    for (int i = threadIdx.x; i < n; i += NT) {
+        const uint64_t k = sh.list[i];
+        int r = 0, e = 0;
+        for (; e + 8 <= n; e += 8)
+#pragma unroll
+            for (int d = 0; d < 8; d += 2) {
+                const ulonglong2 q = *(const ulonglong2*)&sh.list[e + d];
+                r += (q.x > k) + (q.y > k);
+            }
+        for (; e < n; e++) r += sh.list[e] > k;
+        if (r < K) out[r] = k;
+    }
+}
+
 // The K largest of the threads' items, first by bits, then by the lower index,
 // largest first, into out (as comp_of).  A thread has n items (R of them, in
 // registers, or with R 0 n, wherever they are): bits(i), 0 for none, of index
 // id(i).  Returns how many there are, K at most.  What reaches a bound is listed
-// and ranked.  LEAN: in few registers.  MANY: K may be more than 32.  A row of
-// 151 936 random logits takes 17 us with 64 of them, 11.3 with 20; 64 by the
-// quads' bound 21.7 (bf16 31.7), and 20 by the threads' 11.7.
+// and ranked.  LEAN: in few registers.  MANY: K may be more than 32.
 template <int R, bool LEAN, bool MANY, typename F, typename G>
 DEV int pick(RowLds& sh, int n, int K, F bits, G id, uint64_t* out) {
     const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
@@ -312,22 +352,11 @@ DEV int pick(RowLds& sh, int n, int K, F bits, G id, uint64_t* out) {
             for (int i = 0; i < n; i++) f(i);
         }
     };
-    // lists the items whose key reaches the bound, a wave's side by side, each round's by lane
     auto list = [&](uint32_t bound, auto key) {
-        int hits = 0;
-        items([&](int i) { hits += __popcll(__ballot(key(i) >= bound)); });
-        if (hits) {
-            int e = lane == 0 ? (int)atomicAdd(&sh.n, (unsigned)hits) : 0;
-            e = __builtin_amdgcn_readfirstlane(e);
-            items([&](int i) {
-                const bool in = key(i) >= bound;
-                const uint64_t hit = __ballot(in);
-                const int at = e + (int)__builtin_amdgcn_mbcnt_hi((uint32_t)(hit >> 32),
-                                                                  __builtin_amdgcn_mbcnt_lo((uint32_t)hit, 0));
-                if (in && at < LISTED) sh.list[at] = comp_of(bits(i), id(i));
-                e += __popcll(hit);
-            });
-        }
+        append(&sh.n, items, [&](int i) { return key(i) >= bound; },
+               [&](int at, int i) {
+                   if (at < LISTED) sh.list[at] = comp_of(bits(i), id(i));
+               });
         __syncthreads();
         return (int)sh.n;
     };
@@ -345,18 +374,7 @@ DEV int pick(RowLds& sh, int n, int K, F bits, G id, uint64_t* out) {
         listed = list(least, key);
     }
     if (listed <= LISTED) {
-        for (int i = t; i < listed; i += NT) {
-            const uint64_t k = sh.list[i];
-            int r = 0, e = 0;
-            for (; e + 8 <= listed; e += 8)
-#pragma unroll
-                for (int d = 0; d < 8; d += 2) {
-                    const ulonglong2 q = *(const ulonglong2*)&sh.list[e + d];
-                    r += (q.x > k) + (q.y > k);
-                }
-            for (; e < listed; e++) r += sh.list[e] > k;
-            if (r < K) out[r] = k;
-        }
+        rank(sh, listed, K, out);
     } else {
         // too many (long runs of equal ones, or they lie with few of the threads): one at a time
         uint64_t last = ~0ull;
@@ -396,7 +414,9 @@ struct Kept {
     const uint32_t* p;
     DEV uint32_t at(int g) const { return p[g]; }
 };
-template <int R, bool MANY> DEV int pick_stored(RowLds& sh, int n, int K, const Stored& most, uint64_t* out) {
+// f(R, items of a thread, bits, id) of the groups, as in pick.
+template <int N> struct Int { static constexpr int value = N; };
+template <int R, typename F> DEV int of_stored(int n, const Stored& most, F f) {
     uint32_t v[R];
 #pragma unroll
     for (int i = 0; i < R; i++) {
@@ -404,21 +424,81 @@ template <int R, bool MANY> DEV int pick_stored(RowLds& sh, int n, int K, const 
         v[i] = R <= FEW ? most.early[i % FEW] : most.p[min(g, n - 1)];
         if (g >= n) v[i] = 0;
     }
-    return pick<R, false, MANY>(
-        sh, R, K, [&](int i) { return v[i]; }, [&](int i) { return i * NT + threadIdx.x; }, out);
+    return f(Int<R>(), R, [&](int i) { return v[i]; }, [&](int i) { return i * NT + threadIdx.x; });
 }
-template <bool MANY> DEV int pick_groups(RowLds& sh, int n, int K, const Stored& most, uint64_t* out) {
-    return n <= NT * FEW / 2 ? pick_stored<FEW / 2, MANY>(sh, n, K, most, out)
-           : n <= NT * FEW   ? pick_stored<FEW, MANY>(sh, n, K, most, out)
-                             : pick_stored<MOST, MANY>(sh, n, K, most, out);
+template <typename F> DEV int of_groups(int n, const Stored& most, F f) {
+    return n <= NT * FEW / 2 ? of_stored<FEW / 2>(n, most, f)
+           : n <= NT * FEW   ? of_stored<FEW>(n, most, f)
+                             : of_stored<MOST>(n, most, f);
 }
-template <bool MANY> DEV int pick_groups(RowLds& sh, int n, int K, const Kept& most, uint64_t* out) {
-    return pick<0, true, MANY>(sh, (n + NT - 1) / NT, K,
-                   [&](int i) {
-                       const int g = i * NT + threadIdx.x;
-                       return g < n ? most.p[g] : 0;
-                   },
-                   [&](int i) { return i * NT + threadIdx.x; }, out);
+template <typename F> DEV int of_groups(int n, const Kept& most, F f) {
+    return f(
+        Int<0>(), (n + NT - 1) / NT,
+        [&](int i) {
+            const int g = i * NT + threadIdx.x;
+            return g < n ? most.p[g] : 0;
+        },
+        [&](int i) { return i * NT + threadIdx.x; });
+}
+
+// A lane's load of a group's tokens, the e-th of all groups' loads: their first
+// one, and their bits in v; group(i) is the i-th of n.
+template <typename L, typename F>
+DEV int load_group(const LpArgs& a, const void* p, int e, int n, F group, uint32_t* v) {
+    const int tok = e < n * GL ? group(e / GL) * GL * L::VE + e % GL * L::VE : a.V;
+    float x[L::VE];
+    L::get(load<L>(p, tok, a.V), x);
+#pragma unroll
+    for (int j = 0; j < L::VE; j++) v[j] = order_bits(x[j]);
+    return tok;
+}
+
+// The K largest logits into sh.tokens, at once: what at least K groups' largest
+// reach, at least K logits do, and those lie in these groups.  Returns how many,
+// or -1 where that are more than the lists hold.
+template <typename L, bool LEAN, bool MANY, typename M>
+DEV int pick_at_once(const LpArgs& a, RowLds& sh, int K, const M& most, const void* p) {
+    constexpr int VE = L::VE, R = MANY ? 4 : 2;
+    uint32_t bound;
+    const int n = of_groups(a.groups, most, [&](auto r, int n, auto bits, auto id) {
+        auto items = [&](auto f) {
+            if constexpr (r.value > 0) {
+#pragma unroll
+                for (int i = 0; i < r.value; i++) f(i);
+            } else {
+                for (int i = 0; i < n; i++) f(i);
+            }
+        };
+        bound = bound_of<LEAN, MANY>(sh, K, [&](auto f) { items([&](int i) { f(bits(i), i); }); });
+        append(&sh.n, items, [&](int i) { return bits(i) >= bound; },
+               [&](int at, int i) {
+                   if (at < WHICH) sh.which[at] = id(i);
+               });
+        __syncthreads();
+        return (int)sh.n;
+    });
+    if (n > WHICH) return -1;
+    for (int e0 = 0; e0 < n * GL; e0 += R * NT) {
+        uint32_t v[R][VE];
+        int tok[R];
+#pragma unroll
+        for (int i = 0; i < R; i++)
+            tok[i] = load_group<L>(a, p, e0 + i * NT + threadIdx.x, n, [&](int g) { return (int)sh.which[g]; }, v[i]);
+        auto items = [&](auto f) {
+#pragma unroll
+            for (int i = 0; i < R * VE; i++) f(i);
+        };
+        append(&sh.n_tokens, items, [&](int i) { return v[i / VE][i % VE] >= bound; },
+               [&](int at, int i) {
+                   if (at < LISTED) sh.list[at] = comp_of(v[i / VE][i % VE], tok[i / VE] + i % VE);
+               });
+    }
+    __syncthreads();
+    const int listed = sh.n_tokens;
+    if (listed > LISTED) return -1;
+    rank(sh, listed, K, sh.tokens);
+    __syncthreads();
+    return min(listed, K);
 }
 
 // The n groups' tokens, a lane's load of a group at a time, R of them a thread.
@@ -427,16 +507,11 @@ template <typename L, int R, bool LEAN> DEV int pick_tokens(const LpArgs& a, Row
     uint32_t v[R][VE];
     int tok[R];
 #pragma unroll
-    for (int i = 0; i < R; i++) {
-        const int e = i * NT + threadIdx.x;
-        tok[i] = e < n * GL ? (int)index_of(sh.groups[e / GL]) * GL * VE + e % GL * VE : a.V;
-        float x[VE];
-        L::get(load<L>(p, tok[i], a.V), x);
-#pragma unroll
-        for (int j = 0; j < VE; j++) v[i][j] = order_bits(x[j]);
-    }
-    return pick<R * VE, LEAN, (R > 2)>(sh, R * VE, a.n_top, [&](int i) { return v[i / VE][i % VE]; },
-                        [&](int i) { return tok[i / VE] + i % VE; }, sh.tokens);
+    for (int i = 0; i < R; i++)
+        tok[i] = load_group<L>(a, p, i * NT + threadIdx.x, n, [&](int g) { return (int)index_of(sh.groups[g]); }, v[i]);
+    return pick<R * VE, LEAN, (R > 2)>(
+        sh, R * VE, a.n_top, [&](int i) { return v[i / VE][i % VE]; }, [&](int i) { return tok[i / VE] + i % VE; },
+        sh.tokens);
 }
 
 // Loads of a thread for the tokens of K groups: 1, 2 or 4.
@@ -483,9 +558,17 @@ DEV void finish(const LpArgs& a, RowLds& sh, int row, const void* p, Sum s, floa
     if (t == 0 && a.entropy) a.entropy[row] = top > NEG_INF ? fmaxf((log_l - s.u / s.l) * LN2, 0.0f) : 0.0f;
     if constexpr (LOADS > 0) {
         const int K = a.n_top;
-        int n;
+        int n = -1;
         if (M::LEAN || a.groups <= DIRECT) {
-            n = pick_groups<MANY>(sh, a.groups, K, most, sh.groups);
+            n = pick_at_once<L, M::LEAN, MANY>(a, sh, K, most, p);
+            if (n < 0) {
+                // the K largest groups, and then among their tokens
+                __syncthreads();
+                n = of_groups(a.groups, most, [&](auto r, int n, auto bits, auto id) {
+                    return pick<r.value, M::LEAN, MANY>(sh, n, K, bits, id, sh.groups);
+                });
+                n = pick_tokens<L, LOADS, M::LEAN>(a, sh, n, p);
+            }
         } else {
             // bundles of OVER groups first, by the same argument; 4 096 of them at most
             const int bundles = (a.groups + OVER - 1) / OVER;
@@ -497,7 +580,8 @@ DEV void finish(const LpArgs& a, RowLds& sh, int row, const void* p, Sum s, floa
                 for (int g = at * OVER; g < min(a.groups, (at + 1) * OVER); g++) k = max(k, most.at(g));
                 b[i] = at < bundles ? k : 0;
             }
-            n = pick<16, false, MANY>(sh, 16, K, [&](int i) { return b[i]; }, [&](int i) { return i * NT + t; }, sh.tokens);
+            n = pick<16, false, MANY>(
+                sh, 16, K, [&](int i) { return b[i]; }, [&](int i) { return i * NT + t; }, sh.tokens);
             constexpr int RG = MAX_TOP * OVER / NT;
             uint32_t v[RG];
             auto of = [&](int i) {
@@ -507,8 +591,8 @@ DEV void finish(const LpArgs& a, RowLds& sh, int row, const void* p, Sum s, floa
 #pragma unroll
             for (int i = 0; i < RG; i++) v[i] = of(i) < a.groups ? most.at(of(i)) : 0;
             n = pick<RG, false, MANY>(sh, RG, K, [&](int i) { return v[i]; }, of, sh.groups);
+            n = pick_tokens<L, LOADS, M::LEAN>(a, sh, n, p);
         }
-        n = pick_tokens<L, LOADS, M::LEAN>(a, sh, n, p);
         for (int i = t; i < K; i += NT) {
             const int64_t at = (int64_t)row * K + i;
             a.top[at] = i < n ? (int)index_of(sh.tokens[i]) : -1;
@@ -555,7 +639,7 @@ template <typename L, int LOADS> __global__ __launch_bounds__(NT) void k_lp_row(
 }
 
 // Eight workgroups a CU as long as their registers suffice: 2 048 bf16 rows of
-// 151 936 with 20 alternatives 127 us, five a CU 147.  More than 32 alternatives
+// 151 936 with 20 alternatives 124 us, five a CU 147.  More than 32 alternatives
 // take more of them, and none may go to memory.
 template <typename L, int LOADS>
 __global__ __launch_bounds__(NT, LOADS < 4 ? 8 : L::VE < 8 ? 7 : 4) void k_lp_whole(LpArgs a) {
