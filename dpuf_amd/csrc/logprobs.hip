@@ -549,11 +549,13 @@ DEV void finish(const LpArgs& a, RowLds& sh, int row, const void* p, Sum s, floa
         join(sh, s, same);
     }
     const float log_l = log2f(s.l);
+    // (of a token with nearly all the weight d - log_l is what is left of their
+    // roundings, of either sign; p is 1 at most)
     auto logp = [&](float x) {
         if (!(x > NEG_INF)) return NEG_INF;
-        if (far) return (x == top ? 0.0f : x - top) - log_l * LN2;
+        if (far) return fminf((x == top ? 0.0f : x - top) - log_l * LN2, 0.0f);
         const float d = fmaf(x, LOG2E, -s.r);
-        return d > -1e30f ? (d - log_l) * LN2 : x - top;
+        return fminf(d > -1e30f ? (d - log_l) * LN2 : x - top, 0.0f);
     };
     if (t == 0 && a.entropy) a.entropy[row] = top > NEG_INF ? fmaxf((log_l - s.u / s.l) * LN2, 0.0f) : 0.0f;
     if constexpr (LOADS > 0) {

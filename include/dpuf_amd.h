@@ -375,17 +375,17 @@ DPUF_EXPORT int32_t dpuf_amd_sample(int32_t type, int32_t n, int32_t V, int64_t 
 /* Scores of n rows (1 to 65536) of V logits (1 to DPUF_AMD_SAMPLE_MAX_VOCAB;
  * rows row_stride elements apart) as they are, at temperature 1, with
  * p = exp(x) / sum exp(x): NaN logits count as -infinity, +infinity leaves only
- * its like.  d_logprobs [n][n_targets] gets ln p of row i's tokens
+ * its like.  d_logprobs [n][n_targets] gets ln p (0 at most) of row i's tokens
  * d_targets[i * n_targets ...] (0 to DPUF_AMD_LOGPROBS_MAX_TARGETS of them; the
- * same one may be there twice; one outside [0, V) gets -infinity), d_entropy
- * [n] -sum p ln p, d_top_tokens and d_top_logprobs [n][n_top] the n_top (0 to
- * DPUF_AMD_LOGPROBS_MAX_TOP) largest logits' tokens (ties: the lowest indices)
- * and ln p, in that order.  Fewer logits above -infinity than that leave -1 and
- * -infinity; a row without any gives -infinity and an entropy of 0.  d_targets
- * and d_logprobs may be NULL (n_targets 0), as may d_entropy, and d_top_tokens
- * and d_top_logprobs (n_top 0), not all three outputs.  Sums are fp32.  The
- * same inputs give the same bits.  The workspace (on 16 bytes) is that of n
- * rows of V: fewer rows are cut into more chunks and may need more. */
+ * same one may be there twice; one outside [0, V) gets -infinity), d_entropy [n]
+ * -sum p ln p (0 at least), d_top_tokens and d_top_logprobs [n][n_top] the n_top
+ * (0 to DPUF_AMD_LOGPROBS_MAX_TOP) largest logits' tokens (ties: the lowest
+ * indices) and ln p, in that order.  Fewer logits above -infinity than that
+ * leave -1 and -infinity; a row without any gives -infinity and an entropy of
+ * 0.  d_targets and d_logprobs may be NULL (n_targets 0), as may d_entropy, and
+ * d_top_tokens and d_top_logprobs (n_top 0), not all three outputs.  Sums are
+ * fp32.  The same inputs give the same bits.  The workspace (on 16 bytes) is
+ * that of n rows of V: fewer rows are cut into more chunks and may need more. */
 #define DPUF_AMD_LOGPROBS_MAX_TARGETS 1024
 #define DPUF_AMD_LOGPROBS_MAX_TOP 64
 DPUF_EXPORT size_t dpuf_amd_logprobs_workspace(int32_t n, int32_t V, int32_t n_top);

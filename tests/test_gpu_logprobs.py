@@ -346,3 +346,20 @@ def test_two_streams_and_a_graph(eng, hip):
         hip.lib.hipGraphExecDestroy(ge)
         hip.lib.hipGraphDestroy(graph)
         hip.lib.hipStreamDestroy(w["s"])
+
+
+@pytest.mark.parametrize("t", [R.F32, R.BF16, R.F16])
+@pytest.mark.parametrize("V,n", [(5, 1500), (5000, 40), (40000, 12), (300000, 2)])
+def test_no_log_probability_is_above_zero(eng, hip, V, n, t):
+    """Rows of one finite logit, and rows where one token has nearly all the
+    weight: ln p is 0 at most, of targets and of alternatives."""
+    rng = np.random.default_rng(V + t)
+    hot = rng.integers(0, V, n)
+    x = np.full((n, V), -np.inf, F)
+    x[1::2] = (rng.standard_normal((len(x[1::2]), V)) - 40).astype(F)
+    x[np.arange(n), hot] = (5 + 55 * rng.random(n)).astype(F)
+    say(f"one token alone: {n} rows of {V}, type {t}")
+    for k in (0, 1, 33):
+        lp, en, top, tl = run(eng, hip, x, t, np.stack([hot, rng.integers(0, V, n)], 1), k)
+        assert np.all(lp <= 0.0) and np.all(tl <= 0.0) and np.all(en >= 0.0)
+        assert k == 0 or np.array_equal(top[:, 0], hot)
