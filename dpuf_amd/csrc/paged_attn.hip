@@ -989,16 +989,15 @@ void window_ranges(PaPlan& r, const DpufAmdBatch& b, const DpufAmdPages& p, int 
 // keys; but the chunks' ranges by window_ranges, and one range of up to 512 keys
 // of 64 columns (a window of 256, one row 8.1 us a call against 10.3 in two, of
 // 384 8.8 and 10.1; of 128 columns 10.6 and 10.3, 12.2 and 10.5).  A window of
-// 0 here is none, and for the kernels so is one that reaches whatever the table
-// can hold (512 rows over 16 384 keys 157 us instead of 162).
+// 0 here is none.  One that reaches whatever the table can hold stays one: its
+// rows' first ones see few keys too, and what a row gets is not to depend on the
+// table's width.
 PaPlan plan(const DpufAmdBatch& b, const DpufAmdPages& p, int nq, int window, int sink) {
     const int G = nq / p.n_kv_heads;
     PaPlan r;
     r.few = G > 16 ? 32 : 16;
     const int64_t cap = (int64_t)b.table_stride * p.page_size;
     int64_t ctx = b.max_ctx < 1 ? 1 : b.max_ctx < cap ? b.max_ctx : cap;
-    const bool windowed = window > 0;
-    if (window >= cap || sink >= cap) window = 0;
     r.window = window;
     r.sink = window ? sink : 0;
     const int64_t near = (int64_t)r.window + (r.sink + 31) / 32 * 32 + 32;
@@ -1042,8 +1041,7 @@ PaPlan plan(const DpufAmdBatch& b, const DpufAmdPages& p, int nq, int window, in
     r.chunk_many = (ceil_div(ctx, nz) + 127) & ~127;
     if (r.chunk_many < range_of(ctx, 4.0)) r.chunk_many = range_of(ctx, 4.0);
     r.nz_many = ceil_div(ctx, r.chunk_many);
-    if (windowed && r.only != PA_FEW)
-        window_ranges(r, b, p, nq, window && b.max_ctx > r.reach_many ? r.reach_many : ctx);
+    if (window && r.only != PA_FEW) window_ranges(r, b, p, nq, b.max_ctx > r.reach_many ? r.reach_many : ctx);
     const size_t all = (size_t)b.n_rows * nq, some = (size_t)b.n_seqs * p.n_kv_heads * r.few;
     r.few_rows = r.only <= PA_FEW && r.nz_few > 1 ? r.nz_few * (r.only == PA_FEW ? all : some) : 0;
     r.many_rows = r.only != PA_FEW && r.nz_many > 1 ? r.nz_many * all : 0;

@@ -399,3 +399,31 @@ def test_two_streams_and_a_graph(eng, hip):
     hip.lib.hipGraphDestroy(graph)
     for wk in work:
         hip.lib.hipStreamDestroy(wk[-1])
+
+
+@pytest.mark.parametrize("t", [R.BF16, R.F16])
+@pytest.mark.parametrize("hd", [64, 128, 256])
+@pytest.mark.parametrize("rows,ctx,window,sink", [
+    ([70], [70], 100, 0), ([1], [95], 200, 3), ([1, 40, 0, 3], [90, 55, 3, 88], 128, 2), ([33], [3500], 4000, 0),
+    ([140], [2200], 3000, 1), ([1, 1, 1], [20, 1300, 600], 1500, 4), ([70, 2], [70, 90], 3, 150)])
+def test_windows_that_reach_everything_at_any_width_of_the_table(eng, hip, rows, ctx, window, sink, hd, t):
+    """A window or first tokens as long as every sequence: the same bits with a
+    table that holds fewer rows than those, as many or more, and a row that
+    sees itself alone has its v."""
+    got = []
+    reach = max(window, sink)
+    for extra in (0, -(-reach // 16) - -(-max(ctx) // 16), 1 << 12):
+        rng = np.random.default_rng(hd + t)
+        cache = R.Cache(hip, rng, t, rows, ctx, 2, hd, 16, table_extra=extra)
+        q = R.to_type(rng.standard_normal((cache.n_rows, 8, hd)) * 1.5, t)
+        say(f"whole windows: {rows} rows over {ctx}, hd {hd}, type {t}, a table of {cache.table.shape[1]} pages")
+        assert (16 * cache.table.shape[1] < reach) == (extra == 0)
+        out, lse, _ = call(eng, hip, cache, 8, q, 0.1, window, sink)
+        check(cache, 8, q, 0.1, out, lse, t, window, sink)
+        for s, (r, c) in enumerate(zip(rows, ctx)):
+            if r == c:
+                v = R.from_type(cache.row(cache.v, cache.table[s, 0], 0), t)
+                assert np.array_equal(out[cache.starts[s]], np.repeat(v, 4, 0))
+        got.append((out, lse))
+        hip.free_all()
+    assert all(np.array_equal(g[0], got[0][0]) and np.array_equal(g[1], got[0][1]) for g in got[1:])
