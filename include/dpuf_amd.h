@@ -313,14 +313,16 @@ DPUF_EXPORT int32_t dpuf_amd_paged_attn(const DpufAmdBatch* batch, const DpufAmd
  * the row at place p of its sequence (p = ctx_len - n + i) attends to cached
  * rows t <= p with t > p - window or t < sink.  window 1 to 2^30, itself
  * included; sink 0 to 2^30.  Table entries of pages with no row that a new row
- * attends to are not read as pages: they may hold anything, and the pages may
- * be other sequences' by now.  Probabilities that are rounded once (all but
- * bf16 ones of decoding sequences) count in their row's sum as they were rounded,
- * so that a row that sees few keys keeps its values' bits; d_lse has them whole.
- * That holds for windows that reach everything too: such a call differs from
- * dpuf_amd_paged_attn by roundings (its keys may be split otherwise as well), and
- * the table's width does not change its outputs.  The workspace is that of these
- * arguments, window and sink among them.  Everything else as above. */
+ * attends to may hold anything, and pages that they still name may be other
+ * sequences' by now: of the pool's, those beside a window's ends may be loaded,
+ * but nothing of them reaches an output.  Probabilities that are rounded once
+ * (all but bf16 ones of decoding sequences) count in their row's sum as they were
+ * rounded, so that a row that sees one key alone gets its values bit for bit;
+ * d_lse has them whole.  That holds for windows that reach everything too: such a
+ * call differs from dpuf_amd_paged_attn by roundings (its keys may be split
+ * otherwise as well), and the table's width does not change its outputs.  The
+ * workspace is that of these arguments, window and sink among them.  Everything
+ * else as above. */
 DPUF_EXPORT size_t dpuf_amd_paged_attn_window_workspace(const DpufAmdBatch* batch, const DpufAmdPages* pages,
                                                         int32_t n_q_heads, int32_t window, int32_t sink);
 DPUF_EXPORT int32_t dpuf_amd_paged_attn_window(const DpufAmdBatch* batch, const DpufAmdPages* pages, int32_t n_q_heads,

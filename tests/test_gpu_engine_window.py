@@ -222,3 +222,44 @@ def test_scores_of_a_full_call(eng):
         one_lp, one_en = score(at, 1)
         assert abs(one_lp[0] - lp[at]) < 0.1 and abs(one_en[0] - en[at]) < 0.1
     eng.dpuf_engine_destroy(h)
+
+
+def test_entries_of_pages_given_back_stay(eng, orc, hip):
+    """A conversation without end on a few pages: each page that both windows
+    have left is taken again for the next rows, and the table's old entries
+    still name it."""
+    page, windows, sink, n_pages = 16, (20, 33), 4, 7
+    shape = dict(hidden_size=256, intermediate_size=512, num_layers=2, num_q_heads=4, num_kv_heads=2, head_dim=64,
+                 vocab_size=V, tie_word_embeddings=1)
+    m = M.Model.build(shape, max_seq_len=32, seed=79)
+    h = eng.dpuf_engine_create(*m.create_args())
+    assert h
+    assert eng.dpuf_amd_engine_pages_create(h, n_pages, page, R.BF16) == 0
+    assert eng.dpuf_amd_engine_pages_window(h, M.ptr(np.array(windows, np.int32)), sink) == 0
+    parts = Parts(Windowed(eng, windows, sink), orc, hip, m, n_pages, page, R.BF16)
+    rng = np.random.default_rng(80)
+    free, held, ctx, again = list(range(n_pages)), [], 0, 0
+    for rows in [30] + [20, 1, 1, 14, 1, 25] * 3:
+        ctx += rows
+        lo = ctx - rows - max(windows) + 1
+        for j, (pg, there) in enumerate(held):
+            if there and (j + 1) * page <= lo and j * page >= sink:
+                free.append(pg)
+                held[j] = (pg, False)
+        while len(held) * page < ctx:
+            pg = free.pop(0)
+            again += any(pg == old for old, _ in held)
+            held.append((pg, True))
+        stale = np.array([[pg for pg, _ in held]], np.int32)
+        clean = np.array([[pg if there else -1 for pg, there in held]], np.int32)
+        pos, ids = np.arange(ctx - rows, ctx, dtype=np.int32), rng.integers(0, V, rows).astype(np.int32)
+        one = lambda v: np.array([v], np.int32)
+        say(f"  {rows} rows, {ctx} cached, {again} pages taken again")
+        want = parts.forward(one(rows), one(ctx), clean, ids, pos, -1.0)
+        lg = np.zeros((1, V), np.float32)
+        rc = eng.dpuf_amd_engine_forward_pages(h, 1, M.ptr(one(rows)), M.ptr(one(ctx)), M.ptr(stale), stale.shape[1],
+                                               M.ptr(ids), M.ptr(pos), -1.0, None, M.ptr(lg), None, None)
+        assert rc == 0, (rc, eng.dpuf_amd_last_error())
+        assert np.array_equal(lg.view(np.uint32), want.view(np.uint32)), np.abs(lg - want).max()
+    assert again > 5
+    eng.dpuf_engine_destroy(h)

@@ -427,3 +427,46 @@ def test_windows_that_reach_everything_at_any_width_of_the_table(eng, hip, rows,
         got.append((out, lse))
         hip.free_all()
     assert all(np.array_equal(g[0], got[0][0]) and np.array_equal(g[1], got[0][1]) for g in got[1:])
+
+
+@pytest.mark.parametrize("t", [R.BF16, R.F16])
+@pytest.mark.parametrize("mode", MODES)
+def test_pages_outside_every_window_may_be_others(eng, hip, mode, t):
+    """Entries behind a window that still are pages of the pool, as a program
+    leaves them that gives pages back: pages of NaN by now, other sequences'
+    pages, and pages that the row sees at another place: the same bits."""
+    rows, ctx, max_ctx, window, sink = MODES[mode]
+    rng = np.random.default_rng(len(mode) + t)
+    cache = R.Cache(hip, rng, t, rows, ctx, 2, 64, 16, table_extra=300)
+    q = R.to_type(rng.standard_normal((cache.n_rows, 8, 64)) * 1.5, t)
+    say(f"pages of others, {mode}, type {t}")
+    want = call(eng, hip, cache, 8, q, 0.1, window, sink, max_ctx=max_ctx)
+    seen, gone = [], []
+    for s, (r, c) in enumerate(zip(rows, ctx)):
+        lo = max(0, c - r - window + 1) if r else c
+        for j in range(cache.table.shape[1]):
+            out = j * 16 >= c or ((j + 1) * 16 <= lo and (j * 16 >= sink or r == 0))
+            (gone if out else seen).append((s, j))
+    own = cache.table.copy()
+    live = np.array([own[at] for at in seen])
+    nan = np.setdiff1d(np.arange(cache.n), live).astype(np.int32)
+    for pool in (cache.k, cache.v):
+        pool[nan] = R.to_type([np.nan], t)[0]
+    cache.dk.set(cache.k)
+    cache.dv.set(cache.v)
+    for what in ("their own, of NaN", "seen ones", "any"):
+        table = own.copy()
+        for s, j in gone:
+            if what == "seen ones":
+                table[s, j] = rng.choice(live)
+            elif what == "any":
+                table[s, j] = rng.integers(0, cache.n)
+            elif table[s, j] < 0:
+                table[s, j] = rng.choice(nan)
+        assert table.min() >= 0 and table.max() < cache.n
+        cache.d_table.set(table)
+        got = call(eng, hip, cache, 8, q, 0.1, window, sink, max_ctx=max_ctx)
+        assert np.array_equal(got[0], want[0]) and np.array_equal(got[1], want[1]), what
+        out, lse, _ = got
+        cache.table = own
+        check(cache, 8, q, 0.1, out, lse, t, window, sink)
