@@ -263,3 +263,30 @@ def test_entries_of_pages_given_back_stay(eng, orc, hip):
         assert np.array_equal(lg.view(np.uint32), want.view(np.uint32)), np.abs(lg - want).max()
     assert again > 5
     eng.dpuf_engine_destroy(h)
+
+
+def test_every_row_of_a_full_call(eng, orc, hip):
+    """512 scored rows in three sequences: targets, entropies and alternatives
+    against float64 from the logits of the parts put together."""
+    m, h = _engine(eng)
+    page, n_pages = 16, 40
+    assert eng.dpuf_amd_engine_pages_create(h, n_pages, page, R.BF16) == 0
+    parts = AllRows(eng, orc, hip, m, n_pages, page, R.BF16)
+    rng = np.random.default_rng(81)
+    rows = ctx = np.array([300, 1, 211], np.int32)
+    table, order = np.full((3, 19), -1, np.int32), list(rng.permutation(n_pages))
+    for i, c in enumerate(ctx):
+        for j in range(-(-int(c) // page)):
+            table[i, j] = order.pop()
+    pos = np.concatenate([np.arange(c) for c in ctx]).astype(np.int32)
+    ids = rng.integers(0, V, 512).astype(np.int32)
+    say("512 rows of three sequences")
+    parts.forward(rows, ctx, table, ids, pos, -1.0)
+    tg = rng.integers(0, V, (512, 3)).astype(np.int32)
+    lp, en = np.zeros((512, 3), np.float32), np.zeros(512, np.float32)
+    top, tl = np.zeros((512, 5), np.int32), np.zeros((512, 5), np.float32)
+    rc = eng.dpuf_amd_engine_score_pages(h, 3, M.ptr(rows), M.ptr(ctx), M.ptr(table), 19, M.ptr(ids), M.ptr(pos), 3,
+                                         M.ptr(tg), 5, M.ptr(lp), M.ptr(en), M.ptr(top), M.ptr(tl))
+    assert rc == 0, (rc, eng.dpuf_amd_last_error())
+    LP.check(parts.rows.astype(np.float64), tg, 5, (lp, en, top, tl))
+    eng.dpuf_engine_destroy(h)

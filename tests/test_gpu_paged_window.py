@@ -470,3 +470,15 @@ def test_pages_outside_every_window_may_be_others(eng, hip, mode, t):
         out, lse, _ = got
         cache.table = own
         check(cache, 8, q, 0.1, out, lse, t, window, sink)
+
+
+@pytest.mark.parametrize("t", [R.BF16, R.F16])
+def test_a_full_call_of_32_heads(eng, hip, t):
+    """512 rows of 32 heads, 8 kv heads of 128, in fp32 as an engine takes them."""
+    rng = np.random.default_rng(31 + t)
+    cache = R.Cache(hip, rng, t, [512], [1907], 8, 128, 64)
+    q = R.to_type(rng.standard_normal((512, 32, 128)) * 1.5, t)
+    scale = float(np.float32(1 / np.sqrt(128)))
+    say(f"512 rows of 32 heads, type {t}")
+    out, lse, _ = call(eng, hip, cache, 32, q, scale, 300, 5, out_t=R.F32)
+    check(cache, 32, q, scale, out, lse, R.F32, 300, 5)
