@@ -17,8 +17,8 @@
 // or as large and further to the front.  So one pass over the row leaves the
 // groups' largest, and what is read again is k groups; or, without ordering them
 // first, the few more that reach a bound which at least k groups' largest reach
-// (of 151 936 random logits and 20 alternatives 24 groups; one row 9.5 us, 10.7 by
-// the order of the groups), unless those, or their tokens, are many.
+// (of 151 936 random logits and 20 alternatives 24 groups; one row 9.5 to 10 us, 11
+// by the order of the groups), unless those, or their tokens, are many.
 //
 //   k_lp_part   a workgroup per chunk of a row: (r, l, u) and the groups' largest;
 //   k_lp_row    a workgroup per row: joins the chunks, picks groups, the k tokens
@@ -27,10 +27,11 @@
 //
 // Bound by the bytes of the logits, in 16 bits nearly as much by the exponential
 // and ten other instructions of each: 512 rows of 151 936 fp32 logits 54 us, 5.7
-// TB/s, 2 048 in bf16 with 20 alternatives 124 us, 5.0 TB/s.  Few rows are bound
-// by latency: one with 20 alternatives 3.8 us (38 workgroups) and 5.6, of which
-// 1.0 are the first loads, 0.8 the sums, 0.8 the groups' tokens and the rest the
-// bound, the lists and the order.
+// TB/s, 2 048 in bf16 with 20 alternatives 125 us, 5.0 TB/s (the first thirty
+// calls after a pause 142).  Few rows are bound by latency: one with 20
+// alternatives 3.8 us (38 workgroups) and 5.6, of which 1.0 are the first loads,
+// 0.8 the sums, 0.8 the groups' tokens and the rest the bound, the lists and the
+// order.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
@@ -641,7 +642,7 @@ template <typename L, int LOADS> __global__ __launch_bounds__(NT) void k_lp_row(
 }
 
 // Eight workgroups a CU as long as their registers suffice: 2 048 bf16 rows of
-// 151 936 with 20 alternatives 124 us, five a CU 147.  More than 32 alternatives
+// 151 936 with 20 alternatives 125 us, five a CU 147.  More than 32 alternatives
 // take more of them, and none may go to memory.
 template <typename L, int LOADS>
 __global__ __launch_bounds__(NT, LOADS < 4 ? 8 : L::VE < 8 ? 7 : 4) void k_lp_whole(LpArgs a) {

@@ -45,15 +45,18 @@
 // keys of those tiles that a row does not see are masked like those behind its
 // last.  A sequence's keys are split by that run's length, not by its context.
 // 48 single rows of 32 heads, 8 kv heads of 128 over 310 to 30 000 keys with a
-// window of 2 048: 79 us, 4.9 TB/s; 512 rows over 16 384 with one of 4 096: 57 us,
-// 600 TFLOP/s (of the kernel's 49 to 55 us 40 are steps, the rest the way to the
-// first and from the last); eight chunks of 64 rows with one of 128, 8 heads of 64
-// a kv head: 12 us, all but 4 of them latency around the steps.
+// window of 2 048: 79 us, 4.9 TB/s; 512 rows over 16 384 with one of 4 096: 58 us,
+// 590 TFLOP/s (about 40 of the kernel's are steps, the rest the way to the first
+// and from the last); eight chunks of 64 rows with one of 128, 8 heads of 64 a kv
+// head: 12 us, all but 4 of them latency around the steps.
 //
 // A window may hold few keys, one of which has most of the weight, and then o is
 // nearly that key's v, but for the rounding of its p.  So where p is rounded once
 // the W kernels add up the rounded p too and multiply o by l over that sum: what
-// is left of the errors e_t of p_t is sum e_t (v_t - o), not sum e_t v_t.
+// is left of the errors e_t of p_t is sum e_t (v_t - o), not sum e_t v_t.  Outputs
+// are then off from 64 bits by 2.1e-3 to 2.2e-3 of their size in bf16 chunks and
+// 2.5e-4 to 2.8e-4 in fp16, where the outputs' own rounding alone is 1.7e-3 and
+// 2.1e-4; bf16 single rows are at that rounding.
 #include <hip/hip_runtime.h>
 #include <math.h>
 #include <stdint.h>

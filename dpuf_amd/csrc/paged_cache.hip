@@ -18,8 +18,8 @@ namespace {
 // Bound by latency at few rows (8 of 32 and 8 + 8 heads of 128: 5.4 us; one row
 // of them all takes three workgroups) and nearly so at 512 (7.3 us, 1.7 TB/s).
 // With several position axes a pair's angle takes the position on its axis, by
-// compares with the sections' ends or by the remainder of the pair's number: 6.4
-// and 8.1 us for those rows.
+// compares with the sections' ends or by the remainder of the pair's number: 6.9
+// and 8.8 us for those rows.
 // ---------------------------------------------------------------------------
 struct RaArgs {
     DpufAmdBatch b;
