@@ -126,3 +126,17 @@ def test_logprobs_workspace(lib):
 
 def test_structure_size():
     assert C.sizeof(abi.DpufAmdRopeAxes) == 24
+
+
+@pytest.mark.parametrize("n_seqs,n_rows", [(1, 1), (1, 40), (1, 512), (9, 9), (9, 270), (48, 48)])
+def test_workspaces_of_whole_windows_do_not_depend_on_the_table(lib, n_seqs, n_rows):
+    """Windows and first tokens as long as the longest context: the same need
+    where the table holds fewer rows than those, as many or more."""
+    p = pages()
+    for ctx in (100, 1000, 5000, 16384):
+        for w, s in ((2 * ctx, 0), (2 * ctx, 4), (3, 2 * ctx), (1 << 30, 1 << 30)):
+            got = set()
+            for rows in (ctx, 2 * ctx - 16, 2 * ctx, 2 * ctx + 16, 1 << 20):
+                b = batch(n_seqs=n_seqs, n_rows=n_rows, max_ctx=ctx, table_stride=-(-rows // p.page_size))
+                got.add(lib.dpuf_amd_paged_attn_window_workspace(C.byref(b), C.byref(p), 32, w, s))
+            assert len(got) == 1, (ctx, w, s, got)
